@@ -491,6 +491,118 @@ typedef struct {
 int mh_silu_gate_fwd(const mh_gate_args* a, void* stream);
 int mh_silu_gate_bwd(const mh_gate_args* a, void* stream);
 
+/* ------------------------------------------------------------------------
+ * The two ends of a language model and what stands between its layers. Rows are (rows, dim) or (tokens, dim) tensors of
+ * any dim and row stride (elements), aligned to an element; the last dimension is contiguous. A call with no rows
+ * launches nothing (its weight gradients are cleared).
+ * ---------------------------------------------------------------------- */
+
+/* Token table: out[t] = scale * weight[ids[t]], zeros for an id outside [0, vocab). ids are index_bytes (4 or 8) wide. */
+typedef struct {
+  int64_t tokens, vocab, dim;
+  int32_t dtype, index_bytes;
+  float scale;
+  const void* ids;
+  const void* weight; int64_t weight_stride;
+  void* out; int64_t out_stride;
+} mh_embedding_args;
+int mh_embedding_fwd(const mh_embedding_args* a, void* stream);
+
+/* Its gradient: dweight[v] = scale * sum of dy[t] over ids[t] == v, v != padding_idx (-1: none), every row written,
+ *   (vocab, dim) contiguous in dweight_dtype. Tokens are sorted by id and summed in their order, in fp32: the same bits
+ *   at every call. tokens <= 2^30. */
+typedef struct {
+  int64_t tokens, vocab, dim, padding_idx;
+  int32_t dtype, index_bytes, dweight_dtype;
+  float scale;
+  const void* ids;
+  const void* dy; int64_t dy_stride;
+  void* dweight;
+  void* workspace; size_t workspace_bytes;
+} mh_embedding_bwd_args;
+int mh_embedding_bwd_workspace_bytes(const mh_embedding_bwd_args* a, size_t* bytes);
+int mh_embedding_bwd(const mh_embedding_bwd_args* a, void* stream);
+
+/* Layer norm of the residual stream: h = x + residual (rounded to dtype; h = x, not written, if residual is NULL),
+ *   y = (h - mean) / sqrt(var + eps) * weight + bias over dim. weight / bias (dim,) in weight_dtype, each or NULL.
+ *   stats (rows, 2) fp32 (mean, 1 / sqrt(var + eps)) or NULL. codes / exponents: h packed as by mh_pack_activations, or
+ *   both NULL. dim <= 16384. */
+typedef struct {
+  int64_t rows, dim;
+  int32_t dtype, weight_dtype;
+  float eps;
+  const void* x; int64_t x_stride;
+  const void* residual; int64_t residual_stride;
+  const void* weight; const void* bias;
+  void* y; int64_t y_stride;
+  void* h; int64_t h_stride;
+  float* stats;
+  void* codes; void* exponents;
+} mh_layer_norm_args;
+int mh_layer_norm_fwd(const mh_layer_norm_args* a, void* stream);
+
+/* Its backward. h as the forward normalised it, or (h NULL) codes and exponents in its place; d_h, the gradient of the
+ *   stream itself, or NULL. dx, which is the gradient of x and of residual; dweight, dbias (dim,) in weight_dtype, each
+ *   or NULL, written (not added to), the same bits at every call. */
+typedef struct {
+  int64_t rows, dim;
+  int32_t dtype, weight_dtype;
+  const void* dy; int64_t dy_stride;
+  const void* h; int64_t h_stride;
+  const void* codes; const void* exponents;
+  const float* stats;
+  const void* weight;
+  const void* d_h; int64_t d_h_stride;
+  void* dx; int64_t dx_stride;
+  void* dweight; void* dbias;
+  void* workspace; size_t workspace_bytes;
+} mh_layer_norm_bwd_args;
+int mh_layer_norm_bwd_workspace_bytes(const mh_layer_norm_bwd_args* a, size_t* bytes);
+int mh_layer_norm_bwd(const mh_layer_norm_bwd_args* a, void* stream);
+
+/* Activations in 8 bits: each 64 channels of a row share an exponent e, the least (>= -132) with max|x| <= 127 * 2^e, kept
+ *   as the byte e + 132; codes = x * 2^-e to nearest even, int8. A group that holds an infinity or a NaN has the byte 255
+ *   and reads back as NaN. codes (rows, dp) and exponents (rows, dp / 64) contiguous, dp = dim up to a multiple of 64
+ *   (codes beyond dim are 0); codes 8-byte aligned. mh_unpack_activations writes x. */
+typedef struct {
+  int64_t rows, dim;
+  int32_t dtype, reserved;
+  void* x; int64_t x_stride;
+  void* codes; void* exponents;
+} mh_pack_args;
+int mh_pack_activations(const mh_pack_args* a, void* stream);
+int mh_unpack_activations(const mh_pack_args* a, void* stream);
+
+/* Log probabilities of given tokens: with l = logits / temperature, logprobs = l[target] - ln sum exp l (0 where target
+ *   is ignore_index or outside [0, vocab)), entropy = -sum p ln p (or NULL), and the `top` (0 .. 64, <= vocab) largest:
+ *   top_ids (rows, top) int64 and top_logprobs (rows, top), largest first, equal logits by lowest id, NaN first.
+ *   stats (rows, 3) fp32 is what the backward takes. A row of -inf only: logprobs and top_logprobs -inf, entropy 0. */
+typedef struct {
+  int64_t rows, vocab, ignore_index;
+  int32_t dtype, index_bytes, top;
+  float temperature;
+  const void* logits; int64_t logits_stride;
+  const void* targets;
+  float* logprobs; float* entropy; float* stats;
+  int64_t* top_ids; float* top_logprobs;
+  void* workspace; size_t workspace_bytes;
+} mh_logprob_args;
+int mh_token_logprobs_workspace_bytes(const mh_logprob_args* a, size_t* bytes);
+int mh_token_logprobs_fwd(const mh_logprob_args* a, void* stream);
+
+/* Gradient of the logits from those of logprobs and entropy (fp32, each or NULL). A row whose two are zero, or that is
+ *   all -inf, gets zeros whatever its logits are. dlogits may be logits itself (same stride). */
+typedef struct {
+  int64_t rows, vocab, ignore_index;
+  int32_t dtype, index_bytes;
+  float temperature;
+  const void* logits; int64_t logits_stride;
+  const void* targets;
+  const float* stats; const float* d_logprobs; const float* d_entropy;
+  void* dlogits; int64_t dlogits_stride;
+} mh_logprob_bwd_args;
+int mh_token_logprobs_bwd(const mh_logprob_bwd_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -3,7 +3,9 @@
 Public ops (``mamformer_amd.ops``): ``selective_scan`` (SSD chunked-scan
 prefill, differentiable) and ``selective_scan_bwd`` (its backward), ``selective_state_update`` / ``recurrent_step`` (decode step) and
 ``linear_attn_scan`` (KDA gated scan), ``causal_conv1d`` (Mamba layer
-prologue); layer-level counterparts in ``mamformer_amd.layers``.  They run hand-written HIP kernels from
+prologue); layer-level counterparts in ``mamformer_amd.layers``.  The ends of a language
+model and what stands between its layers (``mamformer_amd.token_ops``): ``embedding``, ``layer_norm``,
+``pack_activations``, ``token_logprobs`` and their backward passes.  They run hand-written HIP kernels from
 ``libmamformer_hip.so`` (build with ``python -m mamformer_amd.build``).
 """
 
@@ -12,8 +14,12 @@ from .ops import (Plan, causal_conv1d, diff_lambda, linear_attention_recurrent, 
                   plan_linear_attn_step, plan_selective_scan, plan_selective_scan_bwd, plan_selective_state_update, recurrent_step,
                   recurrent_step_reference, selective_scan_reference, plan_selective_scan_reference,
                   selective_scan, selective_scan_bwd, selective_state_update, ssd_chunk_len, linear_attn_scan_bwd)
+from .token_ops import (PackedActivations, TokenLogprobs, embedding, embedding_bwd, layer_norm, layer_norm_bwd,
+                        pack_activations, token_logprobs, token_logprobs_bwd, unpack_activations)
 
-__all__ = ["selective_scan", "selective_scan_bwd", "selective_state_update", "recurrent_step", "recurrent_step_reference", "selective_scan_reference",
+__all__ = ["embedding", "embedding_bwd", "layer_norm", "layer_norm_bwd", "PackedActivations", "pack_activations",
+           "unpack_activations", "TokenLogprobs", "token_logprobs", "token_logprobs_bwd",
+           "selective_scan", "selective_scan_bwd", "selective_state_update", "recurrent_step", "recurrent_step_reference", "selective_scan_reference",
            "plan_selective_scan_reference", "linear_attn_scan",
            "linear_attn_scan_pair", "linear_attn_scan_single", "linear_attention_scan", "diff_lambda",
            "linear_attn_step", "linear_attention_recurrent",

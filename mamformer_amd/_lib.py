@@ -191,6 +191,78 @@ class LayerStepArgs(ct.Structure):
     ]
 
 
+class EmbeddingArgs(ct.Structure):
+    _fields_ = [
+        ("tokens", _i64), ("vocab", _i64), ("dim", _i64), ("dtype", _i32), ("index_bytes", _i32), ("scale", _f32),
+        ("ids", _vp), ("weight", _vp), ("weight_stride", _i64), ("out", _vp), ("out_stride", _i64),
+    ]
+
+
+class EmbeddingBwdArgs(ct.Structure):
+    _fields_ = [
+        ("tokens", _i64), ("vocab", _i64), ("dim", _i64), ("padding_idx", _i64),
+        ("dtype", _i32), ("index_bytes", _i32), ("dweight_dtype", _i32), ("scale", _f32),
+        ("ids", _vp), ("dy", _vp), ("dy_stride", _i64), ("dweight", _vp),
+        ("workspace", _vp), ("workspace_bytes", _sz),
+    ]
+
+
+class LayerNormArgs(ct.Structure):
+    _fields_ = [
+        ("rows", _i64), ("dim", _i64), ("dtype", _i32), ("weight_dtype", _i32), ("eps", _f32),
+        ("x", _vp), ("x_stride", _i64), ("residual", _vp), ("residual_stride", _i64), ("weight", _vp), ("bias", _vp),
+        ("y", _vp), ("y_stride", _i64), ("h", _vp), ("h_stride", _i64), ("stats", _vp),
+        ("codes", _vp), ("exponents", _vp),
+    ]
+
+
+class LayerNormBwdArgs(ct.Structure):
+    _fields_ = [
+        ("rows", _i64), ("dim", _i64), ("dtype", _i32), ("weight_dtype", _i32),
+        ("dy", _vp), ("dy_stride", _i64), ("h", _vp), ("h_stride", _i64), ("codes", _vp), ("exponents", _vp),
+        ("stats", _vp), ("weight", _vp), ("d_h", _vp), ("d_h_stride", _i64), ("dx", _vp), ("dx_stride", _i64),
+        ("dweight", _vp), ("dbias", _vp), ("workspace", _vp), ("workspace_bytes", _sz),
+    ]
+
+
+class PackArgs(ct.Structure):
+    _fields_ = [
+        ("rows", _i64), ("dim", _i64), ("dtype", _i32), ("reserved", _i32),
+        ("x", _vp), ("x_stride", _i64), ("codes", _vp), ("exponents", _vp),
+    ]
+
+
+class LogprobArgs(ct.Structure):
+    _fields_ = [
+        ("rows", _i64), ("vocab", _i64), ("ignore_index", _i64),
+        ("dtype", _i32), ("index_bytes", _i32), ("top", _i32), ("temperature", _f32),
+        ("logits", _vp), ("logits_stride", _i64), ("targets", _vp),
+        ("logprobs", _vp), ("entropy", _vp), ("stats", _vp), ("top_ids", _vp), ("top_logprobs", _vp),
+        ("workspace", _vp), ("workspace_bytes", _sz),
+    ]
+
+
+class LogprobBwdArgs(ct.Structure):
+    _fields_ = [
+        ("rows", _i64), ("vocab", _i64), ("ignore_index", _i64),
+        ("dtype", _i32), ("index_bytes", _i32), ("temperature", _f32),
+        ("logits", _vp), ("logits_stride", _i64), ("targets", _vp),
+        ("stats", _vp), ("d_logprobs", _vp), ("d_entropy", _vp), ("dlogits", _vp), ("dlogits_stride", _i64),
+    ]
+
+
+# entry points of the language-model ends and their argument blocks; each takes a stream, the queries a size
+_TOKEN_CALLS = {
+    "mh_embedding_fwd": EmbeddingArgs, "mh_embedding_bwd": EmbeddingBwdArgs,
+    "mh_layer_norm_fwd": LayerNormArgs, "mh_layer_norm_bwd": LayerNormBwdArgs,
+    "mh_pack_activations": PackArgs, "mh_unpack_activations": PackArgs,
+    "mh_token_logprobs_fwd": LogprobArgs, "mh_token_logprobs_bwd": LogprobBwdArgs,
+}
+_TOKEN_QUERIES = {
+    "mh_embedding_bwd_workspace_bytes": EmbeddingBwdArgs, "mh_layer_norm_bwd_workspace_bytes": LayerNormBwdArgs,
+    "mh_token_logprobs_workspace_bytes": LogprobArgs,
+}
+
 # every symbol include/mamformer_hip.h declares
 EXPORTS = (
     "mh_abi_version", "mh_last_error",
@@ -207,6 +279,7 @@ EXPORTS = (
     "mh_mamba2_layer_step_workspace_bytes", "mh_mamba2_layer_step",
     "mh_causal_conv1d_fwd",
     "mh_conv1d_bwd_workspace_bytes", "mh_causal_conv1d_bwd",
+    *_TOKEN_CALLS, *_TOKEN_QUERIES,
 )
 
 _lock = threading.Lock()
@@ -278,6 +351,10 @@ def lib():
                          "mh_ssd_ref_scan_bwd_workspace_bytes", "mh_ssd_ref_scan_bwd",
                          "mh_silu_gate_fwd", "mh_silu_gate_bwd"):
                 getattr(h, name).restype = ct.c_int
+            for names, last in ((_TOKEN_CALLS, _vp), (_TOKEN_QUERIES, ct.POINTER(_sz))):
+                for name, block in names.items():
+                    getattr(h, name).argtypes = [ct.POINTER(block), last]
+                    getattr(h, name).restype = ct.c_int
             ver = h.mh_abi_version()
             if ver != ABI_VERSION:
                 raise RuntimeError(f"{LIB_PATH.name} ABI version {ver} != expected {ABI_VERSION}; rebuild")

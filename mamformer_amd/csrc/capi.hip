@@ -816,6 +816,173 @@ int kda_bwd_validate(const mh_kda_bwd_args* a) {
   return MH_OK;
 }
 
+// ------------------------------------------------------------------ language-model ends
+// Rows of dim elements with a stride: the pointer aligned to an element; rows may share memory if only read (stride 0).
+int rows_ok(const char* fn, const char* name, const void* p, int64_t stride, int64_t dim, int es, bool written) {
+  if (!p) return fail(MH_ERR_NULL, "%s: %s is required", fn, name);
+  if ((uintptr_t)p % es) return fail(MH_ERR_ALIGN, "%s: %s must be aligned to an element", fn, name);
+  if (written ? stride < dim : stride < 0)
+    return fail(MH_ERR_STRIDE, "%s: row stride of %s is %lld (dim %lld)", fn, name, (long long)stride, (long long)dim);
+  return MH_OK;
+}
+int vec_ok(const char* fn, const char* name, const void* p, int es, bool required) {
+  if (!p) return required ? fail(MH_ERR_NULL, "%s: %s is required", fn, name) : MH_OK;
+  if ((uintptr_t)p % es) return fail(MH_ERR_ALIGN, "%s: %s must be aligned to an element", fn, name);
+  return MH_OK;
+}
+#define MH_TRY(e)          \
+  do {                     \
+    const int rc_ = (e);   \
+    if (rc_) return rc_;   \
+  } while (0)
+
+int sizes_ok(const char* fn, int64_t rows, int64_t dim, int64_t max_dim, int32_t dtype) {
+  if (rows < 0 || dim <= 0) return fail(MH_ERR_SHAPE, "%s: sizes must be positive (rows=%lld dim=%lld)", fn, (long long)rows, (long long)dim);
+  if (rows > kMaxDim) return fail(MH_ERR_SHAPE, "%s: rows out of range", fn);
+  if (dim > max_dim) return fail(MH_ERR_UNSUPPORTED, "%s: dim %lld above %lld", fn, (long long)dim, (long long)max_dim);
+  if (!elem_size(dtype)) return fail(MH_ERR_DTYPE, "%s: unknown dtype %d", fn, dtype);
+  return MH_OK;
+}
+int index_ok(const char* fn, int32_t bytes, const void* p, const char* name) {
+  if (bytes != 4 && bytes != 8) return fail(MH_ERR_DTYPE, "%s: index_bytes must be 4 or 8, got %d", fn, bytes);
+  return vec_ok(fn, name, p, bytes, true);
+}
+
+constexpr int64_t kNormMaxDim = 16384;
+constexpr int64_t kTokenMaxDim = (int64_t)1 << 24;
+
+int embedding_validate(const mh_embedding_args* a) {
+  const char* fn = "embedding";
+  if (!a) return fail(MH_ERR_NULL, "embedding: args is NULL");
+  MH_TRY(sizes_ok(fn, a->tokens, a->dim, kTokenMaxDim, a->dtype));
+  if (a->vocab <= 0 || a->vocab > kMaxDim) return fail(MH_ERR_SHAPE, "embedding: vocab %lld out of range", (long long)a->vocab);
+  if (a->tokens == 0) return MH_OK;
+  const int es = elem_size(a->dtype);
+  MH_TRY(index_ok(fn, a->index_bytes, a->ids, "ids"));
+  MH_TRY(rows_ok(fn, "weight", a->weight, a->weight_stride, a->dim, es, false));
+  return rows_ok(fn, "out", a->out, a->out_stride, a->dim, es, true);
+}
+
+int embedding_bwd_validate(const mh_embedding_bwd_args* a, mh::EmbedBwdParams& p) {
+  const char* fn = "embedding_bwd";
+  if (!a) return fail(MH_ERR_NULL, "embedding_bwd: args is NULL");
+  MH_TRY(sizes_ok(fn, a->tokens, a->dim, kTokenMaxDim, a->dtype));
+  if (a->vocab <= 0 || a->vocab > kMaxDim) return fail(MH_ERR_SHAPE, "embedding_bwd: vocab %lld out of range", (long long)a->vocab);
+  if (!elem_size(a->dweight_dtype)) return fail(MH_ERR_DTYPE, "embedding_bwd: unknown dweight_dtype %d", a->dweight_dtype);
+  MH_TRY(vec_ok(fn, "dweight", a->dweight, elem_size(a->dweight_dtype), true));
+  if (a->tokens > 0) {
+    MH_TRY(index_ok(fn, a->index_bytes, a->ids, "ids"));
+    MH_TRY(rows_ok(fn, "dy", a->dy, a->dy_stride, a->dim, elem_size(a->dtype), false));
+  }
+  memset(&p, 0, sizeof(p));
+  p.tokens = a->tokens; p.vocab = a->vocab; p.padding_idx = a->padding_idx;
+  p.dim = (int)a->dim; p.dtype = a->dtype; p.i64 = a->index_bytes == 8; p.dw_f32 = a->dweight_dtype == MH_F32;
+  p.scale = a->scale; p.ids = a->ids; p.dy = a->dy; p.dy_s = a->dy_stride; p.dweight = a->dweight;
+  return MH_OK;
+}
+
+int norm_par_ok(const char* fn, const void* w, const void* b, const char* wn, const char* bn, int32_t wdtype) {
+  if (!w && !b) return MH_OK;
+  if (!elem_size(wdtype)) return fail(MH_ERR_DTYPE, "%s: unknown weight_dtype %d", fn, wdtype);
+  MH_TRY(vec_ok(fn, wn, w, elem_size(wdtype), false));
+  return vec_ok(fn, bn, b, elem_size(wdtype), false);
+}
+
+int norm_validate(const mh_layer_norm_args* a) {
+  const char* fn = "layer_norm";
+  if (!a) return fail(MH_ERR_NULL, "layer_norm: args is NULL");
+  MH_TRY(sizes_ok(fn, a->rows, a->dim, kNormMaxDim, a->dtype));
+  if (!(a->eps >= 0.f)) return fail(MH_ERR_SHAPE, "layer_norm: eps must not be negative");
+  MH_TRY(norm_par_ok(fn, a->weight, a->bias, "weight", "bias", a->weight_dtype));
+  if (!a->codes != !a->exponents) return fail(MH_ERR_NULL, "layer_norm: codes and exponents go together");
+  if (a->rows == 0) return MH_OK;
+  const int es = elem_size(a->dtype);
+  MH_TRY(rows_ok(fn, "x", a->x, a->x_stride, a->dim, es, false));
+  MH_TRY(rows_ok(fn, "y", a->y, a->y_stride, a->dim, es, true));
+  if (a->residual) {
+    MH_TRY(rows_ok(fn, "residual", a->residual, a->residual_stride, a->dim, es, false));
+    MH_TRY(rows_ok(fn, "h", a->h, a->h_stride, a->dim, es, true));
+  }
+  if (a->codes && (uintptr_t)a->codes % 8) return fail(MH_ERR_ALIGN, "layer_norm: codes must be 8-byte aligned");
+  return vec_ok(fn, "stats", a->stats, 4, false);
+}
+
+int norm_bwd_validate(const mh_layer_norm_bwd_args* a) {
+  const char* fn = "layer_norm_bwd";
+  if (!a) return fail(MH_ERR_NULL, "layer_norm_bwd: args is NULL");
+  MH_TRY(sizes_ok(fn, a->rows, a->dim, kNormMaxDim, a->dtype));
+  MH_TRY(norm_par_ok(fn, a->weight, nullptr, "weight", "", a->weight_dtype));
+  MH_TRY(norm_par_ok(fn, a->dweight, a->dbias, "dweight", "dbias", a->weight_dtype));
+  if (a->rows == 0) return MH_OK;
+  const int es = elem_size(a->dtype);
+  MH_TRY(rows_ok(fn, "dy", a->dy, a->dy_stride, a->dim, es, false));
+  if (a->h) {
+    MH_TRY(rows_ok(fn, "h", a->h, a->h_stride, a->dim, es, false));
+  } else {
+    if (!a->codes || !a->exponents) return fail(MH_ERR_NULL, "layer_norm_bwd: h, or codes and exponents, are required");
+    if ((uintptr_t)a->codes % 8) return fail(MH_ERR_ALIGN, "layer_norm_bwd: codes must be 8-byte aligned");
+  }
+  MH_TRY(vec_ok(fn, "stats", a->stats, 4, true));
+  if (a->d_h) MH_TRY(rows_ok(fn, "d_h", a->d_h, a->d_h_stride, a->dim, es, false));
+  return rows_ok(fn, "dx", a->dx, a->dx_stride, a->dim, es, true);
+}
+size_t norm_bwd_need(const mh_layer_norm_bwd_args* a) {
+  return a->dweight || a->dbias ? mh::norm_bwd_workspace_bytes(a->rows, (int)a->dim) : 0;
+}
+
+int pack_run(const mh_pack_args* a, bool back, hipStream_t st) {
+  const char* fn = back ? "unpack_activations" : "pack_activations";
+  if (!a) return fail(MH_ERR_NULL, "%s: args is NULL", fn);
+  MH_TRY(sizes_ok(fn, a->rows, a->dim, kTokenMaxDim, a->dtype));
+  if (a->rows == 0) return MH_OK;
+  MH_TRY(rows_ok(fn, "x", a->x, a->x_stride, a->dim, elem_size(a->dtype), back));
+  if (!a->codes || !a->exponents) return fail(MH_ERR_NULL, "%s: codes and exponents are required", fn);
+  if ((uintptr_t)a->codes % 8) return fail(MH_ERR_ALIGN, "%s: codes must be 8-byte aligned", fn);
+  mh::PackParams p;
+  p.rows = a->rows; p.dim = (int)a->dim; p.dtype = a->dtype;
+  p.x = a->x; p.out = a->x; p.x_s = a->x_stride;
+  p.codes = reinterpret_cast<uint8_t*>(a->codes); p.code_s = (a->dim + 63) / 64 * 64;
+  p.exps = reinterpret_cast<uint8_t*>(a->exponents);
+  return hip_status(mh::launch_pack(p, back, st), fn);
+}
+
+int logprob_common(const char* fn, int64_t rows, int64_t vocab, int32_t dtype, float temperature, const void* logits,
+                   int64_t stride, int32_t index_bytes, const void* targets) {
+  MH_TRY(sizes_ok(fn, rows, vocab, kMaxDim, dtype));
+  if (!(temperature > 0.f) || !(1.f / temperature > 0.f) || !(1.f / temperature <= 3.4e38f))
+    return fail(MH_ERR_SHAPE, "%s: temperature must be positive and finite", fn);
+  if (rows == 0) return MH_OK;
+  MH_TRY(rows_ok(fn, "logits", logits, stride, vocab, elem_size(dtype), false));
+  return index_ok(fn, index_bytes, targets, "targets");
+}
+
+int logprob_validate(const mh_logprob_args* a, mh::LogprobParams& p) {
+  const char* fn = "token_logprobs";
+  if (!a) return fail(MH_ERR_NULL, "token_logprobs: args is NULL");
+  MH_TRY(logprob_common(fn, a->rows, a->vocab, a->dtype, a->temperature, a->logits, a->logits_stride, a->index_bytes, a->targets));
+  if (a->top < 0 || a->top > mh::kMaxAlternatives || a->top > a->vocab)
+    return fail(MH_ERR_UNSUPPORTED, "token_logprobs: top %d outside 0 .. min(%d, vocab)", a->top, mh::kMaxAlternatives);
+  if (a->rows > 0) {
+    MH_TRY(vec_ok(fn, "logprobs", a->logprobs, 4, true));
+    MH_TRY(vec_ok(fn, "entropy", a->entropy, 4, false));
+    MH_TRY(vec_ok(fn, "stats", a->stats, 4, true));
+    MH_TRY(vec_ok(fn, "top_ids", a->top_ids, 8, a->top > 0));
+    MH_TRY(vec_ok(fn, "top_logprobs", a->top_logprobs, 4, a->top > 0));
+  }
+  p.rows = a->rows; p.vocab = a->vocab; p.ignore_index = a->ignore_index;
+  p.dtype = a->dtype; p.i64 = a->index_bytes == 8; p.top = a->top; p.inv_temp = 1.f / a->temperature;
+  p.logits = a->logits; p.l_s = a->logits_stride; p.targets = a->targets;
+  p.logprobs = a->logprobs; p.entropy = a->entropy; p.stats = a->stats;
+  p.top_ids = a->top_ids; p.top_logprobs = a->top_logprobs; p.workspace = a->workspace;
+  return MH_OK;
+}
+
+int workspace_ok(const char* fn, const void* ws, size_t got, size_t need) {
+  if (need > 0 && (!ws || got < need || !aligned16(ws)))
+    return fail(MH_ERR_WORKSPACE, "%s: workspace of %zu bytes (16-byte aligned) required, got %zu", fn, need, got);
+  return MH_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1350,6 +1517,106 @@ int mh_ssd_chunk_scan_bwd(const mh_ssd_bwd_args* a, void* stream) {
                 a->workspace_bytes);
   if (!ssd_native_dstate(f->dstate)) return ssd_bwd_wide(a, reinterpret_cast<hipStream_t>(stream));
   return hip_status(ssd_launch_bwd_native(a, reinterpret_cast<hipStream_t>(stream)), "ssd_chunk_scan_bwd");
+}
+
+int mh_embedding_fwd(const mh_embedding_args* a, void* stream) {
+  MH_TRY(embedding_validate(a));
+  mh::EmbedParams p;
+  p.tokens = a->tokens; p.vocab = a->vocab; p.dim = (int)a->dim; p.dtype = a->dtype; p.i64 = a->index_bytes == 8;
+  p.scale = a->scale; p.ids = a->ids; p.weight = a->weight; p.w_s = a->weight_stride;
+  p.out = a->out; p.out_s = a->out_stride;
+  return hip_status(mh::launch_embed_fwd(p, reinterpret_cast<hipStream_t>(stream)), "embedding");
+}
+
+int mh_embedding_bwd_workspace_bytes(const mh_embedding_bwd_args* a, size_t* bytes) {
+  if (!bytes) return fail(MH_ERR_NULL, "embedding_bwd: bytes output is NULL");
+  mh::EmbedBwdParams p;
+  MH_TRY(embedding_bwd_validate(a, p));
+  *bytes = mh::embed_bwd_plan(p, nullptr);
+  return MH_OK;
+}
+
+int mh_embedding_bwd(const mh_embedding_bwd_args* a, void* stream) {
+  mh::EmbedBwdParams p;
+  MH_TRY(embedding_bwd_validate(a, p));
+  MH_TRY(workspace_ok("embedding_bwd", a->workspace, a->workspace_bytes, mh::embed_bwd_plan(p, nullptr)));
+  mh::embed_bwd_plan(p, a->workspace);
+  return hip_status(mh::launch_embed_bwd(p, reinterpret_cast<hipStream_t>(stream)), "embedding_bwd");
+}
+
+int mh_layer_norm_fwd(const mh_layer_norm_args* a, void* stream) {
+  MH_TRY(norm_validate(a));
+  mh::NormParams p;
+  p.rows = a->rows; p.dim = (int)a->dim; p.dtype = a->dtype; p.w_f32 = a->weight_dtype == MH_F32; p.eps = a->eps;
+  p.x = a->x; p.x_s = a->x_stride; p.residual = a->residual; p.res_s = a->residual_stride;
+  p.weight = a->weight; p.bias = a->bias; p.y = a->y; p.y_s = a->y_stride; p.h = a->h; p.h_s = a->h_stride;
+  p.stats = a->stats; p.codes = reinterpret_cast<uint8_t*>(a->codes); p.code_s = (a->dim + 63) / 64 * 64;
+  p.exps = reinterpret_cast<uint8_t*>(a->exponents);
+  return hip_status(mh::launch_norm_fwd(p, reinterpret_cast<hipStream_t>(stream)), "layer_norm");
+}
+
+int mh_layer_norm_bwd_workspace_bytes(const mh_layer_norm_bwd_args* a, size_t* bytes) {
+  if (!bytes) return fail(MH_ERR_NULL, "layer_norm_bwd: bytes output is NULL");
+  MH_TRY(norm_bwd_validate(a));
+  *bytes = norm_bwd_need(a);
+  return MH_OK;
+}
+
+int mh_layer_norm_bwd(const mh_layer_norm_bwd_args* a, void* stream) {
+  MH_TRY(norm_bwd_validate(a));
+  MH_TRY(workspace_ok("layer_norm_bwd", a->workspace, a->workspace_bytes, norm_bwd_need(a)));
+  mh::NormBwdParams p;
+  p.rows = a->rows; p.dim = (int)a->dim; p.dtype = a->dtype; p.w_f32 = a->weight_dtype == MH_F32;
+  p.dy = a->dy; p.dy_s = a->dy_stride; p.h = a->h; p.h_s = a->h_stride;
+  p.codes = a->h ? nullptr : reinterpret_cast<const uint8_t*>(a->codes); p.code_s = (a->dim + 63) / 64 * 64;
+  p.exps = reinterpret_cast<const uint8_t*>(a->exponents);
+  p.stats = a->stats; p.weight = a->weight; p.d_h = a->d_h; p.dh_s = a->d_h_stride;
+  p.dx = a->dx; p.dx_s = a->dx_stride; p.dweight = a->dweight; p.dbias = a->dbias;
+  p.part = a->dweight || a->dbias ? reinterpret_cast<float*>(a->workspace) : nullptr;
+  return hip_status(mh::launch_norm_bwd(p, reinterpret_cast<hipStream_t>(stream)), "layer_norm_bwd");
+}
+
+int mh_pack_activations(const mh_pack_args* a, void* stream) {
+  return pack_run(a, false, reinterpret_cast<hipStream_t>(stream));
+}
+int mh_unpack_activations(const mh_pack_args* a, void* stream) {
+  return pack_run(a, true, reinterpret_cast<hipStream_t>(stream));
+}
+
+int mh_token_logprobs_workspace_bytes(const mh_logprob_args* a, size_t* bytes) {
+  if (!bytes) return fail(MH_ERR_NULL, "token_logprobs: bytes output is NULL");
+  mh::LogprobParams p;
+  MH_TRY(logprob_validate(a, p));
+  *bytes = mh::logprob_workspace_bytes(p);
+  return MH_OK;
+}
+
+int mh_token_logprobs_fwd(const mh_logprob_args* a, void* stream) {
+  mh::LogprobParams p;
+  MH_TRY(logprob_validate(a, p));
+  MH_TRY(workspace_ok("token_logprobs", a->workspace, a->workspace_bytes, mh::logprob_workspace_bytes(p)));
+  return hip_status(mh::launch_logprob(p, reinterpret_cast<hipStream_t>(stream)), "token_logprobs");
+}
+
+int mh_token_logprobs_bwd(const mh_logprob_bwd_args* a, void* stream) {
+  const char* fn = "token_logprobs_bwd";
+  if (!a) return fail(MH_ERR_NULL, "token_logprobs_bwd: args is NULL");
+  MH_TRY(logprob_common(fn, a->rows, a->vocab, a->dtype, a->temperature, a->logits, a->logits_stride, a->index_bytes, a->targets));
+  if (a->rows == 0) return MH_OK;
+  MH_TRY(vec_ok(fn, "stats", a->stats, 4, true));
+  MH_TRY(vec_ok(fn, "d_logprobs", a->d_logprobs, 4, false));
+  MH_TRY(vec_ok(fn, "d_entropy", a->d_entropy, 4, false));
+  const int es = elem_size(a->dtype);
+  MH_TRY(rows_ok(fn, "dlogits", a->dlogits, a->dlogits_stride, a->vocab, es, true));
+  const size_t nl = ((size_t)(a->rows - 1) * a->logits_stride + a->vocab) * es, nd = ((size_t)(a->rows - 1) * a->dlogits_stride + a->vocab) * es;
+  if (overlap(a->logits, nl, a->dlogits, nd) && (a->logits != a->dlogits || (a->rows > 1 && a->logits_stride != a->dlogits_stride)))
+    return fail(MH_ERR_STRIDE, "token_logprobs_bwd: dlogits overlaps logits elsewhere than in place");
+  mh::LogprobBwdParams p;
+  p.rows = a->rows; p.vocab = a->vocab; p.ignore_index = a->ignore_index;
+  p.dtype = a->dtype; p.i64 = a->index_bytes == 8; p.inv_temp = 1.f / a->temperature;
+  p.logits = a->logits; p.l_s = a->logits_stride; p.targets = a->targets; p.stats = a->stats;
+  p.d_logprobs = a->d_logprobs; p.d_entropy = a->d_entropy; p.dlogits = a->dlogits; p.d_s = a->dlogits_stride;
+  return hip_status(mh::launch_logprob_bwd(p, reinterpret_cast<hipStream_t>(stream)), "token_logprobs_bwd");
 }
 
 }  // extern "C"

@@ -351,4 +351,103 @@ struct GateParams {
 };
 hipError_t launch_gate(const GateParams& a, bool backward, hipStream_t st);
 
+// ------------------------------------------------------------- layer norm, 8-bit activations (norm.hip)
+struct NormParams {
+  int64_t rows;
+  int dim, dtype, w_f32;                   // w_f32: weight and bias are fp32, else bf16
+  float eps;
+  const void* x; int64_t x_s;
+  const void* residual; int64_t res_s;     // null: h = x is not written
+  const void* weight; const void* bias;    // or null
+  void* y; int64_t y_s;
+  void* h; int64_t h_s;
+  float* stats;                            // (rows, 2) mean, 1 / std; or null
+  uint8_t* codes; int64_t code_s;          // (rows, code_s), code_s = dim up to a multiple of 64; or null
+  uint8_t* exps;                           // (rows, code_s / 64)
+};
+hipError_t launch_norm_fwd(const NormParams& p, hipStream_t st);
+
+struct NormBwdParams {
+  int64_t rows;
+  int dim, dtype, w_f32;
+  const void* dy; int64_t dy_s;
+  const void* h; int64_t h_s;              // or codes and exps in its place
+  const uint8_t* codes; int64_t code_s;
+  const uint8_t* exps;
+  const float* stats;
+  const void* weight;                      // or null
+  const void* d_h; int64_t dh_s;           // or null
+  void* dx; int64_t dx_s;
+  void* dweight; void* dbias;              // each or null
+  float* part;                             // workspace; null where neither is wanted
+};
+hipError_t launch_norm_bwd(const NormBwdParams& p, hipStream_t st);
+size_t norm_bwd_workspace_bytes(int64_t rows, int dim);
+
+struct PackParams {
+  int64_t rows;
+  int dim, dtype;
+  const void* x; void* out; int64_t x_s;   // packed from x, unpacked to out
+  uint8_t* codes; int64_t code_s;
+  uint8_t* exps;
+};
+hipError_t launch_pack(const PackParams& p, bool back, hipStream_t st);
+
+// ------------------------------------------------------------- token table (embedding.hip)
+struct EmbedParams {
+  int64_t tokens, vocab;
+  int dim, dtype, i64;                     // i64: 64-bit ids, else 32-bit
+  float scale;
+  const void* ids;
+  const void* weight; int64_t w_s;
+  void* out; int64_t out_s;
+};
+hipError_t launch_embed_fwd(const EmbedParams& p, hipStream_t st);
+
+struct EmbedBwdParams {
+  int64_t tokens, vocab, padding_idx;      // padding_idx: -1 for none
+  int dim, dtype, i64, dw_f32;
+  float scale;
+  const void* ids;
+  const void* dy; int64_t dy_s;
+  void* dweight;                           // (vocab, dim) contiguous
+  // by embed_bwd_plan
+  int passes, tiles, cthreads;
+  int64_t tile, piece, pieces;
+  uint32_t* keys[2]; uint32_t* order[2]; uint32_t* hist;
+  float* part;
+};
+// Fills the plan's fields (pointers into `workspace`, if given) and returns the workspace bytes.
+size_t embed_bwd_plan(EmbedBwdParams& p, void* workspace);
+hipError_t launch_embed_bwd(const EmbedBwdParams& p, hipStream_t st);
+
+// ------------------------------------------------------------- log probabilities (logprob.hip)
+constexpr int kMaxAlternatives = 64;
+struct LogprobParams {
+  int64_t rows, vocab, ignore_index;
+  int dtype, i64, top;
+  float inv_temp;
+  const void* logits; int64_t l_s;
+  const void* targets;
+  float* logprobs; float* entropy;         // entropy: or null
+  float* stats;                            // (rows, 3) max, ln of the sum, entropy
+  int64_t* top_ids; float* top_logprobs;
+  void* workspace;
+};
+size_t logprob_workspace_bytes(const LogprobParams& p);
+hipError_t launch_logprob(const LogprobParams& p, hipStream_t st);
+
+struct LogprobBwdParams {
+  int64_t rows, vocab, ignore_index;
+  int dtype, i64;
+  float inv_temp;
+  const void* logits; int64_t l_s;
+  const void* targets;
+  const float* stats;
+  const float* d_logprobs; const float* d_entropy;   // each or null
+  void* dlogits; int64_t d_s;
+  int64_t span;                            // columns of a workgroup
+};
+hipError_t launch_logprob_bwd(LogprobBwdParams p, hipStream_t st);
+
 }  // namespace mh

@@ -1,0 +1,349 @@
+// Layer norm of a residual stream, its backward with the parameters' gradients, and activations in 8 bits.
+//
+//   h = x + residual (rounded to the stream's type, which is what the next layer adds to; without a residual h = x)
+//   mu = mean(h), r = 1 / sqrt(mean((h - mu)^2) + eps), y = (h - mu) r w + b
+// and, with c = (h - mu) r and g = dy w,
+//   dx = r (g - mean(g) - c mean(g c)) + d_h,   dw = sum over rows of dy c,   db = sum over rows of dy.
+//
+// A row lives in the registers of a group of threads (8 channels a thread and step), so every tensor is read and
+// written once and the variance is that of the centred values.  Groups: as many lanes of a wave as the row has chunks,
+// from 8 (heads of 64 channels) to a wave with up to 4 chunks a lane (2048 channels), which needs no barrier; beyond,
+// a workgroup of 256 or 1024 threads.  Sums are fp32.
+#include "common.h"
+#include "launch.h"
+#include "rows.h"
+
+namespace mh {
+
+namespace {
+
+// Sums over the threads of a row's group: in the wave, or over the workgroup through LDS (two buffers by turns, one
+// barrier a sum).
+template <int TPR>
+struct RowSum {
+  __device__ __forceinline__ float operator()(float v) { return group_sum<TPR>(v); }
+};
+template <int NT>
+struct BlockSum {
+  float* buf;                                    // (2, NT / 64)
+  int turn = 0;
+  __device__ __forceinline__ float operator()(float v) {
+    v = group_sum<64>(v);
+    float* b = buf + turn * (NT / 64);
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) b[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) s += b[w];
+    return s;
+  }
+};
+template <> struct RowSum<256> : BlockSum<256> {};
+template <> struct RowSum<1024> : BlockSum<1024> {};
+
+template <int TPR> constexpr int kThreads = TPR <= 64 ? 256 : TPR;
+
+template <typename T, int TPR, int NV>
+__global__ __launch_bounds__(kThreads<TPR>) void norm_fwd_kernel(NormParams p) {
+  __shared__ float sums[2 * 16];
+  const int lane = threadIdx.x % TPR;
+  const int64_t row = (int64_t)blockIdx.x * (kThreads<TPR> / TPR) + threadIdx.x / TPR;
+  if (row >= p.rows) return;                     // whole groups, and whole workgroups where a group is one
+  RowSum<TPR> sum;
+  if constexpr (TPR > 64) sum.buf = sums;
+  const T* x = reinterpret_cast<const T*>(p.x) + row * p.x_s;
+  float v[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = 8 * (i * TPR + lane);
+    load8(x + c, p.dim - c, v[i]);
+  }
+  if (p.residual) {
+    const T* res = reinterpret_cast<const T*>(p.residual) + row * p.res_s;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + lane);
+      float q[8];
+      load8(res + c, p.dim - c, q);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = to_f32(from_f32<T>(v[i][j] + q[j]));   // the stream's own rounding
+      store8(reinterpret_cast<T*>(p.h) + row * p.h_s + c, p.dim - c, v[i]);
+    }
+  }
+  const float n = (float)p.dim;                  // divided by, not multiplied by 1 / n: equal channels give their own mean
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += v[i][j];
+  const float mu = sum(s) / n;
+  float s2 = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float d = 8 * (i * TPR + lane) + j < p.dim ? v[i][j] - mu : 0.f;
+      s2 += d * d;
+    }
+  const float r = 1.f / sqrtf(sum(s2) / n + p.eps);
+  if (p.stats && lane == 0) {
+    p.stats[2 * row] = mu;
+    p.stats[2 * row + 1] = r;
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = 8 * (i * TPR + lane);
+    if (p.codes) {
+      const uint32_t e = pack_exponent(v[i]);
+      if (c < p.code_s) {
+        *reinterpret_cast<uint64_t*>(p.codes + row * p.code_s + c) = pack_codes(v[i], e);
+        if ((lane & 7) == 0) p.exps[(row * p.code_s + c) / kPackGroup] = (uint8_t)e;
+      }
+    }
+    if (c >= p.dim) continue;
+    float w[8], b[8], o[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { w[j] = 1.f; b[j] = 0.f; }
+    if (p.weight) load_par8(p.weight, p.w_f32, c, p.dim, w);
+    if (p.bias) load_par8(p.bias, p.w_f32, c, p.dim, b);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = (v[i][j] - mu) * r * w[j] + b[j];
+    store8(reinterpret_cast<T*>(p.y) + row * p.y_s + c, p.dim - c, o);
+  }
+}
+
+// A workgroup walks rows blockIdx, + gridDim, ...; the sums for dw and db stay in registers until its end and go to
+// its own row of the partials, which norm_params_kernel adds in order: the same bits at every call.
+template <typename T, int TPR, int NV, bool PACKED>
+__global__ __launch_bounds__(kThreads<TPR>) void norm_bwd_kernel(NormBwdParams p) {
+  constexpr int G = kThreads<TPR> / TPR;         // rows at a time
+  __shared__ float sums[2 * 16];
+  __shared__ float park[G > 1 ? G * TPR * NV * 8 : 1];
+  const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  RowSum<TPR> sum;
+  if constexpr (TPR > 64) sum.buf = sums;
+  const float inv = 1.f / (float)p.dim;
+  float w[NV][8], dw[NV][8], db[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = 8 * (i * TPR + lane);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { w[i][j] = 1.f; dw[i][j] = 0.f; db[i][j] = 0.f; }
+    if (p.weight && c < p.dim) load_par8(p.weight, p.w_f32, c, p.dim, w[i]);
+  }
+  for (int64_t row = (int64_t)blockIdx.x * G + group; row < p.rows; row += (int64_t)gridDim.x * G) {
+    const float mu = p.stats[2 * row], r = p.stats[2 * row + 1];
+    float cen[NV][8], g[NV][8];
+    float sg = 0.f, sgc = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + lane);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { cen[i][j] = 0.f; g[i][j] = 0.f; }
+      if (c >= p.dim) continue;
+      if constexpr (PACKED) {
+        const uint64_t code = *reinterpret_cast<const uint64_t*>(p.codes + row * p.code_s + c);
+        unpack_codes(code, p.exps[(row * p.code_s + c) / kPackGroup], cen[i]);
+      } else {
+        load8(reinterpret_cast<const T*>(p.h) + row * p.h_s + c, p.dim - c, cen[i]);
+      }
+      load8(reinterpret_cast<const T*>(p.dy) + row * p.dy_s + c, p.dim - c, g[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        // beyond the row g is 0, which keeps these channels out of every sum
+        cen[i][j] = (cen[i][j] - mu) * r;
+        db[i][j] += g[i][j];
+        dw[i][j] += 8 * (i * TPR + lane) + j < p.dim ? g[i][j] * cen[i][j] : 0.f;
+        g[i][j] *= w[i][j];
+        sg += g[i][j];
+        sgc += 8 * (i * TPR + lane) + j < p.dim ? g[i][j] * cen[i][j] : 0.f;
+      }
+    const float mg = sum(sg) * inv, mgc = sum(sgc) * inv;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + lane);
+      if (c >= p.dim) continue;
+      float o[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = r * (g[i][j] - mg - cen[i][j] * mgc);
+      if (p.d_h) {
+        float q[8];
+        load8(reinterpret_cast<const T*>(p.d_h) + row * p.dh_s + c, p.dim - c, q);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] += q[j];
+      }
+      store8(reinterpret_cast<T*>(p.dx) + row * p.dx_s + c, p.dim - c, o);
+    }
+  }
+  if (!p.part) return;
+  // the groups' sums, first to last, into this workgroup's rows of the partials (dw at 0, db at 1)
+  for (int which = 0; which < 2; ++which) {
+    float* dst = p.part + ((int64_t)which * gridDim.x + blockIdx.x) * p.dim;
+    if constexpr (G > 1) {
+      if (which) __syncthreads();
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          park[(group * NV + i) * TPR * 8 + lane * 8 + j] = which ? db[i][j] : dw[i][j];
+      __syncthreads();
+      for (int c = threadIdx.x; c < p.dim; c += kThreads<TPR>) {
+        float s = 0.f;
+        for (int k = 0; k < G; ++k) s += park[k * NV * TPR * 8 + c];
+        dst[c] = s;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = 8 * (i * TPR + lane);
+        if (c < p.dim) store8(dst + c, p.dim - c, which ? db[i] : dw[i]);
+      }
+    }
+  }
+}
+
+// dw / db: 64 columns a workgroup, the partials' rows dealt to its 4 waves in order and joined in order.
+__global__ __launch_bounds__(256) void norm_params_kernel(const float* part, int nb, int dim, void* dw, void* db,
+                                                          int f32) {
+  __shared__ float park[4][64];
+  const int which = blockIdx.y, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + (threadIdx.x & 63);
+  void* dst = which ? db : dw;
+  if (!dst) return;
+  const float* src = part + (int64_t)which * nb * dim;
+  const int per = (nb + 3) / 4, lo = wave * per, hi = min(nb, lo + per);
+  float s = 0.f;
+  if (c < dim)
+    for (int b = lo; b < hi; ++b) s += src[(int64_t)b * dim + c];
+  park[wave][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (wave == 0 && c < dim) {
+    const float t = park[0][threadIdx.x] + park[1][threadIdx.x] + park[2][threadIdx.x] + park[3][threadIdx.x];
+    if (f32) reinterpret_cast<float*>(dst)[c] = t;
+    else reinterpret_cast<bf16*>(dst)[c] = (bf16)t;
+  }
+}
+
+// One chunk of 8 channels a thread; 8 threads hold a group.
+template <typename T>
+__global__ __launch_bounds__(256) void pack_kernel(PackParams p) {
+  const int64_t per = p.code_s / 8, total = p.rows * per;
+  for (int64_t i0 = (int64_t)blockIdx.x * 256; i0 < total; i0 += (int64_t)gridDim.x * 256) {
+    const int64_t i = i0 + threadIdx.x;          // total is a multiple of 8: groups are whole
+    if (i >= total) break;
+    const int64_t row = i / per;
+    const int c = (int)(i - row * per) * 8;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (c < p.dim) load8(reinterpret_cast<const T*>(p.x) + row * p.x_s + c, p.dim - c, v);
+    const uint32_t e = pack_exponent(v);
+    *reinterpret_cast<uint64_t*>(p.codes + 8 * i) = pack_codes(v, e);
+    if ((threadIdx.x & 7) == 0) p.exps[i / 8] = (uint8_t)e;
+  }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void unpack_kernel(PackParams p) {
+  const int64_t per = (p.dim + 7) / 8, total = p.rows * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / per;
+    const int c = (int)(i - row * per) * 8;
+    const int64_t at = row * p.code_s + c;
+    float v[8];
+    unpack_codes(*reinterpret_cast<const uint64_t*>(p.codes + at), p.exps[at / kPackGroup], v);
+    store8(reinterpret_cast<T*>(p.out) + row * p.x_s + c, p.dim - c, v);
+  }
+}
+
+// Calls f with (TPR, NV) of the group that holds a row of dim channels.
+template <int TPR, int NV> struct Group {};
+template <typename F>
+auto with_group(int dim, F&& f) {
+  if (dim <= 64) return f(Group<8, 1>{});
+  if (dim <= 128) return f(Group<16, 1>{});
+  if (dim <= 256) return f(Group<32, 1>{});
+  if (dim <= 512) return f(Group<64, 1>{});
+  if (dim <= 1024) return f(Group<64, 2>{});
+  if (dim <= 2048) return f(Group<64, 4>{});
+  if (dim <= 4096) return f(Group<256, 2>{});
+  if (dim <= 8192) return f(Group<256, 4>{});
+  return f(Group<1024, 2>{});
+}
+
+template <typename T, int TPR, int NV>
+hipError_t run_fwd(const NormParams& p, hipStream_t st, Group<TPR, NV>) {
+  constexpr int G = kThreads<TPR> / TPR;
+  norm_fwd_kernel<T, TPR, NV><<<(unsigned)((p.rows + G - 1) / G), kThreads<TPR>, 0, st>>>(p);
+  return hipGetLastError();
+}
+
+template <int TPR, int NV>
+int bwd_blocks(int64_t rows, Group<TPR, NV>) {
+  constexpr int G = kThreads<TPR> / TPR;
+  const int64_t need = (rows + G - 1) / G, cap = TPR == 1024 ? 256 : 512;
+  return (int)(need < cap ? need : cap);
+}
+
+template <typename T, int TPR, int NV>
+hipError_t run_bwd(const NormBwdParams& p, hipStream_t st, Group<TPR, NV> gr) {
+  const int nb = bwd_blocks(p.rows, gr);
+  if (p.codes) norm_bwd_kernel<T, TPR, NV, true><<<nb, kThreads<TPR>, 0, st>>>(p);
+  else norm_bwd_kernel<T, TPR, NV, false><<<nb, kThreads<TPR>, 0, st>>>(p);
+  if (p.part)
+    norm_params_kernel<<<dim3((p.dim + 63) / 64, 2), 256, 0, st>>>(p.part, nb, p.dim, p.dweight, p.dbias, p.w_f32);
+  return hipGetLastError();
+}
+
+__global__ __launch_bounds__(256) void zero_params_kernel(void* dw, void* db, int dim, int f32) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  void* dst = blockIdx.y ? db : dw;
+  if (!dst || c >= dim) return;
+  if (f32) reinterpret_cast<float*>(dst)[c] = 0.f;
+  else reinterpret_cast<bf16*>(dst)[c] = (bf16)0.f;
+}
+
+unsigned chunk_blocks(int64_t total) {
+  const int64_t b = (total + 255) / 256;
+  return (unsigned)(b < 8192 ? b : 8192);
+}
+
+}  // namespace
+
+hipError_t launch_norm_fwd(const NormParams& p, hipStream_t st) {
+  if (p.rows == 0) return hipSuccess;
+  return with_group(p.dim, [&](auto g) {
+    return p.dtype == DT_F32 ? run_fwd<float>(p, st, g) : run_fwd<bf16>(p, st, g);
+  });
+}
+
+size_t norm_bwd_workspace_bytes(int64_t rows, int dim) {
+  if (rows == 0) return 0;
+  return (size_t)with_group(dim, [&](auto g) { return bwd_blocks(rows, g); }) * dim * 2 * sizeof(float);
+}
+
+hipError_t launch_norm_bwd(const NormBwdParams& p, hipStream_t st) {
+  if (p.rows == 0) {
+    if (p.dweight || p.dbias)
+      zero_params_kernel<<<dim3((p.dim + 255) / 256, 2), 256, 0, st>>>(p.dweight, p.dbias, p.dim, p.w_f32);
+    return hipGetLastError();
+  }
+  return with_group(p.dim, [&](auto g) {
+    return p.dtype == DT_F32 ? run_bwd<float>(p, st, g) : run_bwd<bf16>(p, st, g);
+  });
+}
+
+hipError_t launch_pack(const PackParams& p, bool back, hipStream_t st) {
+  if (p.rows == 0) return hipSuccess;
+  const unsigned nb = chunk_blocks(p.rows * (p.code_s / 8));
+  if (p.dtype == DT_F32) {
+    if (back) unpack_kernel<float><<<nb, 256, 0, st>>>(p);
+    else pack_kernel<float><<<nb, 256, 0, st>>>(p);
+  } else {
+    if (back) unpack_kernel<bf16><<<nb, 256, 0, st>>>(p);
+    else pack_kernel<bf16><<<nb, 256, 0, st>>>(p);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace mh

@@ -1,0 +1,117 @@
+// Rows of channels as 8-element chunks, for the operators that walk (rows, dim) tensors of any width and row stride.
+// A chunk is one 16-byte (bf16) or two 16-byte (fp32) accesses that need the alignment of an element only (gfx950
+// takes unaligned vector accesses to global memory), so odd widths and strides run the same code as even ones; the
+// last chunk of a row whose width is no multiple of 8 goes element by element.
+#pragma once
+
+#include "common.h"
+
+namespace mh {
+
+typedef bf16x8 bf16x8_any __attribute__((aligned(2)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+
+__device__ __forceinline__ void load8(const bf16* p, float (&v)[8]) {
+  const bf16x8 b = *reinterpret_cast<const bf16x8_any*>(p);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = (float)b[j];
+}
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+  const f32x4 a = reinterpret_cast<const f32x4_any*>(p)[0], b = reinterpret_cast<const f32x4_any*>(p)[1];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+}
+// left: elements from p to the end of the row; those beyond it read as `pad`.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int left, float (&v)[8], float pad = 0.f) {
+  if (left >= 8) {
+    load8(p, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < left ? to_f32(p[j]) : pad;
+  }
+}
+
+__device__ __forceinline__ void store8(bf16* p, const float (&v)[8]) {
+  bf16x8 b;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) b[j] = (bf16)v[j];
+  *reinterpret_cast<bf16x8_any*>(p) = b;
+}
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+  reinterpret_cast<f32x4_any*>(p)[0] = f32x4{v[0], v[1], v[2], v[3]};
+  reinterpret_cast<f32x4_any*>(p)[1] = f32x4{v[4], v[5], v[6], v[7]};
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int left, const float (&v)[8]) {
+  if (left >= 8) {
+    store8(p, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < left) p[j] = from_f32<T>(v[j]);
+  }
+}
+
+// A parameter chunk in fp32 or bf16 (`f32` is uniform); element c of a vector of `dim`.
+__device__ __forceinline__ void load_par8(const void* p, bool f32, int c, int dim, float (&v)[8]) {
+  if (f32) load8(reinterpret_cast<const float*>(p) + c, dim - c, v);
+  else load8(reinterpret_cast<const bf16*>(p) + c, dim - c, v);
+}
+
+// Index i of a vector of 32- or 64-bit indices.
+__device__ __forceinline__ int64_t load_index(const void* p, bool i64, int64_t i) {
+  return i64 ? reinterpret_cast<const int64_t*>(p)[i] : (int64_t) reinterpret_cast<const int32_t*>(p)[i];
+}
+
+// Sum over aligned groups of N lanes (N a power of two up to 64), the same in every lane of the group.
+template <int N>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int off = N / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+// ---------------------------------------------------------------- activations in 8 bits
+// A group of 64 channels (8 lanes of one chunk each) shares an exponent e, the least with max|x| <= 127 2^e; a code
+// is x 2^-e rounded to nearest even, |code| <= 127, and stands for code 2^e: 8 significant bits at most, so a bf16 or
+// fp32 holds it exactly.  A power of two costs up to one bit of the 8 against a scale of max/127 but makes every step
+// exact.  The exponent is kept as a byte e + 132; e is at least -132, where all codes of a group below 2^-126 end.
+// 255 marks a group that holds an infinity or a NaN: all of it reads back as NaN, so that a diverged step is not hidden.
+constexpr int kPackGroup = 64;
+constexpr int kPackBias = 132;
+constexpr int kPackNan = 255;
+
+__device__ __forceinline__ uint32_t pack_exponent(const float (&x)[8]) {
+  uint32_t u = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) u = max(u, __float_as_uint(x[j]) & 0x7fffffffu);
+#pragma unroll
+  for (int off = 1; off < 8; off <<= 1) u = max(u, (uint32_t)__shfl_xor((int)u, off, 64));
+  if (u >= 0x7f800000u) return kPackNan;
+  // max = f 2^k, 1 <= f < 2: 127 2^(k - 6) is enough up to f = 127/64 (mantissa 0x7e0000)
+  const int k = max((int)(u >> 23), 1) - 127;
+  return (uint32_t)(k - 6 + ((u & 0x7fffffu) > 0x7e0000u && u >= 0x00800000u) + kPackBias);
+}
+__device__ __forceinline__ uint64_t pack_codes(const float (&x)[8], uint32_t byte) {
+  uint64_t c = 0;
+  if (byte != kPackNan) {
+    const int e = (int)byte - kPackBias;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int q = (int)__builtin_rintf(__builtin_amdgcn_ldexpf(x[j], -e));
+      c |= (uint64_t)(uint8_t)(int8_t)q << (8 * j);
+    }
+  }
+  return c;
+}
+__device__ __forceinline__ void unpack_codes(uint64_t c, uint32_t byte, float (&x)[8]) {
+  const int e = (int)byte - kPackBias;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float q = (float)(int8_t)(uint8_t)(c >> (8 * j));
+    x[j] = byte == kPackNan ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(q, e);
+  }
+}
+
+}  // namespace mh

@@ -10,6 +10,8 @@ This package restates, in float64 numpy, the arithmetic of the reference
   phi(x)=elu(x)+1 scan (mamformer/layers/kda_diff.py:67-89, 357-478, 564-605;
   mamformer/kernels/triton_ssd.py:121-181) and the decay-gated un-normalised
   recurrence that has no reference function (stated in closed form).
+* ``oracle.tokens`` -- the operators at the ends of a language model (token
+  table, layer norm, 8-bit activations, log probabilities) and their gradients.
 * ``oracle.baseline`` -- a torch-CPU restatement that keeps the reference's
   *cost structure* (materialised (b,L,d_inner,N) tensors and a per-timestep
   loop) so ``bench.py`` can time "the reference's CPU path".
