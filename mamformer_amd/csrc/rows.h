@@ -53,6 +53,37 @@ __device__ __forceinline__ void store8(T* p, int left, const float (&v)[8]) {
   }
 }
 
+// A chunk as it was loaded, so that what is fetched ahead holds no more registers than its bytes.
+template <typename T> struct Raw8;
+template <> struct Raw8<bf16> {
+  bf16x8 v;
+  __device__ __forceinline__ void load(const bf16* p, int left) {
+    if (left >= 8) {
+      v = *reinterpret_cast<const bf16x8_any*>(p);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j < left ? p[j] : (bf16)0.f;
+    }
+  }
+  __device__ __forceinline__ float get(int j) const { return (float)v[j]; }
+};
+template <> struct Raw8<float> {
+  f32x4 a, b;
+  __device__ __forceinline__ void load(const float* p, int left) {
+    if (left >= 8) {
+      a = reinterpret_cast<const f32x4_any*>(p)[0];
+      b = reinterpret_cast<const f32x4_any*>(p)[1];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        a[j] = j < left ? p[j] : 0.f;
+        b[j] = 4 + j < left ? p[4 + j] : 0.f;
+      }
+    }
+  }
+  __device__ __forceinline__ float get(int j) const { return j < 4 ? a[j] : b[j & 3]; }
+};
+
 // A parameter chunk in fp32 or bf16 (`f32` is uniform); element c of a vector of `dim`.
 __device__ __forceinline__ void load_par8(const void* p, bool f32, int c, int dim, float (&v)[8]) {
   if (f32) load8(reinterpret_cast<const float*>(p) + c, dim - c, v);
@@ -64,11 +95,18 @@ __device__ __forceinline__ int64_t load_index(const void* p, bool i64, int64_t i
   return i64 ? reinterpret_cast<const int64_t*>(p)[i] : (int64_t) reinterpret_cast<const int32_t*>(p)[i];
 }
 
-// Sum over aligned groups of N lanes (N a power of two up to 64), the same in every lane of the group.
+// Sum over aligned groups of N = 8, 16, 32 or 64 lanes, the same in every lane of the group: quad permutes and mirrors on
+// the DPP crossbar, then row and half swaps -- no LDS permutes.
 template <int N>
 __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-  for (int off = N / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  v = sum_quad(v);
+  v += dppf<0x141>(v);                           // row_half_mirror: the other quad of 8
+  if constexpr (N >= 16) v += dppf<0x140>(v);    // row_mirror: the other 8 of 16
+  if constexpr (N >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if constexpr (N >= 64) v = sum_halves(v);
   return v;
 }
 
@@ -105,13 +143,10 @@ __device__ __forceinline__ uint64_t pack_codes(const float (&x)[8], uint32_t byt
   }
   return c;
 }
-__device__ __forceinline__ void unpack_codes(uint64_t c, uint32_t byte, float (&x)[8]) {
-  const int e = (int)byte - kPackBias;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float q = (float)(int8_t)(uint8_t)(c >> (8 * j));
-    x[j] = byte == kPackNan ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(q, e);
-  }
+// What a code of 1 stands for (2^e, exact; NaN for the byte of a group that holds one).
+__device__ __forceinline__ float pack_step(uint32_t byte) {
+  return byte == kPackNan ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(1.f, (int)byte - kPackBias);
 }
+__device__ __forceinline__ float pack_code(uint64_t c, int j) { return (float)(int8_t)(uint8_t)(c >> (8 * j)); }
 
 }  // namespace mh
