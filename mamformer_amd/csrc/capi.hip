@@ -970,7 +970,8 @@ int logprob_validate(const mh_logprob_args* a, mh::LogprobParams& p) {
     MH_TRY(vec_ok(fn, "top_logprobs", a->top_logprobs, 4, a->top > 0));
   }
   p.rows = a->rows; p.vocab = a->vocab; p.ignore_index = a->ignore_index;
-  p.dtype = a->dtype; p.i64 = a->index_bytes == 8; p.top = a->top; p.inv_temp = 1.f / a->temperature;
+  p.dtype = a->dtype; p.i64 = a->index_bytes == 8; p.top = a->top;
+  p.k = (float)(1.4426950408889634 / a->temperature);
   p.logits = a->logits; p.l_s = a->logits_stride; p.targets = a->targets;
   p.logprobs = a->logprobs; p.entropy = a->entropy; p.stats = a->stats;
   p.top_ids = a->top_ids; p.top_logprobs = a->top_logprobs; p.workspace = a->workspace;
@@ -1587,14 +1588,14 @@ int mh_token_logprobs_workspace_bytes(const mh_logprob_args* a, size_t* bytes) {
   if (!bytes) return fail(MH_ERR_NULL, "token_logprobs: bytes output is NULL");
   mh::LogprobParams p;
   MH_TRY(logprob_validate(a, p));
-  *bytes = mh::logprob_workspace_bytes(p);
+  *bytes = mh::logprob_plan(p);
   return MH_OK;
 }
 
 int mh_token_logprobs_fwd(const mh_logprob_args* a, void* stream) {
   mh::LogprobParams p;
   MH_TRY(logprob_validate(a, p));
-  MH_TRY(workspace_ok("token_logprobs", a->workspace, a->workspace_bytes, mh::logprob_workspace_bytes(p)));
+  MH_TRY(workspace_ok("token_logprobs", a->workspace, a->workspace_bytes, mh::logprob_plan(p)));
   return hip_status(mh::launch_logprob(p, reinterpret_cast<hipStream_t>(stream)), "token_logprobs");
 }
 
@@ -1614,6 +1615,7 @@ int mh_token_logprobs_bwd(const mh_logprob_bwd_args* a, void* stream) {
   mh::LogprobBwdParams p;
   p.rows = a->rows; p.vocab = a->vocab; p.ignore_index = a->ignore_index;
   p.dtype = a->dtype; p.i64 = a->index_bytes == 8; p.inv_temp = 1.f / a->temperature;
+  p.k = (float)(1.4426950408889634 / a->temperature);
   p.logits = a->logits; p.l_s = a->logits_stride; p.targets = a->targets; p.stats = a->stats;
   p.d_logprobs = a->d_logprobs; p.d_entropy = a->d_entropy; p.dlogits = a->dlogits; p.d_s = a->dlogits_stride;
   return hip_status(mh::launch_logprob_bwd(p, reinterpret_cast<hipStream_t>(stream)), "token_logprobs_bwd");

@@ -426,21 +426,26 @@ constexpr int kMaxAlternatives = 64;
 struct LogprobParams {
   int64_t rows, vocab, ignore_index;
   int dtype, i64, top;
-  float inv_temp;
+  float k;                                 // log2(e) / temperature
   const void* logits; int64_t l_s;
   const void* targets;
   float* logprobs; float* entropy;         // entropy: or null
-  float* stats;                            // (rows, 3) max, ln of the sum, entropy
+  float* stats;                            // (rows, 3) offset, log2 of the sum, entropy
   int64_t* top_ids; float* top_logprobs;
   void* workspace;
+  // by logprob_plan
+  int64_t span;                            // columns of a workgroup, a multiple of 8
+  int spans;                               // of a row, up to 64
+  size_t keys_at;
 };
-size_t logprob_workspace_bytes(const LogprobParams& p);
+// Fills the plan's fields and returns the workspace bytes.
+size_t logprob_plan(LogprobParams& p);
 hipError_t launch_logprob(const LogprobParams& p, hipStream_t st);
 
 struct LogprobBwdParams {
   int64_t rows, vocab, ignore_index;
   int dtype, i64;
-  float inv_temp;
+  float inv_temp, k;
   const void* logits; int64_t l_s;
   const void* targets;
   const float* stats;

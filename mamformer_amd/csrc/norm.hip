@@ -54,7 +54,7 @@ template <typename T, int TPR, int NV>
 __global__ __launch_bounds__(kThreads<TPR>) void norm_fwd_kernel(NormParams p) {
   __shared__ float2 sums[2 * 16];
   const int lane = threadIdx.x % TPR;
-  const int64_t row = (int64_t)blockIdx.x * (kThreads<TPR> / TPR) + threadIdx.x / TPR;
+  const int64_t row = grid_row() * (kThreads<TPR> / TPR) + threadIdx.x / TPR;
   if (row >= p.rows) return;                     // whole groups, and whole workgroups where a group is one
   RowSum<TPR> sum(sums);
   const T* x = reinterpret_cast<const T*>(p.x) + row * p.x_s;
@@ -345,7 +345,7 @@ auto with_bwd_group(int dim, F&& f) {
 template <typename T, int TPR, int NV>
 hipError_t run_fwd(const NormParams& p, hipStream_t st, Group<TPR, NV>) {
   constexpr int G = kThreads<TPR> / TPR;
-  norm_fwd_kernel<T, TPR, NV><<<(unsigned)((p.rows + G - 1) / G), kThreads<TPR>, 0, st>>>(p);
+  norm_fwd_kernel<T, TPR, NV><<<row_grid((p.rows + G - 1) / G, 1), kThreads<TPR>, 0, st>>>(p);
   return hipGetLastError();
 }
 

@@ -95,6 +95,15 @@ __device__ __forceinline__ int64_t load_index(const void* p, bool i64, int64_t i
   return i64 ? reinterpret_cast<const int64_t*>(p)[i] : (int64_t) reinterpret_cast<const int32_t*>(p)[i];
 }
 
+// One workgroup for each of `n` things along a grid of at most 2^20 by z (a grid's threads along x have to stay below
+// 2^32); grid_row() is the workgroup's own, which may lie behind the last one.
+constexpr int64_t kGridRows = (int64_t)1 << 20;
+inline dim3 row_grid(int64_t n, unsigned y) {
+  const int64_t x = n < kGridRows ? n : kGridRows;
+  return dim3((unsigned)x, y, (unsigned)((n + x - 1) / x));
+}
+__device__ __forceinline__ int64_t grid_row() { return (int64_t)blockIdx.z * kGridRows + blockIdx.x; }
+
 // Sum over aligned groups of N = 8, 16, 32 or 64 lanes, the same in every lane of the group: quad permutes and mirrors on
 // the DPP crossbar, then row and half swaps -- no LDS permutes.
 template <int N>

@@ -420,6 +420,60 @@ def test_alternatives_in_hard_orders(dtype):
         assert np.array_equal(out.top_ids.cpu().numpy(), order)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("temp", [0.4, 1.0, 3.0])
+def test_long_rows_with_masks(temp, dtype):
+    """Few long rows, which are cut into spans: spans that hold nothing, the type's lowest value in whole spans and in whole
+    rows (over a temperature below 1 it leaves the type's range), a NaN, equal values over the borders."""
+    V, top = 20011, 64
+    low = torch.finfo(dtype).min
+    z = torch.randn(7, V, device="cuda").to(dtype)
+    z[0, 9000:] = -float("inf")
+    z[0, :30] = -float("inf")
+    z[1] = -float("inf")
+    z[1, V - 3:] = torch.tensor([1.0, 3.0, 2.0], dtype=dtype, device="cuda")
+    z[2] = low
+    z[3, 5000:] = low
+    z[4, 12345] = float("nan")
+    z[5] = 0.25
+    z[6] = low
+    z[6, ::7] = -float("inf")
+    t = torch.tensor([100, V - 2, 5, 3, 0, V - 1, 8], device="cuda")
+    say(f"long masked rows {dtype} T={temp}")
+    out = mh.token_logprobs(z, t, temperature=temp, top=top)
+    with np.errstate(invalid="ignore"):
+        lp, ent, ids, alt, lnp = tk.token_logprobs(host(z), host(t).astype(int), temp, top)
+    assert np.array_equal(out.top_ids.cpu().numpy(), ids)
+    # sums of V / 256 + 8 values a thread at most, 6 + 4 + 6 joins of 4 roundings, and |l| <= ln V + 6 / temp
+    k = 2 * (V / 256 + 64) + 4 * np.log(V) + 16
+    scale = 1 + np.log(V) + 6 / temp
+    near("logprobs", out.logprobs, lp, scale, k)
+    near("entropy", out.entropy, ent, scale, k)
+    near("top_logprobs", out.top_logprobs, alt, scale, k)
+    g = torch.linspace(0.5, 1.5, 7, device="cuda")
+    d = mh.token_logprobs_bwd(z, t, out.stats, g, -g, temperature=temp)
+    ok = [0, 1, 2, 3, 5, 6]
+    ref = tk.token_logprobs_bwd(lnp, ent, host(t).astype(int), host(g), -host(g), temp)
+    with np.errstate(invalid="ignore"):
+        mag = np.exp(lnp) * (2 + ent[:, None] + np.where(np.isfinite(lnp), np.abs(lnp), 0))
+    mag[np.arange(7), host(t).astype(int)] += 1
+    near("dlogits", d[ok], ref[ok], mag[ok] * host(g)[ok, None] / temp, k + 4 * np.abs(lnp[ok][np.isfinite(lnp[ok])]).max() + 8)
+    assert d[4].isnan().all()
+
+
+def test_token_logprobs_of_very_many_rows():
+    """More rows than a grid takes along one axis: each row is the same as in a call of its own."""
+    R = (1 << 20) + 5
+    z = torch.randn(R, 3, device="cuda").to(BF)
+    t = torch.arange(R, device="cuda") % 3
+    out = mh.token_logprobs(z, t, top=2)
+    d = mh.token_logprobs_bwd(z, t, out.stats, out.entropy)
+    for s in (slice(0, 9), slice(R - 9, R)):
+        want = mh.token_logprobs(z[s], t[s], top=2)
+        assert all(torch.equal(p[s], q) for p, q in zip(out, want))
+        assert torch.equal(d[s], mh.token_logprobs_bwd(z[s], t[s], want.stats, want.entropy))
+
+
 def test_token_logprobs_strides_and_in_place():
     wide = torch.randn(2, 6, 515, device="cuda").to(BF)
     z = wide[:, :, 1:502]
