@@ -4,7 +4,9 @@
 //   dW[v] = scale sum of dy[t] over the tokens t with ids[t] = v != padding_idx, in the order of t.
 //
 // The gradient sorts (id, t) by id with a stable radix sort of 9 bits a pass (two passes up to 2^18 rows), so that the
-// sum of a row runs in the order of its tokens and gives the same bits at every call; no floating-point atomics.  The
+// sum of a row runs in the order of its tokens and gives the same bits at every call; no floating-point atomics.  Most of
+// what has to be moved is the table's zeros: the sort's launches carry them in workgroups of their own, a share a pass, so
+// that a pass (a chain of dependent steps on few CUs) costs no time of its own where the table is large.  The
 // sorted tokens are cut into pieces of equal length whatever their ids, so a word that fills a tenth of the batch is
 // summed by many workgroups.  A run of one id that lies within a piece is written to dW at once; a run that crosses a
 // border leaves fp32 partial rows, which embed_join_kernel adds in order.  Dropped tokens (padding, ids out of range)
@@ -18,21 +20,37 @@ namespace mh {
 namespace {
 
 constexpr int kBits = 9, kDigits = 1 << kBits;   // a pass: 512 counters, two a thread
+constexpr int kSortThreads = 1024;               // 64 tokens a wave of the smallest tile
+constexpr int64_t kDirect = 16384;               // up to here a pass counts all tokens by itself
 
+// cthreads threads (a power of two) take 8 columns each of kRows tokens, whose loads are all on their way at once.
 template <typename T>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(EmbedParams p) {
-  const int64_t per = (p.dim + 7) / 8, total = p.tokens * per;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t t = i / per;
-    const int c = (int)(i - t * per) * 8;
-    const int64_t id = load_index(p.ids, p.i64, t);
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (id >= 0 && id < p.vocab) {
-      load8(reinterpret_cast<const T*>(p.weight) + id * p.w_s + c, p.dim - c, v);
+  constexpr int kRows = 2;
+  const int lane = threadIdx.x & (p.cthreads - 1), groups = 256 / p.cthreads;
+  const int c = 8 * (blockIdx.y * p.cthreads + lane), left = p.dim - c;
+  const int64_t t0 = grid_row() * groups * kRows + threadIdx.x / p.cthreads;
+  if (left <= 0) return;
+  int64_t id[kRows];
+  Raw8<T> v[kRows];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= p.scale;
-    }
-    store8(reinterpret_cast<T*>(p.out) + t * p.out_s + c, p.dim - c, v);
+  for (int i = 0; i < kRows; ++i) {
+    const int64_t t = t0 + i * groups;
+    id[i] = t < p.tokens ? load_index(p.ids, p.i64, t) : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    v[i].clear();
+    if (id[i] >= 0 && id[i] < p.vocab) v[i].load(reinterpret_cast<const T*>(p.weight) + id[i] * p.w_s + c, left);
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int64_t t = t0 + i * groups;
+    if (t >= p.tokens) return;
+    float o[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = v[i].get(j) * p.scale;
+    store8(reinterpret_cast<T*>(p.out) + t * p.out_s + c, left, o);
   }
 }
 
@@ -59,99 +77,151 @@ __global__ __launch_bounds__(256) void embed_count_kernel(EmbedBwdParams p) {
   h[threadIdx.x + 256] = cnt[threadIdx.x + 256];
 }
 
-// One stable pass.  Each wave owns a quarter of the tile and walks it 64 tokens at a time: a token's place is its
-// digit's start (all smaller digits, then the digit's tokens of earlier tiles, earlier waves and earlier steps) plus
-// the number of lanes before it with the same digit (ballots over the digit's bits).
-__global__ __launch_bounds__(256) void embed_sort_kernel(EmbedBwdParams p, int pass) {
-  __shared__ uint32_t at[4][kDigits];
-  __shared__ uint32_t wsum[4];
+// Zeros for share `pass` of the table's `passes` equal shares, by workgroup b of n.
+__device__ void clear_share(const EmbedBwdParams& p, int pass, int64_t b, int64_t n) {
+  typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+  const int64_t bytes = p.vocab * p.dim * (p.dw_f32 ? 4 : 2), share = (bytes / p.passes + 15) / 16 * 16;
+  const int64_t lo = pass * share, hi = pass + 1 == p.passes ? bytes : min(bytes, lo + share);
+  char* base = reinterpret_cast<char*>(p.dweight);
+  const u32x4_any z = {0u, 0u, 0u, 0u};
+  int64_t at = lo + 16 * (b * kSortThreads + threadIdx.x);
+  for (; at + 16 <= hi; at += 16 * kSortThreads * n) *reinterpret_cast<u32x4_any*>(base + at) = z;
+  for (; at < hi; at += 2) *reinterpret_cast<uint16_t*>(base + at) = 0;         // the last thread's tail, if any
+}
+__global__ __launch_bounds__(kSortThreads) void embed_clear_kernel(EmbedBwdParams p) {
+  for (int pass = 0; pass < p.passes; ++pass) clear_share(p, pass, blockIdx.x, gridDim.x);
+}
+
+// One stable pass.  Each of a workgroup's 16 waves owns a share of the tile and walks it 64 tokens at a time: a token's
+// place is its digit's start (all smaller digits, then the digit's tokens of earlier tiles, earlier waves and earlier
+// steps) plus the number of lanes before it with the same digit (ballots over the digit's bits).  The digits of the other
+// tiles are counted here from their keys where there are few (DIRECT: no launch and no atomics in memory for it; the
+// keys of 16384 tokens are 64 KB), or come from `hist`.  Workgroups beyond the tiles clear their share of the table.
+template <bool DIRECT>
+__global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedBwdParams p, int pass) {
+  constexpr int kWaves = kSortThreads / 64;
+  constexpr int kAhead = 4;                      // steps whose loads are on their way together
+  __shared__ uint32_t at[kWaves][kDigits];
+  __shared__ uint32_t early[DIRECT ? kDigits : 1], late[DIRECT ? kDigits : 1];
+  __shared__ uint32_t wsum[kDigits / 64];
+  if ((int)blockIdx.x >= p.tiles) return clear_share(p, pass, blockIdx.x - p.tiles, gridDim.x - p.tiles);
   const int lane = lane_id(), wave = wave_id(), shift = pass * kBits;
   const uint32_t* key_in = p.keys[pass & 1];
   const uint32_t* tok_in = p.order[pass & 1];
   uint32_t* key_out = p.keys[(pass & 1) ^ 1];
   uint32_t* tok_out = p.order[(pass & 1) ^ 1];
-  for (int i = threadIdx.x; i < 4 * kDigits; i += 256) at[0][i] = 0;
+  for (int i = threadIdx.x; i < kWaves * kDigits; i += kSortThreads) at[0][i] = 0;
+  if (DIRECT && threadIdx.x < kDigits) early[threadIdx.x] = late[threadIdx.x] = 0;
   __syncthreads();
-  const int64_t quarter = p.tile / 4, lo = (int64_t)blockIdx.x * p.tile + wave * quarter;
-  const int64_t hi = min(p.tokens, lo + quarter);
-  for (int64_t t = lo + lane; t < hi; t += 64) {
-    const uint32_t k = pass ? key_in[t] : token_key(p, t);
-    atomicAdd(&at[wave][(k >> shift) & (kDigits - 1)], 1u);
+  const int64_t part = p.tile / kWaves, first = (int64_t)blockIdx.x * p.tile, lo = first + wave * part;
+  const int64_t hi = min(p.tokens, lo + part);
+  auto digit = [&](int64_t t) {
+    return ((pass ? key_in[t] : token_key(p, t)) >> shift) & (kDigits - 1);
+  };
+  // digit x of thread x: its counts in earlier tiles and in all
+  uint32_t before = 0, total = 0;
+  if (DIRECT) {
+    const int bits = __builtin_ctzll(part);
+    for (int64_t t0 = threadIdx.x; t0 < p.tokens; t0 += kSortThreads * kAhead) {
+      uint32_t d[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) d[i] = t0 + kSortThreads * i < p.tokens ? digit(t0 + kSortThreads * i) : 0;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int64_t t = t0 + kSortThreads * i;
+        if (t >= p.tokens) break;
+        uint32_t* n = t < first ? early : t >= first + p.tile ? late : at[(t - first) >> bits];
+        atomicAdd(&n[d[i]], 1u);
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x < kDigits) {
+      before = early[threadIdx.x];
+      total = before + late[threadIdx.x];
+      for (int w = 0; w < kWaves; ++w) total += at[w][threadIdx.x];
+    }
+  } else {
+    for (int64_t t0 = lo + lane; t0 < hi; t0 += 64 * kAhead) {
+      uint32_t d[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) d[i] = t0 + 64 * i < hi ? digit(t0 + 64 * i) : 0;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (t0 + 64 * i < hi) atomicAdd(&at[wave][d[i]], 1u);
+    }
+    if (threadIdx.x < kDigits) {
+      const uint32_t* hist = p.hist + (int64_t)pass * p.tiles * kDigits + threadIdx.x;
+#pragma unroll 8
+      for (int b = 0; b < p.tiles; ++b) {
+        const uint32_t n = hist[b * kDigits];
+        before += b < (int)blockIdx.x ? n : 0;
+        total += n;
+      }
+    }
   }
-  // digits 2 x, 2 x + 1 of thread x: their counts in earlier tiles and in all
-  const uint32_t* hist = p.hist + (int64_t)pass * p.tiles * kDigits;
-  uint32_t before[2] = {0, 0}, total[2] = {0, 0};
-  for (int b = 0; b < p.tiles; ++b) {
-    const uint2 n = reinterpret_cast<const uint2*>(hist + (int64_t)b * kDigits)[threadIdx.x];
-    if (b < (int)blockIdx.x) { before[0] += n.x; before[1] += n.y; }
-    total[0] += n.x;
-    total[1] += n.y;
-  }
-  uint32_t incl = total[0] + total[1];
+  uint32_t incl = total;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
     const uint32_t o = (uint32_t)__shfl_up((int)incl, off, 64);
     if (lane >= off) incl += o;
   }
-  if (lane == 63) wsum[wave] = incl;
+  if (lane == 63 && wave < kDigits / 64) wsum[wave] = incl;
   __syncthreads();                               // also: every wave's counts are in `at`
-  uint32_t base = incl - total[0] - total[1];
-  for (int w = 0; w < wave; ++w) base += wsum[w];
-  uint32_t start[2] = {base + before[0], base + total[0] + before[1]};
+  if (threadIdx.x < kDigits) {
+    uint32_t start = incl - total + before;
+    for (int w = 0; w < wave; ++w) start += wsum[w];
 #pragma unroll
-  for (int d = 0; d < 2; ++d)
-    for (int w = 0; w < 4; ++w) {
-      const uint32_t n = at[w][2 * threadIdx.x + d];
-      at[w][2 * threadIdx.x + d] = start[d];
-      start[d] += n;
+    for (int w = 0; w < kWaves; ++w) {
+      const uint32_t n = at[w][threadIdx.x];
+      at[w][threadIdx.x] = start;
+      start += n;
     }
+  }
   __syncthreads();
-  uint32_t* next = pass + 1 < p.passes ? p.hist + (int64_t)(pass + 1) * p.tiles * kDigits : nullptr;
+  uint32_t* next = !DIRECT && pass + 1 < p.passes ? p.hist + (int64_t)(pass + 1) * p.tiles * kDigits : nullptr;
   volatile uint32_t* mine = at[wave];
-  for (int64_t t0 = lo; t0 < hi; t0 += 64) {
-    const int64_t t = t0 + lane;
-    const bool live = t < hi;
-    uint32_t k = 0, tok = 0;
-    if (live) {
-      k = pass ? key_in[t] : token_key(p, t);
-      tok = pass ? tok_in[t] : (uint32_t)t;
-    }
-    const uint32_t d = (k >> shift) & (kDigits - 1);
-    uint64_t same = __ballot(live);
+  for (int64_t t0 = lo; t0 < hi; t0 += 64 * kAhead) {
+    uint32_t key[kAhead], tok[kAhead];
 #pragma unroll
-    for (int bit = 0; bit < kBits; ++bit) {
-      const bool on = (d >> bit) & 1;
-      const uint64_t b = __ballot(on);
-      same &= on ? b : ~b;
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t t = t0 + 64 * i + lane;
+      key[i] = tok[i] = 0;
+      if (t < hi) {
+        key[i] = pass ? key_in[t] : token_key(p, t);
+        tok[i] = pass ? tok_in[t] : (uint32_t)t;
+      }
     }
-    const int rank = __popcll(same & (((uint64_t)1 << lane) - 1));
-    if (live) {
-      const uint32_t first = mine[d], pos = first + rank;
-      __builtin_amdgcn_wave_barrier();           // every lane has read its digit's place before the first lane moves it
-      if (rank == 0) mine[d] = first + (uint32_t)__popcll(same);
-      key_out[pos] = k;
-      tok_out[pos] = tok;
-      if (next) atomicAdd(&next[(int64_t)(pos / (uint32_t)p.tile) * kDigits + ((k >> (shift + kBits)) & (kDigits - 1))], 1u);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (t0 + 64 * i >= hi) break;
+      const bool live = t0 + 64 * i + lane < hi;
+      const uint32_t k = key[i], d = (k >> shift) & (kDigits - 1);
+      uint64_t same = __ballot(live);
+#pragma unroll
+      for (int bit = 0; bit < kBits; ++bit) {
+        const bool on = (d >> bit) & 1;
+        const uint64_t b = __ballot(on);
+        same &= on ? b : ~b;
+      }
+      const int rank = __popcll(same & (((uint64_t)1 << lane) - 1));
+      if (live) {
+        const uint32_t place = mine[d], pos = place + rank;
+        __builtin_amdgcn_wave_barrier();         // every lane has read its digit's place before the first lane moves it
+        if (rank == 0) mine[d] = place + (uint32_t)__popcll(same);
+        key_out[pos] = k;
+        tok_out[pos] = tok[i];
+        if (next) atomicAdd(&next[(int64_t)(pos / (uint32_t)p.tile) * kDigits + ((k >> (shift + kBits)) & (kDigits - 1))], 1u);
+      }
+      __builtin_amdgcn_wave_barrier();
     }
-    __builtin_amdgcn_wave_barrier();
   }
 }
 
-template <typename TW>
-__global__ __launch_bounds__(256) void embed_clear_kernel(EmbedBwdParams p) {
-  const int64_t per = (p.dim + 7) / 8, total = p.vocab * per;
-  const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t v = i / per;
-    const int c = (int)(i - v * per) * 8;
-    store8(reinterpret_cast<TW*>(p.dweight) + v * p.dim + c, p.dim - c, z);
-  }
-}
-
-// A piece of the sorted tokens and up to 2048 columns of it, 8 a thread.
+// A piece of the sorted tokens and up to 2048 columns of it, 8 a thread; the rows of 8 tokens are on their way at once.
 template <typename T, typename TW>
 __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedBwdParams p) {
-  const int lane = threadIdx.x % p.cthreads;
+  constexpr int kAhead = 8;                      // pieces are multiples of it
+  const int lane = threadIdx.x & (p.cthreads - 1);
   const int64_t piece = (int64_t)blockIdx.x * (256 / p.cthreads) + threadIdx.x / p.cthreads;
   const int c = 8 * (blockIdx.y * p.cthreads + lane), left = p.dim - c;
   if (piece >= p.pieces || left <= 0) return;
@@ -160,8 +230,9 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedBwdParams p) {
   const int64_t lo = piece * p.piece, hi = min(p.tokens, lo + p.piece);
   const T* dy = reinterpret_cast<const T*>(p.dy) + c;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const uint32_t prev = lo > 0 ? keys[lo - 1] : 0xffffffffu, after = hi < p.tokens ? keys[hi] : 0xffffffffu;
   uint32_t cur = keys[lo];
-  bool cont = lo > 0 && keys[lo - 1] == cur;     // the run began in an earlier piece
+  bool cont = prev == cur;                       // the run began in an earlier piece
   auto flush = [&](bool goes_on) {
     if (cont || goes_on) {
       store8(p.part + (2 * piece + (cont ? 0 : 1)) * (int64_t)p.dim + c, left, acc);
@@ -171,73 +242,123 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedBwdParams p) {
       store8(reinterpret_cast<TW*>(p.dweight) + (int64_t)cur * p.dim + c, left, acc);
     }
   };
-  for (int64_t i = lo; i < hi; ++i) {
-    const uint32_t k = keys[i];
-    if (k != cur) {
-      flush(false);
+  for (int64_t i0 = lo; i0 < hi; i0 += kAhead) {
+    uint32_t k[kAhead], tok[kAhead];
+    Raw8<T> v[kAhead];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-      cur = k;
-      cont = false;
+    for (int i = 0; i < kAhead; ++i) {
+      k[i] = i0 + i < hi ? keys[i0 + i] : 0xffffffffu;
+      tok[i] = i0 + i < hi ? order[i0 + i] : 0u;
     }
-    if (k >= (uint32_t)p.vocab) return;          // only dropped tokens follow
-    float v[8];
-    load8(dy + (int64_t)order[i] * p.dy_s, left, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] += v[j];
+    for (int i = 0; i < kAhead; ++i)
+      if (k[i] < (uint32_t)p.vocab) v[i].load(dy + (int64_t)tok[i] * p.dy_s, left);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (i0 + i >= hi) break;
+      if (k[i] != cur) {
+        flush(false);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+        cur = k[i];
+        cont = false;
+      }
+      if (k[i] >= (uint32_t)p.vocab) return;     // only dropped tokens follow
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] += v[i].get(j);
+    }
   }
-  flush(hi < p.tokens && keys[hi] == cur);
+  flush(after == cur);
 }
 
-// The run that begins in this piece and goes beyond it, if there is one: its partial rows in order.
+// The run that begins in this piece and goes beyond it, if there is one: 512 columns of its partial rows, a quarter of the
+// rows a wave, the quarters joined in order.
 template <typename TW>
 __global__ __launch_bounds__(256) void embed_join_kernel(EmbedBwdParams p) {
+  __shared__ float park[3][8][64];
   const uint32_t* keys = p.keys[p.passes & 1];
+  const int lane = lane_id(), wave = wave_id();
   const int64_t piece = blockIdx.x, lo = piece * p.piece, hi = lo + p.piece;
   if (hi >= p.tokens) return;
-  const uint32_t cur = keys[hi - 1];
-  if (cur >= (uint32_t)p.vocab || keys[hi] != cur) return;
-  if (keys[lo] == cur && lo > 0 && keys[lo - 1] == cur) return;       // an earlier piece's
-  const int c = 8 * (blockIdx.y * 256 + threadIdx.x), left = p.dim - c;
-  if (left <= 0) return;
-  float acc[8], v[8];
-  load8(p.part + (2 * piece + 1) * (int64_t)p.dim + c, left, acc);
-  for (int64_t q = piece + 1; q < p.pieces && keys[q * p.piece] == cur; ++q) {
-    load8(p.part + 2 * q * (int64_t)p.dim + c, left, v);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] += v[j];
+  const uint32_t cur = keys[hi - 1], after = keys[hi], first = keys[lo], prev = lo > 0 ? keys[lo - 1] : 0xffffffffu;
+  if (cur >= (uint32_t)p.vocab || after != cur) return;
+  if (first == cur && prev == cur) return;       // an earlier piece's
+  int n = 1;                                     // the pieces that begin in the run follow this one
+  for (int64_t q = piece + 1;; q += 64) {
+    const bool in = q + lane < p.pieces && keys[(q + lane) * p.piece] == cur;
+    const uint64_t out = ~__ballot(in);
+    n += out ? __builtin_ctzll(out) : 64;
+    if (out) break;
   }
+  const int c = 8 * (blockIdx.y * 64 + lane), left = p.dim - c;
+  const int per = (n + 3) / 4, from = wave * per, to = min(n, from + per);
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (left > 0) {
+#pragma unroll 4
+    for (int i = from; i < to; ++i) {
+      float v[8];
+      load8(p.part + (2 * (piece + i) + (i ? 0 : 1)) * (int64_t)p.dim + c, left, v);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) acc[j] *= p.scale;
+      for (int j = 0; j < 8; ++j) acc[j] += v[j];
+    }
+  }
+  if (wave > 0)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) park[wave - 1][j][lane] = acc[j];
+  __syncthreads();
+  if (wave > 0 || left <= 0) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    for (int w = 0; w < 3; ++w) acc[j] += park[w][j][lane];
+    acc[j] *= p.scale;
+  }
   store8(reinterpret_cast<TW*>(p.dweight) + (int64_t)cur * p.dim + c, left, acc);
 }
 
-unsigned chunk_blocks(int64_t total) {
-  const int64_t b = (total + 255) / 256;
-  return (unsigned)(b < 8192 ? b : 8192);
+// 64 KB a workgroup, two workgroups a CU at most.
+unsigned clear_blocks(int64_t bytes) {
+  const int64_t b = (bytes + 65535) / 65536;
+  return (unsigned)(b < 512 ? b : 512);
+}
+
+// Threads a row, a power of two from 8 to 256, of 8 columns each.
+int row_threads(int dim) {
+  int n = 8;
+  while (n < 256 && 8 * n < dim) n *= 2;
+  return n;
 }
 
 template <typename T, typename TW>
 hipError_t run_bwd(const EmbedBwdParams& p, hipStream_t st) {
-  embed_clear_kernel<TW><<<chunk_blocks(p.vocab * ((p.dim + 7) / 8)), 256, 0, st>>>(p);
-  if (p.tokens == 0) return hipGetLastError();
-  embed_count_kernel<<<p.tiles, 256, 0, st>>>(p);
-  for (int pass = 0; pass < p.passes; ++pass) embed_sort_kernel<<<p.tiles, 256, 0, st>>>(p, pass);
+  const int64_t bytes = p.vocab * p.dim * (int64_t)sizeof(TW);
+  if (p.tokens == 0) {
+    embed_clear_kernel<<<clear_blocks(bytes), kSortThreads, 0, st>>>(p);
+    return hipGetLastError();
+  }
+  const unsigned grid = p.tiles + clear_blocks(bytes / p.passes + 16);
+  const bool direct = p.tokens <= kDirect;
+  if (!direct) embed_count_kernel<<<p.tiles, 256, 0, st>>>(p);
+  for (int pass = 0; pass < p.passes; ++pass) {
+    if (direct) embed_sort_kernel<true><<<grid, kSortThreads, 0, st>>>(p, pass);
+    else embed_sort_kernel<false><<<grid, kSortThreads, 0, st>>>(p, pass);
+  }
   const int groups = 256 / p.cthreads;
   const unsigned slabs = (unsigned)((p.dim + 8 * p.cthreads - 1) / (8 * p.cthreads));
   embed_sum_kernel<T, TW><<<dim3((unsigned)((p.pieces + groups - 1) / groups), slabs), 256, 0, st>>>(p);
   if (p.pieces > 1)
-    embed_join_kernel<TW><<<dim3((unsigned)p.pieces, (unsigned)((p.dim + 2047) / 2048)), 256, 0, st>>>(p);
+    embed_join_kernel<TW><<<dim3((unsigned)p.pieces, (unsigned)((p.dim + 511) / 512)), 256, 0, st>>>(p);
   return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_embed_fwd(const EmbedParams& p, hipStream_t st) {
-  const int64_t total = p.tokens * ((p.dim + 7) / 8);
-  if (total == 0) return hipSuccess;
-  if (p.dtype == DT_F32) embed_fwd_kernel<float><<<chunk_blocks(total), 256, 0, st>>>(p);
-  else embed_fwd_kernel<bf16><<<chunk_blocks(total), 256, 0, st>>>(p);
+hipError_t launch_embed_fwd(EmbedParams p, hipStream_t st) {
+  if (p.tokens == 0) return hipSuccess;
+  p.cthreads = row_threads(p.dim);
+  const int64_t rows = 2 * (256 / p.cthreads);
+  const dim3 g = row_grid((p.tokens + rows - 1) / rows, (unsigned)((p.dim + 8 * p.cthreads - 1) / (8 * p.cthreads)));
+  if (p.dtype == DT_F32) embed_fwd_kernel<float><<<g, 256, 0, st>>>(p);
+  else embed_fwd_kernel<bf16><<<g, 256, 0, st>>>(p);
   return hipGetLastError();
 }
 
@@ -250,8 +371,7 @@ size_t embed_bwd_plan(EmbedBwdParams& p, void* workspace) {
   p.piece = 8;
   while (p.piece < 256 && p.tokens / p.piece > 1024) p.piece *= 2;
   p.pieces = (p.tokens + p.piece - 1) / p.piece;
-  p.cthreads = 8;
-  while (p.cthreads < 256 && 8 * p.cthreads < p.dim) p.cthreads *= 2;
+  p.cthreads = row_threads(p.dim);
   size_t off = 0;
   auto take = [&](size_t bytes) {
     void* q = workspace ? reinterpret_cast<char*>(workspace) + off : nullptr;

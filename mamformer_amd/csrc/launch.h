@@ -401,8 +401,9 @@ struct EmbedParams {
   const void* ids;
   const void* weight; int64_t w_s;
   void* out; int64_t out_s;
+  int cthreads;                            // by the launch: threads a row
 };
-hipError_t launch_embed_fwd(const EmbedParams& p, hipStream_t st);
+hipError_t launch_embed_fwd(EmbedParams p, hipStream_t st);
 
 struct EmbedBwdParams {
   int64_t tokens, vocab, padding_idx;      // padding_idx: -1 for none

@@ -65,6 +65,7 @@ template <> struct Raw8<bf16> {
       for (int j = 0; j < 8; ++j) v[j] = j < left ? p[j] : (bf16)0.f;
     }
   }
+  __device__ __forceinline__ void clear() { v = bf16x8{}; }
   __device__ __forceinline__ float get(int j) const { return (float)v[j]; }
 };
 template <> struct Raw8<float> {
@@ -81,6 +82,7 @@ template <> struct Raw8<float> {
       }
     }
   }
+  __device__ __forceinline__ void clear() { a = b = f32x4{}; }
   __device__ __forceinline__ float get(int j) const { return j < 4 ? a[j] : b[j & 3]; }
 };
 

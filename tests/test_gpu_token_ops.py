@@ -100,6 +100,25 @@ def test_embedding_of_one_token_only():
     assert not mh.embedding_bwd(dyg, ids + 2, 4).any()
 
 
+def test_embedding_of_very_many_tokens():
+    """More workgroups than a grid takes along one axis (64 tokens of one column each)."""
+    W = torch.randn(5, 1, device="cuda")
+    ids = torch.arange((1 << 26) + 3, device="cuda", dtype=torch.int32) % 5
+    assert torch.equal(mh.embedding(ids, W), W[ids.long()])
+
+
+@pytest.mark.parametrize("T", [1023, 1024, 1025, 16384, 16385])
+def test_embedding_gradient_at_the_borders_of_the_sort(T):
+    """Whole tiles, one token more and less, and both ways of counting; whole numbers, so every sum is exact."""
+    V, D = 1500, 5
+    g = torch.Generator(device="cuda").manual_seed(T)
+    ids = torch.randint(-1, V, (T,), generator=g, device="cuda")
+    dy = torch.randint(-8, 9, (T, D), generator=g, device="cuda").float()
+    live = ids >= 0
+    want = torch.zeros(V, D, device="cuda", dtype=torch.float64).index_add_(0, ids[live], dy[live].double())
+    assert torch.equal(mh.embedding_bwd(dy, ids, V), want.float())
+
+
 def test_embedding_strides_and_autograd():
     W, Wg = draw(5, 20, 24, dtype=BF)
     wide = torch.zeros(20, 50, device="cuda", dtype=BF)
