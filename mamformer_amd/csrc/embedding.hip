@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(EmbedParams p) {
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
     v[i].clear();
-    if (id[i] >= 0 && id[i] < p.vocab) v[i].load(reinterpret_cast<const T*>(p.weight) + id[i] * p.w_s + c, left);
+    if (id[i] >= 0 && id[i] < p.vocab) load_raw(v[i], reinterpret_cast<const T*>(p.weight) + id[i] * p.w_s + c, left);
   }
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
@@ -252,7 +252,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedBwdParams p) {
     }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
-      if (k[i] < (uint32_t)p.vocab) v[i].load(dy + (int64_t)tok[i] * p.dy_s, left);
+      if (k[i] < (uint32_t)p.vocab) load_raw(v[i], dy + (int64_t)tok[i] * p.dy_s, left);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       if (i0 + i >= hi) break;
@@ -319,13 +319,6 @@ __global__ __launch_bounds__(256) void embed_join_kernel(EmbedBwdParams p) {
 unsigned clear_blocks(int64_t bytes) {
   const int64_t b = (bytes + 65535) / 65536;
   return (unsigned)(b < 512 ? b : 512);
-}
-
-// Threads a row, a power of two from 8 to 256, of 8 columns each.
-int row_threads(int dim) {
-  int n = 8;
-  while (n < 256 && 8 * n < dim) n *= 2;
-  return n;
 }
 
 template <typename T, typename TW>

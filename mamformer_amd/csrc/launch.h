@@ -390,8 +390,9 @@ struct PackParams {
   const void* x; void* out; int64_t x_s;   // packed from x, unpacked to out
   uint8_t* codes; int64_t code_s;
   uint8_t* exps;
+  int cthreads;                            // by the launch: threads a row
 };
-hipError_t launch_pack(const PackParams& p, bool back, hipStream_t st);
+hipError_t launch_pack(PackParams p, bool back, hipStream_t st);
 
 // ------------------------------------------------------------- token table (embedding.hip)
 struct EmbedParams {

@@ -23,6 +23,7 @@
 // A row is one workgroup's, or where the rows are too few to fill the card the row is cut into spans, whose sums and
 // sorted alternatives logprob_join_kernel puts together.
 #include <float.h>
+#include <type_traits>
 
 #include "common.h"
 #include "launch.h"
@@ -39,6 +40,16 @@ constexpr float kSlack = 8.f;
 constexpr float kLn2 = 0.693147180559945f;
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The forward leaves the last rows, as many as the 256 MB cache in front of the memory holds, in it for the backward, which
+// takes the rows last to first; the rows before them, `left` and more from the end, go past it in both, and so does the
+// gradient.  8192 x 32000 bf16, forward and backward: 259 us (232 MB so: 262, 192 MB: 272, all rows past it: 291, all through
+// it: 318); 777 x 50001 fp32, whose logits fit: 91 us (gradient through it: 107, logits past it: 112).
+constexpr int64_t kCacheBytes = (int64_t)256 << 20;
+template <typename T>
+__device__ __forceinline__ bool past_cache(int64_t left, int64_t vocab) {
+  return left * vocab * (int64_t)sizeof(T) > kCacheBytes;
+}
 
 struct Soft {
   float m, s, u;
@@ -250,25 +261,29 @@ __global__ __launch_bounds__(kNT) void logprob_kernel(LogprobParams p) {
     }
     soft_add(a, v, cm, p.k);
   };
-  int64_t c = lo + 8 * threadIdx.x;
-  for (; c + 8 * kNT * (kAhead - 1) + 8 <= hi; c += 8 * kNT * kAhead) {
-    float v[kAhead][8];
+  auto read = [&](auto past) {
+    constexpr bool NT = decltype(past)::value;
+    int64_t c = lo + 8 * threadIdx.x;
+    for (; c + 8 * kNT * (kAhead - 1) + 8 <= hi; c += 8 * kNT * kAhead) {
+      float v[kAhead][8];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) load8(row + c + 8 * kNT * i, v[i]);
+      for (int i = 0; i < kAhead; ++i) load8<NT>(row + c + 8 * kNT * i, v[i]);
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) add(v[i], c + 8 * kNT * i);
-  }
-  for (; c < hi; c += 8 * kNT) {
-    float v[8];
-    const int left = (int)min(hi - c, (int64_t)8);
-    load8(row + c, left, v, -INFINITY);
-    add(v, c);
-  }
+      for (int i = 0; i < kAhead; ++i) add(v[i], c + 8 * kNT * i);
+    }
+    for (; c < hi; c += 8 * kNT) {
+      float v[8];
+      load8<NT>(row + c, (int)min(hi - c, (int64_t)8), v, -INFINITY);
+      add(v, c);
+    }
+  };
+  if (!TOP && past_cache<T>(p.rows - r, p.vocab)) read(std::true_type{});       // alternatives are read a second time
+  else read(std::false_type{});
   uint64_t bound = 0;
   if constexpr (TOP) {
     if (a.s != a.s) {                            // a NaN or an infinity in the share, which the maximum may have passed by
       uint64_t k = 0;
-      for (c = lo + 8 * threadIdx.x; c < hi; c += 8 * kNT)
+      for (int64_t c = lo + 8 * threadIdx.x; c < hi; c += 8 * kNT)
         for (int j = 0; j < 8 && c + j < hi; ++j) k = max(k, alt_key(to_f32(row[c + j]), (uint32_t)(c + j)));
       best = alt_value(k);
       best_at = lo + (alt_id(k) - lo) / 8 * 8;
@@ -329,7 +344,7 @@ __global__ __launch_bounds__(kNT) void logprob_join_kernel(LogprobParams p) {
   finish<T>(p, r, total, out);
 }
 
-// Rows last to first: what the forward read last is what the 256 MB cache in front of the memory still holds.
+// Rows last to first: what the forward read last is what the cache still holds.
 template <typename T>
 __global__ __launch_bounds__(kNT) void logprob_bwd_kernel(LogprobBwdParams p) {
   constexpr int kAhead = 2;
@@ -361,23 +376,28 @@ __global__ __launch_bounds__(kNT) void logprob_bwd_kernel(LogprobBwdParams p) {
       for (int j = 0; j < 8; ++j) v[j] += at + j == tgt ? g : 0.f;
     }
   };
-  for (; c + 8 * kNT * (kAhead - 1) + 8 <= hi; c += 8 * kNT * kAhead) {
-    float v[kAhead][8];
+  auto walk = [&](auto past) {
+    constexpr bool NT = decltype(past)::value;
+    for (; c + 8 * kNT * (kAhead - 1) + 8 <= hi; c += 8 * kNT * kAhead) {
+      float v[kAhead][8];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) load8(row + c + 8 * kNT * i, v[i]);
+      for (int i = 0; i < kAhead; ++i) load8<NT>(row + c + 8 * kNT * i, v[i]);
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      grad(v[i], c + 8 * kNT * i);
-      store8(out + c + 8 * kNT * i, v[i]);
+      for (int i = 0; i < kAhead; ++i) {
+        grad(v[i], c + 8 * kNT * i);
+        store8<true>(out + c + 8 * kNT * i, v[i]);
+      }
     }
-  }
-  for (; c < hi; c += 8 * kNT) {
-    float v[8];
-    const int left = (int)min(hi - c, (int64_t)8);
-    load8(row + c, left, v);
-    grad(v, c);
-    store8(out + c, left, v);
-  }
+    for (; c < hi; c += 8 * kNT) {
+      float v[8];
+      const int left = (int)min(hi - c, (int64_t)8);
+      load8<NT>(row + c, left, v);
+      grad(v, c);
+      store8<true>(out + c, left, v);
+    }
+  };
+  if (past_cache<T>(p.rows - r, p.vocab)) walk(std::true_type{});
+  else walk(std::false_type{});
 }
 
 }  // namespace

@@ -463,20 +463,20 @@ def test_long_rows_with_masks(temp, dtype):
     with np.errstate(invalid="ignore"):
         lp, ent, ids, alt, lnp = tk.token_logprobs(host(z), host(t).astype(int), temp, top)
     assert np.array_equal(out.top_ids.cpu().numpy(), ids)
-    # sums of V / 256 + 8 values a thread at most, 6 + 4 + 6 joins of 4 roundings, and |l| <= ln V + 6 / temp
-    k = 2 * (V / 256 + 64) + 4 * np.log(V) + 16
-    scale = 1 + np.log(V) + 6 / temp
-    near("logprobs", out.logprobs, lp, scale, k)
-    near("entropy", out.entropy, ent, scale, k)
-    near("top_logprobs", out.top_logprobs, alt, scale, k)
-    g = torch.linspace(0.5, 1.5, 7, device="cuda")
-    d = mh.token_logprobs_bwd(z, t, out.stats, g, -g, temperature=temp)
-    ok = [0, 1, 2, 3, 5, 6]
-    ref = tk.token_logprobs_bwd(lnp, ent, host(t).astype(int), host(g), -host(g), temp)
-    with np.errstate(invalid="ignore"):
+    with np.errstate(invalid="ignore"):                  # infinite and NaN entries are compared by their places
+        # sums of V / 256 + 8 values a thread at most, 6 + 4 + 6 joins of 4 roundings, and |l| <= ln V + 6 / temp
+        k = 2 * (V / 256 + 64) + 4 * np.log(V) + 16
+        scale = 1 + np.log(V) + 6 / temp
+        near("logprobs", out.logprobs, lp, scale, k)
+        near("entropy", out.entropy, ent, scale, k)
+        near("top_logprobs", out.top_logprobs, alt, scale, k)
+        g = torch.linspace(0.5, 1.5, 7, device="cuda")
+        d = mh.token_logprobs_bwd(z, t, out.stats, g, -g, temperature=temp)
+        ok = [0, 1, 2, 3, 5, 6]
+        ref = tk.token_logprobs_bwd(lnp, ent, host(t).astype(int), host(g), -host(g), temp)
         mag = np.exp(lnp) * (2 + ent[:, None] + np.where(np.isfinite(lnp), np.abs(lnp), 0))
-    mag[np.arange(7), host(t).astype(int)] += 1
-    near("dlogits", d[ok], ref[ok], mag[ok] * host(g)[ok, None] / temp, k + 4 * np.abs(lnp[ok][np.isfinite(lnp[ok])]).max() + 8)
+        mag[np.arange(7), host(t).astype(int)] += 1
+        near("dlogits", d[ok], ref[ok], mag[ok] * host(g)[ok, None] / temp, k + 4 * np.abs(lnp[ok][np.isfinite(lnp[ok])]).max() + 8)
     assert d[4].isnan().all()
 
 
