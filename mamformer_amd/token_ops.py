@@ -55,6 +55,11 @@ def _rows(t, D):
     return t if t.stride(1) == 1 or D == 1 else t.contiguous()
 
 
+def _empty(t):
+    """A contiguous tensor of the shape and dtype of t (for a contiguous t by the shorter way)."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, device=t.device, dtype=t.dtype)
+
+
 def _like(name, what, t, shape, dtype):
     if t.shape != shape or t.dtype is not dtype:
         raise ValueError(f"{name}: {what} must be {tuple(shape)} {dtype}, got {tuple(t.shape)} {t.dtype}")
@@ -72,15 +77,16 @@ def embedding(ids, weight, *, scale=1.0, padding_idx=None):
     _require_cuda("embedding", ids, weight)
     if weight.dim() != 2:
         raise ValueError(f"embedding: weight must be (V, D), got {tuple(weight.shape)}")
-    padding_idx = _padding(padding_idx, weight.shape[0])
-    if torch.is_grad_enabled() and weight.requires_grad:
+    if padding_idx is not None:
+        padding_idx = _padding(padding_idx, weight.shape[0])
+    if weight.requires_grad and torch.is_grad_enabled():
         return _EmbeddingFn.apply(weight, ids, scale, padding_idx)
     return _embedding_fwd(weight, ids, scale)
 
 
 def _padding(padding_idx, V):
     if padding_idx is None:
-        return -1
+        return -1                                # no row has it
     if not -V <= padding_idx < V:
         raise ValueError(f"embedding: padding_idx {padding_idx} outside a table of {V} rows")
     return padding_idx % V
@@ -91,7 +97,7 @@ def _embedding_fwd(weight, ids, scale):
     ids = _indices("embedding", "ids", ids)
     V, D = weight.shape
     w = _rows(weight, D)
-    out = torch.empty((*ids.shape, D), device=w.device, dtype=w.dtype)
+    out = w.new_empty((*ids.shape, D))
     n = ids.numel()
     if n and D:
         a = EmbeddingArgs(n, V, D, dt, ids.element_size(), scale, ids.data_ptr(), w.data_ptr(), w.stride(0),
@@ -143,7 +149,7 @@ class _EmbeddingFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         V, dtype, scale, pad = ctx.cfg
-        dw = embedding_bwd(dy, ctx.saved_tensors[0], V, scale=scale, padding_idx=None if pad < 0 else pad, dtype=dtype)
+        dw = embedding_bwd(dy, ctx.saved_tensors[0], V, scale=scale, padding_idx=pad, dtype=dtype)
         return dw, None, None, None
 
 
@@ -235,7 +241,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, residual=None, packed=Fal
     if residual is not None:
         _like(name, "residual", residual, x.shape, x.dtype)
     _norm_params(name, weight, bias, D)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad
+                                    or bias is not None and bias.requires_grad
+                                    or residual is not None and residual.requires_grad):
         y, h, codes, exps, stats = _LayerNormFn.apply(x, residual, weight, bias, eps, packed)
     else:
         y, h, codes, exps, stats = _layer_norm_fwd(x, residual, weight, bias, eps, packed, return_stats)
@@ -250,9 +258,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, residual=None, packed=Fal
 
 
 def _norm_params(name, weight, bias, D):
-    for what, t in (("weight", weight), ("bias", bias)):
-        if t is not None and (t.shape != (D,) or t.dtype not in _DT):
-            raise ValueError(f"{name}: {what} must be ({D},) float32 or bfloat16, got {tuple(t.shape)} {t.dtype}")
+    if weight is not None and (weight.shape != (D,) or weight.dtype not in _DT):
+        raise ValueError(f"{name}: weight must be ({D},) float32 or bfloat16, got {tuple(weight.shape)} {weight.dtype}")
+    if bias is not None and (bias.shape != (D,) or bias.dtype not in _DT):
+        raise ValueError(f"{name}: bias must be ({D},) float32 or bfloat16, got {tuple(bias.shape)} {bias.dtype}")
     if weight is not None and bias is not None and weight.dtype is not bias.dtype:
         raise TypeError(f"{name}: weight and bias must have one dtype, got {weight.dtype} and {bias.dtype}")
 
@@ -265,11 +274,11 @@ def _layer_norm_fwd(x, residual, weight, bias, eps, packed, stats):
     D, dev = x.shape[-1], x.device
     x2 = _rows(x, D)
     weight, bias = _vec(weight), _vec(bias)
-    y = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    y = _empty(x)
     h = codes = exps = st = res = None
     if residual is not None:
         res = _rows(residual, D)
-        h = torch.empty(x.shape, device=dev, dtype=x.dtype)
+        h = _empty(x)
     if packed:
         codes, exps = _packed_buffers(x.shape[:-1], D, dev)
     if stats:
@@ -313,8 +322,8 @@ def layer_norm_bwd(dy, h, stats, weight=None, *, d_h=None, bias=True):
         _like(name, "d_h", d_h, shape, dy.dtype)
         d_h = _rows(d_h, D)
     _norm_params(name, weight, None, D)
+    dx = _empty(dy)
     weight, stats, dy = _vec(weight), _vec(stats), _rows(dy, D)
-    dx = torch.empty(shape, device=dev, dtype=dy.dtype)
     par_dtype = dy.dtype if weight is None else weight.dtype
     dpar = None
     if weight is not None or bias:
@@ -389,7 +398,7 @@ def token_logprobs(logits, targets, *, temperature=1.0, top=0, ignore_index=-100
     name = "token_logprobs"
     _require_cuda(name, logits, targets)
     _logprob_shapes(name, logits, targets)
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if logits.requires_grad and torch.is_grad_enabled():
         return TokenLogprobs(*_TokenLogprobsFn.apply(logits, targets, temperature, top, ignore_index))
     return TokenLogprobs(*_token_logprobs_fwd(logits, targets, temperature, top, ignore_index))
 
@@ -447,7 +456,7 @@ def token_logprobs_bwd(logits, targets, stats, d_logprobs=None, d_entropy=None, 
         grads.append(t)
     l2 = _rows(logits, V)
     if out is None:
-        out = torch.empty(logits.shape, device=dev, dtype=logits.dtype)
+        out = _empty(logits)
         o2 = out if out.dim() == 2 else out.view(-1, V)
     else:
         _like(name, "out", out, logits.shape, logits.dtype)
