@@ -417,7 +417,7 @@ def _token_logprobs_fwd(logits, targets, temperature, top, ignore_index):
     rows = l2.shape[0]
     vals = torch.empty((2, *lead), device=dev, dtype=torch.float32)
     stats = torch.empty((*lead, 3), device=dev, dtype=torch.float32)
-    lp, ent = vals[0], vals[1]
+    lp, ent = vals.unbind(0)
     ids = alt = None
     if top:
         ids = torch.empty((*lead, top), device=dev, dtype=torch.int64)
