@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kBits = 9, kDigits = 1 << kBits;   // a pass: 512 counters, two a thread
 constexpr int kSortThreads = 1024;               // 64 tokens a wave of the smallest tile
+constexpr int64_t kSmall = 2048;                 // up to here one workgroup sorts, two tokens a thread
 constexpr int64_t kDirect = 16384;               // up to here a pass counts all tokens by itself
 
 // cthreads threads (a power of two) take 8 columns each of kRows tokens, whose loads are all on their way at once.
@@ -90,6 +91,18 @@ __device__ void clear_share(const EmbedBwdParams& p, int pass, int64_t b, int64_
 }
 __global__ __launch_bounds__(kSortThreads) void embed_clear_kernel(EmbedBwdParams p) {
   for (int pass = 0; pass < p.passes; ++pass) clear_share(p, pass, blockIdx.x, gridDim.x);
+}
+
+// The lanes with this lane's digit (`same`), and how many of them come before it.
+__device__ __forceinline__ int digit_rank(uint32_t d, bool live, int lane, uint64_t& same) {
+  same = __ballot(live);
+#pragma unroll
+  for (int bit = 0; bit < kBits; ++bit) {
+    const bool on = (d >> bit) & 1;
+    const uint64_t b = __ballot(on);
+    same &= on ? b : ~b;
+  }
+  return __popcll(same & (((uint64_t)1 << lane) - 1));
 }
 
 // One stable pass.  Each of a workgroup's 16 waves owns a share of the tile and walks it 64 tokens at a time: a token's
@@ -196,14 +209,8 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedBwdParams
       if (t0 + 64 * i >= hi) break;
       const bool live = t0 + 64 * i + lane < hi;
       const uint32_t k = key[i], d = (k >> shift) & (kDigits - 1);
-      uint64_t same = __ballot(live);
-#pragma unroll
-      for (int bit = 0; bit < kBits; ++bit) {
-        const bool on = (d >> bit) & 1;
-        const uint64_t b = __ballot(on);
-        same &= on ? b : ~b;
-      }
-      const int rank = __popcll(same & (((uint64_t)1 << lane) - 1));
+      uint64_t same;
+      const int rank = digit_rank(d, live, lane, same);
       if (live) {
         const uint32_t place = mine[d], pos = place + rank;
         __builtin_amdgcn_wave_barrier();         // every lane has read its digit's place before the first lane moves it
@@ -214,6 +221,85 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedBwdParams
       }
       __builtin_amdgcn_wave_barrier();
     }
+  }
+}
+
+// Up to kSmall tokens: all passes in one workgroup, the tokens in registers and LDS, as embed_sort_kernel's otherwise.  The
+// other workgroups clear the table.
+__global__ __launch_bounds__(kSortThreads) void embed_sort_small_kernel(EmbedBwdParams p) {
+  constexpr int kWaves = kSortThreads / 64, kSteps = (int)(kSmall / kSortThreads);
+  __shared__ uint32_t at[kWaves][kDigits];
+  __shared__ uint32_t keys[kSmall], toks[kSmall];
+  __shared__ uint32_t wsum[kDigits / 64];
+  if (blockIdx.x > 0) {
+    for (int q = 0; q < p.passes; ++q) clear_share(p, q, blockIdx.x - 1, gridDim.x - 1);
+    return;
+  }
+  const int lane = lane_id(), wave = wave_id(), n = (int)p.tokens, lo = wave * 64 * kSteps + lane;
+  uint32_t key[kSteps], tok[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    tok[i] = lo + 64 * i;
+    key[i] = lo + 64 * i < n ? token_key(p, lo + 64 * i) : 0;
+  }
+  for (int pass = 0; pass < p.passes; ++pass) {
+    const int shift = pass * kBits;
+    for (int i = threadIdx.x; i < kWaves * kDigits; i += kSortThreads) at[0][i] = 0;
+    if (pass) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        key[i] = keys[lo + 64 * i];
+        tok[i] = toks[lo + 64 * i];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+      if (lo + 64 * i < n) atomicAdd(&at[wave][(key[i] >> shift) & (kDigits - 1)], 1u);
+    __syncthreads();
+    uint32_t total = 0;
+    if (threadIdx.x < kDigits)
+      for (int w = 0; w < kWaves; ++w) total += at[w][threadIdx.x];
+    uint32_t incl = total;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const uint32_t o = (uint32_t)__shfl_up((int)incl, off, 64);
+      if (lane >= off) incl += o;
+    }
+    if (lane == 63 && wave < kDigits / 64) wsum[wave] = incl;
+    __syncthreads();
+    if (threadIdx.x < kDigits) {
+      uint32_t start = incl - total;
+      for (int w = 0; w < wave; ++w) start += wsum[w];
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const uint32_t c = at[w][threadIdx.x];
+        at[w][threadIdx.x] = start;
+        start += c;
+      }
+    }
+    __syncthreads();
+    volatile uint32_t* mine = at[wave];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const bool live = lo + 64 * i < n;
+      const uint32_t d = (key[i] >> shift) & (kDigits - 1);
+      uint64_t same;
+      const int rank = digit_rank(d, live, lane, same);
+      if (live) {
+        const uint32_t place = mine[d], pos = place + rank;
+        __builtin_amdgcn_wave_barrier();         // every lane has read its digit's place before the first lane moves it
+        if (rank == 0) mine[d] = place + (uint32_t)__popcll(same);
+        keys[pos] = key[i];
+        toks[pos] = tok[i];
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < n; i += kSortThreads) {
+    p.keys[p.passes & 1][i] = keys[i];
+    p.order[p.passes & 1][i] = toks[i];
   }
 }
 
@@ -271,48 +357,53 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedBwdParams p) {
   flush(after == cur);
 }
 
-// The run that begins in this piece and goes beyond it, if there is one: 512 columns of its partial rows, a quarter of the
-// rows a wave, the quarters joined in order.
-template <typename TW>
+// The runs that begin in this workgroup's pieces and go beyond their piece: cthreads threads, a wave (WAVE) at most, of 8 columns each,
+// the partial rows in equal shares to the workgroup's groups of threads, the shares joined in order.
+template <typename TW, bool WAVE>
 __global__ __launch_bounds__(256) void embed_join_kernel(EmbedBwdParams p) {
-  __shared__ float park[3][8][64];
+  __shared__ float park[8][256];
   const uint32_t* keys = p.keys[p.passes & 1];
-  const int lane = lane_id(), wave = wave_id();
-  const int64_t piece = blockIdx.x, lo = piece * p.piece, hi = lo + p.piece;
-  if (hi >= p.tokens) return;
-  const uint32_t cur = keys[hi - 1], after = keys[hi], first = keys[lo], prev = lo > 0 ? keys[lo - 1] : 0xffffffffu;
-  if (cur >= (uint32_t)p.vocab || after != cur) return;
-  if (first == cur && prev == cur) return;       // an earlier piece's
-  int n = 1;                                     // the pieces that begin in the run follow this one
-  for (int64_t q = piece + 1;; q += 64) {
-    const bool in = q + lane < p.pieces && keys[(q + lane) * p.piece] == cur;
-    const uint64_t out = ~__ballot(in);
-    n += out ? __builtin_ctzll(out) : 64;
-    if (out) break;
-  }
-  const int c = 8 * (blockIdx.y * 64 + lane), left = p.dim - c;
-  const int per = (n + 3) / 4, from = wave * per, to = min(n, from + per);
-  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (left > 0) {
-#pragma unroll 4
-    for (int i = from; i < to; ++i) {
-      float v[8];
-      load8(p.part + (2 * (piece + i) + (i ? 0 : 1)) * (int64_t)p.dim + c, left, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] += v[j];
+  const int jt = WAVE ? 64 : p.cthreads, groups = 256 / jt, group = WAVE ? wave_id() : threadIdx.x / jt;
+  const int c = 8 * (blockIdx.y * jt + (threadIdx.x & (jt - 1))), left = p.dim - c;
+  const int64_t end = min(p.pieces, (int64_t)(blockIdx.x + 1) * p.join);
+  for (int64_t piece = (int64_t)blockIdx.x * p.join; piece < end; ++piece) {
+    const int64_t lo = piece * p.piece, hi = lo + p.piece;
+    if (hi >= p.tokens) return;
+    const uint32_t cur = keys[hi - 1], after = keys[hi], first = keys[lo], prev = lo > 0 ? keys[lo - 1] : 0xffffffffu;
+    if (cur >= (uint32_t)p.vocab) return;
+    if (after != cur || (first == cur && prev == cur)) continue;      // ends here, or is an earlier piece's
+    int n = 1;                                   // the pieces that begin in the run follow this one
+    for (int64_t q = piece + 1;; q += 64) {
+      const bool in = q + lane_id() < p.pieces && keys[(q + lane_id()) * p.piece] == cur;
+      const uint64_t out = ~__ballot(in);
+      n += out ? __builtin_ctzll(out) : 64;
+      if (out) break;
     }
-  }
-  if (wave > 0)
+    const int per = (n + groups - 1) / groups, from = group * per, to = min(n, from + per);
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (left > 0) {
+#pragma unroll 4
+      for (int i = from; i < to; ++i) {
+        float v[8];
+        load8(p.part + (2 * (piece + i) + (i ? 0 : 1)) * (int64_t)p.dim + c, left, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) park[wave - 1][j][lane] = acc[j];
-  __syncthreads();
-  if (wave > 0 || left <= 0) return;
+        for (int j = 0; j < 8; ++j) acc[j] += v[j];
+      }
+    }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    for (int w = 0; w < 3; ++w) acc[j] += park[w][j][lane];
-    acc[j] *= p.scale;
+    for (int j = 0; j < 8; ++j) park[j][threadIdx.x] = acc[j];
+    __syncthreads();
+    if (group == 0 && left > 0) {
+      const int used = (n + per - 1) / per;
+      for (int w = 1; w < used; ++w)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] += park[j][w * jt + threadIdx.x];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] *= p.scale;
+      store8(reinterpret_cast<TW*>(p.dweight) + (int64_t)cur * p.dim + c, left, acc);
+    }
+    __syncthreads();
   }
-  store8(reinterpret_cast<TW*>(p.dweight) + (int64_t)cur * p.dim + c, left, acc);
 }
 
 // 64 KB a workgroup, two workgroups a CU at most.
@@ -329,17 +420,21 @@ hipError_t run_bwd(const EmbedBwdParams& p, hipStream_t st) {
     return hipGetLastError();
   }
   const unsigned grid = p.tiles + clear_blocks(bytes / p.passes + 16);
-  const bool direct = p.tokens <= kDirect;
+  const bool direct = p.tokens <= kDirect, small = p.tokens <= kSmall;
+  if (small) embed_sort_small_kernel<<<1 + clear_blocks(bytes), kSortThreads, 0, st>>>(p);
   if (!direct) embed_count_kernel<<<p.tiles, 256, 0, st>>>(p);
-  for (int pass = 0; pass < p.passes; ++pass) {
+  for (int pass = 0; pass < p.passes && !small; ++pass) {
     if (direct) embed_sort_kernel<true><<<grid, kSortThreads, 0, st>>>(p, pass);
     else embed_sort_kernel<false><<<grid, kSortThreads, 0, st>>>(p, pass);
   }
-  const int groups = 256 / p.cthreads;
+  const int groups = 256 / p.cthreads, jt = p.cthreads < 64 ? p.cthreads : 64;
   const unsigned slabs = (unsigned)((p.dim + 8 * p.cthreads - 1) / (8 * p.cthreads));
   embed_sum_kernel<T, TW><<<dim3((unsigned)((p.pieces + groups - 1) / groups), slabs), 256, 0, st>>>(p);
-  if (p.pieces > 1)
-    embed_join_kernel<TW><<<dim3((unsigned)p.pieces, (unsigned)((p.dim + 511) / 512)), 256, 0, st>>>(p);
+  if (p.pieces > 1) {
+    const dim3 g((unsigned)((p.pieces + p.join - 1) / p.join), (unsigned)((p.dim + 8 * jt - 1) / (8 * jt)));
+    if (jt == 64) embed_join_kernel<TW, true><<<g, 256, 0, st>>>(p);
+    else embed_join_kernel<TW, false><<<g, 256, 0, st>>>(p);
+  }
   return hipGetLastError();
 }
 
@@ -361,10 +456,12 @@ size_t embed_bwd_plan(EmbedBwdParams& p, void* workspace) {
   p.tile = 1024;
   while ((p.tokens + p.tile - 1) / p.tile > 128) p.tile *= 2;
   p.tiles = (int)((p.tokens + p.tile - 1) / p.tile);
-  p.piece = 8;
-  while (p.piece < 256 && p.tokens / p.piece > 1024) p.piece *= 2;
-  p.pieces = (p.tokens + p.piece - 1) / p.piece;
   p.cthreads = row_threads(p.dim);
+  // the shortest pieces (their rows' loads go out together) that make no more than 8 workgroups a CU of the sums
+  p.piece = 8;
+  while (p.piece < 256 && p.tokens / p.piece * p.cthreads > (int64_t)2048 * 256) p.piece *= 2;
+  p.pieces = (p.tokens + p.piece - 1) / p.piece;
+  p.join = (p.pieces + 2047) / 2048;
   size_t off = 0;
   auto take = [&](size_t bytes) {
     void* q = workspace ? reinterpret_cast<char*>(workspace) + off : nullptr;

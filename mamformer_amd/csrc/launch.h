@@ -415,7 +415,7 @@ struct EmbedBwdParams {
   void* dweight;                           // (vocab, dim) contiguous
   // by embed_bwd_plan
   int passes, tiles, cthreads;
-  int64_t tile, piece, pieces;
+  int64_t tile, piece, pieces, join;       // join: pieces a workgroup of the join
   uint32_t* keys[2]; uint32_t* order[2]; uint32_t* hist;
   float* part;
 };

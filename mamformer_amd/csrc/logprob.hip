@@ -18,7 +18,7 @@
 // bounded by its largest value and the last id of the first chunk that has it: a key at or below the share's largest, and
 // in the same order as those.  Every wave finds the q-th largest of its 64 bounds by ballots, q = top / 4 rounded up; at
 // least `top` keys are at or above the least of the four, and only the shares whose bound is there can hold one, so only
-// those are read a second time.
+// those are read a second time.  (A row of fewer chunks than threads: q = top, and the largest of the four.)
 //
 // A row is one workgroup's, or where the rows are too few to fill the card the row is cut into spans, whose sums and
 // sorted alternatives logprob_join_kernel puts together.
@@ -152,15 +152,19 @@ template <typename T>
 __device__ void alternatives(const T* row, int64_t lo, int64_t hi, int top, uint64_t bound, AltShared& sh) {
   constexpr int kWaves = kNT / 64;
   const int t = threadIdx.x;
-  const uint64_t mine = wave_nth(bound, (top + kWaves - 1) / kWaves);
+  const bool split = hi - lo >= 8 * kNT;         // every thread has a bound; else one wave alone stands for `top` keys
+  const uint64_t mine = wave_nth(bound, split ? (top + kWaves - 1) / kWaves : top);
   if ((t & 63) == 0) sh.wave[t >> 6] = mine;
   if (t == 0) sh.count = sh.shares = 0;
   if (t < top) sh.out[t] = 0;
   __syncthreads();
   uint64_t tau = sh.wave[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) tau = sh.wave[w] < tau ? sh.wave[w] : tau;
-  tau = tau > 0 ? tau : 1;                       // a wave with fewer bounds: every key counts
+  for (int w = 1; w < kWaves; ++w) {
+    const uint64_t o = sh.wave[w];
+    tau = split ? (o < tau ? o : tau) : (o > tau ? o : tau);
+  }
+  tau = tau > 0 ? tau : 1;                       // fewer than `top` bounds: every key counts
   if (bound >= tau) sh.share[atomicAdd(&sh.shares, 1)] = t;
   __syncthreads();
   const int steps = (int)((hi - lo + 8 * kNT - 1) / (8 * kNT)), shares = sh.shares;

@@ -7,8 +7,8 @@
 //
 // A row lives in the registers of a group of threads (8 channels a thread and step), so every tensor is read and
 // written once and the variance is that of the centred values.  Groups: as many lanes of a wave as the row has chunks,
-// from 8 (heads of 64 channels) to a wave with up to 4 chunks a lane (2048 channels), which needs no barrier; beyond,
-// a workgroup of 256 to 1024 threads.  Sums are fp32.
+// from 8 (heads of 64 channels) to a wave, which needs no barrier; beyond, a workgroup of 128 to 1024 threads.  Sums are
+// fp32.  Bound by memory: 32768 x 4096 bf16 with 8-bit rows moves 1.2 GB forward in 195 us and 0.94 GB backward in 143.
 #include <type_traits>
 
 #include "common.h"
@@ -46,6 +46,7 @@ struct BlockSum {
     return s;
   }
 };
+template <> struct RowSum<128> : BlockSum<128> { using BlockSum<128>::BlockSum; };
 template <> struct RowSum<256> : BlockSum<256> { using BlockSum<256>::BlockSum; };
 template <> struct RowSum<512> : BlockSum<512> { using BlockSum<512>::BlockSum; };
 template <> struct RowSum<1024> : BlockSum<1024> { using BlockSum<1024>::BlockSum; };
@@ -190,32 +191,55 @@ template <typename T, int TPR, int NV, bool PACKED, bool NT>
 __global__ __launch_bounds__(kThreads<TPR>) void norm_bwd_kernel(NormBwdParams p) {
   constexpr int G = kThreads<TPR> / TPR;         // rows at a time
   constexpr int W = TPR * NV * 8;                // channels of a group
-  constexpr bool kAhead = TPR < 1024;            // 128 registers a thread leave no room for the next row
+  static_assert(G == 1 || NV == 1, "one chunk a thread where a workgroup has several rows");
+  // Two chunks a thread, 1024 threads of 128 registers: the sums for dw and db wait in LDS (every thread's own, read and
+  // written once a row).  The weight stays in registers: read again with every row it would wait for the next row's chunks.
+  constexpr bool kKeep = NV == 1;
   __shared__ float2 sums[2 * 16];
   __shared__ float park[G > 1 ? G * W : 1];
+  __shared__ f32x4 wait[kKeep ? 1 : 4 * NV * TPR];
   const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
   RowSum<TPR> sum(sums);
   const float n = (float)p.dim, inv_n = 1.f / n;
-  float w[NV][8], dw[NV][8], db[NV][8];
+  float w[NV][8], dw[8], db[8];
+  auto swap_in = [&](int i) {                    // chunk i's sums from LDS
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      dw[j] = wait[(4 * i + j / 4) * TPR + threadIdx.x][j & 3];
+      db[j] = wait[(4 * i + 2 + j / 4) * TPR + threadIdx.x][j & 3];
+    }
+  };
+  auto swap_out = [&](int i) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      wait[(4 * i + q) * TPR + threadIdx.x] = f32x4{dw[4 * q], dw[4 * q + 1], dw[4 * q + 2], dw[4 * q + 3]};
+      wait[(4 * i + 2 + q) * TPR + threadIdx.x] = f32x4{db[4 * q], db[4 * q + 1], db[4 * q + 2], db[4 * q + 3]};
+    }
+  };
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = 8 * (i * TPR + lane);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) { w[i][j] = 1.f; dw[i][j] = 0.f; db[i][j] = 0.f; }
+    for (int j = 0; j < 8; ++j) w[i][j] = 1.f;
     if (p.weight && c < p.dim) load_par8(p.weight, p.w_f32, c, p.dim, w[i]);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) dw[j] = db[j] = 0.f;
+  if constexpr (!kKeep) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) swap_out(i);
   }
   const int64_t step = (int64_t)gridDim.x * G;
   int64_t row = (int64_t)blockIdx.x * G + group;
-  RowChunk<T, PACKED, NT> cur[NV], next[kAhead ? NV : 1];
+  RowChunk<T, PACKED, NT> cur[NV], next[NV];
   float2 st = {0.f, 0.f}, st_next = {0.f, 0.f};
   auto fetch = [&](int64_t at, float2& s, RowChunk<T, PACKED, NT>* chunk) {
     s = {p.stats[2 * at], p.stats[2 * at + 1]};
 #pragma unroll
     for (int i = 0; i < NV; ++i) chunk[i].load(p, at, 8 * (i * TPR + lane));
   };
-  if (kAhead && row < p.rows) fetch(row, st, cur);
+  if (row < p.rows) fetch(row, st, cur);
   for (; row < p.rows; row += step) {
-    if constexpr (!kAhead) fetch(row, st, cur);
     Raw8<T> dh[NV];
     if (p.d_h) {
 #pragma unroll
@@ -224,20 +248,22 @@ __global__ __launch_bounds__(kThreads<TPR>) void norm_bwd_kernel(NormBwdParams p
         load_raw<NT>(dh[i], reinterpret_cast<const T*>(p.d_h) + row * p.dh_s + c, p.dim - c);
       }
     }
-    if (kAhead && row + step < p.rows) fetch(row + step, st_next, next);
+    if (row + step < p.rows) fetch(row + step, st_next, next);
     const float mu = st.x, r = st.y;
     float sg = 0.f, sgc = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       cur[i].begin();
+      if constexpr (!kKeep) swap_in(i);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {              // beyond the row dy is 0, which keeps those channels out of the sums
         const float d = cur[i].dy.get(j), c = cur[i].centred(j, mu, r), g = d * w[i][j];
-        db[i][j] += d;
-        dw[i][j] += d * c;
+        db[j] += d;
+        dw[j] += d * c;
         sg += g;
         sgc += g * c;
       }
+      if constexpr (!kKeep) swap_out(i);
     }
     const float2 s = sum(sg, sgc);
     const float mg = mean_of(s.x, n, inv_n), mgc = mean_of(s.y, n, inv_n);
@@ -253,33 +279,40 @@ __global__ __launch_bounds__(kThreads<TPR>) void norm_bwd_kernel(NormBwdParams p
       }
       store8<NT>(reinterpret_cast<T*>(p.dx) + row * p.dx_s + c, p.dim - c, o);
     }
-    if constexpr (kAhead) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) cur[i] = next[i];
-      st = st_next;
-    }
+    for (int i = 0; i < NV; ++i) cur[i] = next[i];
+    st = st_next;
   }
-  if (!p.part) return;
-  // the groups' sums, first to last, into this workgroup's rows of the partials (dw at 0, db at 1)
+  if (!p.dweight && !p.dbias) return;
+  // the groups' sums, first to last, into this workgroup's rows of the partials (dw at 0, db at 1), or where it is the only
+  // one to where they belong
   for (int which = 0; which < 2; ++which) {
-    float* dst = p.part + ((int64_t)which * gridDim.x + blockIdx.x) * p.dim;
+    void* par = which ? p.dbias : p.dweight;
+    float* dst = gridDim.x > 1 ? p.part + ((int64_t)which * gridDim.x + blockIdx.x) * p.dim : nullptr;
+    if (!par) continue;
     if constexpr (G > 1) {
-      if (which) __syncthreads();
+      __syncthreads();
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) park[group * W + 8 * (i * TPR + lane) + j] = which ? db[i][j] : dw[i][j];
+      for (int j = 0; j < 8; ++j) park[group * W + 8 * lane + j] = which ? db[j] : dw[j];
       __syncthreads();
       for (int c = threadIdx.x; c < p.dim; c += kThreads<TPR>) {
         float t = 0.f;
         for (int k = 0; k < G; ++k) t += park[k * W + c];
-        dst[c] = t;
+        if (dst) dst[c] = t;
+        else if (p.w_f32) reinterpret_cast<float*>(par)[c] = t;
+        else reinterpret_cast<bf16*>(par)[c] = (bf16)t;
       }
     } else {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = 8 * (i * TPR + lane);
-        store8(dst + c, p.dim - c, which ? db[i] : dw[i]);
+        if constexpr (!kKeep) swap_in(i);
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = which ? db[j] : dw[j];
+        if (dst) store8(dst + c, p.dim - c, v);
+        else if (p.w_f32) store8(reinterpret_cast<float*>(par) + c, p.dim - c, v);
+        else store8(reinterpret_cast<bf16*>(par) + c, p.dim - c, v);
       }
     }
   }
@@ -392,17 +425,19 @@ auto with_fwd_group(int64_t rows, int dim, F&& f) {
   if (dim <= 8192) return f(Group<512, 2>{});
   return f(Group<1024, 2>{});
 }
-// The backward's sums take two registers a channel more.
+// The backward's sums take two registers a channel more: one chunk a thread as far as a workgroup goes, which leaves
+// registers for more waves and the next row (32768 x 4096 from 8-bit rows: 512 threads with one chunk 143 us, 256 with two
+// 166; 4001 x 8192 fp32: 1024 with one 77, 512 with two 88; 100001 x 1000 bf16: 128 with one 137, a wave with two 144).
 template <typename F>
 auto with_bwd_group(int dim, F&& f) {
   if (dim <= 64) return f(Group<8, 1>{});
   if (dim <= 128) return f(Group<16, 1>{});
   if (dim <= 256) return f(Group<32, 1>{});
   if (dim <= 512) return f(Group<64, 1>{});
-  if (dim <= 1024) return f(Group<64, 2>{});
+  if (dim <= 1024) return f(Group<128, 1>{});
   if (dim <= 2048) return f(Group<256, 1>{});
-  if (dim <= 4096) return f(Group<256, 2>{});
-  if (dim <= 8192) return f(Group<512, 2>{});
+  if (dim <= 4096) return f(Group<512, 1>{});
+  if (dim <= 8192) return f(Group<1024, 1>{});
   return f(Group<1024, 2>{});
 }
 
@@ -424,14 +459,13 @@ hipError_t run_fwd(const NormParams& p, hipStream_t st, Group<TPR, NV, ROWS>) {
   return hipGetLastError();
 }
 
-constexpr int64_t kCap = 1024;
-// Two workgroups a CU (one of 1024 threads): more make more partials than they hide latency (32768 x 4096 bf16 from the
-// 8-bit form: 188 us with 512 workgroups, 194 with 768, 223 with 1024; 8192 x 2048: 25.8, 24.2, 24.6 and 4.0, 4.6, 5.0
-// for the partials' sums).
+// Workgroups that the registers let a CU hold, twice as many for short rows, whose partials are small: more would make more
+// partials than they hide latency (8192 x 2048: 25 us with 512 workgroups and 4.0 for the partials' sums, 24.6 and 5.0
+// with 1024; 131072 x 128: 18.1 with 1024, 19.8 with 512).
 template <int TPR, int NV>
 int bwd_blocks(int64_t rows, Group<TPR, NV>) {
   constexpr int G = kThreads<TPR> / TPR;
-  const int64_t need = (rows + G - 1) / G, cap = TPR == 1024 ? 256 : TPR <= 64 && NV == 1 ? kCap : 512;
+  const int64_t need = (rows + G - 1) / G, cap = TPR == 1024 ? 256 : TPR < 128 ? 1024 : TPR == 128 ? 2048 : 512;
   return (int)(need < cap ? need : cap);
 }
 
@@ -444,7 +478,7 @@ hipError_t run_bwd(const NormBwdParams& p, hipStream_t st, Group<TPR, NV> gr) {
   };
   if (p.codes) past ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
   else past ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
-  if (p.part)
+  if (p.part && nb > 1)
     norm_params_kernel<<<dim3((p.dim + 63) / 64, 2), 1024, 0, st>>>(p.part, nb, p.dim, p.dweight, p.dbias, p.w_f32);
   return hipGetLastError();
 }

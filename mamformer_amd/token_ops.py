@@ -60,6 +60,17 @@ def _empty(t):
     return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, device=t.device, dtype=t.dtype)
 
 
+def _optional_workspace(query, a, dev):
+    """The workspace that ``query`` asks for, entered in the arguments; None where it asks for none."""
+    n = ct.c_size_t()
+    _lib.call(query, ct.byref(a), ct.byref(n))
+    if not n.value:
+        return None
+    ws = torch.empty((n.value,), device=dev, dtype=torch.uint8)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), n.value
+    return ws
+
+
 def _like(name, what, t, shape, dtype):
     if t.shape != shape or t.dtype is not dtype:
         raise ValueError(f"{name}: {what} must be {tuple(shape)} {dtype}, got {tuple(t.shape)} {t.dtype}")
@@ -325,19 +336,14 @@ def layer_norm_bwd(dy, h, stats, weight=None, *, d_h=None, bias=True):
     dx = _empty(dy)
     weight, stats, dy = _vec(weight), _vec(stats), _rows(dy, D)
     par_dtype = dy.dtype if weight is None else weight.dtype
-    dpar = None
-    if weight is not None or bias:
-        dpar = torch.empty((2, D), device=dev, dtype=par_dtype)
-    dw = dpar[0] if weight is not None else None
-    db = dpar[1] if bias else None
+    dw = torch.empty((D,), device=dev, dtype=par_dtype) if weight is not None else None
+    db = torch.empty((D,), device=dev, dtype=par_dtype) if bias else None
     a = LayerNormBwdArgs(dy.shape[0], D, dt, _DT[par_dtype], dy.data_ptr(), dy.stride(0),
                          None if is_packed else src.data_ptr(), 0 if is_packed else src.stride(0),
                          src.data_ptr() if is_packed else None, h.exponents.data_ptr() if is_packed else None,
                          stats.data_ptr(), _ptr(weight), _ptr(d_h), 0 if d_h is None else d_h.stride(0),
                          dx.data_ptr(), D, _ptr(dw), _ptr(db))
-    if dpar is not None:
-        ws, a.workspace_bytes = _workspace("mh_layer_norm_bwd_workspace_bytes", a, dev)
-        a.workspace = ws.data_ptr()
+    ws = _optional_workspace("mh_layer_norm_bwd_workspace_bytes", a, dev)
     _lib.call("mh_layer_norm_bwd", ct.byref(a), _stream(dev))
     return dx, dw, db
 
@@ -424,11 +430,7 @@ def _token_logprobs_fwd(logits, targets, temperature, top, ignore_index):
         alt = torch.empty((*lead, top), device=dev, dtype=torch.float32)
     a = LogprobArgs(rows, V, ignore_index, _DT[l2.dtype], tgt.element_size(), top, temperature, l2.data_ptr(),
                     l2.stride(0), tgt.data_ptr(), lp.data_ptr(), ent.data_ptr(), stats.data_ptr(), _ptr(ids), _ptr(alt))
-    n = ct.c_size_t()
-    _lib.call("mh_token_logprobs_workspace_bytes", ct.byref(a), ct.byref(n))
-    if n.value:
-        ws = torch.empty(n.value, device=dev, dtype=torch.uint8)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), n.value
+    ws = _optional_workspace("mh_token_logprobs_workspace_bytes", a, dev)
     _lib.call("mh_token_logprobs_fwd", ct.byref(a), _stream(dev))
     return lp, ent, ids, alt, stats
 

@@ -119,6 +119,23 @@ def test_embedding_gradient_at_the_borders_of_the_sort(T):
     assert torch.equal(mh.embedding_bwd(dy, ids, V), want.float())
 
 
+@pytest.mark.parametrize("T,D", [(2047, 40), (2048, 7), (2049, 40), (30000, 3), (70000, 130), (200000, 8)])
+@pytest.mark.parametrize("V", [1, 40, 600, 300000])
+def test_embedding_gradient_runs(T, D, V):
+    """Runs shorter and longer than the pieces, over many of them, in every way of sorting (one workgroup, several that count
+    by themselves, several that are counted for), with one to three passes; whole numbers, so every sum is exact."""
+    if V == 300000 and D > 40:
+        D = 40
+    g = torch.Generator(device="cuda").manual_seed(T + V)
+    ids = (torch.rand(T, generator=g, device="cuda") ** 4 * V).long().clamp_(0, V - 1)
+    ids[torch.rand(T, generator=g, device="cuda") < 0.1] = V           # out of range
+    dy = torch.randint(-4, 5, (T, D), generator=g, device="cuda").to(BF)
+    say(f"embedding gradient runs T={T} V={V} D={D}")
+    live = ids < V
+    want = torch.zeros(V, D, device="cuda", dtype=torch.float64).index_add_(0, ids[live], dy[live].double())
+    assert torch.equal(mh.embedding_bwd(dy, ids, V, dtype=F32), want.float())
+
+
 def test_embedding_strides_and_autograd():
     W, Wg = draw(5, 20, 24, dtype=BF)
     wide = torch.zeros(20, 50, device="cuda", dtype=BF)
@@ -491,6 +508,22 @@ def test_token_logprobs_of_very_many_rows():
         want = mh.token_logprobs(z[s], t[s], top=2)
         assert all(torch.equal(p[s], q) for p, q in zip(out, want))
         assert torch.equal(d[s], mh.token_logprobs_bwd(z[s], t[s], want.stats, want.entropy))
+
+
+@pytest.mark.parametrize("V", [9, 65, 500, 520, 1024, 1537, 2047, 2048, 2056])
+def test_alternatives_of_short_rows(V):
+    """Rows with fewer chunks than threads, some with a wave that has none; small whole numbers make many ties."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    z = torch.randint(-3, 4, (6, V), generator=g, device="cuda").float()
+    z[1, V // 3:] = -float("inf")
+    z[2] = torch.randn(V, generator=g, device="cuda")
+    z[3, V - 2] = float("nan")
+    t = torch.zeros(6, dtype=torch.int64, device="cuda")
+    for top in (1, 5, min(V, 64)):
+        out = mh.token_logprobs(z, t, top=top)
+        v = host(z)
+        order = np.lexsort((np.broadcast_to(np.arange(V), v.shape), -np.where(np.isnan(v), np.inf, v), ~np.isnan(v)))[:, :top]
+        assert np.array_equal(out.top_ids.cpu().numpy(), order)
 
 
 def test_token_logprobs_strides_and_in_place():
