@@ -3,7 +3,9 @@
 //   out[t] = scale W[ids[t]]  (zeros for an id outside [0, vocab));
 //   dW[v] = scale sum of dy[t] over the tokens t with ids[t] = v != padding_idx, in the order of t.
 //
-// The gradient sorts (id, t) by id with a stable radix sort of 9 bits a pass (two passes up to 2^18 rows), so that the
+// The gradient of up to 2048 tokens is one launch that compares every token's id with all others (embed_few_kernel: 1927
+// tokens, 10777 x 1000 fp32: 17 us, sorted 24).  Otherwise it sorts (id, t) by id with a stable radix sort of 9 bits a
+// pass (two passes up to 2^18 rows), so that the
 // sum of a row runs in the order of its tokens and gives the same bits at every call; no floating-point atomics.  Most of
 // what has to be moved is the table's zeros: the sort's launches carry them in workgroups of their own, a share a pass, so
 // that a pass (a chain of dependent steps on few CUs) costs no time of its own where the table is large.  The
@@ -21,7 +23,8 @@ namespace {
 
 constexpr int kBits = 9, kDigits = 1 << kBits;   // a pass: 512 counters, two a thread
 constexpr int kSortThreads = 1024;               // 64 tokens a wave of the smallest tile
-constexpr int64_t kSmall = 2048;                 // up to here one workgroup sorts, two tokens a thread
+constexpr int kFew = 2048;                       // up to here, in a table of up to kFewRows, nothing is sorted
+constexpr int kFewRows = 1 << 18;
 constexpr int64_t kDirect = 16384;               // up to here a pass counts all tokens by itself
 
 // cthreads threads (a power of two) take 8 columns each of kRows tokens, whose loads are all on their way at once.
@@ -78,7 +81,8 @@ __global__ __launch_bounds__(256) void embed_count_kernel(EmbedBwdParams p) {
   h[threadIdx.x + 256] = cnt[threadIdx.x + 256];
 }
 
-// Zeros for share `pass` of the table's `passes` equal shares, by workgroup b of n.
+// Zeros for share `pass` of the table's `passes` equal shares, by workgroup b of n, past the caches (131 MB of a table with its
+// sort: 45 us, through them 55).
 __device__ void clear_share(const EmbedBwdParams& p, int pass, int64_t b, int64_t n) {
   typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
   const int64_t bytes = p.vocab * p.dim * (p.dw_f32 ? 4 : 2), share = (bytes / p.passes + 15) / 16 * 16;
@@ -86,7 +90,7 @@ __device__ void clear_share(const EmbedBwdParams& p, int pass, int64_t b, int64_
   char* base = reinterpret_cast<char*>(p.dweight);
   const u32x4_any z = {0u, 0u, 0u, 0u};
   int64_t at = lo + 16 * (b * kSortThreads + threadIdx.x);
-  for (; at + 16 <= hi; at += 16 * kSortThreads * n) *reinterpret_cast<u32x4_any*>(base + at) = z;
+  for (; at + 16 <= hi; at += 16 * kSortThreads * n) __builtin_nontemporal_store(z, reinterpret_cast<u32x4_any*>(base + at));
   for (; at < hi; at += 2) *reinterpret_cast<uint16_t*>(base + at) = 0;         // the last thread's tail, if any
 }
 __global__ __launch_bounds__(kSortThreads) void embed_clear_kernel(EmbedBwdParams p) {
@@ -224,82 +228,162 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedBwdParams
   }
 }
 
-// Up to kSmall tokens: all passes in one workgroup, the tokens in registers and LDS, as embed_sort_kernel's otherwise.  The
-// other workgroups clear the table.
-__global__ __launch_bounds__(kSortThreads) void embed_sort_small_kernel(EmbedBwdParams p) {
-  constexpr int kWaves = kSortThreads / 64, kSteps = (int)(kSmall / kSortThreads);
-  __shared__ uint32_t at[kWaves][kDigits];
-  __shared__ uint32_t keys[kSmall], toks[kSmall];
-  __shared__ uint32_t wsum[kDigits / 64];
-  if (blockIdx.x > 0) {
-    for (int q = 0; q < p.passes; ++q) clear_share(p, q, blockIdx.x - 1, gridDim.x - 1);
+// Zeros for the rows whose bit is not set, by workgroup b of n: 16 bytes a thread along the table whatever its rows' length,
+// so that stores stay whole and in line; the pieces at the ends of rows that have a token go by elements.
+template <typename TW>
+__device__ void clear_absent(const EmbedBwdParams& p, const uint32_t* bits, int64_t b, int64_t n) {
+  typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+  const u32x4_any z = {0u, 0u, 0u, 0u};
+  const int64_t row_bytes = p.dim * (int64_t)sizeof(TW), bytes = p.vocab * row_bytes, step = 16 * kSortThreads * n;
+  const int64_t rows = step / row_bytes, rest = step % row_bytes;
+  char* base = reinterpret_cast<char*>(p.dweight);
+  int64_t at = 16 * (b * kSortThreads + threadIdx.x), row = at / row_bytes, in = at % row_bytes;   // byte `in` of `row`
+  auto has = [&](int64_t v) { return bits[v / 32] >> (v % 32) & 1; };
+  for (; at < bytes; at += step) {
+    const bool whole = at + 16 <= bytes, one = in + 16 <= row_bytes;
+    if (whole && (one || (row_bytes >= 16 && has(row) == has(row + 1)))) {
+      if (!has(row)) __builtin_nontemporal_store(z, reinterpret_cast<u32x4_any*>(base + at));
+    } else {
+      int64_t v = row, e = in;
+      for (int64_t q = at; q < min(bytes, at + 16); q += sizeof(TW), e += sizeof(TW)) {
+        if (e >= row_bytes) { e -= row_bytes; ++v; }
+        if (!has(v)) *reinterpret_cast<TW*>(base + q) = from_f32<TW>(0.f);
+      }
+    }
+    row += rows;
+    in += rest;
+    if (in >= row_bytes) { in -= row_bytes; ++row; }
+  }
+}
+
+// Few tokens: one launch without a sort.  The first workgroups take 16 tokens each, a wave a token and up to 512 columns of
+// it: the wave compares the token's row with all tokens' (in LDS), and the one occurrence that is to answer for the row
+// sums its tokens in their order.  Which occurrence that is goes by the row, so that a few frequent rows, all of which
+// show up among the first tokens, are not one workgroup's.  A row with more than kList tokens is summed by the whole
+// workgroup, an equal share of its tokens a wave, the shares joined in order.  The other workgroups write the zeros of the
+// rows that have no token, which a bit for each row in LDS tells.
+template <typename T, typename TW>
+__global__ __launch_bounds__(kSortThreads) void embed_few_kernel(EmbedBwdParams p, int sums) {
+  constexpr int kWaves = kSortThreads / 64, kList = 32, kAhead = 8;
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  struct Sum {
+    u32x4 keys[kFew / 4];
+    uint16_t list[kWaves][kList], run[kFew];
+    uint32_t longs[kWaves];
+    float park[kWaves][8][64];
+    int n_longs, found;
+  };
+  __shared__ union {
+    Sum s;
+    uint32_t bits[kFewRows / 32];
+  } sh;
+  const int n = (int)p.tokens, lane = lane_id(), wave = wave_id();
+  if ((int)blockIdx.x >= sums) {
+    const int words = (int)((p.vocab + 31) / 32);
+    for (int i = threadIdx.x; i < words; i += kSortThreads) sh.bits[i] = 0;
+    __syncthreads();
+    for (int t = threadIdx.x; t < n; t += kSortThreads) {
+      const uint32_t k = token_key(p, t);
+      if (k < (uint32_t)p.vocab) atomicOr(&sh.bits[k / 32], 1u << (k % 32));
+    }
+    __syncthreads();
+    clear_absent<TW>(p, sh.bits, blockIdx.x - sums, gridDim.x - sums);
     return;
   }
-  const int lane = lane_id(), wave = wave_id(), n = (int)p.tokens, lo = wave * 64 * kSteps + lane;
-  uint32_t key[kSteps], tok[kSteps];
+  const int slabs = (p.dim + 511) / 512, slab = blockIdx.x % slabs, t = blockIdx.x / slabs * kWaves + wave;
+  const int c = 512 * slab + 8 * lane, left = p.dim - c;
+  const T* dy = reinterpret_cast<const T*>(p.dy) + c;
+  const int n256 = (n + 255) / 256 * 256;
+  uint32_t* keys = reinterpret_cast<uint32_t*>(sh.s.keys);
+  for (int i = threadIdx.x; i < n256; i += kSortThreads) keys[i] = i < n ? token_key(p, i) : 0xffffffffu;
+  if (threadIdx.x == 0) sh.s.n_longs = 0;
+  __syncthreads();
+  // the tokens of row `key` in order into list (as many as it holds); their number, and how many come before token t.  Four
+  // tokens a lane at a time, most of which are other rows'.
+  auto find = [&](uint32_t key, uint16_t* list, int room, int& before) {
+    int found = 0;
+    before = 0;
+#pragma unroll 2
+    for (int q = 0; q < n256; q += 256) {
+      const u32x4 k = sh.s.keys[q / 4 + lane];
+      const bool hit[4] = {k[0] == key, k[1] == key, k[2] == key, k[3] == key};
+      if (!__ballot(hit[0] | hit[1] | hit[2] | hit[3])) continue;
+      const uint64_t lower = ((uint64_t)1 << lane) - 1;
+      int at = found;
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    tok[i] = lo + 64 * i;
-    key[i] = lo + 64 * i < n ? token_key(p, lo + 64 * i) : 0;
+      for (int j = 0; j < 4; ++j) at += __popcll(__ballot(hit[j]) & lower);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int token = q + 4 * lane + j;
+        before += __popcll(__ballot(hit[j] && token < t));
+        found += __popcll(__ballot(hit[j]));
+        if (hit[j]) {
+          if (at < room) list[at] = (uint16_t)token;
+          ++at;
+        }
+      }
+    }
+    return found;
+  };
+  // dy of tokens list[from .. to) added up in order
+  auto sum = [&](const uint16_t* list, int from, int to, float (&acc)[8]) {
+    for (int i0 = from; i0 < to; i0 += kAhead) {
+      Raw8<T> v[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (i0 + i < to && left > 0) load_raw(v[i], dy + (int64_t)list[i0 + i] * p.dy_s, left);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (i0 + i < to && left > 0) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[j] += v[i].get(j);
+        }
+    }
+  };
+  auto put = [&](uint32_t key, float (&acc)[8]) {
+    if (left <= 0) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] *= p.scale;
+    store8(reinterpret_cast<TW*>(p.dweight) + (int64_t)key * p.dim + c, left, acc);
+  };
+  const uint32_t key = t < n ? keys[t] : (uint32_t)p.vocab;
+  if (key < (uint32_t)p.vocab) {
+    int before;
+    const int found = find(key, sh.s.list[wave], kList, before);
+    if ((uint32_t)before == key % (uint32_t)found) {
+      if (found <= kList) {
+        __builtin_amdgcn_wave_barrier();
+        float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        sum(sh.s.list[wave], 0, found, acc);
+        put(key, acc);
+      } else if (lane == 0) {
+        sh.s.longs[atomicAdd(&sh.s.n_longs, 1)] = key;
+      }
+    }
   }
-  for (int pass = 0; pass < p.passes; ++pass) {
-    const int shift = pass * kBits;
-    for (int i = threadIdx.x; i < kWaves * kDigits; i += kSortThreads) at[0][i] = 0;
-    if (pass) {
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        key[i] = keys[lo + 64 * i];
-        tok[i] = toks[lo + 64 * i];
-      }
+  __syncthreads();
+  const int longs = sh.s.n_longs;
+  for (int r = 0; r < longs; ++r) {
+    const uint32_t k = sh.s.longs[r];
+    int before;
+    if (wave == 0) {
+      const int found = find(k, sh.s.run, kFew, before);
+      if (lane == 0) sh.s.found = found;
     }
     __syncthreads();
+    const int found = sh.s.found, per = (found + kWaves - 1) / kWaves, from = wave * per;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    sum(sh.s.run, from, min(found, from + per), acc);
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i)
-      if (lo + 64 * i < n) atomicAdd(&at[wave][(key[i] >> shift) & (kDigits - 1)], 1u);
+    for (int j = 0; j < 8; ++j) sh.s.park[wave][j][lane] = acc[j];
     __syncthreads();
-    uint32_t total = 0;
-    if (threadIdx.x < kDigits)
-      for (int w = 0; w < kWaves; ++w) total += at[w][threadIdx.x];
-    uint32_t incl = total;
+    if (wave == 0) {
+      for (int w = 1; w < kWaves; ++w)
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const uint32_t o = (uint32_t)__shfl_up((int)incl, off, 64);
-      if (lane >= off) incl += o;
-    }
-    if (lane == 63 && wave < kDigits / 64) wsum[wave] = incl;
-    __syncthreads();
-    if (threadIdx.x < kDigits) {
-      uint32_t start = incl - total;
-      for (int w = 0; w < wave; ++w) start += wsum[w];
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const uint32_t c = at[w][threadIdx.x];
-        at[w][threadIdx.x] = start;
-        start += c;
-      }
+        for (int j = 0; j < 8; ++j) acc[j] += sh.s.park[w][j][lane];
+      put(k, acc);
     }
     __syncthreads();
-    volatile uint32_t* mine = at[wave];
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      const bool live = lo + 64 * i < n;
-      const uint32_t d = (key[i] >> shift) & (kDigits - 1);
-      uint64_t same;
-      const int rank = digit_rank(d, live, lane, same);
-      if (live) {
-        const uint32_t place = mine[d], pos = place + rank;
-        __builtin_amdgcn_wave_barrier();         // every lane has read its digit's place before the first lane moves it
-        if (rank == 0) mine[d] = place + (uint32_t)__popcll(same);
-        keys[pos] = key[i];
-        toks[pos] = tok[i];
-      }
-      __builtin_amdgcn_wave_barrier();
-    }
-    __syncthreads();
-  }
-  for (int i = threadIdx.x; i < n; i += kSortThreads) {
-    p.keys[p.passes & 1][i] = keys[i];
-    p.order[p.passes & 1][i] = toks[i];
   }
 }
 
@@ -406,10 +490,11 @@ __global__ __launch_bounds__(256) void embed_join_kernel(EmbedBwdParams p) {
   }
 }
 
-// 64 KB a workgroup, two workgroups a CU at most.
+// 64 KB a workgroup, 2048 at most: the ones that clear follow the ones that sum as those end (1999 tokens, 49999 x 1001 fp32:
+// 43 us, with 512 at most 52; with 32 KB each and 4096 at most 51, each having the rows' bits to set first).
 unsigned clear_blocks(int64_t bytes) {
   const int64_t b = (bytes + 65535) / 65536;
-  return (unsigned)(b < 512 ? b : 512);
+  return (unsigned)(b < 2048 ? b : 2048);
 }
 
 template <typename T, typename TW>
@@ -420,10 +505,14 @@ hipError_t run_bwd(const EmbedBwdParams& p, hipStream_t st) {
     return hipGetLastError();
   }
   const unsigned grid = p.tiles + clear_blocks(bytes / p.passes + 16);
-  const bool direct = p.tokens <= kDirect, small = p.tokens <= kSmall;
-  if (small) embed_sort_small_kernel<<<1 + clear_blocks(bytes), kSortThreads, 0, st>>>(p);
+  if (p.tokens <= kFew && p.vocab <= kFewRows && p.dim <= (1 << 16)) {
+    const int sums = (int)((p.tokens + 15) / 16) * ((p.dim + 511) / 512);
+    embed_few_kernel<T, TW><<<sums + clear_blocks(bytes), kSortThreads, 0, st>>>(p, sums);
+    return hipGetLastError();
+  }
+  const bool direct = p.tokens <= kDirect;
   if (!direct) embed_count_kernel<<<p.tiles, 256, 0, st>>>(p);
-  for (int pass = 0; pass < p.passes && !small; ++pass) {
+  for (int pass = 0; pass < p.passes; ++pass) {
     if (direct) embed_sort_kernel<true><<<grid, kSortThreads, 0, st>>>(p, pass);
     else embed_sort_kernel<false><<<grid, kSortThreads, 0, st>>>(p, pass);
   }

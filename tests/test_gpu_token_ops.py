@@ -136,6 +136,45 @@ def test_embedding_gradient_runs(T, D, V):
     assert torch.equal(mh.embedding_bwd(dy, ids, V, dtype=F32), want.float())
 
 
+@pytest.mark.parametrize("V", [1, 2, 33, 4096, 262144, 262145])
+@pytest.mark.parametrize("T,D", [(1, 5), (16, 600), (17, 512), (31, 8), (33, 520), (1000, 513), (2048, 64)])
+def test_embedding_gradient_of_few_tokens(T, D, V):
+    """Rows with one token, with as many as a wave takes and with more, all rows alike, several columns' worth of workgroups."""
+    g = torch.Generator(device="cuda").manual_seed(T + V)
+    ids = torch.where(torch.rand(T, generator=g, device="cuda") < 0.5, min(V, 3) - 1,
+                      torch.randint(-1, V + 1, (T,), generator=g, device="cuda"))
+    dy = torch.randint(-4, 5, (T, D), generator=g, device="cuda").float()
+    say(f"embedding gradient of few tokens T={T} V={V} D={D}")
+    for pad in (None, V - 1):
+        live = (ids >= 0) & (ids < V) if pad is None else (ids >= 0) & (ids < V) & (ids != pad)
+        want = torch.zeros(V, D, device="cuda", dtype=torch.float64).index_add_(0, ids[live], dy[live].double())
+        for dtype in (F32, BF):                  # sums up to 4096: bf16 rounds them once
+            assert torch.equal(mh.embedding_bwd(dy, ids, V, padding_idx=pad, dtype=dtype), want.float().to(dtype))
+
+
+def test_offsets_beyond_32_bits():
+    """Rows 2^31 elements apart: every operator reads and writes them where they are."""
+    D, far = 200, (1 << 31) + 64
+    big = torch.empty(2 * far + D, device="cuda", dtype=BF)
+    rows = big.as_strided((3, D), (far, 1))
+    x = torch.randn(3, D, device="cuda").to(BF)
+    rows.copy_(x)
+    ids, w = torch.tensor([2, 0, 1, 2], device="cuda"), torch.randn(D, device="cuda").to(BF)
+    assert torch.equal(mh.embedding(ids, rows), x[ids])
+    assert torch.equal(mh.embedding_bwd(rows, ids[:3], 5), mh.embedding_bwd(x, ids[:3], 5))
+    for p, q in zip(mh.layer_norm(rows, w, residual=rows, return_stats=True), mh.layer_norm(x, w, residual=x, return_stats=True)):
+        assert torch.equal(p, q)
+    _, st = mh.layer_norm(x, w, return_stats=True)
+    for p, q in zip(mh.layer_norm_bwd(rows, rows, st, w, d_h=rows), mh.layer_norm_bwd(x, x, st, w, d_h=x)):
+        assert torch.equal(p, q)
+    assert torch.equal(mh.pack_activations(rows).codes, mh.pack_activations(x).codes)
+    out, want = mh.token_logprobs(rows, ids[:3], top=3), mh.token_logprobs(x, ids[:3], top=3)
+    assert all(torch.equal(p, q) for p, q in zip(out, want))
+    d = mh.token_logprobs_bwd(x, ids[:3], want.stats, want.entropy)
+    mh.token_logprobs_bwd(rows, ids[:3], want.stats, want.entropy, out=rows)
+    assert torch.equal(rows, d)
+
+
 def test_embedding_strides_and_autograd():
     W, Wg = draw(5, 20, 24, dtype=BF)
     wide = torch.zeros(20, 50, device="cuda", dtype=BF)
