@@ -234,20 +234,23 @@ template <typename TW>
 __device__ void clear_absent(const EmbedBwdParams& p, const uint32_t* bits, int64_t b, int64_t n) {
   typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
   const u32x4_any z = {0u, 0u, 0u, 0u};
-  const int64_t row_bytes = p.dim * (int64_t)sizeof(TW), bytes = p.vocab * row_bytes, step = 16 * kSortThreads * n;
-  const int64_t rows = step / row_bytes, rest = step % row_bytes;
-  char* base = reinterpret_cast<char*>(p.dweight);
-  int64_t at = 16 * (b * kSortThreads + threadIdx.x), row = at / row_bytes, in = at % row_bytes;   // byte `in` of `row`
-  auto has = [&](int64_t v) { return bits[v / 32] >> (v % 32) & 1; };
-  for (; at < bytes; at += step) {
-    const bool whole = at + 16 <= bytes, one = in + 16 <= row_bytes;
-    if (whole && (one || (row_bytes >= 16 && has(row) == has(row + 1)))) {
-      if (!has(row)) __builtin_nontemporal_store(z, reinterpret_cast<u32x4_any*>(base + at));
+  // rows and bytes of a row in 32 bits (2^18 each at most): the arithmetic of a piece is what a store has to hide
+  const int row_bytes = p.dim * (int)sizeof(TW);
+  const int64_t bytes = p.vocab * row_bytes, step = 16 * kSortThreads * n, at = 16 * (b * kSortThreads + threadIdx.x);
+  const int rows = (int)(step / row_bytes), rest = (int)(step % row_bytes);
+  int row = (int)(at / row_bytes), in = (int)(at % row_bytes);        // the piece begins at byte `in` of `row`
+  char* q = reinterpret_cast<char*>(p.dweight) + at;
+  const char* end = reinterpret_cast<char*>(p.dweight) + bytes;
+  auto has = [&](int v) { return bits[v >> 5] >> (v & 31) & 1; };
+  for (; q < end; q += step) {
+    const bool whole = q + 16 <= end, mine = has(row);
+    if (whole && (in + 16 <= row_bytes || (row_bytes >= 16 && mine == has(row + 1)))) {
+      if (!mine) __builtin_nontemporal_store(z, reinterpret_cast<u32x4_any*>(q));
     } else {
-      int64_t v = row, e = in;
-      for (int64_t q = at; q < min(bytes, at + 16); q += sizeof(TW), e += sizeof(TW)) {
+      int v = row, e = in;
+      for (int o = 0; o < 16 && q + o < end; o += sizeof(TW), e += sizeof(TW)) {
         if (e >= row_bytes) { e -= row_bytes; ++v; }
-        if (!has(v)) *reinterpret_cast<TW*>(base + q) = from_f32<TW>(0.f);
+        if (!has(v)) *reinterpret_cast<TW*>(q + o) = from_f32<TW>(0.f);
       }
     }
     row += rows;
@@ -497,6 +500,10 @@ unsigned clear_blocks(int64_t bytes) {
   return (unsigned)(b < 2048 ? b : 2048);
 }
 
+bool few_tokens(const EmbedBwdParams& p) {
+  return p.tokens <= kFew && p.vocab <= kFewRows && p.dim <= (1 << 16);
+}
+
 template <typename T, typename TW>
 hipError_t run_bwd(const EmbedBwdParams& p, hipStream_t st) {
   const int64_t bytes = p.vocab * p.dim * (int64_t)sizeof(TW);
@@ -505,7 +512,7 @@ hipError_t run_bwd(const EmbedBwdParams& p, hipStream_t st) {
     return hipGetLastError();
   }
   const unsigned grid = p.tiles + clear_blocks(bytes / p.passes + 16);
-  if (p.tokens <= kFew && p.vocab <= kFewRows && p.dim <= (1 << 16)) {
+  if (few_tokens(p)) {
     const int sums = (int)((p.tokens + 15) / 16) * ((p.dim + 511) / 512);
     embed_few_kernel<T, TW><<<sums + clear_blocks(bytes), kSortThreads, 0, st>>>(p, sums);
     return hipGetLastError();
@@ -561,6 +568,7 @@ size_t embed_bwd_plan(EmbedBwdParams& p, void* workspace) {
     p.keys[i] = reinterpret_cast<uint32_t*>(take((size_t)p.tokens * 4));
     p.order[i] = reinterpret_cast<uint32_t*>(take((size_t)p.tokens * 4));
   }
+  if (few_tokens(p)) return off;                 // which neither counts nor has partial rows
   p.hist = reinterpret_cast<uint32_t*>(take((size_t)p.passes * p.tiles * kDigits * 4));
   p.part = reinterpret_cast<float*>(take((size_t)2 * p.pieces * p.dim * 4));
   return off;

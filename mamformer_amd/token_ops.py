@@ -302,14 +302,14 @@ def _layer_norm_fwd(x, residual, weight, bias, eps, packed, stats):
     return y, h, codes, exps, st
 
 
-def layer_norm_bwd(dy, h, stats, weight=None, *, d_h=None, bias=True):
+def layer_norm_bwd(dy, h, stats, weight=None, *, d_h=None, bias=True, dtype=None):
     """Gradients of ``layer_norm``: (dx, dweight, dbias).
 
     dy (..., D); h: what was normalised (x, or the sum with the residual), a tensor like dy or ``PackedActivations``;
     stats (..., 2) as ``layer_norm`` returns them; ``d_h``: the gradient that reaches the stream h by its other uses,
     added into dx.  dx (like dy) is the gradient of x and of residual alike.  dweight (None without ``weight``) and dbias
-    (None unless ``bias``) have the weight's dtype (without one, that of dy); both are fp32 sums over the rows in a
-    fixed order, rounded once.
+    (None unless ``bias``) have the weight's dtype (without one ``dtype``, None: that of dy); both are fp32 sums over the
+    rows in a fixed order, rounded once.
     """
     name = "layer_norm_bwd"
     is_packed = isinstance(h, PackedActivations)
@@ -335,7 +335,9 @@ def layer_norm_bwd(dy, h, stats, weight=None, *, d_h=None, bias=True):
     _norm_params(name, weight, None, D)
     dx = _empty(dy)
     weight, stats, dy = _vec(weight), _vec(stats), _rows(dy, D)
-    par_dtype = dy.dtype if weight is None else weight.dtype
+    par_dtype = weight.dtype if weight is not None else dy.dtype if dtype is None else dtype
+    if par_dtype not in _DT:
+        raise TypeError(f"{name}: dtype {par_dtype} not supported (float32, bfloat16)")
     dw = torch.empty((D,), device=dev, dtype=par_dtype) if weight is not None else None
     db = torch.empty((D,), device=dev, dtype=par_dtype) if bias else None
     a = LayerNormBwdArgs(dy.shape[0], D, dt, _DT[par_dtype], dy.data_ptr(), dy.stride(0),
@@ -359,7 +361,6 @@ class _LayerNormFn(torch.autograd.Function):
         kept = codes if packed else x if h is None else h
         ctx.save_for_backward(kept, exps, stats, weight)
         ctx.packed = (x.shape[-1], x.dtype) if packed else None
-        ctx.bias = bias is not None
         ctx.par_dtype = None if bias is None else bias.dtype
         return y, h, codes, exps, stats
 
@@ -371,9 +372,7 @@ class _LayerNormFn(torch.autograd.Function):
         if dy is None:                           # only the stream was used
             return d_h if need_x else None, d_h if need_res else None, None, None, None, None
         h = PackedActivations(kept, exps, *ctx.packed) if ctx.packed else kept
-        dx, dw, db = layer_norm_bwd(dy, h, stats, weight, d_h=d_h, bias=need_b)
-        if db is not None:
-            db = db.to(ctx.par_dtype)
+        dx, dw, db = layer_norm_bwd(dy, h, stats, weight, d_h=d_h, bias=need_b, dtype=ctx.par_dtype)
         return dx if need_x else None, dx if need_res else None, dw if need_w else None, db, None, None
 
 

@@ -327,6 +327,22 @@ def test_layer_norm_autograd(packed):
     assert torch.equal(only, db)
 
 
+def test_layer_norm_bias_alone():
+    """A bias of 32 bits without a weight: its gradient is not rounded to the rows' 16."""
+    x, dy = torch.randn(2, 700, 40, device="cuda").to(BF)
+    b = torch.randn(40, device="cuda", requires_grad=True)
+    y = mh.layer_norm(x, None, b)
+    gb, = torch.autograd.grad(y, b, dy)
+    ref, mag = host(dy).sum(0), np.abs(host(dy)).sum(0)
+    assert gb.dtype is F32
+    near("dbias", gb, ref, mag, 700 + 32)
+    _, st = mh.layer_norm(x, return_stats=True)
+    _, dw, db = mh.layer_norm_bwd(dy, x, st, dtype=F32)
+    assert dw is None and torch.equal(db, gb) and mh.layer_norm_bwd(dy, x, st)[2].dtype is BF
+    with pytest.raises(TypeError):
+        mh.layer_norm_bwd(dy, x, st, dtype=torch.half)
+
+
 def test_layer_norm_against_differences():
     """The directional derivative of the kernels' own forward: steps of 2^-6 leave a truncation of about 2^-12 (third
     order) and a rounding of 2^-24 * 2^6 of y's size, both against a derivative of the order of sqrt(R D)."""
