@@ -509,8 +509,8 @@ typedef struct {
 int mh_embedding_fwd(const mh_embedding_args* a, void* stream);
 
 /* Its gradient: dweight[v] = scale * sum of dy[t] over ids[t] == v, v != padding_idx (-1: none), every row written,
- *   (vocab, dim) contiguous in dweight_dtype. Tokens are sorted by id and summed in their order, in fp32: the same bits
- *   at every call. tokens <= 2^30. */
+ *   (vocab, dim) contiguous in dweight_dtype. A row's tokens are summed in their order, many of them by equal shares, in
+ *   fp32: the same bits at every call. tokens <= 2^30. */
 typedef struct {
   int64_t tokens, vocab, dim, padding_idx;
   int32_t dtype, index_bytes, dweight_dtype;

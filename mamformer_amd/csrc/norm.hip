@@ -408,8 +408,10 @@ __global__ __launch_bounds__(256) void unpack_kernel(PackParams p) {
 }
 
 // Calls f with (TPR, NV, ROWS) of the group that holds a row of dim channels.  Rows of up to 512 channels, one chunk a
-// thread, go two to a group where that leaves 8 workgroups a CU; rows of up to 2048 to a workgroup each where there
-// are fewer than 8 a CU of them, and to a wave each beyond.
+// thread, go two to a group where that leaves 8 workgroups a CU (131072 x 128 bf16: 13.0 us, 13.8 by one; 60000 x 512:
+// 24.0 and 26.0).  Rows of up to 2048 go to a workgroup each where there are up to four a CU of them (256 x 2048: 4.8
+// us, a wave each 5.4; 1024 x 2048: 5.1 and 5.6), and to a wave each beyond (2048 x 1000: 4.4 us, a workgroup each 5.2;
+// 4096 x 1000: 5.8 and 8.0).
 template <int TPR, int NV, int ROWS = 1> struct Group {};
 template <typename F>
 auto with_fwd_group(int64_t rows, int dim, F&& f) {
@@ -418,7 +420,7 @@ auto with_fwd_group(int64_t rows, int dim, F&& f) {
   if (dim <= 128) return many ? f(Group<16, 1, 2>{}) : f(Group<16, 1>{});
   if (dim <= 256) return many ? f(Group<32, 1, 2>{}) : f(Group<32, 1>{});
   if (dim <= 512) return many ? f(Group<64, 1, 2>{}) : f(Group<64, 1>{});
-  if (rows <= 2048 && dim <= 2048) return f(Group<256, 1>{});
+  if (rows <= 1024 && dim <= 2048) return f(Group<256, 1>{});
   if (dim <= 1024) return f(Group<64, 2>{});
   if (dim <= 2048) return f(Group<64, 4>{});
   if (dim <= 4096) return f(Group<256, 2>{});
@@ -442,8 +444,8 @@ auto with_bwd_group(int dim, F&& f) {
 }
 
 // Calls whose tensors together are larger than the cache in front of the memory read and write them past it (32768 x 4096
-// bf16 with 8-bit rows, 1.2 GB forward and 0.9 GB backward: 206 -> 195 us and 188 -> 166); smaller ones leave there what the
-// next call will read (8192 x 2048, backward on what the forward left: 25 us against 31).
+// bf16 with 8-bit rows: backward, 0.9 GB, 152 us, through it 179; forward, 1.2 GB, after a backward 195 and 206); smaller
+// ones leave there what the next call will read (8192 x 2048, backward on what the forward left: 25 us, past it 31).
 bool past_cache(int64_t rows, int dim, int tensors, size_t es) {
   return rows * dim * tensors * (int64_t)es > (int64_t)256 << 20;
 }

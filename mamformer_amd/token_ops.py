@@ -1,7 +1,7 @@
 """Operators at the two ends of a language model and between its layers, beside the scans of ``ops``.
 
 =====================================  ====================================================================
-``embedding``, ``embedding_bwd``        scaled token lookup, and the table's gradient by sorted tokens
+``embedding``, ``embedding_bwd``        scaled token lookup, and the table's gradient
 ``layer_norm``, ``layer_norm_bwd``      layer norm of the residual stream (the sum with a layer's output fused),
                                         and its backward with the weight's and bias's gradients
 ``pack_activations``,                   activations in 8 bits with an exponent for each 64 channels, for what a
@@ -121,8 +121,8 @@ def embedding_bwd(dy, ids, num_embeddings, *, scale=1.0, padding_idx=None, dtype
     """Gradient of ``embedding`` with respect to its table, (num_embeddings, D) in ``dtype`` (float32 or bfloat16; None:
     that of dy).
 
-    dy (*ids.shape, D).  The tokens are sorted by id and each row is the fp32 sum over its tokens in their order, times
-    ``scale``, rounded once; rows without tokens are zero.
+    dy (*ids.shape, D).  Each row is the fp32 sum over its tokens in their order (of many tokens: of equal shares of them,
+    joined in order), times ``scale``, rounded once; rows without tokens are zero.
     """
     name = "embedding_bwd"
     _require_cuda(name, dy, ids)
