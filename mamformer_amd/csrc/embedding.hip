@@ -23,6 +23,7 @@ namespace {
 
 constexpr int kBits = 9, kDigits = 1 << kBits;   // a pass: 512 counters, two a thread
 constexpr int kSortThreads = 1024;               // 64 tokens a wave of the smallest tile
+constexpr int kClearThreads = 256;               // of these, the ones that clear beside a sort
 constexpr int kFew = 2048;                       // up to here, in a table of up to kFewRows, nothing is sorted
 constexpr int kFewRows = 1 << 18;
 // up to here a pass counts all tokens by itself (32000 x 1024 bf16: 4096 tokens 28 us, counted for 40; 16000: both 49;
@@ -84,15 +85,17 @@ __global__ __launch_bounds__(256) void embed_count_kernel(EmbedBwdParams p) {
 }
 
 // Zeros for share `pass` of the table's `passes` equal shares, by workgroup b of n, past the caches (131 MB of a table with its
-// sort: 45 us, through them 55).
+// sort: 45 us, through them 48) and by a quarter of the threads: 2 x 256 a CU that move along the table together write
+// faster than 2 x 1024 (200 MB alone: 33 us, 39; with the sort: 43 us, 45).
 __device__ void clear_share(const EmbedBwdParams& p, int pass, int64_t b, int64_t n) {
   typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
   const int64_t bytes = p.vocab * p.dim * (p.dw_f32 ? 4 : 2), share = (bytes / p.passes + 15) / 16 * 16;
   const int64_t lo = pass * share, hi = pass + 1 == p.passes ? bytes : min(bytes, lo + share);
   char* base = reinterpret_cast<char*>(p.dweight);
   const u32x4_any z = {0u, 0u, 0u, 0u};
-  int64_t at = lo + 16 * (b * kSortThreads + threadIdx.x);
-  for (; at + 16 <= hi; at += 16 * kSortThreads * n) __builtin_nontemporal_store(z, reinterpret_cast<u32x4_any*>(base + at));
+  if (threadIdx.x >= kClearThreads) return;
+  int64_t at = lo + 16 * (b * kClearThreads + threadIdx.x);
+  for (; at + 16 <= hi; at += 16 * kClearThreads * n) __builtin_nontemporal_store(z, reinterpret_cast<u32x4_any*>(base + at));
   for (; at < hi; at += 2) *reinterpret_cast<uint16_t*>(base + at) = 0;         // the last thread's tail, if any
 }
 __global__ __launch_bounds__(kSortThreads) void embed_clear_kernel(EmbedBwdParams p) {
@@ -495,11 +498,12 @@ __global__ __launch_bounds__(256) void embed_join_kernel(EmbedBwdParams p) {
   }
 }
 
-// 64 KB a workgroup, 2048 at most: the ones that clear follow the ones that sum as those end (1999 tokens, 49999 x 1001 fp32:
-// 43 us, with 512 at most 52; with 32 KB each and 4096 at most 51, each having the rows' bits to set first).
-unsigned clear_blocks(int64_t bytes) {
+// Workgroups that clear: 64 KB each, `most` at most.  Beside the sort two a CU.  Beside the sums of few tokens 2048, which
+// follow the sums' as those end (1999 tokens, 49999 x 1001 fp32: 43 us, with 512 at most 52; with 32 KB each and 4096 at
+// most 51, each having the rows' bits to set first).
+unsigned clear_blocks(int64_t bytes, int64_t most) {
   const int64_t b = (bytes + 65535) / 65536;
-  return (unsigned)(b < 2048 ? b : 2048);
+  return (unsigned)(b < most ? b : most);
 }
 
 bool few_tokens(const EmbedBwdParams& p) {
@@ -510,13 +514,13 @@ template <typename T, typename TW>
 hipError_t run_bwd(const EmbedBwdParams& p, hipStream_t st) {
   const int64_t bytes = p.vocab * p.dim * (int64_t)sizeof(TW);
   if (p.tokens == 0) {
-    embed_clear_kernel<<<clear_blocks(bytes), kSortThreads, 0, st>>>(p);
+    embed_clear_kernel<<<clear_blocks(bytes, 512), kSortThreads, 0, st>>>(p);
     return hipGetLastError();
   }
-  const unsigned grid = p.tiles + clear_blocks(bytes / p.passes + 16);
+  const unsigned grid = p.tiles + clear_blocks(bytes / p.passes + 16, 512);
   if (few_tokens(p)) {
     const int sums = (int)((p.tokens + 15) / 16) * ((p.dim + 511) / 512);
-    embed_few_kernel<T, TW><<<sums + clear_blocks(bytes), kSortThreads, 0, st>>>(p, sums);
+    embed_few_kernel<T, TW><<<sums + clear_blocks(bytes, 2048), kSortThreads, 0, st>>>(p, sums);
     return hipGetLastError();
   }
   const bool direct = p.tokens <= kDirect;
