@@ -1,4 +1,4 @@
-// Token table: scaled lookup, and its gradient by sorted tokens.
+// Token table: scaled lookup, and its gradient, of many tokens by sorting them.
 //
 //   out[t] = scale W[ids[t]]  (zeros for an id outside [0, vocab));
 //   dW[v] = scale sum of dy[t] over the tokens t with ids[t] = v != padding_idx, in the order of t.
