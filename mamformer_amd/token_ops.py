@@ -439,8 +439,10 @@ def token_logprobs_bwd(logits, targets, stats, d_logprobs=None, d_entropy=None, 
     """Gradient of ``token_logprobs`` with respect to the logits, (..., V) in their dtype.
 
     stats: the forward's; d_logprobs, d_entropy (...): the gradients of the two results, each optional.  ``out``: where
-    to write it, which may be ``logits`` itself (a loss that needs its logits no more saves their size so).  A row
-    whose gradients are both zero, or that has only -inf, gets zeros whatever its logits are.
+    to write it, which may be ``logits`` itself (a loss that needs its logits no more saves their size so).  To autograd
+    that is an in-place change like torch's own: a backward pass that still has to read the tensor raises, and ``out`` may
+    not be a leaf that requires a gradient, nor a view of one, where gradients are recorded.  A row whose gradients are
+    both zero, or that has only -inf, gets zeros whatever its logits are.
     """
     name = "token_logprobs_bwd"
     _require_cuda(name, logits, targets, stats, d_logprobs, d_entropy, out)
@@ -456,11 +458,15 @@ def token_logprobs_bwd(logits, targets, stats, d_logprobs=None, d_entropy=None, 
             t = t.to(torch.float32).contiguous()
         grads.append(t)
     l2 = _rows(logits, V)
-    if out is None:
+    given = out is not None
+    if not given:
         out = _empty(logits)
         o2 = out if out.dim() == 2 else out.view(-1, V)
     else:
         _like(name, "out", out, logits.shape, logits.dtype)
+        owner = out if out._base is None else out._base
+        if owner.requires_grad and owner.is_leaf and torch.is_grad_enabled():
+            raise RuntimeError(f"{name}: out is a leaf that requires a gradient, or a view of one")
         o2 = out if out.dim() == 2 else out.view(-1, V)      # raises where no rows can be written in place
         if o2.stride(1) != 1 and V > 1:
             raise ValueError(f"{name}: out must have contiguous rows")
@@ -469,6 +475,8 @@ def token_logprobs_bwd(logits, targets, stats, d_logprobs=None, d_entropy=None, 
                        l2.stride(0), tgt.data_ptr(), stats.data_ptr(), _ptr(grads[0]), _ptr(grads[1]), o2.data_ptr(),
                        o2.stride(0))
     _lib.call("mh_token_logprobs_bwd", ct.byref(a), _stream(dev))
+    if given:
+        torch.autograd.graph.increment_version(out)      # the kernel writes where torch does not see it
     return out
 
 

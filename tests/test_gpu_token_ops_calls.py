@@ -1,0 +1,63 @@
+"""Token operators as torch sees their calls: in-place writes and autograd's checks, results that are overwritten, forward-mode
+levels, gradients written beside or in place of the logits, outputs at the C entry points that are their inputs."""
+
+import pytest
+import torch
+
+import mamformer_amd as mh
+from tests.gpu_helpers import say
+
+pytestmark = pytest.mark.gpu
+
+# ------------------------------------------------------------------------------------------------ in-place gradient
+
+def loss_inputs(R=6, V=500):
+    z = torch.randn(R, V, device="cuda")
+    return z, torch.arange(R, device="cuda") % V
+
+
+@pytest.mark.parametrize("reader", ["token_logprobs", "logsumexp"])
+def test_gradient_in_place_of_saved_logits(reader):
+    """Logits that a backward pass still has to read are written over: that pass must say so, not go on from the gradient."""
+    z, t = loss_inputs()
+    leaf = z.clone().requires_grad_(True)
+    logits = leaf * 1.0
+    y = mh.token_logprobs(logits, t).logprobs if reader == "token_logprobs" else torch.logsumexp(logits, -1)
+    out = mh.token_logprobs(z, t)
+    buf, was = logits.detach(), logits._version
+    mh.token_logprobs_bwd(buf, t, out.stats, torch.ones(6, device="cuda"), out=buf)
+    assert logits._version > was
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_gradient_in_place_where_nothing_reads_the_logits_again():
+    """The use that the argument is for: logits of a product, whose backward does not need them."""
+    h, W = torch.randn(6, 32, device="cuda"), torch.randn(500, 32, device="cuda", requires_grad=True)
+    t = torch.arange(6, device="cuda")
+    logits = h @ W.t()
+    want, = torch.autograd.grad(mh.token_logprobs(logits, t).logprobs.sum(), W, retain_graph=True)
+    buf = logits.detach()
+    out = mh.token_logprobs(buf, t)
+    mh.token_logprobs_bwd(buf, t, out.stats, torch.ones(6, device="cuda"), out=buf)
+    got, = torch.autograd.grad(logits, W, buf)
+    assert torch.equal(got, want)
+    with torch.inference_mode():                 # tensors without a version
+        z = torch.randn(6, 500, device="cuda")
+        out = mh.token_logprobs(z, t)
+        want = mh.token_logprobs_bwd(z, t, out.stats, out.entropy)
+        assert torch.equal(mh.token_logprobs_bwd(z, t, out.stats, out.entropy, out=z), want)
+
+
+def test_gradient_into_a_leaf_is_refused():
+    z, t = loss_inputs()
+    out = mh.token_logprobs(z, t)
+    g = torch.ones(6, device="cuda")
+    leaf = z.clone().requires_grad_(True)
+    for target in (leaf, leaf[:, :]):            # the leaf, and a view of it
+        with pytest.raises(RuntimeError, match="leaf"):
+            mh.token_logprobs_bwd(z, t, out.stats, g, out=target)
+    assert torch.equal(leaf.detach(), z)
+    with torch.no_grad():                        # as torch's own in-place operations
+        mh.token_logprobs_bwd(z, t, out.stats, g, out=leaf)
+    assert torch.equal(leaf.detach(), mh.token_logprobs_bwd(z, t, out.stats, g))
