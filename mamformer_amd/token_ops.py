@@ -420,9 +420,10 @@ def _token_logprobs_fwd(logits, targets, temperature, top, ignore_index):
     V, dev, lead = logits.shape[-1], logits.device, tgt.shape
     l2 = _rows(logits, V)
     rows = l2.shape[0]
-    vals = torch.empty((2, *lead), device=dev, dtype=torch.float32)
+    # tensors of their own, not views of one: either may be changed in place without the other
+    lp = torch.empty(lead, device=dev, dtype=torch.float32)
+    ent = torch.empty(lead, device=dev, dtype=torch.float32)
     stats = torch.empty((*lead, 3), device=dev, dtype=torch.float32)
-    lp, ent = vals.unbind(0)
     ids = alt = None
     if top:
         ids = torch.empty((*lead, top), device=dev, dtype=torch.int64)

@@ -61,3 +61,28 @@ def test_gradient_into_a_leaf_is_refused():
     with torch.no_grad():                        # as torch's own in-place operations
         mh.token_logprobs_bwd(z, t, out.stats, g, out=leaf)
     assert torch.equal(leaf.detach(), mh.token_logprobs_bwd(z, t, out.stats, g))
+
+
+# ------------------------------------------------------------------------------------------------ results that are changed
+
+def test_results_changed_in_place():
+    """Log probabilities masked in place, entropies overwritten before the backward: the gradient is that of the masked sum."""
+    z, t = loss_inputs()
+    z.requires_grad_(True)
+    drop = torch.arange(6, device="cuda") % 2 == 0
+    out = mh.token_logprobs(z, t)
+    want, = torch.autograd.grad((out.logprobs.masked_fill(drop, 0.0) * 3).sum() + out.entropy.clamp(min=0).sum(), z)
+    out = mh.token_logprobs(z, t)
+    out.logprobs.masked_fill_(drop, 0.0)
+    out.logprobs.mul_(3)
+    out.entropy.clamp_(min=0)
+    got, = torch.autograd.grad(out.logprobs.sum() + out.entropy.sum(), z)
+    assert torch.equal(got, want)
+    out = mh.token_logprobs(z, t)
+    want, = torch.autograd.grad((out.logprobs ** 2).sum(), z)
+    out = mh.token_logprobs(z, t)
+    loss = (out.logprobs ** 2).sum()             # keeps the log probabilities for its backward
+    with torch.no_grad():
+        out.entropy.zero_()
+    got, = torch.autograd.grad(loss, z)
+    assert torch.equal(got, want)
