@@ -10,10 +10,11 @@
 ``token_logprobs_bwd``                  alternatives, and the logits' gradient
 =====================================  ====================================================================
 
-The first of each pair is differentiable; the ``_bwd`` functions give its gradients explicitly.  bf16 and fp32 tensors
-of any width and row stride (a last dimension that is not contiguous is copied).  As in ``ops``, every call launches
-kernels of ``libmamformer_hip.so`` on the current torch stream, does not synchronise, and has no CPU path.  All results
-are the same bits at every call with the same inputs.
+``embedding``, ``layer_norm`` and ``token_logprobs`` are differentiable (a tensor with a forward-mode tangent is refused);
+the ``_bwd`` functions give their gradients explicitly, and results of those and of packing carry none.  bf16 and fp32
+tensors of any width and row stride (a last dimension that is not contiguous is copied).  As in ``ops``, every call
+launches kernels of ``libmamformer_hip.so`` on the current torch stream, does not synchronise, and has no CPU path.  All
+results are the same bits at every call with the same inputs.
 """
 
 from __future__ import annotations
@@ -22,6 +23,7 @@ import ctypes as ct
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -71,6 +73,19 @@ def _optional_workspace(query, a, dev):
     return ws
 
 
+def _through_autograd(*ts):
+    """Whether a call goes through its autograd function: one of its tensors requires a gradient, or a forward-mode level is
+    open.  A tensor with a tangent does not require a gradient; the functions have no forward-mode rule, so that autograd
+    raises for it rather than take a lost tangent as zero."""
+    if _forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 def _like(name, what, t, shape, dtype):
     if t.shape != shape or t.dtype is not dtype:
         raise ValueError(f"{name}: {what} must be {tuple(shape)} {dtype}, got {tuple(t.shape)} {t.dtype}")
@@ -90,7 +105,7 @@ def embedding(ids, weight, *, scale=1.0, padding_idx=None):
         raise ValueError(f"embedding: weight must be (V, D), got {tuple(weight.shape)}")
     if padding_idx is not None:
         padding_idx = _padding(padding_idx, weight.shape[0])
-    if weight.requires_grad and torch.is_grad_enabled():
+    if _through_autograd(weight):
         return _EmbeddingFn.apply(weight, ids, scale, padding_idx)
     return _embedding_fwd(weight, ids, scale)
 
@@ -252,9 +267,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, residual=None, packed=Fal
     if residual is not None:
         _like(name, "residual", residual, x.shape, x.dtype)
     _norm_params(name, weight, bias, D)
-    if torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad
-                                    or bias is not None and bias.requires_grad
-                                    or residual is not None and residual.requires_grad):
+    if _through_autograd(x, weight, bias, residual):
         y, h, codes, exps, stats = _LayerNormFn.apply(x, residual, weight, bias, eps, packed)
     else:
         y, h, codes, exps, stats = _layer_norm_fwd(x, residual, weight, bias, eps, packed, return_stats)
@@ -403,7 +416,7 @@ def token_logprobs(logits, targets, *, temperature=1.0, top=0, ignore_index=-100
     name = "token_logprobs"
     _require_cuda(name, logits, targets)
     _logprob_shapes(name, logits, targets)
-    if logits.requires_grad and torch.is_grad_enabled():
+    if _through_autograd(logits):
         return TokenLogprobs(*_TokenLogprobsFn.apply(logits, targets, temperature, top, ignore_index))
     return TokenLogprobs(*_token_logprobs_fwd(logits, targets, temperature, top, ignore_index))
 

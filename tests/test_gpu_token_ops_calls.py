@@ -3,6 +3,7 @@ levels, gradients written beside or in place of the logits, outputs at the C ent
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import mamformer_amd as mh
 from tests.gpu_helpers import say
@@ -86,3 +87,31 @@ def test_results_changed_in_place():
         out.entropy.zero_()
     got, = torch.autograd.grad(loss, z)
     assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------------------------------------ forward mode
+
+def test_forward_mode_is_refused():
+    """The operators have no forward-mode rule: a call that a tangent reaches raises rather than drop it."""
+    W, x = torch.randn(20, 8, device="cuda"), torch.randn(3, 8, device="cuda")
+    w, b = torch.randn(2, 8, device="cuda")
+    ids = torch.tensor([0, 4, 7], device="cuda")
+    calls = {
+        "embedding": (lambda p: mh.embedding(ids, p), W),
+        "layer_norm x": (lambda p: mh.layer_norm(p, w, b), x),
+        "layer_norm residual": (lambda p: mh.layer_norm(x, w, b, residual=p), x),
+        "layer_norm weight": (lambda p: mh.layer_norm(x, p, b), w),
+        "layer_norm bias": (lambda p: mh.layer_norm(x, w, p), b),
+        "layer_norm packed": (lambda p: mh.layer_norm(p, w, b, packed=True, return_stats=True), x),
+        "token_logprobs": (lambda p: mh.token_logprobs(p, ids), x),
+    }
+    first = lambda r: r if torch.is_tensor(r) else r[0]
+    for what, (f, p) in calls.items():
+        want = first(f(p))
+        with forward_ad.dual_level():
+            d = forward_ad.make_dual(p, torch.ones_like(p))
+            for grad in (True, False):
+                say(f"{what}, grad mode {grad}")
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+                    f(d)
+            assert torch.equal(first(f(p)), want)        # a level alone, without a tangent, changes nothing
