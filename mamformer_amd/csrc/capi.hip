@@ -2,6 +2,7 @@
 // Every entry point validates its argument block completely before the first
 // HIP call, records a message for mh_last_error() on failure, then fills the
 // internal parameter block and launches on the caller's stream.
+#include <float.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
@@ -946,11 +947,14 @@ int pack_run(const mh_pack_args* a, bool back, hipStream_t st) {
   return hip_status(mh::launch_pack(p, back, st), fn);
 }
 
+constexpr double kLog2e = 1.4426950408889634;
+
 int logprob_common(const char* fn, int64_t rows, int64_t vocab, int32_t dtype, float temperature, const void* logits,
                    int64_t stride, int32_t index_bytes, const void* targets) {
   MH_TRY(sizes_ok(fn, rows, vocab, kMaxDim, dtype));
-  if (!(temperature > 0.f) || !(1.f / temperature > 0.f) || !(1.f / temperature <= 3.4e38f))
-    return fail(MH_ERR_SHAPE, "%s: temperature must be positive and finite", fn);
+  // what the kernels multiply by, 1 / temperature and log2(e) / temperature, has to stay in fp32's range
+  if (!(temperature > 0.f) || !(1.f / temperature > 0.f) || !(kLog2e / temperature <= FLT_MAX))
+    return fail(MH_ERR_SHAPE, "%s: temperature must be positive and finite (at least 4.25e-39)", fn);
   if (rows == 0) return MH_OK;
   MH_TRY(rows_ok(fn, "logits", logits, stride, vocab, elem_size(dtype), false));
   return index_ok(fn, index_bytes, targets, "targets");
@@ -971,7 +975,7 @@ int logprob_validate(const mh_logprob_args* a, mh::LogprobParams& p) {
   }
   p.rows = a->rows; p.vocab = a->vocab; p.ignore_index = a->ignore_index;
   p.dtype = a->dtype; p.i64 = a->index_bytes == 8; p.top = a->top;
-  p.k = (float)(1.4426950408889634 / a->temperature);
+  p.k = (float)(kLog2e / a->temperature);
   p.logits = a->logits; p.l_s = a->logits_stride; p.targets = a->targets;
   p.logprobs = a->logprobs; p.entropy = a->entropy; p.stats = a->stats;
   p.top_ids = a->top_ids; p.top_logprobs = a->top_logprobs; p.workspace = a->workspace;
@@ -1615,7 +1619,7 @@ int mh_token_logprobs_bwd(const mh_logprob_bwd_args* a, void* stream) {
   mh::LogprobBwdParams p;
   p.rows = a->rows; p.vocab = a->vocab; p.ignore_index = a->ignore_index;
   p.dtype = a->dtype; p.i64 = a->index_bytes == 8; p.inv_temp = 1.f / a->temperature;
-  p.k = (float)(1.4426950408889634 / a->temperature);
+  p.k = (float)(kLog2e / a->temperature);
   p.logits = a->logits; p.l_s = a->logits_stride; p.targets = a->targets; p.stats = a->stats;
   p.d_logprobs = a->d_logprobs; p.d_entropy = a->d_entropy; p.dlogits = a->dlogits; p.d_s = a->dlogits_stride;
   return hip_status(mh::launch_logprob_bwd(p, reinterpret_cast<hipStream_t>(stream)), "token_logprobs_bwd");

@@ -6,6 +6,7 @@ import torch
 from torch.autograd import forward_ad
 
 import mamformer_amd as mh
+from mamformer_amd import _lib
 from tests.gpu_helpers import say
 
 pytestmark = pytest.mark.gpu
@@ -115,3 +116,27 @@ def test_forward_mode_is_refused():
                 with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
                     f(d)
             assert torch.equal(first(f(p)), want)        # a level alone, without a tangent, changes nothing
+
+
+# ------------------------------------------------------------------------------------------------ temperature
+
+@pytest.mark.parametrize("temp", [4.5e-39, 3e38])
+def test_temperatures_at_the_ends_of_the_range(temp):
+    """Towards 0 the largest logit has all the weight, towards infinity all have the same."""
+    z = torch.tensor([[1.0, 3.0, 2.0, -5.0], [7.0, 7.0, -float("inf"), 0.0]], device="cuda")
+    out = mh.token_logprobs(z, torch.tensor([1, 0], device="cuda"), temperature=temp, top=2)
+    counts = torch.tensor([1.0, 2.0] if temp < 1 else [4.0, 3.0], device="cuda")
+    # exponents, the sum, its base-2 logarithm and the way back: up to 16 roundings of numbers below 4
+    assert (out.logprobs + counts.log()).abs().max() <= 16 * 4 * 2 ** -24
+    assert (out.entropy - counts.log()).abs().max() <= 16 * 4 * 2 ** -24
+    assert out.top_ids.tolist() == [[1, 2], [0, 1]]
+
+
+@pytest.mark.parametrize("temp", [3.5e-39, 4.2e-39])
+def test_temperature_whose_scale_leaves_the_range(temp):
+    z, t = loss_inputs()
+    st = mh.token_logprobs(z, t).stats
+    with pytest.raises(_lib.MHError, match="temperature"):
+        mh.token_logprobs(z, t, temperature=temp)
+    with pytest.raises(_lib.MHError, match="temperature"):
+        mh.token_logprobs_bwd(z, t, st, st[:, 2], temperature=temp)

@@ -132,3 +132,12 @@ def test_cpu_tensors_are_refused():
                  lambda: mh.token_logprobs(x, ids), lambda: mh.token_logprobs_bwd(x, ids, torch.zeros(3, 3))):
         with pytest.raises(RuntimeError, match="no CPU path"):
             call()
+
+
+@pytest.mark.parametrize("temperature", [3e-39, 3.5e-39, 4.23e-39])
+def test_temperature_whose_scale_leaves_fp32(temperature):
+    """1 / temperature is in fp32's range, log2(e) / temperature is not."""
+    for fn, make in (("mh_token_logprobs_fwd", logprob), ("mh_token_logprobs_bwd", logprob_bwd)):
+        a = make()
+        a.temperature = temperature
+        assert 1 / a.temperature < 3.4e38 and _rc(fn, ct.byref(a), None) == -2
