@@ -493,8 +493,8 @@ int mh_silu_gate_bwd(const mh_gate_args* a, void* stream);
 
 /* ------------------------------------------------------------------------
  * The two ends of a language model and what stands between its layers. Rows are (rows, dim) or (tokens, dim) tensors of
- * any dim and row stride (elements), aligned to an element; the last dimension is contiguous. A call with no rows
- * launches nothing (its weight gradients are cleared).
+ * any dim and row stride (elements; of one row it does not matter), aligned to an element; the last dimension is
+ * contiguous. A call with no rows launches nothing (its weight gradients are cleared).
  * ---------------------------------------------------------------------- */
 
 /* Token table: out[t] = scale * weight[ids[t]], zeros for an id outside [0, vocab). ids are index_bytes (4 or 8) wide. */

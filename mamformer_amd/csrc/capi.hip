@@ -818,11 +818,12 @@ int kda_bwd_validate(const mh_kda_bwd_args* a) {
 }
 
 // ------------------------------------------------------------------ language-model ends
-// Rows of dim elements with a stride: the pointer aligned to an element; rows may share memory if only read (stride 0).
-int rows_ok(const char* fn, const char* name, const void* p, int64_t stride, int64_t dim, int es, bool written) {
+// Rows of dim elements with a stride: the pointer aligned to an element; rows may share memory if only read (stride 0),
+// and one row alone has no use for its stride.
+int rows_ok(const char* fn, const char* name, const void* p, int64_t rows, int64_t stride, int64_t dim, int es, bool written) {
   if (!p) return fail(MH_ERR_NULL, "%s: %s is required", fn, name);
   if ((uintptr_t)p % es) return fail(MH_ERR_ALIGN, "%s: %s must be aligned to an element", fn, name);
-  if (written ? stride < dim : stride < 0)
+  if (written && rows > 1 ? stride < dim : stride < 0)
     return fail(MH_ERR_STRIDE, "%s: row stride of %s is %lld (dim %lld)", fn, name, (long long)stride, (long long)dim);
   return MH_OK;
 }
@@ -860,8 +861,8 @@ int embedding_validate(const mh_embedding_args* a) {
   if (a->tokens == 0) return MH_OK;
   const int es = elem_size(a->dtype);
   MH_TRY(index_ok(fn, a->index_bytes, a->ids, "ids"));
-  MH_TRY(rows_ok(fn, "weight", a->weight, a->weight_stride, a->dim, es, false));
-  return rows_ok(fn, "out", a->out, a->out_stride, a->dim, es, true);
+  MH_TRY(rows_ok(fn, "weight", a->weight, a->vocab, a->weight_stride, a->dim, es, false));
+  return rows_ok(fn, "out", a->out, a->tokens, a->out_stride, a->dim, es, true);
 }
 
 int embedding_bwd_validate(const mh_embedding_bwd_args* a, mh::EmbedBwdParams& p) {
@@ -873,7 +874,7 @@ int embedding_bwd_validate(const mh_embedding_bwd_args* a, mh::EmbedBwdParams& p
   MH_TRY(vec_ok(fn, "dweight", a->dweight, elem_size(a->dweight_dtype), true));
   if (a->tokens > 0) {
     MH_TRY(index_ok(fn, a->index_bytes, a->ids, "ids"));
-    MH_TRY(rows_ok(fn, "dy", a->dy, a->dy_stride, a->dim, elem_size(a->dtype), false));
+    MH_TRY(rows_ok(fn, "dy", a->dy, a->tokens, a->dy_stride, a->dim, elem_size(a->dtype), false));
   }
   memset(&p, 0, sizeof(p));
   p.tokens = a->tokens; p.vocab = a->vocab; p.padding_idx = a->padding_idx;
@@ -898,11 +899,11 @@ int norm_validate(const mh_layer_norm_args* a) {
   if (!a->codes != !a->exponents) return fail(MH_ERR_NULL, "layer_norm: codes and exponents go together");
   if (a->rows == 0) return MH_OK;
   const int es = elem_size(a->dtype);
-  MH_TRY(rows_ok(fn, "x", a->x, a->x_stride, a->dim, es, false));
-  MH_TRY(rows_ok(fn, "y", a->y, a->y_stride, a->dim, es, true));
+  MH_TRY(rows_ok(fn, "x", a->x, a->rows, a->x_stride, a->dim, es, false));
+  MH_TRY(rows_ok(fn, "y", a->y, a->rows, a->y_stride, a->dim, es, true));
   if (a->residual) {
-    MH_TRY(rows_ok(fn, "residual", a->residual, a->residual_stride, a->dim, es, false));
-    MH_TRY(rows_ok(fn, "h", a->h, a->h_stride, a->dim, es, true));
+    MH_TRY(rows_ok(fn, "residual", a->residual, a->rows, a->residual_stride, a->dim, es, false));
+    MH_TRY(rows_ok(fn, "h", a->h, a->rows, a->h_stride, a->dim, es, true));
   }
   if (a->codes && (uintptr_t)a->codes % 8) return fail(MH_ERR_ALIGN, "layer_norm: codes must be 8-byte aligned");
   return vec_ok(fn, "stats", a->stats, 4, false);
@@ -916,16 +917,16 @@ int norm_bwd_validate(const mh_layer_norm_bwd_args* a) {
   MH_TRY(norm_par_ok(fn, a->dweight, a->dbias, "dweight", "dbias", a->weight_dtype));
   if (a->rows == 0) return MH_OK;
   const int es = elem_size(a->dtype);
-  MH_TRY(rows_ok(fn, "dy", a->dy, a->dy_stride, a->dim, es, false));
+  MH_TRY(rows_ok(fn, "dy", a->dy, a->rows, a->dy_stride, a->dim, es, false));
   if (a->h) {
-    MH_TRY(rows_ok(fn, "h", a->h, a->h_stride, a->dim, es, false));
+    MH_TRY(rows_ok(fn, "h", a->h, a->rows, a->h_stride, a->dim, es, false));
   } else {
     if (!a->codes || !a->exponents) return fail(MH_ERR_NULL, "layer_norm_bwd: h, or codes and exponents, are required");
     if ((uintptr_t)a->codes % 8) return fail(MH_ERR_ALIGN, "layer_norm_bwd: codes must be 8-byte aligned");
   }
   MH_TRY(vec_ok(fn, "stats", a->stats, 4, true));
-  if (a->d_h) MH_TRY(rows_ok(fn, "d_h", a->d_h, a->d_h_stride, a->dim, es, false));
-  return rows_ok(fn, "dx", a->dx, a->dx_stride, a->dim, es, true);
+  if (a->d_h) MH_TRY(rows_ok(fn, "d_h", a->d_h, a->rows, a->d_h_stride, a->dim, es, false));
+  return rows_ok(fn, "dx", a->dx, a->rows, a->dx_stride, a->dim, es, true);
 }
 size_t norm_bwd_need(const mh_layer_norm_bwd_args* a) {
   return a->dweight || a->dbias ? mh::norm_bwd_workspace_bytes(a->rows, (int)a->dim) : 0;
@@ -936,7 +937,7 @@ int pack_run(const mh_pack_args* a, bool back, hipStream_t st) {
   if (!a) return fail(MH_ERR_NULL, "%s: args is NULL", fn);
   MH_TRY(sizes_ok(fn, a->rows, a->dim, kTokenMaxDim, a->dtype));
   if (a->rows == 0) return MH_OK;
-  MH_TRY(rows_ok(fn, "x", a->x, a->x_stride, a->dim, elem_size(a->dtype), back));
+  MH_TRY(rows_ok(fn, "x", a->x, a->rows, a->x_stride, a->dim, elem_size(a->dtype), back));
   if (!a->codes || !a->exponents) return fail(MH_ERR_NULL, "%s: codes and exponents are required", fn);
   if ((uintptr_t)a->codes % 8) return fail(MH_ERR_ALIGN, "%s: codes must be 8-byte aligned", fn);
   mh::PackParams p;
@@ -956,7 +957,7 @@ int logprob_common(const char* fn, int64_t rows, int64_t vocab, int32_t dtype, f
   if (!(temperature > 0.f) || !(1.f / temperature > 0.f) || !(kLog2e / temperature <= FLT_MAX))
     return fail(MH_ERR_SHAPE, "%s: temperature must be positive and finite (at least 4.25e-39)", fn);
   if (rows == 0) return MH_OK;
-  MH_TRY(rows_ok(fn, "logits", logits, stride, vocab, elem_size(dtype), false));
+  MH_TRY(rows_ok(fn, "logits", logits, rows, stride, vocab, elem_size(dtype), false));
   return index_ok(fn, index_bytes, targets, "targets");
 }
 
@@ -1612,7 +1613,7 @@ int mh_token_logprobs_bwd(const mh_logprob_bwd_args* a, void* stream) {
   MH_TRY(vec_ok(fn, "d_logprobs", a->d_logprobs, 4, false));
   MH_TRY(vec_ok(fn, "d_entropy", a->d_entropy, 4, false));
   const int es = elem_size(a->dtype);
-  MH_TRY(rows_ok(fn, "dlogits", a->dlogits, a->dlogits_stride, a->vocab, es, true));
+  MH_TRY(rows_ok(fn, "dlogits", a->dlogits, a->rows, a->dlogits_stride, a->vocab, es, true));
   const size_t nl = ((size_t)(a->rows - 1) * a->logits_stride + a->vocab) * es, nd = ((size_t)(a->rows - 1) * a->dlogits_stride + a->vocab) * es;
   if (overlap(a->logits, nl, a->dlogits, nd) && (a->logits != a->dlogits || (a->rows > 1 && a->logits_stride != a->dlogits_stride)))
     return fail(MH_ERR_STRIDE, "token_logprobs_bwd: dlogits overlaps logits elsewhere than in place");

@@ -1,6 +1,8 @@
 """Token operators as torch sees their calls: in-place writes and autograd's checks, results that are overwritten, forward-mode
 levels, gradients written beside or in place of the logits, outputs at the C entry points that are their inputs."""
 
+import ctypes as ct
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -10,6 +12,8 @@ from mamformer_amd import _lib
 from tests.gpu_helpers import say
 
 pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
 
 # ------------------------------------------------------------------------------------------------ in-place gradient
 
@@ -140,3 +144,20 @@ def test_temperature_whose_scale_leaves_the_range(temp):
         mh.token_logprobs(z, t, temperature=temp)
     with pytest.raises(_lib.MHError, match="temperature"):
         mh.token_logprobs_bwd(z, t, st, st[:, 2], temperature=temp)
+
+
+# ------------------------------------------------------------------------------------------------ where outputs may lie
+
+def test_gradient_of_one_row_of_any_stride():
+    """A single row that is the transpose of a column has a row stride of 1."""
+    z, t = torch.randn(500, 1, device="cuda").t(), torch.tensor([7], device="cuda")
+    assert z.stride(0) == 1
+    leaf = torch.randn(500, 1, device="cuda", requires_grad=True)
+    got, = torch.autograd.grad(mh.token_logprobs(leaf.t(), t).logprobs.sum(), leaf)
+    row = leaf.detach().reshape(1, 500).requires_grad_(True)
+    want, = torch.autograd.grad(mh.token_logprobs(row, t).logprobs.sum(), row)
+    assert torch.equal(got, want.t())
+    out = mh.token_logprobs(z, t)
+    want = mh.token_logprobs_bwd(z, t, out.stats, out.entropy)
+    assert torch.equal(mh.token_logprobs_bwd(z, t, out.stats, out.entropy, out=torch.empty(500, 1, device="cuda").t()), want)
+    assert torch.equal(mh.token_logprobs_bwd(z, t, out.stats, out.entropy, out=z), want)
