@@ -591,7 +591,8 @@ int mh_token_logprobs_workspace_bytes(const mh_logprob_args* a, size_t* bytes);
 int mh_token_logprobs_fwd(const mh_logprob_args* a, void* stream);
 
 /* Gradient of the logits from those of logprobs and entropy (fp32, each or NULL). A row whose two are zero, or that is
- *   all -inf, gets zeros whatever its logits are. dlogits may be logits itself (same stride). */
+ *   all -inf, gets zeros whatever its logits are. dlogits may be logits itself (same stride), or rows
+ *   beside its rows in a wider buffer; it may not overlap it otherwise. */
 typedef struct {
   int64_t rows, vocab, ignore_index;
   int32_t dtype, index_bytes;

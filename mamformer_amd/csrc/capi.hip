@@ -832,6 +832,42 @@ int vec_ok(const char* fn, const char* name, const void* p, int es, bool require
   if ((uintptr_t)p % es) return fail(MH_ERR_ALIGN, "%s: %s must be aligned to an element", fn, name);
   return MH_OK;
 }
+// Memory that a call reads or writes: rows of `width` bytes, `stride` bytes apart (a vector is one row).
+struct Region {
+  const char* name;
+  const void* p;
+  int64_t rows, stride, width;
+  bool written;
+  bool by_row;                                   // each element is read and written by one thread, which reads it first
+};
+Region row_region(const char* name, const void* p, int64_t rows, int64_t stride, int64_t dim, int es, bool written) {
+  return {name, p, rows, stride * es, dim * es, written, true};
+}
+Region flat_region(const char* name, const void* p, int64_t bytes, bool written) {
+  return {name, p, 1, bytes, bytes, written, false};
+}
+bool regions_overlap(Region a, Region b) {
+  if ((uintptr_t)a.p > (uintptr_t)b.p) std::swap(a, b);
+  if (!overlap(a.p, (size_t)((a.rows - 1) * a.stride + a.width), b.p, (size_t)((b.rows - 1) * b.stride + b.width))) return false;
+  // rows of one stride are apart where they lie beside each other in a wider buffer
+  if (a.rows > 1 && b.rows > 1 && a.stride != b.stride) return true;
+  const int64_t s = a.rows > 1 ? a.stride : b.stride;
+  if (s < a.width) return true;
+  const int64_t d = (int64_t)(((uintptr_t)b.p - (uintptr_t)a.p) % (uint64_t)s);
+  return d < a.width || d + b.width > s;
+}
+// No region that is written shares memory with another, except one row tensor that is exactly another.
+int regions_ok(const char* fn, const Region* r, int n) {
+  for (int i = 0; i < n; ++i)
+    for (int j = 0; j < i; ++j) {
+      const Region &a = r[i], &b = r[j];
+      if (!(a.written || b.written) || !a.p || !b.p || a.rows <= 0 || b.rows <= 0 || !regions_overlap(a, b)) continue;
+      const bool same = a.p == b.p && a.rows == b.rows && a.width == b.width && (a.rows == 1 || a.stride == b.stride);
+      if (!same || !a.by_row || !b.by_row || (a.written && b.written))
+        return fail(MH_ERR_STRIDE, "%s: %s and %s overlap%s", fn, a.name, b.name, a.by_row && b.by_row ? " elsewhere than in place" : "");
+    }
+  return MH_OK;
+}
 #define MH_TRY(e)          \
   do {                     \
     const int rc_ = (e);   \
@@ -1614,9 +1650,9 @@ int mh_token_logprobs_bwd(const mh_logprob_bwd_args* a, void* stream) {
   MH_TRY(vec_ok(fn, "d_entropy", a->d_entropy, 4, false));
   const int es = elem_size(a->dtype);
   MH_TRY(rows_ok(fn, "dlogits", a->dlogits, a->rows, a->dlogits_stride, a->vocab, es, true));
-  const size_t nl = ((size_t)(a->rows - 1) * a->logits_stride + a->vocab) * es, nd = ((size_t)(a->rows - 1) * a->dlogits_stride + a->vocab) * es;
-  if (overlap(a->logits, nl, a->dlogits, nd) && (a->logits != a->dlogits || (a->rows > 1 && a->logits_stride != a->dlogits_stride)))
-    return fail(MH_ERR_STRIDE, "token_logprobs_bwd: dlogits overlaps logits elsewhere than in place");
+  const Region regions[] = {row_region("dlogits", a->dlogits, a->rows, a->dlogits_stride, a->vocab, es, true),
+                            row_region("logits", a->logits, a->rows, a->logits_stride, a->vocab, es, false)};
+  MH_TRY(regions_ok(fn, regions, 2));
   mh::LogprobBwdParams p;
   p.rows = a->rows; p.vocab = a->vocab; p.ignore_index = a->ignore_index;
   p.dtype = a->dtype; p.i64 = a->index_bytes == 8; p.inv_temp = 1.f / a->temperature;

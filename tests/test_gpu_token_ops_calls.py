@@ -1,8 +1,6 @@
 """Token operators as torch sees their calls: in-place writes and autograd's checks, results that are overwritten, forward-mode
 levels, gradients written beside or in place of the logits, outputs at the C entry points that are their inputs."""
 
-import ctypes as ct
-
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -147,6 +145,23 @@ def test_temperature_whose_scale_leaves_the_range(temp):
 
 
 # ------------------------------------------------------------------------------------------------ where outputs may lie
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_gradient_in_other_columns_of_the_logits_buffer(dtype):
+    R, V = 7, 501
+    t = torch.arange(R, device="cuda")
+    for gap in (0, 3):
+        wide = torch.randn(R, 2 * V + gap, device="cuda").to(dtype)
+        left, right = wide[:, :V], wide[:, V + gap:]
+        for z, d in ((left, right), (right, left)):
+            keep = z.clone()
+            out = mh.token_logprobs(z, t)
+            want = mh.token_logprobs_bwd(keep, t, out.stats, out.entropy)
+            assert torch.equal(mh.token_logprobs_bwd(z, t, out.stats, out.entropy, out=d), want)
+            assert torch.equal(z, keep)
+        with pytest.raises(_lib.MHError, match="overlap"):
+            mh.token_logprobs_bwd(left, t, out.stats, out.entropy, out=wide[:, V - 1:2 * V - 1])
+
 
 def test_gradient_of_one_row_of_any_stride():
     """A single row that is the transpose of a column has a row stride of 1."""
