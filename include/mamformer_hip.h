@@ -494,7 +494,9 @@ int mh_silu_gate_bwd(const mh_gate_args* a, void* stream);
 /* ------------------------------------------------------------------------
  * The two ends of a language model and what stands between its layers. Rows are (rows, dim) or (tokens, dim) tensors of
  * any dim and row stride (elements; of one row it does not matter), aligned to an element; the last dimension is
- * contiguous. A call with no rows launches nothing (its weight gradients are cleared).
+ * contiguous. A call with no rows launches nothing (its weight gradients are cleared). What a call writes may overlap
+ * nothing else that it is given (MH_ERR_STRIDE), except that y and h of a layer norm may each be x or residual itself, dx
+ * dy, h or d_h itself, and dlogits logits itself, with the same stride.
  * ---------------------------------------------------------------------- */
 
 /* Token table: out[t] = scale * weight[ids[t]], zeros for an id outside [0, vocab). ids are index_bytes (4 or 8) wide. */
@@ -591,8 +593,7 @@ int mh_token_logprobs_workspace_bytes(const mh_logprob_args* a, size_t* bytes);
 int mh_token_logprobs_fwd(const mh_logprob_args* a, void* stream);
 
 /* Gradient of the logits from those of logprobs and entropy (fp32, each or NULL). A row whose two are zero, or that is
- *   all -inf, gets zeros whatever its logits are. dlogits may be logits itself (same stride), or rows
- *   beside its rows in a wider buffer; it may not overlap it otherwise. */
+ *   all -inf, gets zeros whatever its logits are. */
 typedef struct {
   int64_t rows, vocab, ignore_index;
   int32_t dtype, index_bytes;

@@ -846,8 +846,9 @@ Region row_region(const char* name, const void* p, int64_t rows, int64_t stride,
 Region flat_region(const char* name, const void* p, int64_t bytes, bool written) {
   return {name, p, 1, bytes, bytes, written, false};
 }
-bool regions_overlap(Region a, Region b) {
-  if ((uintptr_t)a.p > (uintptr_t)b.p) std::swap(a, b);
+bool regions_overlap(const Region& x, const Region& y) {
+  const bool in_order = (uintptr_t)x.p <= (uintptr_t)y.p;
+  const Region &a = in_order ? x : y, &b = in_order ? y : x;
   if (!overlap(a.p, (size_t)((a.rows - 1) * a.stride + a.width), b.p, (size_t)((b.rows - 1) * b.stride + b.width))) return false;
   // rows of one stride are apart where they lie beside each other in a wider buffer
   if (a.rows > 1 && b.rows > 1 && a.stride != b.stride) return true;
@@ -898,7 +899,11 @@ int embedding_validate(const mh_embedding_args* a) {
   const int es = elem_size(a->dtype);
   MH_TRY(index_ok(fn, a->index_bytes, a->ids, "ids"));
   MH_TRY(rows_ok(fn, "weight", a->weight, a->vocab, a->weight_stride, a->dim, es, false));
-  return rows_ok(fn, "out", a->out, a->tokens, a->out_stride, a->dim, es, true);
+  MH_TRY(rows_ok(fn, "out", a->out, a->tokens, a->out_stride, a->dim, es, true));
+  const Region regions[] = {row_region("out", a->out, a->tokens, a->out_stride, a->dim, es, true),
+                            {"weight", a->weight, a->vocab, a->weight_stride * es, a->dim * es, false, false},
+                            flat_region("ids", a->ids, a->tokens * a->index_bytes, false)};
+  return regions_ok(fn, regions, 3);
 }
 
 int embedding_bwd_validate(const mh_embedding_bwd_args* a, mh::EmbedBwdParams& p) {
@@ -942,7 +947,19 @@ int norm_validate(const mh_layer_norm_args* a) {
     MH_TRY(rows_ok(fn, "h", a->h, a->rows, a->h_stride, a->dim, es, true));
   }
   if (a->codes && (uintptr_t)a->codes % 8) return fail(MH_ERR_ALIGN, "layer_norm: codes must be 8-byte aligned");
-  return vec_ok(fn, "stats", a->stats, 4, false);
+  MH_TRY(vec_ok(fn, "stats", a->stats, 4, false));
+  const int ws = elem_size(a->weight_dtype);
+  const int64_t groups = a->rows * ((a->dim + 63) / 64);
+  const Region regions[] = {row_region("y", a->y, a->rows, a->y_stride, a->dim, es, true),
+                            row_region("h", a->residual ? a->h : nullptr, a->rows, a->h_stride, a->dim, es, true),
+                            row_region("x", a->x, a->rows, a->x_stride, a->dim, es, false),
+                            row_region("residual", a->residual, a->rows, a->residual_stride, a->dim, es, false),
+                            flat_region("weight", a->weight, a->dim * ws, false),
+                            flat_region("bias", a->bias, a->dim * ws, false),
+                            flat_region("stats", a->stats, a->rows * 8, true),
+                            flat_region("codes", a->codes, groups * 64, true),
+                            flat_region("exponents", a->exponents, groups, true)};
+  return regions_ok(fn, regions, 9);
 }
 
 int norm_bwd_validate(const mh_layer_norm_bwd_args* a) {
@@ -976,6 +993,11 @@ int pack_run(const mh_pack_args* a, bool back, hipStream_t st) {
   MH_TRY(rows_ok(fn, "x", a->x, a->rows, a->x_stride, a->dim, elem_size(a->dtype), back));
   if (!a->codes || !a->exponents) return fail(MH_ERR_NULL, "%s: codes and exponents are required", fn);
   if ((uintptr_t)a->codes % 8) return fail(MH_ERR_ALIGN, "%s: codes must be 8-byte aligned", fn);
+  const int64_t groups = a->rows * ((a->dim + 63) / 64);
+  const Region regions[] = {{"x", a->x, a->rows, a->x_stride * elem_size(a->dtype), a->dim * elem_size(a->dtype), back, false},
+                            flat_region("codes", a->codes, groups * 64, !back),
+                            flat_region("exponents", a->exponents, groups, !back)};
+  MH_TRY(regions_ok(fn, regions, 3));
   mh::PackParams p;
   p.rows = a->rows; p.dim = (int)a->dim; p.dtype = a->dtype;
   p.x = a->x; p.out = a->x; p.x_s = a->x_stride;
@@ -1581,7 +1603,16 @@ int mh_embedding_bwd_workspace_bytes(const mh_embedding_bwd_args* a, size_t* byt
 int mh_embedding_bwd(const mh_embedding_bwd_args* a, void* stream) {
   mh::EmbedBwdParams p;
   MH_TRY(embedding_bwd_validate(a, p));
-  MH_TRY(workspace_ok("embedding_bwd", a->workspace, a->workspace_bytes, mh::embed_bwd_plan(p, nullptr)));
+  const size_t need = mh::embed_bwd_plan(p, nullptr);
+  MH_TRY(workspace_ok("embedding_bwd", a->workspace, a->workspace_bytes, need));
+  if (a->tokens > 0) {
+    const int es = elem_size(a->dtype);
+    const Region regions[] = {flat_region("dweight", a->dweight, a->vocab * a->dim * elem_size(a->dweight_dtype), true),
+                              {"dy", a->dy, a->tokens, a->dy_stride * es, a->dim * es, false, false},
+                              flat_region("ids", a->ids, a->tokens * a->index_bytes, false),
+                              flat_region("workspace", need ? a->workspace : nullptr, (int64_t)need, true)};
+    MH_TRY(regions_ok("embedding_bwd", regions, 4));
+  }
   mh::embed_bwd_plan(p, a->workspace);
   return hip_status(mh::launch_embed_bwd(p, reinterpret_cast<hipStream_t>(stream)), "embedding_bwd");
 }
@@ -1606,7 +1637,24 @@ int mh_layer_norm_bwd_workspace_bytes(const mh_layer_norm_bwd_args* a, size_t* b
 
 int mh_layer_norm_bwd(const mh_layer_norm_bwd_args* a, void* stream) {
   MH_TRY(norm_bwd_validate(a));
-  MH_TRY(workspace_ok("layer_norm_bwd", a->workspace, a->workspace_bytes, norm_bwd_need(a)));
+  const size_t need = norm_bwd_need(a);
+  MH_TRY(workspace_ok("layer_norm_bwd", a->workspace, a->workspace_bytes, need));
+  if (a->rows > 0) {
+    const int es = elem_size(a->dtype), ws = elem_size(a->weight_dtype);
+    const int64_t groups = a->rows * ((a->dim + 63) / 64);
+    const Region regions[] = {row_region("dx", a->dx, a->rows, a->dx_stride, a->dim, es, true),
+                              flat_region("dweight", a->dweight, a->dim * ws, true),
+                              flat_region("dbias", a->dbias, a->dim * ws, true),
+                              row_region("dy", a->dy, a->rows, a->dy_stride, a->dim, es, false),
+                              row_region("h", a->h, a->rows, a->h_stride, a->dim, es, false),
+                              row_region("d_h", a->d_h, a->rows, a->d_h_stride, a->dim, es, false),
+                              flat_region("codes", a->h ? nullptr : a->codes, groups * 64, false),
+                              flat_region("exponents", a->h ? nullptr : a->exponents, groups, false),
+                              flat_region("stats", a->stats, a->rows * 8, false),
+                              flat_region("weight", a->weight, a->dim * ws, false),
+                              flat_region("workspace", need ? a->workspace : nullptr, (int64_t)need, true)};
+    MH_TRY(regions_ok("layer_norm_bwd", regions, 11));
+  }
   mh::NormBwdParams p;
   p.rows = a->rows; p.dim = (int)a->dim; p.dtype = a->dtype; p.w_f32 = a->weight_dtype == MH_F32;
   p.dy = a->dy; p.dy_s = a->dy_stride; p.h = a->h; p.h_s = a->h_stride;
@@ -1636,7 +1684,20 @@ int mh_token_logprobs_workspace_bytes(const mh_logprob_args* a, size_t* bytes) {
 int mh_token_logprobs_fwd(const mh_logprob_args* a, void* stream) {
   mh::LogprobParams p;
   MH_TRY(logprob_validate(a, p));
-  MH_TRY(workspace_ok("token_logprobs", a->workspace, a->workspace_bytes, mh::logprob_plan(p)));
+  const size_t need = mh::logprob_plan(p);
+  MH_TRY(workspace_ok("token_logprobs", a->workspace, a->workspace_bytes, need));
+  if (a->rows > 0) {
+    const int64_t es = elem_size(a->dtype), tops = a->rows * a->top;
+    const Region regions[] = {flat_region("logprobs", a->logprobs, a->rows * 4, true),
+                              flat_region("entropy", a->entropy, a->rows * 4, true),
+                              flat_region("stats", a->stats, a->rows * 12, true),
+                              flat_region("top_ids", a->top ? a->top_ids : nullptr, tops * 8, true),
+                              flat_region("top_logprobs", a->top ? a->top_logprobs : nullptr, tops * 4, true),
+                              {"logits", a->logits, a->rows, a->logits_stride * es, a->vocab * es, false, false},
+                              flat_region("targets", a->targets, a->rows * a->index_bytes, false),
+                              flat_region("workspace", need ? a->workspace : nullptr, (int64_t)need, true)};
+    MH_TRY(regions_ok("token_logprobs", regions, 8));
+  }
   return hip_status(mh::launch_logprob(p, reinterpret_cast<hipStream_t>(stream)), "token_logprobs");
 }
 
@@ -1651,8 +1712,12 @@ int mh_token_logprobs_bwd(const mh_logprob_bwd_args* a, void* stream) {
   const int es = elem_size(a->dtype);
   MH_TRY(rows_ok(fn, "dlogits", a->dlogits, a->rows, a->dlogits_stride, a->vocab, es, true));
   const Region regions[] = {row_region("dlogits", a->dlogits, a->rows, a->dlogits_stride, a->vocab, es, true),
-                            row_region("logits", a->logits, a->rows, a->logits_stride, a->vocab, es, false)};
-  MH_TRY(regions_ok(fn, regions, 2));
+                            row_region("logits", a->logits, a->rows, a->logits_stride, a->vocab, es, false),
+                            flat_region("targets", a->targets, a->rows * a->index_bytes, false),
+                            flat_region("stats", a->stats, a->rows * 12, false),
+                            flat_region("d_logprobs", a->d_logprobs, a->rows * 4, false),
+                            flat_region("d_entropy", a->d_entropy, a->rows * 4, false)};
+  MH_TRY(regions_ok(fn, regions, 6));
   mh::LogprobBwdParams p;
   p.rows = a->rows; p.vocab = a->vocab; p.ignore_index = a->ignore_index;
   p.dtype = a->dtype; p.i64 = a->index_bytes == 8; p.inv_temp = 1.f / a->temperature;

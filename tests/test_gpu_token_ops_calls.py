@@ -1,6 +1,8 @@
 """Token operators as torch sees their calls: in-place writes and autograd's checks, results that are overwritten, forward-mode
 levels, gradients written beside or in place of the logits, outputs at the C entry points that are their inputs."""
 
+import ctypes as ct
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -176,3 +178,41 @@ def test_gradient_of_one_row_of_any_stride():
     want = mh.token_logprobs_bwd(z, t, out.stats, out.entropy)
     assert torch.equal(mh.token_logprobs_bwd(z, t, out.stats, out.entropy, out=torch.empty(500, 1, device="cuda").t()), want)
     assert torch.equal(mh.token_logprobs_bwd(z, t, out.stats, out.entropy, out=z), want)
+
+
+@pytest.mark.parametrize("R,D", [(9, 64), (40, 1000), (1100, 1000), (5, 3000), (3, 9000)])
+def test_layer_norm_in_place_at_the_c_entry(R, D):
+    """y, h and dx may be the row tensors that they are computed from."""
+    st = torch.cuda.current_stream().cuda_stream
+    x, res, dy, d_h = torch.randn(4, R, D, device="cuda").to(BF)
+    w, b = torch.randn(2, D, device="cuda")
+    y, h, stats = mh.layer_norm(x, w, b, residual=res, return_stats=True)
+    want = mh.layer_norm_bwd(dy, h, stats, w, d_h=d_h)
+
+    def fwd(x, res, y, h):
+        s = torch.empty(R, 2, device="cuda")
+        a = _lib.LayerNormArgs(R, D, _lib.MH_BF16, _lib.MH_F32, 1e-5, x.data_ptr(), D, res.data_ptr(), D, w.data_ptr(),
+                               b.data_ptr(), y.data_ptr(), D, h.data_ptr(), D, s.data_ptr(), None, None)
+        _lib.call("mh_layer_norm_fwd", ct.byref(a), st)
+
+    def bwd(dy, h, d_h, dx):
+        dw, db = torch.empty(2, D, device="cuda")
+        n = ct.c_size_t()
+        a = _lib.LayerNormBwdArgs(R, D, _lib.MH_BF16, _lib.MH_F32, dy.data_ptr(), D, h.data_ptr(), D, None, None,
+                                  stats.data_ptr(), w.data_ptr(), d_h.data_ptr(), D, dx.data_ptr(), D, dw.data_ptr(),
+                                  db.data_ptr())
+        _lib.call("mh_layer_norm_bwd_workspace_bytes", ct.byref(a), ct.byref(n))
+        ws = torch.empty(max(n.value, 16), device="cuda", dtype=torch.uint8)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), n.value
+        _lib.call("mh_layer_norm_bwd", ct.byref(a), st)
+        torch.cuda.synchronize()
+        return dw, db
+
+    for y_in, h_in in ((0, 1), (1, 0)):                  # y over x and h over residual, and the other way round
+        both = [x.clone(), res.clone()]
+        fwd(*both, both[y_in], both[h_in])
+        assert torch.equal(both[y_in], y) and torch.equal(both[h_in], h)
+    for over in range(3):
+        bufs = [dy.clone(), h.clone(), d_h.clone()]
+        dw, db = bwd(*bufs, bufs[over])
+        assert torch.equal(bufs[over], want[0]) and torch.equal(dw, want[1]) and torch.equal(db, want[2])
