@@ -73,17 +73,13 @@ def _optional_workspace(query, a, dev):
     return ws
 
 
-def _through_autograd(*ts):
+def _through_autograd(a, b=None, c=None, d=None):
     """Whether a call goes through its autograd function: one of its tensors requires a gradient, or a forward-mode level is
     open.  A tensor with a tangent does not require a gradient; the functions have no forward-mode rule, so that autograd
     raises for it rather than take a lost tangent as zero."""
-    if _forward_ad._current_level >= 0:
-        return True
-    if torch.is_grad_enabled():
-        for t in ts:
-            if t is not None and t.requires_grad:
-                return True
-    return False
+    return _forward_ad._current_level >= 0 or (
+        a.requires_grad or b is not None and b.requires_grad or c is not None and c.requires_grad
+        or d is not None and d.requires_grad) and torch.is_grad_enabled()
 
 
 def _like(name, what, t, shape, dtype):
@@ -434,9 +430,10 @@ def _token_logprobs_fwd(logits, targets, temperature, top, ignore_index):
     l2 = _rows(logits, V)
     rows = l2.shape[0]
     # tensors of their own, not views of one: either may be changed in place without the other
-    lp = torch.empty(lead, device=dev, dtype=torch.float32)
-    ent = torch.empty(lead, device=dev, dtype=torch.float32)
-    stats = torch.empty((*lead, 3), device=dev, dtype=torch.float32)
+    # (made from others, which is the shorter way)
+    lp = torch.empty_like(tgt, dtype=torch.float32)
+    ent = torch.empty_like(lp)
+    stats = lp.new_empty((*lead, 3))
     ids = alt = None
     if top:
         ids = torch.empty((*lead, top), device=dev, dtype=torch.int64)
