@@ -24,7 +24,12 @@ namespace {
 constexpr int kBits = 9, kDigits = 1 << kBits;   // a pass: 512 counters, two a thread
 constexpr int kSortThreads = 1024;               // 64 tokens a wave of the smallest tile
 constexpr int kClearThreads = 256;               // of these, the ones that clear beside a sort
-constexpr int kFew = 2048;                       // up to here, in a table of up to kFewRows, nothing is sorted
+// Up to here, in a table of up to kFewRows, nothing is sorted.  us, compared and sorted, for ids whose frequencies fall as the
+// inverse of the rank, for even ones and for one id alone: 32000 x 1024 bf16, 16 tokens 13 and 18, 14 and 19, 14 and 20;
+// 1000 tokens 16 and 21, 16 and 21, 22 and 25; 2000 tokens 21 and 22, 18 and 22, 39 and 32; 3000 tokens (with kFew = 4096) 28
+// and 24, 21 and 24, 65 and 40.  1000 x 1024, 1000 tokens 13 and 18, 6 and 17, 21 and 22; 2000 tokens 17 and 21, 8 and 19,
+// 37 and 30; 3000 tokens 22 and 22, 14 and 21, 54 and 38.  32000 x 2048, 2000 tokens 36 and 33, 31 and 32, 48 and 40.
+constexpr int kFew = 2048;
 constexpr int kFewRows = 1 << 18;
 // up to here a pass counts all tokens by itself (32000 x 1024 bf16: 4096 tokens 28 us, counted for 40; 16000: both 49;
 // 30000: 76 and 68)
@@ -84,9 +89,9 @@ __global__ __launch_bounds__(256) void embed_count_kernel(EmbedBwdParams p) {
   h[threadIdx.x + 256] = cnt[threadIdx.x + 256];
 }
 
-// Zeros for share `pass` of the table's `passes` equal shares, by workgroup b of n, past the caches (131 MB of a table with its
-// sort: 45 us, through them 48) and by a quarter of the threads: 2 x 256 a CU that move along the table together write
-// faster than 2 x 1024 (200 MB alone: 33 us, 39; with the sort: 43 us, 45).
+// Zeros for share `pass` of the table's `passes` equal shares, by workgroup b of n, past the caches (the whole gradient of 8192
+// tokens, 131 MB of table: 45 us, through them 48) and by a quarter of the threads: 2 x 256 a CU that move along the table
+// together write faster than 2 x 1024 (200 MB alone: 33 us, 39; the gradient of the 8192 tokens: 43 us, 45).
 __device__ void clear_share(const EmbedBwdParams& p, int pass, int64_t b, int64_t n) {
   typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
   const int64_t bytes = p.vocab * p.dim * (p.dw_f32 ? 4 : 2), share = (bytes / p.passes + 15) / 16 * 16;
@@ -574,7 +579,7 @@ size_t embed_bwd_plan(EmbedBwdParams& p, void* workspace) {
     p.keys[i] = reinterpret_cast<uint32_t*>(take((size_t)p.tokens * 4));
     p.order[i] = reinterpret_cast<uint32_t*>(take((size_t)p.tokens * 4));
   }
-  if (few_tokens(p)) return off;                 // which neither counts nor has partial rows
+  if (few_tokens(p)) return off;                 // which use none of it; 16 bytes a token are asked for at every size
   p.hist = reinterpret_cast<uint32_t*>(take((size_t)p.passes * p.tiles * kDigits * 4));
   p.part = reinterpret_cast<float*>(take((size_t)2 * p.pieces * p.dim * 4));
   return off;

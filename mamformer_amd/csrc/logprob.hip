@@ -416,7 +416,7 @@ __global__ __launch_bounds__(kNT) void logprob_bwd_kernel(LogprobBwdParams p) {
 
 // Two workgroups a CU are wanted (777 x 50001 fp32 with its gradient, three rows a CU: 88.6 us, in two spans each 90.5; 24 x
 // 128000 with 20 alternatives: 19 us at 528 and at 768 workgroups, 71 us in one kernel of a workgroup a row); a span of a
-// row has 4096 columns at least, two turns of its threads.
+// row has more than 2048 columns, a turn of its threads, and there is one for each 4096 of the row at most.
 size_t logprob_plan(LogprobParams& p) {
   const int64_t want = p.rows ? (512 + p.rows - 1) / p.rows : 1, most = (p.vocab + 4095) / 4096;
   int64_t n = want < most ? want : most;

@@ -8,7 +8,7 @@
 // A row lives in the registers of a group of threads (8 channels a thread and step), so every tensor is read and
 // written once and the variance is that of the centred values.  Groups: as many lanes of a wave as the row has chunks,
 // from 8 (heads of 64 channels) to a wave, which needs no barrier; beyond, a workgroup of 128 to 1024 threads.  Sums are
-// fp32.  Bound by memory: 32768 x 4096 bf16 with 8-bit rows moves 1.2 GB forward in 195 us and 0.94 GB backward in 143.
+// fp32.  Bound by memory: 32768 x 4096 bf16 with 8-bit rows moves 1.2 GB forward in 199 us and 0.94 GB backward in 154.
 #include <type_traits>
 
 #include "common.h"
@@ -194,6 +194,8 @@ __global__ __launch_bounds__(kThreads<TPR>) void norm_bwd_kernel(NormBwdParams p
   static_assert(G == 1 || NV == 1, "one chunk a thread where a workgroup has several rows");
   // Two chunks a thread, 1024 threads of 128 registers: the sums for dw and db wait in LDS (every thread's own, read and
   // written once a row).  The weight stays in registers: read again with every row it would wait for the next row's chunks.
+  // Of bf16 rows that fits (8192 x 12000: 142 us with the join, 590 MB, at a copy's rate 95; from 8 bits 122); of fp32 rows
+  // 80 bytes a lane go to scratch memory, 20 from 8 bits (4096 x 12000: 159 us, 590 MB; 108).
   constexpr bool kKeep = NV == 1;
   __shared__ float2 sums[2 * 16];
   __shared__ float park[G > 1 ? G * W : 1];
@@ -428,8 +430,8 @@ auto with_fwd_group(int64_t rows, int dim, F&& f) {
   return f(Group<1024, 2>{});
 }
 // The backward's sums take two registers a channel more: one chunk a thread as far as a workgroup goes, which leaves
-// registers for more waves and the next row (32768 x 4096 from 8-bit rows: 512 threads with one chunk 143 us, 256 with two
-// 166; 4001 x 8192 fp32: 1024 with one 77, 512 with two 88; 100001 x 1000 bf16: 128 with one 137, a wave with two 144).
+// registers for more waves and the next row (with the join, 32768 x 4096 from 8-bit rows: 512 threads with one chunk 153 us,
+// 256 with two 165; from bf16 rows 187 and 182; 4001 x 8192 fp32: 1024 with one 91, 512 with two 96).
 template <typename F>
 auto with_bwd_group(int dim, F&& f) {
   if (dim <= 64) return f(Group<8, 1>{});
@@ -461,9 +463,12 @@ hipError_t run_fwd(const NormParams& p, hipStream_t st, Group<TPR, NV, ROWS>) {
   return hipGetLastError();
 }
 
-// Workgroups that the registers let a CU hold, twice as many for short rows, whose partials are small: more would make more
-// partials than they hide latency (8192 x 2048: 25 us with 512 workgroups and 4.0 for the partials' sums, 24.6 and 5.0
-// with 1024; 131072 x 128: 18.1 with 1024, 19.8 with 512).
+// Every workgroup leaves a row of partials each for dw and db, written and read again, so there are fewer workgroups than
+// would hide more latency: two a CU, one of 1024 threads (8192 x 2048: 25 us with 512 workgroups and 4.0 for the partials'
+// sums, 24.6 and 5.0 with 1024), four of the short rows, whose partials are small (131072 x 128: 18.1 with 1024, 19.8 with
+// 512).  Of 128 threads, for 513 to 1024 channels, eight: many rows need them (with the join, 32768 x 1024 bf16: 48 us,
+// with 512 in all 80; 100001 x 1000: 146 and 395), few rows pay for the partials (8192 x 1024: 22.5 both, fp32 28 and 25;
+// 2048 x 1024, a row a workgroup: 20 and 11).
 template <int TPR, int NV>
 int bwd_blocks(int64_t rows, Group<TPR, NV>) {
   constexpr int G = kThreads<TPR> / TPR;

@@ -210,8 +210,9 @@ def pack_activations(x):
     """x (..., D) as ``PackedActivations``: about half a bf16 tensor's memory.
 
     Each 64 channels of a row share the exponent e of the least power of two with max|x| <= 127 * 2**e; a code is
-    x * 2**-e rounded to nearest even, so |error| <= 2**(e - 1), at most 1/128 of the group's largest value.  A group
-    that holds an infinity or a NaN reads back as NaN.  Not differentiable: it is for what a backward pass keeps.
+    x * 2**-e rounded to nearest even, so |error| <= 2**(e - 1), less than 1/127 of the group's largest value where that is
+    a normal number (e is at least -132: smaller groups keep an absolute error of 2**-133).  A group that holds an infinity
+    or a NaN reads back as NaN.  Not differentiable: it is for what a backward pass keeps.
     """
     _require_cuda("pack_activations", x)
     dt = _dtype("pack_activations", "x", x)
