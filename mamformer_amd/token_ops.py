@@ -246,7 +246,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, residual=None, packed=Fal
 
     x (..., D), D <= 16384; weight, bias (D,) fp32 or bf16 of one dtype, each optional.  With ``residual`` (like x) what
     is normalised is h = x + residual, rounded to the dtype of x, and h is returned too: the stream that goes on.  Mean
-    and variance are fp32, the variance that of the centred values.
+    and variance are fp32, the variance that of the centred values; a row whose sum or squares leave fp32's range (values
+    beyond about 1e19) is NaN throughout.
 
     Returns y (like x), or a tuple of y, then h (with ``residual``), then h as ``PackedActivations`` (``packed``), then
     the rows' fp32 (mean, 1 / sqrt(var + eps)), shaped (..., 2) (``return_stats``).

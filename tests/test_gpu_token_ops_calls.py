@@ -216,3 +216,20 @@ def test_layer_norm_in_place_at_the_c_entry(R, D):
         bufs = [dy.clone(), h.clone(), d_h.clone()]
         dw, db = bwd(*bufs, bufs[over])
         assert torch.equal(bufs[over], want[0]) and torch.equal(dw, want[1]) and torch.equal(db, want[2])
+
+
+# ------------------------------------------------------------------------------------------------ rows out of range
+
+@pytest.mark.parametrize("D", [40, 600, 2048, 5000, 12000])
+def test_layer_norm_of_rows_out_of_range(D):
+    """Squares or sums beyond fp32: NaN in that row, its statistics' scale and its gradient, and nowhere else."""
+    x = torch.randn(5, D, device="cuda")
+    want, ws = mh.layer_norm(x, return_stats=True)
+    good = [0, 2, 4]
+    x[1] *= 1e25
+    x[3] = 3e38
+    y, st = mh.layer_norm(x, return_stats=True)
+    assert torch.equal(y[good], want[good]) and torch.equal(st[good], ws[good])
+    assert y[[1, 3]].isnan().all() and st[[1, 3], 1].isnan().all()
+    dx, _, _ = mh.layer_norm_bwd(torch.ones_like(x), x, st, bias=False)
+    assert dx[good].isfinite().all() and dx[[1, 3]].isnan().all()
