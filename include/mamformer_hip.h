@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define MH_ABI_VERSION 11
+#define MH_ABI_VERSION 12
 
 /* element types of x / B / C / y / q / k / v / o */
 enum { MH_F32 = 0, MH_BF16 = 1 };
@@ -604,6 +604,116 @@ typedef struct {
   void* dlogits; int64_t dlogits_stride;
 } mh_logprob_bwd_args;
 int mh_token_logprobs_bwd(const mh_logprob_bwd_args* a, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Around and beside the linear-attention scans: the gated delta rule, rotary positions, group norm. Tensors have any strides
+ * (elements, not negative; of a dimension of size 1 they do not matter) with contiguous channels, aligned to an element;
+ * inputs may be broadcast (stride 0). What a call writes may overlap nothing else that it is given, from its first to its
+ * last element (MH_ERR_STRIDE), except where it says so. A call with no rows launches nothing.
+ * ---------------------------------------------------------------------- */
+
+/* Gated delta rule, S (dk, dv) fp32 for each (batch, head):
+ *     S_t = e^{g_t} S_{t-1} + beta_t k_t (v_t - e^{g_t} S_{t-1}^T k_t)^T,   o_t = scale S_t^T q_t.
+ *   q, k (batch, kheads, seqlen, dk), v, o (batch, heads, seqlen, dv) in dtype; heads a multiple of kheads, value head h reads
+ *   key head h / (heads / kheads). g, beta (batch, heads, seqlen) fp32, each or NULL (g = 0, beta = 1); g = -inf clears the
+ *   state. initial_state, final_state (batch, heads, dk, dv) fp32 contiguous, each or NULL. dk <= 128, dv <= 256,
+ *   batch * heads * ceil(seqlen / 64) <= 2^23. A NaN or infinity may reach every result of its head from the 64-token piece
+ *   that holds it on, and no other head's. seqlen = 0 copies the state. The same bits at every call. */
+typedef struct {
+  int64_t batch, heads, kheads, seqlen, dk, dv;
+  int32_t dtype;
+  float scale;
+  const void* q; int64_t q_stride_b, q_stride_h, q_stride_l;
+  const void* k; int64_t k_stride_b, k_stride_h, k_stride_l;
+  const void* v; int64_t v_stride_b, v_stride_h, v_stride_l;
+  const float* g; int64_t g_stride_b, g_stride_h, g_stride_l;
+  const float* beta; int64_t beta_stride_b, beta_stride_h, beta_stride_l;
+  const float* initial_state;
+  float* final_state;
+  void* o; int64_t o_stride_b, o_stride_h, o_stride_l;
+  void* workspace; size_t workspace_bytes;
+} mh_delta_args;
+int mh_delta_rule_workspace_bytes(const mh_delta_args* a, size_t* bytes);
+int mh_delta_rule_fwd(const mh_delta_args* a, void* stream);
+
+/* Its backward. fwd: the forward's arguments (o, final_state and the workspace ignored). d_o like o, d_final_state like
+ *   final_state or NULL; dq, dk, dv like q, k, v (written, the heads that share a key head summed in their order), dg, dbeta
+ *   (batch, heads, seqlen) fp32 contiguous, each or NULL, d_initial_state or NULL. */
+typedef struct {
+  mh_delta_args fwd;
+  const void* d_o; int64_t d_o_stride_b, d_o_stride_h, d_o_stride_l;
+  const float* d_final_state;
+  void* dq; int64_t dq_stride_b, dq_stride_h, dq_stride_l;
+  void* dk; int64_t dk_stride_b, dk_stride_h, dk_stride_l;
+  void* dv; int64_t dv_stride_b, dv_stride_h, dv_stride_l;
+  float* dg; float* dbeta; float* d_initial_state;
+  void* workspace; size_t workspace_bytes;
+} mh_delta_bwd_args;
+int mh_delta_rule_bwd_workspace_bytes(const mh_delta_bwd_args* a, size_t* bytes);
+int mh_delta_rule_bwd(const mh_delta_bwd_args* a, void* stream);
+
+/* One token: q, k (batch, kheads, dk), v, o (batch, heads, dv), g, beta (batch, heads). state_out may be state_in itself. */
+typedef struct {
+  int64_t batch, heads, kheads, dk, dv;
+  int32_t dtype;
+  float scale;
+  const void* q; int64_t q_stride_b, q_stride_h;
+  const void* k; int64_t k_stride_b, k_stride_h;
+  const void* v; int64_t v_stride_b, v_stride_h;
+  const float* g; int64_t g_stride_b, g_stride_h;
+  const float* beta; int64_t beta_stride_b, beta_stride_h;
+  const float* state_in; float* state_out;
+  void* o; int64_t o_stride_b, o_stride_h;
+} mh_delta_step_args;
+int mh_delta_step(const mh_delta_step_args* a, void* stream);
+
+/* Rotary positions: of the first 2 * pairs channels, the pairs (i, pairs + i), or (2 i, 2 i + 1) if interleaved, are turned
+ *   by the angle (positions[b, l] + offset) * inv_freq[i] and scaled; the others are copied. inverse: by the negative angle
+ *   (the gradient). q (batch, q_heads, seqlen, dim) and k (batch, k_heads, seqlen, dim; k_heads may be 0). positions
+ *   (batch, seqlen) of index_bytes (4 or 8), rows positions_stride_b apart (0: one row for all), or NULL for 0 .. seqlen - 1;
+ *   inv_freq (pairs,) fp32 or (freq_f64) fp64. Angles are reduced in fp64. Outputs may be their inputs themselves. */
+typedef struct {
+  int64_t batch, q_heads, k_heads, seqlen, dim, pairs;
+  int32_t dtype, interleaved, inverse, freq_f64, index_bytes;
+  float scale;
+  const void* inv_freq;
+  const void* positions; int64_t positions_stride_b;
+  int64_t offset;
+  const void* q; int64_t q_stride_b, q_stride_h, q_stride_l;
+  const void* k; int64_t k_stride_b, k_stride_h, k_stride_l;
+  void* q_out; int64_t q_out_stride_b, q_out_stride_h, q_out_stride_l;
+  void* k_out; int64_t k_out_stride_b, k_out_stride_h, k_out_stride_l;
+} mh_rotary_args;
+int mh_rotary(const mh_rotary_args* a, void* stream);
+
+/* Group norm, channels last: x, y (batch, space, channels), `groups` of neighbouring channels, mean and variance of each
+ *   (batch, group) over the space and its channels; z = (x - mean) / sqrt(var + eps) * weight + bias, y = z, or z sigmoid(z)
+ *   (silu). weight, bias (channels,) in weight_dtype, each or NULL. stats (batch, groups, 2) fp32 (mean, 1 / sqrt(var + eps))
+ *   or NULL. channels <= 65536, batch * space <= 2^40. */
+typedef struct {
+  int64_t batch, space, channels, groups;
+  int32_t dtype, weight_dtype, silu, reserved;
+  float eps;
+  const void* x; int64_t x_stride_b, x_stride_s;
+  const void* weight; const void* bias;
+  void* y; int64_t y_stride_b, y_stride_s;
+  float* stats;
+  void* workspace; size_t workspace_bytes;
+} mh_group_norm_args;
+int mh_group_norm_workspace_bytes(const mh_group_norm_args* a, size_t* bytes);
+int mh_group_norm_fwd(const mh_group_norm_args* a, void* stream);
+
+/* Its backward. fwd: the forward's arguments (y and the workspace ignored, stats read). dweight, dbias
+ *   (channels,) in weight_dtype, each or NULL, written, the same bits at every call. */
+typedef struct {
+  mh_group_norm_args fwd;
+  const void* dy; int64_t dy_stride_b, dy_stride_s;
+  void* dx; int64_t dx_stride_b, dx_stride_s;
+  void* dweight; void* dbias;
+  void* workspace; size_t workspace_bytes;
+} mh_group_norm_bwd_args;
+int mh_group_norm_bwd_workspace_bytes(const mh_group_norm_bwd_args* a, size_t* bytes);
+int mh_group_norm_bwd(const mh_group_norm_bwd_args* a, void* stream);
 
 #ifdef __cplusplus
 }

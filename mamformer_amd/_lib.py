@@ -12,7 +12,7 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libmamformer_hip.so"
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 # bytes of the static device scratch behind mh_ssd_chunk_scan_fwd_noalloc (MH_NOALLOC_SCRATCH_BYTES)
 NOALLOC_SCRATCH_BYTES = 64 << 20
@@ -251,6 +251,74 @@ class LogprobBwdArgs(ct.Structure):
     ]
 
 
+class DeltaArgs(ct.Structure):
+    _fields_ = [
+        ("batch", _i64), ("heads", _i64), ("kheads", _i64), ("seqlen", _i64), ("dk", _i64), ("dv", _i64),
+        ("dtype", _i32), ("scale", _f32),
+        ("q", _vp), ("q_stride_b", _i64), ("q_stride_h", _i64), ("q_stride_l", _i64),
+        ("k", _vp), ("k_stride_b", _i64), ("k_stride_h", _i64), ("k_stride_l", _i64),
+        ("v", _vp), ("v_stride_b", _i64), ("v_stride_h", _i64), ("v_stride_l", _i64),
+        ("g", _vp), ("g_stride_b", _i64), ("g_stride_h", _i64), ("g_stride_l", _i64),
+        ("beta", _vp), ("beta_stride_b", _i64), ("beta_stride_h", _i64), ("beta_stride_l", _i64),
+        ("initial_state", _vp), ("final_state", _vp),
+        ("o", _vp), ("o_stride_b", _i64), ("o_stride_h", _i64), ("o_stride_l", _i64),
+        ("workspace", _vp), ("workspace_bytes", _sz),
+    ]
+
+
+class DeltaBwdArgs(ct.Structure):
+    _fields_ = [
+        ("fwd", DeltaArgs),
+        ("d_o", _vp), ("d_o_stride_b", _i64), ("d_o_stride_h", _i64), ("d_o_stride_l", _i64),
+        ("d_final_state", _vp),
+        ("dq", _vp), ("dq_stride_b", _i64), ("dq_stride_h", _i64), ("dq_stride_l", _i64),
+        ("dk", _vp), ("dk_stride_b", _i64), ("dk_stride_h", _i64), ("dk_stride_l", _i64),
+        ("dv", _vp), ("dv_stride_b", _i64), ("dv_stride_h", _i64), ("dv_stride_l", _i64),
+        ("dg", _vp), ("dbeta", _vp), ("d_initial_state", _vp),
+        ("workspace", _vp), ("workspace_bytes", _sz),
+    ]
+
+
+class DeltaStepArgs(ct.Structure):
+    _fields_ = [
+        ("batch", _i64), ("heads", _i64), ("kheads", _i64), ("dk", _i64), ("dv", _i64), ("dtype", _i32), ("scale", _f32),
+        ("q", _vp), ("q_stride_b", _i64), ("q_stride_h", _i64), ("k", _vp), ("k_stride_b", _i64), ("k_stride_h", _i64),
+        ("v", _vp), ("v_stride_b", _i64), ("v_stride_h", _i64), ("g", _vp), ("g_stride_b", _i64), ("g_stride_h", _i64),
+        ("beta", _vp), ("beta_stride_b", _i64), ("beta_stride_h", _i64), ("state_in", _vp), ("state_out", _vp),
+        ("o", _vp), ("o_stride_b", _i64), ("o_stride_h", _i64),
+    ]
+
+
+class RotaryArgs(ct.Structure):
+    _fields_ = [
+        ("batch", _i64), ("q_heads", _i64), ("k_heads", _i64), ("seqlen", _i64), ("dim", _i64), ("pairs", _i64),
+        ("dtype", _i32), ("interleaved", _i32), ("inverse", _i32), ("freq_f64", _i32), ("index_bytes", _i32), ("scale", _f32),
+        ("inv_freq", _vp), ("positions", _vp), ("positions_stride_b", _i64), ("offset", _i64),
+        ("q", _vp), ("q_stride_b", _i64), ("q_stride_h", _i64), ("q_stride_l", _i64),
+        ("k", _vp), ("k_stride_b", _i64), ("k_stride_h", _i64), ("k_stride_l", _i64),
+        ("q_out", _vp), ("q_out_stride_b", _i64), ("q_out_stride_h", _i64), ("q_out_stride_l", _i64),
+        ("k_out", _vp), ("k_out_stride_b", _i64), ("k_out_stride_h", _i64), ("k_out_stride_l", _i64),
+    ]
+
+
+class GroupNormArgs(ct.Structure):
+    _fields_ = [
+        ("batch", _i64), ("space", _i64), ("channels", _i64), ("groups", _i64),
+        ("dtype", _i32), ("weight_dtype", _i32), ("silu", _i32), ("reserved", _i32), ("eps", _f32),
+        ("x", _vp), ("x_stride_b", _i64), ("x_stride_s", _i64), ("weight", _vp), ("bias", _vp),
+        ("y", _vp), ("y_stride_b", _i64), ("y_stride_s", _i64), ("stats", _vp),
+        ("workspace", _vp), ("workspace_bytes", _sz),
+    ]
+
+
+class GroupNormBwdArgs(ct.Structure):
+    _fields_ = [
+        ("fwd", GroupNormArgs), ("dy", _vp), ("dy_stride_b", _i64), ("dy_stride_s", _i64),
+        ("dx", _vp), ("dx_stride_b", _i64), ("dx_stride_s", _i64), ("dweight", _vp), ("dbias", _vp),
+        ("workspace", _vp), ("workspace_bytes", _sz),
+    ]
+
+
 # entry points of the language-model ends and their argument blocks; each takes a stream, the queries a size
 _TOKEN_CALLS = {
     "mh_embedding_fwd": EmbeddingArgs, "mh_embedding_bwd": EmbeddingBwdArgs,
@@ -261,6 +329,15 @@ _TOKEN_CALLS = {
 _TOKEN_QUERIES = {
     "mh_embedding_bwd_workspace_bytes": EmbeddingBwdArgs, "mh_layer_norm_bwd_workspace_bytes": LayerNormBwdArgs,
     "mh_token_logprobs_workspace_bytes": LogprobArgs,
+}
+# the same around the linear-attention scans
+_MIXER_CALLS = {
+    "mh_delta_rule_fwd": DeltaArgs, "mh_delta_rule_bwd": DeltaBwdArgs, "mh_delta_step": DeltaStepArgs,
+    "mh_rotary": RotaryArgs, "mh_group_norm_fwd": GroupNormArgs, "mh_group_norm_bwd": GroupNormBwdArgs,
+}
+_MIXER_QUERIES = {
+    "mh_delta_rule_workspace_bytes": DeltaArgs, "mh_delta_rule_bwd_workspace_bytes": DeltaBwdArgs,
+    "mh_group_norm_workspace_bytes": GroupNormArgs, "mh_group_norm_bwd_workspace_bytes": GroupNormBwdArgs,
 }
 
 # every symbol include/mamformer_hip.h declares
@@ -279,7 +356,7 @@ EXPORTS = (
     "mh_mamba2_layer_step_workspace_bytes", "mh_mamba2_layer_step",
     "mh_causal_conv1d_fwd",
     "mh_conv1d_bwd_workspace_bytes", "mh_causal_conv1d_bwd",
-    *_TOKEN_CALLS, *_TOKEN_QUERIES,
+    *_TOKEN_CALLS, *_TOKEN_QUERIES, *_MIXER_CALLS, *_MIXER_QUERIES,
 )
 
 _lock = threading.Lock()
@@ -351,7 +428,8 @@ def lib():
                          "mh_ssd_ref_scan_bwd_workspace_bytes", "mh_ssd_ref_scan_bwd",
                          "mh_silu_gate_fwd", "mh_silu_gate_bwd"):
                 getattr(h, name).restype = ct.c_int
-            for names, last in ((_TOKEN_CALLS, _vp), (_TOKEN_QUERIES, ct.POINTER(_sz))):
+            for names, last in ((_TOKEN_CALLS, _vp), (_TOKEN_QUERIES, ct.POINTER(_sz)), (_MIXER_CALLS, _vp),
+                                (_MIXER_QUERIES, ct.POINTER(_sz))):
                 for name, block in names.items():
                     getattr(h, name).argtypes = [ct.POINTER(block), last]
                     getattr(h, name).restype = ct.c_int

@@ -1047,6 +1047,127 @@ int workspace_ok(const char* fn, const void* ws, size_t got, size_t need) {
   return MH_OK;
 }
 
+// ------------------------------------------------------------------ around the linear-attention scans
+// A tensor (n[0], n[1], n[2], width) with contiguous channels, and its memory from the first to the last element.
+struct Strided {
+  const char* name;
+  const void* p;
+  int64_t n[3], s[3], width;
+  int es;
+  bool written;
+};
+int strided_ok(const char* fn, const Strided& t, Region& r) {
+  r = Region{t.name, nullptr, 0, 0, 0, t.written, false};
+  if (!t.p) return fail(MH_ERR_NULL, "%s: %s is required", fn, t.name);
+  if ((uintptr_t)t.p % t.es) return fail(MH_ERR_ALIGN, "%s: %s must be aligned to an element", fn, t.name);
+  int64_t n[3], s[3];
+  int dims = 0;
+  int64_t last = t.width;
+  for (int i = 0; i < 3; ++i) {
+    if (t.n[i] <= 1) continue;
+    int64_t span;
+    if (t.s[i] < 0 || __builtin_mul_overflow(t.n[i] - 1, t.s[i], &span) || __builtin_add_overflow(last, span, &last) ||
+        last > ((int64_t)1 << 56))
+      return fail(MH_ERR_STRIDE, "%s: stride %lld of %s out of range", fn, (long long)t.s[i], t.name);
+    int at = dims++;
+    for (; at > 0 && s[at - 1] > t.s[i]; --at) {
+      n[at] = n[at - 1];
+      s[at] = s[at - 1];
+    }
+    n[at] = t.n[i];
+    s[at] = t.s[i];
+  }
+  if (t.written) {                               // each dimension steps over all that the smaller ones span
+    int64_t span = t.width;
+    for (int i = 0; i < dims; ++i) {
+      if (s[i] < span) return fail(MH_ERR_STRIDE, "%s: %s overlaps itself (stride %lld)", fn, t.name, (long long)s[i]);
+      span += (n[i] - 1) * s[i];
+    }
+  }
+  r = flat_region(t.name, t.p, last * t.es, t.written);
+  return MH_OK;
+}
+
+constexpr int64_t kDeltaPieces = (int64_t)1 << 23;
+
+int delta_sizes(const char* fn, int64_t batch, int64_t heads, int64_t kheads, int64_t seqlen, int64_t dk, int64_t dv, int32_t dtype) {
+  if (batch < 0 || seqlen < 0 || heads <= 0 || kheads <= 0 || dk <= 0 || dv <= 0)
+    return fail(MH_ERR_SHAPE, "%s: sizes must be positive (batch=%lld heads=%lld kheads=%lld seqlen=%lld dk=%lld dv=%lld)", fn,
+                (long long)batch, (long long)heads, (long long)kheads, (long long)seqlen, (long long)dk, (long long)dv);
+  if (heads % kheads) return fail(MH_ERR_SHAPE, "%s: heads (%lld) must be a multiple of key heads (%lld)", fn, (long long)heads, (long long)kheads);
+  if (!elem_size(dtype)) return fail(MH_ERR_DTYPE, "%s: unknown dtype %d", fn, dtype);
+  if (dk > 128 || dv > 256) return fail(MH_ERR_UNSUPPORTED, "%s: head sizes dk=%lld dv=%lld above 128, 256", fn, (long long)dk, (long long)dv);
+  if (batch > kDeltaPieces || heads > kDeltaPieces || seqlen > kMaxDim ||
+      batch * heads > kDeltaPieces / ((seqlen + 63) / 64 > 0 ? (seqlen + 63) / 64 : 1))
+    return fail(MH_ERR_SHAPE, "%s: more than 2^23 pieces of 64 tokens (batch=%lld heads=%lld seqlen=%lld)", fn, (long long)batch, (long long)heads, (long long)seqlen);
+  return MH_OK;
+}
+
+// The inputs' checks; their regions go to r (at most 6).
+int delta_inputs(const char* fn, const mh_delta_args* a, Region* r, int& n) {
+  MH_TRY(delta_sizes(fn, a->batch, a->heads, a->kheads, a->seqlen, a->dk, a->dv, a->dtype));
+  const int es = elem_size(a->dtype);
+  n = 0;
+  if (a->batch == 0) return MH_OK;
+  if (a->seqlen > 0) {
+    MH_TRY(strided_ok(fn, {"q", a->q, {a->batch, a->kheads, a->seqlen}, {a->q_stride_b, a->q_stride_h, a->q_stride_l}, a->dk, es, false}, r[n++]));
+    MH_TRY(strided_ok(fn, {"k", a->k, {a->batch, a->kheads, a->seqlen}, {a->k_stride_b, a->k_stride_h, a->k_stride_l}, a->dk, es, false}, r[n++]));
+    MH_TRY(strided_ok(fn, {"v", a->v, {a->batch, a->heads, a->seqlen}, {a->v_stride_b, a->v_stride_h, a->v_stride_l}, a->dv, es, false}, r[n++]));
+    if (a->g)
+      MH_TRY(strided_ok(fn, {"g", a->g, {a->batch, a->heads, a->seqlen}, {a->g_stride_b, a->g_stride_h, a->g_stride_l}, 1, 4, false}, r[n++]));
+    if (a->beta)
+      MH_TRY(strided_ok(fn, {"beta", a->beta, {a->batch, a->heads, a->seqlen}, {a->beta_stride_b, a->beta_stride_h, a->beta_stride_l}, 1, 4, false}, r[n++]));
+  }
+  MH_TRY(vec_ok(fn, "initial_state", a->initial_state, 4, false));
+  r[n++] = flat_region("initial_state", a->initial_state, a->batch * a->heads * a->dk * a->dv * 4, false);
+  return MH_OK;
+}
+
+void delta_fill(const mh_delta_args* a, mh::DeltaParams& p) {
+  memset(&p, 0, sizeof(p));
+  p.batch = (int)a->batch; p.heads = (int)a->heads; p.kheads = (int)a->kheads; p.seqlen = (int)a->seqlen;
+  p.dk = (int)a->dk; p.dv = (int)a->dv; p.dtype = a->dtype; p.pieces = (p.seqlen + 63) / 64; p.scale = a->scale;
+  p.q = a->q; p.qs = {a->q_stride_b, a->q_stride_h, a->q_stride_l};
+  p.k = a->k; p.ks = {a->k_stride_b, a->k_stride_h, a->k_stride_l};
+  p.v = a->v; p.vs = {a->v_stride_b, a->v_stride_h, a->v_stride_l};
+  p.g = a->g; p.gs = {a->g_stride_b, a->g_stride_h, a->g_stride_l};
+  p.beta = a->beta; p.bs = {a->beta_stride_b, a->beta_stride_h, a->beta_stride_l};
+  p.initial_state = a->initial_state; p.final_state = a->final_state;
+  p.o = a->o; p.os = {a->o_stride_b, a->o_stride_h, a->o_stride_l};
+}
+
+int group_norm_fill(const char* fn, const mh_group_norm_args* a, mh::GroupNormParams& p) {
+  if (!a) return fail(MH_ERR_NULL, "%s: args is NULL", fn);
+  if (a->batch < 0 || a->space < 0 || a->channels <= 0 || a->groups <= 0)
+    return fail(MH_ERR_SHAPE, "%s: sizes must be positive (batch=%lld space=%lld channels=%lld groups=%lld)", fn,
+                (long long)a->batch, (long long)a->space, (long long)a->channels, (long long)a->groups);
+  if (a->channels % a->groups) return fail(MH_ERR_SHAPE, "%s: channels (%lld) must be a multiple of groups (%lld)", fn, (long long)a->channels, (long long)a->groups);
+  if (a->channels > 65536) return fail(MH_ERR_UNSUPPORTED, "%s: channels %lld above 65536", fn, (long long)a->channels);
+  int64_t rows;
+  if (__builtin_mul_overflow(a->batch, a->space, &rows) || rows > ((int64_t)1 << 40) || a->batch > kMaxDim || a->space > kMaxDim)
+    return fail(MH_ERR_SHAPE, "%s: sizes out of range", fn);
+  if (!elem_size(a->dtype)) return fail(MH_ERR_DTYPE, "%s: unknown dtype %d", fn, a->dtype);
+  if (!(a->eps >= 0.f)) return fail(MH_ERR_SHAPE, "%s: eps must not be negative", fn);
+  MH_TRY(norm_par_ok(fn, a->weight, a->bias, "weight", "bias", a->weight_dtype));
+  memset(&p, 0, sizeof(p));
+  p.batch = a->batch; p.space = a->space; p.channels = (int)a->channels; p.groups = (int)a->groups;
+  p.dtype = a->dtype; p.w_f32 = a->weight_dtype == MH_F32; p.silu = a->silu != 0; p.eps = a->eps;
+  p.x = a->x; p.x_sb = a->x_stride_b; p.x_ss = a->x_stride_s;
+  p.weight = a->weight; p.bias = a->bias; p.y = a->y; p.y_sb = a->y_stride_b; p.y_ss = a->y_stride_s; p.stats = a->stats;
+  return MH_OK;
+}
+int group_norm_bwd_fill(const char* fn, const mh_group_norm_bwd_args* a, mh::GroupNormBwdParams& q) {
+  if (!a) return fail(MH_ERR_NULL, "%s: args is NULL", fn);
+  memset(&q, 0, sizeof(q));
+  MH_TRY(group_norm_fill(fn, &a->fwd, q.f));
+  MH_TRY(norm_par_ok(fn, a->dweight, a->dbias, "dweight", "dbias", a->fwd.weight_dtype));
+  q.dy = a->dy; q.dy_sb = a->dy_stride_b; q.dy_ss = a->dy_stride_s;
+  q.dx = a->dx; q.dx_sb = a->dx_stride_b; q.dx_ss = a->dx_stride_s;
+  q.dweight = a->dweight; q.dbias = a->dbias;
+  q.part = reinterpret_cast<float*>(a->workspace);
+  return MH_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1725,6 +1846,244 @@ int mh_token_logprobs_bwd(const mh_logprob_bwd_args* a, void* stream) {
   p.logits = a->logits; p.l_s = a->logits_stride; p.targets = a->targets; p.stats = a->stats;
   p.d_logprobs = a->d_logprobs; p.d_entropy = a->d_entropy; p.dlogits = a->dlogits; p.d_s = a->dlogits_stride;
   return hip_status(mh::launch_logprob_bwd(p, reinterpret_cast<hipStream_t>(stream)), "token_logprobs_bwd");
+}
+
+int mh_delta_rule_workspace_bytes(const mh_delta_args* a, size_t* bytes) {
+  if (!bytes) return fail(MH_ERR_NULL, "delta_rule: bytes output is NULL");
+  if (!a) return fail(MH_ERR_NULL, "delta_rule: args is NULL");
+  MH_TRY(delta_sizes("delta_rule", a->batch, a->heads, a->kheads, a->seqlen, a->dk, a->dv, a->dtype));
+  mh::DeltaParams p;
+  delta_fill(a, p);
+  *bytes = a->batch && a->seqlen ? mh::delta_workspace_bytes(p) : 0;
+  return MH_OK;
+}
+
+int mh_delta_rule_fwd(const mh_delta_args* a, void* stream) {
+  const char* fn = "delta_rule";
+  if (!a) return fail(MH_ERR_NULL, "delta_rule: args is NULL");
+  Region r[9];
+  int n;
+  MH_TRY(delta_inputs(fn, a, r, n));
+  if (a->batch == 0) return MH_OK;
+  mh::DeltaParams p;
+  delta_fill(a, p);
+  const size_t need = a->seqlen ? mh::delta_workspace_bytes(p) : 0;
+  MH_TRY(workspace_ok(fn, a->workspace, a->workspace_bytes, need));
+  MH_TRY(vec_ok(fn, "final_state", a->final_state, 4, false));
+  r[n++] = flat_region("final_state", a->final_state, a->batch * a->heads * a->dk * a->dv * 4, true);
+  r[n++] = flat_region("workspace", need ? a->workspace : nullptr, (int64_t)need, true);
+  if (a->seqlen > 0)
+    MH_TRY(strided_ok(fn, {"o", a->o, {a->batch, a->heads, a->seqlen}, {a->o_stride_b, a->o_stride_h, a->o_stride_l}, a->dv, elem_size(a->dtype), true}, r[n++]));
+  MH_TRY(regions_ok(fn, r, n));
+  p.workspace = reinterpret_cast<char*>(a->workspace);
+  return hip_status(mh::launch_delta(p, reinterpret_cast<hipStream_t>(stream)), fn);
+}
+
+int mh_delta_rule_bwd_workspace_bytes(const mh_delta_bwd_args* a, size_t* bytes) {
+  if (!bytes) return fail(MH_ERR_NULL, "delta_rule_bwd: bytes output is NULL");
+  if (!a) return fail(MH_ERR_NULL, "delta_rule_bwd: args is NULL");
+  const mh_delta_args* f = &a->fwd;
+  MH_TRY(delta_sizes("delta_rule_bwd", f->batch, f->heads, f->kheads, f->seqlen, f->dk, f->dv, f->dtype));
+  mh::DeltaParams p;
+  delta_fill(f, p);
+  *bytes = f->batch && f->seqlen ? mh::delta_bwd_workspace_bytes(p) : 0;
+  return MH_OK;
+}
+
+int mh_delta_rule_bwd(const mh_delta_bwd_args* a, void* stream) {
+  const char* fn = "delta_rule_bwd";
+  if (!a) return fail(MH_ERR_NULL, "delta_rule_bwd: args is NULL");
+  const mh_delta_args* f = &a->fwd;
+  Region r[16];
+  int n;
+  MH_TRY(delta_inputs(fn, f, r, n));
+  if (f->batch == 0) return MH_OK;
+  mh::DeltaBwdParams q;
+  memset(&q, 0, sizeof(q));
+  delta_fill(f, q.f);
+  q.f.o = nullptr;
+  q.f.final_state = nullptr;
+  const size_t need = f->seqlen ? mh::delta_bwd_workspace_bytes(q.f) : 0;
+  MH_TRY(workspace_ok(fn, a->workspace, a->workspace_bytes, need));
+  const int es = elem_size(f->dtype);
+  const int64_t states = f->batch * f->heads * f->dk * f->dv * 4, gates = f->batch * f->heads * f->seqlen * 4;
+  MH_TRY(vec_ok(fn, "d_final_state", a->d_final_state, 4, false));
+  MH_TRY(vec_ok(fn, "d_initial_state", a->d_initial_state, 4, false));
+  MH_TRY(vec_ok(fn, "dg", a->dg, 4, false));
+  MH_TRY(vec_ok(fn, "dbeta", a->dbeta, 4, false));
+  r[n++] = flat_region("d_final_state", a->d_final_state, states, false);
+  r[n++] = flat_region("d_initial_state", a->d_initial_state, states, true);
+  r[n++] = flat_region("workspace", need ? a->workspace : nullptr, (int64_t)need, true);
+  if (f->seqlen > 0) {
+    r[n++] = flat_region("dg", a->dg, gates, true);
+    r[n++] = flat_region("dbeta", a->dbeta, gates, true);
+    MH_TRY(strided_ok(fn, {"d_o", a->d_o, {f->batch, f->heads, f->seqlen}, {a->d_o_stride_b, a->d_o_stride_h, a->d_o_stride_l}, f->dv, es, false}, r[n++]));
+    MH_TRY(strided_ok(fn, {"dq", a->dq, {f->batch, f->kheads, f->seqlen}, {a->dq_stride_b, a->dq_stride_h, a->dq_stride_l}, f->dk, es, true}, r[n++]));
+    MH_TRY(strided_ok(fn, {"dk", a->dk, {f->batch, f->kheads, f->seqlen}, {a->dk_stride_b, a->dk_stride_h, a->dk_stride_l}, f->dk, es, true}, r[n++]));
+    MH_TRY(strided_ok(fn, {"dv", a->dv, {f->batch, f->heads, f->seqlen}, {a->dv_stride_b, a->dv_stride_h, a->dv_stride_l}, f->dv, es, true}, r[n++]));
+  }
+  MH_TRY(regions_ok(fn, r, n));
+  q.d_o = a->d_o; q.dos = {a->d_o_stride_b, a->d_o_stride_h, a->d_o_stride_l};
+  q.d_final_state = a->d_final_state;
+  q.dq = a->dq; q.dqs = {a->dq_stride_b, a->dq_stride_h, a->dq_stride_l};
+  q.dk = a->dk; q.dks = {a->dk_stride_b, a->dk_stride_h, a->dk_stride_l};
+  q.dv = a->dv; q.dvs = {a->dv_stride_b, a->dv_stride_h, a->dv_stride_l};
+  q.dg = a->dg; q.dbeta = a->dbeta; q.d_initial_state = a->d_initial_state;
+  q.f.workspace = reinterpret_cast<char*>(a->workspace);
+  return hip_status(mh::launch_delta_bwd(q, reinterpret_cast<hipStream_t>(stream)), fn);
+}
+
+int mh_delta_step(const mh_delta_step_args* a, void* stream) {
+  const char* fn = "delta_step";
+  if (!a) return fail(MH_ERR_NULL, "delta_step: args is NULL");
+  MH_TRY(delta_sizes(fn, a->batch, a->heads, a->kheads, 1, a->dk, a->dv, a->dtype));
+  if (a->batch == 0) return MH_OK;
+  const int es = elem_size(a->dtype);
+  Region r[8];
+  int n = 0;
+  MH_TRY(strided_ok(fn, {"q", a->q, {a->batch, a->kheads, 1}, {a->q_stride_b, a->q_stride_h, 0}, a->dk, es, false}, r[n++]));
+  MH_TRY(strided_ok(fn, {"k", a->k, {a->batch, a->kheads, 1}, {a->k_stride_b, a->k_stride_h, 0}, a->dk, es, false}, r[n++]));
+  MH_TRY(strided_ok(fn, {"v", a->v, {a->batch, a->heads, 1}, {a->v_stride_b, a->v_stride_h, 0}, a->dv, es, false}, r[n++]));
+  if (a->g) MH_TRY(strided_ok(fn, {"g", a->g, {a->batch, a->heads, 1}, {a->g_stride_b, a->g_stride_h, 0}, 1, 4, false}, r[n++]));
+  if (a->beta) MH_TRY(strided_ok(fn, {"beta", a->beta, {a->batch, a->heads, 1}, {a->beta_stride_b, a->beta_stride_h, 0}, 1, 4, false}, r[n++]));
+  MH_TRY(strided_ok(fn, {"o", a->o, {a->batch, a->heads, 1}, {a->o_stride_b, a->o_stride_h, 0}, a->dv, es, true}, r[n++]));
+  MH_TRY(vec_ok(fn, "state_in", a->state_in, 4, true));
+  MH_TRY(vec_ok(fn, "state_out", a->state_out, 4, true));
+  // a thread writes the elements that it read: the state may be updated in place
+  const int64_t states = a->batch * a->heads, row = a->dk * a->dv;
+  r[n++] = row_region("state_in", a->state_in, states, row, row, 4, false);
+  r[n++] = row_region("state_out", a->state_out, states, row, row, 4, true);
+  MH_TRY(regions_ok(fn, r, n));
+  mh::DeltaStepParams p;
+  memset(&p, 0, sizeof(p));
+  p.batch = (int)a->batch; p.heads = (int)a->heads; p.kheads = (int)a->kheads; p.dk = (int)a->dk; p.dv = (int)a->dv;
+  p.dtype = a->dtype; p.scale = a->scale;
+  p.q = a->q; p.q_sb = a->q_stride_b; p.q_sh = a->q_stride_h;
+  p.k = a->k; p.k_sb = a->k_stride_b; p.k_sh = a->k_stride_h;
+  p.v = a->v; p.v_sb = a->v_stride_b; p.v_sh = a->v_stride_h;
+  p.g = a->g; p.g_sb = a->g_stride_b; p.g_sh = a->g_stride_h;
+  p.beta = a->beta; p.b_sb = a->beta_stride_b; p.b_sh = a->beta_stride_h;
+  p.state_in = a->state_in; p.state_out = a->state_out;
+  p.o = a->o; p.o_sb = a->o_stride_b; p.o_sh = a->o_stride_h;
+  return hip_status(mh::launch_delta_step(p, reinterpret_cast<hipStream_t>(stream)), fn);
+}
+
+int mh_rotary(const mh_rotary_args* a, void* stream) {
+  const char* fn = "rotary";
+  if (!a) return fail(MH_ERR_NULL, "rotary: args is NULL");
+  if (a->batch < 0 || a->seqlen < 0 || a->q_heads <= 0 || a->k_heads < 0 || a->dim <= 0 || a->pairs <= 0)
+    return fail(MH_ERR_SHAPE, "rotary: sizes must be positive (batch=%lld heads=%lld,%lld seqlen=%lld dim=%lld pairs=%lld)",
+                (long long)a->batch, (long long)a->q_heads, (long long)a->k_heads, (long long)a->seqlen, (long long)a->dim, (long long)a->pairs);
+  if (a->dim > 65536 || a->q_heads > 65536 || a->k_heads > 65536 || a->batch > kMaxDim || a->seqlen > kMaxDim ||
+      a->batch * a->seqlen > ((int64_t)1 << 33) / ((a->dim + 7) / 8 + 1))
+    return fail(MH_ERR_SHAPE, "rotary: sizes out of range");
+  if (2 * a->pairs > a->dim) return fail(MH_ERR_SHAPE, "rotary: %lld pairs in %lld channels", (long long)a->pairs, (long long)a->dim);
+  if (!elem_size(a->dtype)) return fail(MH_ERR_DTYPE, "rotary: unknown dtype %d", a->dtype);
+  if (a->batch == 0 || a->seqlen == 0) return MH_OK;
+  const int es = elem_size(a->dtype);
+  MH_TRY(vec_ok(fn, "inv_freq", a->inv_freq, a->freq_f64 ? 8 : 4, true));
+  Region r[6];
+  int n = 0;
+  r[n++] = flat_region("inv_freq", a->inv_freq, a->pairs * (a->freq_f64 ? 8 : 4), false);
+  if (a->positions) {
+    MH_TRY(index_ok(fn, a->index_bytes, a->positions, "positions"));
+    Region& pos = r[n++];
+    MH_TRY(strided_ok(fn, {"positions", a->positions, {a->batch, 1, 1}, {a->positions_stride_b, 0, 0}, a->seqlen, a->index_bytes, false}, pos));
+  }
+  const int64_t qn[3] = {a->batch, a->q_heads, a->seqlen}, kn[3] = {a->batch, a->k_heads, a->seqlen};
+  const int64_t qi[3] = {a->q_stride_b, a->q_stride_h, a->q_stride_l}, qo[3] = {a->q_out_stride_b, a->q_out_stride_h, a->q_out_stride_l};
+  const int64_t ki[3] = {a->k_stride_b, a->k_stride_h, a->k_stride_l}, ko[3] = {a->k_out_stride_b, a->k_out_stride_h, a->k_out_stride_l};
+  auto tensor = [&](const char* name, const void* p, const int64_t* sz, const int64_t* st, bool written) -> int {
+    return strided_ok(fn, {name, p, {sz[0], sz[1], sz[2]}, {st[0], st[1], st[2]}, a->dim, es, written}, r[n++]);
+  };
+  // a thread writes the channels that it read: an output may be its input with the same strides
+  auto same = [&](const void* x, const void* y, const int64_t* sz, const int64_t* sx, const int64_t* sy) {
+    for (int i = 0; i < 3; ++i)
+      if (sz[i] > 1 && sx[i] != sy[i]) return false;
+    return x == y;
+  };
+  if (same(a->q, a->q_out, qn, qi, qo)) {
+    MH_TRY(tensor("q_out", a->q_out, qn, qo, true));
+  } else {
+    MH_TRY(tensor("q", a->q, qn, qi, false));
+    MH_TRY(tensor("q_out", a->q_out, qn, qo, true));
+  }
+  if (a->k_heads > 0) {
+    if (!same(a->k, a->k_out, kn, ki, ko)) MH_TRY(tensor("k", a->k, kn, ki, false));
+    MH_TRY(tensor("k_out", a->k_out, kn, ko, true));
+  }
+  MH_TRY(regions_ok(fn, r, n));
+  mh::RotaryParams p;
+  memset(&p, 0, sizeof(p));
+  p.batch = (int)a->batch; p.q_heads = (int)a->q_heads; p.k_heads = (int)a->k_heads; p.seqlen = (int)a->seqlen;
+  p.dim = (int)a->dim; p.pairs = (int)a->pairs; p.dtype = a->dtype; p.interleaved = a->interleaved != 0;
+  p.inverse = a->inverse != 0; p.scale = a->scale; p.inv_freq = a->inv_freq; p.freq64 = a->freq_f64 != 0;
+  p.positions = a->positions; p.i64 = a->index_bytes == 8; p.pos_sb = a->positions_stride_b; p.offset = a->offset;
+  p.q = {a->q, {qi[0], qi[1], qi[2]}, a->q_out, {qo[0], qo[1], qo[2]}};
+  p.k = {a->k, {ki[0], ki[1], ki[2]}, a->k_out, {ko[0], ko[1], ko[2]}};
+  return hip_status(mh::launch_rotary(p, reinterpret_cast<hipStream_t>(stream)), fn);
+}
+
+int mh_group_norm_workspace_bytes(const mh_group_norm_args* a, size_t* bytes) {
+  if (!bytes) return fail(MH_ERR_NULL, "group_norm: bytes output is NULL");
+  mh::GroupNormParams p;
+  MH_TRY(group_norm_fill("group_norm", a, p));
+  *bytes = mh::group_norm_workspace_bytes(p);
+  return MH_OK;
+}
+
+int mh_group_norm_fwd(const mh_group_norm_args* a, void* stream) {
+  const char* fn = "group_norm";
+  mh::GroupNormParams p;
+  MH_TRY(group_norm_fill(fn, a, p));
+  if (a->batch == 0 || a->space == 0) return MH_OK;
+  const int es = elem_size(a->dtype), ws = elem_size(a->weight_dtype);
+  const size_t need = mh::group_norm_workspace_bytes(p);
+  MH_TRY(workspace_ok(fn, a->workspace, a->workspace_bytes, need));
+  MH_TRY(vec_ok(fn, "stats", a->stats, 4, false));
+  Region r[6];
+  MH_TRY(strided_ok(fn, {"x", a->x, {a->batch, a->space, 1}, {a->x_stride_b, a->x_stride_s, 0}, a->channels, es, false}, r[0]));
+  MH_TRY(strided_ok(fn, {"y", a->y, {a->batch, a->space, 1}, {a->y_stride_b, a->y_stride_s, 0}, a->channels, es, true}, r[1]));
+  r[2] = flat_region("weight", a->weight, a->channels * ws, false);
+  r[3] = flat_region("bias", a->bias, a->channels * ws, false);
+  r[4] = flat_region("stats", a->stats, a->batch * a->groups * 8, true);
+  r[5] = flat_region("workspace", need ? a->workspace : nullptr, (int64_t)need, true);
+  MH_TRY(regions_ok(fn, r, 6));
+  p.part = reinterpret_cast<double*>(a->workspace);
+  return hip_status(mh::launch_group_norm(p, reinterpret_cast<hipStream_t>(stream)), fn);
+}
+
+int mh_group_norm_bwd_workspace_bytes(const mh_group_norm_bwd_args* a, size_t* bytes) {
+  if (!bytes) return fail(MH_ERR_NULL, "group_norm_bwd: bytes output is NULL");
+  mh::GroupNormBwdParams q;
+  MH_TRY(group_norm_bwd_fill("group_norm_bwd", a, q));
+  *bytes = mh::group_norm_bwd_workspace_bytes(q.f);
+  return MH_OK;
+}
+
+int mh_group_norm_bwd(const mh_group_norm_bwd_args* a, void* stream) {
+  const char* fn = "group_norm_bwd";
+  mh::GroupNormBwdParams q;
+  MH_TRY(group_norm_bwd_fill(fn, a, q));
+  const mh_group_norm_args* f = &a->fwd;
+  const int es = elem_size(f->dtype), ws = elem_size(f->weight_dtype);
+  if (f->batch > 0 && f->space > 0) {
+    const size_t need = mh::group_norm_bwd_workspace_bytes(q.f);
+    MH_TRY(workspace_ok(fn, a->workspace, a->workspace_bytes, need));
+    MH_TRY(vec_ok(fn, "stats", f->stats, 4, true));
+    Region r[9];
+    MH_TRY(strided_ok(fn, {"x", f->x, {f->batch, f->space, 1}, {f->x_stride_b, f->x_stride_s, 0}, f->channels, es, false}, r[0]));
+    MH_TRY(strided_ok(fn, {"dy", a->dy, {f->batch, f->space, 1}, {a->dy_stride_b, a->dy_stride_s, 0}, f->channels, es, false}, r[1]));
+    MH_TRY(strided_ok(fn, {"dx", a->dx, {f->batch, f->space, 1}, {a->dx_stride_b, a->dx_stride_s, 0}, f->channels, es, true}, r[2]));
+    r[3] = flat_region("weight", f->weight, f->channels * ws, false);
+    r[4] = flat_region("bias", f->bias, f->channels * ws, false);
+    r[5] = flat_region("stats", f->stats, f->batch * f->groups * 8, false);
+    r[6] = flat_region("dweight", a->dweight, f->channels * ws, true);
+    r[7] = flat_region("dbias", a->dbias, f->channels * ws, true);
+    r[8] = flat_region("workspace", need ? a->workspace : nullptr, (int64_t)need, true);
+    MH_TRY(regions_ok(fn, r, 9));
+  }
+  return hip_status(mh::launch_group_norm_bwd(q, reinterpret_cast<hipStream_t>(stream)), fn);
 }
 
 }  // extern "C"

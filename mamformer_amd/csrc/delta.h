@@ -1,0 +1,161 @@
+// Pieces shared by the gated delta rule's kernels (gfx950): fp16 operands in two parts, their LDS tiles and fragments,
+// and the workspace's layout.
+//
+// Arithmetic.  The state, its gradient and the gates' gradients leave in fp32, and products of operands rounded once to
+// bf16 or fp16 are too coarse for them (2^-9, 2^-12), while the fp32 matrix instructions run at 1/16 of the 16-bit rate.
+// A matrix x is therefore held as (hi + lo) s: a power of two s that brings its largest magnitude into [2^12, 2^13), hi
+// the fp16 nearest x / s and lo the fp16 nearest what is left.  That is x to 2^-22 of itself down to 2^-16 of the largest
+// value, and to 2^-38 of the largest value below it.  A product is hi hi + hi lo + lo hi in fp32 accumulators (lo lo
+// would add 2^-22); a bf16 matrix is exact in hi alone within 2^-18 of its largest value, which saves a product.
+// The power of two is what fp16's range costs: bf16 parts would need none but take three of them, six products, for the
+// same result.
+//
+// Fragments are those of the 16x16x32 fp16 instruction: lane l holds row (A) or column (B) l % 16 and, with g = l / 16,
+// the k-values KS(g, j) = 4 g + j (j < 4), 16 + 4 g + j - 4 (j >= 4).  The accumulator of a 16x16 tile holds rows
+// 4 g + r of column l % 16, so that two tiles below each other are a B operand as they stand: a wave keeps 16 columns of
+// the state through all of its products without moving a value to another lane.
+#pragma once
+
+#include "launch.h"
+#include "rows.h"
+#include "tiles.h"
+
+namespace mh {
+
+typedef _Float16 f16;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
+
+constexpr int DC = 64;                           // tokens of a piece
+
+__device__ __forceinline__ f32x4 mma_h(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// DC rows of W fp16 (64 or 128), 16-byte chunks XOR-swizzled by row so that both accesses below meet every LDS bank once:
+// 16 rows of 16 bytes (row_frag16's half wave) and 8 rows of 32 bytes (col_frag16's).
+template <int W>
+struct HTile {
+  static constexpr int ELEMS = DC * W;
+  __host__ __device__ static constexpr int swz(int r) {
+    return W == 128 ? ((r & 7) << 1) | ((r >> 3) & 1) : (((r >> 1) & 3) << 1) | ((r >> 3) & 1);
+  }
+  __host__ __device__ static constexpr int at(int r, int c) { return r * W + (((c >> 3) ^ swz(r)) << 3) + (c & 7); }
+};
+
+// Operand with k along the rows' columns: row r0 + l % 16, k0 + KS(g, j).
+template <int W>
+__device__ __forceinline__ f16x8 row_frag16(const f16* t, int r0, int k0, int lane) {
+  const int r = r0 + (lane & 15), k = k0 + 4 * (lane >> 4);
+  const f16x4 a = *reinterpret_cast<const f16x4*>(t + HTile<W>::at(r, k));
+  const f16x4 b = *reinterpret_cast<const f16x4*>(t + HTile<W>::at(r, k + 16));
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// Operand with k down the rows: rows k0 + KS(g, j) of column c0 + l % 16, by two transposing reads (each 16 lanes name 4
+// elements of each of 4 rows, lane i receives the i-th of the 16 columns).
+template <int W>
+__device__ __forceinline__ f16x8 col_frag16(const f16* t, int c0, int k0, int lane) {
+  const int i = lane & 15, r = k0 + 4 * (lane >> 4) + (i >> 2), c = c0 + 4 * (i & 3);
+  const i16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(t + HTile<W>::at(r, c)));
+  const i16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(t + HTile<W>::at(r + 16, c)));
+  return __builtin_bit_cast(f16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// The largest of a value over the wave, in every lane.
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, dppf<0xB1>(v));
+  v = fmaxf(v, dppf<0x4E>(v));
+  v = fmaxf(v, dppf<0x141>(v));
+  v = fmaxf(v, dppf<0x140>(v));
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// The power of two s (`inv`) with amax / s in [2^12, 2^13), and 1 / s (`mult`).  A maximum below 2^-114 is taken as that;
+// an infinity stays one in every part, so that it reaches the results.
+struct Scale {
+  float mult, inv;
+  __device__ __forceinline__ explicit Scale(float amax) {
+    const int e = max((int)(__float_as_uint(amax) >> 23) & 0xff, 13);
+    mult = __uint_as_float((uint32_t)(266 - e) << 23);
+    inv = __uint_as_float((uint32_t)(e - 12) << 23);
+  }
+};
+__device__ __forceinline__ f16 part_hi(float x, float mult) { return (f16)(x * mult); }
+__device__ __forceinline__ f16 part_lo(float x, float mult, f16 hi) { return (f16)__builtin_fmaf(x, mult, -(float)hi); }
+
+// B operand of k-step c from accumulator tiles 2 c and 2 c + 1 (rows 32 c .. 32 c + 31).
+template <int PLANES, int N>
+__device__ __forceinline__ void parts_of(const f32x4 (&t)[N], float mult, f16x8 (&hi)[N / 2], f16x8 (&lo)[N / 2]) {
+#pragma unroll
+  for (int c = 0; c < N / 2; ++c)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float x = t[2 * c + (j >> 2)][j & 3];
+      hi[c][j] = part_hi(x, mult);
+      if constexpr (PLANES == 2) lo[c][j] = part_lo(x, mult, hi[c][j]);
+    }
+}
+template <int N>
+__device__ __forceinline__ float abs_max(const f32x4 (&t)[N], float m = 0.f) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) m = fmaxf(m, fabsf(t[i][r]));
+  return m;
+}
+
+// A gate's logarithm as the kernels take it: e^-200 is 0 in fp32 as e^-inf is, and sums of it stay finite.
+__device__ __forceinline__ float gate_log(float g) { return g < -200.f ? -200.f : g; }
+
+// Inclusive sums over the wave's 64 lanes in fp64: differences of sums keep fp32's precision however far the sums went.
+__device__ __forceinline__ double wave_scan64(double v) {
+  const int l = threadIdx.x & 63;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const double o = __shfl_up(v, off, 64);
+    if (l >= off) v += o;
+  }
+  return v;
+}
+
+// ------------------------------------------------------------------ workspace
+// For each (batch, key head, piece): the parts of K, then of Q.  For each (batch, value head, piece): T and P (two parts
+// each) and `vec`: e^{G_t}, beta_t e^{G_end - G_t}, then e^{G_end} and the scales of T, P, K and Q.  For the backward,
+// for each (batch, value head, piece, 16 columns of v): the entering state, its gradient behind the piece, delta and y,
+// two parts each, transposed ([column][row]), and their four scales.
+constexpr int kVecFloats = 256;
+enum { VEC_W = 64, VEC_GAMMA = 128, VEC_ST, VEC_SP, VEC_SK, VEC_SQ };
+enum { KEEP_S, KEEP_DS, KEEP_D, KEEP_Y };        // order of the scales
+template <int DKP> constexpr size_t keep_halfs() { return 2 * (2 * 16 * DKP) + 2 * (2 * 16 * DC); }
+
+struct DeltaLayout {
+  size_t kq, tp, vec, keep, scales, total;       // byte offsets
+  __host__ DeltaLayout(const DeltaParams& p, bool backward) {
+    const size_t np = p.dtype == DT_F32 ? 2 : 1, dkp = p.dk <= 64 ? 64 : 128;
+    const size_t kpieces = (size_t)p.batch * p.kheads * p.pieces, pieces = (size_t)p.batch * p.heads * p.pieces;
+    const size_t blocks = backward ? pieces * ((p.dv + 15) / 16) : 0;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t was = at; at += (bytes + 1023) / 1024 * 1024; return was; };
+    kq = take(kpieces * 2 * np * DC * dkp * 2);
+    tp = take(pieces * 4 * DC * DC * 2);
+    vec = take(pieces * kVecFloats * 4);
+    keep = take(blocks * (dkp == 64 ? keep_halfs<64>() : keep_halfs<128>()) * 2);
+    scales = take(blocks * 16);
+    total = at;
+  }
+};
+
+// Workgroup n of heads x blocks, with the blocks of a head on one XCD (workgroups go to the 8 XCDs in turn): they share the
+// head's tiles through its L2.  False beyond the last head.
+__device__ __forceinline__ bool head_block(int n, int heads, int blocks, int& head, int& block) {
+  const int y = n >> 3;
+  head = (y / blocks) * 8 + (n & 7);
+  block = y % blocks;
+  return head < heads;
+}
+inline unsigned head_block_grid(int heads, int blocks) { return (unsigned)((heads + 7) / 8 * 8 * blocks); }
+
+}  // namespace mh

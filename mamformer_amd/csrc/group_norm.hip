@@ -1,0 +1,533 @@
+// Group norm, channels last: x (batch, space, channels), mean and variance of each (batch, group) over the space and the
+// group's channels, z = (x - mean) / sqrt(var + eps) * weight + bias, y = z or silu(z).  Backward, with dz = dy act'(z),
+// gw = dz weight and xh the normalised x: dx = (gw - mean(gw) - xh mean(gw xh)) / sqrt(var + eps), dweight = sum dz xh,
+// dbias = sum dz.  Bound by the tensors' bytes.
+//
+// Two ways.  One position in the space (a token's heads): the lanes of a group hold its channels, one reading of x, the
+// variance that of the centred values.  Otherwise the sums of a (batch, group) come from many workgroups: a pass for the
+// sums, then a pass that reads x again (from the caches where it fits).  There the sums are fp64: squares of fp32 values
+// are exact in it, so that no mean however far from zero costs the variance its digits, in one reading.
+// Channels are taken 8 at a time within a group, so that a chunk never belongs to two groups.
+#include <type_traits>
+
+#include "launch.h"
+#include "rows.h"
+
+namespace mh {
+namespace {
+
+constexpr int kRowsMax = 512;                    // channels of a group that one wave holds
+
+template <int N> __device__ __forceinline__ float lanes_sum(float v) {
+  if constexpr (N == 1) return v;
+  else if constexpr (N == 2) return v + dppf<0xB1>(v);
+  else if constexpr (N == 4) return sum_quad(v);
+  else return group_sum<N>(v);
+}
+
+// z to y; and the factor of dy in dz
+__device__ __forceinline__ float act(bool silu, float z) { return silu ? silu_f(z) : z; }
+__device__ __forceinline__ float act_slope(bool silu, float z) {
+  if (!silu) return 1.f;
+  const float s = sigmoid_f(z);
+  return s * (1.f + z * (1.f - s));
+}
+
+struct Affine {
+  float w[8], b[8];
+  __device__ __forceinline__ Affine(const GroupNormParams& p, int c, int end) {      // channels c .. of a group ending at `end`
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      w[j] = 1.f;
+      b[j] = 0.f;
+    }
+    if (p.weight) load_par8(p.weight, p.w_f32, c, end, w);
+    if (p.bias) load_par8(p.bias, p.w_f32, c, end, b);
+  }
+};
+
+// ------------------------------------------------------------------ one position
+template <typename T, int TG>
+__global__ __launch_bounds__(256) void group_rows_kernel(GroupNormParams p) {
+  const int cg = p.channels / p.groups, c8 = threadIdx.x % TG * 8, left = cg - c8;
+  const int64_t items = p.batch * p.groups;
+  for (int64_t it = (int64_t)blockIdx.x * (256 / TG) + threadIdx.x / TG; it < items; it += (int64_t)gridDim.x * (256 / TG)) {
+    const int64_t n = it / p.groups;
+    const int g = (int)(it % p.groups), c = g * cg + c8;
+    float x[8] = {};
+    if (left > 0) load8(reinterpret_cast<const T*>(p.x) + n * p.x_sb + c, left, x);
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += x[j];
+    const float mean = lanes_sum<TG>(s) / (float)cg;
+    float q = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] -= mean;
+      q += j < left ? x[j] * x[j] : 0.f;
+    }
+    const float rstd = 1.f / sqrtf(lanes_sum<TG>(q) / (float)cg + p.eps);
+    if (left > 0) {
+      const Affine a(p, c, (g + 1) * cg);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = act(p.silu, x[j] * rstd * a.w[j] + a.b[j]);
+      store8(reinterpret_cast<T*>(p.y) + n * p.y_sb + c, left, x);
+    }
+    if (p.stats && c8 == 0) {
+      p.stats[2 * it] = mean;
+      p.stats[2 * it + 1] = rstd;
+    }
+  }
+}
+
+// A workgroup takes 256 / TG groups (or all, and several batch entries at once) and walks the batch with them, so that a
+// thread adds its channels' gradients in registers; `part` (rows, channels, 2) gets a row for each that walked.
+template <typename T, int TG>
+__global__ __launch_bounds__(256) void group_rows_bwd_kernel(GroupNormBwdParams q, int gb, int side) {
+  const GroupNormParams& p = q.f;
+  const int cg = p.channels / p.groups, c8 = threadIdx.x % TG * 8, left = cg - c8, slot = threadIdx.x / TG;
+  const int g = blockIdx.y * gb + slot % gb, sub = slot / gb;
+  if (sub >= side || g >= p.groups) return;      // no barrier follows; lanes of a group go together
+  const int c = g * cg + c8;
+  const Affine a(p, left > 0 ? c : 0, (g + 1) * cg);
+  float A[8] = {}, B[8] = {};
+  for (int64_t n = (int64_t)blockIdx.x * side + sub; n < p.batch; n += (int64_t)gridDim.x * side) {
+    float x[8] = {}, d[8] = {};
+    if (left > 0) {
+      load8(reinterpret_cast<const T*>(p.x) + n * p.x_sb + c, left, x);
+      load8(reinterpret_cast<const T*>(q.dy) + n * q.dy_sb + c, left, d);
+    }
+    const float mean = p.stats[2 * (n * p.groups + g)], rstd = p.stats[2 * (n * p.groups + g) + 1];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = (x[j] - mean) * rstd;
+      const float dz = j < left ? d[j] * act_slope(p.silu, x[j] * a.w[j] + a.b[j]) : 0.f;
+      A[j] += dz;
+      B[j] += dz * x[j];
+      d[j] = dz * a.w[j];
+      s1 += d[j];
+      s2 += d[j] * x[j];
+    }
+    s1 = lanes_sum<TG>(s1) / (float)cg;
+    s2 = lanes_sum<TG>(s2) / (float)cg;
+    if (left > 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = rstd * (d[j] - s1 - x[j] * s2);
+      store8(reinterpret_cast<T*>(q.dx) + n * q.dx_sb + c, left, x);
+    }
+  }
+  if (q.part && left > 0) {
+    float* to = q.part + (((int64_t)blockIdx.x * side + sub) * p.channels + c) * 2;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < left) {
+        to[2 * j] = A[j];
+        to[2 * j + 1] = B[j];
+      }
+  }
+}
+
+// dbias and dweight: sums over the rows of part (rows, channels, 2), 16 lanes of rows a channel, in a fixed order.
+__global__ __launch_bounds__(256) void group_params_kernel(const float* part, int64_t rows, int channels, void* dweight, void* dbias,
+                                                           int f32) {
+  __shared__ float sa[16][17], sb[16][17];
+  const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
+  float a = 0.f, b = 0.f;
+  if (c < channels)
+    for (int64_t r = rl; r < rows; r += 16) {
+      const f32x2 v = *reinterpret_cast<const f32x2*>(part + (r * channels + c) * 2);
+      a += v[0];
+      b += v[1];
+    }
+  sa[rl][cl] = a;
+  sb[rl][cl] = b;
+  __syncthreads();
+  if (rl == 0 && c < channels) {
+    for (int i = 1; i < 16; ++i) {
+      a += sa[i][cl];
+      b += sb[i][cl];
+    }
+    if (dbias) {
+      if (f32) reinterpret_cast<float*>(dbias)[c] = a;
+      else reinterpret_cast<bf16*>(dbias)[c] = (bf16)a;
+    }
+    if (dweight) {
+      if (f32) reinterpret_cast<float*>(dweight)[c] = b;
+      else reinterpret_cast<bf16*>(dweight)[c] = (bf16)b;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ many positions
+// A workgroup's part of (batch, space, groups): gb groups of cpg chunks, `side` positions at once, `rows` positions.
+struct Split {
+  int cg, cpg, gb, ub, side, cblocks, splits;
+  int64_t rows, units;
+  __host__ explicit Split(const GroupNormParams& p) {
+    cg = p.channels / p.groups;
+    cpg = (cg + 7) / 8;
+    gb = cpg >= 256 ? 1 : 256 / cpg < p.groups ? 256 / cpg : p.groups;
+    ub = gb * cpg;
+    side = ub <= 256 ? 256 / ub : 1;
+    cblocks = (p.groups + gb - 1) / gb;
+    // enough workgroups for the card, each with at least 4 passes over its positions
+    int64_t want = 1024 / (p.batch * cblocks) + 1, most = (p.space + 4 * side - 1) / (4 * side);
+    splits = (int)(want < most ? want : most);
+    rows = (p.space + splits - 1) / splits;
+    splits = (int)((p.space + rows - 1) / rows);
+    units = p.batch * splits * cblocks;
+  }
+  __device__ __forceinline__ void at(int64_t u, int64_t& n, int& s, int& cb) const {
+    cb = (int)(u % cblocks);
+    const int64_t v = u / cblocks;
+    s = (int)(v % splits);
+    n = v / splits;
+  }
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void group_sums_kernel(GroupNormParams p, Split sp) {
+  __shared__ double sa[256], sb[256];
+  const int tid = threadIdx.x, u0 = sp.ub <= 256 ? tid % sp.ub : tid, sub = sp.ub <= 256 ? tid / sp.ub : 0;
+  for (int64_t unit = blockIdx.x; unit < sp.units; unit += gridDim.x) {
+    int64_t n;
+    int s, cb;
+    sp.at(unit, n, s, cb);
+    const int64_t r0 = s * sp.rows, r1 = min(p.space, r0 + sp.rows);
+    double a = 0., b = 0.;
+    for (int u = u0; u < sp.ub && sub < sp.side; u += 256) {
+      const int g = cb * sp.gb + u / sp.cpg, c8 = u % sp.cpg * 8;
+      if (g >= p.groups) break;
+      const T* src = reinterpret_cast<const T*>(p.x) + n * p.x_sb + g * sp.cg + c8;
+      for (int64_t r = r0 + sub; r < r1; r += sp.side) {
+        float x[8];
+        load8(src + r * p.x_ss, sp.cg - c8, x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          a += (double)x[j];
+          b += (double)x[j] * (double)x[j];
+        }
+      }
+    }
+    __syncthreads();
+    sa[tid] = a;
+    sb[tid] = b;
+    __syncthreads();
+    if (tid < sp.gb && cb * sp.gb + tid < p.groups) {
+      const int per = sp.cpg < 256 ? sp.cpg : 256;
+      a = b = 0.;
+      for (int i = 0; i < sp.side; ++i)
+        for (int j = 0; j < per; ++j) {
+          a += sa[i * sp.ub + tid * sp.cpg + j];
+          b += sb[i * sp.ub + tid * sp.cpg + j];
+        }
+      double* to = p.part + ((n * sp.splits + s) * p.groups + cb * sp.gb + tid) * 2;
+      to[0] = a;
+      to[1] = b;
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void group_apply_kernel(GroupNormParams p, Split sp) {
+  __shared__ float sm[256], sr[256];
+  const int tid = threadIdx.x, u0 = sp.ub <= 256 ? tid % sp.ub : tid, sub = sp.ub <= 256 ? tid / sp.ub : 0;
+  for (int64_t unit = blockIdx.x; unit < sp.units; unit += gridDim.x) {
+    int64_t n;
+    int s, cb;
+    sp.at(unit, n, s, cb);
+    __syncthreads();
+    if (tid < sp.gb && cb * sp.gb + tid < p.groups) {
+      const int g = cb * sp.gb + tid;
+      double a = 0., b = 0.;
+#pragma unroll 8
+      for (int i = 0; i < sp.splits; ++i) {
+        const double* from = p.part + ((n * sp.splits + i) * p.groups + g) * 2;
+        a += from[0];
+        b += from[1];
+      }
+      const double count = (double)p.space * sp.cg, mean = a / count, var = b / count - mean * mean;
+      sm[tid] = (float)mean;
+      sr[tid] = 1.f / sqrtf((float)(var > 0. ? var : var == var ? 0. : var) + p.eps);
+      if (p.stats && s == 0) {
+        p.stats[2 * (n * p.groups + g)] = sm[tid];
+        p.stats[2 * (n * p.groups + g) + 1] = sr[tid];
+      }
+    }
+    __syncthreads();
+    const int64_t r0 = s * sp.rows, r1 = min(p.space, r0 + sp.rows);
+    for (int u = u0; u < sp.ub && sub < sp.side; u += 256) {
+      const int g = cb * sp.gb + u / sp.cpg, c8 = u % sp.cpg * 8, left = sp.cg - c8;
+      if (g >= p.groups) break;
+      const int c = g * sp.cg + c8;
+      const Affine a(p, c, (g + 1) * sp.cg);
+      const float mean = sm[u / sp.cpg], rstd = sr[u / sp.cpg];
+      const T* src = reinterpret_cast<const T*>(p.x) + n * p.x_sb + c;
+      T* dst = reinterpret_cast<T*>(p.y) + n * p.y_sb + c;
+      for (int64_t r = r0 + sub; r < r1; r += sp.side) {
+        float x[8];
+        load8(src + r * p.x_ss, left, x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = act(p.silu, (x[j] - mean) * rstd * a.w[j] + a.b[j]);
+        store8(dst + r * p.y_ss, left, x);
+      }
+    }
+  }
+}
+
+// Sums of dz and dz xh for every channel of a workgroup's positions: part (batch, splits, channels, 2).
+template <typename T>
+__global__ __launch_bounds__(256) void group_bwd_sums_kernel(GroupNormBwdParams q, Split sp) {
+  __shared__ float sa[256][17];
+  const GroupNormParams& p = q.f;
+  const int tid = threadIdx.x, u0 = sp.ub <= 256 ? tid % sp.ub : tid, sub = sp.ub <= 256 ? tid / sp.ub : 0;
+  for (int64_t unit = blockIdx.x; unit < sp.units; unit += gridDim.x) {
+    int64_t n;
+    int s, cb;
+    sp.at(unit, n, s, cb);
+    const int64_t r0 = s * sp.rows, r1 = min(p.space, r0 + sp.rows);
+    for (int base = 0; base < sp.ub; base += 256) {
+      const int u = base + u0, g = cb * sp.gb + u / sp.cpg, c8 = u % sp.cpg * 8, left = sp.cg - c8;
+      const bool on = u < sp.ub && sub < sp.side && g < p.groups;
+      const int c = g * sp.cg + c8;
+      float A[8] = {}, B[8] = {};
+      if (on) {
+        const Affine a(p, c, (g + 1) * sp.cg);
+        const float mean = p.stats[2 * (n * p.groups + g)], rstd = p.stats[2 * (n * p.groups + g) + 1];
+        const T* xs = reinterpret_cast<const T*>(p.x) + n * p.x_sb + c;
+        const T* ds = reinterpret_cast<const T*>(q.dy) + n * q.dy_sb + c;
+        for (int64_t r = r0 + sub; r < r1; r += sp.side) {
+          float x[8], d[8];
+          load8(xs + r * p.x_ss, left, x);
+          load8(ds + r * q.dy_ss, left, d);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            x[j] = (x[j] - mean) * rstd;
+            const float dz = j < left ? d[j] * act_slope(p.silu, x[j] * a.w[j] + a.b[j]) : 0.f;
+            A[j] += dz;
+            B[j] += dz * x[j];
+          }
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        sa[tid][j] = A[j];
+        sa[tid][8 + j] = B[j];
+      }
+      __syncthreads();
+      if (on && sub == 0) {
+        float* to = q.part + ((n * sp.splits + s) * p.channels + c) * 2;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          for (int i = 1; i < sp.side; ++i) {
+            A[j] += sa[tid + i * sp.ub][j];
+            B[j] += sa[tid + i * sp.ub][8 + j];
+          }
+          if (j < left) {
+            to[2 * j] = A[j];
+            to[2 * j + 1] = B[j];
+          }
+        }
+      }
+    }
+  }
+}
+
+// The splits joined: `whole` (batch, channels, 2), and mean(gw), mean(gw xh) of each (batch, group) into `means`.  A wave
+// for each (batch, group).
+__global__ __launch_bounds__(256) void group_bwd_join_kernel(GroupNormBwdParams q, Split sp, float* whole, float* means) {
+  const GroupNormParams& p = q.f;
+  const int lane = threadIdx.x & 63;
+  const int64_t items = p.batch * p.groups;
+  for (int64_t it = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); it < items; it += (int64_t)gridDim.x * 4) {
+    const int64_t n = it / p.groups;
+    const int g = (int)(it % p.groups);
+    float s1 = 0.f, s2 = 0.f;
+    for (int i = lane; i < sp.cg; i += 64) {
+      const int c = g * sp.cg + i;
+      float a = 0.f, b = 0.f;
+#pragma unroll 8
+      for (int s = 0; s < sp.splits; ++s) {
+        const f32x2 v = *reinterpret_cast<const f32x2*>(q.part + ((n * sp.splits + s) * p.channels + c) * 2);
+        a += v[0];
+        b += v[1];
+      }
+      whole[(n * p.channels + c) * 2] = a;
+      whole[(n * p.channels + c) * 2 + 1] = b;
+      const float w = !p.weight ? 1.f : p.w_f32 ? reinterpret_cast<const float*>(p.weight)[c] : to_f32(reinterpret_cast<const bf16*>(p.weight)[c]);
+      s1 += w * a;
+      s2 += w * b;
+    }
+    s1 = group_sum<64>(s1);
+    s2 = group_sum<64>(s2);
+    if (lane == 0) {
+      const float count = (float)p.space * (float)sp.cg;
+      means[2 * it] = s1 / count;
+      means[2 * it + 1] = s2 / count;
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void group_bwd_apply_kernel(GroupNormBwdParams q, Split sp, const float* means) {
+  const GroupNormParams& p = q.f;
+  const int tid = threadIdx.x, u0 = sp.ub <= 256 ? tid % sp.ub : tid, sub = sp.ub <= 256 ? tid / sp.ub : 0;
+  if (sub >= sp.side) return;
+  for (int64_t unit = blockIdx.x; unit < sp.units; unit += gridDim.x) {
+    int64_t n;
+    int s, cb;
+    sp.at(unit, n, s, cb);
+    const int64_t r0 = s * sp.rows, r1 = min(p.space, r0 + sp.rows);
+    for (int u = u0; u < sp.ub; u += 256) {
+      const int g = cb * sp.gb + u / sp.cpg, c8 = u % sp.cpg * 8, left = sp.cg - c8;
+      if (g >= p.groups) break;
+      const int c = g * sp.cg + c8;
+      const int64_t ng = n * p.groups + g;
+      const Affine a(p, c, (g + 1) * sp.cg);
+      const float mean = p.stats[2 * ng], rstd = p.stats[2 * ng + 1], m1 = means[2 * ng], m2 = means[2 * ng + 1];
+      const T* xs = reinterpret_cast<const T*>(p.x) + n * p.x_sb + c;
+      const T* ds = reinterpret_cast<const T*>(q.dy) + n * q.dy_sb + c;
+      T* out = reinterpret_cast<T*>(q.dx) + n * q.dx_sb + c;
+      for (int64_t r = r0 + sub; r < r1; r += sp.side) {
+        float x[8], d[8];
+        load8(xs + r * p.x_ss, left, x);
+        load8(ds + r * q.dy_ss, left, d);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[j] = (x[j] - mean) * rstd;
+          const float gw = d[j] * act_slope(p.silu, x[j] * a.w[j] + a.b[j]) * a.w[j];
+          x[j] = rstd * (gw - m1 - x[j] * m2);
+        }
+        store8(out + r * q.dx_ss, left, x);
+      }
+    }
+  }
+}
+
+bool by_rows(const GroupNormParams& p) { return p.space == 1 && p.channels / p.groups <= kRowsMax; }
+
+int rows_lanes(const GroupNormParams& p) {
+  int n = 1;
+  while (8 * n < p.channels / p.groups) n *= 2;
+  return n;
+}
+
+struct RowsGrid {
+  int gb, side, x, y;
+  explicit RowsGrid(const GroupNormParams& p) {
+    const int slots = 256 / rows_lanes(p);
+    gb = slots < p.groups ? slots : p.groups;
+    side = slots / gb;
+    y = (p.groups + gb - 1) / gb;
+    const int64_t most = (p.batch + side - 1) / side;
+    const int64_t want = 512 / y + 1;
+    x = (int)(want < most ? want : most);
+  }
+};
+
+unsigned grid_of(int64_t n) { return (unsigned)(n < (1 << 20) ? n : 1 << 20); }
+
+template <typename F>
+hipError_t with_lanes(int n, F f) {
+  switch (n) {
+    case 1: f(std::integral_constant<int, 1>()); break;
+    case 2: f(std::integral_constant<int, 2>()); break;
+    case 4: f(std::integral_constant<int, 4>()); break;
+    case 8: f(std::integral_constant<int, 8>()); break;
+    case 16: f(std::integral_constant<int, 16>()); break;
+    case 32: f(std::integral_constant<int, 32>()); break;
+    default: f(std::integral_constant<int, 64>()); break;
+  }
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t fwd(const GroupNormParams& p, hipStream_t st) {
+  if (by_rows(p)) {
+    const int lanes = rows_lanes(p);
+    const int64_t blocks = (p.batch * p.groups + 256 / lanes - 1) / (256 / lanes);
+    return with_lanes(lanes, [&](auto n) { group_rows_kernel<T, decltype(n)::value><<<grid_of(blocks), 256, 0, st>>>(p); });
+  }
+  const Split sp(p);
+  group_sums_kernel<T><<<grid_of(sp.units), 256, 0, st>>>(p, sp);
+  group_apply_kernel<T><<<grid_of(sp.units), 256, 0, st>>>(p, sp);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t bwd(const GroupNormBwdParams& q, hipStream_t st) {
+  const GroupNormParams& p = q.f;
+  const bool params = q.dweight || q.dbias;
+  const float* rows = q.part;
+  int64_t nrows = p.batch;
+  if (by_rows(p)) {
+    const RowsGrid rg(p);
+    GroupNormBwdParams r = q;
+    if (!params) r.part = nullptr;
+    const hipError_t e = with_lanes(rows_lanes(p), [&](auto n) {
+      group_rows_bwd_kernel<T, decltype(n)::value><<<dim3(rg.x, rg.y), 256, 0, st>>>(r, rg.gb, rg.side);
+    });
+    if (e != hipSuccess) return e;
+    nrows = (int64_t)rg.x * rg.side;
+  } else {
+    const Split sp(p);
+    float* whole = q.part + p.batch * sp.splits * p.channels * 2;
+    float* means = whole + p.batch * p.channels * 2;
+    group_bwd_sums_kernel<T><<<grid_of(sp.units), 256, 0, st>>>(q, sp);
+    group_bwd_join_kernel<<<grid_of((p.batch * p.groups + 3) / 4), 256, 0, st>>>(q, sp, whole, means);
+    group_bwd_apply_kernel<T><<<grid_of(sp.units), 256, 0, st>>>(q, sp, means);
+    rows = whole;
+  }
+  if (params)
+    group_params_kernel<<<(p.channels + 15) / 16, 256, 0, st>>>(rows, nrows, p.channels, q.dweight, q.dbias, p.w_f32);
+  return hipGetLastError();
+}
+
+// No rows: the parameters' gradients are cleared.
+__global__ void group_clear_kernel(void* dweight, void* dbias, int channels, int f32) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= channels) return;
+  if (dweight) {
+    if (f32) reinterpret_cast<float*>(dweight)[c] = 0.f;
+    else reinterpret_cast<bf16*>(dweight)[c] = (bf16)0.f;
+  }
+  if (dbias) {
+    if (f32) reinterpret_cast<float*>(dbias)[c] = 0.f;
+    else reinterpret_cast<bf16*>(dbias)[c] = (bf16)0.f;
+  }
+}
+
+}  // namespace
+
+size_t group_norm_workspace_bytes(const GroupNormParams& p) {
+  if (by_rows(p) || p.batch == 0 || p.space == 0) return 0;
+  return (size_t)p.batch * Split(p).splits * p.groups * 2 * sizeof(double);
+}
+
+hipError_t launch_group_norm(const GroupNormParams& p, hipStream_t st) {
+  if (p.batch == 0 || p.space == 0) return hipSuccess;
+  return p.dtype == DT_F32 ? fwd<float>(p, st) : fwd<bf16>(p, st);
+}
+
+size_t group_norm_bwd_workspace_bytes(const GroupNormParams& p) {
+  if (p.batch == 0 || p.space == 0) return 0;
+  if (by_rows(p)) {
+    const RowsGrid rg(p);
+    return (size_t)rg.x * rg.side * p.channels * 2 * sizeof(float);
+  }
+  return ((size_t)p.batch * (Split(p).splits + 1) * p.channels + (size_t)p.batch * p.groups) * 2 * sizeof(float);
+}
+
+hipError_t launch_group_norm_bwd(const GroupNormBwdParams& q, hipStream_t st) {
+  const GroupNormParams& p = q.f;
+  if (p.batch == 0 || p.space == 0) {
+    if (!q.dweight && !q.dbias) return hipSuccess;
+    group_clear_kernel<<<(p.channels + 255) / 256, 256, 0, st>>>(q.dweight, q.dbias, p.channels, p.w_f32);
+    return hipGetLastError();
+  }
+  return p.dtype == DT_F32 ? bwd<float>(q, st) : bwd<bf16>(q, st);
+}
+
+}  // namespace mh

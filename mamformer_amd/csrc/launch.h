@@ -457,4 +457,84 @@ struct LogprobBwdParams {
 };
 hipError_t launch_logprob_bwd(LogprobBwdParams p, hipStream_t st);
 
+// ------------------------------------------------------------- gated delta rule (delta_*.hip)
+struct DeltaStrides { int64_t b, h, l; };  // elements; channels contiguous
+struct DeltaParams {
+  int batch, heads, kheads, seqlen, dk, dv, dtype;
+  int pieces;                              // ceil(seqlen / 64)
+  float scale;
+  const void *q, *k, *v; DeltaStrides qs, ks, vs;
+  const float *g, *beta; DeltaStrides gs, bs;        // each or null
+  const float* initial_state;              // (b, H, dk, dv) contiguous or null
+  float* final_state;                      // or null
+  void* o; DeltaStrides os;                // null: not computed
+  char* workspace;
+};
+size_t delta_workspace_bytes(const DeltaParams& p);
+hipError_t launch_delta(const DeltaParams& p, hipStream_t st);
+
+struct DeltaBwdParams {
+  DeltaParams f;                           // o, final_state null
+  const void* d_o; DeltaStrides dos;
+  const float* d_final_state;              // or null
+  void *dq, *dk, *dv; DeltaStrides dqs, dks, dvs;
+  float *dg, *dbeta;                       // (b, H, L) contiguous
+  float* d_initial_state;                  // or null
+};
+size_t delta_bwd_workspace_bytes(const DeltaParams& p);
+hipError_t launch_delta_bwd(const DeltaBwdParams& p, hipStream_t st);
+// The forward's parts that the backward runs again: the pieces' triangular systems, and the scan that keeps the entering
+// states and the corrections.
+hipError_t launch_delta_prep(const DeltaParams& p, bool backward, hipStream_t st);
+hipError_t launch_delta_keep(const DeltaParams& p, hipStream_t st);
+
+struct DeltaStepParams {
+  int batch, heads, kheads, dk, dv, dtype;
+  float scale;
+  const void *q, *k, *v; int64_t q_sb, q_sh, k_sb, k_sh, v_sb, v_sh;
+  const float *g, *beta; int64_t g_sb, g_sh, b_sb, b_sh;     // each or null
+  const float* state_in; float* state_out;
+  void* o; int64_t o_sb, o_sh;
+};
+hipError_t launch_delta_step(const DeltaStepParams& p, hipStream_t st);
+
+// ------------------------------------------------------------- rotary positions
+struct RotaryTensor {
+  const void* in; DeltaStrides in_s;       // (batch, heads, seqlen, dim), channels contiguous
+  void* out; DeltaStrides out_s;
+};
+struct RotaryParams {
+  int batch, q_heads, k_heads, seqlen, dim, pairs, dtype, interleaved, inverse;
+  float scale;
+  const void* inv_freq; int freq64;        // (pairs,) fp64 or fp32
+  const void* positions; int i64; int64_t pos_sb;    // (batch, seqlen) with rows pos_sb apart, or null: 0 .. seqlen - 1
+  int64_t offset;                          // added to every position
+  RotaryTensor q, k;                       // k_heads = 0: q alone
+};
+hipError_t launch_rotary(const RotaryParams& p, hipStream_t st);
+
+// ------------------------------------------------------------- group norm, channels last
+struct GroupNormParams {
+  int64_t batch, space;                    // x (batch, space, channels)
+  int channels, groups, dtype, w_f32, silu;
+  float eps;
+  const void* x; int64_t x_sb, x_ss;
+  const void* weight; const void* bias;    // each or null
+  void* y; int64_t y_sb, y_ss;
+  float* stats;                            // (batch, groups, 2) or null
+  double* part;                            // workspace
+};
+size_t group_norm_workspace_bytes(const GroupNormParams& p);
+hipError_t launch_group_norm(const GroupNormParams& p, hipStream_t st);
+
+struct GroupNormBwdParams {
+  GroupNormParams f;                       // y null; stats as the forward wrote them
+  const void* dy; int64_t dy_sb, dy_ss;
+  void* dx; int64_t dx_sb, dx_ss;
+  void* dweight; void* dbias;              // each or null
+  float* part;                             // workspace
+};
+size_t group_norm_bwd_workspace_bytes(const GroupNormParams& p);
+hipError_t launch_group_norm_bwd(const GroupNormBwdParams& p, hipStream_t st);
+
 }  // namespace mh
