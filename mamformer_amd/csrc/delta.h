@@ -61,17 +61,20 @@ __device__ __forceinline__ f16x8 col_frag16(const f16* t, int c0, int k0, int la
   return __builtin_bit_cast(f16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// The largest of a value over the wave, in every lane.
-__device__ __forceinline__ float wave_max(float v) {
-  v = fmaxf(v, dppf<0xB1>(v));
-  v = fmaxf(v, dppf<0x4E>(v));
-  v = fmaxf(v, dppf<0x141>(v));
-  v = fmaxf(v, dppf<0x140>(v));
+template <int CTRL> __device__ __forceinline__ float max_dpp(float v) {
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true)));
+}
+// The largest of a value over the lanes of a column (l % 16), and over the wave, in every lane.
+__device__ __forceinline__ float col_max(float v) {
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
+__device__ __forceinline__ float row16_max(float v) {
+  return max_dpp<0x140>(max_dpp<0x141>(max_dpp<0x4E>(max_dpp<0xB1>(v))));
+}
+__device__ __forceinline__ float wave_max(float v) { return col_max(row16_max(v)); }
 
 // The power of two s (`inv`) with amax / s in [2^12, 2^13), and 1 / s (`mult`).  A maximum below 2^-114 is taken as that;
 // an infinity stays one in every part, so that it reaches the results.
@@ -86,15 +89,19 @@ struct Scale {
 __device__ __forceinline__ f16 part_hi(float x, float mult) { return (f16)(x * mult); }
 __device__ __forceinline__ f16 part_lo(float x, float mult, f16 hi) { return (f16)__builtin_fmaf(x, mult, -(float)hi); }
 
-// B operand of k-step c from accumulator tiles 2 c and 2 c + 1 (rows 32 c .. 32 c + 31).
+// B operand of k-step c from accumulator tiles 2 c and 2 c + 1 (rows 32 c .. 32 c + 31), on a scale of the lane's column.
+// `zero` is a 0 that the compiler does not see through: x mult + 0 rounded to fp16 is one instruction, the product alone
+// one and a half.
 template <int PLANES, int N>
 __device__ __forceinline__ void parts_of(const f32x4 (&t)[N], float mult, f16x8 (&hi)[N / 2], f16x8 (&lo)[N / 2]) {
+  float zero = 0.f;
+  asm volatile("" : "+v"(zero));
 #pragma unroll
   for (int c = 0; c < N / 2; ++c)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float x = t[2 * c + (j >> 2)][j & 3];
-      hi[c][j] = part_hi(x, mult);
+      hi[c][j] = (f16)__builtin_fmaf(x, mult, zero);
       if constexpr (PLANES == 2) lo[c][j] = part_lo(x, mult, hi[c][j]);
     }
 }
@@ -122,31 +129,110 @@ __device__ __forceinline__ double wave_scan64(double v) {
 }
 
 // ------------------------------------------------------------------ workspace
-// For each (batch, key head, piece): the parts of K, then of Q.  For each (batch, value head, piece): T and P (two parts
-// each) and `vec`: e^{G_t}, beta_t e^{G_end - G_t}, then e^{G_end} and the scales of T, P, K and Q.  For the backward,
-// for each (batch, value head, piece, 16 columns of v): the entering state, its gradient behind the piece, delta and y,
-// two parts each, transposed ([column][row]), and their four scales.
+// Operands are kept as the instructions take them, a fragment of 64 lanes x 8 values (1 KB) after the other, so that they
+// are read by 16 bytes a lane without conflicts, and the scans need no transposing reads.
+//   For each (batch, key head, piece), NP parts of each: Q by rows (i KS + s: rows 16 i .., k-step s), K by rows, K by
+//     columns (2 n + s: channels 16 n .., tokens 32 s ..), and for the backward Q by columns.
+//   For each (batch, value head, piece), two parts of each: T by rows (its 6 fragments that are not zero), then P by rows,
+//     or for the backward T and P by columns.
+//   `vec` for the same: e^{G_t}, beta_t e^{G_end - G_t}, then e^{G_end} and the scales of T, P, K and Q.
+//   For the backward, for each (batch, value head, piece, 16 columns of v): the entering state, its gradient behind the
+//     piece, delta and y, two parts each, in the order in which waves hold them as operands ([part][k-step]), and the
+//     scales of their columns in either half of the rows ([half][which][column]).
+constexpr int FR = 512;                          // halfs of a fragment
+template <int DKP> constexpr int kKFrags = DKP / 8;                    // of K or Q, rows or columns
+constexpr int kTFrags = 6;
+__device__ __forceinline__ constexpr int t_frag(int i, int s) { return s ? 2 + i : i; }      // by rows: i >= 2 s
+__device__ __forceinline__ constexpr int tt_frag(int i, int s) { return 2 * s + i; }         // by columns: i < 2 + 2 s
+__device__ __forceinline__ f16x8 frag(const f16* t, int f, int lane) { return *reinterpret_cast<const f16x8*>(t + f * FR + lane * 8); }
+__device__ __forceinline__ void put_frag(f16* t, int f, int lane, f16x8 v) { *reinterpret_cast<f16x8*>(t + f * FR + lane * 8) = v; }
+
 constexpr int kVecFloats = 256;
 enum { VEC_W = 64, VEC_GAMMA = 128, VEC_ST, VEC_SP, VEC_SK, VEC_SQ };
-enum { KEEP_S, KEEP_DS, KEEP_D, KEEP_Y };        // order of the scales
+enum { KEEP_S, KEEP_DS, KEEP_D, KEEP_Y };
 template <int DKP> constexpr size_t keep_halfs() { return 2 * (2 * 16 * DKP) + 2 * (2 * 16 * DC); }
+template <int DKP> constexpr int keep_at(int which) {                  // where one of the four begins, in halfs
+  return which < KEEP_D ? which * 2 * 16 * DKP : 4 * 16 * DKP + (which - KEEP_D) * 2 * 16 * DC;
+}
+// k-steps s0 .. s0 + N - 1 of ALL.
+template <int ALL, int N>
+__device__ __forceinline__ void keep_parts(f16* to, int s0, const f16x8 (&hi)[N], const f16x8 (&lo)[N], int lane) {
+#pragma unroll
+  for (int s = 0; s < N; ++s) {
+    put_frag(to, s0 + s, lane, hi[s]);
+    put_frag(to, ALL + s0 + s, lane, lo[s]);
+  }
+}
 
 struct DeltaLayout {
   size_t kq, tp, vec, keep, scales, total;       // byte offsets
+  size_t kq_unit, tp_unit;                       // bytes of a piece
   __host__ DeltaLayout(const DeltaParams& p, bool backward) {
     const size_t np = p.dtype == DT_F32 ? 2 : 1, dkp = p.dk <= 64 ? 64 : 128;
     const size_t kpieces = (size_t)p.batch * p.kheads * p.pieces, pieces = (size_t)p.batch * p.heads * p.pieces;
     const size_t blocks = backward ? pieces * ((p.dv + 15) / 16) : 0;
+    kq_unit = (backward ? 4 : 3) * np * (dkp / 8) * FR * 2;
+    tp_unit = (backward ? 6 : 4) * kTFrags * FR * 2;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t was = at; at += (bytes + 1023) / 1024 * 1024; return was; };
-    kq = take(kpieces * 2 * np * DC * dkp * 2);
-    tp = take(pieces * 4 * DC * DC * 2);
+    kq = take(kpieces * kq_unit);
+    tp = take(pieces * tp_unit);
     vec = take(pieces * kVecFloats * 4);
     keep = take(blocks * (dkp == 64 ? keep_halfs<64>() : keep_halfs<128>()) * 2);
-    scales = take(blocks * 16);
+    scales = take(blocks * 512);
     total = at;
   }
 };
+
+// N fragments by LDS DMA, wave w of NW taking N / NW in a row.
+template <int N, int NW>
+__device__ __forceinline__ void fetch_share(f16* to, const char* from, int w, int lane) {
+  static_assert(N % NW == 0, "equal shares");
+  const char* src = from + w * (N / NW) * 1024;
+  f16* dst = to + w * (N / NW) * FR;
+  uint32_t off = 16u * lane;
+  asm volatile("" : "+v"(off));                  // 32 bits beside a scalar base, not a 64-bit address held for the loop
+#pragma unroll
+  for (int i = 0; i < N / NW; ++i) dma_lds<16>(src + i * 1024, off, dst + i * FR);
+}
+
+// 32 rows of 16 columns in the accumulators' order: v[i] is row 16 (i / 4) + 4 g + i % 4 of column l % 16.  `at` is the
+// first row at the first column; rows beyond `len` read the last one, or row 0 (their gates are zero), columns beyond the
+// last one as 0.  A row's address is the wave's, one offset the lane's.
+template <typename T>
+__device__ __forceinline__ void load_rows8(const T* at, int64_t stride, int len, bool cv, bool all_cv, int l16, int g4, T (&v)[8]) {
+  int c = cv ? l16 : 0;
+  asm volatile("" : "+v"(c), "+v"(g4));          // addresses formed here, not held for the loop
+  if (len >= 32) {
+    const uint32_t off = (uint32_t)(4 * g4 * (int)stride + c) * (uint32_t)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] = *reinterpret_cast<const T*>(reinterpret_cast<const char*>(at + (16 * (i >> 2) + (i & 3)) * stride) + off);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = at[(int64_t)min(16 * (i >> 2) + 4 * g4 + (i & 3), len - 1) * stride + c];
+  }
+  if (!all_cv)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = cv ? v[i] : from_f32<T>(0.f);
+}
+template <typename T>
+__device__ __forceinline__ void store_rows8(T* at, int64_t stride, int len, bool cv, int l16, int g4, const float (&v)[8]) {
+  if (!cv) return;
+  asm volatile("" : "+v"(l16), "+v"(g4));
+  if (len >= 32) {
+    const uint32_t off = (uint32_t)(4 * g4 * (int)stride + l16) * (uint32_t)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      *reinterpret_cast<T*>(reinterpret_cast<char*>(at + (16 * (i >> 2) + (i & 3)) * stride) + off) = from_f32<T>(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 16 * (i >> 2) + 4 * g4 + (i & 3);
+      if (r < len) at[(int64_t)r * stride + l16] = from_f32<T>(v[i]);
+    }
+  }
+}
 
 // Workgroup n of heads x blocks, with the blocks of a head on one XCD (workgroups go to the 8 XCDs in turn): they share the
 // head's tiles through its L2.  False beyond the last head.

@@ -17,220 +17,318 @@
 namespace mh {
 namespace {
 
-template <typename T, int DKP, int NW>
-__global__ __launch_bounds__(64 * NW) void delta_back_scan_kernel(DeltaBwdParams q, DeltaLayout lay, int nblk, int nwg) {
+// Two waves hold the gradient of 16 columns of the state as the forward's scan holds the state: half of its rows and half of
+// a piece's tokens each.  y = T^T ddelta is upper triangular, so that here the first wave needs the second one's ddelta.
+template <typename T, int DKP>
+__global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 320) void delta_back_scan_kernel(DeltaBwdParams q, DeltaLayout lay, int nblk, int nwg) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
-  constexpr int NBUF = NP == 1 ? 2 : 1;
-  using TK = HTile<DKP>;
-  using TC = HTile<64>;
-  constexpr int KQ = 2 * NP * TK::ELEMS, TP = 4 * TC::ELEMS, BUF = KQ + TP + kVecFloats * 2;
-  constexpr int NS = DKP / 16, KS = DKP / 32;
-  __shared__ __align__(1024) f16 smem[NBUF * BUF];
+  constexpr bool AHEAD = NP == 1;
+  constexpr int FW = AHEAD ? 1 : 4;
+  constexpr int KS = DKP / 32, KSH = KS / 2, NSH = DKP / 32, F = kKFrags<DKP>;
+  constexpr int GA = NP * F + 2 * kTFrags;                           // fragments of K by rows and P by columns: before barrier 1
+  constexpr int GB = 2 * NP * F + 2 * kTFrags + 1;                   // K and Q by columns, T by columns, vec: after it
+  constexpr int EX = (2 * 2 + 2 + 2 * 4 + 1) * FR;                   // halfs of a pair's exchange
+  __shared__ __align__(1024) f16 smem[(GA + (AHEAD ? 2 : 1) * GB) * FR + 2 * EX];
   const DeltaParams& p = q.f;
 
-  const int lane = threadIdx.x & 63, w = wave_id(), l16 = lane & 15, g4 = lane >> 4;
+  const int lane = threadIdx.x & 63, w = wave_id(), l16 = lane & 15, g4 = lane >> 4, hf = w & 1;
   int bh, wg;
   if (!head_block(blockIdx.x, p.batch * p.heads, nwg, bh, wg)) return;
   const int b = bh / p.heads, h = bh % p.heads, hk = h / (p.heads / p.kheads);
-  const int blk = wg * NW + w, col = 16 * blk + l16;
-  const bool live = blk < nblk, cv = col < p.dv;
+  const int blk = 2 * wg + (w >> 1), col = 16 * blk + l16;
+  const bool live = blk < nblk, cv = col < p.dv, all_cv = 16 * blk + 16 <= p.dv;
   const int64_t kunit0 = ((int64_t)b * p.kheads + hk) * p.pieces, vunit0 = (int64_t)bh * p.pieces;
 
-  auto fetch = [&](int c, int buf) {
-    char* to = reinterpret_cast<char*>(smem + buf * BUF);
-    const char* kq = p.workspace + lay.kq + (kunit0 + c) * (int64_t)(KQ * 2);
-    const char* tp = p.workspace + lay.tp + (vunit0 + c) * (int64_t)(TP * 2);
-    const char* vec = p.workspace + lay.vec + (vunit0 + c) * (int64_t)(kVecFloats * 4);
-#pragma unroll
-    for (int i = w; i < KQ / 512; i += NW) dma_lds<16>(kq + i * 1024, 16u * lane, to + i * 1024);
-#pragma unroll
-    for (int i = w; i < TP / 512; i += NW) dma_lds<16>(tp + i * 1024, 16u * lane, to + KQ * 2 + i * 1024);
-    if (w == 0) dma_lds<16>(vec, 16u * lane, to + (KQ + TP) * 2);
-  };
+  f16* ex = smem + (GA + (AHEAD ? 2 : 1) * GB) * FR + (w >> 1) * EX;
+  f32x4* const xSend = reinterpret_cast<f32x4*>(ex) + hf * 2 * 64 + lane;
+  const f32x4* const xRecv = reinterpret_cast<const f32x4*>(ex) + (1 - hf) * 2 * 64 + lane;
+  f16* const eZ = ex + 4 * FR;                                       // the second half's ddelta
+  f16* const eU = eZ + 2 * FR;                                       // the terms of Q and K, two parts of each half
+  float* const eS = reinterpret_cast<float*>(eU + 8 * FR);
 
-  f32x4 dS[NS];
+  const int fw = AHEAD ? 0 : w;
+  auto fetch_a = [&](int c) {
+    fetch_share<NP * F, FW>(smem, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + NP * F * 1024, fw, lane);
+    fetch_share<2 * kTFrags, FW>(smem + NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit + 4 * kTFrags * 1024, fw, lane);
+  };
+  auto fetch_b = [&](int c) {
+    f16* to = smem + (GA + (AHEAD ? (c & 1) * GB : 0)) * FR;
+    fetch_share<2 * NP * F, FW>(to, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + 2 * NP * F * 1024, fw, lane);
+    fetch_share<2 * kTFrags, FW>(to + 2 * NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit + 2 * kTFrags * 1024, fw, lane);
+    if (fw == 0) dma_lds<16>(p.workspace + lay.vec + (vunit0 + c) * (int64_t)(kVecFloats * 4), 16u * lane, to + (2 * NP * F + 2 * kTFrags) * FR);
+  };
+  if constexpr (AHEAD) if (w == 4) {                         // as in the forward's scan
+    fetch_a(p.pieces - 1);
+    fetch_b(p.pieces - 1);
+    wait_vmem_n<GB>();
+    lds_barrier();
+    for (int c = p.pieces - 1; c >= 0; --c) {
+      wait_vmem();
+      lds_barrier();                             // 1
+      if (c > 0) fetch_a(c - 1);
+      lds_barrier();                             // 2
+      if (c > 0) {
+        fetch_b(c - 1);
+        wait_vmem_n<GB>();
+      }
+      lds_barrier();                             // 3
+    }
+    return;
+  }
+
+  f32x4 dS[NSH];
 #pragma unroll
-  for (int n = 0; n < NS; ++n)
+  for (int n = 0; n < NSH; ++n)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int row = 16 * n + 4 * g4 + r;
+      const int row = DKP / 2 * hf + 16 * n + 4 * g4 + r;
       dS[n][r] = q.d_final_state && cv && row < p.dk ? q.d_final_state[((int64_t)bh * p.dk + row) * p.dv + col] : 0.f;
     }
-  const T* osrc = reinterpret_cast<const T*>(q.d_o) + b * q.dos.b + h * q.dos.h + col;
-  T on[16];
+  // dO of one's own tokens; the first wave's P^T dO takes the other's too
+  const T* osrc = reinterpret_cast<const T*>(q.d_o) + b * q.dos.b + h * q.dos.h + 16 * blk;
+  T on[2][8];
   auto load_o = [&](int c) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int t = c * DC + 16 * (i >> 2) + 4 * g4 + (i & 3);
-      on[i] = cv && t < p.seqlen ? osrc[(int64_t)t * q.dos.l] : from_f32<T>(0.f);
+    for (int x = 0; x < 2; ++x) {
+      if (x && hf) break;
+      const int t = c * DC + 32 * (hf + x), len = p.seqlen - t;
+      const int from = min(t, p.seqlen - 1);
+      load_rows8<T>(osrc + from * q.dos.l, q.dos.l, p.seqlen - from, cv, all_cv, l16, g4, on[x]);
+      if (len < 32)                              // no output, no gradient
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (16 * (i >> 2) + 4 * g4 + (i & 3) >= len) on[x][i] = from_f32<T>(0.f);
     }
   };
-  load_o(p.pieces - 1);
-  if (NBUF == 2) fetch(p.pieces - 1, (p.pieces - 1) & 1);
+  if (live) load_o(p.pieces - 1);
+  if (AHEAD) lds_barrier();
 
   for (int c = p.pieces - 1; c >= 0; --c) {
-    const f16* buf = smem + (NBUF == 2 ? (c & 1) * BUF : 0);
-    if (NBUF == 2) {
+    if (!AHEAD) {
+      lds_barrier();
+      fetch_a(c);
+      fetch_b(c);
       wait_vmem();
-      __syncthreads();
-      if (c > 0) fetch(c - 1, (c - 1) & 1);
-    } else {
-      __syncthreads();
-      fetch(c, 0);
-      wait_vmem();
-      __syncthreads();
+      lds_barrier();
     }
-    if (!live) continue;
-    const f16 *Kt = buf, *Qt = buf + NP * TK::ELEMS, *Tt = buf + KQ, *Pt = Tt + 2 * TC::ELEMS;
-    const float* vec = reinterpret_cast<const float*>(buf + KQ + TP);
-    f32x4 U[4];
+    const f16 *Kr = smem, *Pt = smem + NP * F * FR;
+    const f16 *Kc = smem + (GA + (AHEAD ? (c & 1) * GB : 0)) * FR, *Qc = Kc + NP * F * FR, *Tt = Qc + NP * F * FR;
+    const float* vec = reinterpret_cast<const float*>(Tt + 2 * kTFrags * FR);
+    f16x8 sh[KSH], sl[KSH];
+    f32x4 X[2] = {}, Z[2] = {}, U[2];
+    float ss_inv = 0.f, so_inv = 0.f;
+    if (live) {
+      f16x8 ka[KSH][4];                          // tiles 0, 1: one's own tokens, 2, 3: the other's
 #pragma unroll
-    for (int i = 0; i < 16; ++i) U[i >> 2][i & 3] = to_f32(on[i]);
-    if (c > 0) load_o(c - 1);
-
-    const int64_t at = (vunit0 + c) * nblk + blk;
-    f16* keep = reinterpret_cast<f16*>(p.workspace + lay.keep) + at * (int64_t)keep_halfs<DKP>();
-    float* scales = reinterpret_cast<float*>(p.workspace + lay.scales) + at * 4;
-    f16x8 sh[KS], sl[KS];
-    const Scale ss(wave_max(abs_max(dS)));
-    parts_of<2>(dS, ss.mult, sh, sl);
+      for (int s = 0; s < KSH; ++s)
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      f16* to = keep + 2 * 16 * DKP + l16 * DKP + 16 * n + 4 * g4;
-      *reinterpret_cast<f16x4*>(to) = n & 1 ? __builtin_shufflevector(sh[n >> 1], sh[n >> 1], 4, 5, 6, 7)
-                                            : __builtin_shufflevector(sh[n >> 1], sh[n >> 1], 0, 1, 2, 3);
-      *reinterpret_cast<f16x4*>(to + 16 * DKP) = n & 1 ? __builtin_shufflevector(sl[n >> 1], sl[n >> 1], 4, 5, 6, 7)
-                                                       : __builtin_shufflevector(sl[n >> 1], sl[n >> 1], 0, 1, 2, 3);
-    }
-    if (lane == 0) scales[KEEP_DS] = ss.inv;
-    // K dS
-    f32x4 X[4] = {};
+        for (int i = 0; i < 4; ++i) ka[s][i] = frag(Kr, ((2 * hf + i) & 3) * KS + hf * KSH + s, lane);
+      const Scale ss(col_max(abs_max(dS)));
+      ss_inv = ss.inv;
+      parts_of<2>(dS, ss.mult, sh, sl);
+      f32x4 XO[2] = {};
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+      for (int s = 0; s < KSH; ++s) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f16x8 a = row_frag16<DKP>(Kt, 16 * i, 32 * s, lane);
-        X[i] = mma_h(a, sh[s], X[i]);
-        X[i] = mma_h(a, sl[s], X[i]);
-        if constexpr (NP == 2) X[i] = mma_h(row_frag16<DKP>(Kt + TK::ELEMS, 16 * i, 32 * s, lane), sh[s], X[i]);
+        for (int i = 0; i < 4; ++i) (i < 2 ? X[i & 1] : XO[i & 1]) = mma_h(ka[s][i], sh[s], i < 2 ? X[i & 1] : XO[i & 1]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) (i < 2 ? X[i & 1] : XO[i & 1]) = mma_h(ka[s][i], sl[s], i < 2 ? X[i & 1] : XO[i & 1]);
+        if constexpr (NP == 2)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            (i < 2 ? X[i & 1] : XO[i & 1]) = mma_h(frag(Kr, F + ((2 * hf + i) & 3) * KS + hf * KSH + s, lane), sh[s], i < 2 ? X[i & 1] : XO[i & 1]);
       }
-    // P^T dO
-    f16x8 oh[2], ol[2];
-    const Scale so(wave_max(abs_max(U)));
-    parts_of<NP>(U, so.mult, oh, ol);
-    f32x4 Z[4] = {};
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+      for (int i = 0; i < 2; ++i) xSend[i * 64] = XO[i] * ss_inv;
+      // P^T dO
 #pragma unroll
-      for (int i = 0; i < 2 + 2 * s; ++i) {
-        const f16x8 a = col_frag16<64>(Pt, 16 * i, 32 * s, lane);
-        Z[i] = mma_h(a, oh[s], Z[i]);
-        if constexpr (NP == 2) Z[i] = mma_h(a, ol[s], Z[i]);
-        Z[i] = mma_h(col_frag16<64>(Pt + TC::ELEMS, 16 * i, 32 * s, lane), oh[s], Z[i]);
+      for (int i = 0; i < 8; ++i) U[i >> 2][i & 3] = to_f32(on[0][i]);
+      f32x4 V[2];
+      float om = abs_max(U);
+      if (hf == 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) V[i >> 2][i & 3] = to_f32(on[1][i]);
+        om = abs_max(V, om);
       }
-    const float zs = p.scale * (so.inv * vec[VEC_SP]), xs = ss.inv * vec[VEC_SK];
+      const Scale so(col_max(om));
+      so_inv = so.inv;
+      f16x8 oh[1], ol[1];
+      parts_of<NP>(U, so.mult, oh, ol);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x4 wt = *reinterpret_cast<const f32x4*>(vec + VEC_W + 16 * i + 4 * g4);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) Z[i][r] = zs * Z[i][r] + wt[r] * (xs * X[i][r]);
-    }
-    // y = T^T ddelta
-    f16x8 zh[2], zl[2];
-    const Scale sz(wave_max(abs_max(Z)));
-    parts_of<2>(Z, sz.mult, zh, zl);
-    f32x4 Y[4] = {};
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int i = 0; i < 2 + 2 * s; ++i) {
-        const f16x8 a = col_frag16<64>(Tt, 16 * i, 32 * s, lane);
-        Y[i] = mma_h(a, zh[s], Y[i]);
-        Y[i] = mma_h(a, zl[s], Y[i]);
-        Y[i] = mma_h(col_frag16<64>(Tt + TC::ELEMS, 16 * i, 32 * s, lane), zh[s], Y[i]);
+      for (int i = 0; i < 2; ++i) {
+        const f16x8 a = frag(Pt, tt_frag(2 * hf + i, hf), lane);
+        Z[i] = mma_h(a, oh[0], Z[i]);
+        if constexpr (NP == 2) Z[i] = mma_h(a, ol[0], Z[i]);
+        Z[i] = mma_h(frag(Pt, kTFrags + tt_frag(2 * hf + i, hf), lane), oh[0], Z[i]);
       }
-    const float ysc = sz.inv * vec[VEC_ST];
-    T* dv = reinterpret_cast<T*>(q.dv) + b * q.dvs.b + h * q.dvs.h + col;
+      if (hf == 0) {
+        parts_of<NP>(V, so.mult, oh, ol);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float y = Y[i >> 2][i & 3] *= ysc;
-      const int t = c * DC + 16 * (i >> 2) + 4 * g4 + (i & 3);
-      if (cv && t < p.seqlen) dv[(int64_t)t * q.dvs.l] = from_f32<T>(y);
-    }
-    f16x8 yh[2], yl[2];
-    const Scale sy(wave_max(abs_max(Y)));
-    parts_of<2>(Y, sy.mult, yh, yl);
-    {
-      f16* to = keep + 2 * (2 * 16 * DKP) + 2 * 16 * DC + l16 * DC + 4 * g4;
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        *reinterpret_cast<f16x4*>(to + 16 * n) = n & 1 ? __builtin_shufflevector(yh[n >> 1], yh[n >> 1], 4, 5, 6, 7)
-                                                       : __builtin_shufflevector(yh[n >> 1], yh[n >> 1], 0, 1, 2, 3);
-        *reinterpret_cast<f16x4*>(to + 16 * DC + 16 * n) = n & 1 ? __builtin_shufflevector(yl[n >> 1], yl[n >> 1], 4, 5, 6, 7)
-                                                                 : __builtin_shufflevector(yl[n >> 1], yl[n >> 1], 0, 1, 2, 3);
-      }
-      if (lane == 0) scales[KEEP_Y] = sy.inv;
-    }
-    // the gradient before the piece: both terms on one scale, those of Q's and K's parts in it
-    const float uq = p.scale * vec[VEC_SQ], uk = -vec[VEC_SK];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x4 eg = *reinterpret_cast<const f32x4*>(vec + 16 * i + 4 * g4);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        U[i][r] *= uq * eg[r];
-        Y[i][r] *= uk * eg[r];
-      }
-    }
-    const Scale su(wave_max(abs_max(Y, abs_max(U))));
-    parts_of<2>(U, su.mult, oh, ol);
-    parts_of<2>(Y, su.mult, yh, yl);
-    const float gamma = vec[VEC_GAMMA];
-#pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      f32x4 u = {};
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const f16x8 a = col_frag16<DKP>(Qt, 16 * n, 32 * s, lane), k = col_frag16<DKP>(Kt, 16 * n, 32 * s, lane);
-        u = mma_h(a, oh[s], u);
-        u = mma_h(a, ol[s], u);
-        u = mma_h(k, yh[s], u);
-        u = mma_h(k, yl[s], u);
-        if constexpr (NP == 2) {
-          u = mma_h(col_frag16<DKP>(Qt + TK::ELEMS, 16 * n, 32 * s, lane), oh[s], u);
-          u = mma_h(col_frag16<DKP>(Kt + TK::ELEMS, 16 * n, 32 * s, lane), yh[s], u);
+        for (int i = 0; i < 2; ++i) {
+          const f16x8 a = frag(Pt, tt_frag(i, 1), lane);
+          Z[i] = mma_h(a, oh[0], Z[i]);
+          if constexpr (NP == 2) Z[i] = mma_h(a, ol[0], Z[i]);
+          Z[i] = mma_h(frag(Pt, kTFrags + tt_frag(i, 1), lane), oh[0], Z[i]);
         }
       }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) dS[n][r] = gamma * dS[n][r] + su.inv * u[r];
     }
+    lds_barrier();                               // 1
+    if (live && c > 0) load_o(c - 1);
+    f32x4 Yv[2] = {};
+    float zi = 0.f;
+    if (live) {
+      const float zs = p.scale * (so_inv * vec[VEC_SP]), sK = vec[VEC_SK];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const f32x4 wt = *reinterpret_cast<const f32x4*>(vec + VEC_W + 32 * hf + 16 * i + 4 * g4);
+        const f32x4 xr = xRecv[i * 64];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) Z[i][r] = zs * Z[i][r] + wt[r] * (sK * (ss_inv * X[i][r] + xr[r]));
+      }
+      // y = T^T ddelta
+      f16x8 zh[1], zl[1];
+      const Scale sz(col_max(abs_max(Z)));
+      zi = sz.inv;
+      parts_of<2>(Z, sz.mult, zh, zl);
+      if (hf == 1) {
+        put_frag(eZ, 0, lane, zh[0]);
+        put_frag(eZ, 1, lane, zl[0]);
+        eS[lane] = zi;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const f16x8 a = frag(Tt, tt_frag(2 * hf + i, hf), lane), a1 = frag(Tt, kTFrags + tt_frag(2 * hf + i, hf), lane);
+        Yv[i] = mma_h(a, zh[0], Yv[i]);
+        Yv[i] = mma_h(a, zl[0], Yv[i]);
+        Yv[i] = mma_h(a1, zh[0], Yv[i]);
+      }
+    }
+    lds_barrier();                               // 2
+    f16x8 uh[1], ul[1], vh[1], vl[1], yh[1], yl[1];
+    float own = 0.f, sy_inv = 0.f;
+    if (live) {
+      if (hf == 0) {
+        const f16x8 z0 = frag(eZ, 0, lane), z1 = frag(eZ, 1, lane);
+        f32x4 E[2] = {};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const f16x8 a = frag(Tt, tt_frag(i, 1), lane), a1 = frag(Tt, kTFrags + tt_frag(i, 1), lane);
+          E[i] = mma_h(a, z0, E[i]);
+          E[i] = mma_h(a, z1, E[i]);
+          E[i] = mma_h(a1, z0, E[i]);
+        }
+        const float es = eS[lane];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) Yv[i][r] = zi * Yv[i][r] + es * E[i][r];
+        zi = 1.f;
+      }
+      // both terms of the gradient before the piece on one scale, those of Q's and K's parts in it
+      const float ysc = zi * vec[VEC_ST], uq = p.scale * vec[VEC_SQ], uk = -(ysc * vec[VEC_SK]);
+      f32x4 V[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const f32x4 eg = *reinterpret_cast<const f32x4*>(vec + 32 * hf + 16 * i + 4 * g4);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          U[i][r] *= uq * eg[r];
+          V[i][r] = uk * eg[r] * Yv[i][r];
+        }
+      }
+      const Scale su(col_max(abs_max(V, abs_max(U))));
+      own = su.inv;
+      parts_of<2>(U, su.mult, uh, ul);
+      parts_of<2>(V, su.mult, vh, vl);
+      put_frag(eU, 4 * hf, lane, uh[0]);
+      put_frag(eU, 4 * hf + 1, lane, ul[0]);
+      put_frag(eU, 4 * hf + 2, lane, vh[0]);
+      put_frag(eU, 4 * hf + 3, lane, vl[0]);
+      eS[(2 + hf) * 64 + lane] = own;
+      const Scale sy(col_max(abs_max(Yv)));
+      parts_of<2>(Yv, sy.mult, yh, yl);
+      sy_inv = sy.inv * ysc;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) Yv[i] *= ysc;
+    }
+    lds_barrier();                               // 3
+    if (!live) continue;
+    {
+      const f16* eO = eU + 4 * (1 - hf) * FR;
+      const f16x8 o0 = frag(eO, 0, lane), o1 = frag(eO, 1, lane), o2 = frag(eO, 2, lane), o3 = frag(eO, 3, lane);
+      const float gamma = vec[VEC_GAMMA], other = eS[(3 - hf) * 64 + lane];
+#pragma unroll
+      for (int n = 0; n < NSH; ++n) {
+        const int at = 2 * (hf * NSH + n);
+        const f16x8 qa = frag(Qc, at + hf, lane), qo = frag(Qc, at + 1 - hf, lane);
+        const f16x8 ka = frag(Kc, at + hf, lane), ko = frag(Kc, at + 1 - hf, lane);
+        f32x4 u0 = {}, u1 = {};
+        u0 = mma_h(qa, uh[0], u0);
+        u1 = mma_h(qo, o0, u1);
+        u0 = mma_h(qa, ul[0], u0);
+        u1 = mma_h(qo, o1, u1);
+        u0 = mma_h(ka, vh[0], u0);
+        u1 = mma_h(ko, o2, u1);
+        u0 = mma_h(ka, vl[0], u0);
+        u1 = mma_h(ko, o3, u1);
+        if constexpr (NP == 2) {
+          u0 = mma_h(frag(Qc, F + at + hf, lane), uh[0], u0);
+          u1 = mma_h(frag(Qc, F + at + 1 - hf, lane), o0, u1);
+          u0 = mma_h(frag(Kc, F + at + hf, lane), vh[0], u0);
+          u1 = mma_h(frag(Kc, F + at + 1 - hf, lane), o2, u1);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) dS[n][r] = gamma * dS[n][r] + own * u0[r] + other * u1[r];
+      }
+    }
+    const int64_t at = (vunit0 + c) * nblk + blk;
+    f16* keep = reinterpret_cast<f16*>(p.workspace + lay.keep) + at * (int64_t)keep_halfs<DKP>();
+    float* scales = reinterpret_cast<float*>(p.workspace + lay.scales) + at * 128 + 64 * hf + l16;
+    keep_parts<KS>(keep + keep_at<DKP>(KEEP_DS), hf * KSH, sh, sl, lane);
+    keep_parts<2>(keep + keep_at<DKP>(KEEP_Y), hf, yh, yl, lane);
+    if (g4 == 0) {
+      scales[16 * KEEP_DS] = ss_inv;
+      scales[16 * KEEP_Y] = sy_inv;
+    }
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = Yv[i >> 2][i & 3];
+    const int t = c * DC + 32 * hf;
+    store_rows8<T>(reinterpret_cast<T*>(q.dv) + b * q.dvs.b + h * q.dvs.h + t * q.dvs.l + 16 * blk, q.dvs.l, p.seqlen - t, cv, l16, g4, y);
   }
   if (q.d_initial_state && live && cv) {
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
+    for (int n = 0; n < NSH; ++n)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int row = 16 * n + 4 * g4 + r;
+        const int row = DKP / 2 * hf + 16 * n + 4 * g4 + r;
         if (row < p.dk) q.d_initial_state[((int64_t)bh * p.dk + row) * p.dv + col] = dS[n][r];
       }
   }
 }
 
+// A lane's 8 values of a k-step (keep_parts): columns c .. c + 3 and c + 16 .. c + 19 of row r.
+template <int W>
+__device__ __forceinline__ void put_halves(f16* t, int r, int c, f16x8 v) {
+  *reinterpret_cast<f16x4*>(t + HTile<W>::at(r, c)) = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+  *reinterpret_cast<f16x4*>(t + HTile<W>::at(r, c + 16)) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+}
+
 // One workgroup of 4 waves for a piece of a key head, its value heads one after the other (their dQ and dK are added in
 // that order).  Wave w holds rows 16 w .. 16 w + 15 of the three products with the states (64 x dk) and of A' and P'.  The
-// columns of v pass through LDS DVB at a time, every matrix brought to one scale on the way (the wave's 16 columns that
-// made it had their own).
+// columns of v pass through LDS DVB at a time, every matrix brought to one scale on the way (its columns
+// have their own).
 template <typename T, int DKP>
 __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, DeltaLayout lay, int nblk) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
   constexpr int DVB = NP == 1 ? 64 : 32;
-  constexpr int NS = DKP / 16;
+  constexpr int NS = DKP / 16, KS = DKP / 32, F = kKFrags<DKP>;
   using TK = HTile<DKP>;
   using TC = HTile<64>;
   constexpr int SE = DVB * DKP, YE = DVB * 64;   // elements of a part of S / dS and of delta / y
   static_assert(4 * SE + 4 * YE >= 2 * NP * TC::ELEMS, "the pair terms take the place of the states, delta and y");
-  __shared__ __align__(1024) f16 smem[4 * SE + 4 * YE + NP * TC::ELEMS + 2 * NP * TK::ELEMS];
-  f16 *sS = smem, *sN = sS + 2 * SE, *sY = sN + 2 * SE, *sD = sY + 2 * YE, *sO = sD + 2 * YE, *sKQ = sO + NP * TC::ELEMS;
+  __shared__ __align__(1024) f16 smem[4 * SE + 4 * YE + NP * TC::ELEMS + 2 * NP * F * FR];
+  f16 *sS = smem, *sN = sS + 2 * SE, *sY = sN + 2 * SE, *sD = sY + 2 * YE, *sO = sD + 2 * YE, *sK = sO + NP * TC::ELEMS, *sQ = sK + NP * F * FR;
   f16 *sXa = smem, *sXp = smem + NP * TC::ELEMS;                       // where those were
   __shared__ double sG[DC];
   __shared__ float sB[DC], sEG[DC], sEnd[DC], sRow[DC], sH[DC], sB2[DC], sCol[4][DC], red[4][4];
@@ -240,37 +338,30 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
   const int64_t unit = blockIdx.x;
   const int c = (int)(unit % p.pieces), bk = (int)(unit / p.pieces), hk = bk % p.kheads, b = bk / p.kheads;
   const int t0 = c * DC, len = min(DC, p.seqlen - t0), rep = p.heads / p.kheads;
-  {
-    const uint4* kq = reinterpret_cast<const uint4*>(p.workspace + lay.kq) + unit * (2 * NP * TK::ELEMS / 8);
-    for (int i = tid; i < 2 * NP * TK::ELEMS / 8; i += 256) reinterpret_cast<uint4*>(sKQ)[i] = kq[i];
-  }
-  const f16 *Kt = sKQ, *Qt = sKQ + NP * TK::ELEMS;
+  const f16* kq = reinterpret_cast<const f16*>(p.workspace + lay.kq + unit * lay.kq_unit);       // Q, K by rows
+  for (int i = tid; i < 2 * NP * F * 64; i += 256)                     // K, Q by columns
+    reinterpret_cast<f16x8*>(sK)[i] = reinterpret_cast<const f16x8*>(kq + 2 * NP * F * FR)[i];
   const float* vec0 = reinterpret_cast<const float*>(p.workspace + lay.vec) +
                       (((int64_t)b * p.heads + hk * rep) * p.pieces + c) * kVecFloats;
   const float sk = vec0[VEC_SK], sq = vec0[VEC_SQ];
   __syncthreads();
-  auto value = [&](const f16* t, int r, int col) {                     // K or Q without its scale
-    float v = (float)t[TK::at(r, col)];
-    if constexpr (NP == 2) v += (float)t[TK::ELEMS + TK::at(r, col)];
-    return v;
-  };
   f32x4 kk[4] = {}, qk[4] = {};
 #pragma unroll
   for (int s = 0; s < DKP / 32; ++s) {
     f16x8 ka[NP], qa[NP];
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
-      ka[n] = row_frag16<DKP>(Kt + n * TK::ELEMS, 16 * w, 32 * s, lane);
-      qa[n] = row_frag16<DKP>(Qt + n * TK::ELEMS, 16 * w, 32 * s, lane);
+      ka[n] = frag(kq, (NP + n) * F + w * KS + s, lane);
+      qa[n] = frag(kq, n * F + w * KS + s, lane);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (j > w) continue;
-      const f16x8 kb = row_frag16<DKP>(Kt, 16 * j, 32 * s, lane);
+      const f16x8 kb = frag(kq, NP * F + j * KS + s, lane);
       kk[j] = mma_h(ka[0], kb, kk[j]);
       qk[j] = mma_h(qa[0], kb, qk[j]);
       if constexpr (NP == 2) {
-        const f16x8 kl = row_frag16<DKP>(Kt + TK::ELEMS, 16 * j, 32 * s, lane);
+        const f16x8 kl = frag(kq, (NP + 1) * F + j * KS + s, lane);
         kk[j] = mma_h(ka[0], kl, kk[j]);
         kk[j] = mma_h(ka[1], kb, kk[j]);
         qk[j] = mma_h(qa[0], kl, qk[j]);
@@ -301,11 +392,10 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
       for (int j = 0; j < 8; ++j) om = fmaxf(om, fabsf(v[j]));
     }
     om = wave_max(om);
-    const float* scales = reinterpret_cast<const float*>(p.workspace + lay.scales) + vunit * nblk * 4;
-    float mx[4] = {};
-    for (int i = 0; i < nblk; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) mx[j] = fmaxf(mx[j], scales[4 * i + j]);
+    const float* scales = reinterpret_cast<const float*>(p.workspace + lay.scales) + vunit * nblk * 128;
+    float mx = 0.f;                              // lane 16 i + column: of scale i
+    for (int i = 0; i < 2 * nblk; ++i) mx = fmaxf(mx, scales[64 * i + lane]);
+    mx = row16_max(mx);
     __syncthreads();                             // the last head's use of the LDS is over
     if (lane == 0) red[w][0] = om;
     if (w == 0) {
@@ -323,23 +413,27 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
     }
     __syncthreads();
     const Scale so(fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0])));
-    const float mS = mx[KEEP_S], mN = mx[KEEP_DS], mD = mx[KEEP_D], mY = mx[KEEP_Y];
+    const float mS = lane_val(mx, 16 * KEEP_S), mN = lane_val(mx, 16 * KEEP_DS), mD = lane_val(mx, 16 * KEEP_D),
+                mY = lane_val(mx, 16 * KEEP_Y);
 
     f32x4 aq[NS] = {}, al[NS] = {}, ar[NS] = {}, pA[4] = {}, pP[4] = {};
     float dot = 0.f;                             // <S, dS>
     const f16* keep0 = reinterpret_cast<const f16*>(p.workspace + lay.keep) + vunit * nblk * (int64_t)keep_halfs<DKP>();
     for (int v0 = 0; v0 < 16 * nblk; v0 += DVB) {
       if (v0) __syncthreads();
+      // 16 columns of v at a time, a lane's 8 values of a k-step: rows 4 g .. and 16 + 4 g .. of 32, of column l % 16
       for (int u = tid; u < SE / 8; u += 256) {
-        const int r = u / (DKP / 8), c8 = u % (DKP / 8) * 8, blk = (v0 + r) / 16;
+        const int ln = u & 63, r = u / (16 * DKP / 8) * 16 + (ln & 15), k = u / 64 % (DKP / 32), blk = (v0 + r) / 16;
+        const int c = 32 * k + 4 * (ln >> 4);
         f16x8 s0 = {}, s1 = {}, n0 = {}, n1 = {};
         if (blk < nblk) {
-          const f16* from = keep0 + blk * (int64_t)keep_halfs<DKP>() + (r & 15) * DKP + c8;
-          s0 = *reinterpret_cast<const f16x8*>(from);
-          s1 = *reinterpret_cast<const f16x8*>(from + 16 * DKP);
-          n0 = *reinterpret_cast<const f16x8*>(from + 32 * DKP);
-          n1 = *reinterpret_cast<const f16x8*>(from + 48 * DKP);
-          const float fs = scales[4 * blk + KEEP_S], fn = scales[4 * blk + KEEP_DS];
+          const f16* from = keep0 + blk * (int64_t)keep_halfs<DKP>() + (k * 64 + ln) * 8;
+          s0 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_S));
+          s1 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_S) + 16 * DKP);
+          n0 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_DS));
+          n1 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_DS) + 16 * DKP);
+          const float* f = scales + 128 * blk + (k >= KS / 2 ? 64 : 0) + (r & 15);
+          const float fs = f[16 * KEEP_S], fn = f[16 * KEEP_DS];
           float d = 0.f;
 #pragma unroll
           for (int j = 0; j < 8; ++j) d += ((float)s0[j] + (float)s1[j]) * ((float)n0[j] + (float)n1[j]);
@@ -350,28 +444,27 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
           n0 *= hn;
           n1 *= hn;
         }
-        const int at = TK::at(r, c8);
-        *reinterpret_cast<f16x8*>(sS + at) = s0;
-        *reinterpret_cast<f16x8*>(sS + SE + at) = s1;
-        *reinterpret_cast<f16x8*>(sN + at) = n0;
-        *reinterpret_cast<f16x8*>(sN + SE + at) = n1;
+        put_halves<DKP>(sS, r, c, s0);
+        put_halves<DKP>(sS + SE, r, c, s1);
+        put_halves<DKP>(sN, r, c, n0);
+        put_halves<DKP>(sN + SE, r, c, n1);
       }
       for (int u = tid; u < YE / 8; u += 256) {
-        const int r = u / 8, c8 = u % 8 * 8, blk = (v0 + r) / 16;
+        const int ln = u & 63, r = u / 128 * 16 + (ln & 15), k = u / 64 % 2, blk = (v0 + r) / 16, c = 32 * k + 4 * (ln >> 4);
         f16x8 d0 = {}, d1 = {}, y0 = {}, y1 = {};
         if (blk < nblk) {
-          const f16* from = keep0 + blk * (int64_t)keep_halfs<DKP>() + 64 * DKP + (r & 15) * DC + c8;
-          const f16 hd = (f16)(scales[4 * blk + KEEP_D] / mD), hy = (f16)(scales[4 * blk + KEEP_Y] / mY);
-          d0 = *reinterpret_cast<const f16x8*>(from) * hd;
-          d1 = *reinterpret_cast<const f16x8*>(from + 16 * DC) * hd;
-          y0 = *reinterpret_cast<const f16x8*>(from + 32 * DC) * hy;
-          y1 = *reinterpret_cast<const f16x8*>(from + 48 * DC) * hy;
+          const f16* from = keep0 + blk * (int64_t)keep_halfs<DKP>() + (k * 64 + ln) * 8;
+          const float* f = scales + 128 * blk + 64 * k + (r & 15);
+          const f16 hd = (f16)(f[16 * KEEP_D] / mD), hy = (f16)(f[16 * KEEP_Y] / mY);
+          d0 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_D)) * hd;
+          d1 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_D) + 16 * DC) * hd;
+          y0 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_Y)) * hy;
+          y1 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_Y) + 16 * DC) * hy;
         }
-        const int at = TC::at(r, c8);
-        *reinterpret_cast<f16x8*>(sD + at) = d0;
-        *reinterpret_cast<f16x8*>(sD + YE + at) = d1;
-        *reinterpret_cast<f16x8*>(sY + at) = y0;
-        *reinterpret_cast<f16x8*>(sY + YE + at) = y1;
+        put_halves<64>(sD, r, c, d0);
+        put_halves<64>(sD + YE, r, c, d1);
+        put_halves<64>(sY, r, c, y0);
+        put_halves<64>(sY + YE, r, c, y1);
       }
       for (int u = tid; u < DC * DVB / 8; u += 256) {
         const int r = u / (DVB / 8), c8 = u % (DVB / 8) * 8;
@@ -460,23 +553,35 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
       red[w][3] = dot;
     }
     const float fq = p.scale * (so.inv * mS), fl = -(mY * mS), fr = mD * mN;
+    float dots[4] = {}, rights[4] = {};
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      // rows 16 w + 4 g + r of channel 16 n + l % 16: half of a fragment by columns
+      f16x8 kf[NP], qf[NP];
+#pragma unroll
+      for (int m = 0; m < NP; ++m) {
+        kf[m] = frag(sK, m * F + 2 * n + (w >> 1), lane);
+        qf[m] = frag(sQ, m * F + 2 * n + (w >> 1), lane);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int t = 16 * w + 4 * g4 + r;
+        float kv = (float)(w & 1 ? kf[0][4 + r] : kf[0][r]), qv = (float)(w & 1 ? qf[0][4 + r] : qf[0][r]);
+        if constexpr (NP == 2) {
+          kv += (float)(w & 1 ? kf[1][4 + r] : kf[1][r]);
+          qv += (float)(w & 1 ? qf[1][4 + r] : qf[1][r]);
+        }
+        const float q1 = aq[n][r] * (fq * sEG[t]), l1 = al[n][r] * (fl * sEG[t]), r1 = ar[n][r] * (fr * sEnd[t]);
+        dots[r] += sq * (qv * q1) + sk * (kv * l1);
+        rights[r] += kv * r1;
+        tq[n][r] += q1;
+        tk[n][r] += l1 + sB[t] * r1;
+      }
+    }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int t = 16 * w + 4 * g4 + r;
-      float dq = 0.f, dl = 0.f, dr = 0.f;
-#pragma unroll
-      for (int n = 0; n < NS; ++n) {
-        const float kv = value(Kt, t, 16 * n + l16), qv = value(Qt, t, 16 * n + l16);
-        aq[n][r] *= fq * sEG[t];
-        al[n][r] *= fl * sEG[t];
-        ar[n][r] *= fr * sEnd[t];
-        dq += qv * aq[n][r];
-        dl += kv * al[n][r];
-        dr += kv * ar[n][r];
-        tq[n][r] += aq[n][r];
-        tk[n][r] += al[n][r] + sB[t] * ar[n][r];
-      }
-      const float left = group_sum<16>(sq * dq + sk * dl + rows[r]), right = sk * group_sum<16>(dr);
+      const float left = group_sum<16>(dots[r] + rows[r]), right = sk * group_sum<16>(rights[r]);
       if (l16 == 0) {
         sRow[t] = left;
         sB2[t] = right;
@@ -532,14 +637,14 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
       f32x4 u1 = {}, u2 = {}, u3 = {};
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const f16x8 k0 = col_frag16<DKP>(Kt, 16 * n, 32 * s, lane), q0 = col_frag16<DKP>(Qt, 16 * n, 32 * s, lane);
+        const f16x8 k0 = frag(sK, 2 * n + s, lane), q0 = frag(sQ, 2 * n + s, lane);
         u1 = mma_h(rp[s][0], k0, u1);
         u2 = mma_h(ra[s][0], k0, u2);
         u2 = mma_h(ca[s][0], k0, u2);
         u3 = mma_h(cp[s][0], q0, u3);
         if constexpr (NP == 2) {
-          const f16x8 k1 = col_frag16<DKP>(Kt + TK::ELEMS, 16 * n, 32 * s, lane);
-          const f16x8 q1 = col_frag16<DKP>(Qt + TK::ELEMS, 16 * n, 32 * s, lane);
+          const f16x8 k1 = frag(sK, F + 2 * n + s, lane);
+          const f16x8 q1 = frag(sQ, F + 2 * n + s, lane);
           u1 = mma_h(rp[s][0], k1, u1);
           u1 = mma_h(rp[s][1], k0, u1);
           u2 = mma_h(ra[s][0], k1, u2);
@@ -575,9 +680,8 @@ template <typename T, int DKP>
 hipError_t run_bwd(const DeltaBwdParams& q, hipStream_t st) {
   const DeltaParams& p = q.f;
   const DeltaLayout lay(p, true);
-  constexpr int NW = 2;
-  const int nblk = (p.dv + 15) / 16, nwg = (nblk + NW - 1) / NW;
-  delta_back_scan_kernel<T, DKP, NW><<<head_block_grid(p.batch * p.heads, nwg), 64 * NW, 0, st>>>(q, lay, nblk, nwg);
+  const int nblk = (p.dv + 15) / 16, nwg = (nblk + 1) / 2;
+  delta_back_scan_kernel<T, DKP><<<head_block_grid(p.batch * p.heads, nwg), sizeof(T) == 4 ? 256 : 320, 0, st>>>(q, lay, nblk, nwg);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   delta_grads_kernel<T, DKP><<<(unsigned)((int64_t)p.batch * p.kheads * p.pieces), 256, 0, st>>>(q, lay, nblk);

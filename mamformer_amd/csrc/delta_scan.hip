@@ -18,7 +18,7 @@ namespace {
 // wave j builds block column j downwards, T_ij = -T_ii sum_k A_ik T_kj, with fp32 matrix instructions, T_kj staying in
 // accumulators, which are the B operand of the next product.
 template <typename T, int DKP>
-__global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p, DeltaLayout lay, int p_planes) {
+__global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p, DeltaLayout lay, int backward) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
   constexpr int CPR = DKP / 8;                   // threads of 8 channels for a row
   constexpr int RPP = 256 / CPR;                 // rows of a pass
@@ -82,8 +82,25 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p, DeltaLay
     }
   __syncthreads();
   {
-    uint4* out = reinterpret_cast<uint4*>(p.workspace + lay.kq) + unit * (2 * NP * TK::ELEMS / 8);
-    for (int i = tid; i < 2 * NP * TK::ELEMS / 8; i += 256) out[i] = reinterpret_cast<const uint4*>(tiles)[i];
+    constexpr int F = kKFrags<DKP>, KS = DKP / 32;
+    f16* out = reinterpret_cast<f16*>(p.workspace + lay.kq + unit * lay.kq_unit);
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+      const f16 *kt = tiles + n * TK::ELEMS, *qt = tiles + (NP + n) * TK::ELEMS;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {             // rows 16 w ..
+        put_frag(out, n * F + w * KS + s, lane, row_frag16<DKP>(qt, 16 * w, 32 * s, lane));
+        put_frag(out, (NP + n) * F + w * KS + s, lane, row_frag16<DKP>(kt, 16 * w, 32 * s, lane));
+      }
+#pragma unroll
+      for (int m = 0; m < DKP / 64; ++m)         // channels 16 (4 m + w) ..
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const int at = 2 * (4 * m + w) + s;
+          put_frag(out, (2 * NP + n) * F + at, lane, col_frag16<DKP>(kt, 16 * (4 * m + w), 32 * s, lane));
+          if (backward) put_frag(out, (3 * NP + n) * F + at, lane, col_frag16<DKP>(qt, 16 * (4 * m + w), 32 * s, lane));
+        }
+    }
   }
   // rows 16 w .. of K K^T and Q K^T, tiles j <= w
   f32x4 kk[4] = {}, qk[4] = {};
@@ -218,11 +235,25 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p, DeltaLay
         tiles[at] = th;
         tiles[TC::ELEMS + at] = part_lo(v, st.mult, th);
         tiles[2 * TC::ELEMS + pt] = ph;
-        if (p_planes == 2) tiles[3 * TC::ELEMS + pt] = part_lo(P[i][r], sp.mult, ph);
+        tiles[3 * TC::ELEMS + pt] = part_lo(P[i][r], sp.mult, ph);
       }
     __syncthreads();
-    uint4* out = reinterpret_cast<uint4*>(p.workspace + lay.tp) + vunit * (4 * TC::ELEMS / 8);
-    for (int i = tid; i < (2 + p_planes) * TC::ELEMS / 8; i += 256) out[i] = reinterpret_cast<const uint4*>(tiles)[i];
+    f16* out = reinterpret_cast<f16*>(p.workspace + lay.tp + vunit * lay.tp_unit);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {                // wave w: block row (or column) w
+      const f16 *tt = tiles + n * TC::ELEMS, *pt = tiles + (2 + n) * TC::ELEMS;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (w >= 2 * s) {
+          put_frag(out, n * kTFrags + t_frag(w, s), lane, row_frag16<64>(tt, 16 * w, 32 * s, lane));
+          if (!backward) put_frag(out, (2 + n) * kTFrags + t_frag(w, s), lane, row_frag16<64>(pt, 16 * w, 32 * s, lane));
+        }
+        if (backward && w < 2 + 2 * s) {
+          put_frag(out, (2 + n) * kTFrags + tt_frag(w, s), lane, col_frag16<64>(tt, 16 * w, 32 * s, lane));
+          put_frag(out, (4 + n) * kTFrags + tt_frag(w, s), lane, col_frag16<64>(pt, 16 * w, 32 * s, lane));
+        }
+      }
+    }
     float* vec = reinterpret_cast<float*>(p.workspace + lay.vec) + vunit * kVecFloats;
     if (tid < 2 * DC) vec[tid] = sVec[tid];
     if (tid == 2 * DC) {
@@ -236,215 +267,297 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p, DeltaLay
 }
 
 // ------------------------------------------------------------------ the state from piece to piece
-// A wave holds 16 columns of the state (dk x 16, fp32) and runs the whole recurrence for them without exchanging anything
-// with another; the NW waves of a workgroup read the same tiles, fetched by LDS DMA one piece ahead (NBUF = 2).
+// Two waves hold 16 columns of the state, half of its rows each (fp32), and half of a piece's tokens; a workgroup has two
+// such pairs, which read the same fragments, fetched by LDS DMA a piece ahead.  For a piece:
+//   each wave multiplies K (and Q) by its rows of S and gives the other its part of the other's tokens;   [barrier 1]
+//   R = V - e^G K S of its tokens; T is lower triangular, so that the second wave needs the first one's R;  [barrier 2]
+//   U = beta e^{G_end - G} delta of its tokens goes to the other, each adds K^T U to its rows.              [barrier 3]
 // KEEP: the entering states and delta are stored for the backward.  OUT: o is computed.
-template <typename T, int DKP, int NW, bool OUT, bool KEEP>
-__global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p, DeltaLayout lay, int nblk, int nwg) {
+//
+// Bound by the latency of one piece on waves that have a SIMD to themselves, most of it the conversions (an instruction of
+// 4 cycles for each value and part); b 2, H 16, L 4096 has 256 sets of 16 columns for 1024 SIMDs.
+template <typename T, int DKP, bool OUT, bool KEEP>
+__global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 320) void delta_scan_kernel(DeltaParams p, DeltaLayout lay, int nblk, int nwg) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
-  constexpr int NBUF = NP == 1 ? 2 : 1;
-  using TK = HTile<DKP>;
-  using TC = HTile<64>;
-  constexpr int KQ = (OUT ? 2 : 1) * NP * TK::ELEMS;                 // halfs of K (and Q)
-  constexpr int TP = (2 + (OUT ? NP : 0)) * TC::ELEMS;               // halfs of T (and P)
-  constexpr int BUF = KQ + TP + kVecFloats * 2;                      // halfs of a buffer
-  constexpr int NS = DKP / 16, KS = DKP / 32;
-  __shared__ __align__(1024) f16 smem[NBUF * BUF];
+  constexpr bool AHEAD = NP == 1;                // fp32: the fragments of a piece fill the LDS
+  constexpr int FW = AHEAD ? 1 : 4;              // waves that fetch: the fifth, or all four
+  constexpr int KS = DKP / 32, KSH = KS / 2, NSH = DKP / 32, F = kKFrags<DKP>;
+  constexpr int GA = (OUT ? 2 : 1) * NP * F;                         // fragments of (Q and) K by rows: before barrier 1
+  constexpr int TPF = OUT ? (NP == 1 ? 20 : 24) : 12;                // of T (and P; two beyond it)
+  constexpr int GB = NP * F + TPF + 1;                               // with K by columns and vec: after it
+  constexpr int XF = OUT ? 4 : 2, DF = OUT ? NP : 0;
+  constexpr int EX = (2 * XF + 2 + 4 + DF + 1) * FR;                 // halfs of a pair's exchange
+  __shared__ __align__(1024) f16 smem[(GA + (AHEAD ? 2 : 1) * GB) * FR + 2 * EX];
 
-  const int lane = threadIdx.x & 63, w = wave_id(), l16 = lane & 15, g4 = lane >> 4;
+  const int lane = threadIdx.x & 63, w = wave_id(), l16 = lane & 15, g4 = lane >> 4, hf = w & 1;
   int bh, wg;
   if (!head_block(blockIdx.x, p.batch * p.heads, nwg, bh, wg)) return;
   const int b = bh / p.heads, h = bh % p.heads, hk = h / (p.heads / p.kheads);
-  const int blk = wg * NW + w, col = 16 * blk + l16;
-  const bool live = blk < nblk, cv = col < p.dv;
+  const int blk = 2 * wg + (w >> 1), col = 16 * blk + l16;
+  const bool live = blk < nblk, cv = col < p.dv, all_cv = 16 * blk + 16 <= p.dv;
   const int64_t kunit0 = ((int64_t)b * p.kheads + hk) * p.pieces, vunit0 = (int64_t)bh * p.pieces;
 
-  auto fetch = [&](int c, int buf) {             // 1 KB blocks, the waves in turn
-    char* to = reinterpret_cast<char*>(smem + buf * BUF);
-    const char* kq = p.workspace + lay.kq + (kunit0 + c) * (int64_t)(2 * NP * TK::ELEMS * 2);
-    const char* tp = p.workspace + lay.tp + (vunit0 + c) * (int64_t)(4 * TC::ELEMS * 2);
-    const char* vec = p.workspace + lay.vec + (vunit0 + c) * (int64_t)(kVecFloats * 4);
-#pragma unroll
-    for (int q = w; q < KQ / 512; q += NW) dma_lds<16>(kq + q * 1024, 16u * lane, to + q * 1024);
-#pragma unroll
-    for (int q = w; q < TP / 512; q += NW) dma_lds<16>(tp + q * 1024, 16u * lane, to + KQ * 2 + q * 1024);
-    if (w == 0) dma_lds<16>(vec, 16u * lane, to + (KQ + TP) * 2);
-  };
+  f16* ex = smem + (GA + (AHEAD ? 2 : 1) * GB) * FR + (w >> 1) * EX;
+  f32x4* const xSend = reinterpret_cast<f32x4*>(ex) + hf * XF * 64 + lane;             // X (and Y) of the other's tokens
+  const f32x4* const xRecv = reinterpret_cast<const f32x4*>(ex) + (1 - hf) * XF * 64 + lane;
+  f16* const eR = ex + 2 * XF * FR;                                                    // the first half's R
+  f16* const eU = eR + 2 * FR;                                                         // U, two parts of each half
+  f16* const eD = eU + 4 * FR;                                                         // the first half's delta
+  float* const eS = reinterpret_cast<float*>(eD + DF * FR);                            // scales: R, D, U of each half
 
-  f32x4 S[NS];                                   // rows 16 n + 4 g4 + r, column col
+  const int fw = AHEAD ? 0 : w;
+  auto fetch_a = [&](int c) { fetch_share<GA, FW>(smem, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + (OUT ? 0 : NP * F * 1024), fw, lane); };
+  auto fetch_b = [&](int c) {
+    f16* to = smem + (GA + (AHEAD ? (c & 1) * GB : 0)) * FR;
+    fetch_share<NP * F, FW>(to, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + 2 * NP * F * 1024, fw, lane);
+    fetch_share<TPF, FW>(to + NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit, fw, lane);
+    if (fw == 0) dma_lds<16>(p.workspace + lay.vec + (vunit0 + c) * (int64_t)(kVecFloats * 4), 16u * lane, to + (NP * F + TPF) * FR);
+  };
+  if constexpr (AHEAD) if (w == 4) {
+    // the fifth wave fetches: a wave that issues these loads stands still while they drain
+    fetch_a(0);
+    fetch_b(0);
+    wait_vmem_n<GB>();
+    lds_barrier();
+    for (int c = 0; c < p.pieces; ++c) {
+      const bool more = c + 1 < p.pieces;
+      wait_vmem();                               // T, P and K by columns of this piece
+      lds_barrier();                             // 1
+      if (more) fetch_a(c + 1);                  // where the last ones have been read
+      lds_barrier();                             // 2
+      if (more) {
+        fetch_b(c + 1);
+        wait_vmem_n<GB>();
+      }
+      lds_barrier();                             // 3
+    }
+    return;
+  }
+
+  f32x4 S[NSH];                                  // rows DKP / 2 hf + 16 n + 4 g4 + r, column col
 #pragma unroll
-  for (int n = 0; n < NS; ++n)
+  for (int n = 0; n < NSH; ++n)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int row = 16 * n + 4 * g4 + r;
+      const int row = DKP / 2 * hf + 16 * n + 4 * g4 + r;
       S[n][r] = p.initial_state && cv && row < p.dk ? p.initial_state[((int64_t)bh * p.dk + row) * p.dv + col] : 0.f;
     }
-  const T* vsrc = reinterpret_cast<const T*>(p.v) + b * p.vs.b + h * p.vs.h + col;
-  T vn[16];
-  auto load_v = [&](int c) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int t = c * DC + 16 * (i >> 2) + 4 * g4 + (i & 3);
-      vn[i] = cv && t < p.seqlen ? vsrc[(int64_t)t * p.vs.l] : from_f32<T>(0.f);
-    }
+  const T* vsrc = reinterpret_cast<const T*>(p.v) + b * p.vs.b + h * p.vs.h + 16 * blk;
+  T vn[8];
+  auto load_v = [&](int c) {                     // a half that lies beyond the sequence reads the last token
+    const int t = min(c * DC + 32 * hf, p.seqlen - 1);
+    load_rows8<T>(vsrc + t * p.vs.l, p.vs.l, p.seqlen - t, cv, all_cv, l16, g4, vn);
   };
-  load_v(0);
-  if (NBUF == 2) fetch(0, 0);
+  if (live) load_v(0);
+  if (AHEAD) lds_barrier();
 
   for (int c = 0; c < p.pieces; ++c) {
-    const f16* buf = smem + (NBUF == 2 ? (c & 1) * BUF : 0);
-    if (NBUF == 2) {
+    if (!AHEAD) {
+      lds_barrier();
+      fetch_a(c);
+      fetch_b(c);
       wait_vmem();
-      __syncthreads();                           // the piece has arrived, the other buffer has been read
-      if (c + 1 < p.pieces) fetch(c + 1, (c + 1) & 1);
-    } else {
-      __syncthreads();
-      fetch(c, 0);
-      wait_vmem();
-      __syncthreads();
+      lds_barrier();
     }
-    if (!live) continue;
-    const f16 *Kt = buf, *Qt = buf + NP * TK::ELEMS, *Tt = buf + KQ, *Pt = Tt + 2 * TC::ELEMS;
-    const float* vec = reinterpret_cast<const float*>(buf + KQ + TP);
-    f32x4 R[4];
+    const f16 *Qr = smem, *Kr = Qr + (OUT ? NP * F * FR : 0);
+    const f16 *Kc = smem + (GA + (AHEAD ? (c & 1) * GB : 0)) * FR, *Tt = Kc + NP * F * FR, *Pt = Tt + 2 * kTFrags * FR;
+    const float* vec = reinterpret_cast<const float*>(Tt + TPF * FR);
+    f16x8 sh[KSH], sl[KSH];
+    f32x4 X[2] = {}, Y[2] = {};                  // of one's own tokens
+    float ss_inv = 0.f;
+    if (live) {
+      f16x8 ka[KSH][4];                          // tiles 0, 1: one's own tokens, 2, 3: the other's
 #pragma unroll
-    for (int i = 0; i < 16; ++i) R[i >> 2][i & 3] = to_f32(vn[i]);
-    if (c + 1 < p.pieces) load_v(c + 1);
-
-    f16x8 sh[KS], sl[KS];
-    const Scale ss(wave_max(abs_max(S)));
-    parts_of<2>(S, ss.mult, sh, sl);
-    f16* keep = nullptr;
-    float* scales = nullptr;
-    if constexpr (KEEP) {
-      const int64_t at = (vunit0 + c) * nblk + blk;
-      keep = reinterpret_cast<f16*>(p.workspace + lay.keep) + at * (int64_t)keep_halfs<DKP>();
-      scales = reinterpret_cast<float*>(p.workspace + lay.scales) + at * 4;
+      for (int s = 0; s < KSH; ++s)
 #pragma unroll
-      for (int n = 0; n < NS; ++n) {             // [column][row]: 4 rows of a column a lane
-        f16* to = keep + l16 * DKP + 16 * n + 4 * g4;
-        *reinterpret_cast<f16x4*>(to) = n & 1 ? __builtin_shufflevector(sh[n >> 1], sh[n >> 1], 4, 5, 6, 7)
-                                              : __builtin_shufflevector(sh[n >> 1], sh[n >> 1], 0, 1, 2, 3);
-        *reinterpret_cast<f16x4*>(to + 16 * DKP) = n & 1 ? __builtin_shufflevector(sl[n >> 1], sl[n >> 1], 4, 5, 6, 7)
-                                                         : __builtin_shufflevector(sl[n >> 1], sl[n >> 1], 0, 1, 2, 3);
-      }
-      if (lane == 0) scales[KEEP_S] = ss.inv;
-    }
-    // K S, and Q S for the output
-    f32x4 X[4] = {}, Y[4] = {};
+        for (int i = 0; i < 4; ++i) ka[s][i] = frag(Kr, ((2 * hf + i) & 3) * KS + hf * KSH + s, lane);
+      const Scale ss(col_max(abs_max(S)));
+      ss_inv = ss.inv;
+      parts_of<2>(S, ss.mult, sh, sl);
+      f32x4 XO[2] = {}, YO[2] = {};
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+      for (int s = 0; s < KSH; ++s) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f16x8 a = row_frag16<DKP>(Kt, 16 * i, 32 * s, lane);
-        X[i] = mma_h(a, sh[s], X[i]);
-        X[i] = mma_h(a, sl[s], X[i]);
-        if constexpr (NP == 2) X[i] = mma_h(row_frag16<DKP>(Kt + TK::ELEMS, 16 * i, 32 * s, lane), sh[s], X[i]);
-        if constexpr (OUT) {
-          const f16x8 q = row_frag16<DKP>(Qt, 16 * i, 32 * s, lane);
-          Y[i] = mma_h(q, sh[s], Y[i]);          // o is rounded to T: one part is enough for bf16
-          if constexpr (NP == 2) {
-            Y[i] = mma_h(q, sl[s], Y[i]);
-            Y[i] = mma_h(row_frag16<DKP>(Qt + TK::ELEMS, 16 * i, 32 * s, lane), sh[s], Y[i]);
-          }
-        }
-      }
-    const float xs = ss.inv * vec[VEC_SK];
-    f32x4 eg[4];
+        for (int i = 0; i < 4; ++i) (i < 2 ? X[i & 1] : XO[i & 1]) = mma_h(ka[s][i], sh[s], i < 2 ? X[i & 1] : XO[i & 1]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      eg[i] = *reinterpret_cast<const f32x4*>(vec + 16 * i + 4 * g4);
+        for (int i = 0; i < 4; ++i) (i < 2 ? X[i & 1] : XO[i & 1]) = mma_h(ka[s][i], sl[s], i < 2 ? X[i & 1] : XO[i & 1]);
+        if constexpr (NP == 2)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) R[i][r] -= eg[i][r] * (xs * X[i][r]);
-    }
-    // delta = T R; T is lower triangular
-    f16x8 rh[2], rl[2];
-    const Scale sr(wave_max(abs_max(R)));
-    parts_of<2>(R, sr.mult, rh, rl);
-    f32x4 D[4] = {};
+          for (int i = 0; i < 4; ++i)
+            (i < 2 ? X[i & 1] : XO[i & 1]) = mma_h(frag(Kr, F + ((2 * hf + i) & 3) * KS + hf * KSH + s, lane), sh[s], i < 2 ? X[i & 1] : XO[i & 1]);
+        if constexpr (OUT)                       // o is rounded to T: one part of the state is enough for bf16
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int i = 2 * s; i < 4; ++i) {
-        const f16x8 a = row_frag16<64>(Tt, 16 * i, 32 * s, lane);
-        D[i] = mma_h(a, rh[s], D[i]);
-        D[i] = mma_h(a, rl[s], D[i]);
-        D[i] = mma_h(row_frag16<64>(Tt + TC::ELEMS, 16 * i, 32 * s, lane), rh[s], D[i]);
-      }
-    const float ds = sr.inv * vec[VEC_ST];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) D[i][r] *= ds;
-    if constexpr (OUT || KEEP) {
-      f16x8 dh[2], dl[2];
-      const Scale sd(wave_max(abs_max(D)));
-      parts_of<(KEEP || NP == 2) ? 2 : 1>(D, sd.mult, dh, dl);
-      if constexpr (KEEP) {
-        f16* to = keep + 2 * (2 * 16 * DKP) + l16 * DC + 4 * g4;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          *reinterpret_cast<f16x4*>(to + 16 * n) = n & 1 ? __builtin_shufflevector(dh[n >> 1], dh[n >> 1], 4, 5, 6, 7)
-                                                         : __builtin_shufflevector(dh[n >> 1], dh[n >> 1], 0, 1, 2, 3);
-          *reinterpret_cast<f16x4*>(to + 16 * DC + 16 * n) = n & 1 ? __builtin_shufflevector(dl[n >> 1], dl[n >> 1], 4, 5, 6, 7)
-                                                                   : __builtin_shufflevector(dl[n >> 1], dl[n >> 1], 0, 1, 2, 3);
-        }
-        if (lane == 0) scales[KEEP_D] = sd.inv;
-      }
-      if constexpr (OUT) {
-        f32x4 O[4] = {};
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int i = 2 * s; i < 4; ++i) {
-            const f16x8 a = row_frag16<64>(Pt, 16 * i, 32 * s, lane);
-            O[i] = mma_h(a, dh[s], O[i]);
+          for (int i = 0; i < 4; ++i) {
+            f32x4& y = i < 2 ? Y[i & 1] : YO[i & 1];
+            const f16x8 q = frag(Qr, ((2 * hf + i) & 3) * KS + hf * KSH + s, lane);
+            y = mma_h(q, sh[s], y);
             if constexpr (NP == 2) {
-              O[i] = mma_h(a, dl[s], O[i]);
-              O[i] = mma_h(row_frag16<64>(Pt + TC::ELEMS, 16 * i, 32 * s, lane), dh[s], O[i]);
+              y = mma_h(q, sl[s], y);
+              y = mma_h(frag(Qr, F + ((2 * hf + i) & 3) * KS + hf * KSH + s, lane), sh[s], y);
             }
           }
-        const float ys = ss.inv * vec[VEC_SQ], os = sd.inv * vec[VEC_SP];
-        T* out = reinterpret_cast<T*>(p.o) + b * p.os.b + h * p.os.h + col;
+      }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int t = c * DC + 16 * (i >> 2) + 4 * g4 + (i & 3);
-          const float o = p.scale * (eg[i >> 2][i & 3] * (ys * Y[i >> 2][i & 3]) + os * O[i >> 2][i & 3]);
-          if (cv && t < p.seqlen) out[(int64_t)t * p.os.l] = from_f32<T>(o);
+      for (int i = 0; i < 2; ++i) {
+        xSend[i * 64] = XO[i] * ss_inv;
+        if constexpr (OUT) xSend[(2 + i) * 64] = YO[i] * ss_inv;
+      }
+    }
+    lds_barrier();                               // 1
+    f32x4 R[2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) R[i >> 2][i & 3] = to_f32(vn[i]);
+    if (live && c + 1 < p.pieces) load_v(c + 1);
+    f32x4 eg[2], D[2] = {}, E[2] = {};
+    float rs = 0.f;
+    if (live) {
+      const float sK = vec[VEC_SK];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        eg[i] = *reinterpret_cast<const f32x4*>(vec + 32 * hf + 16 * i + 4 * g4);
+        const f32x4 xr = xRecv[i * 64];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) R[i][r] -= eg[i][r] * (sK * (ss_inv * X[i][r] + xr[r]));
+      }
+      // delta = T R: one's own tokens, and for the second wave those of the first
+      f16x8 rh[1], rl[1];
+      const Scale sr(col_max(abs_max(R)));
+      rs = sr.inv;
+      parts_of<2>(R, sr.mult, rh, rl);
+      if (hf == 0) {
+        put_frag(eR, 0, lane, rh[0]);
+        put_frag(eR, 1, lane, rl[0]);
+        eS[lane] = rs;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const f16x8 a = frag(Tt, t_frag(2 * hf + i, hf), lane), a1 = frag(Tt, kTFrags + t_frag(2 * hf + i, hf), lane);
+        D[i] = mma_h(a, rh[0], D[i]);
+        D[i] = mma_h(a, rl[0], D[i]);
+        D[i] = mma_h(a1, rh[0], D[i]);
+      }
+    }
+    lds_barrier();                               // 2
+    f32x4 U[2];
+    float own_us = 0.f;
+    f16x8 wh[1], wl[1], dh[1], dl[1];
+    Scale sd(0.f);
+    if (live) {
+      if (hf == 1) {
+        const f16x8 r0 = frag(eR, 0, lane), r1 = frag(eR, 1, lane);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const f16x8 a = frag(Tt, t_frag(2 + i, 0), lane), a1 = frag(Tt, kTFrags + t_frag(2 + i, 0), lane);
+          E[i] = mma_h(a, r0, E[i]);
+          E[i] = mma_h(a, r1, E[i]);
+          E[i] = mma_h(a1, r0, E[i]);
+        }
+        const float es = eS[lane];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) D[i][r] = rs * D[i][r] + es * E[i][r];
+        rs = 1.f;
+      }
+      const float ds = rs * vec[VEC_ST];         // of D, and of U until it leaves its own scale
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const f32x4 wt = *reinterpret_cast<const f32x4*>(vec + VEC_W + 32 * hf + 16 * i + 4 * g4);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) U[i][r] = wt[r] * D[i][r];
+      }
+      const Scale su(col_max(abs_max(U)));
+      parts_of<2>(U, su.mult, wh, wl);
+      own_us = su.inv * ds * vec[VEC_SK];
+      put_frag(eU, 2 * hf, lane, wh[0]);
+      put_frag(eU, 2 * hf + 1, lane, wl[0]);
+      eS[(2 + hf) * 64 + lane] = own_us;
+      sd = Scale(col_max(abs_max(D)));
+      parts_of<(KEEP || NP == 2) ? 2 : 1>(D, sd.mult, dh, dl);
+      sd.inv *= ds;
+      if constexpr (OUT)
+        if (hf == 0) {
+          put_frag(eD, 0, lane, dh[0]);
+          if constexpr (NP == 2) put_frag(eD, 1, lane, dl[0]);
+          eS[64 + lane] = sd.inv;
+        }
+    }
+    lds_barrier();                               // 3
+    if (!live) continue;
+    {
+      const f16x8 oh = frag(eU, 2 - 2 * hf, lane), ol = frag(eU, 3 - 2 * hf, lane);
+      const float gamma = vec[VEC_GAMMA], other_us = eS[(3 - hf) * 64 + lane];
+#pragma unroll
+      for (int n = 0; n < NSH; ++n) {
+        const f16x8 a = frag(Kc, 2 * (hf * NSH + n) + hf, lane), o = frag(Kc, 2 * (hf * NSH + n) + 1 - hf, lane);
+        f32x4 u0 = {}, u1 = {};
+        u0 = mma_h(a, wh[0], u0);
+        u1 = mma_h(o, oh, u1);
+        u0 = mma_h(a, wl[0], u0);
+        u1 = mma_h(o, ol, u1);
+        if constexpr (NP == 2) {
+          u0 = mma_h(frag(Kc, F + 2 * (hf * NSH + n) + hf, lane), wh[0], u0);
+          u1 = mma_h(frag(Kc, F + 2 * (hf * NSH + n) + 1 - hf, lane), oh, u1);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[n][r] = gamma * S[n][r] + own_us * u0[r] + other_us * u1[r];
+      }
+    }
+    if constexpr (KEEP) {
+      const int64_t at = (vunit0 + c) * nblk + blk;
+      f16* keep = reinterpret_cast<f16*>(p.workspace + lay.keep) + at * (int64_t)keep_halfs<DKP>();
+      float* scales = reinterpret_cast<float*>(p.workspace + lay.scales) + at * 128 + 64 * hf + l16;
+      keep_parts<KS>(keep + keep_at<DKP>(KEEP_S), hf * KSH, sh, sl, lane);
+      keep_parts<2>(keep + keep_at<DKP>(KEEP_D), hf, dh, dl, lane);
+      if (g4 == 0) {
+        scales[16 * KEEP_S] = ss_inv;
+        scales[16 * KEEP_D] = sd.inv;
+      }
+    }
+    if constexpr (OUT) {
+      f32x4 O[2] = {}, O0[2] = {};
+      float o0 = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const f16x8 a = frag(Pt, t_frag(2 * hf + i, hf), lane);
+        O[i] = mma_h(a, dh[0], O[i]);
+        if constexpr (NP == 2) {
+          O[i] = mma_h(a, dl[0], O[i]);
+          O[i] = mma_h(frag(Pt, kTFrags + t_frag(2 * hf + i, hf), lane), dh[0], O[i]);
         }
       }
-    }
-    // the state behind the piece
+      if (hf == 1) {
+        const f16x8 d0 = frag(eD, 0, lane);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x4 wt = *reinterpret_cast<const f32x4*>(vec + VEC_W + 16 * i + 4 * g4);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) D[i][r] *= wt[r];
-    }
-    f16x8 wh[2], wl[2];
-    const Scale sw(wave_max(abs_max(D)));
-    parts_of<2>(D, sw.mult, wh, wl);
-    const float gamma = vec[VEC_GAMMA], us = sw.inv * vec[VEC_SK];
-#pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      f32x4 u = {};
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const f16x8 a = col_frag16<DKP>(Kt, 16 * n, 32 * s, lane);
-        u = mma_h(a, wh[s], u);
-        u = mma_h(a, wl[s], u);
-        if constexpr (NP == 2) u = mma_h(col_frag16<DKP>(Kt + TK::ELEMS, 16 * n, 32 * s, lane), wh[s], u);
+        for (int i = 0; i < 2; ++i) {
+          const f16x8 a = frag(Pt, t_frag(2 + i, 0), lane);
+          O0[i] = mma_h(a, d0, O0[i]);
+          if constexpr (NP == 2) {
+            O0[i] = mma_h(a, frag(eD, 1, lane), O0[i]);
+            O0[i] = mma_h(frag(Pt, kTFrags + t_frag(2 + i, 0), lane), d0, O0[i]);
+          }
+        }
+        o0 = p.scale * (eS[64 + lane] * vec[VEC_SP]);
       }
+      const float yq = p.scale * vec[VEC_SQ], os = p.scale * (sd.inv * vec[VEC_SP]);
+      float o[8];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) S[n][r] = gamma * S[n][r] + us * u[r];
+      for (int i = 0; i < 2; ++i) {
+        const f32x4 yr = xRecv[(2 + i) * 64];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          o[4 * i + r] = eg[i][r] * (yq * (ss_inv * Y[i][r] + yr[r])) + (os * O[i][r] + o0 * O0[i][r]);
+      }
+      const int t = c * DC + 32 * hf;
+      store_rows8<T>(reinterpret_cast<T*>(p.o) + b * p.os.b + h * p.os.h + t * p.os.l + 16 * blk, p.os.l, p.seqlen - t, cv, l16, g4, o);
     }
   }
   if (p.final_state && live && cv) {
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
+    for (int n = 0; n < NSH; ++n)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int row = 16 * n + 4 * g4 + r;
+        const int row = DKP / 2 * hf + 16 * n + 4 * g4 + r;
         if (row < p.dk) p.final_state[((int64_t)bh * p.dk + row) * p.dv + col] = S[n][r];
       }
   }
@@ -452,18 +565,16 @@ __global__ __launch_bounds__(64 * NW) void delta_scan_kernel(DeltaParams p, Delt
 
 template <typename T, int DKP, bool OUT, bool KEEP>
 hipError_t launch_scan(const DeltaParams& p, const DeltaLayout& lay, hipStream_t st) {
-  constexpr int NW = 2;
-  const int nblk = (p.dv + 15) / 16, nwg = (nblk + NW - 1) / NW;
-  delta_scan_kernel<T, DKP, NW, OUT, KEEP><<<head_block_grid(p.batch * p.heads, nwg), 64 * NW, 0, st>>>(p, lay, nblk, nwg);
+  const int nblk = (p.dv + 15) / 16, nwg = (nblk + 1) / 2;
+  delta_scan_kernel<T, DKP, OUT, KEEP><<<head_block_grid(p.batch * p.heads, nwg), sizeof(T) == 4 ? 256 : 320, 0, st>>>(p, lay, nblk, nwg);
   return hipGetLastError();
 }
 
 template <typename T>
 hipError_t run_prep(const DeltaParams& p, const DeltaLayout& lay, bool backward, hipStream_t st) {
   const unsigned grid = (unsigned)((int64_t)p.batch * p.kheads * p.pieces);
-  const int planes = sizeof(T) == 4 || backward ? 2 : 1;
-  if (p.dk <= 64) delta_prep_kernel<T, 64><<<grid, 256, 0, st>>>(p, lay, planes);
-  else delta_prep_kernel<T, 128><<<grid, 256, 0, st>>>(p, lay, planes);
+  if (p.dk <= 64) delta_prep_kernel<T, 64><<<grid, 256, 0, st>>>(p, lay, backward);
+  else delta_prep_kernel<T, 128><<<grid, 256, 0, st>>>(p, lay, backward);
   return hipGetLastError();
 }
 
