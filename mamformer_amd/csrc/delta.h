@@ -185,15 +185,17 @@ struct DeltaLayout {
 };
 
 // N fragments by LDS DMA, wave w of NW taking N / NW in a row.
+typedef __attribute__((address_space(3))) f16 lds_f16_t;
 template <int N, int NW>
-__device__ __forceinline__ void fetch_share(f16* to, const char* from, int w, int lane) {
+__device__ __forceinline__ void fetch_share(lds_f16_t* to, const char* from, int w, int lane) {
   static_assert(N % NW == 0, "equal shares");
   const char* src = from + w * (N / NW) * 1024;
-  f16* dst = to + w * (N / NW) * FR;
+  lds_f16_t* dst = to + w * (N / NW) * FR;
   uint32_t off = 16u * lane;
   asm volatile("" : "+v"(off));                  // 32 bits beside a scalar base, not a 64-bit address held for the loop
 #pragma unroll
-  for (int i = 0; i < N / NW; ++i) dma_lds<16>(src + i * 1024, off, dst + i * FR);
+  for (int i = 0; i < N / NW; ++i)
+    __builtin_amdgcn_global_load_lds((glb_void_t*)(src + i * 1024 + off), (lds_void_t*)(dst + i * FR), 16, 0, 0);
 }
 
 // 32 rows of 16 columns in the accumulators' order: v[i] is row 16 (i / 4) + 4 g + i % 4 of column l % 16.  `at` is the
@@ -233,6 +235,43 @@ __device__ __forceinline__ void store_rows8(T* at, int64_t stride, int len, bool
     }
   }
 }
+
+// 32 columns of a piece's rows by a wave that does nothing else, a token a lane, to and from LDS by columns
+// ([column][token]), where the waves that compute read and write 4 tokens of a column at once.
+constexpr int IO_COLS = 32, IO_PITCH = 68;       // 34 banks a column: 16 columns of 8 bytes meet every bank once
+constexpr int IO_HALFS = IO_COLS * IO_PITCH;
+struct IoRows {
+  bf16x8 v[IO_COLS / 8];
+  // `at`: column 0 of the lane's token, of which `left` columns exist
+  __device__ __forceinline__ void load(const bf16* at, bool row, int left) {
+#pragma unroll
+    for (int i = 0; i < IO_COLS / 8; ++i) {
+      Raw8<bf16> r;
+      r.clear();
+      if (row && left > 8 * i) load_raw(r, at + 8 * i, left - 8 * i);
+      v[i] = r.v;
+    }
+  }
+  __device__ __forceinline__ void store(bf16* at, bool row, int left) const {
+#pragma unroll
+    for (int i = 0; i < IO_COLS / 8; ++i) {
+      if (!row || left <= 8 * i) continue;
+      if (left >= 8 * i + 8) put_vec<false>(at + 8 * i, v[i]);
+      else
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (8 * i + j < left) at[8 * i + j] = v[i][j];
+    }
+  }
+  __device__ __forceinline__ void to_lds(bf16* t, int lane) const {
+#pragma unroll
+    for (int c = 0; c < IO_COLS; ++c) t[c * IO_PITCH + lane] = v[c / 8][c % 8];
+  }
+  __device__ __forceinline__ void from_lds(const bf16* t, int lane) {
+#pragma unroll
+    for (int c = 0; c < IO_COLS; ++c) v[c / 8][c % 8] = t[c * IO_PITCH + lane];
+  }
+};
 
 // Workgroup n of heads x blocks, with the blocks of a head on one XCD (workgroups go to the 8 XCDs in turn): they share the
 // head's tiles through its L2.  False beyond the last head.

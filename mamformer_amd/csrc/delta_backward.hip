@@ -18,9 +18,10 @@ namespace mh {
 namespace {
 
 // Two waves hold the gradient of 16 columns of the state as the forward's scan holds the state: half of its rows and half of
-// a piece's tokens each.  y = T^T ddelta is upper triangular, so that here the first wave needs the second one's ddelta.
+// a piece's tokens each, with a fifth and a sixth wave that fetch.  y = T^T ddelta is upper triangular, so that here the
+// first wave needs the second one's ddelta.
 template <typename T, int DKP>
-__global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 320) void delta_back_scan_kernel(DeltaBwdParams q, DeltaLayout lay, int nblk, int nwg) {
+__global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_back_scan_kernel(DeltaBwdParams q, DeltaLayout lay, int nblk, int nwg) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
   constexpr bool AHEAD = NP == 1;
   constexpr int FW = AHEAD ? 1 : 4;
@@ -28,53 +29,78 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 320) void delta_back_scan_ke
   constexpr int GA = NP * F + 2 * kTFrags;                           // fragments of K by rows and P by columns: before barrier 1
   constexpr int GB = 2 * NP * F + 2 * kTFrags + 1;                   // K and Q by columns, T by columns, vec: after it
   constexpr int EX = (2 * 2 + 2 + 2 * 4 + 1) * FR;                   // halfs of a pair's exchange
-  __shared__ __align__(1024) f16 smem[(GA + (AHEAD ? 2 : 1) * GB) * FR + 2 * EX];
+  constexpr int IO = AHEAD ? 2 * IO_HALFS : 0;
+  __shared__ __align__(1024) f16 smem[(GA + (AHEAD ? 2 : 1) * GB) * FR + 2 * EX + IO];
   const DeltaParams& p = q.f;
 
   const int lane = threadIdx.x & 63, w = wave_id(), l16 = lane & 15, g4 = lane >> 4, hf = w & 1;
   int bh, wg;
   if (!head_block(blockIdx.x, p.batch * p.heads, nwg, bh, wg)) return;
   const int b = bh / p.heads, h = bh % p.heads, hk = h / (p.heads / p.kheads);
-  const int blk = 2 * wg + (w >> 1), col = 16 * blk + l16;
-  const bool live = blk < nblk, cv = col < p.dv, all_cv = 16 * blk + 16 <= p.dv;
   const int64_t kunit0 = ((int64_t)b * p.kheads + hk) * p.pieces, vunit0 = (int64_t)bh * p.pieces;
+  constexpr int DOUT = (GA + (AHEAD ? 2 : 1) * GB) * FR + 2 * EX;    // where dO of two pieces is
 
+  const int fw = AHEAD ? 0 : w;
+  lds_f16_t* const lds = (lds_f16_t*)smem;
+  auto fetch_a = [&](int c) {
+    fetch_share<NP * F, FW>(lds, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + NP * F * 1024, fw, lane);
+    fetch_share<2 * kTFrags, FW>(lds + NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit + 4 * kTFrags * 1024, fw, lane);
+  };
+  auto fetch_b = [&](int c) {
+    lds_f16_t* to = lds + (GA + (AHEAD ? (c & 1) * GB : 0)) * FR;
+    fetch_share<2 * NP * F, FW>(to, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + 2 * NP * F * 1024, fw, lane);
+    fetch_share<2 * kTFrags, FW>(to + 2 * NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit + 2 * kTFrags * 1024, fw, lane);
+    if (fw == 0) fetch_share<1, 1>(to + (2 * NP * F + 2 * kTFrags) * FR, p.workspace + lay.vec + (vunit0 + c) * (int64_t)(kVecFloats * 4), 0, lane);
+  };
+  if constexpr (AHEAD) {
+    if (w == 4) {
+      fetch_a(p.pieces - 1);
+      fetch_b(p.pieces - 1);
+      wait_vmem_n<GB>();
+      lds_barrier();
+      for (int c = p.pieces - 1; c >= 0; --c) {
+        wait_vmem();
+        lds_barrier();                           // 1
+        if (c > 0) fetch_a(c - 1);
+        lds_barrier();                           // 2
+        if (c > 0) {
+          fetch_b(c - 1);
+          wait_vmem_n<GB>();
+        }
+        lds_barrier();                           // 3
+      }
+      return;
+    }
+    if (w == 5) {                                // dO; tokens beyond the sequence have none
+      const int col0 = IO_COLS * wg;
+      const bf16* src = reinterpret_cast<const bf16*>(q.d_o) + b * q.dos.b + h * q.dos.h + col0;
+      IoRows v;
+      auto load = [&](int c) {
+        const int t = c * DC + lane;
+        v.load(src + t * q.dos.l, c >= 0 && t < p.seqlen, p.dv - col0);
+      };
+      load(p.pieces - 1);
+      v.to_lds(reinterpret_cast<bf16*>(smem + DOUT + ((p.pieces - 1) & 1) * IO_HALFS), lane);
+      load(p.pieces - 2);
+      lds_barrier();
+      for (int c = p.pieces - 1; c >= 0; --c) {
+        lds_barrier();                           // 1
+        v.to_lds(reinterpret_cast<bf16*>(smem + DOUT + ((c + 1) & 1) * IO_HALFS), lane);
+        load(c - 2);
+        lds_barrier();                           // 2
+        lds_barrier();                           // 3
+      }
+      return;
+    }
+  }
+  const int blk = 2 * wg + (w >> 1), col = 16 * blk + l16;
+  const bool live = blk < nblk, cv = col < p.dv;
   f16* ex = smem + (GA + (AHEAD ? 2 : 1) * GB) * FR + (w >> 1) * EX;
   f32x4* const xSend = reinterpret_cast<f32x4*>(ex) + hf * 2 * 64 + lane;
   const f32x4* const xRecv = reinterpret_cast<const f32x4*>(ex) + (1 - hf) * 2 * 64 + lane;
   f16* const eZ = ex + 4 * FR;                                       // the second half's ddelta
   f16* const eU = eZ + 2 * FR;                                       // the terms of Q and K, two parts of each half
   float* const eS = reinterpret_cast<float*>(eU + 8 * FR);
-
-  const int fw = AHEAD ? 0 : w;
-  auto fetch_a = [&](int c) {
-    fetch_share<NP * F, FW>(smem, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + NP * F * 1024, fw, lane);
-    fetch_share<2 * kTFrags, FW>(smem + NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit + 4 * kTFrags * 1024, fw, lane);
-  };
-  auto fetch_b = [&](int c) {
-    f16* to = smem + (GA + (AHEAD ? (c & 1) * GB : 0)) * FR;
-    fetch_share<2 * NP * F, FW>(to, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + 2 * NP * F * 1024, fw, lane);
-    fetch_share<2 * kTFrags, FW>(to + 2 * NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit + 2 * kTFrags * 1024, fw, lane);
-    if (fw == 0) dma_lds<16>(p.workspace + lay.vec + (vunit0 + c) * (int64_t)(kVecFloats * 4), 16u * lane, to + (2 * NP * F + 2 * kTFrags) * FR);
-  };
-  if constexpr (AHEAD) if (w == 4) {                         // as in the forward's scan
-    fetch_a(p.pieces - 1);
-    fetch_b(p.pieces - 1);
-    wait_vmem_n<GB>();
-    lds_barrier();
-    for (int c = p.pieces - 1; c >= 0; --c) {
-      wait_vmem();
-      lds_barrier();                             // 1
-      if (c > 0) fetch_a(c - 1);
-      lds_barrier();                             // 2
-      if (c > 0) {
-        fetch_b(c - 1);
-        wait_vmem_n<GB>();
-      }
-      lds_barrier();                             // 3
-    }
-    return;
-  }
 
   f32x4 dS[NSH];
 #pragma unroll
@@ -85,23 +111,48 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 320) void delta_back_scan_ke
       dS[n][r] = q.d_final_state && cv && row < p.dk ? q.d_final_state[((int64_t)bh * p.dk + row) * p.dv + col] : 0.f;
     }
   // dO of one's own tokens; the first wave's P^T dO takes the other's too
-  const T* osrc = reinterpret_cast<const T*>(q.d_o) + b * q.dos.b + h * q.dos.h + 16 * blk;
   T on[2][8];
   auto load_o = [&](int c) {
+    if constexpr (AHEAD) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      if (x && hf) break;
-      const int t = c * DC + 32 * (hf + x), len = p.seqlen - t;
-      const int from = min(t, p.seqlen - 1);
-      load_rows8<T>(osrc + from * q.dos.l, q.dos.l, p.seqlen - from, cv, all_cv, l16, g4, on[x]);
-      if (len < 32)                              // no output, no gradient
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (16 * (i >> 2) + 4 * g4 + (i & 3) >= len) on[x][i] = from_f32<T>(0.f);
+        for (int i = 0; i < 2; ++i) {
+          const bf16x4 v = *reinterpret_cast<const bf16x4*>(smem + DOUT + (c & 1) * IO_HALFS + ((w >> 1) * 16 + l16) * IO_PITCH + 32 * (x ? 1 - hf : hf) + 16 * i + 4 * g4);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) on[x][4 * i + r] = v[r];
+        }
+    } else {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int t = c * DC + 32 * (x ? 1 - hf : hf), len = p.seqlen - t, from = min(t, p.seqlen - 1);
+        const T* osrc = reinterpret_cast<const T*>(q.d_o) + b * q.dos.b + h * q.dos.h + (live ? 16 * blk : 0);
+        load_rows8<T>(osrc + from * q.dos.l, q.dos.l, p.seqlen - from, cv, 16 * blk + 16 <= p.dv, l16, g4, on[x]);
+        if (len < 32)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (16 * (i >> 2) + 4 * g4 + (i & 3) >= len) on[x][i] = from_f32<T>(0.f);
+      }
     }
   };
-  if (live) load_o(p.pieces - 1);
   if (AHEAD) lds_barrier();
+
+  f16x8 ka[KSH][4], p0[2], p1[2], q0[2], q1[2];  // P^T on one's own tokens; on the second half's
+  auto load_a = [&](int c) {
+#pragma unroll
+    for (int s = 0; s < KSH; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ka[s][i] = frag(smem, ((2 * hf + i) & 3) * KS + hf * KSH + s, lane);
+    load_o(c);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      p0[i] = frag(smem, NP * F + tt_frag(2 * hf + i, hf), lane);
+      p1[i] = frag(smem, NP * F + kTFrags + tt_frag(2 * hf + i, hf), lane);
+      q0[i] = frag(smem, NP * F + tt_frag(i, 1), lane);
+      q1[i] = frag(smem, NP * F + kTFrags + tt_frag(i, 1), lane);
+    }
+  };
+  if (AHEAD) load_a(p.pieces - 1);
 
   for (int c = p.pieces - 1; c >= 0; --c) {
     if (!AHEAD) {
@@ -110,193 +161,188 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 320) void delta_back_scan_ke
       fetch_b(c);
       wait_vmem();
       lds_barrier();
+      load_a(c);
     }
-    const f16 *Kr = smem, *Pt = smem + NP * F * FR;
-    const f16 *Kc = smem + (GA + (AHEAD ? (c & 1) * GB : 0)) * FR, *Qc = Kc + NP * F * FR, *Tt = Qc + NP * F * FR;
-    const float* vec = reinterpret_cast<const float*>(Tt + 2 * kTFrags * FR);
+    const int kc0 = GA + (AHEAD ? (c & 1) * GB : 0), qc0 = kc0 + NP * F, tt0 = qc0 + NP * F;         // fragments
+    const float* vec = reinterpret_cast<const float*>(smem + (tt0 + 2 * kTFrags) * FR);
     f16x8 sh[KSH], sl[KSH];
-    f32x4 X[2] = {}, Z[2] = {}, U[2];
-    float ss_inv = 0.f, so_inv = 0.f;
-    if (live) {
-      f16x8 ka[KSH][4];                          // tiles 0, 1: one's own tokens, 2, 3: the other's
+    f32x4 X[4] = {}, Z[2] = {}, U[2], V[2];
+    const Scale ss(col_max(abs_max(dS)));
+    parts_of<2>(dS, ss.mult, sh, sl);
 #pragma unroll
-      for (int s = 0; s < KSH; ++s)
+    for (int s = 0; s < KSH; ++s) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ka[s][i] = frag(Kr, ((2 * hf + i) & 3) * KS + hf * KSH + s, lane);
-      const Scale ss(col_max(abs_max(dS)));
-      ss_inv = ss.inv;
-      parts_of<2>(dS, ss.mult, sh, sl);
-      f32x4 XO[2] = {};
+      for (int i = 0; i < 4; ++i) X[i] = mma_h(ka[s][i], sh[s], X[i]);
 #pragma unroll
-      for (int s = 0; s < KSH; ++s) {
+      for (int i = 0; i < 4; ++i) X[i] = mma_h(ka[s][i], sl[s], X[i]);
+      if constexpr (NP == 2)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) (i < 2 ? X[i & 1] : XO[i & 1]) = mma_h(ka[s][i], sh[s], i < 2 ? X[i & 1] : XO[i & 1]);
+        for (int i = 0; i < 4; ++i) X[i] = mma_h(frag(smem, F + ((2 * hf + i) & 3) * KS + hf * KSH + s, lane), sh[s], X[i]);
+    }
+    // P^T dO
 #pragma unroll
-        for (int i = 0; i < 4; ++i) (i < 2 ? X[i & 1] : XO[i & 1]) = mma_h(ka[s][i], sl[s], i < 2 ? X[i & 1] : XO[i & 1]);
-        if constexpr (NP == 2)
+    for (int i = 0; i < 8; ++i) {
+      U[i >> 2][i & 3] = to_f32(on[0][i]);
+      V[i >> 2][i & 3] = to_f32(on[1][i]);
+    }
+    f16x8 oh[1], ol[1];
+    const Scale so(col_max(abs_max(V, abs_max(U))));
+    parts_of<NP>(U, so.mult, oh, ol);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            (i < 2 ? X[i & 1] : XO[i & 1]) = mma_h(frag(Kr, F + ((2 * hf + i) & 3) * KS + hf * KSH + s, lane), sh[s], i < 2 ? X[i & 1] : XO[i & 1]);
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) xSend[i * 64] = XO[i] * ss_inv;
-      // P^T dO
-#pragma unroll
-      for (int i = 0; i < 8; ++i) U[i >> 2][i & 3] = to_f32(on[0][i]);
-      f32x4 V[2];
-      float om = abs_max(U);
-      if (hf == 0) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) V[i >> 2][i & 3] = to_f32(on[1][i]);
-        om = abs_max(V, om);
-      }
-      const Scale so(col_max(om));
-      so_inv = so.inv;
-      f16x8 oh[1], ol[1];
-      parts_of<NP>(U, so.mult, oh, ol);
+    for (int i = 0; i < 2; ++i) {
+      Z[i] = mma_h(p0[i], oh[0], Z[i]);
+      if constexpr (NP == 2) Z[i] = mma_h(p0[i], ol[0], Z[i]);
+      Z[i] = mma_h(p1[i], oh[0], Z[i]);
+    }
+    if (hf == 0) {
+      parts_of<NP>(V, so.mult, oh, ol);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const f16x8 a = frag(Pt, tt_frag(2 * hf + i, hf), lane);
-        Z[i] = mma_h(a, oh[0], Z[i]);
-        if constexpr (NP == 2) Z[i] = mma_h(a, ol[0], Z[i]);
-        Z[i] = mma_h(frag(Pt, kTFrags + tt_frag(2 * hf + i, hf), lane), oh[0], Z[i]);
-      }
-      if (hf == 0) {
-        parts_of<NP>(V, so.mult, oh, ol);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const f16x8 a = frag(Pt, tt_frag(i, 1), lane);
-          Z[i] = mma_h(a, oh[0], Z[i]);
-          if constexpr (NP == 2) Z[i] = mma_h(a, ol[0], Z[i]);
-          Z[i] = mma_h(frag(Pt, kTFrags + tt_frag(i, 1), lane), oh[0], Z[i]);
-        }
+        Z[i] = mma_h(q0[i], oh[0], Z[i]);
+        if constexpr (NP == 2) Z[i] = mma_h(q0[i], ol[0], Z[i]);
+        Z[i] = mma_h(q1[i], oh[0], Z[i]);
       }
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) xSend[i * 64] = X[2 + i] * ss.inv;
     lds_barrier();                               // 1
-    if (live && c > 0) load_o(c - 1);
-    f32x4 Yv[2] = {};
-    float zi = 0.f;
-    if (live) {
-      const float zs = p.scale * (so_inv * vec[VEC_SP]), sK = vec[VEC_SK];
+    f32x4 xr[2], wt[2], eg[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const f32x4 wt = *reinterpret_cast<const f32x4*>(vec + VEC_W + 32 * hf + 16 * i + 4 * g4);
-        const f32x4 xr = xRecv[i * 64];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) Z[i][r] = zs * Z[i][r] + wt[r] * (sK * (ss_inv * X[i][r] + xr[r]));
-      }
-      // y = T^T ddelta
-      f16x8 zh[1], zl[1];
-      const Scale sz(col_max(abs_max(Z)));
-      zi = sz.inv;
-      parts_of<2>(Z, sz.mult, zh, zl);
-      if (hf == 1) {
-        put_frag(eZ, 0, lane, zh[0]);
-        put_frag(eZ, 1, lane, zl[0]);
-        eS[lane] = zi;
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const f16x8 a = frag(Tt, tt_frag(2 * hf + i, hf), lane), a1 = frag(Tt, kTFrags + tt_frag(2 * hf + i, hf), lane);
-        Yv[i] = mma_h(a, zh[0], Yv[i]);
-        Yv[i] = mma_h(a, zl[0], Yv[i]);
-        Yv[i] = mma_h(a1, zh[0], Yv[i]);
-      }
+    for (int i = 0; i < 2; ++i) {
+      xr[i] = xRecv[i * 64];
+      wt[i] = *reinterpret_cast<const f32x4*>(vec + VEC_W + 32 * hf + 16 * i + 4 * g4);
     }
+    const f32x4 cs = *reinterpret_cast<const f32x4*>(vec + VEC_GAMMA);                 // gamma, scales of T, P, K
+    const float sQ = vec[VEC_SQ];
+    f16x8 t0[2], t1[2], x0[2], x1[2];            // T^T on one's own tokens; on the second half's
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      t0[i] = frag(smem, tt0 + tt_frag(2 * hf + i, hf), lane);
+      t1[i] = frag(smem, tt0 + kTFrags + tt_frag(2 * hf + i, hf), lane);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      x0[i] = frag(smem, tt0 + tt_frag(i, 1), lane);
+      x1[i] = frag(smem, tt0 + kTFrags + tt_frag(i, 1), lane);
+      eg[i] = *reinterpret_cast<const f32x4*>(vec + 32 * hf + 16 * i + 4 * g4);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    const float zs = p.scale * (so.inv * cs[2]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) Z[i][r] = zs * Z[i][r] + wt[i][r] * (cs[3] * (ss.inv * X[i][r] + xr[i][r]));
+    // y = T^T ddelta
+    f16x8 zh[1], zl[1];
+    const Scale sz(col_max(abs_max(Z)));
+    parts_of<2>(Z, sz.mult, zh, zl);
+    if (hf == 1) {
+      put_frag(eZ, 0, lane, zh[0]);
+      put_frag(eZ, 1, lane, zl[0]);
+      eS[lane] = sz.inv;
+    }
+    f32x4 Yv[2] = {}, E[2] = {};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) Yv[i] = mma_h(t0[i], zh[0], Yv[i]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) Yv[i] = mma_h(t0[i], zl[0], Yv[i]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) Yv[i] = mma_h(t1[i], zh[0], Yv[i]);
     lds_barrier();                               // 2
-    f16x8 uh[1], ul[1], vh[1], vl[1], yh[1], yl[1];
-    float own = 0.f, sy_inv = 0.f;
-    if (live) {
-      if (hf == 0) {
-        const f16x8 z0 = frag(eZ, 0, lane), z1 = frag(eZ, 1, lane);
-        f32x4 E[2] = {};
+    const f16x8 z0 = frag(eZ, 0, lane), z1 = frag(eZ, 1, lane);
+    const float es = eS[lane];
+    f16x8 kc[NSH][2], qc[NSH][2];                // K and Q by columns, one's own tokens first
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const f16x8 a = frag(Tt, tt_frag(i, 1), lane), a1 = frag(Tt, kTFrags + tt_frag(i, 1), lane);
-          E[i] = mma_h(a, z0, E[i]);
-          E[i] = mma_h(a, z1, E[i]);
-          E[i] = mma_h(a1, z0, E[i]);
-        }
-        const float es = eS[lane];
+    for (int n = 0; n < NSH; ++n)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) Yv[i][r] = zi * Yv[i][r] + es * E[i][r];
-        zi = 1.f;
+      for (int x = 0; x < 2; ++x) {
+        qc[n][x] = frag(smem, qc0 + 2 * (hf * NSH + n) + (x ? 1 - hf : hf), lane);
+        kc[n][x] = frag(smem, kc0 + 2 * (hf * NSH + n) + (x ? 1 - hf : hf), lane);
       }
-      // both terms of the gradient before the piece on one scale, those of Q's and K's parts in it
-      const float ysc = zi * vec[VEC_ST], uq = p.scale * vec[VEC_SQ], uk = -(ysc * vec[VEC_SK]);
-      f32x4 V[2];
+    __builtin_amdgcn_sched_barrier(0);
+    float zi = sz.inv;
+    if (hf == 0) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const f32x4 eg = *reinterpret_cast<const f32x4*>(vec + 32 * hf + 16 * i + 4 * g4);
+      for (int i = 0; i < 2; ++i) E[i] = mma_h(x0[i], z0, E[i]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          U[i][r] *= uq * eg[r];
-          V[i][r] = uk * eg[r] * Yv[i][r];
-        }
-      }
-      const Scale su(col_max(abs_max(V, abs_max(U))));
-      own = su.inv;
-      parts_of<2>(U, su.mult, uh, ul);
-      parts_of<2>(V, su.mult, vh, vl);
-      put_frag(eU, 4 * hf, lane, uh[0]);
-      put_frag(eU, 4 * hf + 1, lane, ul[0]);
-      put_frag(eU, 4 * hf + 2, lane, vh[0]);
-      put_frag(eU, 4 * hf + 3, lane, vl[0]);
-      eS[(2 + hf) * 64 + lane] = own;
-      const Scale sy(col_max(abs_max(Yv)));
-      parts_of<2>(Yv, sy.mult, yh, yl);
-      sy_inv = sy.inv * ysc;
+      for (int i = 0; i < 2; ++i) E[i] = mma_h(x0[i], z1, E[i]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) Yv[i] *= ysc;
+      for (int i = 0; i < 2; ++i) E[i] = mma_h(x1[i], z0, E[i]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) Yv[i][r] = zi * Yv[i][r] + es * E[i][r];
+      zi = 1.f;
     }
+    // both terms of the gradient before the piece on one scale, those of Q's and K's parts in it
+    const float ysc = zi * cs[1], uq = p.scale * sQ, uk = -(ysc * cs[3]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        U[i][r] *= uq * eg[i][r];
+        V[i][r] = uk * eg[i][r] * Yv[i][r];
+      }
+    f16x8 uh[1], ul[1], vh[1], vl[1], yh[1], yl[1];
+    const Scale su(col_max(abs_max(V, abs_max(U))));
+    parts_of<2>(U, su.mult, uh, ul);
+    parts_of<2>(V, su.mult, vh, vl);
+    put_frag(eU, 4 * hf, lane, uh[0]);
+    put_frag(eU, 4 * hf + 1, lane, ul[0]);
+    put_frag(eU, 4 * hf + 2, lane, vh[0]);
+    put_frag(eU, 4 * hf + 3, lane, vl[0]);
+    eS[(2 + hf) * 64 + lane] = su.inv;
     lds_barrier();                               // 3
-    if (!live) continue;
-    {
-      const f16* eO = eU + 4 * (1 - hf) * FR;
-      const f16x8 o0 = frag(eO, 0, lane), o1 = frag(eO, 1, lane), o2 = frag(eO, 2, lane), o3 = frag(eO, 3, lane);
-      const float gamma = vec[VEC_GAMMA], other = eS[(3 - hf) * 64 + lane];
+    const f16* eO = eU + 4 * (1 - hf) * FR;
+    const f16x8 o0 = frag(eO, 0, lane), o1 = frag(eO, 1, lane), o2 = frag(eO, 2, lane), o3 = frag(eO, 3, lane);
+    const float other = eS[(3 - hf) * 64 + lane];
+    if (AHEAD && c > 0) load_a(c - 1);
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4 u0[NSH] = {}, u1[NSH] = {};
+#pragma unroll
+    for (int n = 0; n < NSH; ++n) u0[n] = mma_h(qc[n][0], uh[0], u0[n]);
+#pragma unroll
+    for (int n = 0; n < NSH; ++n) u0[n] = mma_h(qc[n][0], ul[0], u0[n]);
+#pragma unroll
+    for (int n = 0; n < NSH; ++n) u0[n] = mma_h(kc[n][0], vh[0], u0[n]);
+#pragma unroll
+    for (int n = 0; n < NSH; ++n) u0[n] = mma_h(kc[n][0], vl[0], u0[n]);
+#pragma unroll
+    for (int n = 0; n < NSH; ++n) u1[n] = mma_h(qc[n][1], o0, u1[n]);
+#pragma unroll
+    for (int n = 0; n < NSH; ++n) u1[n] = mma_h(qc[n][1], o1, u1[n]);
+#pragma unroll
+    for (int n = 0; n < NSH; ++n) u1[n] = mma_h(kc[n][1], o2, u1[n]);
+#pragma unroll
+    for (int n = 0; n < NSH; ++n) u1[n] = mma_h(kc[n][1], o3, u1[n]);
+    if constexpr (NP == 2)
 #pragma unroll
       for (int n = 0; n < NSH; ++n) {
-        const int at = 2 * (hf * NSH + n);
-        const f16x8 qa = frag(Qc, at + hf, lane), qo = frag(Qc, at + 1 - hf, lane);
-        const f16x8 ka = frag(Kc, at + hf, lane), ko = frag(Kc, at + 1 - hf, lane);
-        f32x4 u0 = {}, u1 = {};
-        u0 = mma_h(qa, uh[0], u0);
-        u1 = mma_h(qo, o0, u1);
-        u0 = mma_h(qa, ul[0], u0);
-        u1 = mma_h(qo, o1, u1);
-        u0 = mma_h(ka, vh[0], u0);
-        u1 = mma_h(ko, o2, u1);
-        u0 = mma_h(ka, vl[0], u0);
-        u1 = mma_h(ko, o3, u1);
-        if constexpr (NP == 2) {
-          u0 = mma_h(frag(Qc, F + at + hf, lane), uh[0], u0);
-          u1 = mma_h(frag(Qc, F + at + 1 - hf, lane), o0, u1);
-          u0 = mma_h(frag(Kc, F + at + hf, lane), vh[0], u0);
-          u1 = mma_h(frag(Kc, F + at + 1 - hf, lane), o2, u1);
-        }
+        const int at = F + 2 * (hf * NSH + n);
+        u0[n] = mma_h(frag(smem, qc0 + at + hf, lane), uh[0], u0[n]);
+        u1[n] = mma_h(frag(smem, qc0 + at + 1 - hf, lane), o0, u1[n]);
+        u0[n] = mma_h(frag(smem, kc0 + at + hf, lane), vh[0], u0[n]);
+        u1[n] = mma_h(frag(smem, kc0 + at + 1 - hf, lane), o2, u1[n]);
+      }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) dS[n][r] = gamma * dS[n][r] + own * u0[r] + other * u1[r];
+    for (int n = 0; n < NSH; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) dS[n][r] = cs[0] * dS[n][r] + su.inv * u0[n][r] + other * u1[n][r];
+    if (live) {
+      const Scale sy(col_max(abs_max(Yv)));
+      parts_of<2>(Yv, sy.mult, yh, yl);
+      const int64_t at = (vunit0 + c) * nblk + blk;
+      f16* keep = reinterpret_cast<f16*>(p.workspace + lay.keep) + at * (int64_t)keep_halfs<DKP>();
+      float* scales = reinterpret_cast<float*>(p.workspace + lay.scales) + at * 128 + 64 * hf + l16;
+      keep_parts<KS>(keep + keep_at<DKP>(KEEP_DS), hf * KSH, sh, sl, lane);
+      keep_parts<2>(keep + keep_at<DKP>(KEEP_Y), hf, yh, yl, lane);
+      if (g4 == 0) {
+        scales[16 * KEEP_DS] = ss.inv;
+        scales[16 * KEEP_Y] = sy.inv * ysc;
       }
     }
-    const int64_t at = (vunit0 + c) * nblk + blk;
-    f16* keep = reinterpret_cast<f16*>(p.workspace + lay.keep) + at * (int64_t)keep_halfs<DKP>();
-    float* scales = reinterpret_cast<float*>(p.workspace + lay.scales) + at * 128 + 64 * hf + l16;
-    keep_parts<KS>(keep + keep_at<DKP>(KEEP_DS), hf * KSH, sh, sl, lane);
-    keep_parts<2>(keep + keep_at<DKP>(KEEP_Y), hf, yh, yl, lane);
-    if (g4 == 0) {
-      scales[16 * KEEP_DS] = ss_inv;
-      scales[16 * KEEP_Y] = sy_inv;
-    }
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = Yv[i >> 2][i & 3];
-    const int t = c * DC + 32 * hf;
-    store_rows8<T>(reinterpret_cast<T*>(q.dv) + b * q.dvs.b + h * q.dvs.h + t * q.dvs.l + 16 * blk, q.dvs.l, p.seqlen - t, cv, l16, g4, y);
   }
-  if (q.d_initial_state && live && cv) {
+  if (q.d_initial_state && cv) {
 #pragma unroll
     for (int n = 0; n < NSH; ++n)
 #pragma unroll
@@ -382,6 +428,7 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
     const int h = hk * rep + hr;
     const int64_t vunit = ((int64_t)b * p.heads + h) * p.pieces + c;
     const T* osrc = reinterpret_cast<const T*>(q.d_o) + b * q.dos.b + h * q.dos.h + (int64_t)t0 * q.dos.l;
+    T* dvo = reinterpret_cast<T*>(q.dv) + b * q.dvs.b + h * q.dvs.h + (int64_t)t0 * q.dvs.l;
     // dO's largest magnitude, the matrices' scales
     float om = 0.f;
     for (int u = tid; u < len * ((p.dv + 7) / 8); u += 256) {
@@ -458,8 +505,17 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
           const f16 hd = (f16)(f[16 * KEEP_D] / mD), hy = (f16)(f[16 * KEEP_Y] / mY);
           d0 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_D)) * hd;
           d1 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_D) + 16 * DC) * hd;
-          y0 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_Y)) * hy;
-          y1 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_Y) + 16 * DC) * hy;
+          y0 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_Y));
+          y1 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_Y) + 16 * DC);
+          if (v0 + r < p.dv) {                   // dV
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int t = c + (j & 3) + 4 * (j & 4);
+              if (t < len) dvo[t * q.dvs.l + v0 + r] = from_f32<T>(((float)y0[j] + (float)y1[j]) * f[16 * KEEP_Y]);
+            }
+          }
+          y0 *= hy;
+          y1 *= hy;
         }
         put_halves<64>(sD, r, c, d0);
         put_halves<64>(sD + YE, r, c, d1);
@@ -681,7 +737,7 @@ hipError_t run_bwd(const DeltaBwdParams& q, hipStream_t st) {
   const DeltaParams& p = q.f;
   const DeltaLayout lay(p, true);
   const int nblk = (p.dv + 15) / 16, nwg = (nblk + 1) / 2;
-  delta_back_scan_kernel<T, DKP><<<head_block_grid(p.batch * p.heads, nwg), sizeof(T) == 4 ? 256 : 320, 0, st>>>(q, lay, nblk, nwg);
+  delta_back_scan_kernel<T, DKP><<<head_block_grid(p.batch * p.heads, nwg), sizeof(T) == 4 ? 256 : 384, 0, st>>>(q, lay, nblk, nwg);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   delta_grads_kernel<T, DKP><<<(unsigned)((int64_t)p.batch * p.kheads * p.pieces), 256, 0, st>>>(q, lay, nblk);

@@ -268,35 +268,105 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p, DeltaLay
 
 // ------------------------------------------------------------------ the state from piece to piece
 // Two waves hold 16 columns of the state, half of its rows each (fp32), and half of a piece's tokens; a workgroup has two
-// such pairs, which read the same fragments, fetched by LDS DMA a piece ahead.  For a piece:
+// such pairs, which read the same fragments.  For a piece:
 //   each wave multiplies K (and Q) by its rows of S and gives the other its part of the other's tokens;   [barrier 1]
 //   R = V - e^G K S of its tokens; T is lower triangular, so that the second wave needs the first one's R;  [barrier 2]
 //   U = beta e^{G_end - G} delta of its tokens goes to the other, each adds K^T U to its rows.              [barrier 3]
+// bf16: a fifth wave fetches the next piece's fragments by LDS DMA and a sixth one v, and stores o: a wave that issues such
+// loads stands still while they drain (2000 of the 8000 cycles that a piece took before), which those two may.
 // KEEP: the entering states and delta are stored for the backward.  OUT: o is computed.
 //
 // Bound by the latency of one piece on waves that have a SIMD to themselves, most of it the conversions (an instruction of
-// 4 cycles for each value and part); b 2, H 16, L 4096 has 256 sets of 16 columns for 1024 SIMDs.
+// 4 cycles for each value and part); b 2, H 16, L 4096 has 256 sets of 16 columns for 1024 SIMDs.  Operands that no other
+// wave has to finish first are read from LDS right behind a barrier, ahead of what they are needed for.
 template <typename T, int DKP, bool OUT, bool KEEP>
-__global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 320) void delta_scan_kernel(DeltaParams p, DeltaLayout lay, int nblk, int nwg) {
+__global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_scan_kernel(DeltaParams p, DeltaLayout lay, int nblk, int nwg) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
   constexpr bool AHEAD = NP == 1;                // fp32: the fragments of a piece fill the LDS
-  constexpr int FW = AHEAD ? 1 : 4;              // waves that fetch: the fifth, or all four
+  constexpr int FW = AHEAD ? 1 : 4;              // waves that fetch
   constexpr int KS = DKP / 32, KSH = KS / 2, NSH = DKP / 32, F = kKFrags<DKP>;
   constexpr int GA = (OUT ? 2 : 1) * NP * F;                         // fragments of (Q and) K by rows: before barrier 1
-  constexpr int TPF = OUT ? (NP == 1 ? 20 : 24) : 12;                // of T (and P; two beyond it)
+  constexpr int TPF = OUT ? 4 * kTFrags : 2 * kTFrags;               // of T (and P)
   constexpr int GB = NP * F + TPF + 1;                               // with K by columns and vec: after it
   constexpr int XF = OUT ? 4 : 2, DF = OUT ? NP : 0;
   constexpr int EX = (2 * XF + 2 + 4 + DF + 1) * FR;                 // halfs of a pair's exchange
-  __shared__ __align__(1024) f16 smem[(GA + (AHEAD ? 2 : 1) * GB) * FR + 2 * EX];
+  constexpr int IO = AHEAD ? (OUT ? 3 : 2) * IO_HALFS : 0;           // v of two pieces, o of one
+  __shared__ __align__(1024) f16 smem[(GA + (AHEAD ? 2 : 1) * GB) * FR + 2 * EX + IO];
 
   const int lane = threadIdx.x & 63, w = wave_id(), l16 = lane & 15, g4 = lane >> 4, hf = w & 1;
   int bh, wg;
   if (!head_block(blockIdx.x, p.batch * p.heads, nwg, bh, wg)) return;
   const int b = bh / p.heads, h = bh % p.heads, hk = h / (p.heads / p.kheads);
-  const int blk = 2 * wg + (w >> 1), col = 16 * blk + l16;
-  const bool live = blk < nblk, cv = col < p.dv, all_cv = 16 * blk + 16 <= p.dv;
   const int64_t kunit0 = ((int64_t)b * p.kheads + hk) * p.pieces, vunit0 = (int64_t)bh * p.pieces;
+  bf16* const sV = reinterpret_cast<bf16*>(smem + (GA + (AHEAD ? 2 : 1) * GB) * FR + 2 * EX);
+  bf16* const sO = sV + 2 * IO_HALFS;
 
+  const int fw = AHEAD ? 0 : w;
+  lds_f16_t* const lds = (lds_f16_t*)smem;
+  auto fetch_a = [&](int c) { fetch_share<GA, FW>(lds, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + (OUT ? 0 : NP * F * 1024), fw, lane); };
+  auto fetch_b = [&](int c) {
+    lds_f16_t* to = lds + (GA + (AHEAD ? (c & 1) * GB : 0)) * FR;
+    fetch_share<NP * F, FW>(to, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + 2 * NP * F * 1024, fw, lane);
+    fetch_share<TPF, FW>(to + NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit, fw, lane);
+    if (fw == 0) fetch_share<1, 1>(to + (NP * F + TPF) * FR, p.workspace + lay.vec + (vunit0 + c) * (int64_t)(kVecFloats * 4), 0, lane);
+  };
+  if constexpr (AHEAD) {
+    if (w == 4) {
+      fetch_a(0);
+      fetch_b(0);
+      wait_vmem_n<GB>();
+      lds_barrier();
+      for (int c = 0; c < p.pieces; ++c) {
+        const bool more = c + 1 < p.pieces;
+        wait_vmem();                             // T, P and K by columns of this piece
+        lds_barrier();                           // 1
+        if (more) fetch_a(c + 1);                // where the last ones have been read
+        lds_barrier();                           // 2
+        if (more) {
+          fetch_b(c + 1);
+          wait_vmem_n<GB>();
+        }
+        lds_barrier();                           // 3
+      }
+      lds_barrier();
+      return;
+    }
+    if (w == 5) {
+      const int col0 = IO_COLS * wg, left = p.dv - col0;
+      const bf16* vs = reinterpret_cast<const bf16*>(p.v) + b * p.vs.b + h * p.vs.h + col0;
+      bf16* os = reinterpret_cast<bf16*>(p.o) + b * p.os.b + h * p.os.h + col0;
+      IoRows v, o;
+      auto load_v = [&](int c) {
+        const int t = c * DC + lane;
+        v.load(vs + t * p.vs.l, t < p.seqlen, left);
+      };
+      load_v(0);
+      v.to_lds(sV, lane);
+      load_v(1);
+      lds_barrier();
+      for (int c = 0; c <= p.pieces; ++c) {
+        if (c == p.pieces) {
+          lds_barrier();                         // the last piece's o is whole
+        } else {
+          lds_barrier();                         // 1
+          v.to_lds(sV + ((c + 1) & 1) * IO_HALFS, lane);
+          load_v(c + 2);
+        }
+        if (OUT && c > 0) {
+          const int t = (c - 1) * DC + lane;
+          o.from_lds(sO, lane);
+          o.store(os + t * p.os.l, t < p.seqlen, left);
+        }
+        if (c < p.pieces) {
+          lds_barrier();                         // 2
+          lds_barrier();                         // 3
+        }
+      }
+      return;
+    }
+  }
+  const int blk = 2 * wg + (w >> 1), col = 16 * blk + l16;
+  const bool live = blk < nblk, cv = col < p.dv;                     // a pair beyond the last columns has zeros
   f16* ex = smem + (GA + (AHEAD ? 2 : 1) * GB) * FR + (w >> 1) * EX;
   f32x4* const xSend = reinterpret_cast<f32x4*>(ex) + hf * XF * 64 + lane;             // X (and Y) of the other's tokens
   const f32x4* const xRecv = reinterpret_cast<const f32x4*>(ex) + (1 - hf) * XF * 64 + lane;
@@ -304,35 +374,6 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 320) void delta_scan_kernel(
   f16* const eU = eR + 2 * FR;                                                         // U, two parts of each half
   f16* const eD = eU + 4 * FR;                                                         // the first half's delta
   float* const eS = reinterpret_cast<float*>(eD + DF * FR);                            // scales: R, D, U of each half
-
-  const int fw = AHEAD ? 0 : w;
-  auto fetch_a = [&](int c) { fetch_share<GA, FW>(smem, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + (OUT ? 0 : NP * F * 1024), fw, lane); };
-  auto fetch_b = [&](int c) {
-    f16* to = smem + (GA + (AHEAD ? (c & 1) * GB : 0)) * FR;
-    fetch_share<NP * F, FW>(to, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + 2 * NP * F * 1024, fw, lane);
-    fetch_share<TPF, FW>(to + NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit, fw, lane);
-    if (fw == 0) dma_lds<16>(p.workspace + lay.vec + (vunit0 + c) * (int64_t)(kVecFloats * 4), 16u * lane, to + (NP * F + TPF) * FR);
-  };
-  if constexpr (AHEAD) if (w == 4) {
-    // the fifth wave fetches: a wave that issues these loads stands still while they drain
-    fetch_a(0);
-    fetch_b(0);
-    wait_vmem_n<GB>();
-    lds_barrier();
-    for (int c = 0; c < p.pieces; ++c) {
-      const bool more = c + 1 < p.pieces;
-      wait_vmem();                               // T, P and K by columns of this piece
-      lds_barrier();                             // 1
-      if (more) fetch_a(c + 1);                  // where the last ones have been read
-      lds_barrier();                             // 2
-      if (more) {
-        fetch_b(c + 1);
-        wait_vmem_n<GB>();
-      }
-      lds_barrier();                             // 3
-    }
-    return;
-  }
 
   f32x4 S[NSH];                                  // rows DKP / 2 hf + 16 n + 4 g4 + r, column col
 #pragma unroll
@@ -342,14 +383,29 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 320) void delta_scan_kernel(
       const int row = DKP / 2 * hf + 16 * n + 4 * g4 + r;
       S[n][r] = p.initial_state && cv && row < p.dk ? p.initial_state[((int64_t)bh * p.dk + row) * p.dv + col] : 0.f;
     }
-  const T* vsrc = reinterpret_cast<const T*>(p.v) + b * p.vs.b + h * p.vs.h + 16 * blk;
   T vn[8];
   auto load_v = [&](int c) {                     // a half that lies beyond the sequence reads the last token
     const int t = min(c * DC + 32 * hf, p.seqlen - 1);
-    load_rows8<T>(vsrc + t * p.vs.l, p.vs.l, p.seqlen - t, cv, all_cv, l16, g4, vn);
+    const T* vsrc = reinterpret_cast<const T*>(p.v) + b * p.vs.b + h * p.vs.h + (live ? 16 * blk : 0);
+    load_rows8<T>(vsrc + t * p.vs.l, p.vs.l, p.seqlen - t, cv, 16 * blk + 16 <= p.dv, l16, g4, vn);
   };
-  if (live) load_v(0);
   if (AHEAD) lds_barrier();
+  else load_v(0);
+
+  const f16 *Qr = smem, *Kr = smem + (OUT ? NP * F * FR : 0);
+  f16x8 ka[KSH][4], qa[OUT ? KSH : 1][4];        // the next piece's; tiles 0, 1: one's own tokens, 2, 3: the other's
+  auto load_a = [&]() {
+#pragma unroll
+    for (int s = 0; s < KSH; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ka[s][i] = frag(Kr, ((2 * hf + i) & 3) * KS + hf * KSH + s, lane);
+    if constexpr (OUT)
+#pragma unroll
+      for (int s = 0; s < KSH; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) qa[s][i] = frag(Qr, ((2 * hf + i) & 3) * KS + hf * KSH + s, lane);
+  };
+  if (AHEAD) load_a();
 
   for (int c = 0; c < p.pieces; ++c) {
     if (!AHEAD) {
@@ -358,201 +414,227 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 320) void delta_scan_kernel(
       fetch_b(c);
       wait_vmem();
       lds_barrier();
+      load_a();
     }
-    const f16 *Qr = smem, *Kr = Qr + (OUT ? NP * F * FR : 0);
     const f16 *Kc = smem + (GA + (AHEAD ? (c & 1) * GB : 0)) * FR, *Tt = Kc + NP * F * FR, *Pt = Tt + 2 * kTFrags * FR;
     const float* vec = reinterpret_cast<const float*>(Tt + TPF * FR);
     f16x8 sh[KSH], sl[KSH];
-    f32x4 X[2] = {}, Y[2] = {};                  // of one's own tokens
-    float ss_inv = 0.f;
-    if (live) {
-      f16x8 ka[KSH][4];                          // tiles 0, 1: one's own tokens, 2, 3: the other's
+    f32x4 X[4] = {}, Y[4] = {};
+    const Scale ss(col_max(abs_max(S)));
+    parts_of<2>(S, ss.mult, sh, sl);
+#pragma unroll
+    for (int s = 0; s < KSH; ++s) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) X[i] = mma_h(ka[s][i], sh[s], X[i]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) X[i] = mma_h(ka[s][i], sl[s], X[i]);
+      if constexpr (NP == 2)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) X[i] = mma_h(frag(Kr, F + ((2 * hf + i) & 3) * KS + hf * KSH + s, lane), sh[s], X[i]);
+    }
+    if constexpr (OUT)                           // o is rounded to T: one part of the state is enough for bf16
 #pragma unroll
       for (int s = 0; s < KSH; ++s)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ka[s][i] = frag(Kr, ((2 * hf + i) & 3) * KS + hf * KSH + s, lane);
-      const Scale ss(col_max(abs_max(S)));
-      ss_inv = ss.inv;
-      parts_of<2>(S, ss.mult, sh, sl);
-      f32x4 XO[2] = {}, YO[2] = {};
-#pragma unroll
-      for (int s = 0; s < KSH; ++s) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) (i < 2 ? X[i & 1] : XO[i & 1]) = mma_h(ka[s][i], sh[s], i < 2 ? X[i & 1] : XO[i & 1]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) (i < 2 ? X[i & 1] : XO[i & 1]) = mma_h(ka[s][i], sl[s], i < 2 ? X[i & 1] : XO[i & 1]);
-        if constexpr (NP == 2)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            (i < 2 ? X[i & 1] : XO[i & 1]) = mma_h(frag(Kr, F + ((2 * hf + i) & 3) * KS + hf * KSH + s, lane), sh[s], i < 2 ? X[i & 1] : XO[i & 1]);
-        if constexpr (OUT)                       // o is rounded to T: one part of the state is enough for bf16
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            f32x4& y = i < 2 ? Y[i & 1] : YO[i & 1];
-            const f16x8 q = frag(Qr, ((2 * hf + i) & 3) * KS + hf * KSH + s, lane);
-            y = mma_h(q, sh[s], y);
-            if constexpr (NP == 2) {
-              y = mma_h(q, sl[s], y);
-              y = mma_h(frag(Qr, F + ((2 * hf + i) & 3) * KS + hf * KSH + s, lane), sh[s], y);
-            }
+        for (int i = 0; i < 4; ++i) {
+          Y[i] = mma_h(qa[s][i], sh[s], Y[i]);
+          if constexpr (NP == 2) {
+            Y[i] = mma_h(qa[s][i], sl[s], Y[i]);
+            Y[i] = mma_h(frag(Qr, F + ((2 * hf + i) & 3) * KS + hf * KSH + s, lane), sh[s], Y[i]);
           }
-      }
+        }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        xSend[i * 64] = XO[i] * ss_inv;
-        if constexpr (OUT) xSend[(2 + i) * 64] = YO[i] * ss_inv;
-      }
+    for (int i = 0; i < 2; ++i) {
+      xSend[i * 64] = X[2 + i] * ss.inv;
+      if constexpr (OUT) xSend[(2 + i) * 64] = Y[2 + i] * ss.inv;
     }
     lds_barrier();                               // 1
-    f32x4 R[2];
+    f32x4 xr[2], yr[2], eg[2], wt[2];
+    bf16x4 vb[2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) R[i >> 2][i & 3] = to_f32(vn[i]);
-    if (live && c + 1 < p.pieces) load_v(c + 1);
-    f32x4 eg[2], D[2] = {}, E[2] = {};
-    float rs = 0.f;
-    if (live) {
-      const float sK = vec[VEC_SK];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        eg[i] = *reinterpret_cast<const f32x4*>(vec + 32 * hf + 16 * i + 4 * g4);
-        const f32x4 xr = xRecv[i * 64];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) R[i][r] -= eg[i][r] * (sK * (ss_inv * X[i][r] + xr[r]));
-      }
-      // delta = T R: one's own tokens, and for the second wave those of the first
-      f16x8 rh[1], rl[1];
-      const Scale sr(col_max(abs_max(R)));
-      rs = sr.inv;
-      parts_of<2>(R, sr.mult, rh, rl);
-      if (hf == 0) {
-        put_frag(eR, 0, lane, rh[0]);
-        put_frag(eR, 1, lane, rl[0]);
-        eS[lane] = rs;
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const f16x8 a = frag(Tt, t_frag(2 * hf + i, hf), lane), a1 = frag(Tt, kTFrags + t_frag(2 * hf + i, hf), lane);
-        D[i] = mma_h(a, rh[0], D[i]);
-        D[i] = mma_h(a, rl[0], D[i]);
-        D[i] = mma_h(a1, rh[0], D[i]);
-      }
+    for (int i = 0; i < 2; ++i) {
+      xr[i] = xRecv[i * 64];
+      eg[i] = *reinterpret_cast<const f32x4*>(vec + 32 * hf + 16 * i + 4 * g4);
+      if constexpr (AHEAD)
+        vb[i] = *reinterpret_cast<const bf16x4*>(sV + (c & 1) * IO_HALFS + ((w >> 1) * 16 + l16) * IO_PITCH + 32 * hf + 16 * i + 4 * g4);
     }
+    const f32x4 cs = *reinterpret_cast<const f32x4*>(vec + VEC_GAMMA);                 // gamma, scales of T, P, K
+    f16x8 t0[2], t1[2], x0[2], x1[2];            // T on one's own tokens; on the first half's
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      t0[i] = frag(Tt, t_frag(2 * hf + i, hf), lane);
+      t1[i] = frag(Tt, kTFrags + t_frag(2 * hf + i, hf), lane);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      x0[i] = frag(Tt, t_frag(2 + i, 0), lane);
+      x1[i] = frag(Tt, kTFrags + t_frag(2 + i, 0), lane);
+      wt[i] = *reinterpret_cast<const f32x4*>(vec + VEC_W + 32 * hf + 16 * i + 4 * g4);
+      if constexpr (OUT) yr[i] = xRecv[(2 + i) * 64];
+    }
+    const float sQ = vec[VEC_SQ];
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4 R[2], D[2] = {}, E[2] = {};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float v = AHEAD ? (float)vb[i][r] : to_f32(vn[4 * i + r]);
+        R[i][r] = v - eg[i][r] * (cs[3] * (ss.inv * X[i][r] + xr[i][r]));
+      }
+    if (!AHEAD && c + 1 < p.pieces) load_v(c + 1);
+    // delta = T R: one's own tokens, and for the second wave those of the first
+    f16x8 rh[1], rl[1];
+    const Scale sr(col_max(abs_max(R)));
+    parts_of<2>(R, sr.mult, rh, rl);
+    if (hf == 0) {
+      put_frag(eR, 0, lane, rh[0]);
+      put_frag(eR, 1, lane, rl[0]);
+      eS[lane] = sr.inv;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) D[i] = mma_h(t0[i], rh[0], D[i]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) D[i] = mma_h(t0[i], rl[0], D[i]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) D[i] = mma_h(t1[i], rh[0], D[i]);
     lds_barrier();                               // 2
-    f32x4 U[2];
-    float own_us = 0.f;
-    f16x8 wh[1], wl[1], dh[1], dl[1];
-    Scale sd(0.f);
-    if (live) {
-      if (hf == 1) {
-        const f16x8 r0 = frag(eR, 0, lane), r1 = frag(eR, 1, lane);
+    float rs = sr.inv;
+    const f16x8 r0 = frag(eR, 0, lane), r1 = frag(eR, 1, lane);
+    const float es = eS[lane];
+    f16x8 kc[NSH][2], pa[2], px[2];              // K by columns, one's own tokens first; P as T
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const f16x8 a = frag(Tt, t_frag(2 + i, 0), lane), a1 = frag(Tt, kTFrags + t_frag(2 + i, 0), lane);
-          E[i] = mma_h(a, r0, E[i]);
-          E[i] = mma_h(a, r1, E[i]);
-          E[i] = mma_h(a1, r0, E[i]);
-        }
-        const float es = eS[lane];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) D[i][r] = rs * D[i][r] + es * E[i][r];
-        rs = 1.f;
-      }
-      const float ds = rs * vec[VEC_ST];         // of D, and of U until it leaves its own scale
+    for (int n = 0; n < NSH; ++n) {
+      kc[n][0] = frag(Kc, 2 * (hf * NSH + n) + hf, lane);
+      kc[n][1] = frag(Kc, 2 * (hf * NSH + n) + 1 - hf, lane);
+    }
+    if constexpr (OUT)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const f32x4 wt = *reinterpret_cast<const f32x4*>(vec + VEC_W + 32 * hf + 16 * i + 4 * g4);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) U[i][r] = wt[r] * D[i][r];
+        pa[i] = frag(Pt, t_frag(2 * hf + i, hf), lane);
+        px[i] = frag(Pt, t_frag(2 + i, 0), lane);
       }
-      const Scale su(col_max(abs_max(U)));
-      parts_of<2>(U, su.mult, wh, wl);
-      own_us = su.inv * ds * vec[VEC_SK];
-      put_frag(eU, 2 * hf, lane, wh[0]);
-      put_frag(eU, 2 * hf + 1, lane, wl[0]);
-      eS[(2 + hf) * 64 + lane] = own_us;
-      sd = Scale(col_max(abs_max(D)));
-      parts_of<(KEEP || NP == 2) ? 2 : 1>(D, sd.mult, dh, dl);
-      sd.inv *= ds;
-      if constexpr (OUT)
-        if (hf == 0) {
-          put_frag(eD, 0, lane, dh[0]);
-          if constexpr (NP == 2) put_frag(eD, 1, lane, dl[0]);
-          eS[64 + lane] = sd.inv;
-        }
+    __builtin_amdgcn_sched_barrier(0);
+    if (hf == 1) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) E[i] = mma_h(x0[i], r0, E[i]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) E[i] = mma_h(x0[i], r1, E[i]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) E[i] = mma_h(x1[i], r0, E[i]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) D[i][r] = rs * D[i][r] + es * E[i][r];
+      rs = 1.f;
     }
+    const float ds = rs * cs[1];                 // of D, and of U until it leaves its own scale
+    f32x4 U[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) U[i][r] = wt[i][r] * D[i][r];
+    f16x8 wh[1], wl[1], dh[1], dl[1];
+    const Scale su(col_max(abs_max(U)));
+    parts_of<2>(U, su.mult, wh, wl);
+    const float own_us = su.inv * ds * cs[3];
+    put_frag(eU, 2 * hf, lane, wh[0]);
+    put_frag(eU, 2 * hf + 1, lane, wl[0]);
+    eS[(2 + hf) * 64 + lane] = own_us;
+    const Scale sd(col_max(abs_max(D)));
+    parts_of<(KEEP || NP == 2) ? 2 : 1>(D, sd.mult, dh, dl);
+    if constexpr (OUT)
+      if (hf == 0) {
+        put_frag(eD, 0, lane, dh[0]);
+        if constexpr (NP == 2) put_frag(eD, 1, lane, dl[0]);
+        eS[64 + lane] = sd.inv * ds;
+      }
     lds_barrier();                               // 3
-    if (!live) continue;
-    {
-      const f16x8 oh = frag(eU, 2 - 2 * hf, lane), ol = frag(eU, 3 - 2 * hf, lane);
-      const float gamma = vec[VEC_GAMMA], other_us = eS[(3 - hf) * 64 + lane];
+    const f16x8 oh = frag(eU, 2 - 2 * hf, lane), ol = frag(eU, 3 - 2 * hf, lane);
+    const float other_us = eS[(3 - hf) * 64 + lane];
+    f16x8 d0, d1;
+    float od = 0.f;
+    if constexpr (OUT) {
+      d0 = frag(eD, 0, lane);
+      if constexpr (NP == 2) d1 = frag(eD, 1, lane);
+      od = eS[64 + lane];
+    }
+    if (AHEAD && c + 1 < p.pieces) load_a();
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4 u0[NSH] = {}, u1[NSH] = {};
+#pragma unroll
+    for (int n = 0; n < NSH; ++n) u0[n] = mma_h(kc[n][0], wh[0], u0[n]);
+#pragma unroll
+    for (int n = 0; n < NSH; ++n) u0[n] = mma_h(kc[n][0], wl[0], u0[n]);
+#pragma unroll
+    for (int n = 0; n < NSH; ++n) u1[n] = mma_h(kc[n][1], oh, u1[n]);
+#pragma unroll
+    for (int n = 0; n < NSH; ++n) u1[n] = mma_h(kc[n][1], ol, u1[n]);
+    if constexpr (NP == 2)
 #pragma unroll
       for (int n = 0; n < NSH; ++n) {
-        const f16x8 a = frag(Kc, 2 * (hf * NSH + n) + hf, lane), o = frag(Kc, 2 * (hf * NSH + n) + 1 - hf, lane);
-        f32x4 u0 = {}, u1 = {};
-        u0 = mma_h(a, wh[0], u0);
-        u1 = mma_h(o, oh, u1);
-        u0 = mma_h(a, wl[0], u0);
-        u1 = mma_h(o, ol, u1);
-        if constexpr (NP == 2) {
-          u0 = mma_h(frag(Kc, F + 2 * (hf * NSH + n) + hf, lane), wh[0], u0);
-          u1 = mma_h(frag(Kc, F + 2 * (hf * NSH + n) + 1 - hf, lane), oh, u1);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) S[n][r] = gamma * S[n][r] + own_us * u0[r] + other_us * u1[r];
+        u0[n] = mma_h(frag(Kc, F + 2 * (hf * NSH + n) + hf, lane), wh[0], u0[n]);
+        u1[n] = mma_h(frag(Kc, F + 2 * (hf * NSH + n) + 1 - hf, lane), oh, u1[n]);
       }
-    }
+#pragma unroll
+    for (int n = 0; n < NSH; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) S[n][r] = cs[0] * S[n][r] + own_us * u0[n][r] + other_us * u1[n][r];
     if constexpr (KEEP) {
-      const int64_t at = (vunit0 + c) * nblk + blk;
-      f16* keep = reinterpret_cast<f16*>(p.workspace + lay.keep) + at * (int64_t)keep_halfs<DKP>();
-      float* scales = reinterpret_cast<float*>(p.workspace + lay.scales) + at * 128 + 64 * hf + l16;
-      keep_parts<KS>(keep + keep_at<DKP>(KEEP_S), hf * KSH, sh, sl, lane);
-      keep_parts<2>(keep + keep_at<DKP>(KEEP_D), hf, dh, dl, lane);
-      if (g4 == 0) {
-        scales[16 * KEEP_S] = ss_inv;
-        scales[16 * KEEP_D] = sd.inv;
+      if (live) {
+        const int64_t at = (vunit0 + c) * nblk + blk;
+        f16* keep = reinterpret_cast<f16*>(p.workspace + lay.keep) + at * (int64_t)keep_halfs<DKP>();
+        float* scales = reinterpret_cast<float*>(p.workspace + lay.scales) + at * 128 + 64 * hf + l16;
+        keep_parts<KS>(keep + keep_at<DKP>(KEEP_S), hf * KSH, sh, sl, lane);
+        keep_parts<2>(keep + keep_at<DKP>(KEEP_D), hf, dh, dl, lane);
+        if (g4 == 0) {
+          scales[16 * KEEP_S] = ss.inv;
+          scales[16 * KEEP_D] = sd.inv * ds;
+        }
       }
     }
     if constexpr (OUT) {
-      f32x4 O[2] = {}, O0[2] = {};
-      float o0 = 0.f;
+      f32x4 O[2] = {}, OX[2] = {};
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const f16x8 a = frag(Pt, t_frag(2 * hf + i, hf), lane);
-        O[i] = mma_h(a, dh[0], O[i]);
+        O[i] = mma_h(pa[i], dh[0], O[i]);
         if constexpr (NP == 2) {
-          O[i] = mma_h(a, dl[0], O[i]);
+          O[i] = mma_h(pa[i], dl[0], O[i]);
           O[i] = mma_h(frag(Pt, kTFrags + t_frag(2 * hf + i, hf), lane), dh[0], O[i]);
         }
       }
       if (hf == 1) {
-        const f16x8 d0 = frag(eD, 0, lane);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const f16x8 a = frag(Pt, t_frag(2 + i, 0), lane);
-          O0[i] = mma_h(a, d0, O0[i]);
+          OX[i] = mma_h(px[i], d0, OX[i]);
           if constexpr (NP == 2) {
-            O0[i] = mma_h(a, frag(eD, 1, lane), O0[i]);
-            O0[i] = mma_h(frag(Pt, kTFrags + t_frag(2 + i, 0), lane), d0, O0[i]);
+            OX[i] = mma_h(px[i], d1, OX[i]);
+            OX[i] = mma_h(frag(Pt, kTFrags + t_frag(2 + i, 0), lane), d0, OX[i]);
           }
         }
-        o0 = p.scale * (eS[64 + lane] * vec[VEC_SP]);
       }
-      const float yq = p.scale * vec[VEC_SQ], os = p.scale * (sd.inv * vec[VEC_SP]);
+      const float yq = p.scale * sQ, os = p.scale * (sd.inv * ds * cs[2]), ox = p.scale * (od * cs[2]);
       float o[8];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const f32x4 yr = xRecv[(2 + i) * 64];
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          o[4 * i + r] = eg[i][r] * (yq * (ss_inv * Y[i][r] + yr[r])) + (os * O[i][r] + o0 * O0[i][r]);
+        for (int r = 0; r < 4; ++r) {
+          o[4 * i + r] = eg[i][r] * (yq * (ss.inv * Y[i][r] + yr[i][r])) + os * O[i][r];
+          if (hf == 1) o[4 * i + r] += ox * OX[i][r];
+        }
+      if constexpr (AHEAD) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          *reinterpret_cast<bf16x4*>(sO + ((w >> 1) * 16 + l16) * IO_PITCH + 32 * hf + 16 * i + 4 * g4) =
+              bf16x4{(bf16)o[4 * i], (bf16)o[4 * i + 1], (bf16)o[4 * i + 2], (bf16)o[4 * i + 3]};
+      } else {
+        const int t = c * DC + 32 * hf;
+        store_rows8<T>(reinterpret_cast<T*>(p.o) + b * p.os.b + h * p.os.h + t * p.os.l + 16 * blk, p.os.l, p.seqlen - t, cv, l16, g4, o);
       }
-      const int t = c * DC + 32 * hf;
-      store_rows8<T>(reinterpret_cast<T*>(p.o) + b * p.os.b + h * p.os.h + t * p.os.l + 16 * blk, p.os.l, p.seqlen - t, cv, l16, g4, o);
     }
   }
-  if (p.final_state && live && cv) {
+  if (AHEAD) lds_barrier();
+  if (p.final_state && cv) {
 #pragma unroll
     for (int n = 0; n < NSH; ++n)
 #pragma unroll
@@ -566,7 +648,7 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 320) void delta_scan_kernel(
 template <typename T, int DKP, bool OUT, bool KEEP>
 hipError_t launch_scan(const DeltaParams& p, const DeltaLayout& lay, hipStream_t st) {
   const int nblk = (p.dv + 15) / 16, nwg = (nblk + 1) / 2;
-  delta_scan_kernel<T, DKP, OUT, KEEP><<<head_block_grid(p.batch * p.heads, nwg), sizeof(T) == 4 ? 256 : 320, 0, st>>>(p, lay, nblk, nwg);
+  delta_scan_kernel<T, DKP, OUT, KEEP><<<head_block_grid(p.batch * p.heads, nwg), sizeof(T) == 4 ? 256 : 384, 0, st>>>(p, lay, nblk, nwg);
   return hipGetLastError();
 }
 
