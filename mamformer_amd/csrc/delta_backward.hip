@@ -360,15 +360,17 @@ __device__ __forceinline__ void put_halves(f16* t, int r, int c, f16x8 v) {
   *reinterpret_cast<f16x4*>(t + HTile<W>::at(r, c + 16)) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
 }
 
-// One workgroup of 4 waves for a piece of a key head, its value heads one after the other (their dQ and dK are added in
-// that order).  Wave w holds rows 16 w .. 16 w + 15 of the three products with the states (64 x dk) and of A' and P'.  The
+// One workgroup of 8 waves for a piece of a key head, its value heads one after the other (their dQ and dK are added in
+// that order).  Waves w and w + 4 hold rows 16 w .. 16 w + 15: of the three products with the states (64 x dk) half of the
+// channels each, of A' and P' every other tile.  (Four waves with all of it spilled 150 registers: 407 us against 300 at
+// b 2, H 16 over 8, L 4096.)  The
 // columns of v pass through LDS DVB at a time, every matrix brought to one scale on the way (its columns
 // have their own).
 template <typename T, int DKP>
-__global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, DeltaLayout lay, int nblk) {
+__global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, DeltaLayout lay, int nblk) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
   constexpr int DVB = NP == 1 ? 64 : 32;
-  constexpr int NS = DKP / 16, KS = DKP / 32, F = kKFrags<DKP>;
+  constexpr int NSH = DKP / 32, KS = DKP / 32, F = kKFrags<DKP>;
   using TK = HTile<DKP>;
   using TC = HTile<64>;
   constexpr int SE = DVB * DKP, YE = DVB * 64;   // elements of a part of S / dS and of delta / y
@@ -377,21 +379,21 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
   f16 *sS = smem, *sN = sS + 2 * SE, *sY = sN + 2 * SE, *sD = sY + 2 * YE, *sO = sD + 2 * YE, *sK = sO + NP * TC::ELEMS, *sQ = sK + NP * F * FR;
   f16 *sXa = smem, *sXp = smem + NP * TC::ELEMS;                       // where those were
   __shared__ double sG[DC];
-  __shared__ float sB[DC], sEG[DC], sEnd[DC], sRow[DC], sH[DC], sB2[DC], sCol[4][DC], red[4][4];
+  __shared__ float sB[DC], sEG[DC], sEnd[DC], sRow[2][DC], sB2[2][DC], sCol[4][DC], red[8][4];
   const DeltaParams& p = q.f;
 
-  const int tid = threadIdx.x, lane = tid & 63, w = wave_id(), l16 = lane & 15, g4 = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), w = wave & 3, hf = wave >> 2, l16 = lane & 15, g4 = lane >> 4;
   const int64_t unit = blockIdx.x;
   const int c = (int)(unit % p.pieces), bk = (int)(unit / p.pieces), hk = bk % p.kheads, b = bk / p.kheads;
   const int t0 = c * DC, len = min(DC, p.seqlen - t0), rep = p.heads / p.kheads;
   const f16* kq = reinterpret_cast<const f16*>(p.workspace + lay.kq + unit * lay.kq_unit);       // Q, K by rows
-  for (int i = tid; i < 2 * NP * F * 64; i += 256)                     // K, Q by columns
+  for (int i = tid; i < 2 * NP * F * 64; i += 512)                     // K, Q by columns
     reinterpret_cast<f16x8*>(sK)[i] = reinterpret_cast<const f16x8*>(kq + 2 * NP * F * FR)[i];
   const float* vec0 = reinterpret_cast<const float*>(p.workspace + lay.vec) +
                       (((int64_t)b * p.heads + hk * rep) * p.pieces + c) * kVecFloats;
   const float sk = vec0[VEC_SK], sq = vec0[VEC_SQ];
   __syncthreads();
-  f32x4 kk[4] = {}, qk[4] = {};
+  f32x4 kk[2] = {}, qk[2] = {};                  // tiles 2 m + hf of A' and P'
 #pragma unroll
   for (int s = 0; s < DKP / 32; ++s) {
     f16x8 ka[NP], qa[NP];
@@ -401,29 +403,30 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
       qa[n] = frag(kq, n * F + w * KS + s, lane);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int m = 0; m < 2; ++m) {
+      const int j = 2 * m + hf;
       if (j > w) continue;
       const f16x8 kb = frag(kq, NP * F + j * KS + s, lane);
-      kk[j] = mma_h(ka[0], kb, kk[j]);
-      qk[j] = mma_h(qa[0], kb, qk[j]);
+      kk[m] = mma_h(ka[0], kb, kk[m]);
+      qk[m] = mma_h(qa[0], kb, qk[m]);
       if constexpr (NP == 2) {
         const f16x8 kl = frag(kq, (NP + 1) * F + j * KS + s, lane);
-        kk[j] = mma_h(ka[0], kl, kk[j]);
-        kk[j] = mma_h(ka[1], kb, kk[j]);
-        qk[j] = mma_h(qa[0], kl, qk[j]);
-        qk[j] = mma_h(qa[1], kb, qk[j]);
+        kk[m] = mma_h(ka[0], kl, kk[m]);
+        kk[m] = mma_h(ka[1], kb, kk[m]);
+        qk[m] = mma_h(qa[0], kl, qk[m]);
+        qk[m] = mma_h(qa[1], kb, qk[m]);
       }
     }
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      kk[j][r] = kk[j][r] * sk * sk;
-      qk[j][r] = qk[j][r] * sq * sk;
+      kk[m][r] = kk[m][r] * sk * sk;
+      qk[m][r] = qk[m][r] * sq * sk;
     }
 
-  f32x4 tq[NS] = {}, tk[NS] = {};                // dQ and dK over the value heads
+  f32x4 tq[NSH] = {}, tk[NSH] = {};              // dQ and dK over the value heads, channels 16 (hf NSH + n) ..
   for (int hr = 0; hr < rep; ++hr) {
     const int h = hk * rep + hr;
     const int64_t vunit = ((int64_t)b * p.heads + h) * p.pieces + c;
@@ -431,7 +434,7 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
     T* dvo = reinterpret_cast<T*>(q.dv) + b * q.dvs.b + h * q.dvs.h + (int64_t)t0 * q.dvs.l;
     // dO's largest magnitude, the matrices' scales
     float om = 0.f;
-    for (int u = tid; u < len * ((p.dv + 7) / 8); u += 256) {
+    for (int u = tid; u < len * ((p.dv + 7) / 8); u += 512) {
       const int r = u / ((p.dv + 7) / 8), c8 = u % ((p.dv + 7) / 8) * 8;
       float v[8];
       load8(osrc + r * q.dos.l + c8, p.dv - c8, v);
@@ -444,8 +447,8 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
     for (int i = 0; i < 2 * nblk; ++i) mx = fmaxf(mx, scales[64 * i + lane]);
     mx = row16_max(mx);
     __syncthreads();                             // the last head's use of the LDS is over
-    if (lane == 0) red[w][0] = om;
-    if (w == 0) {
+    if (lane == 0) red[wave][0] = om;
+    if (wave == 0) {
       float gv = 0.f, bv = 0.f;
       if (lane < len) {
         if (p.g) gv = gate_log(p.g[b * p.gs.b + h * p.gs.h + (int64_t)(t0 + lane) * p.gs.l]);
@@ -459,17 +462,21 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
       sEnd[lane] = expf((float)(end - G));
     }
     __syncthreads();
-    const Scale so(fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0])));
+    auto most = [&](int i) {
+      return fmaxf(fmaxf(fmaxf(red[0][i], red[1][i]), fmaxf(red[2][i], red[3][i])), fmaxf(fmaxf(red[4][i], red[5][i]), fmaxf(red[6][i], red[7][i])));
+    };
+    const Scale so(most(0));
     const float mS = lane_val(mx, 16 * KEEP_S), mN = lane_val(mx, 16 * KEEP_DS), mD = lane_val(mx, 16 * KEEP_D),
                 mY = lane_val(mx, 16 * KEEP_Y);
 
-    f32x4 aq[NS] = {}, al[NS] = {}, ar[NS] = {}, pA[4] = {}, pP[4] = {};
+    f32x4 aq[NSH] = {}, al[NSH] = {}, ar[NSH] = {}, pA[2] = {}, pP[2] = {};
     float dot = 0.f;                             // <S, dS>
     const f16* keep0 = reinterpret_cast<const f16*>(p.workspace + lay.keep) + vunit * nblk * (int64_t)keep_halfs<DKP>();
     for (int v0 = 0; v0 < 16 * nblk; v0 += DVB) {
       if (v0) __syncthreads();
+      const int lane = lane_id_here(), tid = 64 * wave + lane;         // addresses formed here, not held for the loops
       // 16 columns of v at a time, a lane's 8 values of a k-step: rows 4 g .. and 16 + 4 g .. of 32, of column l % 16
-      for (int u = tid; u < SE / 8; u += 256) {
+      for (int u = tid; u < SE / 8; u += 512) {
         const int ln = u & 63, r = u / (16 * DKP / 8) * 16 + (ln & 15), k = u / 64 % (DKP / 32), blk = (v0 + r) / 16;
         const int c = 32 * k + 4 * (ln >> 4);
         f16x8 s0 = {}, s1 = {}, n0 = {}, n1 = {};
@@ -496,7 +503,7 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
         put_halves<DKP>(sN, r, c, n0);
         put_halves<DKP>(sN + SE, r, c, n1);
       }
-      for (int u = tid; u < YE / 8; u += 256) {
+      for (int u = tid; u < YE / 8; u += 512) {
         const int ln = u & 63, r = u / 128 * 16 + (ln & 15), k = u / 64 % 2, blk = (v0 + r) / 16, c = 32 * k + 4 * (ln >> 4);
         f16x8 d0 = {}, d1 = {}, y0 = {}, y1 = {};
         if (blk < nblk) {
@@ -522,7 +529,7 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
         put_halves<64>(sY, r, c, y0);
         put_halves<64>(sY + YE, r, c, y1);
       }
-      for (int u = tid; u < DC * DVB / 8; u += 256) {
+      for (int u = tid; u < DC * DVB / 8; u += 512) {
         const int r = u / (DVB / 8), c8 = u % (DVB / 8) * 8;
         float v[8] = {};
         if (r < len && v0 + c8 < p.dv) load8(osrc + r * q.dos.l + v0 + c8, p.dv - v0 - c8, v);
@@ -544,40 +551,44 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
         const f16x8 y0 = col_frag16<64>(sY, 16 * w, 32 * s, lane), y1 = col_frag16<64>(sY + YE, 16 * w, 32 * s, lane);
         const f16x8 d0 = col_frag16<64>(sD, 16 * w, 32 * s, lane), d1 = col_frag16<64>(sD + YE, 16 * w, 32 * s, lane);
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-          const f16x8 b0 = col_frag16<DKP>(sS, 16 * n, 32 * s, lane), b1 = col_frag16<DKP>(sS + SE, 16 * n, 32 * s, lane);
+        for (int n = 0; n < NSH; ++n) {
+          const int at = 16 * (hf * NSH + n);
+          const f16x8 b0 = col_frag16<DKP>(sS, at, 32 * s, lane), b1 = col_frag16<DKP>(sS + SE, at, 32 * s, lane);
+          const f16x8 n0 = col_frag16<DKP>(sN, at, 32 * s, lane), n1 = col_frag16<DKP>(sN + SE, at, 32 * s, lane);
           aq[n] = mma_h(o0, b0, aq[n]);
-          aq[n] = mma_h(o0, b1, aq[n]);
-          if constexpr (NP == 2) aq[n] = mma_h(o1, b0, aq[n]);
           al[n] = mma_h(y0, b0, al[n]);
-          al[n] = mma_h(y0, b1, al[n]);
-          al[n] = mma_h(y1, b0, al[n]);
-          const f16x8 n0 = col_frag16<DKP>(sN, 16 * n, 32 * s, lane), n1 = col_frag16<DKP>(sN + SE, 16 * n, 32 * s, lane);
           ar[n] = mma_h(d0, n0, ar[n]);
+          aq[n] = mma_h(o0, b1, aq[n]);
+          al[n] = mma_h(y0, b1, al[n]);
           ar[n] = mma_h(d0, n1, ar[n]);
+          if constexpr (NP == 2) aq[n] = mma_h(o1, b0, aq[n]);
+          al[n] = mma_h(y1, b0, al[n]);
           ar[n] = mma_h(d1, n0, ar[n]);
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int m = 0; m < 2; ++m) {
+          const int j = 2 * m + hf;
           if (j > w) continue;
           const f16x8 b0 = col_frag16<64>(sD, 16 * j, 32 * s, lane), b1 = col_frag16<64>(sD + YE, 16 * j, 32 * s, lane);
-          pA[j] = mma_h(y0, b0, pA[j]);
-          pA[j] = mma_h(y0, b1, pA[j]);
-          pA[j] = mma_h(y1, b0, pA[j]);
-          pP[j] = mma_h(o0, b0, pP[j]);
-          pP[j] = mma_h(o0, b1, pP[j]);
-          if constexpr (NP == 2) pP[j] = mma_h(o1, b0, pP[j]);
+          pA[m] = mma_h(y0, b0, pA[m]);
+          pP[m] = mma_h(o0, b0, pP[m]);
+          pA[m] = mma_h(y0, b1, pA[m]);
+          pP[m] = mma_h(o0, b1, pP[m]);
+          pA[m] = mma_h(y1, b0, pA[m]);
+          if constexpr (NP == 2) pP[m] = mma_h(o1, b0, pP[m]);
         }
       }
     }
     // A' and P', what they give dbeta and dG, and the pair terms' matrices
+    const int lane = lane_id_here(), l16 = lane & 15, g4 = lane >> 4;
     const float fA = -(mY * mD), fP = p.scale * (so.inv * mD);
     float rows[4] = {}, xam = 0.f, xpm = 0.f;
     double Gt[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) Gt[r] = sG[16 * w + 4 * g4 + r];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int m = 0; m < 2; ++m) {
+      const int j = 2 * m + hf;
       float colb = 0.f;
       if (j <= w) {
         const double Gj = sG[16 * j + l16];
@@ -586,14 +597,14 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
         for (int r = 0; r < 4; ++r) {
           const int below = 16 * (w - j) + 4 * g4 + r - l16;
           const float d = below >= 0 ? expf((float)(Gt[r] - Gj)) : 0.f;
-          const float xa = below > 0 ? fA * pA[j][r] * d : 0.f, xp = below >= 0 ? fP * pP[j][r] * d : 0.f;
-          const float m = (below > 0 ? xa * kk[j][r] : 0.f) + (below >= 0 ? xp * qk[j][r] : 0.f);
-          colb += m;
-          rows[r] += m * bj;
-          pA[j][r] = xa * bj;
-          pP[j][r] = xp * bj;
-          xam = fmaxf(xam, fabsf(pA[j][r]));
-          xpm = fmaxf(xpm, fabsf(pP[j][r]));
+          const float xa = below > 0 ? fA * pA[m][r] * d : 0.f, xp = below >= 0 ? fP * pP[m][r] * d : 0.f;
+          const float v = (below > 0 ? xa * kk[m][r] : 0.f) + (below >= 0 ? xp * qk[m][r] : 0.f);
+          colb += v;
+          rows[r] += v * bj;
+          pA[m][r] = xa * bj;
+          pP[m][r] = xp * bj;
+          xam = fmaxf(xam, fabsf(pA[m][r]));
+          xpm = fmaxf(xpm, fabsf(pP[m][r]));
         }
       }
       colb += __shfl_xor(colb, 16);
@@ -604,20 +615,20 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
     xpm = wave_max(xpm);
     dot = group_sum<64>(dot);
     if (lane == 0) {
-      red[w][1] = xam;
-      red[w][2] = xpm;
-      red[w][3] = dot;
+      red[wave][1] = xam;
+      red[wave][2] = xpm;
+      red[wave][3] = dot;
     }
     const float fq = p.scale * (so.inv * mS), fl = -(mY * mS), fr = mD * mN;
     float dots[4] = {}, rights[4] = {};
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      // rows 16 w + 4 g + r of channel 16 n + l % 16: half of a fragment by columns
+    for (int n = 0; n < NSH; ++n) {
+      // rows 16 w + 4 g + r of channel l % 16 of tile hf NSH + n: half of a fragment by columns
       f16x8 kf[NP], qf[NP];
 #pragma unroll
       for (int m = 0; m < NP; ++m) {
-        kf[m] = frag(sK, m * F + 2 * n + (w >> 1), lane);
-        qf[m] = frag(sQ, m * F + 2 * n + (w >> 1), lane);
+        kf[m] = frag(sK, m * F + 2 * (hf * NSH + n) + (w >> 1), lane);
+        qf[m] = frag(sQ, m * F + 2 * (hf * NSH + n) + (w >> 1), lane);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -639,17 +650,19 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
       const int t = 16 * w + 4 * g4 + r;
       const float left = group_sum<16>(dots[r] + rows[r]), right = sk * group_sum<16>(rights[r]);
       if (l16 == 0) {
-        sRow[t] = left;
-        sB2[t] = right;
-        sH[t] = sB[t] * right;
+        sRow[hf][t] = left;
+        sB2[hf][t] = right;
       }
     }
     __syncthreads();
-    if (w == 0) {                                // the gates' gradients, a token a lane
+    if (wave == 0) {                             // the gates' gradients, a token a lane
       const float col = (sCol[0][lane] + sCol[1][lane]) + (sCol[2][lane] + sCol[3][lane]);
-      const float hs = group_sum<64>(sH[lane]), all = (red[0][3] + red[1][3]) + (red[2][3] + red[3][3]);
-      float dG = sRow[lane] - sB[lane] * col - sH[lane];
-      const double mine = (double)dG + (lane == 63 ? (double)hs + (double)(sEG[63] * all) : 0.0);
+      const float b2 = sB2[0][lane] + sB2[1][lane], H = sB[lane] * b2;
+      const float hs = group_sum<64>(H);
+      float all = 0.f;
+      for (int i = 0; i < 8; ++i) all += red[i][3];
+      const double mine = (double)(sRow[0][lane] + sRow[1][lane] - sB[lane] * col - H) +
+                          (lane == 63 ? (double)hs + (double)(sEG[63] * all) : 0.0);
       const double upto = wave_scan64(mine);
       const double total = __shfl(upto, 63);
       if (lane < len) {
@@ -658,22 +671,21 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
           const float gv = p.g ? p.g[b * p.gs.b + h * p.gs.h + (int64_t)(t0 + lane) * p.gs.l] : 0.f;
           q.dg[at] = gv < -200.f ? 0.f : (float)(total - upto + mine);
         }
-        if (q.dbeta) q.dbeta[at] = col + sB2[lane];
+        if (q.dbeta) q.dbeta[at] = col + b2;
       }
     }
-    const Scale xa(fmaxf(fmaxf(red[0][1], red[1][1]), fmaxf(red[2][1], red[3][1])));
-    const Scale xp(fmaxf(fmaxf(red[0][2], red[1][2]), fmaxf(red[2][2], red[3][2])));
+    const Scale xa(most(1)), xp(most(2));
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {              // block row w; zeros above the diagonal
-        const int at = TC::at(16 * w + 4 * g4 + r, 16 * j + l16);
-        const f16 a = part_hi(pA[j][r], xa.mult), e = part_hi(pP[j][r], xp.mult);
+        const int at = TC::at(16 * w + 4 * g4 + r, 16 * (2 * m + hf) + l16);
+        const f16 a = part_hi(pA[m][r], xa.mult), e = part_hi(pP[m][r], xp.mult);
         sXa[at] = a;
         sXp[at] = e;
         if constexpr (NP == 2) {
-          sXa[TC::ELEMS + at] = part_lo(pA[j][r], xa.mult, a);
-          sXp[TC::ELEMS + at] = part_lo(pP[j][r], xp.mult, e);
+          sXa[TC::ELEMS + at] = part_lo(pA[m][r], xa.mult, a);
+          sXp[TC::ELEMS + at] = part_lo(pP[m][r], xp.mult, e);
         }
       }
     __syncthreads();
@@ -689,18 +701,18 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
       }
     const float f1 = xp.inv * sk, f2 = xa.inv * sk, f3 = xp.inv * sq;
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
+    for (int n = 0; n < NSH; ++n) {
       f32x4 u1 = {}, u2 = {}, u3 = {};
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const f16x8 k0 = frag(sK, 2 * n + s, lane), q0 = frag(sQ, 2 * n + s, lane);
+        const f16x8 k0 = frag(sK, 2 * (hf * NSH + n) + s, lane), q0 = frag(sQ, 2 * (hf * NSH + n) + s, lane);
         u1 = mma_h(rp[s][0], k0, u1);
         u2 = mma_h(ra[s][0], k0, u2);
         u2 = mma_h(ca[s][0], k0, u2);
         u3 = mma_h(cp[s][0], q0, u3);
         if constexpr (NP == 2) {
-          const f16x8 k1 = frag(sK, F + 2 * n + s, lane);
-          const f16x8 q1 = frag(sQ, F + 2 * n + s, lane);
+          const f16x8 k1 = frag(sK, F + 2 * (hf * NSH + n) + s, lane);
+          const f16x8 q1 = frag(sQ, F + 2 * (hf * NSH + n) + s, lane);
           u1 = mma_h(rp[s][0], k1, u1);
           u1 = mma_h(rp[s][1], k0, u1);
           u2 = mma_h(ra[s][0], k1, u2);
@@ -721,10 +733,10 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaBwdParams q, Delt
   T* dq = reinterpret_cast<T*>(q.dq) + b * q.dqs.b + hk * q.dqs.h;
   T* dk = reinterpret_cast<T*>(q.dk) + b * q.dks.b + hk * q.dks.h;
 #pragma unroll
-  for (int n = 0; n < NS; ++n)
+  for (int n = 0; n < NSH; ++n)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int t = 16 * w + 4 * g4 + r, col = 16 * n + l16;
+      const int t = 16 * w + 4 * g4 + r, col = 16 * (hf * NSH + n) + l16;
       if (t < len && col < p.dk) {
         dq[(int64_t)(t0 + t) * q.dqs.l + col] = from_f32<T>(tq[n][r]);
         dk[(int64_t)(t0 + t) * q.dks.l + col] = from_f32<T>(tk[n][r]);
@@ -740,7 +752,7 @@ hipError_t run_bwd(const DeltaBwdParams& q, hipStream_t st) {
   delta_back_scan_kernel<T, DKP><<<head_block_grid(p.batch * p.heads, nwg), sizeof(T) == 4 ? 256 : 384, 0, st>>>(q, lay, nblk, nwg);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  delta_grads_kernel<T, DKP><<<(unsigned)((int64_t)p.batch * p.kheads * p.pieces), 256, 0, st>>>(q, lay, nblk);
+  delta_grads_kernel<T, DKP><<<(unsigned)((int64_t)p.batch * p.kheads * p.pieces), 512, 0, st>>>(q, lay, nblk);
   return hipGetLastError();
 }
 

@@ -18,7 +18,7 @@ namespace {
 // wave j builds block column j downwards, T_ij = -T_ii sum_k A_ik T_kj, with fp32 matrix instructions, T_kj staying in
 // accumulators, which are the B operand of the next product.
 template <typename T, int DKP>
-__global__ __launch_bounds__(256) void delta_prep_kernel(DeltaParams p, DeltaLayout lay, int backward) {
+__global__ __launch_bounds__(256, 2) void delta_prep_kernel(DeltaParams p, DeltaLayout lay, int backward) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
   constexpr int CPR = DKP / 8;                   // threads of 8 channels for a row
   constexpr int RPP = 256 / CPR;                 // rows of a pass
