@@ -117,16 +117,31 @@ __device__ __forceinline__ float abs_max(const f32x4 (&t)[N], float m = 0.f) {
 // A gate's logarithm as the kernels take it: e^-200 is 0 in fp32 as e^-inf is, and sums of it stay finite.
 __device__ __forceinline__ float gate_log(float g) { return g < -200.f ? -200.f : g; }
 
-// Inclusive sums over the wave's 64 lanes in fp64: differences of sums keep fp32's precision however far the sums went.
-__device__ __forceinline__ double wave_scan64(double v) {
-  const int l = threadIdx.x & 63;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const double o = __shfl_up(v, off, 64);
-    if (l >= off) v += o;
-  }
-  return v;
+// Inclusive sums over the wave's 64 lanes in fp64 (differences of sums keep fp32's precision however far the sums went), by
+// the row shifts and broadcasts of wave_incl_scan_dpp on both halves of a value.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double add_dpp64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+  return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
+__device__ __forceinline__ double wave_scan64(double v) {
+  v = add_dpp64<0x111, 0xf>(v);
+  v = add_dpp64<0x112, 0xf>(v);
+  v = add_dpp64<0x114, 0xf>(v);
+  v = add_dpp64<0x118, 0xf>(v);
+  v = add_dpp64<0x142, 0xa>(v);
+  return add_dpp64<0x143, 0xc>(v);
+}
+__device__ __forceinline__ double last_lane64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, 63), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), 63);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// e^x for x log2 e in fp64 (sums of gates are kept so): v_exp_f32, 1 ulp, of its nearest fp32.
+constexpr double kLog2e64 = 1.4426950408889634;
+__device__ __forceinline__ float exp_of(double x) { return __builtin_amdgcn_exp2f((float)x); }
 
 // ------------------------------------------------------------------ workspace
 // Operands are kept as the instructions take them, a fragment of 64 lanes x 8 values (1 KB) after the other, so that they

@@ -383,8 +383,8 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
   const DeltaParams& p = q.f;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), w = wave & 3, hf = wave >> 2, l16 = lane & 15, g4 = lane >> 4;
-  const int64_t unit = blockIdx.x;
-  const int c = (int)(unit % p.pieces), bk = (int)(unit / p.pieces), hk = bk % p.kheads, b = bk / p.kheads;
+  const int unit = blockIdx.x;
+  const int c = unit % p.pieces, bk = unit / p.pieces, hk = bk % p.kheads, b = bk / p.kheads;
   const int t0 = c * DC, len = min(DC, p.seqlen - t0), rep = p.heads / p.kheads;
   const f16* kq = reinterpret_cast<const f16*>(p.workspace + lay.kq + unit * lay.kq_unit);       // Q, K by rows
   for (int i = tid; i < 2 * NP * F * 64; i += 512)                     // K, Q by columns
@@ -454,12 +454,11 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
         if (p.g) gv = gate_log(p.g[b * p.gs.b + h * p.gs.h + (int64_t)(t0 + lane) * p.gs.l]);
         bv = p.beta ? p.beta[b * p.bs.b + h * p.bs.h + (int64_t)(t0 + lane) * p.bs.l] : 1.f;
       }
-      const double G = wave_scan64((double)gv);
-      const double end = __shfl(G, 63);
+      const double G = wave_scan64((double)gv * kLog2e64), end = last_lane64(G);
       sG[lane] = G;
       sB[lane] = bv;
-      sEG[lane] = expf((float)G);
-      sEnd[lane] = expf((float)(end - G));
+      sEG[lane] = exp_of(G);
+      sEnd[lane] = exp_of(end - G);
     }
     __syncthreads();
     auto most = [&](int i) {
@@ -596,7 +595,7 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int below = 16 * (w - j) + 4 * g4 + r - l16;
-          const float d = below >= 0 ? expf((float)(Gt[r] - Gj)) : 0.f;
+          const float d = below >= 0 ? exp_of(Gt[r] - Gj) : 0.f;
           const float xa = below > 0 ? fA * pA[m][r] * d : 0.f, xp = below >= 0 ? fP * pP[m][r] * d : 0.f;
           const float v = (below > 0 ? xa * kk[m][r] : 0.f) + (below >= 0 ? xp * qk[m][r] : 0.f);
           colb += v;
@@ -664,7 +663,7 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
       const double mine = (double)(sRow[0][lane] + sRow[1][lane] - sB[lane] * col - H) +
                           (lane == 63 ? (double)hs + (double)(sEG[63] * all) : 0.0);
       const double upto = wave_scan64(mine);
-      const double total = __shfl(upto, 63);
+      const double total = last_lane64(upto);
       if (lane < len) {
         const int64_t at = ((int64_t)b * p.heads + h) * p.seqlen + t0 + lane;
         if (q.dg) {

@@ -12,51 +12,77 @@ namespace mh {
 namespace {
 
 // ------------------------------------------------------------------ pieces side by side
-// One workgroup of 4 waves for a piece of a key head: K and Q into their fp16 parts (kept for the scan), K K^T and Q K^T
-// once (wave w: rows 16 w .. 16 w + 15, tiles up to the diagonal), then for each value head that shares them A, its
-// inverse and P.  The inverse in fp32: every wave solves one 16 x 16 diagonal block by substitution, a column a lane, then
-// wave j builds block column j downwards, T_ij = -T_ii sum_k A_ik T_kj, with fp32 matrix instructions, T_kj staying in
-// accumulators, which are the B operand of the next product.
+// One workgroup of 4 waves for a piece of a key head: K and Q into their fp16 parts and fragments (kept for the scans), K K^T
+// and K Q^T once, then for each value head that shares them A, its inverse and P.  Everything is transposed: wave w has the
+// tokens t = 16 w + l % 16 as columns and the tokens j <= t as rows of its accumulators, which are then the fragments of T
+// and P by rows as they stand.  The inverse in fp32: every wave solves one 16 x 16 diagonal block by substitution, a column
+// a lane, then wave w builds block row w of T from the diagonal outwards, T_wj = -(sum over j < k <= w of T_wk A_kj) T_jj,
+// with fp32 matrix instructions, T_wk staying in accumulators, which are the B operand of the next product.
+// Bound by latencies (LDS, substitution); four workgroups a CU hide each other's.
 template <typename T, int DKP>
-__global__ __launch_bounds__(256, 2) void delta_prep_kernel(DeltaParams p, DeltaLayout lay, int backward) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void delta_prep_kernel(DeltaParams p, DeltaLayout lay, int backward) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
   constexpr int CPR = DKP / 8;                   // threads of 8 channels for a row
   constexpr int RPP = 256 / CPR;                 // rows of a pass
+  constexpr int F = kKFrags<DKP>, KS = DKP / 32;
   using TK = HTile<DKP>;
   using TC = HTile<64>;
-  constexpr int AP = 68;                         // pitch of A and of the diagonal blocks' inverses
-  __shared__ __align__(16) f16 tiles[2 * NP * TK::ELEMS > 4 * TC::ELEMS ? 2 * NP * TK::ELEMS : 4 * TC::ELEMS];
-  __shared__ __align__(16) float sA[DC * AP];
+  constexpr int AP = 68;                         // pitch of A
+  constexpr int HALFS = 2 * NP * TK::ELEMS > 4 * TC::ELEMS ? 2 * NP * TK::ELEMS : 4 * TC::ELEMS;
+  static_assert(HALFS * 2 >= DC * AP * 4, "A takes the tiles' place");
+  __shared__ __align__(16) f16 tiles[HALFS];     // K and Q, then A, then T and P for the fragments by columns
   __shared__ __align__(16) float sD[4 * 16 * 20];
-  __shared__ double sG[DC];
-  __shared__ float sB[DC], sVec[2 * DC], red[4][2];
+  __shared__ __align__(16) double sG[DC];        // sums of gates times log2 e
+  __shared__ __align__(16) float sB[DC], sVec[2 * DC];
+  __shared__ float red[4][2];
+  float* const sA = reinterpret_cast<float*>(tiles);                   // A^T: row j, column t
 
   const int tid = threadIdx.x, lane = tid & 63, w = wave_id(), l16 = lane & 15, g4 = lane >> 4;
-  const int64_t unit = blockIdx.x;               // (batch, key head, piece)
-  const int c = (int)(unit % p.pieces), bk = (int)(unit / p.pieces), hk = bk % p.kheads, b = bk / p.kheads;
+  const int unit = blockIdx.x;                   // (batch, key head, piece)
+  const int c = unit % p.pieces, bk = unit / p.pieces, hk = bk % p.kheads, b = bk / p.kheads;
   const int t0 = c * DC, len = min(DC, p.seqlen - t0), rep = p.heads / p.kheads;
 
-  // K and Q: largest magnitudes, then parts into the tiles
+  float gv = 0.f, bv = 0.f;                      // wave 0: of the lane's token, a head ahead
+  auto load_gates = [&](int h) {
+    if (w != 0) return;
+    const int t = t0 + min(lane, len - 1);
+    gv = p.g ? p.g[b * p.gs.b + h * p.gs.h + t * p.gs.l] : 0.f;
+    bv = p.beta ? p.beta[b * p.bs.b + h * p.bs.h + t * p.bs.l] : 1.f;
+  };
+
+  // K and Q: largest magnitudes, then parts into the tiles.  Rows and channels beyond the last are read within the tensor
+  // and cleared, so that all loads are under way at once.
   Raw8<T> raw[2][DC / RPP];
   const int cc = tid % CPR, rr = tid / CPR;
-  const T* src[2] = {reinterpret_cast<const T*>(p.k) + b * p.ks.b + hk * p.ks.h + (int64_t)t0 * p.ks.l + cc * 8,
-                     reinterpret_cast<const T*>(p.q) + b * p.qs.b + hk * p.qs.h + (int64_t)t0 * p.qs.l + cc * 8};
+  const bool cok = cc * 8 < p.dk;
+  const T* src[2] = {reinterpret_cast<const T*>(p.k) + b * p.ks.b + hk * p.ks.h + t0 * p.ks.l,
+                     reinterpret_cast<const T*>(p.q) + b * p.qs.b + hk * p.qs.h + t0 * p.qs.l};
   const int64_t sl[2] = {p.ks.l, p.qs.l};
+  if (p.dk % 8 == 0) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int i = 0; i < DC / RPP; ++i) raw[x][i].load(src[x] + min(i * RPP + rr, len - 1) * sl[x] + (cok ? cc * 8 : 0));
+    load_gates(hk * rep);
+  } else {
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int i = 0; i < DC / RPP; ++i) {
+        raw[x][i].clear();
+        if (cok) load_raw(raw[x][i], src[x] + min(i * RPP + rr, len - 1) * sl[x] + cc * 8, p.dk - cc * 8);
+      }
+    load_gates(hk * rep);
+  }
   float amax[2] = {0.f, 0.f};
-#pragma unroll
-  for (int x = 0; x < 2; ++x)
-#pragma unroll
-    for (int i = 0; i < DC / RPP; ++i) {
-      const int r = i * RPP + rr;
-      if (r < len && cc * 8 < p.dk) load_raw(raw[x][i], src[x] + r * sl[x], p.dk - cc * 8);
-      else raw[x][i].clear();
-    }
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
 #pragma unroll
-    for (int i = 0; i < DC / RPP; ++i)
+    for (int i = 0; i < DC / RPP; ++i) {
+      if (!cok || i * RPP + rr >= len) raw[x][i].clear();
 #pragma unroll
       for (int j = 0; j < 8; ++j) amax[x] = fmaxf(amax[x], fabsf(raw[x][i].get(j)));
+    }
     amax[x] = wave_max(amax[x]);
     if (lane == 0) red[w][x] = amax[x];
   }
@@ -67,7 +93,6 @@ __global__ __launch_bounds__(256, 2) void delta_prep_kernel(DeltaParams p, Delta
   for (int x = 0; x < 2; ++x)
 #pragma unroll
     for (int i = 0; i < DC / RPP; ++i) {
-      const int r = i * RPP + rr;
       const float mult = x ? sq.mult : sk.mult;
       f16x8 hi, lo;
 #pragma unroll
@@ -76,56 +101,49 @@ __global__ __launch_bounds__(256, 2) void delta_prep_kernel(DeltaParams p, Delta
         hi[j] = part_hi(v, mult);
         if constexpr (NP == 2) lo[j] = part_lo(v, mult, hi[j]);
       }
-      f16* to = tiles + x * NP * TK::ELEMS + TK::at(r, cc * 8);
+      f16* to = tiles + x * NP * TK::ELEMS + TK::at(i * RPP + rr, cc * 8);
       *reinterpret_cast<f16x8*>(to) = hi;
       if constexpr (NP == 2) *reinterpret_cast<f16x8*>(to + TK::ELEMS) = lo;
     }
   __syncthreads();
+  f32x4 kk[4] = {}, qk[4] = {};                  // rows j = 16 n + 4 g4 + r, column t = 16 w + l16
   {
-    constexpr int F = kKFrags<DKP>, KS = DKP / 32;
     f16* out = reinterpret_cast<f16*>(p.workspace + lay.kq + unit * lay.kq_unit);
 #pragma unroll
-    for (int n = 0; n < NP; ++n) {
-      const f16 *kt = tiles + n * TK::ELEMS, *qt = tiles + (NP + n) * TK::ELEMS;
+    for (int s = 0; s < KS; ++s) {
+      f16x8 kb[NP], qb[NP];
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {             // rows 16 w ..
-        put_frag(out, n * F + w * KS + s, lane, row_frag16<DKP>(qt, 16 * w, 32 * s, lane));
-        put_frag(out, (NP + n) * F + w * KS + s, lane, row_frag16<DKP>(kt, 16 * w, 32 * s, lane));
+      for (int n = 0; n < NP; ++n) {
+        qb[n] = row_frag16<DKP>(tiles + (NP + n) * TK::ELEMS, 16 * w, 32 * s, lane);
+        kb[n] = row_frag16<DKP>(tiles + n * TK::ELEMS, 16 * w, 32 * s, lane);
+        put_frag(out, n * F + w * KS + s, lane, qb[n]);
+        put_frag(out, (NP + n) * F + w * KS + s, lane, kb[n]);
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (j > w) continue;
+        const f16x8 a0 = row_frag16<DKP>(tiles, 16 * j, 32 * s, lane);
+        kk[j] = mma_h(a0, kb[0], kk[j]);
+        qk[j] = mma_h(a0, qb[0], qk[j]);
+        if constexpr (NP == 2) {
+          const f16x8 a1 = row_frag16<DKP>(tiles + TK::ELEMS, 16 * j, 32 * s, lane);
+          kk[j] = mma_h(a1, kb[0], kk[j]);
+          kk[j] = mma_h(a0, kb[1], kk[j]);
+          qk[j] = mma_h(a1, qb[0], qk[j]);
+          qk[j] = mma_h(a0, qb[1], qk[j]);
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NP; ++n)
 #pragma unroll
       for (int m = 0; m < DKP / 64; ++m)         // channels 16 (4 m + w) ..
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const int at = 2 * (4 * m + w) + s;
-          put_frag(out, (2 * NP + n) * F + at, lane, col_frag16<DKP>(kt, 16 * (4 * m + w), 32 * s, lane));
-          if (backward) put_frag(out, (3 * NP + n) * F + at, lane, col_frag16<DKP>(qt, 16 * (4 * m + w), 32 * s, lane));
+          put_frag(out, (2 * NP + n) * F + at, lane, col_frag16<DKP>(tiles + n * TK::ELEMS, 16 * (4 * m + w), 32 * s, lane));
+          if (backward) put_frag(out, (3 * NP + n) * F + at, lane, col_frag16<DKP>(tiles + (NP + n) * TK::ELEMS, 16 * (4 * m + w), 32 * s, lane));
         }
-    }
-  }
-  // rows 16 w .. of K K^T and Q K^T, tiles j <= w
-  f32x4 kk[4] = {}, qk[4] = {};
-#pragma unroll
-  for (int s = 0; s < DKP / 32; ++s) {
-    f16x8 ka[NP], qa[NP];
-#pragma unroll
-    for (int n = 0; n < NP; ++n) {
-      ka[n] = row_frag16<DKP>(tiles + n * TK::ELEMS, 16 * w, 32 * s, lane);
-      qa[n] = row_frag16<DKP>(tiles + (NP + n) * TK::ELEMS, 16 * w, 32 * s, lane);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (j > w) continue;
-      const f16x8 kb = row_frag16<DKP>(tiles, 16 * j, 32 * s, lane);
-      kk[j] = mma_h(ka[0], kb, kk[j]);
-      qk[j] = mma_h(qa[0], kb, qk[j]);
-      if constexpr (NP == 2) {
-        const f16x8 kl = row_frag16<DKP>(tiles + TK::ELEMS, 16 * j, 32 * s, lane);
-        kk[j] = mma_h(ka[0], kl, kk[j]);
-        kk[j] = mma_h(ka[1], kb, kk[j]);
-        qk[j] = mma_h(qa[0], kl, qk[j]);
-        qk[j] = mma_h(qa[1], kb, qk[j]);
-      }
-    }
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j)
@@ -138,81 +156,80 @@ __global__ __launch_bounds__(256, 2) void delta_prep_kernel(DeltaParams p, Delta
   for (int hr = 0; hr < rep; ++hr) {
     const int h = hk * rep + hr;
     const int64_t vunit = ((int64_t)b * p.heads + h) * p.pieces + c;
-    __syncthreads();                             // the tiles and the last head's parts have been read
     if (w == 0) {
-      float gv = 0.f, bv = 0.f;
-      if (lane < len) {
-        if (p.g) gv = gate_log(p.g[b * p.gs.b + h * p.gs.h + (int64_t)(t0 + lane) * p.gs.l]);
-        bv = p.beta ? p.beta[b * p.bs.b + h * p.bs.h + (int64_t)(t0 + lane) * p.bs.l] : 1.f;
-      }
-      const double G = wave_scan64((double)gv);
-      const double end = __shfl(G, 63);
+      const double G = wave_scan64(lane < len ? (double)gate_log(gv) * kLog2e64 : 0.);
+      const double end = last_lane64(G);
+      const float beta = lane < len ? bv : 0.f;
       sG[lane] = G;
-      sB[lane] = bv;
-      sVec[lane] = expf((float)G);
-      sVec[DC + lane] = bv * expf((float)(end - G));
+      sB[lane] = beta;
+      sVec[lane] = exp_of(G);
+      sVec[DC + lane] = beta * exp_of(end - G);
+      if (hr + 1 < rep) load_gates(h + 1);
     }
-    __syncthreads();
-    double Gt[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) Gt[r] = sG[16 * w + 4 * g4 + r];
+    __syncthreads();                             // and the tiles or the last head's parts have been read
+    const double Gt = sG[16 * w + l16];
     f32x4 P[4] = {};
     float pmax = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (j > w) continue;
-      const double Gj = sG[16 * j + l16];
-      const float bj = sB[16 * j + l16];
+      const f32x4 bj = *reinterpret_cast<const f32x4*>(sB + 16 * j + 4 * g4);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int below = 16 * (w - j) + 4 * g4 + r - l16;               // t - j
-        const float d = below >= 0 ? expf((float)(Gt[r] - Gj)) * bj : 0.f;
+        const int below = 16 * (w - j) + l16 - 4 * g4 - r;               // t - j
+        const float d = below >= 0 ? exp_of(Gt - sG[16 * j + 4 * g4 + r]) * bj[r] : 0.f;
         P[j][r] = below >= 0 ? qk[j][r] * d : 0.f;
         pmax = fmaxf(pmax, fabsf(P[j][r]));
-        sA[(16 * w + 4 * g4 + r) * AP + 16 * j + l16] = below > 0 ? kk[j][r] * d : 0.f;
+        sA[(16 * j + 4 * g4 + r) * AP + 16 * w + l16] = below > 0 ? kk[j][r] * d : 0.f;
       }
     }
     __syncthreads();
-    // diagonal block w, a column a lane (the four groups of 16 lanes do the same)
+    // T^T of diagonal block w, a column a lane (the four groups of 16 lanes do the same), from the last row up
     {
+      const float* at = sA + (16 * w) * AP + 16 * w;
       float x[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float s = i == l16 ? 1.f : 0.f;
+      for (int i = 15; i >= 0; --i) {
+        float s0 = i == l16 ? 1.f : 0.f, s1 = 0.f;
 #pragma unroll
-        for (int j4 = 0; j4 < (i + 3) / 4; ++j4) {
-          const f32x4 a = *reinterpret_cast<const f32x4*>(sA + (16 * w + i) * AP + 16 * w + 4 * j4);
+        for (int j4 = (i + 1) / 4; j4 < 4; ++j4) {
+          const f32x4 a = *reinterpret_cast<const f32x4*>(at + i * AP + 4 * j4);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (4 * j4 + j < i) s -= a[j] * x[4 * j4 + j];
+            if (4 * j4 + j > i) (j & 1 ? s1 : s0) -= a[j] * x[4 * j4 + j];
         }
-        x[i] = s;
+        x[i] = s0 + s1;
+        if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);             // the rows' reads in four lots, not all held at once
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (g4 == i >> 2) sD[(w * 16 + i) * 20 + l16] = x[i];
     }
     __syncthreads();
-    // block column w downwards
+    // block row w of T, transposed, from the diagonal outwards
     f32x4 t[4] = {};
 #pragma unroll
-    for (int r = 0; r < 4; ++r) t[0][r] = sD[(w * 16 + 4 * g4 + r) * 20 + l16];      // t[n]: block row w + n
+    for (int i = 0; i < 4; ++i)
+      if (i == w)
 #pragma unroll
-    for (int n = 1; n < 4; ++n) {
-      if (w + n > 3) continue;
-      f32x4 m = {};
+        for (int r = 0; r < 4; ++r) t[i][r] = sD[(w * 16 + 4 * g4 + r) * 20 + l16];
 #pragma unroll
-      for (int k = 0; k < n; ++k) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(sA + (16 * (w + n) + l16) * AP + 16 * (w + k) + 4 * g4);
+    for (int j = 2; j >= 0; --j) {
+      if (j >= w) continue;
+      f32x4 m0 = {}, m1 = {};
 #pragma unroll
-        for (int s = 0; s < 4; ++s) m = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], t[k][s], m, 0, 0, 0);
+      for (int k = j + 1; k < 4; ++k) {
+        if (k > w) continue;
+        const f32x4 a = *reinterpret_cast<const f32x4*>(sA + (16 * j + l16) * AP + 16 * k + 4 * g4);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) (s & 1 ? m1 : m0) = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], t[k][s], s & 1 ? m1 : m0, 0, 0, 0);
       }
-      const f32x4 d = *reinterpret_cast<const f32x4*>(sD + ((w + n) * 16 + l16) * 20 + 4 * g4);
-      f32x4 y = {};
+      const f32x4 d = *reinterpret_cast<const f32x4*>(sD + (j * 16 + l16) * 20 + 4 * g4);
+      f32x4 y0 = {}, y1 = {};
 #pragma unroll
-      for (int s = 0; s < 4; ++s) y = __builtin_amdgcn_mfma_f32_16x16x4f32(d[s], m[s], y, 0, 0, 0);
+      for (int s = 0; s < 4; ++s) (s & 1 ? y1 : y0) = __builtin_amdgcn_mfma_f32_16x16x4f32(d[s], m0[s] + m1[s], s & 1 ? y1 : y0, 0, 0, 0);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) t[n][r] = -y[r];
+      for (int r = 0; r < 4; ++r) t[j][r] = -(y0[r] + y1[r]);
     }
     const float tm = wave_max(abs_max(t)), pm = wave_max(pmax);
     if (lane == 0) {
@@ -222,47 +239,51 @@ __global__ __launch_bounds__(256, 2) void delta_prep_kernel(DeltaParams p, Delta
     __syncthreads();
     const Scale st(fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0])));
     const Scale sp(fmaxf(fmaxf(red[0][1], red[1][1]), fmaxf(red[2][1], red[3][1])));
-#pragma unroll
-    for (int i = 0; i < 4; ++i)                  // T: block rows i of block column w; P: block columns i of block row w
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float v = 0.f;
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-          if (i == w + n) v = t[n][r];
-        const int at = TC::at(16 * i + 4 * g4 + r, 16 * w + l16), pt = TC::at(16 * w + 4 * g4 + r, 16 * i + l16);
-        const f16 th = part_hi(v, st.mult), ph = part_hi(P[i][r], sp.mult);
-        tiles[at] = th;
-        tiles[TC::ELEMS + at] = part_lo(v, st.mult, th);
-        tiles[2 * TC::ELEMS + pt] = ph;
-        tiles[3 * TC::ELEMS + pt] = part_lo(P[i][r], sp.mult, ph);
-      }
-    __syncthreads();
+    f16x8 th[2], tl[2], ph[2], pl[2];
+    parts_of<2>(t, st.mult, th, tl);
+    parts_of<2>(P, sp.mult, ph, pl);
     f16* out = reinterpret_cast<f16*>(p.workspace + lay.tp + vunit * lay.tp_unit);
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {                // wave w: block row (or column) w
-      const f16 *tt = tiles + n * TC::ELEMS, *pt = tiles + (2 + n) * TC::ELEMS;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if (w >= 2 * s) {
-          put_frag(out, n * kTFrags + t_frag(w, s), lane, row_frag16<64>(tt, 16 * w, 32 * s, lane));
-          if (!backward) put_frag(out, (2 + n) * kTFrags + t_frag(w, s), lane, row_frag16<64>(pt, 16 * w, 32 * s, lane));
-        }
-        if (backward && w < 2 + 2 * s) {
-          put_frag(out, (2 + n) * kTFrags + tt_frag(w, s), lane, col_frag16<64>(tt, 16 * w, 32 * s, lane));
-          put_frag(out, (4 + n) * kTFrags + tt_frag(w, s), lane, col_frag16<64>(pt, 16 * w, 32 * s, lane));
+    for (int s = 0; s < 2; ++s)
+      if (w >= 2 * s) {
+        put_frag(out, t_frag(w, s), lane, th[s]);
+        put_frag(out, kTFrags + t_frag(w, s), lane, tl[s]);
+        if (!backward) {
+          put_frag(out, 2 * kTFrags + t_frag(w, s), lane, ph[s]);
+          put_frag(out, 3 * kTFrags + t_frag(w, s), lane, pl[s]);
         }
       }
+    if (backward) {                              // by columns: through LDS, as T^T and P^T (row j, column t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int at = TC::at(16 * j + 4 * g4 + r, 16 * w + l16), e = 4 * (j & 1) + r;
+          tiles[at] = th[j >> 1][e];
+          tiles[TC::ELEMS + at] = tl[j >> 1][e];
+          tiles[2 * TC::ELEMS + at] = ph[j >> 1][e];
+          tiles[3 * TC::ELEMS + at] = pl[j >> 1][e];
+        }
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+          if (w < 2 + 2 * s) {
+            put_frag(out, (2 + n) * kTFrags + tt_frag(w, s), lane, row_frag16<64>(tiles + n * TC::ELEMS, 16 * w, 32 * s, lane));
+            put_frag(out, (4 + n) * kTFrags + tt_frag(w, s), lane, row_frag16<64>(tiles + (2 + n) * TC::ELEMS, 16 * w, 32 * s, lane));
+          }
     }
     float* vec = reinterpret_cast<float*>(p.workspace + lay.vec) + vunit * kVecFloats;
     if (tid < 2 * DC) vec[tid] = sVec[tid];
     if (tid == 2 * DC) {
-      vec[VEC_W + DC] = sVec[DC - 1];
+      vec[VEC_GAMMA] = sVec[DC - 1];
       vec[VEC_ST] = st.inv;
       vec[VEC_SP] = sp.inv;
       vec[VEC_SK] = sk.inv;
       vec[VEC_SQ] = sq.inv;
     }
+    if (hr + 1 < rep) __syncthreads();           // sVec and the parts have been read
   }
 }
 
