@@ -153,7 +153,7 @@ __device__ __forceinline__ float exp_of(double x) { return __builtin_amdgcn_exp2
 //   `vec` for the same: e^{G_t}, beta_t e^{G_end - G_t}, then e^{G_end} and the scales of T, P, K and Q.
 //   For the backward, for each (batch, value head, piece, 16 columns of v): the entering state, its gradient behind the
 //     piece, delta and y, two parts each, in the order in which waves hold them as operands ([part][k-step]), and the
-//     scales of their columns in either half of the rows ([half][which][column]).
+//     scales of their columns in either half of the rows ([half][which][column]), then those of dO's columns.
 constexpr int FR = 512;                          // halfs of a fragment
 template <int DKP> constexpr int kKFrags = DKP / 8;                    // of K or Q, rows or columns
 constexpr int kTFrags = 6;
@@ -165,6 +165,7 @@ __device__ __forceinline__ void put_frag(f16* t, int f, int lane, f16x8 v) { *re
 constexpr int kVecFloats = 256;
 enum { VEC_W = 64, VEC_GAMMA = 128, VEC_ST, VEC_SP, VEC_SK, VEC_SQ };
 enum { KEEP_S, KEEP_DS, KEEP_D, KEEP_Y };
+constexpr int kScales = 160;                     // floats, 16 of them unused
 template <int DKP> constexpr size_t keep_halfs() { return 2 * (2 * 16 * DKP) + 2 * (2 * 16 * DC); }
 template <int DKP> constexpr int keep_at(int which) {                  // where one of the four begins, in halfs
   return which < KEEP_D ? which * 2 * 16 * DKP : 4 * 16 * DKP + (which - KEEP_D) * 2 * 16 * DC;
@@ -194,7 +195,7 @@ struct DeltaLayout {
     tp = take(pieces * tp_unit);
     vec = take(pieces * kVecFloats * 4);
     keep = take(blocks * (dkp == 64 ? keep_halfs<64>() : keep_halfs<128>()) * 2);
-    scales = take(blocks * 512);
+    scales = take(blocks * kScales * 4);
     total = at;
   }
 };

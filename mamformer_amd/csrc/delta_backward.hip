@@ -333,12 +333,13 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_back_scan_ke
       parts_of<2>(Yv, sy.mult, yh, yl);
       const int64_t at = (vunit0 + c) * nblk + blk;
       f16* keep = reinterpret_cast<f16*>(p.workspace + lay.keep) + at * (int64_t)keep_halfs<DKP>();
-      float* scales = reinterpret_cast<float*>(p.workspace + lay.scales) + at * 128 + 64 * hf + l16;
+      float* scales = reinterpret_cast<float*>(p.workspace + lay.scales) + at * kScales + 64 * hf + l16;
       keep_parts<KS>(keep + keep_at<DKP>(KEEP_DS), hf * KSH, sh, sl, lane);
       keep_parts<2>(keep + keep_at<DKP>(KEEP_Y), hf, yh, yl, lane);
       if (g4 == 0) {
         scales[16 * KEEP_DS] = ss.inv;
         scales[16 * KEEP_Y] = sy.inv * ysc;
+        if (hf == 0) scales[128] = so.inv;       // over all tokens in either half
       }
     }
   }
@@ -387,8 +388,13 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
   const int c = unit % p.pieces, bk = unit / p.pieces, hk = bk % p.kheads, b = bk / p.kheads;
   const int t0 = c * DC, len = min(DC, p.seqlen - t0), rep = p.heads / p.kheads;
   const f16* kq = reinterpret_cast<const f16*>(p.workspace + lay.kq + unit * lay.kq_unit);       // Q, K by rows
-  for (int i = tid; i < 2 * NP * F * 64; i += 512)                     // K, Q by columns
-    reinterpret_cast<f16x8*>(sK)[i] = reinterpret_cast<const f16x8*>(kq + 2 * NP * F * FR)[i];
+  {
+    f16x8 v[2 * NP * F / 8];                     // K, Q by columns
+#pragma unroll
+    for (int i = 0; i < 2 * NP * F / 8; ++i) v[i] = frag(kq, 2 * NP * F + 8 * i + wave, lane);
+#pragma unroll
+    for (int i = 0; i < 2 * NP * F / 8; ++i) put_frag(sK, 8 * i + wave, lane, v[i]);
+  }
   const float* vec0 = reinterpret_cast<const float*>(p.workspace + lay.vec) +
                       (((int64_t)b * p.heads + hk * rep) * p.pieces + c) * kVecFloats;
   const float sk = vec0[VEC_SK], sq = vec0[VEC_SQ];
@@ -426,122 +432,152 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
       qk[m][r] = qk[m][r] * sq * sk;
     }
 
+  // What a stage (DVB columns of v of a head) has to load, under way while the one before it is multiplied: a lane's 8
+  // values of a k-step (rows 4 g .. and 16 + 4 g .. of 32, of column l % 16) of S, dS, delta and y, 8 columns of dO's row.
+  constexpr int SU = (SE / 8 + 511) / 512, YU = YE / 8, OU = DC * DVB / 8;
+  static_assert(YU <= 512 && OU <= 512, "one unit a thread");
+  f16x8 ps[SU][4], pd[4];
+  Raw8<T> po;
+  float fs[SU][2], fd[2], mx = 0.f, mo = 0.f;    // scales of the units' columns; a head's, lane 16 i + column: of scale i
+  auto vunit_of = [&](int hr) { return ((int64_t)b * p.heads + hk * rep + hr) * p.pieces + c; };
+  auto scales_of = [&](int hr) { return reinterpret_cast<const float*>(p.workspace + lay.scales) + vunit_of(hr) * nblk * kScales; };
+  auto load_stage = [&](int hr, int v0) {
+    const int lane = lane_id_here(), tid = 64 * wave + lane;           // addresses formed here, not held for the loops
+    const f16* keep0 = reinterpret_cast<const f16*>(p.workspace + lay.keep) + vunit_of(hr) * nblk * (int64_t)keep_halfs<DKP>();
+    const float* scales = scales_of(hr);
+#pragma unroll
+    for (int i = 0; i < SU; ++i) {
+      const int u = tid + 512 * i, blk = v0 / 16 + u / (16 * DKP / 8), k = u / 64 % KS;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ps[i][j] = f16x8{};
+      fs[i][0] = fs[i][1] = 0.f;
+      if (u < SE / 8 && blk < nblk) {
+        const f16* from = keep0 + blk * (int64_t)keep_halfs<DKP>() + (k * 64 + lane) * 8;
+        ps[i][0] = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_S));
+        ps[i][1] = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_S) + 16 * DKP);
+        ps[i][2] = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_DS));
+        ps[i][3] = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_DS) + 16 * DKP);
+        const float* f = scales + kScales * blk + (k >= KS / 2 ? 64 : 0) + (lane & 15);
+        fs[i][0] = f[16 * KEEP_S];
+        fs[i][1] = f[16 * KEEP_DS];
+      }
+    }
+    {
+      const int blk = v0 / 16 + tid / 128, k = tid / 64 % 2;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) pd[j] = f16x8{};
+      fd[0] = fd[1] = 0.f;
+      if (tid < YU && blk < nblk) {
+        const f16* from = keep0 + blk * (int64_t)keep_halfs<DKP>() + (k * 64 + lane) * 8;
+        pd[0] = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_D));
+        pd[1] = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_D) + 16 * DC);
+        pd[2] = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_Y));
+        pd[3] = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_Y) + 16 * DC);
+        const float* f = scales + kScales * blk + 64 * k + (lane & 15);
+        fd[0] = f[16 * KEEP_D];
+        fd[1] = f[16 * KEEP_Y];
+      }
+    }
+    const int r = tid / (DVB / 8), c8 = v0 + tid % (DVB / 8) * 8;
+    po.clear();
+    if (tid < OU && r < len && c8 < p.dv)
+      load_raw(po, reinterpret_cast<const T*>(q.d_o) + b * q.dos.b + (hk * rep + hr) * q.dos.h + (int64_t)(t0 + r) * q.dos.l + c8, p.dv - c8);
+  };
+  auto load_scales = [&](int hr) {
+    const int lane = lane_id_here();
+    const float* scales = scales_of(hr);
+    mx = mo = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < nblk; ++i) {
+      mx = fmaxf(mx, fmaxf(scales[kScales * i + lane], scales[kScales * i + 64 + lane]));
+      mo = fmaxf(mo, scales[kScales * i + 128 + (lane & 15)]);
+    }
+  };
+  float gv = 0.f, bv = 0.f;                      // wave 0: of the lane's token
+  auto load_gates = [&](int hr) {
+    if (wave != 0) return;
+    const int h = hk * rep + hr, t = t0 + min(lane, len - 1);
+    gv = p.g ? p.g[b * p.gs.b + h * p.gs.h + t * p.gs.l] : 0.f;
+    bv = p.beta ? p.beta[b * p.bs.b + h * p.bs.h + t * p.bs.l] : 1.f;
+  };
+  load_stage(0, 0);
+  load_scales(0);
+  load_gates(0);
+
   f32x4 tq[NSH] = {}, tk[NSH] = {};              // dQ and dK over the value heads, channels 16 (hf NSH + n) ..
   for (int hr = 0; hr < rep; ++hr) {
     const int h = hk * rep + hr;
-    const int64_t vunit = ((int64_t)b * p.heads + h) * p.pieces + c;
-    const T* osrc = reinterpret_cast<const T*>(q.d_o) + b * q.dos.b + h * q.dos.h + (int64_t)t0 * q.dos.l;
     T* dvo = reinterpret_cast<T*>(q.dv) + b * q.dvs.b + h * q.dvs.h + (int64_t)t0 * q.dvs.l;
-    // dO's largest magnitude, the matrices' scales
-    float om = 0.f;
-    for (int u = tid; u < len * ((p.dv + 7) / 8); u += 512) {
-      const int r = u / ((p.dv + 7) / 8), c8 = u % ((p.dv + 7) / 8) * 8;
-      float v[8];
-      load8(osrc + r * q.dos.l + c8, p.dv - c8, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) om = fmaxf(om, fabsf(v[j]));
-    }
-    om = wave_max(om);
-    const float* scales = reinterpret_cast<const float*>(p.workspace + lay.scales) + vunit * nblk * 128;
-    float mx = 0.f;                              // lane 16 i + column: of scale i
-    for (int i = 0; i < 2 * nblk; ++i) mx = fmaxf(mx, scales[64 * i + lane]);
-    mx = row16_max(mx);
     __syncthreads();                             // the last head's use of the LDS is over
-    if (lane == 0) red[wave][0] = om;
+    const float raw_g = gv;
     if (wave == 0) {
-      float gv = 0.f, bv = 0.f;
-      if (lane < len) {
-        if (p.g) gv = gate_log(p.g[b * p.gs.b + h * p.gs.h + (int64_t)(t0 + lane) * p.gs.l]);
-        bv = p.beta ? p.beta[b * p.bs.b + h * p.bs.h + (int64_t)(t0 + lane) * p.bs.l] : 1.f;
-      }
-      const double G = wave_scan64((double)gv * kLog2e64), end = last_lane64(G);
+      const double G = wave_scan64(lane < len ? (double)gate_log(gv) * kLog2e64 : 0.), end = last_lane64(G);
       sG[lane] = G;
-      sB[lane] = bv;
+      sB[lane] = lane < len ? bv : 0.f;
       sEG[lane] = exp_of(G);
       sEnd[lane] = exp_of(end - G);
     }
-    __syncthreads();
+    if (hr + 1 < rep) load_gates(hr + 1);
+    mx = row16_max(mx);
+    const float mS = lane_val(mx, 16 * KEEP_S), mN = lane_val(mx, 16 * KEEP_DS), mD = lane_val(mx, 16 * KEEP_D),
+                mY = lane_val(mx, 16 * KEEP_Y);
+    const float so_inv = row16_max(mo), so_mult = 1.f / so_inv;        // a power of two
     auto most = [&](int i) {
       return fmaxf(fmaxf(fmaxf(red[0][i], red[1][i]), fmaxf(red[2][i], red[3][i])), fmaxf(fmaxf(red[4][i], red[5][i]), fmaxf(red[6][i], red[7][i])));
     };
-    const Scale so(most(0));
-    const float mS = lane_val(mx, 16 * KEEP_S), mN = lane_val(mx, 16 * KEEP_DS), mD = lane_val(mx, 16 * KEEP_D),
-                mY = lane_val(mx, 16 * KEEP_Y);
 
     f32x4 aq[NSH] = {}, al[NSH] = {}, ar[NSH] = {}, pA[2] = {}, pP[2] = {};
     float dot = 0.f;                             // <S, dS>
-    const f16* keep0 = reinterpret_cast<const f16*>(p.workspace + lay.keep) + vunit * nblk * (int64_t)keep_halfs<DKP>();
     for (int v0 = 0; v0 < 16 * nblk; v0 += DVB) {
       if (v0) __syncthreads();
-      const int lane = lane_id_here(), tid = 64 * wave + lane;         // addresses formed here, not held for the loops
-      // 16 columns of v at a time, a lane's 8 values of a k-step: rows 4 g .. and 16 + 4 g .. of 32, of column l % 16
-      for (int u = tid; u < SE / 8; u += 512) {
-        const int ln = u & 63, r = u / (16 * DKP / 8) * 16 + (ln & 15), k = u / 64 % (DKP / 32), blk = (v0 + r) / 16;
-        const int c = 32 * k + 4 * (ln >> 4);
-        f16x8 s0 = {}, s1 = {}, n0 = {}, n1 = {};
-        if (blk < nblk) {
-          const f16* from = keep0 + blk * (int64_t)keep_halfs<DKP>() + (k * 64 + ln) * 8;
-          s0 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_S));
-          s1 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_S) + 16 * DKP);
-          n0 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_DS));
-          n1 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_DS) + 16 * DKP);
-          const float* f = scales + 128 * blk + (k >= KS / 2 ? 64 : 0) + (r & 15);
-          const float fs = f[16 * KEEP_S], fn = f[16 * KEEP_DS];
-          float d = 0.f;
+      const int lane = lane_id_here(), tid = 64 * wave + lane;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) d += ((float)s0[j] + (float)s1[j]) * ((float)n0[j] + (float)n1[j]);
-          dot += d * fs * fn;
-          const f16 hs = (f16)(fs / mS), hn = (f16)(fn / mN);          // powers of two, at most 1
-          s0 *= hs;
-          s1 *= hs;
-          n0 *= hn;
-          n1 *= hn;
+      for (int i = 0; i < SU; ++i) {
+        const int u = tid + 512 * i, r = u / (16 * DKP / 8) * 16 + (lane & 15), ch = u / 64 % KS * 32 + 4 * (lane >> 4);
+        float d = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d += ((float)ps[i][0][j] + (float)ps[i][1][j]) * ((float)ps[i][2][j] + (float)ps[i][3][j]);
+        dot += d * fs[i][0] * fs[i][1];
+        const f16 hs = (f16)(fs[i][0] / mS), hn = (f16)(fs[i][1] / mN);  // powers of two, at most 1
+        if (u < SE / 8) {
+          put_halves<DKP>(sS, r, ch, ps[i][0] * hs);
+          put_halves<DKP>(sS + SE, r, ch, ps[i][1] * hs);
+          put_halves<DKP>(sN, r, ch, ps[i][2] * hn);
+          put_halves<DKP>(sN + SE, r, ch, ps[i][3] * hn);
         }
-        put_halves<DKP>(sS, r, c, s0);
-        put_halves<DKP>(sS + SE, r, c, s1);
-        put_halves<DKP>(sN, r, c, n0);
-        put_halves<DKP>(sN + SE, r, c, n1);
       }
-      for (int u = tid; u < YE / 8; u += 512) {
-        const int ln = u & 63, r = u / 128 * 16 + (ln & 15), k = u / 64 % 2, blk = (v0 + r) / 16, c = 32 * k + 4 * (ln >> 4);
-        f16x8 d0 = {}, d1 = {}, y0 = {}, y1 = {};
-        if (blk < nblk) {
-          const f16* from = keep0 + blk * (int64_t)keep_halfs<DKP>() + (k * 64 + ln) * 8;
-          const float* f = scales + 128 * blk + 64 * k + (r & 15);
-          const f16 hd = (f16)(f[16 * KEEP_D] / mD), hy = (f16)(f[16 * KEEP_Y] / mY);
-          d0 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_D)) * hd;
-          d1 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_D) + 16 * DC) * hd;
-          y0 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_Y));
-          y1 = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_Y) + 16 * DC);
-          if (v0 + r < p.dv) {                   // dV
+      if (tid < YU) {
+        const int r = tid / 128 * 16 + (lane & 15), ch = tid / 64 % 2 * 32 + 4 * (lane >> 4);
+        const f16 hd = (f16)(fd[0] / mD), hy = (f16)(fd[1] / mY);
+        put_halves<64>(sD, r, ch, pd[0] * hd);
+        put_halves<64>(sD + YE, r, ch, pd[1] * hd);
+        put_halves<64>(sY, r, ch, pd[2] * hy);
+        put_halves<64>(sY + YE, r, ch, pd[3] * hy);
+        if (v0 + r < p.dv)                       // dV
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int t = c + (j & 3) + 4 * (j & 4);
-              if (t < len) dvo[t * q.dvs.l + v0 + r] = from_f32<T>(((float)y0[j] + (float)y1[j]) * f[16 * KEEP_Y]);
-            }
+          for (int j = 0; j < 8; ++j) {
+            const int t = ch + (j & 3) + 4 * (j & 4);
+            if (t < len) dvo[t * q.dvs.l + v0 + r] = from_f32<T>(((float)pd[2][j] + (float)pd[3][j]) * fd[1]);
           }
-          y0 *= hy;
-          y1 *= hy;
-        }
-        put_halves<64>(sD, r, c, d0);
-        put_halves<64>(sD + YE, r, c, d1);
-        put_halves<64>(sY, r, c, y0);
-        put_halves<64>(sY + YE, r, c, y1);
       }
-      for (int u = tid; u < DC * DVB / 8; u += 512) {
-        const int r = u / (DVB / 8), c8 = u % (DVB / 8) * 8;
-        float v[8] = {};
-        if (r < len && v0 + c8 < p.dv) load8(osrc + r * q.dos.l + v0 + c8, p.dv - v0 - c8, v);
+      if (tid < OU) {
+        const int r = tid / (DVB / 8), c8 = tid % (DVB / 8) * 8;
         f16x8 hi, lo;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          hi[j] = part_hi(v[j], so.mult);
-          if constexpr (NP == 2) lo[j] = part_lo(v[j], so.mult, hi[j]);
+          hi[j] = part_hi(po.get(j), so_mult);
+          if constexpr (NP == 2) lo[j] = part_lo(po.get(j), so_mult, hi[j]);
         }
         *reinterpret_cast<f16x8*>(sO + TC::at(r, c8)) = hi;
         if constexpr (NP == 2) *reinterpret_cast<f16x8*>(sO + TC::ELEMS + TC::at(r, c8)) = lo;
       }
       __syncthreads();
+      if (v0 + DVB < 16 * nblk) {
+        load_stage(hr, v0 + DVB);
+      } else if (hr + 1 < rep) {
+        load_stage(hr + 1, 0);
+        load_scales(hr + 1);
+      }
 #pragma unroll
       for (int s = 0; s < DVB / 32; ++s) {
         const f16x8 o0 = row_frag16<64>(sO, 16 * w, 32 * s, lane);
@@ -580,7 +616,7 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
     }
     // A' and P', what they give dbeta and dG, and the pair terms' matrices
     const int lane = lane_id_here(), l16 = lane & 15, g4 = lane >> 4;
-    const float fA = -(mY * mD), fP = p.scale * (so.inv * mD);
+    const float fA = -(mY * mD), fP = p.scale * (so_inv * mD);
     float rows[4] = {}, xam = 0.f, xpm = 0.f;
     double Gt[4];
 #pragma unroll
@@ -618,7 +654,7 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
       red[wave][2] = xpm;
       red[wave][3] = dot;
     }
-    const float fq = p.scale * (so.inv * mS), fl = -(mY * mS), fr = mD * mN;
+    const float fq = p.scale * (so_inv * mS), fl = -(mY * mS), fr = mD * mN;
     float dots[4] = {}, rights[4] = {};
 #pragma unroll
     for (int n = 0; n < NSH; ++n) {
@@ -666,10 +702,7 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
       const double total = last_lane64(upto);
       if (lane < len) {
         const int64_t at = ((int64_t)b * p.heads + h) * p.seqlen + t0 + lane;
-        if (q.dg) {
-          const float gv = p.g ? p.g[b * p.gs.b + h * p.gs.h + (int64_t)(t0 + lane) * p.gs.l] : 0.f;
-          q.dg[at] = gv < -200.f ? 0.f : (float)(total - upto + mine);
-        }
+        if (q.dg) q.dg[at] = raw_g < -200.f ? 0.f : (float)(total - upto + mine);
         if (q.dbeta) q.dbeta[at] = col + b2;
       }
     }

@@ -605,7 +605,7 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_scan_kernel(
       if (live) {
         const int64_t at = (vunit0 + c) * nblk + blk;
         f16* keep = reinterpret_cast<f16*>(p.workspace + lay.keep) + at * (int64_t)keep_halfs<DKP>();
-        float* scales = reinterpret_cast<float*>(p.workspace + lay.scales) + at * 128 + 64 * hf + l16;
+        float* scales = reinterpret_cast<float*>(p.workspace + lay.scales) + at * kScales + 64 * hf + l16;
         keep_parts<KS>(keep + keep_at<DKP>(KEEP_S), hf * KSH, sh, sl, lane);
         keep_parts<2>(keep + keep_at<DKP>(KEEP_D), hf, dh, dl, lane);
         if (g4 == 0) {
