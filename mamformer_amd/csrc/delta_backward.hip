@@ -370,7 +370,7 @@ __device__ __forceinline__ void put_halves(f16* t, int r, int c, f16x8 v) {
 template <typename T, int DKP>
 __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, DeltaLayout lay, int nblk) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
-  constexpr int DVB = NP == 1 ? 64 : 32;
+  constexpr int DVB = 32;
   constexpr int NSH = DKP / 32, KS = DKP / 32, F = kKFrags<DKP>;
   using TK = HTile<DKP>;
   using TC = HTile<64>;
@@ -401,28 +401,28 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
   __syncthreads();
   f32x4 kk[2] = {}, qk[2] = {};                  // tiles 2 m + hf of A' and P'
 #pragma unroll
-  for (int s = 0; s < DKP / 32; ++s) {
-    f16x8 ka[NP], qa[NP];
+  for (int n = 0; n < NP; ++n) {                 // with part n of K's rows j
+    f16x8 kb[2][KS], ka[NP][KS], qa[NP][KS];
 #pragma unroll
-    for (int n = 0; n < NP; ++n) {
-      ka[n] = frag(kq, (NP + n) * F + w * KS + s, lane);
-      qa[n] = frag(kq, n * F + w * KS + s, lane);
-    }
+    for (int s = 0; s < KS; ++s) {
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      const int j = 2 * m + hf;
-      if (j > w) continue;
-      const f16x8 kb = frag(kq, NP * F + j * KS + s, lane);
-      kk[m] = mma_h(ka[0], kb, kk[m]);
-      qk[m] = mma_h(qa[0], kb, qk[m]);
-      if constexpr (NP == 2) {
-        const f16x8 kl = frag(kq, (NP + 1) * F + j * KS + s, lane);
-        kk[m] = mma_h(ka[0], kl, kk[m]);
-        kk[m] = mma_h(ka[1], kb, kk[m]);
-        qk[m] = mma_h(qa[0], kl, qk[m]);
-        qk[m] = mma_h(qa[1], kb, qk[m]);
+      for (int m = 0; m < 2; ++m) kb[m][s] = frag(kq, (NP + n) * F + min(2 * m + hf, w) * KS + s, lane);
+#pragma unroll
+      for (int x = 0; x < NP - n; ++x) {         // lo lo is left out
+        ka[x][s] = frag(kq, (NP + x) * F + w * KS + s, lane);
+        qa[x][s] = frag(kq, x * F + w * KS + s, lane);
       }
     }
+    __builtin_amdgcn_sched_barrier(0);           // all of it under way before the first product
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int x = 0; x < NP - n; ++x) {
+          kk[m] = mma_h(ka[x][s], kb[m][s], kk[m]);
+          qk[m] = mma_h(qa[x][s], kb[m][s], qk[m]);
+        }
   }
 #pragma unroll
   for (int m = 0; m < 2; ++m)
