@@ -618,7 +618,9 @@ int mh_token_logprobs_bwd(const mh_logprob_bwd_args* a, void* stream);
  *   key head h / (heads / kheads). g, beta (batch, heads, seqlen) fp32, each or NULL (g = 0, beta = 1); g = -inf clears the
  *   state. initial_state, final_state (batch, heads, dk, dv) fp32 contiguous, each or NULL. dk <= 128, dv <= 256,
  *   batch * heads * ceil(seqlen / 64) <= 2^23. A NaN or infinity may reach every result of its head from the 64-token piece
- *   that holds it on, and no other head's. seqlen = 0 copies the state. The same bits at every call. */
+ *   that holds it on, and no other head's. seqlen = 0 copies the state. The same bits at every call.
+ *   keep: the workspace is larger and holds afterwards what a backward of the same arguments needs (its `kept`), about
+ *   2.7 KB a token and head of 128 x 128; a backward only reads it. */
 typedef struct {
   int64_t batch, heads, kheads, seqlen, dk, dv;
   int32_t dtype;
@@ -632,11 +634,13 @@ typedef struct {
   float* final_state;
   void* o; int64_t o_stride_b, o_stride_h, o_stride_l;
   void* workspace; size_t workspace_bytes;
+  int32_t keep;
 } mh_delta_args;
 int mh_delta_rule_workspace_bytes(const mh_delta_args* a, size_t* bytes);
 int mh_delta_rule_fwd(const mh_delta_args* a, void* stream);
 
-/* Its backward. fwd: the forward's arguments (o, final_state and the workspace ignored). d_o like o, d_final_state like
+/* Its backward. fwd: the forward's arguments (o, final_state, the workspace and keep ignored). kept: the workspace of a forward
+ *   of the same arguments with `keep`, or NULL: the pieces' systems and states are computed again. d_o like o, d_final_state like
  *   final_state or NULL; dq, dk, dv like q, k, v (written, the heads that share a key head summed in their order), dg, dbeta
  *   (batch, heads, seqlen) fp32 contiguous, each or NULL, d_initial_state or NULL. */
 typedef struct {
@@ -648,6 +652,7 @@ typedef struct {
   void* dv; int64_t dv_stride_b, dv_stride_h, dv_stride_l;
   float* dg; float* dbeta; float* d_initial_state;
   void* workspace; size_t workspace_bytes;
+  const void* kept; size_t kept_bytes;
 } mh_delta_bwd_args;
 int mh_delta_rule_bwd_workspace_bytes(const mh_delta_bwd_args* a, size_t* bytes);
 int mh_delta_rule_bwd(const mh_delta_bwd_args* a, void* stream);

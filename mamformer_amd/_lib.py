@@ -263,6 +263,7 @@ class DeltaArgs(ct.Structure):
         ("initial_state", _vp), ("final_state", _vp),
         ("o", _vp), ("o_stride_b", _i64), ("o_stride_h", _i64), ("o_stride_l", _i64),
         ("workspace", _vp), ("workspace_bytes", _sz),
+        ("keep", _i32),
     ]
 
 
@@ -276,6 +277,7 @@ class DeltaBwdArgs(ct.Structure):
         ("dv", _vp), ("dv_stride_b", _i64), ("dv_stride_h", _i64), ("dv_stride_l", _i64),
         ("dg", _vp), ("dbeta", _vp), ("d_initial_state", _vp),
         ("workspace", _vp), ("workspace_bytes", _sz),
+        ("kept", _vp), ("kept_bytes", _sz),
     ]
 
 

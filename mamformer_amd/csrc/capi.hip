@@ -1134,6 +1134,7 @@ void delta_fill(const mh_delta_args* a, mh::DeltaParams& p) {
   p.beta = a->beta; p.bs = {a->beta_stride_b, a->beta_stride_h, a->beta_stride_l};
   p.initial_state = a->initial_state; p.final_state = a->final_state;
   p.o = a->o; p.os = {a->o_stride_b, a->o_stride_h, a->o_stride_l};
+  p.keep = a->keep != 0;
 }
 
 int group_norm_fill(const char* fn, const mh_group_norm_args* a, mh::GroupNormParams& p) {
@@ -1886,7 +1887,8 @@ int mh_delta_rule_bwd_workspace_bytes(const mh_delta_bwd_args* a, size_t* bytes)
   MH_TRY(delta_sizes("delta_rule_bwd", f->batch, f->heads, f->kheads, f->seqlen, f->dk, f->dv, f->dtype));
   mh::DeltaParams p;
   delta_fill(f, p);
-  *bytes = f->batch && f->seqlen ? mh::delta_bwd_workspace_bytes(p) : 0;
+  p.keep = 1;
+  *bytes = f->batch && f->seqlen ? mh::delta_scratch_bytes(p) + (a->kept ? 0 : mh::delta_workspace_bytes(p)) : 0;
   return MH_OK;
 }
 
@@ -1894,7 +1896,7 @@ int mh_delta_rule_bwd(const mh_delta_bwd_args* a, void* stream) {
   const char* fn = "delta_rule_bwd";
   if (!a) return fail(MH_ERR_NULL, "delta_rule_bwd: args is NULL");
   const mh_delta_args* f = &a->fwd;
-  Region r[16];
+  Region r[17];
   int n;
   MH_TRY(delta_inputs(fn, f, r, n));
   if (f->batch == 0) return MH_OK;
@@ -1903,8 +1905,12 @@ int mh_delta_rule_bwd(const mh_delta_bwd_args* a, void* stream) {
   delta_fill(f, q.f);
   q.f.o = nullptr;
   q.f.final_state = nullptr;
-  const size_t need = f->seqlen ? mh::delta_bwd_workspace_bytes(q.f) : 0;
+  q.f.keep = 1;
+  q.kept = a->kept != nullptr;
+  const size_t scratch = f->seqlen ? mh::delta_scratch_bytes(q.f) : 0, operands = f->seqlen ? mh::delta_workspace_bytes(q.f) : 0;
+  const size_t need = scratch + (q.kept ? 0 : operands);
   MH_TRY(workspace_ok(fn, a->workspace, a->workspace_bytes, need));
+  if (q.kept) MH_TRY(workspace_ok(fn, a->kept, a->kept_bytes, operands));
   const int es = elem_size(f->dtype);
   const int64_t states = f->batch * f->heads * f->dk * f->dv * 4, gates = f->batch * f->heads * f->seqlen * 4;
   MH_TRY(vec_ok(fn, "d_final_state", a->d_final_state, 4, false));
@@ -1914,6 +1920,7 @@ int mh_delta_rule_bwd(const mh_delta_bwd_args* a, void* stream) {
   r[n++] = flat_region("d_final_state", a->d_final_state, states, false);
   r[n++] = flat_region("d_initial_state", a->d_initial_state, states, true);
   r[n++] = flat_region("workspace", need ? a->workspace : nullptr, (int64_t)need, true);
+  r[n++] = flat_region("kept", operands ? a->kept : nullptr, (int64_t)operands, false);
   if (f->seqlen > 0) {
     r[n++] = flat_region("dg", a->dg, gates, true);
     r[n++] = flat_region("dbeta", a->dbeta, gates, true);
@@ -1929,7 +1936,8 @@ int mh_delta_rule_bwd(const mh_delta_bwd_args* a, void* stream) {
   q.dk = a->dk; q.dks = {a->dk_stride_b, a->dk_stride_h, a->dk_stride_l};
   q.dv = a->dv; q.dvs = {a->dv_stride_b, a->dv_stride_h, a->dv_stride_l};
   q.dg = a->dg; q.dbeta = a->dbeta; q.d_initial_state = a->d_initial_state;
-  q.f.workspace = reinterpret_cast<char*>(a->workspace);
+  q.scratch = reinterpret_cast<char*>(a->workspace);
+  q.f.workspace = q.kept ? reinterpret_cast<char*>(const_cast<void*>(a->kept)) : q.scratch + scratch;
   return hip_status(mh::launch_delta_bwd(q, reinterpret_cast<hipStream_t>(stream)), fn);
 }
 

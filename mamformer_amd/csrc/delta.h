@@ -148,12 +148,13 @@ __device__ __forceinline__ float exp_of(double x) { return __builtin_amdgcn_exp2
 // are read by 16 bytes a lane without conflicts, and the scans need no transposing reads.
 //   For each (batch, key head, piece), NP parts of each: Q by rows (i KS + s: rows 16 i .., k-step s), K by rows, K by
 //     columns (2 n + s: channels 16 n .., tokens 32 s ..), and for the backward Q by columns.
-//   For each (batch, value head, piece), two parts of each: T by rows (its 6 fragments that are not zero), then P by rows,
-//     or for the backward T and P by columns.
+//   For each (batch, value head, piece), two parts of each: T by rows (its 6 fragments that are not zero), P by rows, then
+//     for the backward T and P by columns.
 //   `vec` for the same: e^{G_t}, beta_t e^{G_end - G_t}, then e^{G_end} and the scales of T, P, K and Q.
-//   For the backward, for each (batch, value head, piece, 16 columns of v): the entering state, its gradient behind the
-//     piece, delta and y, two parts each, in the order in which waves hold them as operands ([part][k-step]), and the
-//     scales of their columns in either half of the rows ([half][which][column]), then those of dO's columns.
+//   For the backward, for each (batch, value head, piece, 16 columns of v): the entering state and delta, two parts each,
+//     in the order in which waves hold them as operands ([part][k-step]), and the scales of their columns in either half
+//     of the rows ([half][which][column]).  In a room of their own (DeltaScratch), as only the backward writes them: the
+//     state's gradient behind the piece and y in the same way, and the scales of dO's columns behind theirs.
 constexpr int FR = 512;                          // halfs of a fragment
 template <int DKP> constexpr int kKFrags = DKP / 8;                    // of K or Q, rows or columns
 constexpr int kTFrags = 6;
@@ -164,12 +165,9 @@ __device__ __forceinline__ void put_frag(f16* t, int f, int lane, f16x8 v) { *re
 
 constexpr int kVecFloats = 256;
 enum { VEC_W = 64, VEC_GAMMA = 128, VEC_ST, VEC_SP, VEC_SK, VEC_SQ };
-enum { KEEP_S, KEEP_DS, KEEP_D, KEEP_Y };
-constexpr int kScales = 160;                     // floats, 16 of them unused
-template <int DKP> constexpr size_t keep_halfs() { return 2 * (2 * 16 * DKP) + 2 * (2 * 16 * DC); }
-template <int DKP> constexpr int keep_at(int which) {                  // where one of the four begins, in halfs
-  return which < KEEP_D ? which * 2 * 16 * DKP : 4 * 16 * DKP + (which - KEEP_D) * 2 * 16 * DC;
-}
+constexpr int kScales = 64, kGradScales = 80;    // floats
+template <int DKP> constexpr int keep_halfs() { return 2 * 16 * DKP + 2 * 16 * DC; }
+template <int DKP> constexpr int kTokens = 2 * 16 * DKP;               // where delta and y begin, behind the states
 // k-steps s0 .. s0 + N - 1 of ALL.
 template <int ALL, int N>
 __device__ __forceinline__ void keep_parts(f16* to, int s0, const f16x8 (&hi)[N], const f16x8 (&lo)[N], int lane) {
@@ -188,7 +186,7 @@ struct DeltaLayout {
     const size_t kpieces = (size_t)p.batch * p.kheads * p.pieces, pieces = (size_t)p.batch * p.heads * p.pieces;
     const size_t blocks = backward ? pieces * ((p.dv + 15) / 16) : 0;
     kq_unit = (backward ? 4 : 3) * np * (dkp / 8) * FR * 2;
-    tp_unit = (backward ? 6 : 4) * kTFrags * FR * 2;
+    tp_unit = (backward ? 8 : 4) * kTFrags * FR * 2;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t was = at; at += (bytes + 1023) / 1024 * 1024; return was; };
     kq = take(kpieces * kq_unit);
@@ -197,6 +195,15 @@ struct DeltaLayout {
     keep = take(blocks * (dkp == 64 ? keep_halfs<64>() : keep_halfs<128>()) * 2);
     scales = take(blocks * kScales * 4);
     total = at;
+  }
+};
+struct DeltaScratch {
+  size_t keep, scales, total;
+  __host__ explicit DeltaScratch(const DeltaParams& p) {
+    const size_t blocks = (size_t)p.batch * p.heads * p.pieces * ((p.dv + 15) / 16);
+    keep = 0;
+    scales = (blocks * (p.dk <= 64 ? keep_halfs<64>() : keep_halfs<128>()) * 2 + 1023) / 1024 * 1024;
+    total = scales + (blocks * kGradScales * 4 + 1023) / 1024 * 1024;
   }
 };
 

@@ -21,7 +21,7 @@ namespace {
 // a piece's tokens each, with a fifth and a sixth wave that fetch.  y = T^T ddelta is upper triangular, so that here the
 // first wave needs the second one's ddelta.
 template <typename T, int DKP>
-__global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_back_scan_kernel(DeltaBwdParams q, DeltaLayout lay, int nblk, int nwg) {
+__global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_back_scan_kernel(DeltaBwdParams q, DeltaLayout lay, DeltaScratch scr, int nblk, int nwg) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
   constexpr bool AHEAD = NP == 1;
   constexpr int FW = AHEAD ? 1 : 4;
@@ -44,12 +44,12 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_back_scan_ke
   lds_f16_t* const lds = (lds_f16_t*)smem;
   auto fetch_a = [&](int c) {
     fetch_share<NP * F, FW>(lds, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + NP * F * 1024, fw, lane);
-    fetch_share<2 * kTFrags, FW>(lds + NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit + 4 * kTFrags * 1024, fw, lane);
+    fetch_share<2 * kTFrags, FW>(lds + NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit + 6 * kTFrags * 1024, fw, lane);
   };
   auto fetch_b = [&](int c) {
     lds_f16_t* to = lds + (GA + (AHEAD ? (c & 1) * GB : 0)) * FR;
     fetch_share<2 * NP * F, FW>(to, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + 2 * NP * F * 1024, fw, lane);
-    fetch_share<2 * kTFrags, FW>(to + 2 * NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit + 2 * kTFrags * 1024, fw, lane);
+    fetch_share<2 * kTFrags, FW>(to + 2 * NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit + 4 * kTFrags * 1024, fw, lane);
     if (fw == 0) fetch_share<1, 1>(to + (2 * NP * F + 2 * kTFrags) * FR, p.workspace + lay.vec + (vunit0 + c) * (int64_t)(kVecFloats * 4), 0, lane);
   };
   if constexpr (AHEAD) {
@@ -332,14 +332,14 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_back_scan_ke
       const Scale sy(col_max(abs_max(Yv)));
       parts_of<2>(Yv, sy.mult, yh, yl);
       const int64_t at = (vunit0 + c) * nblk + blk;
-      f16* keep = reinterpret_cast<f16*>(p.workspace + lay.keep) + at * (int64_t)keep_halfs<DKP>();
-      float* scales = reinterpret_cast<float*>(p.workspace + lay.scales) + at * kScales + 64 * hf + l16;
-      keep_parts<KS>(keep + keep_at<DKP>(KEEP_DS), hf * KSH, sh, sl, lane);
-      keep_parts<2>(keep + keep_at<DKP>(KEEP_Y), hf, yh, yl, lane);
+      f16* keep = reinterpret_cast<f16*>(q.scratch + scr.keep) + at * (int64_t)keep_halfs<DKP>();
+      float* scales = reinterpret_cast<float*>(q.scratch + scr.scales) + at * kGradScales + 32 * hf + l16;
+      keep_parts<KS>(keep, hf * KSH, sh, sl, lane);
+      keep_parts<2>(keep + kTokens<DKP>, hf, yh, yl, lane);
       if (g4 == 0) {
-        scales[16 * KEEP_DS] = ss.inv;
-        scales[16 * KEEP_Y] = sy.inv * ysc;
-        if (hf == 0) scales[128] = so.inv;       // over all tokens in either half
+        scales[0] = ss.inv;
+        scales[16] = sy.inv * ysc;
+        if (hf == 0) scales[64] = so.inv;       // over all tokens in either half
       }
     }
   }
@@ -368,7 +368,7 @@ __device__ __forceinline__ void put_halves(f16* t, int r, int c, f16x8 v) {
 // columns of v pass through LDS DVB at a time, every matrix brought to one scale on the way (its columns
 // have their own).
 template <typename T, int DKP>
-__global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, DeltaLayout lay, int nblk) {
+__global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, DeltaLayout lay, DeltaScratch scr, int nblk) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
   constexpr int DVB = 32;
   constexpr int NSH = DKP / 32, KS = DKP / 32, F = kKFrags<DKP>;
@@ -438,13 +438,15 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
   static_assert(YU <= 512 && OU <= 512, "one unit a thread");
   f16x8 ps[SU][4], pd[4];
   Raw8<T> po;
-  float fs[SU][2], fd[2], mx = 0.f, mo = 0.f;    // scales of the units' columns; a head's, lane 16 i + column: of scale i
+  float fs[SU][2], fd[2], mx = 0.f, mg = 0.f, mo = 0.f;     // scales of the units' columns; a head's largest, lanes as the scales
   auto vunit_of = [&](int hr) { return ((int64_t)b * p.heads + hk * rep + hr) * p.pieces + c; };
   auto scales_of = [&](int hr) { return reinterpret_cast<const float*>(p.workspace + lay.scales) + vunit_of(hr) * nblk * kScales; };
+  auto grad_scales_of = [&](int hr) { return reinterpret_cast<const float*>(q.scratch + scr.scales) + vunit_of(hr) * nblk * kGradScales; };
   auto load_stage = [&](int hr, int v0) {
     const int lane = lane_id_here(), tid = 64 * wave + lane;           // addresses formed here, not held for the loops
-    const f16* keep0 = reinterpret_cast<const f16*>(p.workspace + lay.keep) + vunit_of(hr) * nblk * (int64_t)keep_halfs<DKP>();
-    const float* scales = scales_of(hr);
+    const int64_t at0 = vunit_of(hr) * nblk * (int64_t)keep_halfs<DKP>();
+    const f16 *keep0 = reinterpret_cast<const f16*>(p.workspace + lay.keep) + at0, *grad0 = reinterpret_cast<const f16*>(q.scratch + scr.keep) + at0;
+    const float *scales = scales_of(hr), *grad_scales = grad_scales_of(hr);
 #pragma unroll
     for (int i = 0; i < SU; ++i) {
       const int u = tid + 512 * i, blk = v0 / 16 + u / (16 * DKP / 8), k = u / 64 % KS;
@@ -452,14 +454,13 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
       for (int j = 0; j < 4; ++j) ps[i][j] = f16x8{};
       fs[i][0] = fs[i][1] = 0.f;
       if (u < SE / 8 && blk < nblk) {
-        const f16* from = keep0 + blk * (int64_t)keep_halfs<DKP>() + (k * 64 + lane) * 8;
-        ps[i][0] = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_S));
-        ps[i][1] = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_S) + 16 * DKP);
-        ps[i][2] = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_DS));
-        ps[i][3] = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_DS) + 16 * DKP);
-        const float* f = scales + kScales * blk + (k >= KS / 2 ? 64 : 0) + (lane & 15);
-        fs[i][0] = f[16 * KEEP_S];
-        fs[i][1] = f[16 * KEEP_DS];
+        const int at = blk * keep_halfs<DKP>() + (k * 64 + lane) * 8, f = (k >= KS / 2 ? 32 : 0) + (lane & 15);
+        ps[i][0] = *reinterpret_cast<const f16x8*>(keep0 + at);
+        ps[i][1] = *reinterpret_cast<const f16x8*>(keep0 + at + 16 * DKP);
+        ps[i][2] = *reinterpret_cast<const f16x8*>(grad0 + at);
+        ps[i][3] = *reinterpret_cast<const f16x8*>(grad0 + at + 16 * DKP);
+        fs[i][0] = scales[kScales * blk + f];
+        fs[i][1] = grad_scales[kGradScales * blk + f];
       }
     }
     {
@@ -468,14 +469,13 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
       for (int j = 0; j < 4; ++j) pd[j] = f16x8{};
       fd[0] = fd[1] = 0.f;
       if (tid < YU && blk < nblk) {
-        const f16* from = keep0 + blk * (int64_t)keep_halfs<DKP>() + (k * 64 + lane) * 8;
-        pd[0] = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_D));
-        pd[1] = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_D) + 16 * DC);
-        pd[2] = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_Y));
-        pd[3] = *reinterpret_cast<const f16x8*>(from + keep_at<DKP>(KEEP_Y) + 16 * DC);
-        const float* f = scales + kScales * blk + 64 * k + (lane & 15);
-        fd[0] = f[16 * KEEP_D];
-        fd[1] = f[16 * KEEP_Y];
+        const int at = blk * keep_halfs<DKP>() + kTokens<DKP> + (k * 64 + lane) * 8, f = 32 * k + 16 + (lane & 15);
+        pd[0] = *reinterpret_cast<const f16x8*>(keep0 + at);
+        pd[1] = *reinterpret_cast<const f16x8*>(keep0 + at + 16 * DC);
+        pd[2] = *reinterpret_cast<const f16x8*>(grad0 + at);
+        pd[3] = *reinterpret_cast<const f16x8*>(grad0 + at + 16 * DC);
+        fd[0] = scales[kScales * blk + f];
+        fd[1] = grad_scales[kGradScales * blk + f];
       }
     }
     const int r = tid / (DVB / 8), c8 = v0 + tid % (DVB / 8) * 8;
@@ -485,12 +485,13 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
   };
   auto load_scales = [&](int hr) {
     const int lane = lane_id_here();
-    const float* scales = scales_of(hr);
-    mx = mo = 0.f;
+    const float *scales = scales_of(hr), *grad_scales = grad_scales_of(hr);
+    mx = mg = mo = 0.f;
 #pragma unroll 4
     for (int i = 0; i < nblk; ++i) {
-      mx = fmaxf(mx, fmaxf(scales[kScales * i + lane], scales[kScales * i + 64 + lane]));
-      mo = fmaxf(mo, scales[kScales * i + 128 + (lane & 15)]);
+      mx = fmaxf(mx, scales[kScales * i + lane]);
+      mg = fmaxf(mg, grad_scales[kGradScales * i + lane]);
+      mo = fmaxf(mo, grad_scales[kGradScales * i + 64 + (lane & 15)]);
     }
   };
   float gv = 0.f, bv = 0.f;                      // wave 0: of the lane's token
@@ -519,8 +520,9 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
     }
     if (hr + 1 < rep) load_gates(hr + 1);
     mx = row16_max(mx);
-    const float mS = lane_val(mx, 16 * KEEP_S), mN = lane_val(mx, 16 * KEEP_DS), mD = lane_val(mx, 16 * KEEP_D),
-                mY = lane_val(mx, 16 * KEEP_Y);
+    mg = row16_max(mg);
+    const float mS = fmaxf(lane_val(mx, 0), lane_val(mx, 32)), mD = fmaxf(lane_val(mx, 16), lane_val(mx, 48)),
+                mN = fmaxf(lane_val(mg, 0), lane_val(mg, 32)), mY = fmaxf(lane_val(mg, 16), lane_val(mg, 48));
     const float so_inv = row16_max(mo), so_mult = 1.f / so_inv;        // a power of two
     auto most = [&](int i) {
       return fmaxf(fmaxf(fmaxf(red[0][i], red[1][i]), fmaxf(red[2][i], red[3][i])), fmaxf(fmaxf(red[4][i], red[5][i]), fmaxf(red[6][i], red[7][i])));
@@ -780,11 +782,12 @@ template <typename T, int DKP>
 hipError_t run_bwd(const DeltaBwdParams& q, hipStream_t st) {
   const DeltaParams& p = q.f;
   const DeltaLayout lay(p, true);
+  const DeltaScratch scr(p);
   const int nblk = (p.dv + 15) / 16, nwg = (nblk + 1) / 2;
-  delta_back_scan_kernel<T, DKP><<<head_block_grid(p.batch * p.heads, nwg), sizeof(T) == 4 ? 256 : 384, 0, st>>>(q, lay, nblk, nwg);
+  delta_back_scan_kernel<T, DKP><<<head_block_grid(p.batch * p.heads, nwg), sizeof(T) == 4 ? 256 : 384, 0, st>>>(q, lay, scr, nblk, nwg);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  delta_grads_kernel<T, DKP><<<(unsigned)((int64_t)p.batch * p.kheads * p.pieces), 512, 0, st>>>(q, lay, nblk);
+  delta_grads_kernel<T, DKP><<<(unsigned)((int64_t)p.batch * p.kheads * p.pieces), 512, 0, st>>>(q, lay, scr, nblk);
   return hipGetLastError();
 }
 
@@ -795,7 +798,7 @@ __global__ void delta_copy_grad_kernel(const float* from, float* to, int64_t n) 
 
 }  // namespace
 
-size_t delta_bwd_workspace_bytes(const DeltaParams& p) { return DeltaLayout(p, true).total; }
+size_t delta_scratch_bytes(const DeltaParams& p) { return DeltaScratch(p).total; }
 
 hipError_t launch_delta_bwd(const DeltaBwdParams& q, hipStream_t st) {
   const DeltaParams& p = q.f;
@@ -805,9 +808,11 @@ hipError_t launch_delta_bwd(const DeltaBwdParams& q, hipStream_t st) {
     delta_copy_grad_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(q.d_final_state, q.d_initial_state, n);
     return hipGetLastError();
   }
-  hipError_t e = launch_delta_prep(p, true, st);
-  if (e == hipSuccess) e = launch_delta_keep(p, st);
-  if (e != hipSuccess) return e;
+  if (!q.kept) {
+    hipError_t e = launch_delta_prep(p, true, st);
+    if (e == hipSuccess) e = launch_delta_keep(p, st);
+    if (e != hipSuccess) return e;
+  }
   if (p.dtype == DT_F32) return p.dk <= 64 ? run_bwd<float, 64>(q, st) : run_bwd<float, 128>(q, st);
   return p.dk <= 64 ? run_bwd<bf16, 64>(q, st) : run_bwd<bf16, 128>(q, st);
 }

@@ -248,10 +248,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void delta_prep_kernel
       if (w >= 2 * s) {
         put_frag(out, t_frag(w, s), lane, th[s]);
         put_frag(out, kTFrags + t_frag(w, s), lane, tl[s]);
-        if (!backward) {
-          put_frag(out, 2 * kTFrags + t_frag(w, s), lane, ph[s]);
-          put_frag(out, 3 * kTFrags + t_frag(w, s), lane, pl[s]);
-        }
+        put_frag(out, 2 * kTFrags + t_frag(w, s), lane, ph[s]);
+        put_frag(out, 3 * kTFrags + t_frag(w, s), lane, pl[s]);
       }
     if (backward) {                              // by columns: through LDS, as T^T and P^T (row j, column t)
 #pragma unroll
@@ -270,8 +268,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void delta_prep_kernel
 #pragma unroll
         for (int s = 0; s < 2; ++s)
           if (w < 2 + 2 * s) {
-            put_frag(out, (2 + n) * kTFrags + tt_frag(w, s), lane, row_frag16<64>(tiles + n * TC::ELEMS, 16 * w, 32 * s, lane));
-            put_frag(out, (4 + n) * kTFrags + tt_frag(w, s), lane, row_frag16<64>(tiles + (2 + n) * TC::ELEMS, 16 * w, 32 * s, lane));
+            put_frag(out, (4 + n) * kTFrags + tt_frag(w, s), lane, row_frag16<64>(tiles + n * TC::ELEMS, 16 * w, 32 * s, lane));
+            put_frag(out, (6 + n) * kTFrags + tt_frag(w, s), lane, row_frag16<64>(tiles + (2 + n) * TC::ELEMS, 16 * w, 32 * s, lane));
           }
     }
     float* vec = reinterpret_cast<float*>(p.workspace + lay.vec) + vunit * kVecFloats;
@@ -605,12 +603,12 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_scan_kernel(
       if (live) {
         const int64_t at = (vunit0 + c) * nblk + blk;
         f16* keep = reinterpret_cast<f16*>(p.workspace + lay.keep) + at * (int64_t)keep_halfs<DKP>();
-        float* scales = reinterpret_cast<float*>(p.workspace + lay.scales) + at * kScales + 64 * hf + l16;
-        keep_parts<KS>(keep + keep_at<DKP>(KEEP_S), hf * KSH, sh, sl, lane);
-        keep_parts<2>(keep + keep_at<DKP>(KEEP_D), hf, dh, dl, lane);
+        float* scales = reinterpret_cast<float*>(p.workspace + lay.scales) + at * kScales + 32 * hf + l16;
+        keep_parts<KS>(keep, hf * KSH, sh, sl, lane);
+        keep_parts<2>(keep + kTokens<DKP>, hf, dh, dl, lane);
         if (g4 == 0) {
-          scales[16 * KEEP_S] = ss.inv;
-          scales[16 * KEEP_D] = sd.inv * ds;
+          scales[0] = ss.inv;
+          scales[16] = sd.inv * ds;
         }
       }
     }
@@ -689,7 +687,7 @@ __global__ void delta_copy_state_kernel(const float* from, float* to, int64_t n)
 
 }  // namespace
 
-size_t delta_workspace_bytes(const DeltaParams& p) { return DeltaLayout(p, false).total; }
+size_t delta_workspace_bytes(const DeltaParams& p) { return DeltaLayout(p, p.keep).total; }
 
 hipError_t launch_delta_prep(const DeltaParams& p, bool backward, hipStream_t st) {
   const DeltaLayout lay(p, backward);
@@ -709,9 +707,13 @@ hipError_t launch_delta(const DeltaParams& p, hipStream_t st) {
     delta_copy_state_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p.initial_state, p.final_state, n);
     return hipGetLastError();
   }
-  const hipError_t e = launch_delta_prep(p, false, st);
+  const hipError_t e = launch_delta_prep(p, p.keep, st);
   if (e != hipSuccess) return e;
-  const DeltaLayout lay(p, false);
+  const DeltaLayout lay(p, p.keep);
+  if (p.keep) {
+    if (p.dtype == DT_F32) return p.dk <= 64 ? launch_scan<float, 64, true, true>(p, lay, st) : launch_scan<float, 128, true, true>(p, lay, st);
+    return p.dk <= 64 ? launch_scan<bf16, 64, true, true>(p, lay, st) : launch_scan<bf16, 128, true, true>(p, lay, st);
+  }
   if (p.dtype == DT_F32) return p.dk <= 64 ? launch_scan<float, 64, true, false>(p, lay, st) : launch_scan<float, 128, true, false>(p, lay, st);
   return p.dk <= 64 ? launch_scan<bf16, 64, true, false>(p, lay, st) : launch_scan<bf16, 128, true, false>(p, lay, st);
 }

@@ -468,6 +468,7 @@ struct DeltaParams {
   const float* initial_state;              // (b, H, dk, dv) contiguous or null
   float* final_state;                      // or null
   void* o; DeltaStrides os;                // null: not computed
+  int keep;                                // the workspace is one for the backward, and holds what that needs afterwards
   char* workspace;
 };
 size_t delta_workspace_bytes(const DeltaParams& p);
@@ -480,11 +481,13 @@ struct DeltaBwdParams {
   void *dq, *dk, *dv; DeltaStrides dqs, dks, dvs;
   float *dg, *dbeta;                       // (b, H, L) contiguous
   float* d_initial_state;                  // or null
+  int kept;                                // f.workspace is what a forward with `keep` left
+  char* scratch;
 };
-size_t delta_bwd_workspace_bytes(const DeltaParams& p);
+size_t delta_scratch_bytes(const DeltaParams& p);
 hipError_t launch_delta_bwd(const DeltaBwdParams& p, hipStream_t st);
-// The forward's parts that the backward runs again: the pieces' triangular systems, and the scan that keeps the entering
-// states and the corrections.
+// The forward's parts that a backward runs again where they were not kept: the pieces' triangular systems, and the scan
+// that keeps the entering states and the corrections.
 hipError_t launch_delta_prep(const DeltaParams& p, bool backward, hipStream_t st);
 hipError_t launch_delta_keep(const DeltaParams& p, hipStream_t st);
 

@@ -182,7 +182,8 @@ class _RotaryFn(torch.autograd.Function):
 
 # ------------------------------------------------------------------------------------------------ gated delta rule
 
-def gated_delta_rule(q, k, v, g=None, beta=None, *, scale=None, initial_state=None, return_final_state=False):
+def gated_delta_rule(q, k, v, g=None, beta=None, *, scale=None, initial_state=None, return_final_state=False,
+                     recompute=False):
     """Gated delta rule over sequences: o (B, H, L, dv) like v, or (o, final state (B, H, dk, dv) float32).
 
     With a state S (dk, dv) in fp32 for each (batch, head), zero or ``initial_state``:
@@ -192,17 +193,19 @@ def gated_delta_rule(q, k, v, g=None, beta=None, *, scale=None, initial_state=No
     dk ** -0.5.  Keys are taken as they are: for a stable state beta |k|^2 <= 2, so normalise them before.
 
     A token with beta = 0 and g = 0 changes nothing, which is what padding behind a sequence takes.  A NaN or infinity may
-    reach every result of its head from the 64-token piece that holds it on.  Differentiable in all tensors
-    (``gated_delta_rule_bwd``, which computes the states again); with L = 0 the state goes through.
+    reach every result of its head from the 64-token piece that holds it on.  With L = 0 the state goes through.
+    Differentiable in all tensors: a call that records a gradient keeps the states and systems of its pieces for it, about
+    2.7 KB a token and head of 128 x 128 (bf16); with ``recompute`` it keeps its inputs alone, and the gradients' pass computes
+    the rest again, a fourth of a training step's time.  The gradients are the same bits.
     """
     name = "gated_delta_rule"
     _require_cuda(name, q, k, v, g, beta, initial_state)
     _delta_shapes(name, q, k, v, g, beta, initial_state, 4)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if _through_autograd(q, k, v, g, beta, initial_state):
-        o, final = _GatedDeltaFn.apply(q, k, v, g, beta, initial_state, scale, return_final_state)
+        o, final = _GatedDeltaFn.apply(q, k, v, g, beta, initial_state, scale, return_final_state, recompute)
     else:
-        o, final = _delta_fwd(q, k, v, g, beta, initial_state, scale, return_final_state)
+        o, final, _ = _delta_fwd(q, k, v, g, beta, initial_state, scale, return_final_state, False)
     return (o, final) if return_final_state else o
 
 
@@ -227,18 +230,18 @@ def _delta_args(q, k, v, g, beta, state, scale):
                      *_strides3(beta), _ptr(state))
 
 
-def _delta_fwd(q, k, v, g, beta, state, scale, want_final):
+def _delta_fwd(q, k, v, g, beta, state, scale, want_final, keep):
     q, k, v, g, beta, state = _channels(q), _channels(k), _channels(v), _f32(g), _f32(beta), _vec(state)
     o = torch.empty_like(v)
     final = None
     if want_final:
         final = torch.empty((*v.shape[:2], q.shape[-1], v.shape[-1]), device=v.device, dtype=torch.float32)
     a = _delta_args(q, k, v, g, beta, state, scale)
-    a.final_state = _ptr(final)
+    a.final_state, a.keep = _ptr(final), keep
     a.o, a.o_stride_b, a.o_stride_h, a.o_stride_l = _strides3(o)
     ws = _optional_workspace("mh_delta_rule_workspace_bytes", a, v.device)
     _lib.call("mh_delta_rule_fwd", ct.byref(a), _stream(v.device))
-    return o, final
+    return o, final, ws if keep else None
 
 
 def gated_delta_rule_bwd(do, q, k, v, g=None, beta=None, *, scale=None, initial_state=None, d_final_state=None):
@@ -254,7 +257,10 @@ def gated_delta_rule_bwd(do, q, k, v, g=None, beta=None, *, scale=None, initial_
     _like(name, "do", do, v.shape, v.dtype)
     if d_final_state is not None:
         _like(name, "d_final_state", d_final_state, (*v.shape[:2], q.shape[-1], v.shape[-1]), torch.float32)
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    return _delta_bwd(do, q, k, v, g, beta, initial_state, d_final_state, q.shape[-1] ** -0.5 if scale is None else float(scale))
+
+
+def _delta_bwd(do, q, k, v, g, beta, initial_state, d_final_state, scale, kept=None):
     q, k, v, do = _channels(q), _channels(k), _channels(v), _channels(do)
     g, beta, initial_state, d_final_state = _f32(g), _f32(beta), _vec(initial_state), _vec(d_final_state)
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
@@ -262,6 +268,8 @@ def gated_delta_rule_bwd(do, q, k, v, g=None, beta=None, *, scale=None, initial_
     d_state = None if initial_state is None else torch.empty_like(initial_state)
     a = DeltaBwdArgs(_delta_args(q, k, v, g, beta, initial_state, scale), *_strides3(do), _ptr(d_final_state), *_strides3(dq),
                      *_strides3(dk), *_strides3(dv), _ptr(dg), _ptr(dbeta), _ptr(d_state))
+    if kept is not None:
+        a.kept, a.kept_bytes = kept.data_ptr(), kept.numel()
     ws = _optional_workspace("mh_delta_rule_bwd_workspace_bytes", a, v.device)
     _lib.call("mh_delta_rule_bwd", ct.byref(a), _stream(v.device))
     return dq, dk, dv, dg, dbeta, d_state
@@ -271,26 +279,27 @@ class _GatedDeltaFn(torch.autograd.Function):
     """Autograd node of the gated delta rule: forward = ``mh_delta_rule_fwd``, backward = ``mh_delta_rule_bwd``."""
 
     @staticmethod
-    def forward(ctx, q, k, v, g, beta, state, scale, want_final):
+    def forward(ctx, q, k, v, g, beta, state, scale, want_final, recompute):
+        o, final, kept = _delta_fwd(q, k, v, g, beta, state, scale, want_final, not recompute)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(q, k, v, g, beta, state)
+        ctx.save_for_backward(q, k, v, g, beta, state, kept)
         ctx.scale = scale
-        return _delta_fwd(q, k, v, g, beta, state, scale, want_final)
+        return o, final
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do, d_final):
-        q, k, v, g, beta, state = ctx.saved_tensors
+        q, k, v, g, beta, state, kept = ctx.saved_tensors
         if do is None and d_final is None:
-            return (None,) * 8
+            return (None,) * 9
         if do is None:
             do = torch.zeros_like(v)
-        grads = gated_delta_rule_bwd(do, q, k, v, g, beta, scale=ctx.scale, initial_state=state, d_final_state=d_final)
+        grads = _delta_bwd(do, q, k, v, g, beta, state, d_final, ctx.scale, kept)
         grads = [d if need else None for d, need in zip(grads, ctx.needs_input_grad)]
         for i, t in ((3, g), (4, beta)):
             if grads[i] is not None and t.dtype is not torch.float32:
                 grads[i] = grads[i].to(t.dtype)
-        return *grads, None, None
+        return *grads, None, None, None
 
 
 def gated_delta_step(state, q, k, v, g=None, beta=None, *, scale=None, state_out=None):
