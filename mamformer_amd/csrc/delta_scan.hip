@@ -467,6 +467,17 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_scan_kernel(
       xSend[i * 64] = X[2 + i] * ss.inv;
       if constexpr (OUT) xSend[(2 + i) * 64] = Y[2 + i] * ss.inv;
     }
+    f16* keep = nullptr;
+    float* scales = nullptr;
+    if constexpr (KEEP) {                        // stored where they are made: held to the end they would spill
+      const int64_t at = (vunit0 + c) * nblk + blk;
+      keep = reinterpret_cast<f16*>(p.workspace + lay.keep) + at * keep_halfs<DKP>();
+      scales = reinterpret_cast<float*>(p.workspace + lay.scales) + at * kScales + 32 * hf + l16;
+      if (live) {
+        keep_parts<KS>(keep, hf * KSH, sh, sl, lane);
+        if (g4 == 0) scales[0] = ss.inv;
+      }
+    }
     lds_barrier();                               // 1
     f32x4 xr[2], yr[2], eg[2], wt[2];
     bf16x4 vb[2];
@@ -562,6 +573,11 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_scan_kernel(
     eS[(2 + hf) * 64 + lane] = own_us;
     const Scale sd(col_max(abs_max(D)));
     parts_of<(KEEP || NP == 2) ? 2 : 1>(D, sd.mult, dh, dl);
+    if constexpr (KEEP)
+      if (live) {
+        keep_parts<2>(keep + kTokens<DKP>, hf, dh, dl, lane);
+        if (g4 == 0) scales[16] = sd.inv * ds;
+      }
     if constexpr (OUT)
       if (hf == 0) {
         put_frag(eD, 0, lane, dh[0]);
@@ -599,19 +615,6 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_scan_kernel(
     for (int n = 0; n < NSH; ++n)
 #pragma unroll
       for (int r = 0; r < 4; ++r) S[n][r] = cs[0] * S[n][r] + own_us * u0[n][r] + other_us * u1[n][r];
-    if constexpr (KEEP) {
-      if (live) {
-        const int64_t at = (vunit0 + c) * nblk + blk;
-        f16* keep = reinterpret_cast<f16*>(p.workspace + lay.keep) + at * (int64_t)keep_halfs<DKP>();
-        float* scales = reinterpret_cast<float*>(p.workspace + lay.scales) + at * kScales + 32 * hf + l16;
-        keep_parts<KS>(keep, hf * KSH, sh, sl, lane);
-        keep_parts<2>(keep + kTokens<DKP>, hf, dh, dl, lane);
-        if (g4 == 0) {
-          scales[0] = ss.inv;
-          scales[16] = sd.inv * ds;
-        }
-      }
-    }
     if constexpr (OUT) {
       f32x4 O[2] = {}, OX[2] = {};
 #pragma unroll
