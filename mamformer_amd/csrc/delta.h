@@ -178,9 +178,13 @@ __device__ __forceinline__ void keep_parts(f16* to, int s0, const f16x8 (&hi)[N]
   }
 }
 
+int delta_segments(const DeltaParams& p);        // how many a sequence is scanned in
+
 struct DeltaLayout {
   size_t kq, tp, vec, keep, scales, total;       // byte offsets
   size_t kq_unit, tp_unit;                       // bytes of a piece
+  size_t seg_states, seg_trans;                  // of segments, each (batch, head, segment)
+  int segs, per;                                 // segments, pieces of one
   __host__ DeltaLayout(const DeltaParams& p, bool backward) {
     const size_t np = p.dtype == DT_F32 ? 2 : 1, dkp = p.dk <= 64 ? 64 : 128;
     const size_t kpieces = (size_t)p.batch * p.kheads * p.pieces, pieces = (size_t)p.batch * p.heads * p.pieces;
@@ -194,6 +198,11 @@ struct DeltaLayout {
     vec = take(pieces * kVecFloats * 4);
     keep = take(blocks * (dkp == 64 ? keep_halfs<64>() : keep_halfs<128>()) * 2);
     scales = take(blocks * kScales * 4);
+    segs = delta_segments(p);
+    per = (p.pieces + segs - 1) / segs;
+    const size_t units = segs > 1 ? (size_t)p.batch * p.heads * segs : 0;
+    seg_states = take(units * p.dk * p.dv * 4);
+    seg_trans = take(units * dkp * dkp * 4);
     total = at;
   }
 };
@@ -229,10 +238,9 @@ __device__ __forceinline__ void load_rows8(const T* at, int64_t stride, int len,
   int c = cv ? l16 : 0;
   asm volatile("" : "+v"(c), "+v"(g4));          // addresses formed here, not held for the loop
   if (len >= 32) {
-    const uint32_t off = (uint32_t)(4 * g4 * (int)stride + c) * (uint32_t)sizeof(T);
+    const int64_t off = 4 * g4 * stride + c;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      v[i] = *reinterpret_cast<const T*>(reinterpret_cast<const char*>(at + (16 * (i >> 2) + (i & 3)) * stride) + off);
+    for (int i = 0; i < 8; ++i) v[i] = (at + (16 * (i >> 2) + (i & 3)) * stride)[off];
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = at[(int64_t)min(16 * (i >> 2) + 4 * g4 + (i & 3), len - 1) * stride + c];
@@ -246,10 +254,9 @@ __device__ __forceinline__ void store_rows8(T* at, int64_t stride, int len, bool
   if (!cv) return;
   asm volatile("" : "+v"(l16), "+v"(g4));
   if (len >= 32) {
-    const uint32_t off = (uint32_t)(4 * g4 * (int)stride + l16) * (uint32_t)sizeof(T);
+    const int64_t off = 4 * g4 * stride + l16;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      *reinterpret_cast<T*>(reinterpret_cast<char*>(at + (16 * (i >> 2) + (i & 3)) * stride) + off) = from_f32<T>(v[i]);
+    for (int i = 0; i < 8; ++i) (at + (16 * (i >> 2) + (i & 3)) * stride)[off] = from_f32<T>(v[i]);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {

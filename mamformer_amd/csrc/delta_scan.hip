@@ -298,27 +298,36 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void delta_prep_kernel
 // Bound by the latency of one piece on waves that have a SIMD to themselves, most of it the conversions (an instruction of
 // 4 cycles for each value and part); b 2, H 16, L 4096 has 256 sets of 16 columns for 1024 SIMDs.  Operands that no other
 // wave has to finish first are read from LDS right behind a barrier, ahead of what they are needed for.
+template <bool WHOLE> constexpr int kScanPairs = WHOLE ? 2 : 4;        // without o the pairs of four fit the LDS
+template <typename T, bool WHOLE> constexpr int kScanThreads = 64 * (2 * kScanPairs<WHOLE> + (sizeof(T) == 4 ? 0 : 1 + kScanPairs<WHOLE> / 2));
 template <typename T, int DKP, bool OUT, bool KEEP>
-__global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_scan_kernel(DeltaParams p, DeltaLayout lay, int nblk, int nwg) {
+__global__ __launch_bounds__((kScanThreads<T, (OUT || KEEP)>)) void delta_scan_kernel(DeltaParams p, DeltaLayout lay, int nblk, int nwg) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
   constexpr bool AHEAD = NP == 1;                // fp32: the fragments of a piece fill the LDS
-  constexpr int FW = AHEAD ? 1 : 4;              // waves that fetch
+  constexpr bool MOVE = !OUT && !KEEP;           // what a segment makes of the state, and of any other
+  constexpr int PAIRS = kScanPairs<OUT || KEEP>, IOW = PAIRS / 2;
+  constexpr int FW = AHEAD ? 1 : 2 * PAIRS;      // waves that fetch
   constexpr int KS = DKP / 32, KSH = KS / 2, NSH = DKP / 32, F = kKFrags<DKP>;
   constexpr int GA = (OUT ? 2 : 1) * NP * F;                         // fragments of (Q and) K by rows: before barrier 1
   constexpr int TPF = OUT ? 4 * kTFrags : 2 * kTFrags;               // of T (and P)
   constexpr int GB = NP * F + TPF + 1;                               // with K by columns and vec: after it
   constexpr int XF = OUT ? 4 : 2, DF = OUT ? NP : 0;
   constexpr int EX = (2 * XF + 2 + 4 + DF + 1) * FR;                 // halfs of a pair's exchange
-  constexpr int IO = AHEAD ? (OUT ? 3 : 2) * IO_HALFS : 0;           // v of two pieces, o of one
-  __shared__ __align__(1024) f16 smem[(GA + (AHEAD ? 2 : 1) * GB) * FR + 2 * EX + IO];
+  constexpr int IO = AHEAD ? (OUT ? 3 : 2) * IOW * IO_HALFS : 0;           // v of two pieces, o of one
+  __shared__ __align__(1024) f16 smem[(GA + (AHEAD ? 2 : 1) * GB) * FR + PAIRS * EX + IO];
 
   const int lane = threadIdx.x & 63, w = wave_id(), l16 = lane & 15, g4 = lane >> 4, hf = w & 1;
-  int bh, wg;
-  if (!head_block(blockIdx.x, p.batch * p.heads, nwg, bh, wg)) return;
+  int part, wg;
+  const int segs = MOVE ? lay.segs - 1 : lay.segs;
+  if (!head_block(blockIdx.x, p.batch * p.heads * segs, nwg, part, wg)) return;
+  const int bh = part / segs, seg = part % segs, c0 = seg * lay.per, c1 = min(c0 + lay.per, p.pieces);
+  const int nv = (nblk + PAIRS - 1) / PAIRS;     // workgroups behind them: the columns of the identity, without v
+  const bool unit = MOVE && wg >= nv;
+  if (unit && seg == 0) return;                  // its state is known
   const int b = bh / p.heads, h = bh % p.heads, hk = h / (p.heads / p.kheads);
   const int64_t kunit0 = ((int64_t)b * p.kheads + hk) * p.pieces, vunit0 = (int64_t)bh * p.pieces;
-  bf16* const sV = reinterpret_cast<bf16*>(smem + (GA + (AHEAD ? 2 : 1) * GB) * FR + 2 * EX);
-  bf16* const sO = sV + 2 * IO_HALFS;
+  bf16* const sV = reinterpret_cast<bf16*>(smem + (GA + (AHEAD ? 2 : 1) * GB) * FR + PAIRS * EX);
+  bf16* const sO = sV + 2 * IOW * IO_HALFS;
 
   const int fw = AHEAD ? 0 : w;
   lds_f16_t* const lds = (lds_f16_t*)smem;
@@ -326,17 +335,17 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_scan_kernel(
   auto fetch_b = [&](int c) {
     lds_f16_t* to = lds + (GA + (AHEAD ? (c & 1) * GB : 0)) * FR;
     fetch_share<NP * F, FW>(to, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + 2 * NP * F * 1024, fw, lane);
-    fetch_share<TPF, FW>(to + NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit, fw, lane);
+    if (FW < 8 || fw < 4) fetch_share<TPF, (FW < 4 ? FW : 4)>(to + NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit, fw, lane);
     if (fw == 0) fetch_share<1, 1>(to + (NP * F + TPF) * FR, p.workspace + lay.vec + (vunit0 + c) * (int64_t)(kVecFloats * 4), 0, lane);
   };
   if constexpr (AHEAD) {
-    if (w == 4) {
-      fetch_a(0);
-      fetch_b(0);
+    if (w == 2 * PAIRS) {
+      fetch_a(c0);
+      fetch_b(c0);
       wait_vmem_n<GB>();
       lds_barrier();
-      for (int c = 0; c < p.pieces; ++c) {
-        const bool more = c + 1 < p.pieces;
+      for (int c = c0; c < c1; ++c) {
+        const bool more = c + 1 < c1;
         wait_vmem();                             // T, P and K by columns of this piece
         lds_barrier();                           // 1
         if (more) fetch_a(c + 1);                // where the last ones have been read
@@ -350,33 +359,34 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_scan_kernel(
       lds_barrier();
       return;
     }
-    if (w == 5) {
-      const int col0 = IO_COLS * wg, left = p.dv - col0;
+    if (w > 2 * PAIRS) {
+      const int io = w - 2 * PAIRS - 1, col0 = IO_COLS * (IOW * wg + io), left = unit ? 0 : p.dv - col0;
       const bf16* vs = reinterpret_cast<const bf16*>(p.v) + b * p.vs.b + h * p.vs.h + col0;
       bf16* os = reinterpret_cast<bf16*>(p.o) + b * p.os.b + h * p.os.h + col0;
+      bf16* const to = sV + io * IO_HALFS;
       IoRows v, o;
       auto load_v = [&](int c) {
         const int t = c * DC + lane;
         v.load(vs + t * p.vs.l, t < p.seqlen, left);
       };
-      load_v(0);
-      v.to_lds(sV, lane);
-      load_v(1);
+      load_v(c0);
+      v.to_lds(to + (c0 & 1) * IOW * IO_HALFS, lane);
+      load_v(c0 + 1);
       lds_barrier();
-      for (int c = 0; c <= p.pieces; ++c) {
-        if (c == p.pieces) {
+      for (int c = c0; c <= c1; ++c) {
+        if (c == c1) {
           lds_barrier();                         // the last piece's o is whole
         } else {
           lds_barrier();                         // 1
-          v.to_lds(sV + ((c + 1) & 1) * IO_HALFS, lane);
+          v.to_lds(to + ((c + 1) & 1) * IOW * IO_HALFS, lane);
           load_v(c + 2);
         }
-        if (OUT && c > 0) {
+        if (OUT && c > c0) {
           const int t = (c - 1) * DC + lane;
-          o.from_lds(sO, lane);
+          o.from_lds(sO + io * IO_HALFS, lane);
           o.store(os + t * p.os.l, t < p.seqlen, left);
         }
-        if (c < p.pieces) {
+        if (c < c1) {
           lds_barrier();                         // 2
           lds_barrier();                         // 3
         }
@@ -384,8 +394,8 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_scan_kernel(
       return;
     }
   }
-  const int blk = 2 * wg + (w >> 1), col = 16 * blk + l16;
-  const bool live = blk < nblk, cv = col < p.dv;                     // a pair beyond the last columns has zeros
+  const int blk = PAIRS * (unit ? wg - nv : wg) + (w >> 1), col = 16 * blk + l16, cols = unit ? p.dk : p.dv;
+  const bool live = 16 * blk < cols, cv = col < cols;                // a pair beyond the last columns has zeros
   f16* ex = smem + (GA + (AHEAD ? 2 : 1) * GB) * FR + (w >> 1) * EX;
   f32x4* const xSend = reinterpret_cast<f32x4*>(ex) + hf * XF * 64 + lane;             // X (and Y) of the other's tokens
   const f32x4* const xRecv = reinterpret_cast<const f32x4*>(ex) + (1 - hf) * XF * 64 + lane;
@@ -394,22 +404,26 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_scan_kernel(
   f16* const eD = eU + 4 * FR;                                                         // the first half's delta
   float* const eS = reinterpret_cast<float*>(eD + DF * FR);                            // scales: R, D, U of each half
 
+  const int64_t states = (int64_t)p.dk * p.dv;   // elements of a state
+  float* const seg_states = reinterpret_cast<float*>(p.workspace + lay.seg_states) + (int64_t)bh * lay.segs * states;
+  const float* entry = seg > 0 ? (MOVE ? nullptr : seg_states + (seg - 1) * states) : p.initial_state ? p.initial_state + bh * states : nullptr;
   f32x4 S[NSH];                                  // rows DKP / 2 hf + 16 n + 4 g4 + r, column col
 #pragma unroll
   for (int n = 0; n < NSH; ++n)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int row = DKP / 2 * hf + 16 * n + 4 * g4 + r;
-      S[n][r] = p.initial_state && cv && row < p.dk ? p.initial_state[((int64_t)bh * p.dk + row) * p.dv + col] : 0.f;
+      if (unit) S[n][r] = row == col && cv ? 1.f : 0.f;
+      else S[n][r] = entry && cv && row < p.dk ? entry[(int64_t)row * p.dv + col] : 0.f;
     }
   T vn[8];
   auto load_v = [&](int c) {                     // a half that lies beyond the sequence reads the last token
     const int t = min(c * DC + 32 * hf, p.seqlen - 1);
-    const T* vsrc = reinterpret_cast<const T*>(p.v) + b * p.vs.b + h * p.vs.h + (live ? 16 * blk : 0);
-    load_rows8<T>(vsrc + t * p.vs.l, p.vs.l, p.seqlen - t, cv, 16 * blk + 16 <= p.dv, l16, g4, vn);
+    const T* vsrc = reinterpret_cast<const T*>(p.v) + b * p.vs.b + h * p.vs.h + (live && !unit ? 16 * blk : 0);
+    load_rows8<T>(vsrc + t * p.vs.l, p.vs.l, p.seqlen - t, cv && !unit, !unit && 16 * blk + 16 <= p.dv, l16, g4, vn);
   };
   if (AHEAD) lds_barrier();
-  else load_v(0);
+  else load_v(c0);
 
   const f16 *Qr = smem, *Kr = smem + (OUT ? NP * F * FR : 0);
   f16x8 ka[KSH][4], qa[OUT ? KSH : 1][4];        // the next piece's; tiles 0, 1: one's own tokens, 2, 3: the other's
@@ -426,7 +440,7 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_scan_kernel(
   };
   if (AHEAD) load_a();
 
-  for (int c = 0; c < p.pieces; ++c) {
+  for (int c = c0; c < c1; ++c) {
     if (!AHEAD) {
       lds_barrier();
       fetch_a(c);
@@ -486,7 +500,7 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_scan_kernel(
       xr[i] = xRecv[i * 64];
       eg[i] = *reinterpret_cast<const f32x4*>(vec + 32 * hf + 16 * i + 4 * g4);
       if constexpr (AHEAD)
-        vb[i] = *reinterpret_cast<const bf16x4*>(sV + (c & 1) * IO_HALFS + ((w >> 1) * 16 + l16) * IO_PITCH + 32 * hf + 16 * i + 4 * g4);
+        vb[i] = *reinterpret_cast<const bf16x4*>(sV + (c & 1) * IOW * IO_HALFS + ((w >> 1) * 16 + l16) * IO_PITCH + 32 * hf + 16 * i + 4 * g4);
     }
     const f32x4 cs = *reinterpret_cast<const f32x4*>(vec + VEC_GAMMA);                 // gamma, scales of T, P, K
     f16x8 t0[2], t1[2], x0[2], x1[2];            // T on one's own tokens; on the first half's
@@ -512,7 +526,7 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_scan_kernel(
         const float v = AHEAD ? (float)vb[i][r] : to_f32(vn[4 * i + r]);
         R[i][r] = v - eg[i][r] * (cs[3] * (ss.inv * X[i][r] + xr[i][r]));
       }
-    if (!AHEAD && c + 1 < p.pieces) load_v(c + 1);
+    if (!AHEAD && c + 1 < c1) load_v(c + 1);
     // delta = T R: one's own tokens, and for the second wave those of the first
     f16x8 rh[1], rl[1];
     const Scale sr(col_max(abs_max(R)));
@@ -594,7 +608,7 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_scan_kernel(
       if constexpr (NP == 2) d1 = frag(eD, 1, lane);
       od = eS[64 + lane];
     }
-    if (AHEAD && c + 1 < p.pieces) load_a();
+    if (AHEAD && c + 1 < c1) load_a();
     __builtin_amdgcn_sched_barrier(0);
     f32x4 u0[NSH] = {}, u1[NSH] = {};
 #pragma unroll
@@ -656,22 +670,95 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_scan_kernel(
     }
   }
   if (AHEAD) lds_barrier();
-  if (p.final_state && cv) {
+  float* out = MOVE ? seg_states + seg * states : seg == lay.segs - 1 && p.final_state ? p.final_state + bh * states : nullptr;
+  if (unit) {                                    // by columns, as the segments' kernel reads it
+    float* trans = reinterpret_cast<float*>(p.workspace + lay.seg_trans) + ((int64_t)bh * lay.segs + seg) * DKP * DKP + (int64_t)col * DKP;
+    if (cv)
+#pragma unroll
+      for (int n = 0; n < NSH; ++n) *reinterpret_cast<f32x4*>(trans + DKP / 2 * hf + 16 * n + 4 * g4) = S[n];
+  } else if (out && cv) {
 #pragma unroll
     for (int n = 0; n < NSH; ++n)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int row = DKP / 2 * hf + 16 * n + 4 * g4 + r;
-        if (row < p.dk) p.final_state[((int64_t)bh * p.dk + row) * p.dv + col] = S[n][r];
+        if (row < p.dk) out[(int64_t)row * p.dv + col] = S[n][r];
       }
+  }
+}
+
+// The states that the segments begin with, S_{s+1} = M_s S_s + N_s, where the scan has left N_s (segment 0: S_1 itself) and
+// M_s: a workgroup takes 16 columns from segment to segment, a wave 16 rows of them by fp32 matrix instructions.  M_s does
+// not wait for a state: that of the next segment is under way during the product (8 heads of 128 x 128, 8 segments: 55 us
+// with the rows a thread each and M read where it is used).
+template <int DKP>
+__global__ __launch_bounds__(4 * DKP) void delta_segments_kernel(DeltaParams p, DeltaLayout lay) {
+  __shared__ float sS[2][DKP][16];
+  const int lane = threadIdx.x & 63, w = wave_id(), l16 = lane & 15, g4 = lane >> 4;
+  const int nblk = (p.dv + 15) / 16, bh = blockIdx.x / nblk, col = blockIdx.x % nblk * 16 + l16;
+  const int64_t states = (int64_t)p.dk * p.dv;
+  const int row0 = 16 * w + 4 * g4;
+  float* const at = reinterpret_cast<float*>(p.workspace + lay.seg_states) + (int64_t)bh * lay.segs * states + (int64_t)row0 * p.dv + col;
+  const float* const M = reinterpret_cast<const float*>(p.workspace + lay.seg_trans) + (int64_t)bh * lay.segs * DKP * DKP + g4 * DKP + 16 * w + l16;
+  auto state_of = [&](int s) {
+    f32x4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = s < lay.segs - 1 && col < p.dv && row0 + r < p.dk ? at[s * states + r * p.dv] : 0.f;
+    return v;
+  };
+  float m[DKP / 4];                              // k = 4 i + g4
+  auto load_m = [&](int s) {
+#pragma unroll
+    for (int i = 0; i < DKP / 4; ++i) m[i] = s < lay.segs - 1 && 4 * i + g4 < p.dk ? M[(int64_t)s * DKP * DKP + 4 * i * DKP] : 0.f;
+  };
+  f32x4 S = state_of(0), N = state_of(1);
+  load_m(1);
+  for (int s = 1; s < lay.segs - 1; ++s) {
+    float(*t)[16] = sS[s & 1];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) t[row0 + r][l16] = S[r];
+    __syncthreads();
+    float b[DKP / 4];
+#pragma unroll
+    for (int i = 0; i < DKP / 4; ++i) b[i] = t[4 * i + g4][l16];
+    f32x4 acc[2] = {N, {}};
+#pragma unroll
+    for (int i = 0; i < DKP / 4; ++i) acc[i & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[i], b[i], acc[i & 1], 0, 0, 0);
+    load_m(s + 1);
+    N = state_of(s + 1);
+    S = acc[0] + acc[1];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (col < p.dv && row0 + r < p.dk) at[s * states + r * p.dv] = S[r];
   }
 }
 
 template <typename T, int DKP, bool OUT, bool KEEP>
 hipError_t launch_scan(const DeltaParams& p, const DeltaLayout& lay, hipStream_t st) {
-  const int nblk = (p.dv + 15) / 16, nwg = (nblk + 1) / 2;
-  delta_scan_kernel<T, DKP, OUT, KEEP><<<head_block_grid(p.batch * p.heads, nwg), sizeof(T) == 4 ? 256 : 384, 0, st>>>(p, lay, nblk, nwg);
+  constexpr int PAIRS = kScanPairs<OUT || KEEP>;
+  const int nblk = (p.dv + 15) / 16, nwg = (nblk + PAIRS - 1) / PAIRS + (OUT || KEEP ? 0 : ((p.dk + 15) / 16 + PAIRS - 1) / PAIRS);
+  const int parts = p.batch * p.heads * (OUT || KEEP ? lay.segs : lay.segs - 1);
+  delta_scan_kernel<T, DKP, OUT, KEEP><<<head_block_grid(parts, nwg), kScanThreads<T, OUT || KEEP>, 0, st>>>(p, lay, nblk, nwg);
   return hipGetLastError();
+}
+template <typename T, int DKP>
+hipError_t launch_segments(const DeltaParams& p, const DeltaLayout& lay, hipStream_t st) {
+  if (lay.segs == 1) return hipSuccess;
+  const hipError_t e = launch_scan<T, DKP, false, false>(p, lay, st);
+  if (e != hipSuccess) return e;
+  delta_segments_kernel<DKP><<<(unsigned)(p.batch * p.heads * ((p.dv + 15) / 16)), 4 * DKP, 0, st>>>(p, lay);
+  return hipGetLastError();
+}
+template <typename T, int DKP>
+hipError_t run_scan(const DeltaParams& p, const DeltaLayout& lay, bool out, bool keep, hipStream_t st) {
+  const hipError_t e = launch_segments<T, DKP>(p, lay, st);
+  if (e != hipSuccess) return e;
+  return !out ? launch_scan<T, DKP, false, true>(p, lay, st) : keep ? launch_scan<T, DKP, true, true>(p, lay, st) : launch_scan<T, DKP, true, false>(p, lay, st);
+}
+hipError_t scan(const DeltaParams& p, bool out, bool keep, hipStream_t st) {
+  const DeltaLayout lay(p, keep);
+  if (p.dtype == DT_F32) return p.dk <= 64 ? run_scan<float, 64>(p, lay, out, keep, st) : run_scan<float, 128>(p, lay, out, keep, st);
+  return p.dk <= 64 ? run_scan<bf16, 64>(p, lay, out, keep, st) : run_scan<bf16, 128>(p, lay, out, keep, st);
 }
 
 template <typename T>
@@ -690,6 +777,25 @@ __global__ void delta_copy_state_kernel(const float* from, float* to, int64_t n)
 
 }  // namespace
 
+// A sequence of few heads leaves most CUs idle while it goes from piece to piece.  It is then cut into segments: a scan
+// without o finds what each makes of no state (N) and of the identity's columns (M), delta_segments_kernel goes from segment
+// to segment, and the scan with o takes all segments at once.  The segments' number is the one with the least time by this
+// count, in tenths of a piece's time (o and all: 10, without o: 9; a segment's product: 10); a gain of less than a fifth is left.
+int delta_segments(const DeltaParams& p) {
+  constexpr int64_t kCUs = 256;                  // a workgroup fills one
+  const int64_t heads = (int64_t)p.batch * p.heads, nblk = (p.dv + 15) / 16, kblk = (p.dk + 15) / 16;
+  const int64_t whole = heads * ((nblk + 1) / 2), move = heads * ((nblk + 3) / 4 + (kblk + 3) / 4);
+  auto rounds = [](int64_t n) { return (n + kCUs - 1) / kCUs; };
+  int64_t best = 1, least = p.pieces * rounds(whole) * 8;
+  for (int64_t n = 2; n <= 64 && 4 * n <= p.pieces; ++n) {
+    const int64_t per = (p.pieces + n - 1) / n;
+    if ((p.pieces + per - 1) / per != n) continue;
+    const int64_t cost = per * (9 * rounds(move * (n - 1)) + 10 * rounds(whole * n)) + 10 * n + 40;
+    if (cost < least) least = cost, best = n;
+  }
+  return (int)best;
+}
+
 size_t delta_workspace_bytes(const DeltaParams& p) { return DeltaLayout(p, p.keep).total; }
 
 hipError_t launch_delta_prep(const DeltaParams& p, bool backward, hipStream_t st) {
@@ -697,11 +803,7 @@ hipError_t launch_delta_prep(const DeltaParams& p, bool backward, hipStream_t st
   return p.dtype == DT_F32 ? run_prep<float>(p, lay, backward, st) : run_prep<bf16>(p, lay, backward, st);
 }
 
-hipError_t launch_delta_keep(const DeltaParams& p, hipStream_t st) {
-  const DeltaLayout lay(p, true);
-  if (p.dtype == DT_F32) return p.dk <= 64 ? launch_scan<float, 64, false, true>(p, lay, st) : launch_scan<float, 128, false, true>(p, lay, st);
-  return p.dk <= 64 ? launch_scan<bf16, 64, false, true>(p, lay, st) : launch_scan<bf16, 128, false, true>(p, lay, st);
-}
+hipError_t launch_delta_keep(const DeltaParams& p, hipStream_t st) { return scan(p, false, true, st); }
 
 hipError_t launch_delta(const DeltaParams& p, hipStream_t st) {
   if (p.seqlen == 0) {
@@ -712,13 +814,7 @@ hipError_t launch_delta(const DeltaParams& p, hipStream_t st) {
   }
   const hipError_t e = launch_delta_prep(p, p.keep, st);
   if (e != hipSuccess) return e;
-  const DeltaLayout lay(p, p.keep);
-  if (p.keep) {
-    if (p.dtype == DT_F32) return p.dk <= 64 ? launch_scan<float, 64, true, true>(p, lay, st) : launch_scan<float, 128, true, true>(p, lay, st);
-    return p.dk <= 64 ? launch_scan<bf16, 64, true, true>(p, lay, st) : launch_scan<bf16, 128, true, true>(p, lay, st);
-  }
-  if (p.dtype == DT_F32) return p.dk <= 64 ? launch_scan<float, 64, true, false>(p, lay, st) : launch_scan<float, 128, true, false>(p, lay, st);
-  return p.dk <= 64 ? launch_scan<bf16, 64, true, false>(p, lay, st) : launch_scan<bf16, 128, true, false>(p, lay, st);
+  return scan(p, true, p.keep, st);
 }
 
 }  // namespace mh
