@@ -16,6 +16,8 @@
 // the state through all of its products without moving a value to another lane.
 #pragma once
 
+#include <type_traits>
+
 #include "launch.h"
 #include "rows.h"
 #include "tiles.h"
@@ -272,21 +274,24 @@ constexpr int IO_COLS = 32, IO_PITCH = 68;       // 34 banks a column: 16 column
 constexpr int IO_HALFS = IO_COLS * IO_PITCH;
 struct IoRows {
   bf16x8 v[IO_COLS / 8];
-  // `at`: column 0 of the lane's token, of which `left` columns exist
-  __device__ __forceinline__ void load(const bf16* at, bool row, int left) {
+  // `at`: column 0 of the lane's token, of which `left` columns exist; FULL: all of them, then without a branch, so that a
+  // load stays under way until to_lds of the piece after next
+  template <bool FULL>
+  __device__ __forceinline__ void load(const bf16* at, int left) {
 #pragma unroll
     for (int i = 0; i < IO_COLS / 8; ++i) {
       Raw8<bf16> r;
-      r.clear();
-      if (row && left > 8 * i) load_raw(r, at + 8 * i, left - 8 * i);
+      if constexpr (!FULL) r.clear();
+      if (FULL || left > 8 * i) load_raw(r, at + 8 * i, FULL ? 8 : left - 8 * i);
       v[i] = r.v;
     }
   }
+  template <bool FULL>
   __device__ __forceinline__ void store(bf16* at, bool row, int left) const {
+    if (!row) return;
 #pragma unroll
     for (int i = 0; i < IO_COLS / 8; ++i) {
-      if (!row || left <= 8 * i) continue;
-      if (left >= 8 * i + 8) put_vec<false>(at + 8 * i, v[i]);
+      if (FULL || left >= 8 * i + 8) put_vec<false>(at + 8 * i, v[i]);
       else
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -296,6 +301,10 @@ struct IoRows {
   __device__ __forceinline__ void to_lds(bf16* t, int lane) const {
 #pragma unroll
     for (int c = 0; c < IO_COLS; ++c) t[c * IO_PITCH + lane] = v[c / 8][c % 8];
+  }
+  __device__ __forceinline__ void zero_unless(bool row) {
+#pragma unroll
+    for (int i = 0; i < IO_COLS / 8; ++i) v[i] = row ? v[i] : bf16x8{};
   }
   __device__ __forceinline__ void from_lds(const bf16* t, int lane) {
 #pragma unroll

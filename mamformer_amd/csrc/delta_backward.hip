@@ -72,24 +72,29 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_back_scan_ke
       return;
     }
     if (w == 5) {                                // dO; tokens beyond the sequence have none
-      const int col0 = IO_COLS * wg;
+      const int col0 = IO_COLS * wg, left = p.dv - col0;
       const bf16* src = reinterpret_cast<const bf16*>(q.d_o) + b * q.dos.b + h * q.dos.h + col0;
-      IoRows v;
-      auto load = [&](int c) {
-        const int t = c * DC + lane;
-        v.load(src + t * q.dos.l, c >= 0 && t < p.seqlen, p.dv - col0);
+      auto run = [&](auto full) {
+        IoRows v;
+        auto load = [&](int c) {
+          const int t = min(max(c, 0) * DC + lane, p.seqlen - 1);
+          v.template load<decltype(full)::value>(src + t * q.dos.l, left);
+        };
+        load(p.pieces - 1);
+        v.zero_unless((p.pieces - 1) * DC + lane < p.seqlen);
+        v.to_lds(reinterpret_cast<bf16*>(smem + DOUT + ((p.pieces - 1) & 1) * IO_HALFS), lane);
+        load(p.pieces - 2);
+        lds_barrier();
+        for (int c = p.pieces - 1; c >= 0; --c) {
+          lds_barrier();                         // 1
+          v.to_lds(reinterpret_cast<bf16*>(smem + DOUT + ((c + 1) & 1) * IO_HALFS), lane);
+          load(c - 2);
+          lds_barrier();                         // 2
+          lds_barrier();                         // 3
+        }
       };
-      load(p.pieces - 1);
-      v.to_lds(reinterpret_cast<bf16*>(smem + DOUT + ((p.pieces - 1) & 1) * IO_HALFS), lane);
-      load(p.pieces - 2);
-      lds_barrier();
-      for (int c = p.pieces - 1; c >= 0; --c) {
-        lds_barrier();                           // 1
-        v.to_lds(reinterpret_cast<bf16*>(smem + DOUT + ((c + 1) & 1) * IO_HALFS), lane);
-        load(c - 2);
-        lds_barrier();                           // 2
-        lds_barrier();                           // 3
-      }
+      if (left >= IO_COLS) run(std::true_type{});
+      else run(std::false_type{});
       return;
     }
   }

@@ -364,33 +364,35 @@ __global__ __launch_bounds__((kScanThreads<T, (OUT || KEEP)>)) void delta_scan_k
       const bf16* vs = reinterpret_cast<const bf16*>(p.v) + b * p.vs.b + h * p.vs.h + col0;
       bf16* os = reinterpret_cast<bf16*>(p.o) + b * p.os.b + h * p.os.h + col0;
       bf16* const to = sV + io * IO_HALFS;
-      IoRows v, o;
-      auto load_v = [&](int c) {
-        const int t = c * DC + lane;
-        v.load(vs + t * p.vs.l, t < p.seqlen, left);
-      };
-      load_v(c0);
-      v.to_lds(to + (c0 & 1) * IOW * IO_HALFS, lane);
-      load_v(c0 + 1);
-      lds_barrier();
-      for (int c = c0; c <= c1; ++c) {
-        if (c == c1) {
-          lds_barrier();                         // the last piece's o is whole
-        } else {
+      auto run = [&](auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        IoRows v, o;
+        auto load_v = [&](int c) {               // tokens beyond the sequence as its last: their gates are zero
+          const int t = min(c * DC + lane, p.seqlen - 1);
+          v.template load<FULL>(vs + t * p.vs.l, left);
+        };
+        auto store_o = [&](int c) {
+          const int t = c * DC + lane;
+          o.from_lds(sO + io * IO_HALFS, lane);
+          o.template store<FULL>(os + t * p.os.l, t < p.seqlen, left);
+        };
+        load_v(c0);
+        v.to_lds(to + (c0 & 1) * IOW * IO_HALFS, lane);
+        load_v(c0 + 1);
+        lds_barrier();
+        for (int c = c0; c < c1; ++c) {
           lds_barrier();                         // 1
           v.to_lds(to + ((c + 1) & 1) * IOW * IO_HALFS, lane);
           load_v(c + 2);
-        }
-        if (OUT && c > c0) {
-          const int t = (c - 1) * DC + lane;
-          o.from_lds(sO + io * IO_HALFS, lane);
-          o.store(os + t * p.os.l, t < p.seqlen, left);
-        }
-        if (c < c1) {
+          if (OUT && c > c0) store_o(c - 1);
           lds_barrier();                         // 2
           lds_barrier();                         // 3
         }
-      }
+        lds_barrier();                           // the last piece's o is whole
+        if (OUT) store_o(c1 - 1);
+      };
+      if (left >= IO_COLS) run(std::true_type{});
+      else run(std::false_type{});
       return;
     }
   }
