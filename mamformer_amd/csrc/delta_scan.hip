@@ -371,10 +371,9 @@ __global__ __launch_bounds__((kScanThreads<T, (OUT || KEEP)>)) void delta_scan_k
           const int t = min(c * DC + lane, p.seqlen - 1);
           v.template load<FULL>(vs + t * p.vs.l, left);
         };
-        auto store_o = [&](int c) {
-          const int t = c * DC + lane;
+        auto store_o = [&](int c, bool row) {
           o.from_lds(sO + io * IO_HALFS, lane);
-          o.template store<FULL>(os + t * p.os.l, t < p.seqlen, left);
+          o.template store<FULL>(os + (c * DC + lane) * p.os.l, row, left);
         };
         load_v(c0);
         v.to_lds(to + (c0 & 1) * IOW * IO_HALFS, lane);
@@ -384,12 +383,12 @@ __global__ __launch_bounds__((kScanThreads<T, (OUT || KEEP)>)) void delta_scan_k
           lds_barrier();                         // 1
           v.to_lds(to + ((c + 1) & 1) * IOW * IO_HALFS, lane);
           load_v(c + 2);
-          if (OUT && c > c0) store_o(c - 1);
+          if (OUT && c > c0) store_o(c - 1, true);
           lds_barrier();                         // 2
           lds_barrier();                         // 3
         }
         lds_barrier();                           // the last piece's o is whole
-        if (OUT) store_o(c1 - 1);
+        if (OUT) store_o(c1 - 1, (c1 - 1) * DC + lane < p.seqlen);
       };
       if (left >= IO_COLS) run(std::true_type{});
       else run(std::false_type{});
