@@ -293,7 +293,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void delta_prep_kernel
 //   U = beta e^{G_end - G} delta of its tokens goes to the other, each adds K^T U to its rows.              [barrier 3]
 // bf16: a fifth wave fetches the next piece's fragments by LDS DMA and a sixth one v, and stores o: a wave that issues such
 // loads stands still while they drain (2000 of the 8000 cycles that a piece took before), which those two may.
-// KEEP: the entering states and delta are stored for the backward.  OUT: o is computed.
+// KEEP: the entering states and delta are stored for the backward.  OUT: o is computed.  What is multiplied and added in
+// one instruction is written out, so that all variants give the same bits.
 //
 // Bound by the latency of one piece on waves that have a SIMD to themselves, most of it the conversions (an instruction of
 // 4 cycles for each value and part); b 2, H 16, L 4096 has 256 sets of 16 columns for 1024 SIMDs.  Operands that no other
@@ -525,7 +526,7 @@ __global__ __launch_bounds__((kScanThreads<T, (OUT || KEEP)>)) void delta_scan_k
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float v = AHEAD ? (float)vb[i][r] : to_f32(vn[4 * i + r]);
-        R[i][r] = v - eg[i][r] * (cs[3] * (ss.inv * X[i][r] + xr[i][r]));
+        R[i][r] = __builtin_fmaf(-eg[i][r], cs[3] * __builtin_fmaf(ss.inv, X[i][r], xr[i][r]), v);
       }
     if (!AHEAD && c + 1 < c1) load_v(c + 1);
     // delta = T R: one's own tokens, and for the second wave those of the first
@@ -570,7 +571,7 @@ __global__ __launch_bounds__((kScanThreads<T, (OUT || KEEP)>)) void delta_scan_k
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) D[i][r] = rs * D[i][r] + es * E[i][r];
+        for (int r = 0; r < 4; ++r) D[i][r] = __builtin_fmaf(es, E[i][r], rs * D[i][r]);
       rs = 1.f;
     }
     const float ds = rs * cs[1];                 // of D, and of U until it leaves its own scale
@@ -629,7 +630,7 @@ __global__ __launch_bounds__((kScanThreads<T, (OUT || KEEP)>)) void delta_scan_k
 #pragma unroll
     for (int n = 0; n < NSH; ++n)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) S[n][r] = cs[0] * S[n][r] + own_us * u0[n][r] + other_us * u1[n][r];
+      for (int r = 0; r < 4; ++r) S[n][r] = __builtin_fmaf(other_us, u1[n][r], __builtin_fmaf(own_us, u0[n][r], cs[0] * S[n][r]));
     if constexpr (OUT) {
       f32x4 O[2] = {}, OX[2] = {};
 #pragma unroll
@@ -656,8 +657,8 @@ __global__ __launch_bounds__((kScanThreads<T, (OUT || KEEP)>)) void delta_scan_k
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          o[4 * i + r] = eg[i][r] * (yq * (ss.inv * Y[i][r] + yr[i][r])) + os * O[i][r];
-          if (hf == 1) o[4 * i + r] += ox * OX[i][r];
+          o[4 * i + r] = __builtin_fmaf(eg[i][r], yq * __builtin_fmaf(ss.inv, Y[i][r], yr[i][r]), os * O[i][r]);
+          if (hf == 1) o[4 * i + r] = __builtin_fmaf(ox, OX[i][r], o[4 * i + r]);
         }
       if constexpr (AHEAD) {
 #pragma unroll
