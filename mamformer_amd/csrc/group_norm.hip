@@ -46,85 +46,126 @@ struct Affine {
   }
 };
 
+// Chunks of rows r, r + step .. (beyond `last` that row again), all under way before the first is used; `full`: no chunk is
+// cut by its group's end.
+template <int U, typename T>
+__device__ __forceinline__ void load_rows(const T* src, int64_t stride, int64_t r, int64_t step, int64_t last, bool full, int left, Raw8<T> (&x)[U]) {
+  if (full) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u].load(src + min(r + u * step, last) * stride);
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u) load_raw(x[u], src + min(r + u * step, last) * stride, left);
+  }
+}
+template <typename T> constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;
+
 // ------------------------------------------------------------------ one position
+// A workgroup takes 256 / TG groups (or all, and several batch entries at once) and walks the batch with them, so that the
+// parameters stay in registers.  The variance is that of values centred by the rounded mean, which is mended by what is left.
 template <typename T, int TG>
-__global__ __launch_bounds__(256) void group_rows_kernel(GroupNormParams p) {
-  const int cg = p.channels / p.groups, c8 = threadIdx.x % TG * 8, left = cg - c8;
-  const int64_t items = p.batch * p.groups;
-  for (int64_t it = (int64_t)blockIdx.x * (256 / TG) + threadIdx.x / TG; it < items; it += (int64_t)gridDim.x * (256 / TG)) {
-    const int64_t n = it / p.groups;
-    const int g = (int)(it % p.groups), c = g * cg + c8;
-    float x[8] = {};
-    if (left > 0) load8(reinterpret_cast<const T*>(p.x) + n * p.x_sb + c, left, x);
-    float s = 0.f;
+__global__ __launch_bounds__(256) void group_rows_kernel(GroupNormParams p, int gb, int side) {
+  constexpr int U = kAhead<T>;
+  const int cg = p.channels / p.groups, c8 = threadIdx.x % TG * 8, left = cg - c8, slot = threadIdx.x / TG;
+  const int g = blockIdx.y * gb + slot % gb, sub = slot / gb;
+  if (sub >= side || g >= p.groups) return;      // no barrier follows; lanes of a group go together
+  const bool full = cg % 8 == 0;
+  const int c = g * cg + (left > 0 ? c8 : 0);
+  const float inv = 1.f / (float)cg;
+  const Affine a(p, c, (g + 1) * cg);
+  const int64_t step = (int64_t)gridDim.x * side;
+  for (int64_t n0 = (int64_t)blockIdx.x * side + sub; n0 < p.batch; n0 += U * step) {
+    Raw8<T> raw[U];
+    load_rows(reinterpret_cast<const T*>(p.x) + c, p.x_sb, n0, step, p.batch - 1, full, left, raw);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s += x[j];
-    const float mean = lanes_sum<TG>(s) / (float)cg;
-    float q = 0.f;
+    for (int u = 0; u < U; ++u) {
+      const int64_t n = n0 + u * step;
+      if (n >= p.batch) break;
+      float x[8], s = 0.f, q = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[j] -= mean;
-      q += j < left ? x[j] * x[j] : 0.f;
-    }
-    const float rstd = 1.f / sqrtf(lanes_sum<TG>(q) / (float)cg + p.eps);
-    if (left > 0) {
-      const Affine a(p, c, (g + 1) * cg);
+      for (int j = 0; j < 8; ++j) {
+        x[j] = j < left ? raw[u].get(j) : 0.f;
+        s += x[j];
+      }
+      const float mean = lanes_sum<TG>(s) * inv;
+      s = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = act(p.silu, x[j] * rstd * a.w[j] + a.b[j]);
-      store8(reinterpret_cast<T*>(p.y) + n * p.y_sb + c, left, x);
-    }
-    if (p.stats && c8 == 0) {
-      p.stats[2 * it] = mean;
-      p.stats[2 * it + 1] = rstd;
+      for (int j = 0; j < 8; ++j) {
+        x[j] = j < left ? x[j] - mean : 0.f;
+        s += x[j];
+        q += x[j] * x[j];
+      }
+      const float rest = lanes_sum<TG>(s) * inv;
+      const float var = lanes_sum<TG>(q) * inv - rest * rest;
+      const float rstd = 1.f / sqrtf((var < 0.f ? 0.f : var) + p.eps);
+      if (left > 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = act(p.silu, (x[j] - rest) * (rstd * a.w[j]) + a.b[j]);
+        store8(reinterpret_cast<T*>(p.y) + n * p.y_sb + c, left, x);
+      }
+      if (p.stats && c8 == 0) {
+        p.stats[2 * (n * p.groups + g)] = mean + rest;
+        p.stats[2 * (n * p.groups + g) + 1] = rstd;
+      }
     }
   }
 }
 
-// A workgroup takes 256 / TG groups (or all, and several batch entries at once) and walks the batch with them, so that a
-// thread adds its channels' gradients in registers; `part` (rows, channels, 2) gets a row for each that walked.
+// The same walk, a thread adding its channels' gradients in registers; `part` (rows, channels, 2) gets a row for each that
+// walked.
 template <typename T, int TG>
 __global__ __launch_bounds__(256) void group_rows_bwd_kernel(GroupNormBwdParams q, int gb, int side) {
+  constexpr int U = kAhead<T>;
   const GroupNormParams& p = q.f;
   const int cg = p.channels / p.groups, c8 = threadIdx.x % TG * 8, left = cg - c8, slot = threadIdx.x / TG;
   const int g = blockIdx.y * gb + slot % gb, sub = slot / gb;
   if (sub >= side || g >= p.groups) return;      // no barrier follows; lanes of a group go together
-  const int c = g * cg + c8;
-  const Affine a(p, left > 0 ? c : 0, (g + 1) * cg);
+  const bool full = cg % 8 == 0;
+  const int c = g * cg + (left > 0 ? c8 : 0);
+  const float inv = 1.f / (float)cg;
+  const Affine a(p, c, (g + 1) * cg);
   float A[8] = {}, B[8] = {};
-  for (int64_t n = (int64_t)blockIdx.x * side + sub; n < p.batch; n += (int64_t)gridDim.x * side) {
-    float x[8] = {}, d[8] = {};
-    if (left > 0) {
-      load8(reinterpret_cast<const T*>(p.x) + n * p.x_sb + c, left, x);
-      load8(reinterpret_cast<const T*>(q.dy) + n * q.dy_sb + c, left, d);
-    }
-    const float mean = p.stats[2 * (n * p.groups + g)], rstd = p.stats[2 * (n * p.groups + g) + 1];
-    float s1 = 0.f, s2 = 0.f;
+  const int64_t step = (int64_t)gridDim.x * side;
+  for (int64_t n0 = (int64_t)blockIdx.x * side + sub; n0 < p.batch; n0 += U * step) {
+    Raw8<T> rx[U], rd[U];
+    float mean[U], rstd[U];
+    load_rows(reinterpret_cast<const T*>(p.x) + c, p.x_sb, n0, step, p.batch - 1, full, left, rx);
+    load_rows(reinterpret_cast<const T*>(q.dy) + c, q.dy_sb, n0, step, p.batch - 1, full, left, rd);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[j] = (x[j] - mean) * rstd;
-      const float dz = j < left ? d[j] * act_slope(p.silu, x[j] * a.w[j] + a.b[j]) : 0.f;
-      A[j] += dz;
-      B[j] += dz * x[j];
-      d[j] = dz * a.w[j];
-      s1 += d[j];
-      s2 += d[j] * x[j];
+    for (int u = 0; u < U; ++u) {
+      const float* st = p.stats + 2 * (min(n0 + u * step, p.batch - 1) * p.groups + g);
+      mean[u] = st[0];
+      rstd[u] = st[1];
     }
-    s1 = lanes_sum<TG>(s1) / (float)cg;
-    s2 = lanes_sum<TG>(s2) / (float)cg;
-    if (left > 0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = rstd * (d[j] - s1 - x[j] * s2);
-      store8(reinterpret_cast<T*>(q.dx) + n * q.dx_sb + c, left, x);
+    for (int u = 0; u < U; ++u) {
+      const int64_t n = n0 + u * step;
+      if (n >= p.batch) break;
+      float x[8], d[8], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[j] = j < left ? (rx[u].get(j) - mean[u]) * rstd[u] : 0.f;
+        const float dz = j < left ? rd[u].get(j) * act_slope(p.silu, x[j] * a.w[j] + a.b[j]) : 0.f;
+        A[j] += dz;
+        B[j] += dz * x[j];
+        d[j] = dz * a.w[j];
+        s1 += d[j];
+        s2 += d[j] * x[j];
+      }
+      s1 = lanes_sum<TG>(s1) * inv;
+      s2 = lanes_sum<TG>(s2) * inv;
+      if (left > 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = rstd[u] * (d[j] - s1 - x[j] * s2);
+        store8(reinterpret_cast<T*>(q.dx) + n * q.dx_sb + c, left, x);
+      }
     }
   }
   if (q.part && left > 0) {
     float* to = q.part + (((int64_t)blockIdx.x * side + sub) * p.channels + c) * 2;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (j < left) {
-        to[2 * j] = A[j];
-        to[2 * j + 1] = B[j];
-      }
+      if (j < left) *reinterpret_cast<f32x2*>(to + 2 * j) = f32x2{A[j], B[j]};
   }
 }
 
@@ -135,10 +176,15 @@ __global__ __launch_bounds__(256) void group_params_kernel(const float* part, in
   const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
   float a = 0.f, b = 0.f;
   if (c < channels)
-    for (int64_t r = rl; r < rows; r += 16) {
-      const f32x2 v = *reinterpret_cast<const f32x2*>(part + (r * channels + c) * 2);
-      a += v[0];
-      b += v[1];
+    for (int64_t r = rl; r < rows; r += 16 * 8) {
+      f32x2 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = *reinterpret_cast<const f32x2*>(part + (min(r + 16 * u, rows - 1) * channels + c) * 2);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        a += r + 16 * u < rows ? v[u][0] : 0.f;
+        b += r + 16 * u < rows ? v[u][1] : 0.f;
+      }
     }
   sa[rl][cl] = a;
   sb[rl][cl] = b;
@@ -188,6 +234,7 @@ struct Split {
 
 template <typename T>
 __global__ __launch_bounds__(256) void group_sums_kernel(GroupNormParams p, Split sp) {
+  constexpr int U = kAhead<T>;
   __shared__ double sa[256], sb[256];
   const int tid = threadIdx.x, u0 = sp.ub <= 256 ? tid % sp.ub : tid, sub = sp.ub <= 256 ? tid / sp.ub : 0;
   for (int64_t unit = blockIdx.x; unit < sp.units; unit += gridDim.x) {
@@ -200,13 +247,18 @@ __global__ __launch_bounds__(256) void group_sums_kernel(GroupNormParams p, Spli
       const int g = cb * sp.gb + u / sp.cpg, c8 = u % sp.cpg * 8;
       if (g >= p.groups) break;
       const T* src = reinterpret_cast<const T*>(p.x) + n * p.x_sb + g * sp.cg + c8;
-      for (int64_t r = r0 + sub; r < r1; r += sp.side) {
-        float x[8];
-        load8(src + r * p.x_ss, sp.cg - c8, x);
+      for (int64_t r = r0 + sub; r < r1; r += U * sp.side) {
+        Raw8<T> raw[U];
+        load_rows(src, p.x_ss, r, sp.side, p.space - 1, sp.cg % 8 == 0, sp.cg - c8, raw);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          a += (double)x[j];
-          b += (double)x[j] * (double)x[j];
+        for (int v = 0; v < U; ++v) {
+          if (r + v * sp.side >= r1) break;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const double x = raw[v].get(j);
+            a += x;
+            b += x * x;
+          }
         }
       }
     }
@@ -231,21 +283,40 @@ __global__ __launch_bounds__(256) void group_sums_kernel(GroupNormParams p, Spli
 
 template <typename T>
 __global__ __launch_bounds__(256) void group_apply_kernel(GroupNormParams p, Split sp) {
+  constexpr int U = kAhead<T>;
   __shared__ float sm[256], sr[256];
+  __shared__ double sa[256], sb[256];
   const int tid = threadIdx.x, u0 = sp.ub <= 256 ? tid % sp.ub : tid, sub = sp.ub <= 256 ? tid / sp.ub : 0;
   for (int64_t unit = blockIdx.x; unit < sp.units; unit += gridDim.x) {
     int64_t n;
     int s, cb;
     sp.at(unit, n, s, cb);
     __syncthreads();
+    const int shares = 256 / sp.gb;              // the splits' sums, by all threads
+    if (tid < sp.gb * shares) {
+      const int g = min(cb * sp.gb + tid % sp.gb, p.groups - 1);
+      double a = 0., b = 0.;
+      for (int i = tid / sp.gb; i < sp.splits; i += 8 * shares) {
+        double2 t[8];
+#pragma unroll
+        for (int v = 0; v < 8; ++v)
+          t[v] = *reinterpret_cast<const double2*>(p.part + ((n * sp.splits + min(i + v * shares, sp.splits - 1)) * p.groups + g) * 2);
+#pragma unroll
+        for (int v = 0; v < 8; ++v) {
+          a += i + v * shares < sp.splits ? t[v].x : 0.;
+          b += i + v * shares < sp.splits ? t[v].y : 0.;
+        }
+      }
+      sa[tid] = a;
+      sb[tid] = b;
+    }
+    __syncthreads();
     if (tid < sp.gb && cb * sp.gb + tid < p.groups) {
       const int g = cb * sp.gb + tid;
-      double a = 0., b = 0.;
-#pragma unroll 8
-      for (int i = 0; i < sp.splits; ++i) {
-        const double* from = p.part + ((n * sp.splits + i) * p.groups + g) * 2;
-        a += from[0];
-        b += from[1];
+      double a = sa[tid], b = sb[tid];
+      for (int i = 1; i < shares; ++i) {
+        a += sa[i * sp.gb + tid];
+        b += sb[i * sp.gb + tid];
       }
       const double count = (double)p.space * sp.cg, mean = a / count, var = b / count - mean * mean;
       sm[tid] = (float)mean;
@@ -263,14 +334,22 @@ __global__ __launch_bounds__(256) void group_apply_kernel(GroupNormParams p, Spl
       const int c = g * sp.cg + c8;
       const Affine a(p, c, (g + 1) * sp.cg);
       const float mean = sm[u / sp.cpg], rstd = sr[u / sp.cpg];
+      float rw[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) rw[j] = rstd * a.w[j];
       const T* src = reinterpret_cast<const T*>(p.x) + n * p.x_sb + c;
       T* dst = reinterpret_cast<T*>(p.y) + n * p.y_sb + c;
-      for (int64_t r = r0 + sub; r < r1; r += sp.side) {
-        float x[8];
-        load8(src + r * p.x_ss, left, x);
+      for (int64_t r = r0 + sub; r < r1; r += U * sp.side) {
+        Raw8<T> raw[U];
+        load_rows(src, p.x_ss, r, sp.side, p.space - 1, sp.cg % 8 == 0, left, raw);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = act(p.silu, (x[j] - mean) * rstd * a.w[j] + a.b[j]);
-        store8(dst + r * p.y_ss, left, x);
+        for (int v = 0; v < U; ++v) {
+          if (r + v * sp.side >= r1) break;
+          float x[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = act(p.silu, (raw[v].get(j) - mean) * rw[j] + a.b[j]);
+          store8(dst + (r + v * sp.side) * p.y_ss, left, x);
+        }
       }
     }
   }
@@ -279,6 +358,7 @@ __global__ __launch_bounds__(256) void group_apply_kernel(GroupNormParams p, Spl
 // Sums of dz and dz xh for every channel of a workgroup's positions: part (batch, splits, channels, 2).
 template <typename T>
 __global__ __launch_bounds__(256) void group_bwd_sums_kernel(GroupNormBwdParams q, Split sp) {
+  constexpr int U = kAhead<T>;
   __shared__ float sa[256][17];
   const GroupNormParams& p = q.f;
   const int tid = threadIdx.x, u0 = sp.ub <= 256 ? tid % sp.ub : tid, sub = sp.ub <= 256 ? tid / sp.ub : 0;
@@ -297,16 +377,20 @@ __global__ __launch_bounds__(256) void group_bwd_sums_kernel(GroupNormBwdParams 
         const float mean = p.stats[2 * (n * p.groups + g)], rstd = p.stats[2 * (n * p.groups + g) + 1];
         const T* xs = reinterpret_cast<const T*>(p.x) + n * p.x_sb + c;
         const T* ds = reinterpret_cast<const T*>(q.dy) + n * q.dy_sb + c;
-        for (int64_t r = r0 + sub; r < r1; r += sp.side) {
-          float x[8], d[8];
-          load8(xs + r * p.x_ss, left, x);
-          load8(ds + r * q.dy_ss, left, d);
+        for (int64_t r = r0 + sub; r < r1; r += U * sp.side) {
+          Raw8<T> rx[U], rd[U];
+          load_rows(xs, p.x_ss, r, sp.side, p.space - 1, sp.cg % 8 == 0, left, rx);
+          load_rows(ds, q.dy_ss, r, sp.side, p.space - 1, sp.cg % 8 == 0, left, rd);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            x[j] = (x[j] - mean) * rstd;
-            const float dz = j < left ? d[j] * act_slope(p.silu, x[j] * a.w[j] + a.b[j]) : 0.f;
-            A[j] += dz;
-            B[j] += dz * x[j];
+          for (int v = 0; v < U; ++v) {
+            if (r + v * sp.side >= r1) break;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float x = (rx[v].get(j) - mean) * rstd;
+              const float dz = j < left ? rd[v].get(j) * act_slope(p.silu, x * a.w[j] + a.b[j]) : 0.f;
+              A[j] += dz;
+              B[j] += dz * x;
+            }
           }
         }
       }
@@ -335,31 +419,38 @@ __global__ __launch_bounds__(256) void group_bwd_sums_kernel(GroupNormBwdParams 
   }
 }
 
-// The splits joined: `whole` (batch, channels, 2), and mean(gw), mean(gw xh) of each (batch, group) into `means`.  A wave
-// for each (batch, group).
+// The splits joined: `whole` (batch, channels, 2), and mean(gw), mean(gw xh) of each (batch, group) into `means`.  A
+// workgroup for each (batch, group), its waves a fourth of the splits each.
 __global__ __launch_bounds__(256) void group_bwd_join_kernel(GroupNormBwdParams q, Split sp, float* whole, float* means) {
+  __shared__ f32x2 sv[4][64];
   const GroupNormParams& p = q.f;
-  const int lane = threadIdx.x & 63;
-  const int64_t items = p.batch * p.groups;
-  for (int64_t it = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); it < items; it += (int64_t)gridDim.x * 4) {
+  const int lane = threadIdx.x & 63, w = wave_id();
+  for (int64_t it = blockIdx.x; it < p.batch * p.groups; it += gridDim.x) {
     const int64_t n = it / p.groups;
     const int g = (int)(it % p.groups);
     float s1 = 0.f, s2 = 0.f;
-    for (int i = lane; i < sp.cg; i += 64) {
-      const int c = g * sp.cg + i;
-      float a = 0.f, b = 0.f;
-#pragma unroll 8
-      for (int s = 0; s < sp.splits; ++s) {
-        const f32x2 v = *reinterpret_cast<const f32x2*>(q.part + ((n * sp.splits + s) * p.channels + c) * 2);
-        a += v[0];
-        b += v[1];
+    for (int i0 = 0; i0 < sp.cg; i0 += 64) {
+      const int i = i0 + lane, c = g * sp.cg + min(i, sp.cg - 1);
+      f32x2 v = {};
+      for (int s = w; s < sp.splits; s += 4 * 8) {
+        f32x2 t[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) t[u] = *reinterpret_cast<const f32x2*>(q.part + ((n * sp.splits + min(s + 4 * u, sp.splits - 1)) * p.channels + c) * 2);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v += s + 4 * u < sp.splits ? t[u] : f32x2{};
       }
-      whole[(n * p.channels + c) * 2] = a;
-      whole[(n * p.channels + c) * 2 + 1] = b;
-      const float w = !p.weight ? 1.f : p.w_f32 ? reinterpret_cast<const float*>(p.weight)[c] : to_f32(reinterpret_cast<const bf16*>(p.weight)[c]);
-      s1 += w * a;
-      s2 += w * b;
+      __syncthreads();
+      sv[w][lane] = v;
+      __syncthreads();
+      if (w == 0 && i < sp.cg) {
+        v = (sv[0][lane] + sv[1][lane]) + (sv[2][lane] + sv[3][lane]);
+        *reinterpret_cast<f32x2*>(whole + (n * p.channels + c) * 2) = v;
+        const float wt = !p.weight ? 1.f : p.w_f32 ? reinterpret_cast<const float*>(p.weight)[c] : to_f32(reinterpret_cast<const bf16*>(p.weight)[c]);
+        s1 += wt * v[0];
+        s2 += wt * v[1];
+      }
     }
+    if (w != 0) continue;
     s1 = group_sum<64>(s1);
     s2 = group_sum<64>(s2);
     if (lane == 0) {
@@ -372,6 +463,7 @@ __global__ __launch_bounds__(256) void group_bwd_join_kernel(GroupNormBwdParams 
 
 template <typename T>
 __global__ __launch_bounds__(256) void group_bwd_apply_kernel(GroupNormBwdParams q, Split sp, const float* means) {
+  constexpr int U = kAhead<T>;
   const GroupNormParams& p = q.f;
   const int tid = threadIdx.x, u0 = sp.ub <= 256 ? tid % sp.ub : tid, sub = sp.ub <= 256 ? tid / sp.ub : 0;
   if (sub >= sp.side) return;
@@ -390,17 +482,22 @@ __global__ __launch_bounds__(256) void group_bwd_apply_kernel(GroupNormBwdParams
       const T* xs = reinterpret_cast<const T*>(p.x) + n * p.x_sb + c;
       const T* ds = reinterpret_cast<const T*>(q.dy) + n * q.dy_sb + c;
       T* out = reinterpret_cast<T*>(q.dx) + n * q.dx_sb + c;
-      for (int64_t r = r0 + sub; r < r1; r += sp.side) {
-        float x[8], d[8];
-        load8(xs + r * p.x_ss, left, x);
-        load8(ds + r * q.dy_ss, left, d);
+      for (int64_t r = r0 + sub; r < r1; r += U * sp.side) {
+        Raw8<T> rx[U], rd[U];
+        load_rows(xs, p.x_ss, r, sp.side, p.space - 1, sp.cg % 8 == 0, left, rx);
+        load_rows(ds, q.dy_ss, r, sp.side, p.space - 1, sp.cg % 8 == 0, left, rd);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x[j] = (x[j] - mean) * rstd;
-          const float gw = d[j] * act_slope(p.silu, x[j] * a.w[j] + a.b[j]) * a.w[j];
-          x[j] = rstd * (gw - m1 - x[j] * m2);
+        for (int v = 0; v < U; ++v) {
+          if (r + v * sp.side >= r1) break;
+          float x[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            x[j] = (rx[v].get(j) - mean) * rstd;
+            const float gw = rd[v].get(j) * act_slope(p.silu, x[j] * a.w[j] + a.b[j]) * a.w[j];
+            x[j] = rstd * (gw - m1 - x[j] * m2);
+          }
+          store8(out + (r + v * sp.side) * q.dx_ss, left, x);
         }
-        store8(out + r * q.dx_ss, left, x);
       }
     }
   }
@@ -416,13 +513,13 @@ int rows_lanes(const GroupNormParams& p) {
 
 struct RowsGrid {
   int gb, side, x, y;
-  explicit RowsGrid(const GroupNormParams& p) {
+  RowsGrid(const GroupNormParams& p, int workgroups) {
     const int slots = 256 / rows_lanes(p);
     gb = slots < p.groups ? slots : p.groups;
     side = slots / gb;
     y = (p.groups + gb - 1) / gb;
     const int64_t most = (p.batch + side - 1) / side;
-    const int64_t want = 512 / y + 1;
+    const int64_t want = workgroups / y + 1;
     x = (int)(want < most ? want : most);
   }
 };
@@ -446,9 +543,8 @@ hipError_t with_lanes(int n, F f) {
 template <typename T>
 hipError_t fwd(const GroupNormParams& p, hipStream_t st) {
   if (by_rows(p)) {
-    const int lanes = rows_lanes(p);
-    const int64_t blocks = (p.batch * p.groups + 256 / lanes - 1) / (256 / lanes);
-    return with_lanes(lanes, [&](auto n) { group_rows_kernel<T, decltype(n)::value><<<grid_of(blocks), 256, 0, st>>>(p); });
+    const RowsGrid rg(p, 2048);
+    return with_lanes(rows_lanes(p), [&](auto n) { group_rows_kernel<T, decltype(n)::value><<<dim3(rg.x, rg.y), 256, 0, st>>>(p, rg.gb, rg.side); });
   }
   const Split sp(p);
   group_sums_kernel<T><<<grid_of(sp.units), 256, 0, st>>>(p, sp);
@@ -463,7 +559,7 @@ hipError_t bwd(const GroupNormBwdParams& q, hipStream_t st) {
   const float* rows = q.part;
   int64_t nrows = p.batch;
   if (by_rows(p)) {
-    const RowsGrid rg(p);
+    const RowsGrid rg(p, 512);
     GroupNormBwdParams r = q;
     if (!params) r.part = nullptr;
     const hipError_t e = with_lanes(rows_lanes(p), [&](auto n) {
@@ -476,7 +572,7 @@ hipError_t bwd(const GroupNormBwdParams& q, hipStream_t st) {
     float* whole = q.part + p.batch * sp.splits * p.channels * 2;
     float* means = whole + p.batch * p.channels * 2;
     group_bwd_sums_kernel<T><<<grid_of(sp.units), 256, 0, st>>>(q, sp);
-    group_bwd_join_kernel<<<grid_of((p.batch * p.groups + 3) / 4), 256, 0, st>>>(q, sp, whole, means);
+    group_bwd_join_kernel<<<grid_of(p.batch * p.groups), 256, 0, st>>>(q, sp, whole, means);
     group_bwd_apply_kernel<T><<<grid_of(sp.units), 256, 0, st>>>(q, sp, means);
     rows = whole;
   }
@@ -514,7 +610,7 @@ hipError_t launch_group_norm(const GroupNormParams& p, hipStream_t st) {
 size_t group_norm_bwd_workspace_bytes(const GroupNormParams& p) {
   if (p.batch == 0 || p.space == 0) return 0;
   if (by_rows(p)) {
-    const RowsGrid rg(p);
+    const RowsGrid rg(p, 512);
     return (size_t)rg.x * rg.side * p.channels * 2 * sizeof(float);
   }
   return ((size_t)p.batch * (Split(p).splits + 1) * p.channels + (size_t)p.batch * p.groups) * 2 * sizeof(float);
