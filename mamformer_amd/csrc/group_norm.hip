@@ -291,6 +291,14 @@ __global__ __launch_bounds__(256) void group_apply_kernel(GroupNormParams p, Spl
     int64_t n;
     int s, cb;
     sp.at(unit, n, s, cb);
+    const int64_t r0 = s * sp.rows, r1 = min(p.space, r0 + sp.rows);
+    const bool full = sp.cg % 8 == 0;
+    Raw8<T> raw[U];
+    auto load = [&](int u, int64_t r) {
+      const int g = min(cb * sp.gb + u / sp.cpg, p.groups - 1), c8 = u % sp.cpg * 8;
+      load_rows(reinterpret_cast<const T*>(p.x) + n * p.x_sb + g * sp.cg + c8, p.x_ss, r, sp.side, p.space - 1, full, sp.cg - c8, raw);
+    };
+    if (u0 < sp.ub && sub < sp.side) load(u0, r0 + sub);               // under way while the sums are joined
     __syncthreads();
     const int shares = 256 / sp.gb;              // the splits' sums, by all threads
     if (tid < sp.gb * shares) {
@@ -327,7 +335,6 @@ __global__ __launch_bounds__(256) void group_apply_kernel(GroupNormParams p, Spl
       }
     }
     __syncthreads();
-    const int64_t r0 = s * sp.rows, r1 = min(p.space, r0 + sp.rows);
     for (int u = u0; u < sp.ub && sub < sp.side; u += 256) {
       const int g = cb * sp.gb + u / sp.cpg, c8 = u % sp.cpg * 8, left = sp.cg - c8;
       if (g >= p.groups) break;
@@ -337,17 +344,19 @@ __global__ __launch_bounds__(256) void group_apply_kernel(GroupNormParams p, Spl
       float rw[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) rw[j] = rstd * a.w[j];
-      const T* src = reinterpret_cast<const T*>(p.x) + n * p.x_sb + c;
       T* dst = reinterpret_cast<T*>(p.y) + n * p.y_sb + c;
+      if (u != u0) load(u, r0 + sub);
       for (int64_t r = r0 + sub; r < r1; r += U * sp.side) {
-        Raw8<T> raw[U];
-        load_rows(src, p.x_ss, r, sp.side, p.space - 1, sp.cg % 8 == 0, left, raw);
+        Raw8<T> now[U];
+#pragma unroll
+        for (int v = 0; v < U; ++v) now[v] = raw[v];
+        if (r + U * sp.side < r1) load(u, r + U * sp.side);
 #pragma unroll
         for (int v = 0; v < U; ++v) {
           if (r + v * sp.side >= r1) break;
           float x[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = act(p.silu, (raw[v].get(j) - mean) * rw[j] + a.b[j]);
+          for (int j = 0; j < 8; ++j) x[j] = act(p.silu, (now[v].get(j) - mean) * rw[j] + a.b[j]);
           store8(dst + (r + v * sp.side) * p.y_ss, left, x);
         }
       }
