@@ -4,12 +4,15 @@
 //
 // Bound by the rows' bytes.  Angles: position * inv_freq / (2 pi) in fp64, of which the fraction of a turn is left, exact
 // to fp32 for positions beyond 2^31 turns; then the sine and cosine of that many turns in fp32.  A thread computes those of
-// its 8 pairs once and runs through its share of the heads of queries and keys with them.
+// its 8 pairs once, while its first heads' channels are under way, and runs through its share of the heads of queries and
+// keys with them.
 #include "launch.h"
 #include "rows.h"
 
 namespace mh {
 namespace {
+
+constexpr int U = 4;                             // heads whose loads are under way at once
 
 template <typename T, bool INTER>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p, int chunks, int shares, int per) {
@@ -25,6 +28,29 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p, int chunks,
   const bool turn = c < turning;
   const int n = turn ? min(8, p.pairs - 8 * c) : 0;
   const int ch = turn ? (INTER ? 16 * c : 8 * c) : 2 * p.pairs + 8 * (c - turning);
+  const int left0 = turn ? (INTER ? 2 * n : n) : p.dim - ch, off1 = turn ? (INTER ? 8 : p.pairs) : 0;
+  const int left1 = turn ? (INTER ? 2 * n - 8 : n) : left0;            // a chunk that passes is read twice, written once
+  const bool full = p.pairs % 8 == 0 && (p.dim - 2 * p.pairs) % 8 == 0;
+  const int total = p.q_heads + p.k_heads, h0 = share * per, h1 = min(total, h0 + per);
+  Raw8<T> a[U], e[U];
+  auto load = [&](int h) {                       // of U heads
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int hu = h + u;
+      if (hu >= h1) break;
+      const bool isq = hu < p.q_heads;
+      const RotaryTensor& x = isq ? p.q : p.k;
+      const T* in = reinterpret_cast<const T*>(x.in) + (isq ? hu : hu - p.q_heads) * x.in_s.h + b * x.in_s.b + l * x.in_s.l + ch;
+      if (full) {
+        a[u].load(in);
+        e[u].load(in + off1);
+      } else {
+        load_raw(a[u], in, left0);
+        load_raw(e[u], in + off1, left1);
+      }
+    }
+  };
+  load(h0);
   float cs[8], sn[8];
   if (turn) {
     const double pos = (double)((p.positions ? load_index(p.positions, p.i64, b * p.pos_sb + l) : (int64_t)l) + p.offset);
@@ -38,48 +64,42 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p, int chunks,
       cs[j] = co * p.scale;
       sn[j] = (p.inverse ? -s : s) * p.scale;
     }
-  }
-  const int total = p.q_heads + p.k_heads, h1 = min(total, (share + 1) * per);
-  for (int h = share * per; h < h1; ++h) {
-    const bool isq = h < p.q_heads;
-    const RotaryTensor& x = isq ? p.q : p.k;
-    const int64_t hh = isq ? h : h - p.q_heads;
-    const T* in = reinterpret_cast<const T*>(x.in) + b * x.in_s.b + hh * x.in_s.h + l * x.in_s.l + ch;
-    T* out = reinterpret_cast<T*>(x.out) + b * x.out_s.b + hh * x.out_s.h + l * x.out_s.l + ch;
-    float a[8], e[8];
-    if (!turn) {
-      load8(in, p.dim - ch, a);
-      store8(out, p.dim - ch, a);
-    } else if (INTER) {
-      load8(in, 2 * n, a);
-      if (n > 4) load8(in + 8, 2 * n - 8, e);
+  } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float x0 = a[2 * j], x1 = a[2 * j + 1];
-        a[2 * j] = x0 * cs[j] - x1 * sn[j];
-        a[2 * j + 1] = x1 * cs[j] + x0 * sn[j];
-      }
-      store8(out, 2 * n, a);
-      if (n > 4) {
+    for (int j = 0; j < 8; ++j) cs[j] = sn[j] = 0.f;
+  }
+  for (int h = h0; h < h1; h += U) {
+    if (h != h0) load(h);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (h + u >= h1) break;
+      const bool isq = h + u < p.q_heads;
+      const RotaryTensor& x = isq ? p.q : p.k;
+      T* out = reinterpret_cast<T*>(x.out) + (isq ? h + u : h + u - p.q_heads) * x.out_s.h + b * x.out_s.b + l * x.out_s.l + ch;
+      float y0[8], y1[8];
+      if (INTER) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float x0 = e[2 * j], x1 = e[2 * j + 1];
-          e[2 * j] = x0 * cs[4 + j] - x1 * sn[4 + j];
-          e[2 * j + 1] = x1 * cs[4 + j] + x0 * sn[4 + j];
+          const float p0 = a[u].get(2 * j), p1 = a[u].get(2 * j + 1), r0 = e[u].get(2 * j), r1 = e[u].get(2 * j + 1);
+          y0[2 * j] = p0 * cs[j] - p1 * sn[j];
+          y0[2 * j + 1] = p1 * cs[j] + p0 * sn[j];
+          y1[2 * j] = r0 * cs[4 + j] - r1 * sn[4 + j];
+          y1[2 * j + 1] = r1 * cs[4 + j] + r0 * sn[4 + j];
         }
-        store8(out + 8, 2 * n - 8, e);
-      }
-    } else {
-      load8(in, n, a);
-      load8(in + p.pairs, n, e);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float x0 = a[j], x1 = e[j];
-        a[j] = x0 * cs[j] - x1 * sn[j];
-        e[j] = x1 * cs[j] + x0 * sn[j];
+        for (int j = 0; j < 8; ++j) {
+          const float x0 = a[u].get(j), x1 = e[u].get(j);
+          y0[j] = x0 * cs[j] - x1 * sn[j];
+          y1[j] = x1 * cs[j] + x0 * sn[j];
+        }
       }
-      store8(out, n, a);
-      store8(out + p.pairs, n, e);
+      if (!turn) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y0[j] = a[u].get(j);
+      }
+      store8(out, left0, y0);
+      if (turn && left1 > 0) store8(out + off1, left1, y1);
     }
   }
 }
@@ -90,7 +110,8 @@ hipError_t run(const RotaryParams& p, hipStream_t st) {
   const int64_t blocks = ((int64_t)p.batch * p.seqlen * chunks + 255) / 256;
   int shares = (int)((1024 + blocks - 1) / blocks);
   if (shares > total) shares = total;
-  const int per = (total + shares - 1) / shares;
+  int per = (total + shares - 1) / shares;
+  if (per > U) per = (per + U - 1) / U * U;
   shares = (total + per - 1) / per;
   const dim3 grid((unsigned)blocks, (unsigned)shares);
   if (p.interleaved) rotary_kernel<T, true><<<grid, 256, 0, st>>>(p, chunks, shares, per);
