@@ -181,6 +181,13 @@ __device__ __forceinline__ void keep_parts(f16* to, int s0, const f16x8 (&hi)[N]
 }
 
 int delta_segments(const DeltaParams& p);        // how many a sequence is scanned in
+constexpr int64_t kCUs = 256;                    // a workgroup of a scan fills one
+// bf16: pairs of waves in workgroups of their own where every one of them has a CU to itself.
+inline bool delta_one_pair(const DeltaParams& p, int segs) { return (int64_t)p.batch * p.heads * segs * ((p.dv + 15) / 16) <= kCUs; }
+// A scan's workgroup: pairs, and for bf16 a wave that fetches and one for each 32 columns of v.
+template <int PAIRS> constexpr int kIoWaves = PAIRS == 4 ? 2 : 1;
+template <int PAIRS> constexpr int kIoCols = PAIRS == 1 ? 16 : 32;
+template <typename T, int PAIRS> constexpr int kDeltaThreads = 64 * (2 * PAIRS + (sizeof(T) == 4 ? 0 : 1 + kIoWaves<PAIRS>));
 
 struct DeltaLayout {
   size_t kq, tp, vec, keep, scales, total;       // byte offsets
@@ -270,16 +277,15 @@ __device__ __forceinline__ void store_rows8(T* at, int64_t stride, int len, bool
 
 // 32 columns of a piece's rows by a wave that does nothing else, a token a lane, to and from LDS by columns
 // ([column][token]), where the waves that compute read and write 4 tokens of a column at once.
-constexpr int IO_COLS = 32, IO_PITCH = 68;       // 34 banks a column: 16 columns of 8 bytes meet every bank once
-constexpr int IO_HALFS = IO_COLS * IO_PITCH;
-struct IoRows {
-  bf16x8 v[IO_COLS / 8];
+constexpr int IO_PITCH = 68;                     // 34 banks a column: 16 columns of 8 bytes meet every bank once
+template <int COLS> struct IoRows {
+  bf16x8 v[COLS / 8];
   // `at`: column 0 of the lane's token, of which `left` columns exist; FULL: all of them, then without a branch, so that a
   // load stays under way until to_lds of the piece after next
   template <bool FULL>
   __device__ __forceinline__ void load(const bf16* at, int left) {
 #pragma unroll
-    for (int i = 0; i < IO_COLS / 8; ++i) {
+    for (int i = 0; i < COLS / 8; ++i) {
       Raw8<bf16> r;
       if constexpr (!FULL) r.clear();
       if (FULL || left > 8 * i) load_raw(r, at + 8 * i, FULL ? 8 : left - 8 * i);
@@ -290,7 +296,7 @@ struct IoRows {
   __device__ __forceinline__ void store(bf16* at, bool row, int left) const {
     if (!row) return;
 #pragma unroll
-    for (int i = 0; i < IO_COLS / 8; ++i) {
+    for (int i = 0; i < COLS / 8; ++i) {
       if (FULL || left >= 8 * i + 8) put_vec<false>(at + 8 * i, v[i]);
       else
 #pragma unroll
@@ -300,15 +306,15 @@ struct IoRows {
   }
   __device__ __forceinline__ void to_lds(bf16* t, int lane) const {
 #pragma unroll
-    for (int c = 0; c < IO_COLS; ++c) t[c * IO_PITCH + lane] = v[c / 8][c % 8];
+    for (int c = 0; c < COLS; ++c) t[c * IO_PITCH + lane] = v[c / 8][c % 8];
   }
   __device__ __forceinline__ void zero_unless(bool row) {
 #pragma unroll
-    for (int i = 0; i < IO_COLS / 8; ++i) v[i] = row ? v[i] : bf16x8{};
+    for (int i = 0; i < COLS / 8; ++i) v[i] = row ? v[i] : bf16x8{};
   }
   __device__ __forceinline__ void from_lds(const bf16* t, int lane) {
 #pragma unroll
-    for (int c = 0; c < IO_COLS; ++c) v[c / 8][c % 8] = t[c * IO_PITCH + lane];
+    for (int c = 0; c < COLS; ++c) v[c / 8][c % 8] = t[c * IO_PITCH + lane];
   }
 };
 

@@ -20,8 +20,8 @@ namespace {
 // Two waves hold the gradient of 16 columns of the state as the forward's scan holds the state: half of its rows and half of
 // a piece's tokens each, with a fifth and a sixth wave that fetch.  y = T^T ddelta is upper triangular, so that here the
 // first wave needs the second one's ddelta.
-template <typename T, int DKP>
-__global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_back_scan_kernel(DeltaBwdParams q, DeltaLayout lay, DeltaScratch scr, int nblk, int nwg) {
+template <typename T, int DKP, int PAIRS>
+__global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_back_scan_kernel(DeltaBwdParams q, DeltaLayout lay, DeltaScratch scr, int nblk, int nwg) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
   constexpr bool AHEAD = NP == 1;
   constexpr int FW = AHEAD ? 1 : 4;
@@ -29,8 +29,8 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_back_scan_ke
   constexpr int GA = NP * F + 2 * kTFrags;                           // fragments of K by rows and P by columns: before barrier 1
   constexpr int GB = 2 * NP * F + 2 * kTFrags + 1;                   // K and Q by columns, T by columns, vec: after it
   constexpr int EX = (2 * 2 + 2 + 2 * 4 + 1) * FR;                   // halfs of a pair's exchange
-  constexpr int IO = AHEAD ? 2 * IO_HALFS : 0;
-  __shared__ __align__(1024) f16 smem[(GA + (AHEAD ? 2 : 1) * GB) * FR + 2 * EX + IO];
+  constexpr int IOC = kIoCols<PAIRS>, IOH = IOC * IO_PITCH, IO = AHEAD ? 2 * IOH : 0;
+  __shared__ __align__(1024) f16 smem[(GA + (AHEAD ? 2 : 1) * GB) * FR + PAIRS * EX + IO];
   const DeltaParams& p = q.f;
 
   const int lane = threadIdx.x & 63, w = wave_id(), l16 = lane & 15, g4 = lane >> 4, hf = w & 1;
@@ -38,7 +38,7 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_back_scan_ke
   if (!head_block(blockIdx.x, p.batch * p.heads, nwg, bh, wg)) return;
   const int b = bh / p.heads, h = bh % p.heads, hk = h / (p.heads / p.kheads);
   const int64_t kunit0 = ((int64_t)b * p.kheads + hk) * p.pieces, vunit0 = (int64_t)bh * p.pieces;
-  constexpr int DOUT = (GA + (AHEAD ? 2 : 1) * GB) * FR + 2 * EX;    // where dO of two pieces is
+  constexpr int DOUT = (GA + (AHEAD ? 2 : 1) * GB) * FR + PAIRS * EX;    // where dO of two pieces is
 
   const int fw = AHEAD ? 0 : w;
   lds_f16_t* const lds = (lds_f16_t*)smem;
@@ -53,7 +53,7 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_back_scan_ke
     if (fw == 0) fetch_share<1, 1>(to + (2 * NP * F + 2 * kTFrags) * FR, p.workspace + lay.vec + (vunit0 + c) * (int64_t)(kVecFloats * 4), 0, lane);
   };
   if constexpr (AHEAD) {
-    if (w == 4) {
+    if (w == 2 * PAIRS) {
       fetch_a(p.pieces - 1);
       fetch_b(p.pieces - 1);
       wait_vmem_n<GB>();
@@ -71,34 +71,34 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_back_scan_ke
       }
       return;
     }
-    if (w == 5) {                                // dO; tokens beyond the sequence have none
-      const int col0 = IO_COLS * wg, left = p.dv - col0;
+    if (w == 2 * PAIRS + 1) {                    // dO; tokens beyond the sequence have none
+      const int col0 = IOC * wg, left = p.dv - col0;
       const bf16* src = reinterpret_cast<const bf16*>(q.d_o) + b * q.dos.b + h * q.dos.h + col0;
       auto run = [&](auto full) {
-        IoRows v;
+        IoRows<IOC> v;
         auto load = [&](int c) {
           const int t = min(max(c, 0) * DC + lane, p.seqlen - 1);
           v.template load<decltype(full)::value>(src + t * q.dos.l, left);
         };
         load(p.pieces - 1);
         v.zero_unless((p.pieces - 1) * DC + lane < p.seqlen);
-        v.to_lds(reinterpret_cast<bf16*>(smem + DOUT + ((p.pieces - 1) & 1) * IO_HALFS), lane);
+        v.to_lds(reinterpret_cast<bf16*>(smem + DOUT + ((p.pieces - 1) & 1) * IOH), lane);
         load(p.pieces - 2);
         lds_barrier();
         for (int c = p.pieces - 1; c >= 0; --c) {
           lds_barrier();                         // 1
-          v.to_lds(reinterpret_cast<bf16*>(smem + DOUT + ((c + 1) & 1) * IO_HALFS), lane);
+          v.to_lds(reinterpret_cast<bf16*>(smem + DOUT + ((c + 1) & 1) * IOH), lane);
           load(c - 2);
           lds_barrier();                         // 2
           lds_barrier();                         // 3
         }
       };
-      if (left >= IO_COLS) run(std::true_type{});
+      if (left >= IOC) run(std::true_type{});
       else run(std::false_type{});
       return;
     }
   }
-  const int blk = 2 * wg + (w >> 1), col = 16 * blk + l16;
+  const int blk = PAIRS * wg + (w >> 1), col = 16 * blk + l16;
   const bool live = blk < nblk, cv = col < p.dv;
   f16* ex = smem + (GA + (AHEAD ? 2 : 1) * GB) * FR + (w >> 1) * EX;
   f32x4* const xSend = reinterpret_cast<f32x4*>(ex) + hf * 2 * 64 + lane;
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(sizeof(T) == 4 ? 256 : 384) void delta_back_scan_ke
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const bf16x4 v = *reinterpret_cast<const bf16x4*>(smem + DOUT + (c & 1) * IO_HALFS + ((w >> 1) * 16 + l16) * IO_PITCH + 32 * (x ? 1 - hf : hf) + 16 * i + 4 * g4);
+          const bf16x4 v = *reinterpret_cast<const bf16x4*>(smem + DOUT + (c & 1) * IOH + ((w >> 1) * 16 + l16) * IO_PITCH + 32 * (x ? 1 - hf : hf) + 16 * i + 4 * g4);
 #pragma unroll
           for (int r = 0; r < 4; ++r) on[x][4 * i + r] = v[r];
         }
@@ -789,7 +789,12 @@ hipError_t run_bwd(const DeltaBwdParams& q, hipStream_t st) {
   const DeltaLayout lay(p, true);
   const DeltaScratch scr(p);
   const int nblk = (p.dv + 15) / 16, nwg = (nblk + 1) / 2;
-  delta_back_scan_kernel<T, DKP><<<head_block_grid(p.batch * p.heads, nwg), sizeof(T) == 4 ? 256 : 384, 0, st>>>(q, lay, scr, nblk, nwg);
+  if (sizeof(T) == 2 && delta_one_pair(p, 1)) {
+    if constexpr (sizeof(T) == 2)
+      delta_back_scan_kernel<T, DKP, 1><<<head_block_grid(p.batch * p.heads, nblk), kDeltaThreads<T, 1>, 0, st>>>(q, lay, scr, nblk, nblk);
+  } else {
+    delta_back_scan_kernel<T, DKP, 2><<<head_block_grid(p.batch * p.heads, nwg), kDeltaThreads<T, 2>, 0, st>>>(q, lay, scr, nblk, nwg);
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   delta_grads_kernel<T, DKP><<<(unsigned)((int64_t)p.batch * p.kheads * p.pieces), 512, 0, st>>>(q, lay, scr, nblk);

@@ -299,14 +299,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void delta_prep_kernel
 // Bound by the latency of one piece on waves that have a SIMD to themselves, most of it the conversions (an instruction of
 // 4 cycles for each value and part); b 2, H 16, L 4096 has 256 sets of 16 columns for 1024 SIMDs.  Operands that no other
 // wave has to finish first are read from LDS right behind a barrier, ahead of what they are needed for.
-template <bool WHOLE> constexpr int kScanPairs = WHOLE ? 2 : 4;        // without o the pairs of four fit the LDS
-template <typename T, bool WHOLE> constexpr int kScanThreads = 64 * (2 * kScanPairs<WHOLE> + (sizeof(T) == 4 ? 0 : 1 + kScanPairs<WHOLE> / 2));
-template <typename T, int DKP, bool OUT, bool KEEP>
-__global__ __launch_bounds__((kScanThreads<T, (OUT || KEEP)>)) void delta_scan_kernel(DeltaParams p, DeltaLayout lay, int nblk, int nwg) {
+template <typename T, int DKP, bool OUT, bool KEEP, int PAIRS>
+__global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(DeltaParams p, DeltaLayout lay, int nblk, int nwg) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
   constexpr bool AHEAD = NP == 1;                // fp32: the fragments of a piece fill the LDS
   constexpr bool MOVE = !OUT && !KEEP;           // what a segment makes of the state, and of any other
-  constexpr int PAIRS = kScanPairs<OUT || KEEP>, IOW = PAIRS / 2;
+  constexpr int IOW = kIoWaves<PAIRS>, IOC = kIoCols<PAIRS>, IOH = IOC * IO_PITCH;
   constexpr int FW = AHEAD ? 1 : 2 * PAIRS;      // waves that fetch
   constexpr int KS = DKP / 32, KSH = KS / 2, NSH = DKP / 32, F = kKFrags<DKP>;
   constexpr int GA = (OUT ? 2 : 1) * NP * F;                         // fragments of (Q and) K by rows: before barrier 1
@@ -314,7 +312,7 @@ __global__ __launch_bounds__((kScanThreads<T, (OUT || KEEP)>)) void delta_scan_k
   constexpr int GB = NP * F + TPF + 1;                               // with K by columns and vec: after it
   constexpr int XF = OUT ? 4 : 2, DF = OUT ? NP : 0;
   constexpr int EX = (2 * XF + 2 + 4 + DF + 1) * FR;                 // halfs of a pair's exchange
-  constexpr int IO = AHEAD ? (OUT ? 3 : 2) * IOW * IO_HALFS : 0;           // v of two pieces, o of one
+  constexpr int IO = AHEAD ? (OUT ? 3 : 2) * IOW * IOH : 0;           // v of two pieces, o of one
   __shared__ __align__(1024) f16 smem[(GA + (AHEAD ? 2 : 1) * GB) * FR + PAIRS * EX + IO];
 
   const int lane = threadIdx.x & 63, w = wave_id(), l16 = lane & 15, g4 = lane >> 4, hf = w & 1;
@@ -328,7 +326,7 @@ __global__ __launch_bounds__((kScanThreads<T, (OUT || KEEP)>)) void delta_scan_k
   const int b = bh / p.heads, h = bh % p.heads, hk = h / (p.heads / p.kheads);
   const int64_t kunit0 = ((int64_t)b * p.kheads + hk) * p.pieces, vunit0 = (int64_t)bh * p.pieces;
   bf16* const sV = reinterpret_cast<bf16*>(smem + (GA + (AHEAD ? 2 : 1) * GB) * FR + PAIRS * EX);
-  bf16* const sO = sV + 2 * IOW * IO_HALFS;
+  bf16* const sO = sV + 2 * IOW * IOH;
 
   const int fw = AHEAD ? 0 : w;
   lds_f16_t* const lds = (lds_f16_t*)smem;
@@ -361,28 +359,28 @@ __global__ __launch_bounds__((kScanThreads<T, (OUT || KEEP)>)) void delta_scan_k
       return;
     }
     if (w > 2 * PAIRS) {
-      const int io = w - 2 * PAIRS - 1, col0 = IO_COLS * (IOW * wg + io), left = unit ? 0 : p.dv - col0;
+      const int io = w - 2 * PAIRS - 1, col0 = IOC * (IOW * wg + io), left = unit ? 0 : p.dv - col0;
       const bf16* vs = reinterpret_cast<const bf16*>(p.v) + b * p.vs.b + h * p.vs.h + col0;
       bf16* os = reinterpret_cast<bf16*>(p.o) + b * p.os.b + h * p.os.h + col0;
-      bf16* const to = sV + io * IO_HALFS;
+      bf16* const to = sV + io * IOH;
       auto run = [&](auto full) {
         constexpr bool FULL = decltype(full)::value;
-        IoRows v, o;
+        IoRows<IOC> v, o;
         auto load_v = [&](int c) {               // tokens beyond the sequence as its last: their gates are zero
           const int t = min(c * DC + lane, p.seqlen - 1);
           v.template load<FULL>(vs + t * p.vs.l, left);
         };
         auto store_o = [&](int c, bool row) {
-          o.from_lds(sO + io * IO_HALFS, lane);
+          o.from_lds(sO + io * IOH, lane);
           o.template store<FULL>(os + (c * DC + lane) * p.os.l, row, left);
         };
         load_v(c0);
-        v.to_lds(to + (c0 & 1) * IOW * IO_HALFS, lane);
+        v.to_lds(to + (c0 & 1) * IOW * IOH, lane);
         load_v(c0 + 1);
         lds_barrier();
         for (int c = c0; c < c1; ++c) {
           lds_barrier();                         // 1
-          v.to_lds(to + ((c + 1) & 1) * IOW * IO_HALFS, lane);
+          v.to_lds(to + ((c + 1) & 1) * IOW * IOH, lane);
           load_v(c + 2);
           if (OUT && c > c0) store_o(c - 1, true);
           lds_barrier();                         // 2
@@ -391,7 +389,7 @@ __global__ __launch_bounds__((kScanThreads<T, (OUT || KEEP)>)) void delta_scan_k
         lds_barrier();                           // the last piece's o is whole
         if (OUT) store_o(c1 - 1, (c1 - 1) * DC + lane < p.seqlen);
       };
-      if (left >= IO_COLS) run(std::true_type{});
+      if (left >= IOC) run(std::true_type{});
       else run(std::false_type{});
       return;
     }
@@ -502,7 +500,7 @@ __global__ __launch_bounds__((kScanThreads<T, (OUT || KEEP)>)) void delta_scan_k
       xr[i] = xRecv[i * 64];
       eg[i] = *reinterpret_cast<const f32x4*>(vec + 32 * hf + 16 * i + 4 * g4);
       if constexpr (AHEAD)
-        vb[i] = *reinterpret_cast<const bf16x4*>(sV + (c & 1) * IOW * IO_HALFS + ((w >> 1) * 16 + l16) * IO_PITCH + 32 * hf + 16 * i + 4 * g4);
+        vb[i] = *reinterpret_cast<const bf16x4*>(sV + (c & 1) * IOW * IOH + ((w >> 1) * 16 + l16) * IO_PITCH + 32 * hf + 16 * i + 4 * g4);
     }
     const f32x4 cs = *reinterpret_cast<const f32x4*>(vec + VEC_GAMMA);                 // gamma, scales of T, P, K
     f16x8 t0[2], t1[2], x0[2], x1[2];            // T on one's own tokens; on the first half's
@@ -735,13 +733,19 @@ __global__ __launch_bounds__(4 * DKP) void delta_segments_kernel(DeltaParams p, 
   }
 }
 
-template <typename T, int DKP, bool OUT, bool KEEP>
-hipError_t launch_scan(const DeltaParams& p, const DeltaLayout& lay, hipStream_t st) {
-  constexpr int PAIRS = kScanPairs<OUT || KEEP>;
+template <typename T, int DKP, bool OUT, bool KEEP, int PAIRS>
+hipError_t launch_scan_of(const DeltaParams& p, const DeltaLayout& lay, hipStream_t st) {
   const int nblk = (p.dv + 15) / 16, nwg = (nblk + PAIRS - 1) / PAIRS + (OUT || KEEP ? 0 : ((p.dk + 15) / 16 + PAIRS - 1) / PAIRS);
   const int parts = p.batch * p.heads * (OUT || KEEP ? lay.segs : lay.segs - 1);
-  delta_scan_kernel<T, DKP, OUT, KEEP><<<head_block_grid(parts, nwg), kScanThreads<T, OUT || KEEP>, 0, st>>>(p, lay, nblk, nwg);
+  delta_scan_kernel<T, DKP, OUT, KEEP, PAIRS><<<head_block_grid(parts, nwg), kDeltaThreads<T, PAIRS>, 0, st>>>(p, lay, nblk, nwg);
   return hipGetLastError();
+}
+template <typename T, int DKP, bool OUT, bool KEEP>
+hipError_t launch_scan(const DeltaParams& p, const DeltaLayout& lay, hipStream_t st) {
+  if constexpr (!OUT && !KEEP) return launch_scan_of<T, DKP, false, false, 4>(p, lay, st);       // without o four pairs fit the LDS
+  else if constexpr (sizeof(T) == 2)
+    if (delta_one_pair(p, lay.segs)) return launch_scan_of<T, DKP, OUT, KEEP, 1>(p, lay, st);
+  return launch_scan_of<T, DKP, OUT, KEEP, (OUT || KEEP ? 2 : 4)>(p, lay, st);
 }
 template <typename T, int DKP>
 hipError_t launch_segments(const DeltaParams& p, const DeltaLayout& lay, hipStream_t st) {
@@ -784,7 +788,6 @@ __global__ void delta_copy_state_kernel(const float* from, float* to, int64_t n)
 // to segment, and the scan with o takes all segments at once.  The segments' number is the one with the least time by this
 // count, in tenths of a piece's time (o and all: 10, without o: 9; a segment's product: 10); a gain of less than a fifth is left.
 int delta_segments(const DeltaParams& p) {
-  constexpr int64_t kCUs = 256;                  // a workgroup fills one
   const int64_t heads = (int64_t)p.batch * p.heads, nblk = (p.dv + 15) / 16, kblk = (p.dk + 15) / 16;
   const int64_t whole = heads * ((nblk + 1) / 2), move = heads * ((nblk + 3) / 4 + (kblk + 3) / 4);
   auto rounds = [](int64_t n) { return (n + kCUs - 1) / kCUs; };
