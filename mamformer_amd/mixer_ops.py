@@ -195,7 +195,7 @@ def gated_delta_rule(q, k, v, g=None, beta=None, *, scale=None, initial_state=No
     A token with beta = 0 and g = 0 changes nothing, which is what padding behind a sequence takes.  A NaN or infinity may
     reach every result of its head from the 64-token piece that holds it on.  With L = 0 the state goes through.
     Differentiable in all tensors: a call that records a gradient keeps the states and systems of its pieces for it, about
-    2.7 KB a token and head of 128 x 128 (bf16); with ``recompute`` it keeps its inputs alone, and the gradients' pass computes
+    3 KB a token and head of 128 x 128 (bf16); with ``recompute`` it keeps its inputs alone, and the gradients' pass computes
     the rest again, a fourth of a training step's time.  The gradients are the same bits.
     """
     name = "gated_delta_rule"
