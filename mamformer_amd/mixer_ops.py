@@ -108,7 +108,8 @@ def rotary(q, k, inv_freq, positions=None, *, offset=0, interleaved=False, scale
     channels the pairs (i, n + i), or with ``interleaved`` (2 i, 2 i + 1), are turned by the angle
     (positions + offset) * inv_freq[i] and multiplied by ``scale``; the others are copied.  ``positions``: int32 or int64
     (L,) or (B, L), None for 0 .. L - 1.  Angles are reduced in 64 bits: far positions cost no precision.
-    ``inverse`` turns back, which with the same ``scale`` is the gradient.  Differentiable in q and k.
+    ``inverse`` turns back, which with the same ``scale`` is the gradient.  Differentiable in q and k (an inv_freq that requires
+    a gradient is refused).
     """
     name = "rotary"
     _require_cuda(name, q, k, inv_freq, positions)
@@ -120,6 +121,8 @@ def rotary(q, k, inv_freq, positions=None, *, offset=0, interleaved=False, scale
     if inv_freq.dim() != 1 or inv_freq.dtype not in (torch.float32, torch.float64) or not 2 <= 2 * len(inv_freq) <= q.shape[3]:
         raise ValueError(f"{name}: inv_freq must be (n,) float32 or float64 with 2 <= 2 n <= {q.shape[3]}, got "
                          f"{tuple(inv_freq.shape)} {inv_freq.dtype}")
+    if inv_freq.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name}: has no gradient for inv_freq; detach it")
     if positions is not None:
         if positions.dtype not in _INDEX_BYTES:
             raise TypeError(f"{name}: positions must be int32 or int64, got {positions.dtype}")
@@ -127,7 +130,7 @@ def rotary(q, k, inv_freq, positions=None, *, offset=0, interleaved=False, scale
             raise ValueError(f"{name}: positions must be (L,) or (B, L), got {tuple(positions.shape)} for q {tuple(q.shape)}")
     cfg = (int(offset), bool(interleaved), float(scale), bool(inverse))
     if _through_autograd(q, k):
-        out = _RotaryFn.apply(q, k, inv_freq.detach(), positions, cfg)
+        out = _RotaryFn.apply(q, k, inv_freq, positions, cfg)
     else:
         out = _rotary(q, k, inv_freq, positions, cfg)
     return out if k is not None else out[0]

@@ -522,7 +522,8 @@ def test_rotary_refusals():
                  lambda: mh.rotary(q, None, torch.ones(5, device="cuda")), lambda: mh.rotary(q, None, f[:0]),
                  lambda: mh.rotary(q, None, f.half()), lambda: mh.rotary(q, None, f, torch.zeros(3, device="cuda")),
                  lambda: mh.rotary(q, None, f, torch.zeros(4, device="cuda", dtype=torch.int64)),
-                 lambda: mh.rotary(q.half(), None, f), lambda: mh.rotary(q, None, f.cpu())):
+                 lambda: mh.rotary(q.half(), None, f), lambda: mh.rotary(q, None, f.cpu()),
+                 lambda: mh.rotary(q, None, f.clone().requires_grad_(True))):
         with pytest.raises((ValueError, TypeError, RuntimeError)):
             call()
 
@@ -678,6 +679,56 @@ def test_group_norm_streams_and_graphs():
             y = mh.group_norm(xl, G, wl, activation="silu")
             return (y.detach(), *torch.autograd.grad(y, (xl, wl), x))
         on_stream_and_captured(step, [x, w])
+
+
+# ------------------------------------------------------------------------------------------------ past 32 bits
+
+def test_large_delta():
+    """Workspaces of more than 4 GiB and results of 2^29 elements: the last sequence's bits are those of it alone, which
+    takes other workgroups."""
+    B, H, HK, L, dk, dv = 16, 32, 16, 8192, 128, 128
+    gen = torch.Generator("cuda").manual_seed(1)
+    q, k = (torch.nn.functional.normalize(torch.randn(B, HK, L, dk, device="cuda", generator=gen), dim=-1).to(BF) for _ in range(2))
+    v, do = (torch.randn(B, H, L, dv, device="cuda", generator=gen, dtype=BF) for _ in range(2))
+    g, beta = -torch.rand(B, H, L, device="cuda", generator=gen), torch.rand(B, H, L, device="cuda", generator=gen)
+    say("delta with more than 4 GiB of workspace")
+    o, s = mh.gated_delta_rule(q, k, v, g, beta, return_final_state=True)
+    last = [a[-1:] for a in (q, k, v, g, beta)]
+    o1, s1 = mh.gated_delta_rule(*last, return_final_state=True)
+    assert torch.equal(o[-1:], o1) and torch.equal(s[-1:], s1)
+    grads = mh.gated_delta_rule_bwd(do, q, k, v, g, beta)
+    for a, b in zip(grads[:5], mh.gated_delta_rule_bwd(do[-1:], *last)[:5]):
+        assert torch.equal(a[-1:], b)
+
+
+def test_large_step():
+    B, H = 4097, 32
+    state = torch.randn(B, H, 128, 128, device="cuda")
+    q, k, v = (torch.randn(B, H, 128, device="cuda", dtype=BF) for _ in range(3))
+    say("step of 2^31 state elements")
+    tail, out = state[-2:].clone(), mh.gated_delta_step(state, q, k, v)
+    assert torch.equal(out[-2:], mh.gated_delta_step(tail, q[-2:], k[-2:], v[-2:])) and torch.equal(state[-2:], tail)
+
+
+def test_large_rotary_and_norm():
+    n = (1 << 24) + 5
+    x = torch.randn(1, 1, n, 128, device="cuda", dtype=BF)
+    f, _ = mh.rotary_frequencies(128)
+    say("rotary of 2^31 elements")
+    y = mh.rotary(x, None, f)
+    assert torch.equal(y[:, :, -9:], mh.rotary(x[:, :, -9:], None, f, offset=n - 9))
+    for x in (x.view(n, 128), x.view(1, n, 128)):
+        say(f"group norm of {tuple(x.shape)}")
+        y, st = mh.group_norm(x, 4, return_stats=True)
+        dx, _, db = mh.group_norm_bwd(x, x, st, 4, dtype=F32)
+        if x.dim() == 2:
+            y1, st1 = mh.group_norm(x[-9:], 4, return_stats=True)
+            assert torch.equal(y[-9:], y1) and torch.equal(dx[-9:], mh.group_norm_bwd(x[-9:], x[-9:], st1, 4)[0])
+        else:
+            m, r = st[0, :, 0].repeat_interleave(32), st[0, :, 1].repeat_interleave(32)
+            want = (x[0, -9:].float() - m) * r
+            assert (y[0, -9:].float() - want).abs().max() <= 2.0 ** -8 * want.abs().max()
+        assert torch.isfinite(db).all()
 
 
 # ------------------------------------------------------------------------------------------------ together
