@@ -113,12 +113,13 @@ def rotary(q, k, inv_freq, positions=None, *, offset=0, interleaved=False, scale
     """
     name = "rotary"
     _require_cuda(name, q, k, inv_freq, positions)
-    if q.dim() != 4 or k is not None and (k.dim() != 4 or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:]
+    qs, ks = q.shape, None if k is None else k.shape
+    if len(qs) != 4 or k is not None and (len(ks) != 4 or ks[0] != qs[0] or ks[2] != qs[2] or ks[3] != qs[3]
                                           or k.dtype is not q.dtype):
         raise ValueError(f"{name}: q and k must be (B, H, L, D) and (B, HK, L, D) of one dtype, got {tuple(q.shape)} and "
                          f"{None if k is None else tuple(k.shape)}")
     _dtype(name, "q", q)
-    if inv_freq.dim() != 1 or inv_freq.dtype not in (torch.float32, torch.float64) or not 2 <= 2 * len(inv_freq) <= q.shape[3]:
+    if inv_freq.dim() != 1 or inv_freq.dtype not in (torch.float32, torch.float64) or not 2 <= 2 * inv_freq.shape[0] <= qs[3]:
         raise ValueError(f"{name}: inv_freq must be (n,) float32 or float64 with 2 <= 2 n <= {q.shape[3]}, got "
                          f"{tuple(inv_freq.shape)} {inv_freq.dtype}")
     if inv_freq.requires_grad and torch.is_grad_enabled():
@@ -126,7 +127,7 @@ def rotary(q, k, inv_freq, positions=None, *, offset=0, interleaved=False, scale
     if positions is not None:
         if positions.dtype not in _INDEX_BYTES:
             raise TypeError(f"{name}: positions must be int32 or int64, got {positions.dtype}")
-        if positions.shape not in ((q.shape[2],), (q.shape[0], q.shape[2])):
+        if positions.shape not in ((qs[2],), (qs[0], qs[2])):
             raise ValueError(f"{name}: positions must be (L,) or (B, L), got {tuple(positions.shape)} for q {tuple(q.shape)}")
     cfg = (int(offset), bool(interleaved), float(scale), bool(inverse))
     if _through_autograd(q, k):
@@ -150,9 +151,14 @@ def _rotary(q, k, inv_freq, positions, cfg):
     if k is not None:
         k = _channels(k)
         ko, HK = torch.empty_like(k), k.shape[1]
+    (qb, qh, ql, _), (ob, oh, ol, _) = q.stride(), qo.stride()
     a = RotaryArgs(B, H, HK, L, D, inv_freq.shape[0], _DT[q.dtype], interleaved, inverse, inv_freq.dtype is torch.float64,
-                   0 if positions is None else positions.element_size(), scale, inv_freq.data_ptr(), _ptr(positions), pos_sb,
-                   offset, *_strides3(q), *_strides3(k if HK else None), *_strides3(qo), *_strides3(ko if HK else None))
+                   0 if positions is None else _INDEX_BYTES[positions.dtype], scale, inv_freq.data_ptr(), _ptr(positions), pos_sb,
+                   offset, q.data_ptr(), qb, qh, ql)
+    a.q_out, a.q_out_stride_b, a.q_out_stride_h, a.q_out_stride_l = qo.data_ptr(), ob, oh, ol
+    if HK:
+        a.k, a.k_stride_b, a.k_stride_h, a.k_stride_l = _strides3(k)
+        a.k_out, a.k_out_stride_b, a.k_out_stride_h, a.k_out_stride_l = _strides3(ko)
     if H:
         _lib.call("mh_rotary", ct.byref(a), _stream(q.device))
     return qo, ko
@@ -213,18 +219,20 @@ def gated_delta_rule(q, k, v, g=None, beta=None, *, scale=None, initial_state=No
 
 
 def _delta_shapes(name, q, k, v, g, beta, state, dims):
-    if q.dim() != dims or v.dim() != dims or q.shape != k.shape or q.shape[0] != v.shape[0] or q.shape[2:-1] != v.shape[2:-1]:
+    qs, vs = q.shape, v.shape
+    if len(qs) != dims or len(vs) != dims or qs != k.shape or qs[0] != vs[0] or dims == 4 and qs[2] != vs[2]:
         t = ", L" if dims == 4 else ""
         raise ValueError(f"{name}: q and k must be (B, HK{t}, dk) and v (B, H{t}, dv), got {tuple(q.shape)}, "
                          f"{tuple(k.shape)} and {tuple(v.shape)}")
     _dtype(name, "q", q)
     if k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise TypeError(f"{name}: q, k and v must have one dtype, got {q.dtype}, {k.dtype} and {v.dtype}")
+    gates = vs[:-1]
     for what, t in (("g", g), ("beta", beta)):
-        if t is not None and (t.shape != v.shape[:-1] or t.dtype not in _DT):
-            raise ValueError(f"{name}: {what} must be {tuple(v.shape[:-1])} float32 or bfloat16, got {tuple(t.shape)} {t.dtype}")
+        if t is not None and (t.shape != gates or t.dtype not in _DT):
+            raise ValueError(f"{name}: {what} must be {tuple(gates)} float32 or bfloat16, got {tuple(t.shape)} {t.dtype}")
     if state is not None:
-        _like(name, "state" if dims == 3 else "initial_state", state, (*v.shape[:2], q.shape[-1], v.shape[-1]), torch.float32)
+        _like(name, "state" if dims == 3 else "initial_state", state, (vs[0], vs[1], qs[-1], vs[-1]), torch.float32)
 
 
 def _delta_args(q, k, v, g, beta, state, scale):
@@ -327,10 +335,11 @@ def gated_delta_step(state, q, k, v, g=None, beta=None, *, scale=None, state_out
         raise RuntimeError(f"{name}: has no backward; call it under torch.no_grad(), or gated_delta_rule with L = 1")
     q, k, v, g, beta = _channels(q), _channels(k), _channels(v), _f32(g), _f32(beta)
     o = torch.empty_like(v)
-    (B, HK, dk), (H, dv) = q.shape, v.shape[1:]
-    a = DeltaStepArgs(B, H, HK, dk, dv, _DT[q.dtype], q.shape[-1] ** -0.5 if scale is None else scale, *_strides2(q),
-                      *_strides2(k), *_strides2(v), *_strides2(g), *_strides2(beta), state.data_ptr(), state_out.data_ptr(),
-                      *_strides2(o))
+    (B, HK, dk), (_, H, dv) = q.shape, v.shape
+    (qb, qh, _), (kb, kh, _), (vb, vh, _), (ob, oh, _) = q.stride(), k.stride(), v.stride(), o.stride()
+    a = DeltaStepArgs(B, H, HK, dk, dv, _DT[q.dtype], dk ** -0.5 if scale is None else scale, q.data_ptr(), qb, qh,
+                      k.data_ptr(), kb, kh, v.data_ptr(), vb, vh, *_strides2(g), *_strides2(beta), state.data_ptr(),
+                      state_out.data_ptr(), o.data_ptr(), ob, oh)
     _lib.call("mh_delta_step", ct.byref(a), _stream(v.device))
     torch.autograd.graph.increment_version(state_out)    # the kernel writes where torch does not see it
     return o

@@ -123,12 +123,13 @@ def _require_cuda(name, *ts):
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise RuntimeError(f"{name}: HIP op needs device tensors (got {t.device}); no CPU path exists")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RuntimeError(f"{name}: tensors on different devices {({u.device for u in ts if u is not None})}")
+        i = t.get_device()                       # no device object for each tensor
+        if i != dev:
+            if not t.is_cuda:
+                raise RuntimeError(f"{name}: HIP op needs device tensors (got {t.device}); no CPU path exists")
+            if dev is not None:
+                raise RuntimeError(f"{name}: tensors on different devices {({u.device for u in ts if u is not None})}")
+            dev = i
 
 
 def _f32c(t: Optional[torch.Tensor]):
