@@ -250,7 +250,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void delta_prep_kernel
         put_frag(out, t_frag(w, s), lane, th[s]);
         put_frag(out, kTFrags + t_frag(w, s), lane, tl[s]);
         put_frag(out, 2 * kTFrags + t_frag(w, s), lane, ph[s]);
-        put_frag(out, 3 * kTFrags + t_frag(w, s), lane, pl[s]);
+        if constexpr (NP == 2) put_frag(out, 3 * kTFrags + t_frag(w, s), lane, pl[s]);
       }
     if (backward) {                              // by columns: through LDS, as T^T and P^T (row j, column t)
 #pragma unroll
@@ -269,8 +269,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void delta_prep_kernel
 #pragma unroll
         for (int s = 0; s < 2; ++s)
           if (w < 2 + 2 * s) {
-            put_frag(out, (4 + n) * kTFrags + tt_frag(w, s), lane, row_frag16<64>(tiles + n * TC::ELEMS, 16 * w, 32 * s, lane));
-            put_frag(out, (6 + n) * kTFrags + tt_frag(w, s), lane, row_frag16<64>(tiles + (2 + n) * TC::ELEMS, 16 * w, 32 * s, lane));
+            put_frag(out, (2 + NP + n) * kTFrags + tt_frag(w, s), lane, row_frag16<64>(tiles + n * TC::ELEMS, 16 * w, 32 * s, lane));
+            put_frag(out, (4 + NP + n) * kTFrags + tt_frag(w, s), lane, row_frag16<64>(tiles + (2 + n) * TC::ELEMS, 16 * w, 32 * s, lane));
           }
     }
     float* vec = reinterpret_cast<float*>(p.workspace + lay.vec) + vunit * kVecFloats;
@@ -311,7 +311,7 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
   constexpr int FW = AHEAD ? 1 : 2 * PAIRS;      // waves that fetch
   constexpr int KS = DKP / 32, KSH = KS / 2, NSH = DKP / 32, F = kKFrags<DKP>;
   constexpr int GA = (OUT ? 2 : 1) * NP * F;                         // fragments of (Q and) K by rows: before barrier 1
-  constexpr int TPF = OUT ? 4 * kTFrags : 2 * kTFrags;               // of T (and P)
+  constexpr int TPF = (OUT ? 2 + NP : 2) * kTFrags;                  // of T (and P)
   constexpr int GB = NP * F + TPF + 1;                               // with K by columns and vec: after it
   constexpr int XF = OUT ? 4 : 2, DF = OUT ? NP : 0;
   constexpr int EX = (2 * XF + 2 + 4 + DF + 1) * FR;                 // halfs of a pair's exchange
