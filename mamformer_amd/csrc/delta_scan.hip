@@ -334,27 +334,37 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
   const int fw = AHEAD ? 0 : w;
   lds_f16_t* const lds = (lds_f16_t*)smem;
   auto fetch_a = [&](int c) { fetch_share<GA, FW>(lds, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + (OUT ? 0 : NP * F * 1024), fw, lane); };
-  auto fetch_b = [&](int c) {
-    lds_f16_t* to = lds + (GA + (AHEAD ? (c & 1) * GB : 0)) * FR;
+  constexpr int GB1 = NP * F + 1, GB2 = TPF;
+  auto b_of = [&](int c) { return lds + (GA + (AHEAD ? (c & 1) * GB : 0)) * FR; };
+  auto fetch_b2 = [&](int c) {
+    if (FW < 8 || fw < 4) fetch_share<TPF, (FW < 4 ? FW : 4)>(b_of(c) + NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit, fw, lane);
+  };
+  auto fetch_b1 = [&](int c) {
+    lds_f16_t* to = b_of(c);
     fetch_share<NP * F, FW>(to, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + 2 * NP * F * 1024, fw, lane);
-    if (FW < 8 || fw < 4) fetch_share<TPF, (FW < 4 ? FW : 4)>(to + NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit, fw, lane);
     if (fw == 0) fetch_share<1, 1>(to + (NP * F + TPF) * FR, p.workspace + lay.vec + (vunit0 + c) * (int64_t)(kVecFloats * 4), 0, lane);
   };
   if constexpr (AHEAD) {
     if (w == 2 * PAIRS) {
       fetch_a(c0);
-      fetch_b(c0);
+      fetch_b1(c0);
+      fetch_b2(c0);
       wait_vmem_n<GB>();
       lds_barrier();
-      for (int c = c0; c < c1; ++c) {
+      for (int c = c0; c < c1; ++c) {            // the next piece's, each where what was there has been read
         const bool more = c + 1 < c1;
-        wait_vmem();                             // T, P and K by columns of this piece
+        if (more) {
+          fetch_b1(c + 1);
+          wait_vmem_n<GB1>();                    // T, P and K by columns of this piece
+        } else {
+          wait_vmem();
+        }
         lds_barrier();                           // 1
-        if (more) fetch_a(c + 1);                // where the last ones have been read
+        if (more) fetch_a(c + 1);
         lds_barrier();                           // 2
         if (more) {
-          fetch_b(c + 1);
-          wait_vmem_n<GB>();
+          fetch_b2(c + 1);
+          wait_vmem_n<GB2>();                    // K and Q by rows of the next piece
         }
         lds_barrier();                           // 3
       }
@@ -447,7 +457,8 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
     if (!AHEAD) {
       lds_barrier();
       fetch_a(c);
-      fetch_b(c);
+      fetch_b1(c);
+      fetch_b2(c);
       wait_vmem();
       lds_barrier();
       load_a();
