@@ -239,6 +239,33 @@ __device__ __forceinline__ void fetch_share(lds_f16_t* to, const char* from, int
     __builtin_amdgcn_global_load_lds((glb_void_t*)(src + i * 1024 + off), (lds_void_t*)(dst + i * FR), 16, 0, 0);
 }
 
+// Lines of a later piece's fragments, read so that the L2 holds them when the waves that fetch ask: `wg` of `nwg` workgroups
+// that want the same takes its share of A + B + 1 KB in blocks of 8 KB, a line a lane.  With a pair a workgroup, eight of
+// which share 128 columns, that takes the scan from 201 to 175 us (b 2, H 16, L 4096); with two pairs, whose share is twice as
+// large and whose fetching waves are as busy, it cost 5 of 86 (b 4, H 16, L 2048), so that those go without.
+struct Warm {
+  static constexpr int N = 5;
+  uint32_t x[N];
+  template <int A, int B>
+  __device__ __forceinline__ void load(const char* a, const char* b, const char* c, int wg, int nwg, int lane) {
+    constexpr int NA = (A + 7) / 8, NB = (B + 7) / 8;
+    asm volatile("" : "+v"(lane));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int j = wg + nwg * i;
+      x[i] = 0;
+      if (j >= NA + NB + 1) continue;
+      const char* from = j < NA ? a + j * 8192 : j < NA + NB ? b + (j - NA) * 8192 : c;
+      const int lines = j < NA ? 8 * A - 64 * j : j < NA + NB ? 8 * B - 64 * (j - NA) : 8;
+      x[i] = *reinterpret_cast<const uint32_t*>(from + 128u * min(lane, lines - 1));
+    }
+  }
+  __device__ __forceinline__ void done() const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" ::"v"(x[i]));
+  }
+};
+
 // 32 rows of 16 columns in the accumulators' order: v[i] is row 16 (i / 4) + 4 g + i % 4 of column l % 16.  `at` is the
 // first row at the first column; rows beyond `len` read the last one, or row 0 (their gates are zero), columns beyond the
 // last one as 0.  A row's address is the wave's, one offset the lane's.
