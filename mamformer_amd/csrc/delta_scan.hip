@@ -717,8 +717,8 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
 
 // The states that the segments begin with, S_{s+1} = M_s S_s + N_s, where the scan has left N_s (segment 0: S_1 itself) and
 // M_s: a workgroup takes 16 columns from segment to segment, a wave 16 rows of them by fp32 matrix instructions.  M_s does
-// not wait for a state: that of the next segment is under way during the product (8 heads of 128 x 128, 8 segments: 55 us
-// with the rows a thread each and M read where it is used, now 33).
+// not wait for a state: those of the next two segments are under way (8 heads of 128 x 128, 8 segments: 55 us with the rows
+// a thread each and M read where it is used, 33 with one segment under way, now 24).
 template <int DKP>
 __global__ __launch_bounds__(4 * DKP) void delta_segments_kernel(DeltaParams p, DeltaLayout lay) {
   __shared__ float sS[2][DKP][16];
@@ -734,30 +734,35 @@ __global__ __launch_bounds__(4 * DKP) void delta_segments_kernel(DeltaParams p, 
     for (int r = 0; r < 4; ++r) v[r] = s < lay.segs - 1 && col < p.dv && row0 + r < p.dk ? at[s * states + r * p.dv] : 0.f;
     return v;
   };
-  float m[DKP / 4];                              // k = 4 i + g4
-  auto load_m = [&](int s) {
+  float m[2][DKP / 4];                           // k = 4 i + g4; of this segment and the next
+  f32x4 N[2], S = state_of(0);
+  auto load = [&](int s, int x) {
 #pragma unroll
-    for (int i = 0; i < DKP / 4; ++i) m[i] = s < lay.segs - 1 && 4 * i + g4 < p.dk ? M[(int64_t)s * DKP * DKP + 4 * i * DKP] : 0.f;
+    for (int i = 0; i < DKP / 4; ++i) m[x][i] = s < lay.segs - 1 && 4 * i + g4 < p.dk ? M[(int64_t)s * DKP * DKP + 4 * i * DKP] : 0.f;
+    N[x] = state_of(s);
   };
-  f32x4 S = state_of(0), N = state_of(1);
-  load_m(1);
-  for (int s = 1; s < lay.segs - 1; ++s) {
-    float(*t)[16] = sS[s & 1];
+  auto step = [&](int s, int x) {
+    float(*t)[16] = sS[x];
 #pragma unroll
     for (int r = 0; r < 4; ++r) t[row0 + r][l16] = S[r];
     __syncthreads();
     float b[DKP / 4];
 #pragma unroll
     for (int i = 0; i < DKP / 4; ++i) b[i] = t[4 * i + g4][l16];
-    f32x4 acc[2] = {N, {}};
+    f32x4 acc[2] = {N[x], {}};
 #pragma unroll
-    for (int i = 0; i < DKP / 4; ++i) acc[i & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[i], b[i], acc[i & 1], 0, 0, 0);
-    load_m(s + 1);
-    N = state_of(s + 1);
+    for (int i = 0; i < DKP / 4; ++i) acc[i & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[x][i], b[i], acc[i & 1], 0, 0, 0);
     S = acc[0] + acc[1];
+    load(s + 2, x);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       if (col < p.dv && row0 + r < p.dk) at[s * states + r * p.dv] = S[r];
+  };
+  load(1, 0);
+  load(2, 1);
+  for (int s = 1; s < lay.segs - 1; s += 2) {
+    step(s, 0);
+    if (s + 1 < lay.segs - 1) step(s + 1, 1);
   }
 }
 
