@@ -13,7 +13,7 @@
 //   A' and P' themselves, in fp32.
 // What it reads of the forward, the pieces' systems, entering states and corrections, a forward kept for it (3 KB a token
 // and head of 128 x 128 in bf16, six times q, k and v) or is computed again, which at b 2, H 16 over 8, L 4096 (bf16) takes
-// 220 us beside the 405 of the two kernels here.
+// 190 us beside the 410 of the two kernels here.
 #include "delta.h"
 
 namespace mh {
@@ -22,7 +22,7 @@ namespace {
 // Two waves hold the gradient of 16 columns of the state as the forward's scan holds the state: half of its rows and half of
 // a piece's tokens each, and (bf16) a wave fetches the fragments and another dO.  y = T^T ddelta is upper triangular, so
 // that here the first wave needs the second one's ddelta.  Bound by a piece's latency as that scan is: 3.0 us for each of
-// the 64 pieces of L 4096 (b 2, H 16, 128 x 128: 192 us; with two pairs a workgroup and half of the CUs idle 226).
+// the 64 pieces of L 4096 (b 2, H 16, 128 x 128: 195 us; with two pairs a workgroup and half of the CUs idle 226).
 template <typename T, int DKP, int PAIRS>
 __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_back_scan_kernel(DeltaBwdParams q, DeltaLayout lay, DeltaScratch scr, int nblk, int nwg) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;

@@ -205,7 +205,7 @@ def gated_delta_rule(q, k, v, g=None, beta=None, *, scale=None, initial_state=No
     reach every result of its head from the 64-token piece that holds it on.  With L = 0 the state goes through.
     Differentiable in all tensors: a call that records a gradient keeps the states and systems of its pieces for it, about
     3 KB a token and head of 128 x 128 (bf16); with ``recompute`` it keeps its inputs alone, and the gradients' pass computes
-    the rest again, a fourth of a training step's time.  The gradients are the same bits.
+    the rest again (a third more time for a training step).  The gradients are the same bits.
     """
     name = "gated_delta_rule"
     _require_cuda(name, q, k, v, g, beta, initial_state)
