@@ -289,7 +289,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void delta_prep_kernel
 // ------------------------------------------------------------------ the state from piece to piece
 // Two waves hold 16 columns of the state, half of its rows each (fp32), and half of a piece's tokens; a workgroup has two
 // such pairs, which read the same fragments, or one where the pairs are no more than the CUs (b 2, H 16, L 4096, o and what
-// a backward keeps: 204 us against 224 when it was chosen, 175 now), or four for a segment without o, whose exchange takes less LDS.  For a piece:
+// a backward keeps: 204 us against 224 when it was chosen, 168 now), or four for a segment without o, whose exchange takes
+// less LDS.  For a piece:
 //   each wave multiplies K (and Q) by its rows of S and gives the other its part of the other's tokens;   [barrier 1]
 //   R = V - e^G K S of its tokens; T is lower triangular, so that the second wave needs the first one's R;  [barrier 2]
 //   U = beta e^{G_end - G} delta of its tokens goes to the other, each adds K^T U to its rows.              [barrier 3]
@@ -300,8 +301,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void delta_prep_kernel
 //
 // Bound by the latency of one piece on waves that have a SIMD to themselves, most of it the conversions (an instruction of
 // 4 cycles for each value and part): 2.7 us a piece (b 4, H 16, L 2048, 128 x 128: 86 us; b 2, H 16, L 4096 with what a
-// backward keeps 175).  About a sixth of it is the wait for the next piece's K and Q at barrier 3.  Operands that no other wave has to finish first are read from LDS right behind a barrier, ahead of what they
-// are needed for.
+// backward keeps 168).  With two pairs about a sixth of it is the wait for the next piece's K and Q at barrier 3.  Operands
+// that no other wave has to finish first are read from LDS right behind a barrier, ahead of what they are needed for.
 template <typename T, int DKP, bool OUT, bool KEEP, int PAIRS>
 __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(DeltaParams p, DeltaLayout lay, int nblk, int nwg) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
@@ -316,7 +317,8 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
   constexpr int XF = OUT ? 4 : 2, DF = OUT ? NP : 0;
   constexpr int EX = (2 * XF + 2 + 4 + DF + 1) * FR;                 // halfs of a pair's exchange
   constexpr int IO = AHEAD ? (OUT ? 3 : 2) * IOW * IOH : 0;           // v of two pieces, o of one
-  __shared__ __align__(1024) f16 smem[(GA + (AHEAD ? 2 : 1) * GB) * FR + PAIRS * EX + IO];
+  constexpr int AB = AHEAD && PAIRS == 1 ? 2 : 1;                    // pieces of which K and Q by rows have room (175 -> 168 us)
+  __shared__ __align__(1024) f16 smem[(AB * GA + (AHEAD ? 2 : 1) * GB) * FR + PAIRS * EX + IO];
 
   const int lane = threadIdx.x & 63, w = wave_id(), l16 = lane & 15, g4 = lane >> 4, hf = w & 1;
   int part, wg;
@@ -328,16 +330,16 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
   if (unit && seg == 0) return;                  // its state is known
   const int b = bh / p.heads, h = bh % p.heads, hk = h / (p.heads / p.kheads);
   const int64_t kunit0 = ((int64_t)b * p.kheads + hk) * p.pieces, vunit0 = (int64_t)bh * p.pieces;
-  bf16* const sV = reinterpret_cast<bf16*>(smem + (GA + (AHEAD ? 2 : 1) * GB) * FR + PAIRS * EX);
+  bf16* const sV = reinterpret_cast<bf16*>(smem + (AB * GA + (AHEAD ? 2 : 1) * GB) * FR + PAIRS * EX);
   bf16* const sO = sV + 2 * IOW * IOH;
 
   const int fw = AHEAD ? 0 : w;
   lds_f16_t* const lds = (lds_f16_t*)smem;
-  auto fetch_a = [&](int c) { fetch_share<GA, FW>(lds, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + (OUT ? 0 : NP * F * 1024), fw, lane); };
+  auto fetch_a = [&](int c) { fetch_share<GA, FW>(lds + (AB == 2 ? (c & 1) * GA * FR : 0), p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + (OUT ? 0 : NP * F * 1024), fw, lane); };
   // The second kind in two parts: K by columns at the top of a piece, T and P behind its barrier 2, so that the next piece's
   // first kind, which has to have landed by barrier 3, waits for less (one part: 89 us against 86 at b 4, H 16, L 2048).
   constexpr int GB1 = NP * F + 1, GB2 = TPF;
-  auto b_of = [&](int c) { return lds + (GA + (AHEAD ? (c & 1) * GB : 0)) * FR; };
+  auto b_of = [&](int c) { return lds + (AB * GA + (AHEAD ? (c & 1) * GB : 0)) * FR; };
   auto fetch_b2 = [&](int c) {
     if (FW < 8 || fw < 4) fetch_share<TPF, (FW < 4 ? FW : 4)>(b_of(c) + NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit, fw, lane);
   };
@@ -356,17 +358,18 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
       for (int c = c0; c < c1; ++c) {            // the next piece's, each where what was there has been read
         const bool more = c + 1 < c1;
         if (more) {
+          if (AB == 2) fetch_a(c + 1);
           fetch_b1(c + 1);
-          wait_vmem_n<GB1>();                    // T, P and K by columns of this piece
+          wait_vmem_n<(AB == 2 ? GA : 0) + GB1>();                     // T, P and K by columns of this piece
         } else {
           wait_vmem();
         }
         lds_barrier();                           // 1
-        if (more) fetch_a(c + 1);
+        if (AB == 1 && more) fetch_a(c + 1);
         lds_barrier();                           // 2
         if (more) {
           fetch_b2(c + 1);
-          wait_vmem_n<GB2>();                    // K and Q by rows of the next piece
+          wait_vmem_n<(AB == 2 ? GB1 : 0) + GB2>();                    // K and Q by rows of the next piece
         }
         lds_barrier();                           // 3
       }
@@ -423,7 +426,7 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
   }
   const int blk = PAIRS * (unit ? wg - nv : wg) + (w >> 1), col = 16 * blk + l16, cols = unit ? p.dk : p.dv;
   const bool live = 16 * blk < cols, cv = col < cols;                // a pair beyond the last columns has zeros
-  f16* ex = smem + (GA + (AHEAD ? 2 : 1) * GB) * FR + (w >> 1) * EX;
+  f16* ex = smem + (AB * GA + (AHEAD ? 2 : 1) * GB) * FR + (w >> 1) * EX;
   f32x4* const xSend = reinterpret_cast<f32x4*>(ex) + hf * XF * 64 + lane;             // X (and Y) of the other's tokens
   const f32x4* const xRecv = reinterpret_cast<const f32x4*>(ex) + (1 - hf) * XF * 64 + lane;
   f16* const eR = ex + 2 * XF * FR;                                                    // the first half's R
@@ -452,20 +455,21 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
   if (AHEAD) lds_barrier();
   else load_v(c0);
 
-  const f16 *Qr = smem, *Kr = smem + (OUT ? NP * F * FR : 0);
+  const f16 *Qr = smem, *Kr = smem + (OUT ? NP * F * FR : 0);        // AB == 1: of the one piece there is
   f16x8 ka[KSH][4], qa[OUT ? KSH : 1][4];        // the next piece's; tiles 0, 1: one's own tokens, 2, 3: the other's
-  auto load_a = [&]() {
+  auto load_a = [&](int c) {
+    const int at = AB == 2 ? (c & 1) * GA : 0;
 #pragma unroll
     for (int s = 0; s < KSH; ++s)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) ka[s][i] = frag(Kr, ((2 * hf + i) & 3) * KS + hf * KSH + s, lane);
+      for (int i = 0; i < 4; ++i) ka[s][i] = frag(Kr, at + ((2 * hf + i) & 3) * KS + hf * KSH + s, lane);
     if constexpr (OUT)
 #pragma unroll
       for (int s = 0; s < KSH; ++s)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) qa[s][i] = frag(Qr, ((2 * hf + i) & 3) * KS + hf * KSH + s, lane);
+        for (int i = 0; i < 4; ++i) qa[s][i] = frag(Qr, at + ((2 * hf + i) & 3) * KS + hf * KSH + s, lane);
   };
-  if (AHEAD) load_a();
+  if (AHEAD) load_a(c0);
 
   for (int c = c0; c < c1; ++c) {
     if (!AHEAD) {
@@ -475,9 +479,9 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
       fetch_b2(c);
       wait_vmem();
       lds_barrier();
-      load_a();
+      load_a(c);
     }
-    const f16 *Kc = smem + (GA + (AHEAD ? (c & 1) * GB : 0)) * FR, *Tt = Kc + NP * F * FR, *Pt = Tt + 2 * kTFrags * FR;
+    const f16 *Kc = smem + (AB * GA + (AHEAD ? (c & 1) * GB : 0)) * FR, *Tt = Kc + NP * F * FR, *Pt = Tt + 2 * kTFrags * FR;
     const float* vec = reinterpret_cast<const float*>(Tt + TPF * FR);
     f16x8 sh[KSH], sl[KSH];
     f32x4 X[4] = {}, Y[4] = {};
@@ -636,7 +640,7 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
       if constexpr (NP == 2) d1 = frag(eD, 1, lane);
       od = eS[64 + lane];
     }
-    if (AHEAD && c + 1 < c1) load_a();
+    if (AHEAD && c + 1 < c1) load_a(c + 1);
     __builtin_amdgcn_sched_barrier(0);
     f32x4 u0[NSH] = {}, u1[NSH] = {};
 #pragma unroll
