@@ -335,7 +335,7 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_back_scan_ker
 #pragma unroll
     for (int n = 0; n < NSH; ++n)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) dS[n][r] = cs[0] * dS[n][r] + su.inv * u0[n][r] + other * u1[n][r];
+      for (int r = 0; r < 4; ++r) dS[n][r] = __builtin_fmaf(other, u1[n][r], __builtin_fmaf(su.inv, u0[n][r], cs[0] * dS[n][r]));
     if (live) {
       const Scale sy(col_max(abs_max(Yv)));
       parts_of<2>(Yv, sy.mult, yh, yl);
@@ -373,7 +373,7 @@ __device__ __forceinline__ void put_halves(f16* t, int r, int c, f16x8 v) {
 // that order).  Waves w and w + 4 hold rows 16 w .. 16 w + 15: of the three products with the states (64 x dk) half of the
 // channels each, of A' and P' every other tile (four waves with all of it spilled 150 registers: 407 us against 300 when
 // this was split).  The columns of v pass through LDS DVB at a time, every matrix brought to one scale on the way (its
-// columns have their own), a stage's loads under way during the one before.  Now 213 us at b 2, H 16 over 8, L 4096: 400 MB
+// columns have their own), a stage's loads under way during the one before.  Now 215 us at b 2, H 16 over 8, L 4096: 400 MB
 // of states, corrections and their gradients, which at a copy's rate take 70; one workgroup fits a CU, so that nothing
 // covers its barriers, and stages of 64 columns (fewer barriers) took 252.
 template <typename T, int DKP>
