@@ -150,8 +150,8 @@ __device__ __forceinline__ float exp_of(double x) { return __builtin_amdgcn_exp2
 // are read by 16 bytes a lane without conflicts, and the scans need no transposing reads.
 //   For each (batch, key head, piece), NP parts of each: Q by rows (i KS + s: rows 16 i .., k-step s), K by rows, K by
 //     columns (2 n + s: channels 16 n .., tokens 32 s ..), and for the backward Q by columns.
-//   For each (batch, value head, piece): T by rows in two parts (its 6 fragments that are not zero), P by rows (bf16: its
-//     first part), then for the backward T and P by columns in two parts each.
+//   For each (batch, value head, piece): T by rows in two parts (its 6 fragments that are not zero), P by rows in two parts,
+//     then for the backward T and P by columns in two parts each.
 //   `vec` for the same: e^{G_t}, beta_t e^{G_end - G_t}, then e^{G_end} and the scales of T, P, K and Q.
 //   For the backward, for each (batch, value head, piece, 16 columns of v): the entering state and delta, two parts each,
 //     in the order in which waves hold them as operands ([part][k-step]), and the scales of their columns in either half
@@ -199,7 +199,7 @@ struct DeltaLayout {
     const size_t kpieces = (size_t)p.batch * p.kheads * p.pieces, pieces = (size_t)p.batch * p.heads * p.pieces;
     const size_t blocks = backward ? pieces * ((p.dv + 15) / 16) : 0;
     kq_unit = (backward ? 4 : 3) * np * (dkp / 8) * FR * 2;
-    tp_unit = ((backward ? 6 : 2) + np) * kTFrags * FR * 2;
+    tp_unit = (backward ? 8 : 4) * kTFrags * FR * 2;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t was = at; at += (bytes + 1023) / 1024 * 1024; return was; };
     kq = take(kpieces * kq_unit);

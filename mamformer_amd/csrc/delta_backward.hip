@@ -47,12 +47,12 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_back_scan_ker
   lds_f16_t* const lds = (lds_f16_t*)smem;
   auto fetch_a = [&](int c) {
     fetch_share<NP * F, FW>(lds, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + NP * F * 1024, fw, lane);
-    fetch_share<2 * kTFrags, FW>(lds + NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit + (4 + NP) * kTFrags * 1024, fw, lane);
+    fetch_share<2 * kTFrags, FW>(lds + NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit + 6 * kTFrags * 1024, fw, lane);
   };
   auto fetch_b = [&](int c) {
     lds_f16_t* to = lds + (GA + (AHEAD ? (c & 1) * GB : 0)) * FR;
     fetch_share<2 * NP * F, FW>(to, p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + 2 * NP * F * 1024, fw, lane);
-    fetch_share<2 * kTFrags, FW>(to + 2 * NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit + (2 + NP) * kTFrags * 1024, fw, lane);
+    fetch_share<2 * kTFrags, FW>(to + 2 * NP * F * FR, p.workspace + lay.tp + (vunit0 + c) * lay.tp_unit + 4 * kTFrags * 1024, fw, lane);
     if (fw == 0) fetch_share<1, 1>(to + (2 * NP * F + 2 * kTFrags) * FR, p.workspace + lay.vec + (vunit0 + c) * (int64_t)(kVecFloats * 4), 0, lane);
   };
   if constexpr (AHEAD) {

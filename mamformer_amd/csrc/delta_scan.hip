@@ -6,6 +6,8 @@
 //   S'    = e^{G_end} S + (beta e^{G_end - G} K)^T delta
 // delta is what each token corrects before its beta, so that beta = 0 divides nothing.  delta_prep_kernel makes T and P of
 // every piece side by side; delta_scan_kernel walks the pieces with the state in registers.
+// o takes both parts of S, P and delta also where it is rounded to bf16: its terms may cancel far below what enters them, and
+// one part, 2^-12 of that, would show (it was 9 of 142 us at b 4, H 16, L 2048).
 #include "delta.h"
 
 namespace mh {
@@ -250,7 +252,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void delta_prep_kernel
         put_frag(out, t_frag(w, s), lane, th[s]);
         put_frag(out, kTFrags + t_frag(w, s), lane, tl[s]);
         put_frag(out, 2 * kTFrags + t_frag(w, s), lane, ph[s]);
-        if constexpr (NP == 2) put_frag(out, 3 * kTFrags + t_frag(w, s), lane, pl[s]);
+        put_frag(out, 3 * kTFrags + t_frag(w, s), lane, pl[s]);
       }
     if (backward) {                              // by columns: through LDS, as T^T and P^T (row j, column t)
 #pragma unroll
@@ -269,8 +271,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void delta_prep_kernel
 #pragma unroll
         for (int s = 0; s < 2; ++s)
           if (w < 2 + 2 * s) {
-            put_frag(out, (2 + NP + n) * kTFrags + tt_frag(w, s), lane, row_frag16<64>(tiles + n * TC::ELEMS, 16 * w, 32 * s, lane));
-            put_frag(out, (4 + NP + n) * kTFrags + tt_frag(w, s), lane, row_frag16<64>(tiles + (2 + n) * TC::ELEMS, 16 * w, 32 * s, lane));
+            put_frag(out, (4 + n) * kTFrags + tt_frag(w, s), lane, row_frag16<64>(tiles + n * TC::ELEMS, 16 * w, 32 * s, lane));
+            put_frag(out, (6 + n) * kTFrags + tt_frag(w, s), lane, row_frag16<64>(tiles + (2 + n) * TC::ELEMS, 16 * w, 32 * s, lane));
           }
     }
     float* vec = reinterpret_cast<float*>(p.workspace + lay.vec) + vunit * kVecFloats;
@@ -312,12 +314,14 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
   constexpr int FW = AHEAD ? 1 : 2 * PAIRS;      // waves that fetch
   constexpr int KS = DKP / 32, KSH = KS / 2, NSH = DKP / 32, F = kKFrags<DKP>;
   constexpr int GA = (OUT ? 2 : 1) * NP * F;                         // fragments of (Q and) K by rows: before barrier 1
-  constexpr int TPF = (OUT ? 2 + NP : 2) * kTFrags;                  // of T (and P)
+  constexpr int TPF = (OUT ? 4 : 2) * kTFrags;                       // of T (and P)
   constexpr int GB = NP * F + TPF + 1;                               // with K by columns and vec: after it
-  constexpr int XF = OUT ? 4 : 2, DF = OUT ? NP : 0;
-  constexpr int EX = (2 * XF + 2 + 4 + DF + 1) * FR;                 // halfs of a pair's exchange
+  constexpr int XF = OUT ? 4 : 2;
+  constexpr int EX = (2 * XF + 2 + 4 + 1) * FR;                      // halfs of a pair's exchange
   constexpr int IO = AHEAD ? (OUT ? 3 : 2) * IOW * IOH : 0;           // v of two pieces, o of one
-  constexpr int AB = AHEAD && PAIRS == 1 ? 2 : 1;                    // pieces of which K and Q by rows have room (175 -> 168 us)
+  // Pieces of which K and Q by rows have room.  A second one's took 4% off the chain (175 -> 168 us at b 2, H 16, L 4096,
+  // where P had one part); with o of 128 channels the two parts of P leave none for it.
+  constexpr int AB = AHEAD && PAIRS == 1 && !(OUT && DKP == 128) ? 2 : 1;
   __shared__ __align__(1024) f16 smem[(AB * GA + (AHEAD ? 2 : 1) * GB) * FR + PAIRS * EX + IO];
 
   const int lane = threadIdx.x & 63, w = wave_id(), l16 = lane & 15, g4 = lane >> 4, hf = w & 1;
@@ -431,8 +435,10 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
   const f32x4* const xRecv = reinterpret_cast<const f32x4*>(ex) + (1 - hf) * XF * 64 + lane;
   f16* const eR = ex + 2 * XF * FR;                                                    // the first half's R
   f16* const eU = eR + 2 * FR;                                                         // U, two parts of each half
-  f16* const eD = eU + 4 * FR;                                                         // the first half's delta
-  float* const eS = reinterpret_cast<float*>(eD + DF * FR);                            // scales: R, D, U of each half
+  // the first half's delta, where the second wave's X was: the first one has read that before barrier 2, and the second
+  // one, which reads delta behind barrier 3, writes its next X itself
+  f16* const eD = ex + XF * FR;
+  float* const eS = reinterpret_cast<float*>(eU + 4 * FR);                             // scales: R, D, U of each half
 
   const int64_t states = (int64_t)p.dk * p.dv;   // elements of a state
   float* const seg_states = reinterpret_cast<float*>(p.workspace + lay.seg_states) + (int64_t)bh * lay.segs * states;
@@ -497,16 +503,14 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
 #pragma unroll
         for (int i = 0; i < 4; ++i) X[i] = mma_h(frag(Kr, F + ((2 * hf + i) & 3) * KS + hf * KSH + s, lane), sh[s], X[i]);
     }
-    if constexpr (OUT)                           // o is rounded to T: one part of the state is enough for bf16
+    if constexpr (OUT)
 #pragma unroll
       for (int s = 0; s < KSH; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           Y[i] = mma_h(qa[s][i], sh[s], Y[i]);
-          if constexpr (NP == 2) {
-            Y[i] = mma_h(qa[s][i], sl[s], Y[i]);
-            Y[i] = mma_h(frag(Qr, F + ((2 * hf + i) & 3) * KS + hf * KSH + s, lane), sh[s], Y[i]);
-          }
+          Y[i] = mma_h(qa[s][i], sl[s], Y[i]);
+          if constexpr (NP == 2) Y[i] = mma_h(frag(Qr, F + ((2 * hf + i) & 3) * KS + hf * KSH + s, lane), sh[s], Y[i]);
         }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -618,7 +622,7 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
     put_frag(eU, 2 * hf + 1, lane, wl[0]);
     eS[(2 + hf) * 64 + lane] = own_us;
     const Scale sd(col_max(abs_max(D)));
-    parts_of<(KEEP || NP == 2) ? 2 : 1>(D, sd.mult, dh, dl);
+    parts_of<KEEP || OUT ? 2 : 1>(D, sd.mult, dh, dl);
     if constexpr (KEEP)
       if (live) {
         keep_parts<2>(keep + kTokens<DKP>, hf, dh, dl, lane);
@@ -627,7 +631,7 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
     if constexpr (OUT)
       if (hf == 0) {
         put_frag(eD, 0, lane, dh[0]);
-        if constexpr (NP == 2) put_frag(eD, 1, lane, dl[0]);
+        put_frag(eD, 1, lane, dl[0]);
         eS[64 + lane] = sd.inv * ds;
       }
     lds_barrier();                               // 3
@@ -637,7 +641,7 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
     float od = 0.f;
     if constexpr (OUT) {
       d0 = frag(eD, 0, lane);
-      if constexpr (NP == 2) d1 = frag(eD, 1, lane);
+      d1 = frag(eD, 1, lane);
       od = eS[64 + lane];
     }
     if (AHEAD && c + 1 < c1) load_a(c + 1);
@@ -666,19 +670,15 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         O[i] = mma_h(pa[i], dh[0], O[i]);
-        if constexpr (NP == 2) {
-          O[i] = mma_h(pa[i], dl[0], O[i]);
-          O[i] = mma_h(frag(Pt, kTFrags + t_frag(2 * hf + i, hf), lane), dh[0], O[i]);
-        }
+        O[i] = mma_h(pa[i], dl[0], O[i]);
+        O[i] = mma_h(frag(Pt, kTFrags + t_frag(2 * hf + i, hf), lane), dh[0], O[i]);
       }
       if (hf == 1) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           OX[i] = mma_h(px[i], d0, OX[i]);
-          if constexpr (NP == 2) {
-            OX[i] = mma_h(px[i], d1, OX[i]);
-            OX[i] = mma_h(frag(Pt, kTFrags + t_frag(2 + i, 0), lane), d0, OX[i]);
-          }
+          OX[i] = mma_h(px[i], d1, OX[i]);
+          OX[i] = mma_h(frag(Pt, kTFrags + t_frag(2 + i, 0), lane), d0, OX[i]);
         }
       }
       const float yq = p.scale * sQ, os = p.scale * (sd.inv * ds * cs[2]), ox = p.scale * (od * cs[2]);

@@ -1,0 +1,82 @@
+"""Gated delta rule, rotary positions and group norm on the GPU where results cancel, variants meet and sizes end, against the
+float64 oracle; tolerances are counted as in test_gpu_mixer_ops."""
+
+import numpy as np
+import pytest
+import torch
+
+import mamformer_amd as mh
+from oracle import mixers as mx
+from tests.gpu_helpers import host, say
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def both(a, dtype):
+    """a rounded to dtype: (float64 array, GPU tensor)."""
+    t = torch.as_tensor(np.asarray(a)).to(dtype)
+    return t.double().numpy(), t.cuda()
+
+
+def rows_within(name, out, ref, enter, k):
+    """Rows' errors in norm against half a step of the result and k 2^-20 of the norm that enters, a number."""
+    half = torch.finfo(out.dtype).eps / 2
+    o = host(out)
+    assert o.shape == ref.shape and np.isfinite(o).all(), name
+    tol = half * np.linalg.norm(ref, axis=-1) + k * 2.0 ** -20 * enter
+    worst = (np.linalg.norm(o - ref, axis=-1) / tol).max()
+    say(f"{name}: error at most {worst:.3f} of the tolerance")
+    assert worst <= 1, f"{name}: {worst:.3f} times the tolerance"
+
+
+# ------------------------------------------------------------------------------------------------ results that cancel
+# o is a sum whose terms may cancel far below what enters it.  Its error before the one rounding is 2^-20 of the norms that
+# enter for each of 12 products on the way, whatever is left of the sum.
+
+def cancelling(rng, *shape):
+    """(r, -r (1 + about 2^-8)) along a new first axis of 2, in fp32."""
+    r = rng.standard_normal(shape).astype(np.float32)
+    return np.stack([r, -r * (1 + 2.0 ** -8 * rng.uniform(0.5, 1, shape))]).astype(np.float32)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("H,L,dk,dv", [(4, 5, 2, 64), (3, 130, 70, 16), (40, 70, 2, 130), (2, 1500, 2, 64)])
+def test_delta_of_a_state_that_cancels(dtype, H, L, dk, dv):
+    """o = scale q^T S with two rows of S that nearly cancel (beta = 0: no token writes)."""
+    rng = np.random.default_rng(L)
+    s = np.zeros((1, H, dk, dv), np.float32)
+    s[:, :, 0], s[:, :, -1] = cancelling(rng, 1, H, dv)
+    q = np.zeros((1, H, L, dk))
+    q[..., 0] = q[..., -1] = rng.uniform(1, 2, (1, H, L))
+    (qh, qg), (kh, kg), (vh, vg) = both(q, dtype), both(rng.standard_normal(q.shape) / dk ** 0.5, dtype), both(rng.standard_normal((1, H, L, dv)), dtype)
+    (sh, sg), (bh, bg) = both(s, F32), both(np.zeros((1, H, L)), F32)
+    say(f"state that cancels H={H} L={L} {dk} {dv} {dtype}")
+    o = mh.gated_delta_rule(qg, kg, vg, None, bg, initial_state=sg)
+    ref, _ = mx.delta_rule(qh, kh, vh, None, bh, None, sh)
+    enter = dk ** -0.5 * np.linalg.norm(qh, axis=-1).max() * np.linalg.norm(sh, axis=(-2, -1)).max()
+    rows_within("o", o, ref, enter, 12 * np.sqrt((L + 63) // 64))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("H,dv,given", [(8, 64, "beta"), (8, 64, "state"), (40, 130, "beta"), (40, 130, "state")])
+def test_delta_of_corrections_that_cancel(dtype, H, dv, given):
+    """o of a second token whose two terms nearly cancel: equal values with nearly equal beta, or what two rows of the state
+    are corrected by.  Keys are the unit vectors, so that each token's correction is v less its row of the state."""
+    rng = np.random.default_rng(dv)
+    k, q = np.broadcast_to(np.eye(2), (1, H, 2, 2)), np.ones((1, H, 2, 2))
+    v, beta, s = np.zeros((1, H, 2, dv)), np.ones((1, H, 2)), np.zeros((1, H, 2, dv))
+    if given == "beta":
+        v[:, :, 0] = rng.standard_normal((1, H, dv))
+        v[:, :, 1] = -v[:, :, 0]
+        beta[..., 0] = rng.uniform(0.5, 1, (1, H))
+        beta[..., 1] = beta[..., 0] * (1 + 2.0 ** -8 * rng.uniform(0.5, 1, (1, H)))
+    else:
+        s[:, :, 0], s[:, :, 1] = cancelling(rng, 1, H, dv)
+        q[:, :, 0] = 0.5
+    (qh, qg), (kh, kg), (vh, vg), (bh, bg), (sh, sg) = (both(a, t) for a, t in ((q, dtype), (k, dtype), (v, dtype), (beta, F32), (s, F32)))
+    say(f"corrections that cancel, {given}, H={H} {dv} {dtype}")
+    o = mh.gated_delta_rule(qg, kg, vg, None, bg, scale=1.0, initial_state=sg)
+    ref, _ = mx.delta_rule(qh, kh, vh, None, bh, 1.0, sh)
+    enter = np.sqrt(2) * (np.linalg.norm(sh, axis=(-2, -1)).max() + np.linalg.norm(vh, axis=(-2, -1)).max())
+    rows_within("o", o, ref, enter, 12)
