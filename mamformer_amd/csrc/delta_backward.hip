@@ -384,10 +384,10 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
   using TK = HTile<DKP>;
   using TC = HTile<64>;
   constexpr int SE = DVB * DKP, YE = DVB * 64;   // elements of a part of S / dS and of delta / y
-  static_assert(4 * SE + 4 * YE >= 2 * NP * TC::ELEMS, "the pair terms take the place of the states, delta and y");
+  static_assert(4 * SE + 4 * YE >= 4 * TC::ELEMS, "the pair terms take the place of the states, delta and y");
   __shared__ __align__(1024) f16 smem[4 * SE + 4 * YE + NP * TC::ELEMS + 2 * NP * F * FR];
   f16 *sS = smem, *sN = sS + 2 * SE, *sY = sN + 2 * SE, *sD = sY + 2 * YE, *sO = sD + 2 * YE, *sK = sO + NP * TC::ELEMS, *sQ = sK + NP * F * FR;
-  f16 *sXa = smem, *sXp = smem + NP * TC::ELEMS;                       // where those were
+  f16 *sXa = smem, *sXp = smem + 2 * TC::ELEMS;                        // where those were
   __shared__ double sG[DC];
   __shared__ float sB[DC], sEG[DC], sEnd[DC], sRow[2][DC], sB2[2][DC], sCol[4][DC], red[8][4];
   const DeltaParams& p = q.f;
@@ -726,17 +726,15 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
         const f16 a = part_hi(pA[m][r], xa.mult), e = part_hi(pP[m][r], xp.mult);
         sXa[at] = a;
         sXp[at] = e;
-        if constexpr (NP == 2) {
-          sXa[TC::ELEMS + at] = part_lo(pA[m][r], xa.mult, a);
-          sXp[TC::ELEMS + at] = part_lo(pP[m][r], xp.mult, e);
-        }
+        sXa[TC::ELEMS + at] = part_lo(pA[m][r], xa.mult, a);
+        sXp[TC::ELEMS + at] = part_lo(pP[m][r], xp.mult, e);
       }
     __syncthreads();
-    f16x8 ra[2][NP], rp[2][NP], ca[2][NP], cp[2][NP];
+    f16x8 ra[2][2], rp[2][2], ca[2][2], cp[2][2]; // both parts also for bf16: rows of dQ and dK may cancel far below them
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int n = 0; n < NP; ++n) {
+      for (int n = 0; n < 2; ++n) {
         ra[s][n] = row_frag16<64>(sXa + n * TC::ELEMS, 16 * w, 32 * s, lane);
         rp[s][n] = row_frag16<64>(sXp + n * TC::ELEMS, 16 * w, 32 * s, lane);
         ca[s][n] = col_frag16<64>(sXa + n * TC::ELEMS, 16 * w, 32 * s, lane);
@@ -749,21 +747,20 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const f16x8 k0 = frag(sK, 2 * (hf * NSH + n) + s, lane), q0 = frag(sQ, 2 * (hf * NSH + n) + s, lane);
-        u1 = mma_h(rp[s][0], k0, u1);
-        u2 = mma_h(ra[s][0], k0, u2);
-        u2 = mma_h(ca[s][0], k0, u2);
-        u3 = mma_h(cp[s][0], q0, u3);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          u1 = mma_h(rp[s][x], k0, u1);
+          u2 = mma_h(ra[s][x], k0, u2);
+          u2 = mma_h(ca[s][x], k0, u2);
+          u3 = mma_h(cp[s][x], q0, u3);
+        }
         if constexpr (NP == 2) {
           const f16x8 k1 = frag(sK, F + 2 * (hf * NSH + n) + s, lane);
           const f16x8 q1 = frag(sQ, F + 2 * (hf * NSH + n) + s, lane);
           u1 = mma_h(rp[s][0], k1, u1);
-          u1 = mma_h(rp[s][1], k0, u1);
           u2 = mma_h(ra[s][0], k1, u2);
-          u2 = mma_h(ra[s][1], k0, u2);
           u2 = mma_h(ca[s][0], k1, u2);
-          u2 = mma_h(ca[s][1], k0, u2);
           u3 = mma_h(cp[s][0], q1, u3);
-          u3 = mma_h(cp[s][1], q0, u3);
         }
       }
 #pragma unroll

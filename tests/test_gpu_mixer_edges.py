@@ -31,8 +31,8 @@ def rows_within(name, out, ref, enter, k):
 
 
 # ------------------------------------------------------------------------------------------------ results that cancel
-# o is a sum whose terms may cancel far below what enters it.  Its error before the one rounding is 2^-20 of the norms that
-# enter for each of 12 products on the way, whatever is left of the sum.
+# o, dq and dk are sums whose terms may cancel far below what enters them.  Their error before the one rounding is 2^-20 of
+# the norms that enter for each product (12 on the way to o, 24 to a gradient), whatever is left of the sum.
 
 def cancelling(rng, *shape):
     """(r, -r (1 + about 2^-8)) along a new first axis of 2, in fp32."""
@@ -80,3 +80,44 @@ def test_delta_of_corrections_that_cancel(dtype, H, dv, given):
     ref, _ = mx.delta_rule(qh, kh, vh, None, bh, 1.0, sh)
     enter = np.sqrt(2) * (np.linalg.norm(sh, axis=(-2, -1)).max() + np.linalg.norm(vh, axis=(-2, -1)).max())
     rows_within("o", o, ref, enter, 12)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("H,dv", [(16, 64), (40, 130)])
+def test_delta_gradients_that_cancel(dtype, H, dv):
+    """dq and dk whose pair terms nearly cancel.  Three tokens of one key: values v0 and -v0 written with nearly the same small
+    beta, and a third that reads and corrects nearly nothing, whose dq and dk are the sum of both; and a key that two opposite
+    queries read under nearly the same decay, whose dk is the sum of theirs."""
+    rng = np.random.default_rng(dv)
+    v0, one = rng.standard_normal((1, H, dv)), np.ones((1, H))
+    v, do, g, beta = np.zeros((1, H, 3, dv)), np.zeros((1, H, 3, dv)), np.zeros((1, H, 3)), np.zeros((1, H, 3))
+    v[:, :, 0], v[:, :, 1], do[:, :, 2] = v0, -v0, v0
+    beta[..., 0] = 2.0 ** -8 * rng.uniform(0.5, 1, (1, H))
+    beta[..., 1] = beta[..., 0] * (1 + 2.0 ** -8 * rng.uniform(0.5, 1, (1, H)))
+    beta[..., 2] = 1
+    key = np.stack([0.6 * one, 0.8 * one], -1)
+    k = np.stack([key] * 3, 2)
+    q = np.zeros_like(k)
+    q[:, :, 2] = key
+    args = [both(a, t) for a, t in ((do, dtype), (q, dtype), (k, dtype), (v, dtype), (g, F32), (beta, F32))]
+    say(f"dq and dk of values that cancel H={H} {dv} {dtype}")
+    got = mh.gated_delta_rule_bwd(*(a for _, a in args), scale=1.0)
+    ref = mx.delta_rule_bwd(*(a for a, _ in args), 1.0)
+    # each of the two terms: do . v0 times beta, by a key of norm 1
+    enter = 2 * (args[0][0] ** 2).sum(-1).max() * args[5][0][..., :2].max()
+    rows_within("dq", got[0][:, :, 2:], ref[0][:, :, 2:], enter, 24)
+    rows_within("dk", got[1][:, :, 2:], ref[1][:, :, 2:], enter, 24)
+
+    v, do, beta = v * 0, do * 0, beta * 0
+    v[:, :, 0] = do[:, :, 1] = do[:, :, 2] = v0
+    beta[..., 0] = rng.uniform(0.5, 1, (1, H))
+    g[..., 1:] = -2.0 ** -8 * rng.uniform(0.5, 1, (1, H, 2))
+    k, q = np.zeros_like(k), np.zeros_like(q)
+    k[..., 0] = 1
+    q[:, :, 1, 1], q[:, :, 2, 1] = 1, -1
+    args = [both(a, t) for a, t in ((do, dtype), (q, dtype), (k, dtype), (v, dtype), (g, F32), (beta, F32))]
+    say("dk of queries that cancel")
+    got = mh.gated_delta_rule_bwd(*(a for _, a in args), scale=1.0)
+    ref = mx.delta_rule_bwd(*(a for a, _ in args), 1.0)
+    enter = 2 * (args[0][0] ** 2).sum(-1).max() * args[5][0].max()
+    rows_within("dk", got[1][:, :, :1], ref[1][:, :, :1], enter, 24)
