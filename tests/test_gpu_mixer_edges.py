@@ -8,6 +8,7 @@ import torch
 import mamformer_amd as mh
 from oracle import mixers as mx
 from tests.gpu_helpers import host, say
+from tests.test_gpu_mixer_ops import compare, delta_inputs
 
 pytestmark = pytest.mark.gpu
 BF, F32 = torch.bfloat16, torch.float32
@@ -121,3 +122,36 @@ def test_delta_gradients_that_cancel(dtype, H, dv):
     ref = mx.delta_rule_bwd(*(a for a, _ in args), 1.0)
     enter = 2 * (args[0][0] ** 2).sum(-1).max() * args[5][0].max()
     rows_within("dk", got[1][:, :, :1], ref[1][:, :, :1], enter, 24)
+
+
+# ------------------------------------------------------------------------------------------------ two pairs a workgroup
+# bf16 scans take two pairs of waves a workgroup, 32 columns of v, where batch * heads * segments * ceil(dv / 16) passes 256.
+
+@pytest.mark.parametrize("B,H,HK,L,dk,dv,opts", [
+    (4, 24, 12, 70, 40, 37, {}),                 # 288 blocks, three a head: a workgroup's second pair without columns
+    (2, 15, 5, 131, 100, 130, {}),               # 270, nine a head, the last of two columns
+    (3, 30, 30, 64, 128, 48, dict(state=False)), (11, 12, 6, 1, 64, 31, {}), (5, 20, 4, 65, 17, 33, dict(gates=False)),
+    (1, 260, 26, 200, 24, 8, dict(decay=3.0)),
+    (1, 8, 4, 2100, 16, 130, {}),                # in segments as well
+])
+def test_delta_of_many_columns(B, H, HK, L, dk, dv, opts):
+    say(f"delta {B} {H} {HK} {L} {dk} {dv} {opts}")
+    compare(*delta_inputs(B, H, HK, L, dk, dv, BF, **opts))
+
+
+@pytest.mark.parametrize("B,H,HK,L,dk,dv", [(4, 24, 12, 70, 40, 37), (3, 20, 10, 190, 100, 130), (5, 20, 20, 129, 64, 48)])
+def test_delta_of_many_columns_is_that_of_few(B, H, HK, L, dk, dv):
+    """The last sequence of a batch alone, which takes one pair a workgroup: the same bits, recomputed or kept."""
+    _, t = delta_inputs(B, H, HK, L, dk, dv, BF)
+    last = [a[-1:] for a in t]
+    do, df = torch.randn_like(t[2]), torch.randn_like(t[5])
+    say(f"last of {B} {H} {HK} {L} {dk} {dv}")
+
+    def run(t, do, df, recompute):
+        leaves = [a.detach().requires_grad_(True) for a in t]
+        out = mh.gated_delta_rule(*leaves[:5], initial_state=leaves[5], return_final_state=True, recompute=recompute)
+        return [a.detach() for a in (*out, *torch.autograd.grad(out, leaves, (do, df)))]
+
+    for recompute in (False, True):
+        for a, b in zip(run(t, do, df, recompute), run(last, do[-1:], df[-1:], recompute)):
+            assert torch.equal(a[-1:], b)
