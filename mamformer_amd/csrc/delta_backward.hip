@@ -235,11 +235,11 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_back_scan_ker
       eg[i] = *reinterpret_cast<const f32x4*>(vec + 32 * hf + 16 * i + 4 * g4);
     }
     __builtin_amdgcn_sched_barrier(0);
-    const float zs = p.scale * (so.inv * cs[2]);
+    const float zs = so.inv * cs[2];             // a power of two, exact also below fp32's normal range, as ysc and uk
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) Z[i][r] = zs * Z[i][r] + wt[i][r] * (cs[3] * (ss.inv * X[i][r] + xr[i][r]));
+      for (int r = 0; r < 4; ++r) Z[i][r] = __builtin_fmaf(p.scale, zs * Z[i][r], wt[i][r] * (cs[3] * __builtin_fmaf(ss.inv, X[i][r], xr[i][r])));
     // y = T^T ddelta
     f16x8 zh[1], zl[1];
     const Scale sz(col_max(abs_max(Z)));
@@ -289,7 +289,7 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_back_scan_ker
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         U[i][r] *= uq * eg[i][r];
-        V[i][r] = uk * eg[i][r] * Yv[i][r];
+        V[i][r] = uk * Yv[i][r] * eg[i][r];
       }
     f16x8 uh[1], ul[1], vh[1], vl[1], yh[1], yl[1];
     const Scale su(col_max(abs_max(V, abs_max(U))));
@@ -625,9 +625,9 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
         }
       }
     }
-    // A' and P', what they give dbeta and dG, and the pair terms' matrices
+    // A' and P', what they give dbeta and dG, and the pair terms' matrices.  The operands' scales, powers of two, go to the
+    // sums one after the other, as their products alone may leave fp32's range where those do not.
     const int lane = lane_id_here(), l16 = lane & 15, g4 = lane >> 4;
-    const float fA = -(mY * mD), fP = p.scale * (so_inv * mD);
     float rows[4] = {}, xam = 0.f, xpm = 0.f;
     double Gt[4];
 #pragma unroll
@@ -643,7 +643,7 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
         for (int r = 0; r < 4; ++r) {
           const int below = 16 * (w - j) + 4 * g4 + r - l16;
           const float d = below >= 0 ? exp_of(Gt[r] - Gj) : 0.f;
-          const float xa = below > 0 ? fA * pA[m][r] * d : 0.f, xp = below >= 0 ? fP * pP[m][r] * d : 0.f;
+          const float xa = below > 0 ? pA[m][r] * -mY * mD * d : 0.f, xp = below >= 0 ? pP[m][r] * so_inv * mD * (p.scale * d) : 0.f;
           const float v = (below > 0 ? xa * kk[m][r] : 0.f) + (below >= 0 ? xp * qk[m][r] : 0.f);
           colb += v;
           rows[r] += v * bj;
@@ -665,7 +665,6 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
       red[wave][2] = xpm;
       red[wave][3] = dot;
     }
-    const float fq = p.scale * (so_inv * mS), fl = -(mY * mS), fr = mD * mN;
     float dots[4] = {}, rights[4] = {};
 #pragma unroll
     for (int n = 0; n < NSH; ++n) {
@@ -684,9 +683,9 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
           kv += (float)(w & 1 ? kf[1][4 + r] : kf[1][r]);
           qv += (float)(w & 1 ? qf[1][4 + r] : qf[1][r]);
         }
-        const float q1 = aq[n][r] * (fq * sEG[t]), l1 = al[n][r] * (fl * sEG[t]), r1 = ar[n][r] * (fr * sEnd[t]);
-        dots[r] += sq * (qv * q1) + sk * (kv * l1);
-        rights[r] += kv * r1;
+        const float q1 = aq[n][r] * so_inv * mS * (p.scale * sEG[t]), l1 = al[n][r] * -mY * mS * sEG[t], r1 = ar[n][r] * mD * mN * sEnd[t];
+        dots[r] += (sq * qv) * q1 + (sk * kv) * l1;
+        rights[r] += (sk * kv) * r1;
         tq[n][r] += q1;
         tk[n][r] += l1 + sB[t] * r1;
       }
@@ -694,7 +693,7 @@ __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, Delt
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int t = 16 * w + 4 * g4 + r;
-      const float left = group_sum<16>(dots[r] + rows[r]), right = sk * group_sum<16>(rights[r]);
+      const float left = group_sum<16>(dots[r] + rows[r]), right = group_sum<16>(rights[r]);
       if (l16 == 0) {
         sRow[hf][t] = left;
         sB2[hf][t] = right;

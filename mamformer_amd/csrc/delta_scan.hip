@@ -681,14 +681,15 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
           OX[i] = mma_h(frag(Pt, kTFrags + t_frag(2 + i, 0), lane), d0, OX[i]);
         }
       }
-      const float yq = p.scale * sQ, os = p.scale * (sd.inv * ds * cs[2]), ox = p.scale * (od * cs[2]);
+      const float os = sd.inv * ds * cs[2], ox = od * cs[2];           // powers of two, exact also below fp32's normal range
       float o[8];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          o[4 * i + r] = __builtin_fmaf(eg[i][r], yq * __builtin_fmaf(ss.inv, Y[i][r], yr[i][r]), os * O[i][r]);
+          o[4 * i + r] = __builtin_fmaf(eg[i][r], sQ * __builtin_fmaf(ss.inv, Y[i][r], yr[i][r]), os * O[i][r]);
           if (hf == 1) o[4 * i + r] = __builtin_fmaf(ox, OX[i][r], o[4 * i + r]);
+          o[4 * i + r] *= p.scale;
         }
       if constexpr (AHEAD) {
 #pragma unroll

@@ -155,3 +155,72 @@ def test_delta_of_many_columns_is_that_of_few(B, H, HK, L, dk, dv):
     for recompute in (False, True):
         for a, b in zip(run(t, do, df, recompute), run(last, do[-1:], df[-1:], recompute)):
             assert torch.equal(a[-1:], b)
+
+
+# ------------------------------------------------------------------------------------------------ far from one
+
+def scaled(t, x, i, size):
+    t[i] = t[i] * size
+    x[i] = t[i].double().cpu().numpy()
+
+
+def sized(name, out, ref, k):
+    """rows_within in units of the largest of ref (squares of its values may leave fp32's range); k products, and the result's
+    rounding in its type."""
+    size = np.abs(ref).max()
+    half = 2.0 ** 20 * torch.finfo(out.dtype).eps / 2
+    rows_within(name, out.double() / size, ref / size, np.linalg.norm(ref / size, axis=-1).max(), k + half)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("values", [1e-34, 1e-30, 1e-18, 1e12, 1e30])
+@pytest.mark.parametrize("L", [130, 1100])
+def test_delta_far_from_one(dtype, values, L):
+    """Values and states far outside fp16's range and near the ends of fp32's: no power of two on the way leaves it before."""
+    x, t = delta_inputs(1, 4, 2, L, 32, 24, dtype)
+    for i in (2, 5):
+        scaled(t, x, i, values)
+    say(f"values of {values}, L={L} {dtype}")
+    o, s = mh.gated_delta_rule(*t[:5], initial_state=t[5], return_final_state=True)
+    ro, rs = mx.delta_rule(*x[:5], None, x[5])
+    sized("o", o, ro, 12 * np.sqrt((L + 63) // 64))
+    sized("state", s, rs, 12 * np.sqrt((L + 63) // 64))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("values,grads", [(1e-18, 1e12), (1e12, 1e-18), (1e12, 1e12), (1e-9, 1e-18), (1e-18, 1e-18),
+                                          (1e-30, 1.0), (1.0, 1e-30), (1.0, 1e-33), (1e-20, 1e-14), (1e18, 1e17)])
+def test_delta_gradients_far_from_one(dtype, values, grads):
+    """The same of gradients, whose products with the values stay within fp32's normal range."""
+    x, t = delta_inputs(1, 4, 2, 130, 32, 24, dtype)
+    for i in (2, 5):
+        scaled(t, x, i, values)
+    do, df = torch.randn_like(t[2]) * grads, torch.randn_like(t[5]) * grads
+    say(f"values of {values}, gradients of {grads}, {dtype}")
+    got = mh.gated_delta_rule_bwd(do, *t[:5], initial_state=t[5], d_final_state=df)
+    ref = mx.delta_rule_bwd(host(do), *x[:5], None, x[5], host(df))
+    for name, a, r in zip(("dq", "dk", "dv", "dg", "dbeta", "d_state"), got, ref):
+        sized(name, *((a, r) if a.dim() == 4 else (a[:, :, None], r[:, :, None])), 24 * np.sqrt(3))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("L", [20, 130, 1500])
+def test_delta_gradients_of_zeros(dtype, L):
+    """Nothing written and no state, or nothing that comes back: what does not depend on it has its gradient, all else is 0."""
+    x, t = delta_inputs(1, 4, 2, L, 32, 24, dtype)
+    do, zero = torch.randn_like(t[2]), torch.zeros_like(t[2])
+    say(f"zeros L={L} {dtype}")
+    for state in (None, torch.zeros_like(t[5])):
+        xs = None if state is None else host(state)
+        got = mh.gated_delta_rule_bwd(do, *t[:2], zero, *t[3:5], initial_state=state)
+        ref = mx.delta_rule_bwd(host(do), *x[:2], host(zero), *x[3:5], None, xs)
+        for name, a, r in zip(("dq", "dk", "dv", "dg", "dbeta", "d_state"), got, ref):
+            if name in ("dv", "d_state"):
+                if a is not None:
+                    rows_within(name, a, r, np.linalg.norm(r, axis=-1).max(), 24 * np.sqrt((L + 63) // 64))
+            else:
+                assert (a == 0).all(), name
+        for a in mh.gated_delta_rule_bwd(zero, *t[:5], initial_state=t[5], d_final_state=state):
+            assert (a == 0).all()
+    o, s = mh.gated_delta_rule(*t[:2], zero, *t[3:5], return_final_state=True)
+    assert (o == 0).all() and (s == 0).all()
