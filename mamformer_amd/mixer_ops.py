@@ -141,6 +141,8 @@ def _rotary(q, k, inv_freq, positions, cfg):
     offset, interleaved, scale, inverse = cfg
     q = _channels(q)
     B, H, L, D = q.shape
+    if not H and k is not None:                  # keys alone
+        return torch.empty_like(q), _rotary(k, None, inv_freq, positions, cfg)[0]
     inv_freq = _vec(inv_freq)
     pos_sb = 0
     if positions is not None:

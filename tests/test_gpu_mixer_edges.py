@@ -224,3 +224,21 @@ def test_delta_gradients_of_zeros(dtype, L):
             assert (a == 0).all()
     o, s = mh.gated_delta_rule(*t[:2], zero, *t[3:5], return_final_state=True)
     assert (o == 0).all() and (s == 0).all()
+
+
+# ------------------------------------------------------------------------------------------------ rotary positions
+
+def test_rotary_without_queries():
+    """q of no heads: keys are turned all the same, and their gradient."""
+    f, _ = mh.rotary_frequencies(16)
+    k = torch.randn(2, 3, 9, 24, device="cuda", requires_grad=True)
+    for H in (0, 1):
+        q = torch.randn(2, H, 9, 24, device="cuda", requires_grad=True)
+        a, b = mh.rotary(q, k, f)
+        assert a.shape == q.shape and torch.equal(b, mh.rotary(k, None, f))
+        dk, = torch.autograd.grad(b, k, torch.ones_like(b), retain_graph=True)
+        assert torch.equal(dk, mh.rotary(torch.ones_like(b), None, f, inverse=True))
+        dq, dk2 = torch.autograd.grad((a, b), (q, k), (torch.ones_like(a), torch.ones_like(b)))
+        assert dq.shape == q.shape and torch.equal(dk, dk2)
+    assert mh.rotary(q[:, :0], None, f).shape == (2, 0, 9, 24)
+    assert [t.shape[1] for t in mh.rotary(q[:, :0], k[:, :0], f)] == [0, 0]
