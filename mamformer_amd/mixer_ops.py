@@ -51,6 +51,12 @@ def _channels(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _result(t):
+    """A new tensor of t's layout, with contiguous channels (torch may order dimensions of equal strides the other way)."""
+    out = torch.empty_like(t)
+    return out if out.stride(-1) == 1 or t.shape[-1] == 1 else torch.empty(t.shape, device=t.device, dtype=t.dtype)
+
+
 def _f32(t):
     return t if t is None or t.dtype is torch.float32 else t.to(torch.float32)
 
@@ -149,10 +155,10 @@ def _rotary(q, k, inv_freq, positions, cfg):
         if positions.stride(-1) != 1 and L != 1:
             positions = positions.contiguous()
         pos_sb = positions.stride(0) if positions.dim() == 2 else 0
-    qo, ko, HK = torch.empty_like(q), None, 0
+    qo, ko, HK = _result(q), None, 0
     if k is not None:
         k = _channels(k)
-        ko, HK = torch.empty_like(k), k.shape[1]
+        ko, HK = _result(k), k.shape[1]
     (qb, qh, ql, _), (ob, oh, ol, _) = q.stride(), qo.stride()
     a = RotaryArgs(B, H, HK, L, D, inv_freq.shape[0], _DT[q.dtype], interleaved, inverse, inv_freq.dtype is torch.float64,
                    0 if positions is None else _INDEX_BYTES[positions.dtype], scale, inv_freq.data_ptr(), _ptr(positions), pos_sb,
@@ -248,7 +254,7 @@ def _delta_args(q, k, v, g, beta, state, scale):
 
 def _delta_fwd(q, k, v, g, beta, state, scale, want_final, keep):
     q, k, v, g, beta, state = _channels(q), _channels(k), _channels(v), _f32(g), _f32(beta), _vec(state)
-    o = torch.empty_like(v)
+    o = _result(v)
     final = None
     if want_final:
         final = torch.empty((*v.shape[:2], q.shape[-1], v.shape[-1]), device=v.device, dtype=torch.float32)
@@ -279,7 +285,7 @@ def gated_delta_rule_bwd(do, q, k, v, g=None, beta=None, *, scale=None, initial_
 def _delta_bwd(do, q, k, v, g, beta, initial_state, d_final_state, scale, kept=None):
     q, k, v, do = _channels(q), _channels(k), _channels(v), _channels(do)
     g, beta, initial_state, d_final_state = _f32(g), _f32(beta), _vec(initial_state), _vec(d_final_state)
-    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    dq, dk, dv = _result(q), _result(k), _result(v)
     dg, dbeta = (None if t is None else torch.empty(v.shape[:-1], device=v.device, dtype=torch.float32) for t in (g, beta))
     d_state = None if initial_state is None else torch.empty_like(initial_state)
     a = DeltaBwdArgs(_delta_args(q, k, v, g, beta, initial_state, scale), *_strides3(do), _ptr(d_final_state), *_strides3(dq),
@@ -339,7 +345,7 @@ def gated_delta_step(state, q, k, v, g=None, beta=None, *, scale=None, state_out
     if _through_autograd(state, q, k, v, g, beta, state_out):
         raise RuntimeError(f"{name}: has no backward; call it under torch.no_grad(), or gated_delta_rule with L = 1")
     q, k, v, g, beta = _channels(q), _channels(k), _channels(v), _f32(g), _f32(beta)
-    o = torch.empty_like(v)
+    o = _result(v)
     (B, HK, dk), (_, H, dv) = q.shape, v.shape
     (qb, qh, _), (kb, kh, _), (vb, vh, _), (ob, oh, _) = q.stride(), k.stride(), v.stride(), o.stride()
     a = DeltaStepArgs(B, H, HK, dk, dv, _DT[q.dtype], dk ** -0.5 if scale is None else scale, q.data_ptr(), qb, qh,

@@ -242,3 +242,27 @@ def test_rotary_without_queries():
         assert dq.shape == q.shape and torch.equal(dk, dk2)
     assert mh.rotary(q[:, :0], None, f).shape == (2, 0, 9, 24)
     assert [t.shape[1] for t in mh.rotary(q[:, :0], k[:, :0], f)] == [0, 0]
+
+
+# ------------------------------------------------------------------------------------------------ strides
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_sliding_windows(dtype):
+    """Tokens that are windows of one signal, an element apart, as unfold gives them: inputs may overlap themselves, the
+    results do not, and they have the bits of a copy."""
+    L, D = 9, 16                                 # fewer tokens than channels: torch would lay a like tensor out by tokens
+    x = torch.randn(2, 3, L + D - 1, device="cuda").to(dtype)
+    w = x.unfold(-1, D, 1)
+    assert w.shape == (2, 3, L, D) and w.stride()[-2:] == (1, 1)
+    c = w.contiguous()
+    f, _ = mh.rotary_frequencies(D)
+    for a, b in zip(mh.rotary(w, w, f), mh.rotary(c, c, f)):
+        assert torch.equal(a, b)
+    assert torch.equal(mh.gated_delta_rule(w, w, w), mh.gated_delta_rule(c, c, c))
+    for a, b in zip(mh.gated_delta_rule_bwd(w, w, w, w)[:3], mh.gated_delta_rule_bwd(c, c, c, c)[:3]):
+        assert torch.equal(a, b)
+    state = torch.randn(2, L, D, D, device="cuda")
+    w3, s2 = w[:, 0], state.clone()
+    assert torch.equal(mh.gated_delta_step(state, w3, w3, w3), mh.gated_delta_step(s2, *(w3.contiguous(),) * 3))
+    assert torch.equal(state, s2)
+    assert torch.equal(mh.group_norm(w[:, 0], 4), mh.group_norm(w[:, 0].contiguous(), 4))
