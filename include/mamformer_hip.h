@@ -617,7 +617,7 @@ int mh_token_logprobs_bwd(const mh_logprob_bwd_args* a, void* stream);
  *   q, k (batch, kheads, seqlen, dk), v, o (batch, heads, seqlen, dv) in dtype; heads a multiple of kheads, value head h reads
  *   key head h / (heads / kheads). g, beta (batch, heads, seqlen) fp32, each or NULL (g = 0, beta = 1); g = -inf clears the
  *   state. initial_state, final_state (batch, heads, dk, dv) fp32 contiguous, each or NULL. dk <= 128, dv <= 256,
- *   batch * heads * ceil(seqlen / 64) <= 2^23. A NaN or infinity may reach every result of its head from the 64-token piece
+ *   batch * heads * ceil(seqlen / 64) and batch * heads * ceil(dv / 32) <= 2^23. A NaN or infinity may reach every result of its head from the 64-token piece
  *   that holds it on, and no other head's. seqlen = 0 copies the state. The same bits at every call. Operands of the products
  *   keep 22 bits of the largest value of their column or piece, sums are fp32.
  *   keep: the workspace is larger and holds afterwards what a backward of the same arguments needs (its `kept`), about

@@ -1103,9 +1103,17 @@ int delta_sizes(const char* fn, int64_t batch, int64_t heads, int64_t kheads, in
   return MH_OK;
 }
 
+// A call over sequences: the scans' grids keep below 2^32 threads, at most 384 for 32 columns of a head.
+int delta_seq_sizes(const char* fn, const mh_delta_args* a) {
+  MH_TRY(delta_sizes(fn, a->batch, a->heads, a->kheads, a->seqlen, a->dk, a->dv, a->dtype));
+  if (a->seqlen > 0 && a->batch * a->heads > kDeltaPieces / ((a->dv + 31) / 32))
+    return fail(MH_ERR_SHAPE, "%s: more than 2^23 heads of 32 columns (batch=%lld heads=%lld dv=%lld)", fn, (long long)a->batch, (long long)a->heads, (long long)a->dv);
+  return MH_OK;
+}
+
 // The inputs' checks; their regions go to r (at most 6).
 int delta_inputs(const char* fn, const mh_delta_args* a, Region* r, int& n) {
-  MH_TRY(delta_sizes(fn, a->batch, a->heads, a->kheads, a->seqlen, a->dk, a->dv, a->dtype));
+  MH_TRY(delta_seq_sizes(fn, a));
   const int es = elem_size(a->dtype);
   n = 0;
   if (a->batch == 0) return MH_OK;
@@ -1852,7 +1860,7 @@ int mh_token_logprobs_bwd(const mh_logprob_bwd_args* a, void* stream) {
 int mh_delta_rule_workspace_bytes(const mh_delta_args* a, size_t* bytes) {
   if (!bytes) return fail(MH_ERR_NULL, "delta_rule: bytes output is NULL");
   if (!a) return fail(MH_ERR_NULL, "delta_rule: args is NULL");
-  MH_TRY(delta_sizes("delta_rule", a->batch, a->heads, a->kheads, a->seqlen, a->dk, a->dv, a->dtype));
+  MH_TRY(delta_seq_sizes("delta_rule", a));
   mh::DeltaParams p;
   delta_fill(a, p);
   *bytes = a->batch && a->seqlen ? mh::delta_workspace_bytes(p) : 0;
@@ -1884,7 +1892,7 @@ int mh_delta_rule_bwd_workspace_bytes(const mh_delta_bwd_args* a, size_t* bytes)
   if (!bytes) return fail(MH_ERR_NULL, "delta_rule_bwd: bytes output is NULL");
   if (!a) return fail(MH_ERR_NULL, "delta_rule_bwd: args is NULL");
   const mh_delta_args* f = &a->fwd;
-  MH_TRY(delta_sizes("delta_rule_bwd", f->batch, f->heads, f->kheads, f->seqlen, f->dk, f->dv, f->dtype));
+  MH_TRY(delta_seq_sizes("delta_rule_bwd", f));
   mh::DeltaParams p;
   delta_fill(f, p);
   p.keep = 1;

@@ -802,7 +802,7 @@ hipError_t run_bwd(const DeltaBwdParams& q, hipStream_t st) {
 }
 
 __global__ void delta_copy_grad_kernel(const float* from, float* to, int64_t n) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = grid_row() * 256 + threadIdx.x;
   if (i < n) to[i] = from ? from[i] : 0.f;
 }
 
@@ -815,7 +815,7 @@ hipError_t launch_delta_bwd(const DeltaBwdParams& q, hipStream_t st) {
   if (p.seqlen == 0) {
     const int64_t n = (int64_t)p.batch * p.heads * p.dk * p.dv;
     if (!q.d_initial_state) return hipSuccess;
-    delta_copy_grad_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(q.d_final_state, q.d_initial_state, n);
+    delta_copy_grad_kernel<<<row_grid((n + 255) / 256, 1), 256, 0, st>>>(q.d_final_state, q.d_initial_state, n);
     return hipGetLastError();
   }
   if (!q.kept) {

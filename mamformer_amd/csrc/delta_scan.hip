@@ -815,7 +815,7 @@ hipError_t run_prep(const DeltaParams& p, const DeltaLayout& lay, bool backward,
 
 // A sequence of no tokens: the state goes through.
 __global__ void delta_copy_state_kernel(const float* from, float* to, int64_t n) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = grid_row() * 256 + threadIdx.x;
   if (i < n) to[i] = from ? from[i] : 0.f;
 }
 
@@ -853,7 +853,7 @@ hipError_t launch_delta(const DeltaParams& p, hipStream_t st) {
   if (p.seqlen == 0) {
     const int64_t n = (int64_t)p.batch * p.heads * p.dk * p.dv;
     if (!p.final_state) return hipSuccess;
-    delta_copy_state_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p.initial_state, p.final_state, n);
+    delta_copy_state_kernel<<<row_grid((n + 255) / 256, 1), 256, 0, st>>>(p.initial_state, p.final_state, n);
     return hipGetLastError();
   }
   const hipError_t e = launch_delta_prep(p, p.keep, st);

@@ -17,7 +17,8 @@ __global__ __launch_bounds__(256) void delta_step_kernel(DeltaStepParams p, int 
   __shared__ float sk[kStepMaxDk], sq[kStepMaxDk];
   __shared__ float part[4][CW][9];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, cw = tid % CW, rg = tid / CW;
-  const int bh = blockIdx.x / blocks, blk = blockIdx.x % blocks;
+  const int at = (int)grid_row(), bh = at / blocks, blk = at % blocks;
+  if (bh >= p.batch * p.heads) return;
   const int b = bh / p.heads, h = bh % p.heads, hk = h / (p.heads / p.kheads);
   const int col = (blk * CW + cw) * 4, left = p.dv - col;
   const float* src = p.state_in + (int64_t)bh * p.dk * p.dv + col;
@@ -101,7 +102,7 @@ __global__ __launch_bounds__(256) void delta_step_kernel(DeltaStepParams p, int 
 template <typename T>
 hipError_t run(const DeltaStepParams& p, hipStream_t st) {
   const int blocks = (p.dv + 31) / 32;
-  delta_step_kernel<T, 8><<<(unsigned)((int64_t)p.batch * p.heads * blocks), 256, 0, st>>>(p, blocks);
+  delta_step_kernel<T, 8><<<row_grid((int64_t)p.batch * p.heads * blocks, 1), 256, 0, st>>>(p, blocks);
   return hipGetLastError();
 }
 

@@ -17,7 +17,7 @@ constexpr int U = 4;                             // heads whose loads are under 
 
 template <typename T, bool INTER>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p, int chunks, int shares, int per) {
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t id = grid_row() * 256 + threadIdx.x;
   const int64_t units = (int64_t)p.batch * p.seqlen * chunks;
   const int share = blockIdx.y;
   if (id >= units) return;
@@ -114,7 +114,7 @@ hipError_t run(const RotaryParams& p, hipStream_t st) {
   int per = (total + shares - 1) / shares;
   if (per > U) per = (per + U - 1) / U * U;
   shares = (total + per - 1) / per;
-  const dim3 grid((unsigned)blocks, (unsigned)shares);
+  const dim3 grid = row_grid(blocks, (unsigned)shares);
   if (p.interleaved) rotary_kernel<T, true><<<grid, 256, 0, st>>>(p, chunks, shares, per);
   else rotary_kernel<T, false><<<grid, 256, 0, st>>>(p, chunks, shares, per);
   return hipGetLastError();

@@ -266,3 +266,40 @@ def test_sliding_windows(dtype):
     assert torch.equal(mh.gated_delta_step(state, w3, w3, w3), mh.gated_delta_step(s2, *(w3.contiguous(),) * 3))
     assert torch.equal(state, s2)
     assert torch.equal(mh.group_norm(w[:, 0], 4), mh.group_norm(w[:, 0].contiguous(), 4))
+
+
+# ------------------------------------------------------------------------------------------------ grids of 2^32 threads
+
+def test_step_of_many_heads():
+    B, H, dv = 1 << 20, 8, 33                    # 2^24 workgroups of 256 threads
+    state = torch.randn(B, H, 1, dv, device="cuda")
+    q, k, v = (torch.randn(B, H, d, device="cuda", dtype=BF) for d in (1, 1, dv))
+    say("step of 2^23 heads")
+    first, last = state[:2].clone(), state[-2:].clone()
+    o = mh.gated_delta_step(state, q, k, v)
+    for part, s in ((slice(None, 2), first), (slice(-2, None), last)):
+        assert torch.equal(o[part], mh.gated_delta_step(s, q[part], k[part], v[part])) and torch.equal(state[part], s)
+
+
+def test_rotary_of_many_tokens():
+    x = torch.randn(4, 1, 1 << 30, 2, device="cuda", dtype=BF)
+    f = torch.full((1,), 1e-3, device="cuda", dtype=torch.float64)
+    say("rotary of 2^32 tokens")
+    y = mh.rotary(x, None, f)
+    for b in (0, 3):
+        for at in (0, (1 << 30) - 300):
+            assert torch.equal(y[b:b + 1, :, at:at + 300], mh.rotary(x[b:b + 1, :, at:at + 300], None, f, offset=at))
+
+
+def test_state_through_no_tokens():
+    """2^32 elements of a state that passes a sequence of none."""
+    B, dk, dv = 1 << 17, 128, 256
+    s = torch.empty(B, 1, dk, dv, device="cuda")
+    s.view(-1)[:] = 1.5
+    s[-1] = torch.randn(1, dk, dv, device="cuda")
+    q, v = torch.zeros(B, 1, 0, dk, device="cuda"), torch.zeros(B, 1, 0, dv, device="cuda")
+    say("no tokens, 16 GiB of state")
+    _, out = mh.gated_delta_rule(q, q, v, initial_state=s, return_final_state=True)
+    assert torch.equal(out[-1], s[-1]) and bool((out[:-1] == 1.5).all())
+    back = mh.gated_delta_rule_bwd(v, q, q, v, initial_state=s, d_final_state=out)[5]
+    assert torch.equal(back[-1], s[-1]) and bool((back[0] == 1.5).all())
