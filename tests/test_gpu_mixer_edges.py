@@ -303,3 +303,40 @@ def test_state_through_no_tokens():
     assert torch.equal(out[-1], s[-1]) and bool((out[:-1] == 1.5).all())
     back = mh.gated_delta_rule_bwd(v, q, q, v, initial_state=s, d_final_state=out)[5]
     assert torch.equal(back[-1], s[-1]) and bool((back[0] == 1.5).all())
+
+
+# ------------------------------------------------------------------------------------------------ group norm
+
+@pytest.mark.parametrize("shape,G", [((48, 256), 4), ((3, 500, 64), 4), ((2, 4001, 20), 4), ((1, 70, 4800), 2)])
+@pytest.mark.parametrize("mean", [4096.0, -1e6, 3e7])
+def test_group_norm_of_a_far_mean(shape, G, mean):
+    """Values far from zero, in either way of taking the sums: centred values keep their digits, whatever fp32 leaves of the
+    mean.  fp32 near 3e7 has steps of 2, so that the values are what they were rounded to."""
+    x = (torch.randn(*shape, generator=torch.Generator().manual_seed(1)) * max(1.0, abs(mean) * 2.0 ** -21) + mean).cuda()
+    b = torch.randn(shape[-1], device="cuda")
+    say(f"group norm of {shape} around {mean}")
+    y, stats = mh.group_norm(x, G, None, b, 1e-5, return_stats=True)
+    ry, rs = mx.group_norm(host(x), G, None, host(b), 1e-5)
+    z = ry - host(b)
+    # x - mean is exact (both within a factor 2 of each other); then what the mean's rounding left, 1 / deviation (the variance
+    # as fp32, eps, the root, the quotient), the product and the sum with b: 8 roundings of what enters them; in the one-position
+    # way the deviations of a first mean off by 4 roundings of it, mended by their own mean, whose sum has another 8 of those
+    first = 4 * 2.0 ** -24 * abs(mean) * rs[..., 1].max()
+    tol = 2.0 ** -24 * (8 * (np.abs(z) + np.abs(host(b))) + 8 * (1 + np.abs(z)) + 8 * first)
+    worst = (np.abs(host(y) - ry) / tol).max()
+    say(f"error at most {worst:.3f} of the tolerance")
+    assert worst <= 1
+    assert np.abs(host(stats[..., 1]) / rs[..., 1] - 1).max() <= 2.0 ** -20
+    assert np.abs(host(stats[..., 0]) - rs[..., 0]).max() <= 2.0 ** -23 * abs(mean)
+
+
+def test_group_norm_of_an_outlier_first():
+    """The value that all others are taken from may lie far from them."""
+    for first in (1e8, -3e12):
+        x = torch.randn(2, 300, 64, device="cuda")
+        x[:, 0, ::16] = first
+        y, stats = mh.group_norm(x, 4, return_stats=True)
+        ry, rs = mx.group_norm(host(x), 4)
+        # all but the first end at -mean / deviation, apart by their own differences over it
+        assert np.abs(host(y) - ry).max() <= 2.0 ** -20 * np.abs(ry).max()
+        assert np.abs(host(stats[..., 1]) / rs[..., 1] - 1).max() <= 2.0 ** -20
