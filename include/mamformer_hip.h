@@ -695,7 +695,7 @@ int mh_rotary(const mh_rotary_args* a, void* stream);
 /* Group norm, channels last: x, y (batch, space, channels), `groups` of neighbouring channels, mean and variance of each
  *   (batch, group) over the space and its channels; z = (x - mean) / sqrt(var + eps) * weight + bias, y = z, or z sigmoid(z)
  *   (silu). weight, bias (channels,) in weight_dtype, each or NULL. stats (batch, groups, 2) fp32 (mean, 1 / sqrt(var + eps))
- *   or NULL. channels <= 65536, batch * space <= 2^40. */
+ *   or NULL. channels <= 65536, batch * space <= 2^40. A group whose squares leave fp32's range is NaN throughout. */
 typedef struct {
   int64_t batch, space, channels, groups;
   int32_t dtype, weight_dtype, silu, reserved;

@@ -14,6 +14,7 @@
 // Measured (bf16, silu): 8192 tokens of 16 groups of 128 channels, one reading: 18 us for 67 MB (3.7 TB/s), backward 29 for
 // 101 MB and 4 for the parameters' sums; 8 x 4096 x 512 in 32 groups: 8.6 for the sums, 17 for the rest.  Where a workgroup
 // has few rows, its first loads, its reduction and its stores follow each other: a copy of these sizes takes 10.
+#include <cfloat>
 #include <type_traits>
 
 #include "launch.h"
@@ -37,6 +38,11 @@ __device__ __forceinline__ float act_slope(bool silu, float z) {
   if (!silu) return 1.f;
   const float s = sigmoid_f(z);
   return s * (1.f + z * (1.f - s));
+}
+
+// 1 / sqrt(var + eps); squares that left fp32's range make a NaN, as an infinite deviation would turn values to the bias.
+__device__ __forceinline__ float deviation(float var, float eps) {
+  return var <= FLT_MAX ? 1.f / sqrtf(fmaxf(var, 0.f) + eps) : __builtin_nanf("");
 }
 
 struct Affine {
@@ -118,7 +124,7 @@ __global__ __launch_bounds__(256) void group_rows_kernel(GroupNormParams p, int 
       }
       const float rest = lanes_sum<TG>(s) * inv;
       const float var = lanes_sum<TG>(q) * inv - rest * rest;
-      const float rstd = 1.f / sqrtf((var < 0.f ? 0.f : var) + p.eps);
+      const float rstd = deviation(var, p.eps);
       if (left > 0) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = act(p.silu, (x[j] - rest) * (rstd * a.w[j]) + a.b[j]);
@@ -358,7 +364,7 @@ __global__ __launch_bounds__(256, 4) void group_apply_kernel(GroupNormParams p, 
       const double count = (double)p.space * sp.cg, off = a / count, mean = first.get() + off, var = b / count - off * off;
       sm[tid] = (float)mean;
       sl[tid] = (float)(mean - sm[tid]);
-      sr[tid] = 1.f / sqrtf((float)(var > 0. ? var : var == var ? 0. : var) + p.eps);
+      sr[tid] = deviation((float)var, p.eps);
       if (p.stats && s == 0) {
         p.stats[2 * (n * p.groups + g)] = sm[tid];
         p.stats[2 * (n * p.groups + g) + 1] = sr[tid];

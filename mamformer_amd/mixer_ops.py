@@ -367,7 +367,9 @@ def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, *, activation=No
     x (N, ..., C), C up to 65536 and a multiple of ``num_groups``; mean and variance of each (batch entry, group of
     neighbouring channels) over the group's channels and all positions between.  A norm of each head of each token, as a
     linear-attention scan is followed by, is that of (tokens, C) with a group a head.  weight, bias (C,) fp32 or bf16 of
-    one dtype, each optional; activation: None or "silu".  Sums are fp64 over positions, fp32 (of centred values) within one.
+    one dtype, each optional; activation: None or "silu".  Sums are fp64 over positions, fp32 (of centred values) within one;
+    values are centred by the mean before its rounding.  A group whose squares leave fp32's range (values beyond about 1e19)
+    is NaN throughout.
 
     ``return_stats``: (y, stats), the groups' fp32 (mean, 1 / sqrt(var + eps)), shaped (N, num_groups, 2).
     Differentiable in x, weight and bias.

@@ -340,3 +340,26 @@ def test_group_norm_of_an_outlier_first():
         # all but the first end at -mean / deviation, apart by their own differences over it
         assert np.abs(host(y) - ry).max() <= 2.0 ** -20 * np.abs(ry).max()
         assert np.abs(host(stats[..., 1]) / rs[..., 1] - 1).max() <= 2.0 ** -20
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("shape,G", [((6, 64), 4), ((2, 300, 64), 4)])
+def test_group_norm_beyond_fp32s_squares(dtype, shape, G):
+    """A group whose variance leaves fp32 says so, and not its bias; the others keep their bits.  Near the end it is right."""
+    x = torch.randn(*shape, device="cuda").to(dtype)
+    w, b = torch.randn(2, 64, device="cuda")
+    want, ws = mh.group_norm(x, G, w, b, return_stats=True)
+    for size in (1e25, 3e38):
+        y = x.clone()
+        y[1, ..., 16:32] = torch.sign(y[1, ..., 16:32]) * size
+        got, st = mh.group_norm(y, G, w, b, return_stats=True)
+        assert got[1, ..., 16:32].isnan().all() and st[1, 1, 1].isnan()
+        got[1, ..., 16:32], st[1, 1] = want[1, ..., 16:32], ws[1, 1]
+        assert torch.equal(got, want) and torch.equal(st, ws)
+    y = x * 1e17
+    got, st = mh.group_norm(y, G, w, b, return_stats=True)
+    ry, rs = mx.group_norm(host(y), G, host(w), host(b))
+    half = torch.finfo(dtype).eps / 2
+    # 16 roundings of what enters, as everywhere (a deviation is taken of at most 4 of them)
+    assert (np.abs(host(got) - ry) <= half * np.abs(ry) + 2.0 ** -19 * (np.abs(ry) + 2 * np.abs(host(b)) + 4 * np.abs(host(w)))).all()
+    assert np.abs(host(st[..., 1]) / rs[..., 1] - 1).max() <= 2.0 ** -19
