@@ -415,6 +415,8 @@ def _group_norm_fwd(x, weight, bias, num_groups, eps, activation, want_stats):
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     y3 = _space(y)
     stats = torch.empty((x3.shape[0], num_groups, 2), device=x.device, dtype=torch.float32) if want_stats else None
+    if want_stats and not x3.shape[1]:
+        stats.fill_(math.nan)                    # the mean of no values; no kernel runs
     a = _group_args(x3, weight, bias, num_groups, eps, activation, stats, None)
     a.y, a.y_stride_b, a.y_stride_s = _strides2(y3)
     ws = _optional_workspace("mh_group_norm_workspace_bytes", a, x.device)

@@ -363,3 +363,14 @@ def test_group_norm_beyond_fp32s_squares(dtype, shape, G):
     # 16 roundings of what enters, as everywhere (a deviation is taken of at most 4 of them)
     assert (np.abs(host(got) - ry) <= half * np.abs(ry) + 2.0 ** -19 * (np.abs(ry) + 2 * np.abs(host(b)) + 4 * np.abs(host(w)))).all()
     assert np.abs(host(st[..., 1]) / rs[..., 1] - 1).max() <= 2.0 ** -19
+
+
+def test_group_norm_statistics_of_no_positions():
+    torch.full((3, 4, 2), 5.0, device="cuda")    # what the next allocation of this size holds
+    y, stats = mh.group_norm(torch.zeros(3, 0, 64, device="cuda"), 4, return_stats=True)
+    assert y.shape == (3, 0, 64) and stats.shape == (3, 4, 2) and stats.isnan().all()
+    y, stats = mh.group_norm(torch.zeros(0, 7, 64, device="cuda"), 4, return_stats=True)
+    assert stats.shape == (0, 4, 2)
+    x, st = torch.zeros(3, 0, 64, device="cuda"), torch.full((3, 4, 2), float("nan"), device="cuda")
+    dx, dw, db = mh.group_norm_bwd(x, x, st, 4, torch.ones(64, device="cuda"))
+    assert dx.shape == (3, 0, 64) and (dw == 0).all() and (db == 0).all()
