@@ -135,7 +135,10 @@ def rotary(q, k, inv_freq, positions=None, *, offset=0, interleaved=False, scale
             raise TypeError(f"{name}: positions must be int32 or int64, got {positions.dtype}")
         if positions.shape not in ((qs[2],), (qs[0], qs[2])):
             raise ValueError(f"{name}: positions must be (L,) or (B, L), got {tuple(positions.shape)} for q {tuple(q.shape)}")
-    cfg = (int(offset), bool(interleaved), float(scale), bool(inverse))
+    offset = int(offset)
+    if not -1 << 63 <= offset < 1 << 63:
+        raise ValueError(f"{name}: offset {offset} outside 64 bits")
+    cfg = (offset, bool(interleaved), float(scale), bool(inverse))
     if _through_autograd(q, k):
         out = _RotaryFn.apply(q, k, inv_freq, positions, cfg)
     else:

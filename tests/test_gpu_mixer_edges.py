@@ -374,3 +374,11 @@ def test_group_norm_statistics_of_no_positions():
     x, st = torch.zeros(3, 0, 64, device="cuda"), torch.full((3, 4, 2), float("nan"), device="cuda")
     dx, dw, db = mh.group_norm_bwd(x, x, st, 4, torch.ones(64, device="cuda"))
     assert dx.shape == (3, 0, 64) and (dw == 0).all() and (db == 0).all()
+
+
+@pytest.mark.parametrize("offset", [1 << 63, -(1 << 63) - 1, 1 << 64])
+def test_rotary_offset_out_of_range(offset):
+    q, f = torch.randn(1, 1, 2, 8, device="cuda"), torch.ones(4, device="cuda")
+    with pytest.raises(ValueError, match="offset"):
+        mh.rotary(q, None, f, offset=offset)
+    mh.rotary(q, None, f, offset=(1 << 63) - 2)
