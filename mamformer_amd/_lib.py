@@ -448,7 +448,24 @@ def check(fn: str, rc: int):
         raise MHError(fn, rc, msg)
 
 
+class StreamElsewhere(int):
+    """The handle of a stream on a device that is not the current one.  A handle does not name its device (that of every default
+    stream is 0), so that ``call`` makes the device current for the launch."""
+
+    def __new__(cls, handle, device):
+        s = super().__new__(cls, handle)
+        s.device = device
+        return s
+
+
 def call(fn: str, *args):
-    rc = getattr(_lib or lib(), fn)(*args)
+    f = getattr(_lib or lib(), fn)
+    if type(args[-1]) is StreamElsewhere:
+        import torch
+
+        with torch.cuda.device(args[-1].device):
+            rc = f(*args)
+    else:
+        rc = f(*args)
     if rc:
         check(fn, rc)

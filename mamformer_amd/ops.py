@@ -115,7 +115,9 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 def _stream(dev: torch.device):
-    return torch._C._cuda_getCurrentRawStream(dev.index)
+    i = dev.index
+    s = torch._C._cuda_getCurrentRawStream(i)
+    return s if i == torch._C._cuda_getDevice() else _lib.StreamElsewhere(s, i)
 
 
 def _require_cuda(name, *ts):
