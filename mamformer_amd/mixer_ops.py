@@ -52,9 +52,14 @@ def _channels(t):
 
 
 def _result(t):
-    """A new tensor of t's layout, with contiguous channels (torch may order dimensions of equal strides the other way)."""
+    """(a new tensor of t's layout, its strides), with contiguous channels: torch may order dimensions of equal strides the
+    other way."""
     out = torch.empty_like(t)
-    return out if out.stride(-1) == 1 or t.shape[-1] == 1 else torch.empty(t.shape, device=t.device, dtype=t.dtype)
+    st = out.stride()
+    if st[-1] != 1 and t.shape[-1] != 1:
+        out = torch.empty(t.shape, device=t.device, dtype=t.dtype)
+        st = out.stride()
+    return out, st
 
 
 def _f32(t):
@@ -158,18 +163,18 @@ def _rotary(q, k, inv_freq, positions, cfg):
         if positions.stride(-1) != 1 and L != 1:
             positions = positions.contiguous()
         pos_sb = positions.stride(0) if positions.dim() == 2 else 0
-    qo, ko, HK = _result(q), None, 0
+    (qo, (ob, oh, ol, _)), ko, HK = _result(q), None, 0
     if k is not None:
         k = _channels(k)
-        ko, HK = _result(k), k.shape[1]
-    (qb, qh, ql, _), (ob, oh, ol, _) = q.stride(), qo.stride()
+        (ko, ks), HK = _result(k), k.shape[1]
+    qb, qh, ql, _ = q.stride()
     a = RotaryArgs(B, H, HK, L, D, inv_freq.shape[0], _DT[q.dtype], interleaved, inverse, inv_freq.dtype is torch.float64,
                    0 if positions is None else _INDEX_BYTES[positions.dtype], scale, inv_freq.data_ptr(), _ptr(positions), pos_sb,
                    offset, q.data_ptr(), qb, qh, ql)
     a.q_out, a.q_out_stride_b, a.q_out_stride_h, a.q_out_stride_l = qo.data_ptr(), ob, oh, ol
     if HK:
         a.k, a.k_stride_b, a.k_stride_h, a.k_stride_l = _strides3(k)
-        a.k_out, a.k_out_stride_b, a.k_out_stride_h, a.k_out_stride_l = _strides3(ko)
+        a.k_out, a.k_out_stride_b, a.k_out_stride_h, a.k_out_stride_l = ko.data_ptr(), *ks[:3]
     if H:
         _lib.call("mh_rotary", ct.byref(a), _stream(q.device))
     return qo, ko
@@ -257,13 +262,13 @@ def _delta_args(q, k, v, g, beta, state, scale):
 
 def _delta_fwd(q, k, v, g, beta, state, scale, want_final, keep):
     q, k, v, g, beta, state = _channels(q), _channels(k), _channels(v), _f32(g), _f32(beta), _vec(state)
-    o = _result(v)
+    o, (ob, oh, ol, _) = _result(v)
     final = None
     if want_final:
         final = torch.empty((*v.shape[:2], q.shape[-1], v.shape[-1]), device=v.device, dtype=torch.float32)
     a = _delta_args(q, k, v, g, beta, state, scale)
     a.final_state, a.keep = _ptr(final), keep
-    a.o, a.o_stride_b, a.o_stride_h, a.o_stride_l = _strides3(o)
+    a.o, a.o_stride_b, a.o_stride_h, a.o_stride_l = o.data_ptr(), ob, oh, ol
     ws = _optional_workspace("mh_delta_rule_workspace_bytes", a, v.device)
     _lib.call("mh_delta_rule_fwd", ct.byref(a), _stream(v.device))
     return o, final, ws if keep else None
@@ -288,7 +293,7 @@ def gated_delta_rule_bwd(do, q, k, v, g=None, beta=None, *, scale=None, initial_
 def _delta_bwd(do, q, k, v, g, beta, initial_state, d_final_state, scale, kept=None):
     q, k, v, do = _channels(q), _channels(k), _channels(v), _channels(do)
     g, beta, initial_state, d_final_state = _f32(g), _f32(beta), _vec(initial_state), _vec(d_final_state)
-    dq, dk, dv = _result(q), _result(k), _result(v)
+    dq, dk, dv = _result(q)[0], _result(k)[0], _result(v)[0]
     dg, dbeta = (None if t is None else torch.empty(v.shape[:-1], device=v.device, dtype=torch.float32) for t in (g, beta))
     d_state = None if initial_state is None else torch.empty_like(initial_state)
     a = DeltaBwdArgs(_delta_args(q, k, v, g, beta, initial_state, scale), *_strides3(do), _ptr(d_final_state), *_strides3(dq),
@@ -348,9 +353,9 @@ def gated_delta_step(state, q, k, v, g=None, beta=None, *, scale=None, state_out
     if _through_autograd(state, q, k, v, g, beta, state_out):
         raise RuntimeError(f"{name}: has no backward; call it under torch.no_grad(), or gated_delta_rule with L = 1")
     q, k, v, g, beta = _channels(q), _channels(k), _channels(v), _f32(g), _f32(beta)
-    o = _result(v)
+    o, (ob, oh, _) = _result(v)
     (B, HK, dk), (_, H, dv) = q.shape, v.shape
-    (qb, qh, _), (kb, kh, _), (vb, vh, _), (ob, oh, _) = q.stride(), k.stride(), v.stride(), o.stride()
+    (qb, qh, _), (kb, kh, _), (vb, vh, _) = q.stride(), k.stride(), v.stride()
     a = DeltaStepArgs(B, H, HK, dk, dv, _DT[q.dtype], dk ** -0.5 if scale is None else scale, q.data_ptr(), qb, qh,
                       k.data_ptr(), kb, kh, v.data_ptr(), vb, vh, *_strides2(g), *_strides2(beta), state.data_ptr(),
                       state_out.data_ptr(), o.data_ptr(), ob, oh)
