@@ -226,6 +226,23 @@ def test_delta_gradients_of_zeros(dtype, L):
     assert (o == 0).all() and (s == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_delta_gradients_nonfinite_stay_in_their_head(dtype, bad):
+    """What comes back of a value or a gradient that is not finite: other heads keep their bits, the head's own tell."""
+    _, t = delta_inputs(1, 3, 3, 200, 32, 32, dtype)
+    do = torch.randn_like(t[2])
+    want = mh.gated_delta_rule_bwd(do, *t[:5], initial_state=t[5])
+    for i in (1, 2, 6):
+        u = [a.clone() for a in (*t, do)]
+        u[i][0, 1, 70, 5] = bad
+        got = mh.gated_delta_rule_bwd(u[6], *u[:5], initial_state=u[5])
+        for a, b in zip(got, want):
+            assert torch.equal(a[:, [0, 2]], b[:, [0, 2]])
+        assert not torch.isfinite(got[2][0, 1]).all() or i == 2
+        assert not torch.isfinite(got[1][0, 1]).all()
+
+
 # ------------------------------------------------------------------------------------------------ rotary positions
 
 def test_rotary_without_queries():
@@ -382,3 +399,31 @@ def test_rotary_offset_out_of_range(offset):
     with pytest.raises(ValueError, match="offset"):
         mh.rotary(q, None, f, offset=offset)
     mh.rotary(q, None, f, offset=(1 << 63) - 2)
+
+
+def test_gradients_of_many_positions():
+    """2^31 elements of one sequence: dx and db against sums in fp64 over all of it, a piece at a time."""
+    n, C, G = (1 << 24) + 5, 128, 4
+    x = torch.randn(1, n, C, device="cuda", dtype=BF)
+    say("group norm's gradients over 2^24 positions")
+    _, st = mh.group_norm(x, G, return_stats=True)
+    db = mh.group_norm_bwd(torch.ones_like(x), x, st, G, dtype=F32)[2]
+    # sums of ones are exact up to 2^24; a few roundings of half a step of 2 above
+    assert (db.double() - n).abs().max() <= 4
+    rows = torch.arange(n, device="cuda")
+    dy = ((rows * 7919 % 13 - 6)[:, None] * (1 + torch.arange(C, device="cuda") % 3)).to(BF)[None]
+    dx, _, db = mh.group_norm_bwd(dy, x, st, G, dtype=F32)
+    m, r = (st[0, :, i].double().repeat_interleave(C // G) for i in (0, 1))
+    s1, s2, mag = (torch.zeros(C, device="cuda", dtype=torch.float64) for _ in range(3))
+    for a in range(0, n, 1 << 20):
+        d = dy[0, a:a + (1 << 20)].double()
+        xh = (x[0, a:a + (1 << 20)].double() - m) * r
+        s1, s2, mag = s1 + d.sum(0), s2 + (d * xh).sum(0), mag + (d * xh).abs().sum(0)
+    mean1, mean2, meanmag = ((t.view(G, -1).sum(-1) / (n * C // G)).repeat_interleave(C // G) for t in (s1, s2, mag))
+    # a thread's sum of up to 1100 terms in fp32, then 16 and a fourth of 1100 of those: 2^11 roundings of their magnitude
+    for part in (slice(0, 9), slice(n // 2, n // 2 + 9), slice(n - 9, n)):
+        d, xh = dy[0, part].double(), (x[0, part].double() - m) * r
+        want = r * (d - mean1 - xh * mean2)
+        tol = 2.0 ** -8 * want.abs() + 2.0 ** -20 * r * (d.abs() + 18) + 2.0 ** -13 * r * xh.abs() * meanmag
+        assert ((dx[0, part].double() - want).abs() <= tol).all()
+    assert ((db.double() - s1).abs() <= 2.0 ** -13 * (dy.abs().float().mean((0, 1)).double() * n)).all()
