@@ -241,7 +241,7 @@ __device__ __forceinline__ void fetch_share(lds_f16_t* to, const char* from, int
 
 // Lines of a later piece's fragments, read so that the L2 holds them when the waves that fetch ask: `wg` of `nwg` workgroups
 // that want the same takes its share of A + B + 1 KB in blocks of 8 KB, a line a lane.  With a pair a workgroup, eight of
-// which share 128 columns, that takes the scan from 201 to 175 us (b 2, H 16, L 4096); with two pairs, whose share is twice as
+// which share 128 columns, that took the scan from 201 to 175 us (b 2, H 16, L 4096); with two pairs, whose share is twice as
 // large and whose fetching waves are as busy, it cost 5 of 86 (b 4, H 16, L 2048), so that those go without.
 struct Warm {
   static constexpr int N = 5;

@@ -13,7 +13,7 @@
 //   A' and P' themselves, in fp32.
 // What it reads of the forward, the pieces' systems, entering states and corrections, a forward kept for it (3 KB a token
 // and head of 128 x 128 in bf16, six times q, k and v) or is computed again, which at b 2, H 16 over 8, L 4096 (bf16) takes
-// 190 us beside the 410 of the two kernels here.
+// 172 us beside the 420 of the two kernels here.
 #include "delta.h"
 
 namespace mh {
@@ -21,8 +21,9 @@ namespace {
 
 // Two waves hold the gradient of 16 columns of the state as the forward's scan holds the state: half of its rows and half of
 // a piece's tokens each, and (bf16) a wave fetches the fragments and another dO.  y = T^T ddelta is upper triangular, so
-// that here the first wave needs the second one's ddelta.  Bound by a piece's latency as that scan is: 3.0 us for each of
-// the 64 pieces of L 4096 (b 2, H 16, 128 x 128: 195 us; with two pairs a workgroup and half of the CUs idle 226).
+// that here the first wave needs the second one's ddelta.  Bound by a piece's chain as that scan is: 3.0 us for each of
+// the 64 pieces of L 4096 (b 2, H 16, 128 x 128: 194 us, with two pairs a workgroup and half of the CUs idle 226; b 3, which
+// takes two pairs, 246, with 27 registers spilled).
 template <typename T, int DKP, int PAIRS>
 __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_back_scan_kernel(DeltaBwdParams q, DeltaLayout lay, DeltaScratch scr, int nblk, int nwg) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
@@ -373,9 +374,10 @@ __device__ __forceinline__ void put_halves(f16* t, int r, int c, f16x8 v) {
 // that order).  Waves w and w + 4 hold rows 16 w .. 16 w + 15: of the three products with the states (64 x dk) half of the
 // channels each, of A' and P' every other tile (four waves with all of it spilled 150 registers: 407 us against 300 when
 // this was split).  The columns of v pass through LDS DVB at a time, every matrix brought to one scale on the way (its
-// columns have their own), a stage's loads under way during the one before.  Now 215 us at b 2, H 16 over 8, L 4096: 400 MB
-// of states, corrections and their gradients, which at a copy's rate take 70; one workgroup fits a CU, so that nothing
-// covers its barriers, and stages of 64 columns (fewer barriers) took 252.
+// columns have their own), a stage's loads under way during the one before.  Now 225 us at b 2, H 16 over 8, L 4096: 400 MB
+// of states, corrections and their gradients, which at a copy's rate take 70; one workgroup fits a CU, two waves a SIMD, which
+// issue vector instructions in 41% of the cycles, matrix products in 11%, and wait for one another at the stages' barriers.
+// Stages of 64 columns (fewer barriers) took 252.
 template <typename T, int DKP>
 __global__ __launch_bounds__(512) void delta_grads_kernel(DeltaBwdParams q, DeltaLayout lay, DeltaScratch scr, int nblk) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;

@@ -7,7 +7,7 @@
 // delta is what each token corrects before its beta, so that beta = 0 divides nothing.  delta_prep_kernel makes T and P of
 // every piece side by side; delta_scan_kernel walks the pieces with the state in registers.
 // o takes both parts of S, P and delta also where it is rounded to bf16: its terms may cancel far below what enters them, and
-// one part, 2^-12 of that, would show (it was 9 of 142 us at b 4, H 16, L 2048).
+// one part, 2^-12 of that, would show (12 of 141 us at b 4, H 16, L 2048).
 #include "delta.h"
 
 namespace mh {
@@ -20,8 +20,8 @@ namespace {
 // and P by rows as they stand.  The inverse in fp32: every wave solves one 16 x 16 diagonal block by substitution, a column
 // a lane, then wave w builds block row w of T from the diagonal outwards, T_wj = -(sum over j < k <= w of T_wk A_kj) T_jj,
 // with fp32 matrix instructions, T_wk staying in accumulators, which are the B operand of the next product.
-// Workgroups on one CU hide each other's latencies (LDS, substitution); what they write, 67 KB a piece of one value head,
-// is what bounds them: b 4, H 16, L 2048 (bf16, 128): 52 us for 2048 pieces, 200 MB read and written, 3.9 TB/s.
+// Workgroups on one CU hide each other's latencies (LDS, substitution); what they write, 73 KB a piece of one value head,
+// is what bounds them: b 4, H 16, L 2048 (bf16, 128): 57 us for 2048 pieces, 220 MB read and written, 3.9 TB/s.
 template <typename T, int DKP>
 __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void delta_prep_kernel(DeltaParams p, DeltaLayout lay, int backward) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
@@ -291,8 +291,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void delta_prep_kernel
 // ------------------------------------------------------------------ the state from piece to piece
 // Two waves hold 16 columns of the state, half of its rows each (fp32), and half of a piece's tokens; a workgroup has two
 // such pairs, which read the same fragments, or one where the pairs are no more than the CUs (b 2, H 16, L 4096, o and what
-// a backward keeps: 204 us against 224 when it was chosen, 168 now), or four for a segment without o, whose exchange takes
-// less LDS.  For a piece:
+// a backward keeps: 204 us against 224 when it was chosen, 188 now; b 3, which takes two pairs, 254), or four for a segment
+// without o, whose exchange takes less LDS.  For a piece:
 //   each wave multiplies K (and Q) by its rows of S and gives the other its part of the other's tokens;   [barrier 1]
 //   R = V - e^G K S of its tokens; T is lower triangular, so that the second wave needs the first one's R;  [barrier 2]
 //   U = beta e^{G_end - G} delta of its tokens goes to the other, each adds K^T U to its rows.              [barrier 3]
@@ -301,10 +301,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void delta_prep_kernel
 // KEEP: the entering states and delta are stored for the backward.  OUT: o is computed.  What is multiplied and added in
 // one instruction is written out, so that all variants give the same bits.
 //
-// Bound by the latency of one piece on waves that have a SIMD to themselves, most of it the conversions (an instruction of
-// 4 cycles for each value and part): 2.7 us a piece (b 4, H 16, L 2048, 128 x 128: 86 us; b 2, H 16, L 4096 with what a
-// backward keeps 168).  With two pairs about a sixth of it is the wait for the next piece's K and Q at barrier 3.  Operands
-// that no other wave has to finish first are read from LDS right behind a barrier, ahead of what they are needed for.
+// Bound by the chain of one piece on waves that have a SIMD to themselves: 3.0 us (b 4, H 16, L 2048, 128 x 128: 95 us; b 2,
+// H 16, L 4096 with what a backward keeps 188).  Of its 6000 cycles a wave issues vector instructions in 2400 (about 500, 66
+// of them matrix products), the matrix units work in 1060 and the CU's LDS in 1360; the rest are waits for one another, for
+// operands and at the three barriers, which nothing on the SIMD fills.  Operands that no other wave has to finish first are
+// read from LDS right behind a barrier, ahead of what they are needed for.
 template <typename T, int DKP, bool OUT, bool KEEP, int PAIRS>
 __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(DeltaParams p, DeltaLayout lay, int nblk, int nwg) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;
@@ -341,7 +342,7 @@ __global__ __launch_bounds__((kDeltaThreads<T, PAIRS>)) void delta_scan_kernel(D
   lds_f16_t* const lds = (lds_f16_t*)smem;
   auto fetch_a = [&](int c) { fetch_share<GA, FW>(lds + (AB == 2 ? (c & 1) * GA * FR : 0), p.workspace + lay.kq + (kunit0 + c) * lay.kq_unit + (OUT ? 0 : NP * F * 1024), fw, lane); };
   // The second kind in two parts: K by columns at the top of a piece, T and P behind its barrier 2, so that the next piece's
-  // first kind, which has to have landed by barrier 3, waits for less (one part: 89 us against 86 at b 4, H 16, L 2048).
+  // first kind, which has to have landed by barrier 3, waits for less (one part: 89 us against 86 when it was chosen, b 4, H 16, L 2048).
   constexpr int GB1 = NP * F + 1, GB2 = TPF;
   auto b_of = [&](int c) { return lds + (AB * GA + (AHEAD ? (c & 1) * GB : 0)) * FR; };
   auto fetch_b2 = [&](int c) {
@@ -825,7 +826,7 @@ __global__ void delta_copy_state_kernel(const float* from, float* to, int64_t n)
 // without o finds what each makes of no state (N) and of the identity's columns (M), delta_segments_kernel goes from segment
 // to segment, and the scan with o takes all segments at once.  The segments' number is the one with the least time by this
 // count, in tenths of a piece's time (o and all: 10, without o: 9; a segment's product: 10); a gain of less than a fifth is
-// left.  H 8, L 32768 of 128 x 128 (bf16): 8 segments, 180 + 24 + 175 us where the scan in one went 1205.
+// left.  H 8, L 32768 of 128 x 128 (bf16): 8 segments, 180 + 24 + 198 us where the scan in one went 1205.
 int delta_segments(const DeltaParams& p) {
   const int64_t heads = (int64_t)p.batch * p.heads, nblk = (p.dv + 15) / 16, kblk = (p.dk + 15) / 16;
   const int64_t whole = heads * ((nblk + 1) / 2), move = heads * ((nblk + 3) / 4 + (kblk + 3) / 4);

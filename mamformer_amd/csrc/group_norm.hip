@@ -12,7 +12,7 @@
 // Channels are taken 8 at a time within a group, so that a chunk never belongs to two groups.
 //
 // Measured (bf16, silu): 8192 tokens of 16 groups of 128 channels, one reading: 18 us for 67 MB (3.7 TB/s), backward 29 for
-// 101 MB and 4 for the parameters' sums; 8 x 4096 x 512 in 32 groups: 8.6 for the sums, 17 for the rest.  Where a workgroup
+// 101 MB and 4 for the parameters' sums; 8 x 4096 x 512 in 32 groups: 10 for the sums, 17 for the rest.  Where a workgroup
 // has few rows, its first loads, its reduction and its stores follow each other: a copy of these sizes takes 10.
 #include <cfloat>
 #include <type_traits>

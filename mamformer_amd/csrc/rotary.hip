@@ -2,9 +2,9 @@
 // the pairs being channels (i, n + i) or (2 i, 2 i + 1) of the first 2 n; the rest pass.  The turn by the negative angle is
 // its gradient (and its inverse where scale is 1).
 //
-// Bound by the rows' bytes.  Angles: position * inv_freq / (2 pi) in fp64, of which the fraction of a turn is left, exact
-// to fp32 for positions beyond 2^31 turns; then the sine and cosine of that many turns in fp32.  A thread computes those of
-// its 8 pairs once, while its first heads' channels are under way, and runs through its share of the heads of queries and
+// Bound by the rows' bytes.  Angles: position * inv_freq / (2 pi) in fp64, three roundings of the whole angle (less than
+// 2^-24 radians up to angles of 2^27), of which the fraction of a turn is left; then the sine and cosine of that many turns
+// in fp32.  A thread computes those of its 8 pairs once, while its first heads' channels are under way, and runs through its share of the heads of queries and
 // keys with them, four heads' loads at once (one at a time: 23.8 us).  b 2, 16 + 8 heads of 128, L 4096 in bf16: 21 us for
 // 101 MB, 4.8 TB/s, of which the angles take about 3 before the first store.
 #include "launch.h"

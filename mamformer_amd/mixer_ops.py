@@ -118,8 +118,8 @@ def rotary(q, k, inv_freq, positions=None, *, offset=0, interleaved=False, scale
     q (B, H, L, D) and k (B, HK, L, D) of one dtype; inv_freq (n,) float32 or float64 with 2 n <= D.  Of the first 2 n
     channels the pairs (i, n + i), or with ``interleaved`` (2 i, 2 i + 1), are turned by the angle
     (positions + offset) * inv_freq[i] and multiplied by ``scale``; the others are copied.  ``positions``: int32 or int64
-    (L,) or (B, L), None for 0 .. L - 1.  Angles are reduced in 64 bits: far positions cost no precision.
-    ``inverse`` turns back, which with the same ``scale`` is the gradient.  Differentiable in q and k (an inv_freq that requires
+    (L,) or (B, L), None for 0 .. L - 1.  Angles are reduced in 64 bits: one of x radians
+    is off by x 2^-51 at most, less than fp32's own rounding up to 2^27.  ``inverse`` turns back, which with the same ``scale`` is the gradient.  Differentiable in q and k (an inv_freq that requires
     a gradient is refused).
     """
     name = "rotary"
@@ -220,11 +220,12 @@ def gated_delta_rule(q, k, v, g=None, beta=None, *, scale=None, initial_state=No
     Operands of the products keep 22 bits of the largest value of their column or piece, sums are fp32: results are exact to
     about 2^-20 of the norms that enter them, before the one rounding to bf16.
 
-    A token with beta = 0 and g = 0 changes nothing, which is what padding behind a sequence takes.  A NaN or infinity may
-    reach every result of its head from the 64-token piece that holds it on.  With L = 0 the state goes through.
+    A token with beta = 0 and g = 0 changes nothing, which is what padding behind a sequence takes, with finite q, k and v: a
+    NaN or infinity, a padding token's too, may reach every result of its head from the 64-token piece that holds it on.
+    With L = 0 the state goes through.
     Differentiable in all tensors: a call that records a gradient keeps the states and systems of its pieces for it, about
     3 KB a token and head of 128 x 128 (bf16); with ``recompute`` it keeps its inputs alone, and the gradients' pass computes
-    the rest again (a third more time for a training step).  The gradients are the same bits.
+    the rest again (a fifth more time for a training step).  The gradients are the same bits.
     """
     name = "gated_delta_rule"
     _require_cuda(name, q, k, v, g, beta, initial_state)
@@ -376,8 +377,8 @@ def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, *, activation=No
     neighbouring channels) over the group's channels and all positions between.  A norm of each head of each token, as a
     linear-attention scan is followed by, is that of (tokens, C) with a group a head.  weight, bias (C,) fp32 or bf16 of
     one dtype, each optional; activation: None or "silu".  Sums are fp64 over positions, fp32 (of centred values) within one;
-    values are centred by the mean before its rounding.  A group whose squares leave fp32's range (values beyond about 1e19)
-    is NaN throughout.
+    values are centred by the mean before its rounding, in the gradients by the fp32 mean.  A group whose squares leave fp32's
+    range (values beyond about 1e19) is NaN throughout.
 
     ``return_stats``: (y, stats), the groups' fp32 (mean, 1 / sqrt(var + eps)), shaped (N, num_groups, 2).
     Differentiable in x, weight and bias.
